@@ -260,16 +260,18 @@ def _rounded(wtype, x):
     """x [n, k] f32 as the product of this weight type sees it"""
     if wtype == "f16":
         return x.half().float()
+    # quotients of two tensors: a number among the operands is multiplied by, as a reciprocal
     if wtype == "q8_0":
         b = x.reshape(-1, 32)
         top = b.abs().amax(1, keepdim=True)
-        q = torch.round(b * torch.where(top > 0, 127.0 / top, 0.0))
-        return (q * (top / 127.0).half().float()).reshape(x.shape)
+        n = torch.full_like(top, 127.0)
+        q = torch.round(b * torch.where(top > 0, n / top, 0.0))
+        return (q * (top / n).half().float()).reshape(x.shape)
     b = x.reshape(-1, 256)
     top = torch.gather(b, 1, b.abs().argmax(1, keepdim=True))  # with its sign
-    scale = torch.where(top != 0, -127.0 / top, 0.0)
+    scale = torch.where(top != 0, torch.full_like(top, -127.0) / top, 0.0)
     q = torch.round(b * scale).clamp_max(127.0)
-    return (q * torch.where(top != 0, 1.0 / scale, 0.0)).reshape(x.shape)
+    return (q * torch.where(top != 0, torch.ones_like(top) / scale, 0.0)).reshape(x.shape)
 
 
 def _weights(wtype, raw, k):
@@ -526,14 +528,14 @@ def _exact_activations(wtype, x):
     if wtype == "q8_0":
         v = x.reshape(-1, 32)
         m = v.abs().max(1, keepdim=True).values
-        q = torch.round(v * (127.0 / m)).nan_to_num(0.0).double()
-        return (q * (m / 127.0).half().double()).reshape(x.shape)
+        q = torch.round(v * (127.0 / m.double()).float()).nan_to_num(0.0).double()
+        return (q * (m.double() / 127.0).float().half().double()).reshape(x.shape)
     v = x.reshape(-1, 256)
     hi, lo = v.max(1, keepdim=True).values, v.min(1, keepdim=True).values
     m = torch.where(hi >= -lo, hi, lo)
-    i = -127.0 / m
+    i = (-127.0 / m.double()).float()
     q = torch.round(v * i).clamp_max(127.0).nan_to_num(0.0).double()
-    return (q * (1.0 / i).double()).reshape(x.shape)
+    return (q * (1.0 / i.double()).float().double()).reshape(x.shape)
 
 
 def _exact_matrix(wtype, raw, k):
