@@ -195,6 +195,12 @@ enum ggml_unary_op {
     GGML_UNARY_OP_COUNT
 };
 
+/* ARGSORT's op_params[0] */
+enum ggml_sort_order {
+    GGML_SORT_ORDER_ASC = 0,
+    GGML_SORT_ORDER_DESC = 1
+};
+
 /* rope modes (ffi.rs:356-362) */
 #define GGML_ROPE_TYPE_NORMAL 0
 #define GGML_ROPE_TYPE_NEOX 2

@@ -93,6 +93,35 @@ struct ggml_tensor * ggml_gelu_erf(struct ggml_context * ctx, struct ggml_tensor
 struct ggml_tensor * ggml_relu(struct ggml_context * ctx, struct ggml_tensor * a);
 struct ggml_tensor * ggml_mul_mat(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b);
 void ggml_mul_mat_set_prec(struct ggml_tensor * a, enum ggml_prec prec);
+/* ---- mixture-of-experts and state-space operators (upstream ggml.h) ----
+ * The constructors of this group return NULL, with a message on stderr, for
+ * shapes or types that do not fit. */
+/* as [K, M, n_expert], b [K, 1 | n_used, n_tokens] f32, ids [n_used, n_tokens]
+ * i32 (rows may be strided) -> [M, n_used, n_tokens]: column (slot, token) is
+ * as[ids[slot, token]] times b's column (slot % b.ne[1], token); zeros where
+ * the id is outside [0, n_expert) */
+struct ggml_tensor * ggml_mul_mat_id(struct ggml_context * ctx, struct ggml_tensor * as, struct ggml_tensor * b,
+                                     struct ggml_tensor * ids);
+/* the indices that sort each row of a; equal elements keep their order, NaN
+ * sorts as the largest */
+struct ggml_tensor * ggml_argsort(struct ggml_context * ctx, struct ggml_tensor * a, enum ggml_sort_order order);
+/* the first k of the descending ARGSORT, a [k, ...] view of it */
+struct ggml_tensor * ggml_top_k(struct ggml_context * ctx, struct ggml_tensor * a, int k);
+struct ggml_tensor * ggml_sum_rows(struct ggml_context * ctx, struct ggml_tensor * a);
+/* depthwise causal convolution of a state-space mixer: sx [d_conv - 1 + n_t,
+ * d_inner, n_s] (the carried columns, then the step's), c [d_conv, d_inner]
+ * -> [d_inner, n_t, n_s] */
+struct ggml_tensor * ggml_ssm_conv(struct ggml_context * ctx, struct ggml_tensor * sx, struct ggml_tensor * c);
+/* selective state-space scan: s [d_state, head_dim, n_head, n_slots], x
+ * [head_dim, n_head, n_t, n_s], dt [n_head, n_t, n_s] (softplus is applied
+ * here), A [1 | d_state, n_head], B and C [d_state, n_group, n_t, n_s], ids
+ * [n_s] i32: sequence i starts from slot ids[i] of s (from zeros where that
+ * is outside [0, n_slots)). The result is one row: y, laid out as a
+ * contiguous x, then each sequence's state after its last token, laid out as
+ * slots of s. s itself is only read. */
+struct ggml_tensor * ggml_ssm_scan(struct ggml_context * ctx, struct ggml_tensor * s, struct ggml_tensor * x,
+                                   struct ggml_tensor * dt, struct ggml_tensor * A, struct ggml_tensor * B,
+                                   struct ggml_tensor * C, struct ggml_tensor * ids);
 struct ggml_tensor * ggml_get_rows(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b);
 struct ggml_tensor * ggml_set_rows(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b,
                                    struct ggml_tensor * c);

@@ -27,8 +27,9 @@
  *   "ggml_backend_get_cancel_observation" -- observation boundary of the last compute
  *   "ggml_backend_device_pci_vendor_id"   -- 0x1002 (backend.rs:1678-1694)
  *   "ggml_backend_mi355x_profile_graph", "ggml_backend_mi355x_set_hip_graphs",
- *   "ggml_backend_mi355x_refuse_next_launch"
- *                                         -- the three functions below
+ *   "ggml_backend_mi355x_refuse_next_launch",
+ *   "ggml_backend_mi355x_buffer_from_device_ptr"
+ *                                         -- the functions below
  */
 #ifndef OPENASR_GGML_MI355X_H
 #define OPENASR_GGML_MI355X_H
@@ -81,6 +82,18 @@ void ggml_backend_mi355x_refuse_next_launch(ggml_backend_t backend);
  * a message. Calls that overlap on one device race on the shared array. */
 enum ggml_status ggml_backend_mi355x_graph_compute_static(ggml_backend_t backend, struct ggml_cgraph * cgraph);
 size_t ggml_backend_mi355x_static_scratch_bytes(void);
+
+/* A buffer over device memory that the caller owns (another runtime's tensor):
+ * tensors placed in it with ggml_backend_tensor_alloc are read and written
+ * where they are. The memory must stay allocated until the buffer is freed
+ * (ggml_backend_buffer_free leaves it alone), and writes that other streams
+ * have pending must be finished before a compute or transfer reads it;
+ * computes and transfers here are finished when they return. NULL, with a
+ * message, unless ptr is 16-byte aligned and [ptr, ptr + size) lies in one
+ * allocation on the device. Q8_0 tensors hold the device's row layout (ggml_backend_tensor_set
+ * converts); other types are as ggml lays them out. Not counted in the memory
+ * ABI's ledger. */
+ggml_backend_buffer_t ggml_backend_mi355x_buffer_from_device_ptr(ggml_backend_dev_t device, void * ptr, size_t size);
 
 #ifdef __cplusplus
 }

@@ -88,6 +88,7 @@ struct buffer_ctx {
     device_state * dev;
     char * base;
     size_t size;
+    bool borrowed = false;  // the caller's memory: neither freed nor in the ledger
 };
 
 static void buf_free(ggml_backend_buffer_t buffer) {
@@ -95,8 +96,10 @@ static void buf_free(ggml_backend_buffer_t buffer) {
     error_scope scope(&c->dev->transfer_error);
     MI_CHECK(hipSetDevice(c->dev->hip_id));
     flush_uploads(c->dev, nullptr, true);  // queued writes into this buffer land before it is freed
-    MI_CHECK(hipFree(c->base));
-    ledger_sub(c->dev, c->size, false);
+    if (!c->borrowed) {
+        MI_CHECK(hipFree(c->base));
+        ledger_sub(c->dev, c->size, false);
+    }
     delete c;
 }
 
@@ -239,6 +242,27 @@ static ggml_backend_buffer_t buft_alloc_buffer(ggml_backend_buffer_type_t buft, 
     ledger_add(dev, alloc, false);
     buffer_ctx * c = new buffer_ctx{dev, (char *) p, alloc};
     return ggml_backend_buffer_init(buft, kBufferIface, c, size);
+}
+
+// a buffer over [ptr, ptr + size) of someone else's allocation on dev
+static ggml_backend_buffer_t borrow_buffer(device_state * dev, void * ptr, size_t size) {
+    if (!ptr || size == 0 || (uintptr_t) ptr % 16 != 0) {
+        std::fprintf(stderr, "mi355x: no buffer over %p + %zu: empty or not 16-byte aligned\n", ptr, size);
+        return nullptr;
+    }
+    MI_CHECK(hipSetDevice(dev->hip_id));
+    hipPointerAttribute_t at{};
+    hipDeviceptr_t base = nullptr;
+    size_t range = 0;
+    const bool ok = hipPointerGetAttributes(&at, ptr) == hipSuccess && at.type == hipMemoryTypeDevice &&
+                    at.device == dev->hip_id && hipMemGetAddressRange(&base, &range, (hipDeviceptr_t) ptr) == hipSuccess &&
+                    size <= range && (size_t) ((char *) ptr - (char *) base) <= range - size;
+    if (!ok) {
+        (void) hipGetLastError();
+        std::fprintf(stderr, "mi355x: %p + %zu is not memory of one allocation on %s\n", ptr, size, dev->name.c_str());
+        return nullptr;
+    }
+    return ggml_backend_buffer_init(&dev->buft, kBufferIface, new buffer_ctx{dev, (char *) ptr, size, true}, size);
 }
 
 static size_t buft_get_alignment(ggml_backend_buffer_type_t) { return 256; }
@@ -485,6 +509,8 @@ static void * reg_get_proc_address(ggml_backend_reg_t, const char * name) {
     if (std::strcmp(name, "ggml_backend_mi355x_set_hip_graphs") == 0) return (void *) ggml_backend_mi355x_set_hip_graphs;
     if (std::strcmp(name, "ggml_backend_mi355x_refuse_next_launch") == 0)
         return (void *) ggml_backend_mi355x_refuse_next_launch;
+    if (std::strcmp(name, "ggml_backend_mi355x_buffer_from_device_ptr") == 0)
+        return (void *) ggml_backend_mi355x_buffer_from_device_ptr;
     if (std::strcmp(name, "ggml_backend_memory_get_api_v1") == 0) return (void *) ggml_backend_memory_get_api_v1;
     return nullptr;
 }
@@ -579,6 +605,11 @@ void ggml_backend_mi355x_set_hip_graphs(ggml_backend_t backend, bool enabled) {
 void ggml_backend_mi355x_refuse_next_launch(ggml_backend_t backend) {
     if (!ggml_backend_is_mi355x(backend)) return;
     ((backend_state *) backend->context)->fail_next_launch = true;
+}
+
+ggml_backend_buffer_t ggml_backend_mi355x_buffer_from_device_ptr(ggml_backend_dev_t device, void * ptr, size_t size) {
+    device_state * dev = device_of(device);
+    return dev ? borrow_buffer(dev, ptr, size) : nullptr;
 }
 
 int ggml_backend_mi355x_device_count(void) { return (int) ggml_backend_mi355x_reg()->iface.get_device_count(nullptr); }

@@ -520,6 +520,9 @@ struct planner {
     bool fattn_kv32(const ggml_tensor * t, const fattn_args & a) const;
     void fattn_quant_out(int i, const ggml_tensor * t, fattn_args & a, const ggml_tensor *& view);
     bool plan_attn_step(int i, const ggml_tensor * t);
+    bool plan_mul_mat_id(const ggml_tensor * t);
+    void plan_ssm_conv(const ggml_tensor * t);
+    bool plan_ssm_scan(const ggml_tensor * t);
 };
 
 // The unfused attention chains of the graph (llm_naive_masked_attention,
@@ -1910,6 +1913,82 @@ bool planner::plan_naive(int i, const ggml_tensor * t) {
 // allocator that reuses dead blocks, a launch between may already have
 // written those bytes. Such a fusion is recorded in no_bypass / no_defer and
 // validate returns false, and the caller plans again without it.
+// whether a node's result overlaps one of its operands (an allocation that a
+// launch reading and writing in no particular order cannot take)
+static bool overlaps_operand(const ggml_tensor * t) {
+    for (int k = 0; k < GGML_MAX_SRC; k++)
+        if (t->src[k] && overlap(span_of(t), span_of(t->src[k]))) return true;
+    return false;
+}
+
+bool planner::plan_mul_mat_id(const ggml_tensor * t) {
+    const ggml_tensor *w = t->src[0], *x = t->src[1], *ids = t->src[2];
+    if (overlaps_operand(t)) return fail(t, "MUL_MAT_ID output overlaps its own input");
+    const int wtype = w->type;
+    mul_mat_id_args a{};
+    a.W = (const char *) w->data, a.W_nb1 = (int64_t) w->nb[1], a.W_nb2 = (int64_t) w->nb[2];
+    a.M = w->ne[1], a.K = w->ne[0], a.experts = w->ne[2];
+    a.b = (const char *) x->data, a.b_ne1 = x->ne[1], a.b_nb1 = (int64_t) x->nb[1], a.b_nb2 = (int64_t) x->nb[2];
+    a.ids = (const char *) ids->data, a.ids_nb0 = (int64_t) ids->nb[0], a.ids_nb1 = (int64_t) ids->nb[1];
+    a.used = ids->ne[0], a.pairs = ids->ne[0] * ids->ne[1];
+    a.out = (float *) t->data;
+    backend_state * b = be;
+    if (wtype == GGML_TYPE_Q8_0 || wtype == GGML_TYPE_Q4_K) {
+        const tview xv = make_view(x);
+        const int64_t N = x->ne[1] * x->ne[2];
+        act_need = std::max(act_need, act_bytes(wtype, a.K, N));
+        const int64_t K = a.K;
+        if (act_src != x || act_wtype != wtype) {
+            add_step([=](hipStream_t s) { launch_quantize_act(xv, wtype, act_carve(wtype, act_base(b), K, N), s); }, t,
+                     "quantize_act", {nullptr});
+            act_src = x;
+            act_wtype = wtype;
+        }
+        add_step(
+            [=](hipStream_t s) {
+                mul_mat_id_args r = a;
+                r.act = act_carve(wtype, act_base(b), K, N);
+                launch_mul_mat_id(wtype, r, s);
+            },
+            t, "mul_mat_id");
+        return true;
+    }
+    add_step([=](hipStream_t s) { launch_mul_mat_id(wtype, a, s); }, t, "mul_mat_id");
+    return true;
+}
+
+void planner::plan_ssm_conv(const ggml_tensor * t) {
+    const ggml_tensor *sx = t->src[0], *w = t->src[1];
+    ssm_conv_args a{};
+    a.sx = (const char *) sx->data;
+    a.sx_nb0 = (int64_t) sx->nb[0], a.sx_nb1 = (int64_t) sx->nb[1], a.sx_nb2 = (int64_t) sx->nb[2];
+    a.w = (const char *) w->data, a.w_nb1 = (int64_t) w->nb[1];
+    a.out = (float *) t->data;
+    a.channels = t->ne[0], a.tokens = t->ne[1], a.seqs = t->ne[2], a.taps = (int) w->ne[0];
+    const int ncu = n_cu;
+    add_step([=](hipStream_t s) { launch_ssm_conv(a, s, ncu); }, t, "ssm_conv");
+}
+
+bool planner::plan_ssm_scan(const ggml_tensor * t) {
+    if (overlaps_operand(t)) return fail(t, "SSM_SCAN output overlaps its own input");
+    const ggml_tensor *s0 = t->src[0], *x = t->src[1], *dt = t->src[2], *A = t->src[3], *B = t->src[4], *C = t->src[5];
+    ssm_scan_args a{};
+    a.s = (const char *) s0->data, a.x = (const char *) x->data, a.dt = (const char *) dt->data;
+    a.A = (const char *) A->data, a.B = (const char *) B->data, a.C = (const char *) C->data;
+    a.ids = (const int32_t *) t->src[6]->data;
+    a.s_nb3 = (int64_t) s0->nb[3];
+    a.x_nb1 = (int64_t) x->nb[1], a.x_nb2 = (int64_t) x->nb[2], a.x_nb3 = (int64_t) x->nb[3];
+    a.dt_nb1 = (int64_t) dt->nb[1], a.dt_nb2 = (int64_t) dt->nb[2], a.A_nb1 = (int64_t) A->nb[1];
+    a.B_nb1 = (int64_t) B->nb[1], a.B_nb2 = (int64_t) B->nb[2], a.B_nb3 = (int64_t) B->nb[3];
+    a.C_nb1 = (int64_t) C->nb[1], a.C_nb2 = (int64_t) C->nb[2], a.C_nb3 = (int64_t) C->nb[3];
+    a.n = (int) s0->ne[0], a.dim = (int) s0->ne[1], a.heads = (int) s0->ne[2], a.slots = s0->ne[3];
+    a.groups = (int) B->ne[1], a.tokens = x->ne[2], a.seqs = (int) x->ne[3], a.a_elem = A->ne[0] != 1;
+    a.y = (float *) t->data;
+    a.out = a.y + nelem(x);
+    add_step([=](hipStream_t s) { launch_ssm_scan(a, s); }, t, "ssm_scan");
+    return true;
+}
+
 bool planner::validate() {
     bool ok = true;
     auto written_between = [&](span src, int from, int to, bool allow_exact_at_to) {
@@ -2155,6 +2234,26 @@ bool planner::plan() {
             case GGML_OP_FLASH_ATTN_EXT:
                 if (!plan_fattn(i, t)) return false;
                 continue;
+            case GGML_OP_MUL_MAT_ID:
+                if (!plan_mul_mat_id(t)) return false;
+                continue;
+            case GGML_OP_ARGSORT: {
+                const tview dv = make_view(t), av = make_view(t->src[0]);
+                const int desc = t->op_params[0] == GGML_SORT_ORDER_DESC;
+                add_step([=](hipStream_t s) { launch_argsort(dv, av, desc, s); }, t, "argsort");
+                break;
+            }
+            case GGML_OP_SUM_ROWS: {
+                const tview dv = make_view(t), av = make_view(t->src[0]);
+                add_step([=](hipStream_t s) { launch_sum_rows(dv, av, s); }, t, "sum_rows");
+                break;
+            }
+            case GGML_OP_SSM_CONV:
+                plan_ssm_conv(t);
+                break;
+            case GGML_OP_SSM_SCAN:
+                if (!plan_ssm_scan(t)) return false;
+                break;
             default:
                 return fail(t, "no launcher");
         }
@@ -2679,6 +2778,52 @@ bool supports_op(const device_state * dev, const ggml_tensor * t) {
             const int64_t K = two_d ? kr->ne[0] * kr->ne[1] * kr->ne[2] : kr->ne[0] * kr->ne[1];
             return t->ne[0] == K && (!two_d || b->nb[1] == 4 * b->ne[0]) && t->ne[1] >= 1 &&
                    t->op_params[0] > 0 && t->op_params[4] > 0 && (!two_d || (t->op_params[1] > 0 && t->op_params[5] > 0));
+        }
+        case GGML_OP_MUL_MAT_ID: {
+            const ggml_tensor *w = t->src[0], *x = t->src[1], *ids = t->src[2];
+            if (!w || !f32(x) || !ids || !f32(t) || !is_contiguous(t)) return false;
+            if (ids->type != GGML_TYPE_I32 || w->ne[3] != 1 || x->nb[0] != 4) return false;
+            if (w->ne[0] != x->ne[0] || t->ne[0] != w->ne[1] || t->ne[1] != ids->ne[0] || t->ne[2] != ids->ne[1] ||
+                x->ne[2] != ids->ne[1] || x->ne[1] < 1 || ids->ne[0] % x->ne[1] != 0 || w->ne[0] < 1)
+                return false;
+            if (w->type == GGML_TYPE_Q8_0 || w->type == GGML_TYPE_Q4_K)
+                return is_contiguous(w) && x->nb[1] % 16 == 0 && x->nb[2] % 16 == 0 &&
+                       w->ne[0] % (w->type == GGML_TYPE_Q4_K ? 256 : 32) == 0;
+            return (w->type == GGML_TYPE_F16 || w->type == GGML_TYPE_F32) &&
+                   rows_contiguous(w, w->type == GGML_TYPE_F16 ? 2 : 4);
+        }
+        case GGML_OP_ARGSORT:
+            return t->type == GGML_TYPE_I32 && f32(t->src[0]) && rows_contiguous(t->src[0], 4) &&
+                   rows_contiguous(t, 4) && argsort_supported(t->ne[0]) &&
+                   (t->op_params[0] == GGML_SORT_ORDER_ASC || t->op_params[0] == GGML_SORT_ORDER_DESC);
+        case GGML_OP_SUM_ROWS:
+            return f32(t) && f32(t->src[0]) && rows_contiguous(t->src[0], 4);
+        case GGML_OP_SSM_CONV: {
+            const ggml_tensor *sx = t->src[0], *w = t->src[1];
+            return f32(t) && f32(sx) && f32(w) && is_contiguous(t) && rows_contiguous(w, 4) && sx->ne[3] == 1 &&
+                   w->ne[1] == sx->ne[1] && w->ne[0] >= 1 && w->ne[0] <= INT32_MAX && t->ne[0] == sx->ne[1] &&
+                   t->ne[1] == sx->ne[0] - (w->ne[0] - 1) && t->ne[2] == sx->ne[2];
+        }
+        case GGML_OP_SSM_SCAN: {
+            for (int k = 0; k < 6; k++)
+                if (!f32(t->src[k])) return false;
+            const ggml_tensor *s0 = t->src[0], *x = t->src[1], *dt = t->src[2], *A = t->src[3], *B = t->src[4],
+                              *C = t->src[5], *ids = t->src[6];
+            if (!ids || ids->type != GGML_TYPE_I32 || !f32(t) || !is_contiguous(t) || !is_contiguous(ids)) return false;
+            const int64_t n = s0->ne[0], p = s0->ne[1], h = s0->ne[2];
+            // a slot's states contiguous; the streams' rows too, at any token and sequence strides
+            if (s0->nb[0] != 4 || (p > 1 && s0->nb[1] != 4 * (size_t) n) || (h > 1 && s0->nb[2] != 4 * (size_t) (n * p)))
+                return false;
+            if (x->nb[0] != 4 || dt->nb[0] != 4 || B->nb[0] != 4 || C->nb[0] != 4 || A->nb[0] != 4) return false;
+            if (x->ne[0] != p || x->ne[1] != h || dt->ne[0] != h || dt->ne[1] != x->ne[2] || dt->ne[2] != x->ne[3] ||
+                dt->ne[3] != 1 || A->ne[1] != h || (A->ne[0] != 1 && A->ne[0] != n) || A->ne[2] != 1 || A->ne[3] != 1)
+                return false;
+            for (const ggml_tensor * y : {B, C})
+                if (y->ne[0] != n || y->ne[1] < 1 || h % y->ne[1] != 0 || y->ne[1] != B->ne[1] ||
+                    y->ne[2] != x->ne[2] || y->ne[3] != x->ne[3])
+                    return false;
+            if (ids->ne[0] != x->ne[3] || t->ne[0] != nelem(x) + n * p * h * x->ne[3]) return false;
+            return p <= INT32_MAX && h <= INT32_MAX && x->ne[3] <= INT32_MAX && ssm_scan_supported(n);
         }
         case GGML_OP_CPY:
         case GGML_OP_CONT:

@@ -384,6 +384,58 @@ struct im2col_args {
 };
 void launch_im2col(void * dst, int dst_f16, const char * src, const im2col_args & a, hipStream_t s);
 bool norm_supported(int64_t ne0);
+
+// GGML_OP_SSM_CONV: sx [taps - 1 + tokens, channels, seqs] f32 (byte strides),
+// w [taps, channels] (taps contiguous) -> out [channels, tokens, seqs]
+struct ssm_conv_args {
+    const char * sx;
+    int64_t sx_nb0, sx_nb1, sx_nb2;
+    const char * w;
+    int64_t w_nb1;
+    float * out;
+    int64_t channels, tokens, seqs;
+    int taps;
+};
+void launch_ssm_conv(const ssm_conv_args & a, hipStream_t s, int n_cu);
+
+// GGML_OP_SSM_SCAN: states s [n, dim, heads] a slot (contiguous, s_nb3 bytes
+// apart), x [dim, heads, tokens, seqs], dt [heads, tokens, seqs], B and C [n,
+// groups, tokens, seqs], A one value (a_elem: n values) a head; sequence i
+// starts from slot ids[i] (from zeros outside [0, slots)); y laid out as a
+// contiguous x, out the sequences' last states
+struct ssm_scan_args {
+    const char *s, *x, *dt, *A, *B, *C;
+    const int32_t * ids;
+    int64_t s_nb3, x_nb1, x_nb2, x_nb3, dt_nb1, dt_nb2, A_nb1;
+    int64_t B_nb1, B_nb2, B_nb3, C_nb1, C_nb2, C_nb3;
+    float *y, *out;
+    int64_t tokens, slots;
+    int n, dim, heads, groups, seqs, a_elem;
+};
+bool ssm_scan_supported(int64_t n);
+void launch_ssm_scan(const ssm_scan_args & a, hipStream_t s);
+
+// GGML_OP_MUL_MAT_ID: column (slot, token) of out [M, used, tokens] is
+// expert ids[slot, token]'s matrix times column (slot % b_ne1, token) of b;
+// zeros for an id outside [0, experts). Quantized weights read the columns
+// from act (quantized in b's order: token by token, b_ne1 a token).
+struct mul_mat_id_args {
+    const char * W;
+    int64_t W_nb1, W_nb2, M, K, experts;
+    const char * b;
+    int64_t b_ne1, b_nb1, b_nb2;
+    const char * ids;
+    int64_t ids_nb0, ids_nb1, used, pairs;
+    act_buffers act;
+    float * out;
+};
+void launch_mul_mat_id(int wtype, const mul_mat_id_args & a, hipStream_t s);
+
+// GGML_OP_ARGSORT: the indices that sort each row, equal elements in their
+// order, NaN the largest; GGML_OP_SUM_ROWS
+bool argsort_supported(int64_t n);
+void launch_argsort(const tview & d, const tview & a, int desc, hipStream_t s);
+void launch_sum_rows(const tview & d, const tview & a, hipStream_t s);
 // a one-wave kernel that returns after `us` microseconds of device wall clock
 void launch_spin_us(double us, int wall_clock_khz, hipStream_t s);
 

@@ -30,6 +30,7 @@ F32, F16, Q4_0, Q8_0, Q3_K, Q4_K, Q8_K, I32, I64 = 0, 1, 2, 8, 11, 12, 15, 26, 2
 TYPE_NAMES = {F32: "f32", F16: "f16", Q8_0: "q8_0", Q3_K: "q3_K", Q4_K: "q4_K", I32: "i32"}
 
 GGML_ROPE_TYPE_NEOX = 2
+GGML_SORT_ORDER_ASC, GGML_SORT_ORDER_DESC = 0, 1
 GGML_PREC_DEFAULT, GGML_PREC_F32 = 0, 10
 STATUS_SUCCESS = 0
 BUFFER_USAGE_WEIGHTS, BUFFER_USAGE_COMPUTE = 1, 2
@@ -112,6 +113,12 @@ def base() -> C.CDLL:
     _sig(lib, "ggml_norm", T, CTX, T, f)
     _sig(lib, "ggml_mul_mat_set_prec", None, T, i)
     _sig(lib, "ggml_set_rows", T, CTX, T, T, T)
+    _sig(lib, "ggml_mul_mat_id", T, CTX, T, T, T)
+    _sig(lib, "ggml_argsort", T, CTX, T, i)
+    _sig(lib, "ggml_top_k", T, CTX, T, i)
+    _sig(lib, "ggml_sum_rows", T, CTX, T)
+    _sig(lib, "ggml_ssm_conv", T, CTX, T, T)
+    _sig(lib, "ggml_ssm_scan", T, CTX, T, T, T, T, T, T, T)
     _sig(lib, "ggml_soft_max_ext", T, CTX, T, T, f, f)
     _sig(lib, "ggml_flash_attn_ext", T, CTX, T, T, T, T, f, f, f)
     _sig(lib, "ggml_flash_attn_ext_set_prec", None, T, i)
@@ -143,6 +150,7 @@ def base() -> C.CDLL:
     _sig(lib, "ggml_backend_tensor_set", i, T, C.c_void_p, sz, sz)
     _sig(lib, "ggml_backend_tensor_get", i, T, C.c_void_p, sz, sz)
     _sig(lib, "ggml_backend_tensor_memset", i, T, C.c_uint8, sz, sz)
+    _sig(lib, "ggml_backend_tensor_alloc", i, C.c_void_p, T, C.c_void_p)
     _sig(lib, "ggml_backend_alloc_ctx_tensors_from_buft", C.c_void_p, CTX, C.c_void_p)
     _sig(lib, "ggml_backend_buffer_free", None, C.c_void_p)
     _sig(lib, "ggml_backend_buffer_set_usage", None, C.c_void_p, i)
@@ -221,6 +229,8 @@ class Plugin:
                                                                C.POINTER(C.c_float), C.c_int, C.c_char_p, C.c_int]
         self.cdll.ggml_backend_mi355x_set_hip_graphs.restype = None
         self.cdll.ggml_backend_mi355x_set_hip_graphs.argtypes = [C.c_void_p, C.c_bool]
+        self.cdll.ggml_backend_mi355x_buffer_from_device_ptr.restype = C.c_void_p
+        self.cdll.ggml_backend_mi355x_buffer_from_device_ptr.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t]
 
     @property
     def name(self) -> str:
@@ -264,6 +274,7 @@ class Graph:
         self.gf = None
         self.galloc = None
         self.wbuf = None
+        self.borrowed = []  # buffers over memory of others, and that memory
         self.lib = lib
 
     # tensors
@@ -278,6 +289,29 @@ class Graph:
             self.lib.ggml_set_name(t, name.encode())
         if not weight:
             self.lib.ggml_set_input(t)
+        return t
+
+    def over(self, typ, *ne, memory):
+        """A graph input whose bytes are the caller's device memory (a contiguous
+        torch tensor, say): read, and written by ops that write in place, where
+        they are, never copied. Writes into it that the device may still be
+        making must be waited for before a compute; a compute's own are done
+        when it returns. The graph keeps `memory` alive."""
+        if typ == Q8_0:
+            raise ValueError("over: Q8_0 tensors hold the device's row layout; allocate and set() them")
+        if not memory.is_contiguous():
+            raise ValueError("over: the memory is not contiguous")
+        t = self.new(typ, *ne)
+        n = self.lib.ggml_nbytes(t)
+        if memory.numel() * memory.element_size() != n:
+            raise ValueError(f"over: {memory.numel() * memory.element_size()} bytes for a {n}-byte tensor")
+        p = plugin()
+        buf = p.cdll.ggml_backend_mi355x_buffer_from_device_ptr(p.dev, memory.data_ptr(), n)
+        if not buf:
+            raise ValueError("over: not memory of the plugin's device")
+        self.borrowed.append((buf, memory))
+        if self.lib.ggml_backend_tensor_alloc(buf, t, memory.data_ptr()) != 0:
+            raise RuntimeError("over: ggml_backend_tensor_alloc failed")
         return t
 
     def build(self, *outputs):
@@ -327,6 +361,9 @@ class Graph:
         if self.wbuf:
             lib.ggml_backend_buffer_free(self.wbuf)
             self.wbuf = None
+        for buf, _ in self.borrowed:
+            lib.ggml_backend_buffer_free(buf)
+        self.borrowed = []
         if self.ctx:
             lib.ggml_free(self.ctx)
             self.ctx = None

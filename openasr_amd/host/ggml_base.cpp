@@ -13,6 +13,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 
 namespace {
 
@@ -68,6 +69,15 @@ type_info type_table(enum ggml_type t) {
 #define GB_REQUIRE(cond, msg) \
     do {                      \
         if (!(cond)) die(msg); \
+    } while (0)
+
+// the same for constructors that refuse: a message and a null result
+#define GB_REFUSE_UNLESS(cond, msg)                        \
+    do {                                                   \
+        if (!(cond)) {                                     \
+            std::fprintf(stderr, "ggml-base: %s\n", msg);  \
+            return nullptr;                                \
+        }                                                  \
     } while (0)
 
 }  // namespace
@@ -437,6 +447,94 @@ struct ggml_tensor * ggml_mul_mat(struct ggml_context * ctx, struct ggml_tensor 
 }
 
 void ggml_mul_mat_set_prec(struct ggml_tensor * a, enum ggml_prec prec) { a->op_params[0] = (int32_t) prec; }
+
+struct ggml_tensor * ggml_mul_mat_id(struct ggml_context * ctx, struct ggml_tensor * as, struct ggml_tensor * b,
+                                     struct ggml_tensor * ids) {
+    GB_REFUSE_UNLESS(as && b && ids, "mul_mat_id: null operand");
+    GB_REFUSE_UNLESS(ids->type == GGML_TYPE_I32 && b->type == GGML_TYPE_F32, "mul_mat_id: f32 columns, i32 ids");
+    GB_REFUSE_UNLESS(as->ne[3] == 1 && b->ne[3] == 1 && ids->ne[2] == 1 && ids->ne[3] == 1,
+                     "mul_mat_id: experts and columns in three dims, ids in two");
+    GB_REFUSE_UNLESS(as->ne[0] == b->ne[0] && ids->ne[1] == b->ne[2], "mul_mat_id: shapes do not contract");
+    GB_REFUSE_UNLESS(b->ne[1] > 0 && ids->ne[0] % b->ne[1] == 0, "mul_mat_id: columns do not divide the slots");
+    GB_REFUSE_UNLESS(!ggml_is_transposed(as), "mul_mat_id: experts must not be transposed");
+    const int64_t ne[4] = {as->ne[1], ids->ne[0], b->ne[2], 1};
+    ggml_tensor * r = ggml_new_tensor(ctx, GGML_TYPE_F32, 4, ne);
+    if (!r) return nullptr;
+    r->op = GGML_OP_MUL_MAT_ID;
+    r->src[0] = as;
+    r->src[1] = b;
+    r->src[2] = ids;
+    return r;
+}
+
+struct ggml_tensor * ggml_argsort(struct ggml_context * ctx, struct ggml_tensor * a, enum ggml_sort_order order) {
+    GB_REFUSE_UNLESS(a && a->type == GGML_TYPE_F32, "argsort: needs f32 rows");
+    GB_REFUSE_UNLESS(order == GGML_SORT_ORDER_ASC || order == GGML_SORT_ORDER_DESC, "argsort: unknown order");
+    GB_REFUSE_UNLESS(a->ne[0] <= INT32_MAX, "argsort: rows past i32 indices");
+    ggml_tensor * r = ggml_new_tensor(ctx, GGML_TYPE_I32, GGML_MAX_DIMS, a->ne);
+    if (!r) return nullptr;
+    r->op_params[0] = (int32_t) order;
+    r->op = GGML_OP_ARGSORT;
+    r->src[0] = a;
+    return r;
+}
+
+struct ggml_tensor * ggml_top_k(struct ggml_context * ctx, struct ggml_tensor * a, int k) {
+    GB_REFUSE_UNLESS(a && k >= 1 && (int64_t) k <= a->ne[0], "top_k: k outside the row");
+    ggml_tensor * r = ggml_argsort(ctx, a, GGML_SORT_ORDER_DESC);
+    if (!r) return nullptr;
+    return ggml_view_4d(ctx, r, k, r->ne[1], r->ne[2], r->ne[3], r->nb[1], r->nb[2], r->nb[3], 0);
+}
+
+struct ggml_tensor * ggml_sum_rows(struct ggml_context * ctx, struct ggml_tensor * a) {
+    GB_REFUSE_UNLESS(a && a->type == GGML_TYPE_F32, "sum_rows: needs f32 rows");
+    const int64_t ne[4] = {1, a->ne[1], a->ne[2], a->ne[3]};
+    ggml_tensor * r = ggml_new_tensor(ctx, GGML_TYPE_F32, 4, ne);
+    if (!r) return nullptr;
+    r->op = GGML_OP_SUM_ROWS;
+    r->src[0] = a;
+    return r;
+}
+
+struct ggml_tensor * ggml_ssm_conv(struct ggml_context * ctx, struct ggml_tensor * sx, struct ggml_tensor * c) {
+    GB_REFUSE_UNLESS(sx && c && sx->type == GGML_TYPE_F32 && c->type == GGML_TYPE_F32, "ssm_conv: f32 operands");
+    GB_REFUSE_UNLESS(sx->ne[3] == 1 && c->ne[2] == 1 && c->ne[3] == 1, "ssm_conv: columns in three dims, taps in two");
+    GB_REFUSE_UNLESS(c->ne[0] >= 1 && c->ne[1] == sx->ne[1], "ssm_conv: taps and channels differ");
+    GB_REFUSE_UNLESS(sx->ne[0] >= c->ne[0] - 1, "ssm_conv: fewer columns than the taps carry");
+    const int64_t ne[4] = {sx->ne[1], sx->ne[0] - (c->ne[0] - 1), sx->ne[2], 1};
+    ggml_tensor * r = ggml_new_tensor(ctx, GGML_TYPE_F32, 4, ne);
+    if (!r) return nullptr;
+    r->op = GGML_OP_SSM_CONV;
+    r->src[0] = sx;
+    r->src[1] = c;
+    return r;
+}
+
+struct ggml_tensor * ggml_ssm_scan(struct ggml_context * ctx, struct ggml_tensor * s, struct ggml_tensor * x,
+                                   struct ggml_tensor * dt, struct ggml_tensor * A, struct ggml_tensor * B,
+                                   struct ggml_tensor * C, struct ggml_tensor * ids) {
+    GB_REFUSE_UNLESS(s && x && dt && A && B && C && ids, "ssm_scan: null operand");
+    for (const ggml_tensor * t : {s, x, dt, A, B, C})
+        GB_REFUSE_UNLESS(t->type == GGML_TYPE_F32, "ssm_scan: f32 operands");
+    GB_REFUSE_UNLESS(ids->type == GGML_TYPE_I32, "ssm_scan: i32 ids");
+    const int64_t n = s->ne[0], p = s->ne[1], h = s->ne[2], t = x->ne[2], ns = x->ne[3];
+    GB_REFUSE_UNLESS(n >= 1 && p >= 1 && h >= 1, "ssm_scan: empty state");
+    GB_REFUSE_UNLESS(x->ne[0] == p && x->ne[1] == h, "ssm_scan: x does not match the state");
+    GB_REFUSE_UNLESS(dt->ne[0] == h && dt->ne[1] == t && dt->ne[2] == ns && dt->ne[3] == 1, "ssm_scan: dt's shape");
+    GB_REFUSE_UNLESS((A->ne[0] == 1 || A->ne[0] == n) && A->ne[1] == h && A->ne[2] == 1 && A->ne[3] == 1,
+                     "ssm_scan: A's shape");
+    GB_REFUSE_UNLESS(B->ne[0] == n && B->ne[1] >= 1 && h % B->ne[1] == 0 && B->ne[2] == t && B->ne[3] == ns,
+                     "ssm_scan: B's shape");
+    for (int d = 0; d < GGML_MAX_DIMS; d++) GB_REFUSE_UNLESS(C->ne[d] == B->ne[d], "ssm_scan: C's shape is not B's");
+    GB_REFUSE_UNLESS(ids->ne[0] == ns && ids->ne[1] == 1 && ids->ne[2] == 1 && ids->ne[3] == 1,
+                     "ssm_scan: one id a sequence");
+    ggml_tensor * r = ggml_new_tensor_1d(ctx, GGML_TYPE_F32, ggml_nelements(x) + n * p * h * ns);
+    if (!r) return nullptr;
+    r->op = GGML_OP_SSM_SCAN;
+    ggml_tensor * src[7] = {s, x, dt, A, B, C, ids};
+    for (int i = 0; i < 7; i++) r->src[i] = src[i];
+    return r;
+}
 
 struct ggml_tensor * ggml_get_rows(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b) {
     GB_REQUIRE(a->ne[2] == b->ne[1] && b->ne[3] == 1 && b->type == GGML_TYPE_I32, "get_rows: bad shapes");
