@@ -1985,7 +1985,10 @@ bool planner::plan_ssm_scan(const ggml_tensor * t) {
     a.groups = (int) B->ne[1], a.tokens = x->ne[2], a.seqs = (int) x->ne[3], a.a_elem = A->ne[0] != 1;
     a.y = (float *) t->data;
     a.out = a.y + nelem(x);
-    add_step([=](hipStream_t s) { launch_ssm_scan(a, s); }, t, "ssm_scan");
+    gen_need = std::max(gen_need, ssm_scan_scratch_bytes(a, n_cu));
+    backend_state * b = be;
+    const int ncu = n_cu;
+    add_step([=](hipStream_t s) { launch_ssm_scan(a, gen_base(b), s, ncu); }, t, "ssm_scan");
     return true;
 }
 

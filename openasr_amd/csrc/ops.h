@@ -413,7 +413,8 @@ struct ssm_scan_args {
     int n, dim, heads, groups, seqs, a_elem;
 };
 bool ssm_scan_supported(int64_t n);
-void launch_ssm_scan(const ssm_scan_args & a, hipStream_t s);
+size_t ssm_scan_scratch_bytes(const ssm_scan_args & a, int n_cu);
+void launch_ssm_scan(const ssm_scan_args & a, void * scratch, hipStream_t s, int n_cu);
 
 // GGML_OP_MUL_MAT_ID: column (slot, token) of out [M, used, tokens] is
 // expert ids[slot, token]'s matrix times column (slot % b_ne1, token) of b;

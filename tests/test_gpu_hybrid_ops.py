@@ -188,7 +188,7 @@ def run_scan(ggml, gpu, s, x, dt, A, B, C, ids, times=3):
 SCAN = [(1, 1, 2, 64, 1, 128, False), (3, 1, 6, 64, 2, 64, False), (5, 1, 3, 32, 1, 128, False), (2, 2, 4, 64, 1, 128, False),
         (1, 63, 4, 64, 1, 128, False), (2, 64, 4, 64, 2, 128, False), (1, 65, 2, 64, 1, 64, False),
         (2, 200, 3, 64, 3, 128, False), (1, 257, 4, 32, 1, 128, False), (1, 130, 2, 24, 1, 20, False),
-        (1, 70, 2, 128, 1, 256, False), (2, 90, 3, 7, 1, 5, False), (1, 333, 2, 64, 2, 64, False),
+        (1, 70, 2, 128, 1, 256, False), (1, 1100, 2, 64, 1, 128, False), (3, 600, 5, 80, 5, 100, False), (2, 90, 3, 7, 1, 5, False), (1, 333, 2, 64, 2, 64, False),
         (1, 1, 40, 1, 1, 16, True), (2, 33, 40, 1, 1, 16, True), (1, 300, 70, 1, 1, 16, True), (1, 45, 6, 4, 2, 16, True),
         (2, 20, 3, 64, 1, 128, True), (1, 700, 5, 1, 1, 8, True), (1, 0, 4, 64, 1, 128, False), (2, 0, 8, 1, 1, 16, True)]
 
@@ -221,6 +221,51 @@ def test_ssm_scan_slots_and_decays(ggml, gpu, T, elem):
     wy, by, wh, bh = scan64(s, x, dt, A, B, C, ids)
     within(y, wy, by + 1e-30, "y")
     within(h, wh, bh + 1e-30, "states")
+
+
+@pytest.mark.parametrize("T", [1, 70, 330])
+@pytest.mark.parametrize("what", ["x", "B", "C", "dt", "state", "long_dt"])
+def test_ssm_scan_keeps_non_finite_values_where_they_are(ggml, gpu, T, what):
+    """a NaN or infinity reaches what the recurrence takes it to: not the
+    tokens before it, not other channels, heads or sequences. A step of dt
+    1e9 forgets the state at once, without spoiling the steps after it."""
+    rng = np.random.default_rng(T)
+    S, H, P, n, at = 2, 3, 64, 64, T // 2
+    s, x, dt, A, B, C = scan_inputs(rng, S, T, H, P, 1, n, False, S)
+    if what == "x":
+        x[0, at, 1, 5] = np.nan
+    elif what == "state":
+        s[0, 1, 5, 3] = np.inf
+    elif what == "long_dt":
+        dt[0, at, 1] = 1e9
+    else:
+        {"B": B, "C": C, "dt": dt[..., None]}[what][0, at, 0, 0] = np.nan
+    y, h = run_scan(ggml, gpu, s, x, dt, A, B, C, range(S))
+    with np.errstate(all="ignore"):
+        wy, by, wh, bh = scan64(s, x, dt, A, B, C, range(S))
+    for got, want, bound in ((y, wy, by), (h, wh, bh)):
+        fine = np.isfinite(want)
+        assert np.array_equal(np.isfinite(got), fine)
+        within(got[fine], want[fine], bound[fine] + 1e-30, what)
+
+
+@pytest.mark.parametrize("scale", [1e-20, 1e-6, 1e12])
+@pytest.mark.parametrize("T", [2, 130])
+def test_ssm_scan_scales(ggml, gpu, T, scale):
+    """inputs far from one: every operand's own scale"""
+    rng = np.random.default_rng(4)
+    S, H, P, n = 1, 3, 64, 128
+    s, x, dt, A, B, C = scan_inputs(rng, S, T, H, P, 1, n, False, S)
+    x[:, :, 0] *= scale
+    B[:, ::3] *= scale
+    C[:, 1::2] /= np.float32(scale)
+    x[..., 5] *= scale
+    x[:, 3::4, 1] *= scale
+    a = (s, x, dt, A, B, C, range(S))
+    y, h = run_scan(ggml, gpu, *a)
+    wy, by, wh, bh = scan64(*a)
+    within(h, wh, bh + 1e-30, "states")
+    within(y, wy, by + 1e-30, "y")
 
 
 @pytest.mark.parametrize("T", [1, 5, 140])
