@@ -100,8 +100,8 @@ __global__ __launch_bounds__(256) void k_ssm_scan_rows(ssm_scan_args a) {
 // k_ssm_split makes the operands that a group's heads share: C in rows and B
 // in columns, split, with their scales, and C_t . B_j. k_ssm_chunks gives a
 // workgroup a (sequence, head, 64 channels, segment of chunks): wave w owns
-// the state's rows n in its quarter (accumulator layout) and, for y, 16
-// tokens. Where there are few heads the sequence is cut into segments: the
+// the state's rows n in its quarter (in accumulators) and, for y, 16 tokens.
+// k_ssm_split also sums the heads' log decays. Where there are few heads the sequence is cut into segments: the
 // first pass (OUT false) makes each segment's own state from zeros, and the
 // second starts from the earlier segments' states, decayed and added.
 //
@@ -111,8 +111,10 @@ __global__ __launch_bounds__(256) void k_ssm_scan_rows(ssm_scan_args a) {
 // (ssm_chunk_slow), where a value reaches what the recurrence takes it to.
 
 typedef float ssm_v4f __attribute__((ext_vector_type(4)));
+typedef float ssm_v2f __attribute__((ext_vector_type(2)));
 typedef _Float16 ssm_v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 ssm_v4h __attribute__((ext_vector_type(4)));
+typedef _Float16 ssm_v2h __attribute__((ext_vector_type(2)));
 
 constexpr int kSsmL = 64;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -129,6 +131,12 @@ __device__ __forceinline__ int ssm_scale(uint32_t bits) {
     return bits == 0 ? 0 : min(13 - e, 74);
 }
 __device__ __forceinline__ uint32_t ssm_mag(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+// an element at a uniform base, a lane's byte offset and a constant one: the
+// address form a load takes without 64-bit vector arithmetic
+template <typename T>
+__device__ __forceinline__ T & ssm_at(const void * base, uint32_t off, int fixed = 0) {
+    return *(T *) ((char *) base + off + fixed);
+}
 template <int W>
 __device__ __forceinline__ uint32_t ssm_group_max(uint32_t v) {
 #pragma unroll
@@ -137,22 +145,93 @@ __device__ __forceinline__ uint32_t ssm_group_max(uint32_t v) {
 }
 __device__ __forceinline__ bool ssm_finite(uint32_t mag) { return mag < 0x7F800000u; }
 
+// f16 hi + lo of N scaled f32 values
+template <int N, typename V>
+__device__ __forceinline__ void ssm_halves(const float (&x)[N], V & hi, V & lo) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+        const ssm_v2f v = {x[e], x[e + 1]};
+        const ssm_v2h h = __builtin_convertvector(v, ssm_v2h);
+        const ssm_v2f d = {fmaf(x[e], 1.0f, -(float) h.x), fmaf(x[e + 1], 1.0f, -(float) h.y)};
+        const ssm_v2h l = __builtin_convertvector(d, ssm_v2h);
+        hi[e] = h.x, hi[e + 1] = h.y;
+        lo[e] = l.x, lo[e + 1] = l.y;
+    }
+}
+
+// what a chunk's decays need besides the tokens' own
+struct ssm_decay {
+    double total;       // its log2 decay
+    int e_dt, e_left;   // the exponents of the largest step, and of the largest step times the decay after it
+    int odd, pad;       // outside what the matrix form takes
+};
+struct ssm_flags {
+    int bad[4];  // a quarter's rows hold a non-finite value
+    int kb;      // B's operand is its value times 2^kb
+    int pad[3];
+};
+
 // the operands' places in scratch, for NP = the padded state size
 struct ssm_chunk_args {
     ssm_scan_args a;
-    _Float16 *c_hi, *c_lo;  // [seq, group][token][NP]
-    _Float16 *b_hi, *b_lo;  // [seq, group][chunk][NP][64 tokens]
-    float *c_s, *b_s;       // [seq, group][token]: a row's value is its operand times this
-    float * cb;             // [seq, group][chunk][64][64]: C_t . B_j for 16-blocks of j up to t's
-    int * bad;              // [seq, group][chunk][4]: whether a quarter's rows hold a non-finite value
+    _Float16 *c_hi, *c_lo;  // [seq, group][token][NP], each token's row scaled
+    _Float16 *b_hi, *b_lo;  // [seq, group][chunk][NP][64 tokens], each chunk scaled
+    float * c_s;            // [seq, group][token]: a row of C is its operand times this
+    float * cb;             // [seq, group][chunk][64][64]: C_t . B_j for j <= t (zeros in the 16-blocks past t's), rows scaled
+    float * cb_s;           // [seq, group][token]: a row of it is its operand times this
+    ssm_flags * flags;      // [seq, group][chunk]
+    // the heads' decays, c_t the sum of the log2 decays from the chunk's start
+    float *dt, *left;       // [seq, head][token]: the step and the step times 2^(c_L - c_t), over 2^(exponents)
+    float *whole, *frac;    // [seq, head][token]: c_t's whole and fractional part
+    ssm_decay * decay;      // [seq, head][chunk]
     float * seg_state;      // [seq, head, channel block][segment][64][NP]
     double * seg_decay;     // [seq, head][segment]: its log2 decay
     int64_t chunks;
     int segs, seg_chunks, pblocks;
+    uint32_t split_blocks;
 };
 
+// the decays of one (sequence, head, chunk): a lane a token, the sums in f64
+__device__ __forceinline__ void ssm_decays(const ssm_chunk_args & q, int64_t unit) {
+    const ssm_scan_args & a = q.a;
+    const int lane = threadIdx.x & 63;
+    const int64_t c = unit % q.chunks, sh = unit / q.chunks;
+    if (sh >= (int64_t) a.seqs * a.heads) return;
+    const int h = (int) (sh % a.heads), s = (int) (sh / a.heads);
+    const int64_t t = c * kSsmL + lane, at = sh * q.chunks * kSsmL + t;
+    const float A = *(const float *) (a.A + h * a.A_nb1);
+    const float dt = t < a.tokens ? ssm_softplus(*(const float *) (a.dt + 4 * h + t * a.dt_nb1 + s * a.dt_nb2)) : 0.0f;
+    double cum = (double) dt * (double) A * 1.4426950408889634074;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double v = __shfl_up(cum, o);
+        if (lane >= o) cum += v;
+    }
+    const double total = __shfl(cum, 63), whole = floor(cum);
+    const float left = dt * __builtin_amdgcn_exp2f((float) (total - cum));
+    // the largest step's exponents: the operands' scales are bounded by them
+    const uint32_t md = ssm_group_max<64>(ssm_mag(dt)), ml = ssm_group_max<64>(ssm_mag(left));
+    ssm_decay d{};
+    d.total = total;
+    d.e_dt = max((int) (md >> 23) - 127, -60);
+    d.e_left = max((int) (ml >> 23) - 127, -60);
+    // A positive, or decays whose whole parts leave f32's exact range
+    d.odd = !(total <= 0.0 && total > -8388608.0) || !ssm_finite(md);
+    q.dt[at] = dt * ssm_pow2(-d.e_dt);
+    q.left[at] = left * ssm_pow2(-d.e_left);
+    q.whole[at] = (float) whole;
+    q.frac[at] = (float) (cum - whole);
+    if (lane == 0) q.decay[sh * q.chunks + c] = d;
+}
+
+// the first blocks the shared operands, a quarter of a chunk's rows each; the
+// others the heads' decays, a wave a chunk
 template <int NP>
 __global__ __launch_bounds__(256) void k_ssm_split(ssm_chunk_args q) {
+    if (blockIdx.x >= q.split_blocks) {
+        ssm_decays(q, (int64_t) (blockIdx.x - q.split_blocks) * 4 + (threadIdx.x >> 6));
+        return;
+    }
     constexpr int kRow = NP + 4;
     __shared__ float sb[kSsmL][kRow];
     __shared__ float sc[16][kRow];
@@ -161,85 +240,126 @@ __global__ __launch_bounds__(256) void k_ssm_split(ssm_chunk_args q) {
     const int64_t chunk = blockIdx.x / 4 % q.chunks, sg = blockIdx.x / 4 / q.chunks;
     const int s = (int) (sg / a.groups), g = (int) (sg % a.groups);
     const int64_t t0 = chunk * kSsmL;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const char * B = a.B + g * a.B_nb1 + s * a.B_nb3;
     const char * C = a.C + g * a.C_nb1 + s * a.C_nb3;
-    for (int i = tid; i < kSsmL * NP; i += 256) {
-        const int t = i / NP, n = i % NP;
-        const bool ok = t0 + t < a.tokens && n < a.n;
-        sb[t][n] = ok ? ((const float *) (B + (t0 + t) * a.B_nb2))[n] : 0.0f;
+    uint32_t mb = 0;
+    const bool vec = a.n % 4 == 0 && (((uintptr_t) B | (uintptr_t) C | (uintptr_t) a.B_nb2 | (uintptr_t) a.C_nb2) & 15) == 0;
+    if (vec) {
+        float4 vb[kSsmL * NP / 1024], vc[16 * NP / 1024];
+#pragma unroll
+        for (int k = 0; k < kSsmL * NP / 1024; k++) {
+            const int i = tid + 256 * k, t = i / (NP / 4), n = i % (NP / 4) * 4;
+            const bool ok = t0 + t < a.tokens && n < a.n;
+            vb[k] = *(const float4 *) (B + (ok ? t0 + t : 0) * a.B_nb2 + (ok ? 4 * n : 0));
+            if (!ok) vb[k] = make_float4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < 16 * NP / 1024; k++) {
+            const int i = tid + 256 * k, t = 16 * part + i / (NP / 4), n = i % (NP / 4) * 4;
+            const bool ok = t0 + t < a.tokens && n < a.n;
+            vc[k] = *(const float4 *) (C + (ok ? t0 + t : 0) * a.C_nb2 + (ok ? 4 * n : 0));
+            if (!ok) vc[k] = make_float4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < kSsmL * NP / 1024; k++) {
+            const int i = tid + 256 * k;
+            *(float4 *) &sb[i / (NP / 4)][i % (NP / 4) * 4] = vb[k];
+            mb = max(max(mb, max(ssm_mag(vb[k].x), ssm_mag(vb[k].y))), max(ssm_mag(vb[k].z), ssm_mag(vb[k].w)));
+        }
+#pragma unroll
+        for (int k = 0; k < 16 * NP / 1024; k++) {
+            const int i = tid + 256 * k;
+            *(float4 *) &sc[i / (NP / 4)][i % (NP / 4) * 4] = vc[k];
+        }
+    } else {
+        for (int i = tid; i < kSsmL * NP; i += 256) {
+            const int t = i / NP, n = i % NP;
+            const bool ok = t0 + t < a.tokens && n < a.n;
+            sb[t][n] = ok ? ((const float *) (B + (t0 + t) * a.B_nb2))[n] : 0.0f;
+            mb = max(mb, ssm_mag(sb[t][n]));
+        }
+        for (int i = tid; i < 16 * NP; i += 256) {
+            const int t = 16 * part + i / NP, n = i % NP;
+            const bool ok = t0 + t < a.tokens && n < a.n;
+            sc[i / NP][n] = ok ? ((const float *) (C + (t0 + t) * a.C_nb2))[n] : 0.0f;
+        }
     }
-    for (int i = tid; i < 16 * NP; i += 256) {
-        const int t = 16 * part + i / NP, n = i % NP;
-        const bool ok = t0 + t < a.tokens && n < a.n;
-        sc[i / NP][n] = ok ? ((const float *) (C + (t0 + t) * a.C_nb2))[n] : 0.0f;
-    }
+    __shared__ uint32_t s_mb[4];
+    mb = ssm_group_max<64>(mb);
+    if (lane == 0) s_mb[wave] = mb;
     __syncthreads();
+    mb = max(max(s_mb[0], s_mb[1]), max(s_mb[2], s_mb[3]));
     const int64_t tp = q.chunks * kSsmL;
-    // rows: 16 threads each
+    // C's rows: 16 threads each
     const int row = tid / 16, sub = tid % 16;
-    uint32_t mb = 0, mc = 0;
-    for (int n = sub; n < NP; n += 16) {
-        mb = max(mb, ssm_mag(sb[16 * part + row][n]));
-        mc = max(mc, ssm_mag(sc[row][n]));
-    }
-    mb = ssm_group_max<16>(mb);
+    uint32_t mc = 0;
+    for (int n = sub; n < NP; n += 16) mc = max(mc, ssm_mag(sc[row][n]));
     mc = ssm_group_max<16>(mc);
     const int kb = ssm_finite(mb) ? ssm_scale(mb) : 0, kc = ssm_finite(mc) ? ssm_scale(mc) : 0;
     const int any = __syncthreads_or(!ssm_finite(mb) || !ssm_finite(mc));
-    if (tid == 0) q.bad[(sg * q.chunks + chunk) * 4 + part] = any;
-    const int64_t t = t0 + 16 * part + row;
-    if (sub == 0) {
-        q.b_s[sg * tp + t] = ssm_pow2(-kb);
-        q.c_s[sg * tp + t] = ssm_pow2(-kc);
+    if (tid == 0) {
+        q.flags[sg * q.chunks + chunk].bad[part] = any;
+        if (part == 0) q.flags[sg * q.chunks + chunk].kb = kb;
     }
+    const int64_t t = t0 + 16 * part + row;
+    if (sub == 0) q.c_s[sg * tp + t] = ssm_pow2(-kc);
     const float fc = ssm_pow2(kc), fb = ssm_pow2(kb);
     for (int n = 8 * sub; n < NP; n += 128) {
+        float v[8];
         ssm_v8h hi, lo;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float v = sc[row][n + e] * fc;
-            hi[e] = (_Float16) v;
-            lo[e] = (_Float16) (v - (float) hi[e]);
-        }
+        for (int e = 0; e < 8; e++) v[e] = sc[row][n + e] * fc;
+        ssm_halves(v, hi, lo);
         *(ssm_v8h *) (q.c_hi + (sg * tp + t) * NP + n) = hi;
         *(ssm_v8h *) (q.c_lo + (sg * tp + t) * NP + n) = lo;
     }
-    // C . B: wave w the block of tokens 16 w .. (not past its own), K in an
-    // order both operands share
-    const int lane = tid & 63, wave = tid >> 6, r = lane & 15, gq = lane >> 4;
-    if (wave <= part) {
-        ssm_v4f acc = {0, 0, 0, 0};
-        for (int n = 4 * gq; n < NP; n += 16) {
-            const float4 x = *(const float4 *) &sc[r][n], y = *(const float4 *) &sb[16 * wave + r][n];
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, y.x, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, y.y, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, y.z, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, y.w, acc, 0, 0, 0);
-        }
-        float * cb = q.cb + ((sg * q.chunks + chunk) * kSsmL + 16 * part) * kSsmL + 16 * wave;
-#pragma unroll
-        for (int i = 0; i < 4; i++) cb[(4 * gq + i) * kSsmL + r] = acc[i];
-    }
-    // B's columns: the rows scaled in place, then 16 tokens of a column a thread
-    __syncthreads();
-    for (int n = sub; n < NP; n += 16) sb[16 * part + row][n] *= fb;
-    __syncthreads();
+    // B's columns: 16 tokens of one a thread
     if (tid < NP) {
         _Float16 * oh = q.b_hi + ((sg * q.chunks + chunk) * NP + tid) * kSsmL + 16 * part;
         _Float16 * ol = q.b_lo + ((sg * q.chunks + chunk) * NP + tid) * kSsmL + 16 * part;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
+            float v[8];
             ssm_v8h hi, lo;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = sb[16 * part + 8 * h + e][tid];
-                hi[e] = (_Float16) v;
-                lo[e] = (_Float16) (v - (float) hi[e]);
-            }
+            for (int e = 0; e < 8; e++) v[e] = sb[16 * part + 8 * h + e][tid] * fb;
+            ssm_halves(v, hi, lo);
             *(ssm_v8h *) (oh + 8 * h) = hi;
             *(ssm_v8h *) (ol + 8 * h) = lo;
         }
+    }
+    // C . B: wave w the 16-block of tokens j from 16 w on, K in an order both operands share
+    const int r = lane & 15, gq = lane >> 4;
+    ssm_v4f acc = {0, 0, 0, 0};
+    if (wave <= part) {
+        ssm_v4f acc2 = {0, 0, 0, 0};
+#pragma unroll 4
+        for (int n = 4 * gq; n < NP; n += 16) {
+            const float4 x = *(const float4 *) &sc[r][n], y = *(const float4 *) &sb[16 * wave + r][n];
+            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, y.x, acc, 0, 0, 0);
+            acc2 = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, y.y, acc2, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, y.z, acc, 0, 0, 0);
+            acc2 = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, y.w, acc2, 0, 0, 0);
+        }
+        acc += acc2;
+    }
+    // rows 4 gq + i, column r: what is past the row's token is not seen
+    __shared__ uint32_t s_row[4][16];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (wave == part && r > 4 * gq + i) acc[i] = 0.0f;
+        const uint32_t m = ssm_group_max<16>(ssm_mag(acc[i]));
+        if (r == 0) s_row[wave][4 * gq + i] = m;
+    }
+    __syncthreads();
+    float * cb = q.cb + ((sg * q.chunks + chunk) * kSsmL + 16 * part) * kSsmL + 16 * wave;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int at = 4 * gq + i;
+        const int k = ssm_scale(max(max(s_row[0][at], s_row[1][at]), max(s_row[2][at], s_row[3][at])));
+        cb[at * kSsmL + r] = acc[i] * ssm_pow2(k);
+        if (wave == 0 && r == 0) q.cb_s[sg * tp + t0 + 16 * part + at] = ssm_pow2(-k);
     }
 }
 
@@ -247,59 +367,55 @@ constexpr int kSsmXRow = kSsmL + 8;  // halfs of a staged channel's tokens, padd
 
 template <int NP>
 struct ssm_lds {
-    _Float16 x[4][64][kSsmXRow];  // u for y (hi, lo), u exp(c_L - c_j) b_s for the state (hi, lo): [channel][token]
+    _Float16 x[4][64][kSsmXRow];  // u for y (hi, lo), u 2^(c_L - c_j) for the state (hi, lo): [channel][token]
     _Float16 st[2][64][NP + 8];   // the entering state (hi, lo): [channel][n]
-    float whole[kSsmL], frac[kSsmL];  // c_t in powers of two
-    uint32_t mag[4][4][64];       // a channel's largest u, u for the state, state, and its first u but 0, by wave
+    float whole[kSsmL], frac[kSsmL];  // c_t
+    uint32_t mag[3][4][64];       // a channel's largest x, state, and its first x but 0, by wave
     float red[4][64];
 };
 
-// token by token: the chunk's tokens t0 .. t0 + nt over the state rows of
-// every wave, for chunks with non-finite values
+// token by token: the chunk's nt tokens from t0 on, for chunks the matrix
+// form cannot take. The state is in LDS (in the place of its split halves,
+// [channel][n]); wave w takes its quarter of n, a lane its channel.
 template <int NP, bool OUT>
-__device__ __noinline__ void ssm_chunk_slow(const ssm_scan_args & a, ssm_lds<NP> & L, ssm_v4f (&st)[NP / 64][4], int s,
-                                            int h, int p0, int64_t t0, int nt, float dt, float z) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, gq = lane >> 4;
-    const int g = h / (a.heads / a.groups);
+__device__ __forceinline__ void ssm_chunk_slow(const ssm_scan_args & a, ssm_lds<NP> & L, int s, int h, int p0, int64_t t0,
+                                               int nt, float A) {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));  // (nothing of this path is kept over the caller's loop)
+    const int wave = threadIdx.x >> 6;
+    const int g = h / (a.heads / a.groups), p = p0 + lane;
+    float * st = (float *) &L.st[0][0][0] + lane * (NP + 8);
+    const int n1 = min((wave + 1) * (NP / 4), a.n);
+#pragma unroll 1
     for (int t = 0; t < nt; t++) {
-        const float d = __shfl(dt, t), ea = __builtin_amdgcn_exp2f(__shfl(z, t));
+        const float d = ssm_softplus(*(const float *) (a.dt + 4 * h + (t0 + t) * a.dt_nb1 + s * a.dt_nb2));
+        const float ea = __builtin_amdgcn_exp2f(d * A * kLog2e);
         const float * b = (const float *) (a.B + g * a.B_nb1 + (t0 + t) * a.B_nb2 + s * a.B_nb3);
         const float * c = (const float *) (a.C + g * a.C_nb1 + (t0 + t) * a.C_nb2 + s * a.C_nb3);
         const float * x = (const float *) (a.x + h * a.x_nb1 + (t0 + t) * a.x_nb2 + s * a.x_nb3);
-#pragma unroll
-        for (int pt = 0; pt < 4; pt++) {
-            const int p = p0 + 16 * pt + r;
-            const float u = p < a.dim ? x[p] * d : 0.0f;
-            float y = 0.0f;
-#pragma unroll
-            for (int k = 0; k < NP / 64; k++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int n = wave * (NP / 4) + 16 * k + 4 * gq + i;
-                    if (n < a.n) {
-                        st[k][pt][i] = fmaf(st[k][pt][i], ea, u * b[n]);
-                        y = fmaf(st[k][pt][i], c[n], y);
-                    }
-                }
-            if constexpr (OUT) {
-                y += __shfl_xor(y, 16);
-                y += __shfl_xor(y, 32);
-                if (gq == 0) L.red[wave][16 * pt + r] = y;
-            }
+        const float u = p < a.dim ? x[p] * d : 0.0f;
+        float y = 0.0f;
+#pragma unroll 1
+        for (int n = wave * (NP / 4); n < n1; n++) {
+            st[n] = fmaf(st[n], ea, u * b[n]);
+            y = fmaf(st[n], c[n], y);
         }
         if constexpr (OUT) {
+            L.red[wave][lane] = y;
             __syncthreads();
-            const int p = p0 + (int) threadIdx.x;
-            if (threadIdx.x < 64 && p < a.dim)
+            if (wave == 0 && p < a.dim)
                 a.y[((s * a.tokens + t0 + t) * a.heads + h) * a.dim + p] =
-                    (L.red[0][threadIdx.x] + L.red[1][threadIdx.x]) + (L.red[2][threadIdx.x] + L.red[3][threadIdx.x]);
+                    (L.red[0][lane] + L.red[1][lane]) + (L.red[2][lane] + L.red[3][lane]);
             __syncthreads();
         }
     }
 }
 
+// (what the launch before wrote and all lanes read alike: scalar loads)
+#define SSM_UNIFORM const __attribute__((address_space(4)))
+
 template <int NP, bool OUT>
-__global__ __launch_bounds__(256, 2) void k_ssm_chunks(ssm_chunk_args q) {
+__global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk_args q) {
     constexpr int NT = NP / 64;  // 16-row tiles of the state a wave owns
     __shared__ __align__(16) ssm_lds<NP> L;
     const ssm_scan_args & a = q.a;
@@ -308,17 +424,19 @@ __global__ __launch_bounds__(256, 2) void k_ssm_chunks(ssm_chunk_args q) {
     const int unit = blockIdx.x, seg = blockIdx.y;
     const int pb = unit % q.pblocks, h = unit / q.pblocks % a.heads, s = unit / (q.pblocks * a.heads);
     const int g = h / (a.heads / a.groups), p0 = 64 * pb;
-    const int64_t sg = (int64_t) s * a.groups + g, tp = q.chunks * kSsmL;
+    const int64_t sg = (int64_t) s * a.groups + g, sh = (int64_t) s * a.heads + h, tp = q.chunks * kSsmL;
     const float A = *(const float *) (a.A + h * a.A_nb1);
     const int nbase = wave * (NP / 4);
 
-    // the state: rows n = nbase + 16 k + 4 gq + i, channels p0 + 16 pt + r
+    // the state: rows n = nbase + 16 k + 4 gq + i, channels 16 pt + r; its
+    // value times 2^ks[pt] (channel lane: 2^kst)
     ssm_v4f st[NT][4];
+    int ks[4] = {0, 0, 0, 0}, kst = 0;
     {
         float carry = 1.0f;
         if constexpr (OUT) {
             double d = 0.0;
-            for (int m = 0; m < seg; m++) d += q.seg_decay[((int64_t) s * a.heads + h) * q.segs + m];
+            for (int m = 0; m < seg; m++) d += q.seg_decay[sh * q.segs + m];
             carry = __builtin_amdgcn_exp2f((float) d);
         }
         const int64_t slot = a.ids[s];
@@ -331,13 +449,12 @@ __global__ __launch_bounds__(256, 2) void k_ssm_chunks(ssm_chunk_args q) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int n = nbase + 16 * k + 4 * gq + i, p = p0 + 16 * pt + r;
-                    const bool ok = has && n < a.n && p < a.dim;
-                    st[k][pt][i] = ok ? s0[(int64_t) p * a.n + n] * carry : 0.0f;
+                    st[k][pt][i] = has && n < a.n && p < a.dim ? s0[(int64_t) p * a.n + n] * carry : 0.0f;
                 }
         if constexpr (OUT) {
             for (int m = 0; m < seg; m++) {
                 double d = 0.0;
-                for (int e = m + 1; e < seg; e++) d += q.seg_decay[((int64_t) s * a.heads + h) * q.segs + e];
+                for (int e = m + 1; e < seg; e++) d += q.seg_decay[sh * q.segs + e];
                 const float f = __builtin_amdgcn_exp2f((float) d);
                 const float * o = q.seg_state + ((int64_t) unit * q.segs + m) * 64 * NP;
 #pragma unroll
@@ -354,54 +471,56 @@ __global__ __launch_bounds__(256, 2) void k_ssm_chunks(ssm_chunk_args q) {
         }
     }
     const int64_t c0 = (int64_t) seg * q.seg_chunks, c1 = min(c0 + q.seg_chunks, q.chunks);
-    const int px = p0 + lane;  // the channel this lane stages
-    auto load_x = [&](int64_t c, float (&x)[16]) {
-        const char * xp = a.x + h * a.x_nb1 + s * a.x_nb3 + 4 * (int64_t) (px < a.dim ? px : 0);
+    const int64_t yrow = (int64_t) a.heads * a.dim;
+    const char * const xbase = a.x + h * a.x_nb1 + s * a.x_nb3;
+    // the next chunk's x and c_t, in flight under this one's products
+    float xn[16], wholen = 0.0f, fracn = 0.0f;
+    // (a lane's part of an address in 32 bits, the rest uniform)
+    auto load_next = [&](int64_t c, int lane) {
+        const int64_t at = sh * tp + c * kSsmL;
+        const uint32_t xo = 4u * (uint32_t) (p0 + lane < a.dim ? p0 + lane : 0), lo4 = 4u * (uint32_t) lane;
+        if (OUT && wave == 0) {
+            wholen = ssm_at<const float>(q.whole + at, lo4);
+            fracn = ssm_at<const float>(q.frac + at, lo4);
+        }
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const int64_t t = c * kSsmL + 16 * wave + i;
-            x[i] = *(const float *) (xp + (t < a.tokens ? t : 0) * a.x_nb2);
+            const int64_t t = c * kSsmL + 16 * wave + i;  // uniform, as the row's address
+            xn[i] = ssm_at<const float>(xbase + (t < a.tokens ? t : 0) * a.x_nb2, xo);
         }
     };
-    auto load_dt = [&](int64_t c) {
-        const int64_t t = c * kSsmL + lane;
-        return *(const float *) (a.dt + 4 * h + (t < a.tokens ? t : 0) * a.dt_nb1 + s * a.dt_nb2);
-    };
-    float xn[16], dtn = 0.0f;
-    if (c0 < c1) {
-        load_x(c0, xn);
-        dtn = load_dt(c0);
-    }
+    if (c0 < c1) load_next(c0, lane);
     double decayed = 0.0;
     for (int64_t c = c0; c < c1; c++) {
+        // The lane is unknown to the compiler anew in every iteration: the
+        // addresses that follow from it, kept over the loop, would spill, and
+        // a spill's reload waits for every load in flight.
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int r = lane & 15, gq = lane >> 4, px = p0 + lane;  // px: the channel this lane stages
+        const uint32_t co = 2u * (uint32_t) ((16 * wave + r) * NP + 8 * gq);
+        const uint32_t bo = 2u * (uint32_t) ((nbase + r) * kSsmL + 8 * gq);
+        const uint32_t cbo = 4u * (uint32_t) ((16 * wave + r) * kSsmL + 8 * gq), cso = 4u * (uint32_t) (16 * wave + 4 * gq);
+        const uint32_t yo = 4u * ((uint32_t) (16 * wave + 4 * gq) * (uint32_t) yrow + (uint32_t) r);
         const int64_t t0 = c * kSsmL;
         const int nt = (int) min((int64_t) kSsmL, a.tokens - t0);
-        // the decays: lane t's step, the inclusive sums in f64
-        const float dt = lane < nt ? ssm_softplus(dtn) : 0.0f;
-        const float z = dt * A * kLog2e;
-        double cum = (double) dt * (double) A * 1.4426950408889634074;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double v = __shfl_up(cum, o);
-            if (lane >= o) cum += v;
-        }
-        const double total = __shfl(cum, 63);
-        const double whole = floor(cum);
-        const float left = __builtin_amdgcn_exp2f((float) (total - cum));
-        const float wj = dt * left * q.b_s[sg * tp + t0 + lane];
-        float u[16], v[16];
-        uint32_t mu = 0, mv = 0, first = 0;
+        const bool inside = nt == kSsmL && p0 + 64 <= a.dim;
+        SSM_UNIFORM ssm_decay * dec = (SSM_UNIFORM ssm_decay *) (q.decay + sh * q.chunks + c);
+        SSM_UNIFORM ssm_flags * fl = (SSM_UNIFORM ssm_flags *) (q.flags + sg * q.chunks + c);
+        SSM_UNIFORM float * dts = (SSM_UNIFORM float *) (q.dt + sh * tp + t0 + 16 * wave);
+        SSM_UNIFORM float * lefts = (SSM_UNIFORM float *) (q.left + sh * tp + t0 + 16 * wave);
+        const double total = dec->total;
+        const int e_dt = dec->e_dt, e_left = dec->e_left, odd = dec->odd;
+        const int bad = fl->bad[0] | fl->bad[1] | fl->bad[2] | fl->bad[3], kb = fl->kb;
+        const float whole = wholen, frac = fracn;
+        float x[16];
+        uint32_t mx = 0, first = 0;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const int t = 16 * wave + i;
-            const float x = px < a.dim && t < nt ? xn[i] : 0.0f;
-            u[i] = x * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(dt), t));
-            v[i] = x * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wj), t));
-            mu = max(mu, ssm_mag(u[i]));
-            first = first ? first : mu;
-            mv = max(mv, ssm_mag(v[i]));
+            x[i] = inside || (px < a.dim && 16 * wave + i < nt) ? xn[i] : 0.0f;
+            mx = max(mx, ssm_mag(x[i]));
+            first = first ? first : mx;
         }
-        uint32_t ms = 0;  // of channel 16 gq + r = lane
 #pragma unroll
         for (int pt = 0; pt < 4; pt++) {
             uint32_t m = 0;
@@ -411,209 +530,238 @@ __global__ __launch_bounds__(256, 2) void k_ssm_chunks(ssm_chunk_args q) {
                 for (int i = 0; i < 4; i++) m = max(m, ssm_mag(st[k][pt][i]));
             m = max(m, (uint32_t) __shfl_xor((int) m, 16));
             m = max(m, (uint32_t) __shfl_xor((int) m, 32));
-            ms = gq == pt ? m : ms;
+            if (gq == 0) L.mag[1][wave][16 * pt + r] = m;
         }
-        // (past 2^23 the whole powers are no longer exact in f32)
-        const bool odd = !(fabs(total) < 8388608.0);
-        L.mag[0][wave][lane] = mu;
-        L.mag[1][wave][lane] = mv;
-        L.mag[2][wave][lane] = ms;
-        L.mag[3][wave][lane] = first;
-        if (c + 1 < c1) {
-            load_x(c + 1, xn);
-            dtn = load_dt(c + 1);
-        }
+        L.mag[0][wave][lane] = mx;
+        L.mag[2][wave][lane] = first;
         __syncthreads();  // the magnitudes; every wave is done with the chunk before
-        auto largest = [&](int kind) {
-            return max(max(L.mag[kind][0][lane], L.mag[kind][1][lane]), max(L.mag[kind][2][lane], L.mag[kind][3][lane]));
-        };
-        mu = largest(0), mv = largest(1), ms = largest(2);
-        first = L.mag[3][0][lane] ? L.mag[3][0][lane] : L.mag[3][1][lane] ? L.mag[3][1][lane] : L.mag[3][2][lane] ? L.mag[3][2][lane] : mu;
-        // one step of the exponent is 2^23 in a float's bits
-        const bool rising = mu > first && (mu >> 23) - (first >> 23) > 24;
-        decayed += total;
-        {
-            const int4 bad = *(const int4 *) (q.bad + (sg * q.chunks + c) * 4);
-            // the same for every wave: they see the same magnitudes
-            if (odd || __any(rising || !ssm_finite(mu) || !ssm_finite(mv) || !ssm_finite(ms)) || (bad.x | bad.y | bad.z | bad.w)) {
-                ssm_chunk_slow<NP, OUT>(a, L, st, s, h, p0, t0, nt, dt, z);
-                __syncthreads();
-                continue;
+        // The chunk's operands, requested where the arithmetic up to their use
+        // covers their latency, and ahead of the next chunk's x: loads return
+        // in order, and x comes from HBM.
+        ssm_v8h ch[OUT ? NP / 32 : 1], cl[OUT ? NP / 32 : 1];
+        float cbv[2][8], cs[4], cbs[4];
+        if constexpr (OUT) {
+            const _Float16 *hp = q.c_hi + (sg * tp + t0) * NP, *lp = q.c_lo + (sg * tp + t0) * NP;
+#pragma unroll
+            for (int kk = 0; kk < NP / 32; kk++) {
+                ch[kk] = ssm_at<const ssm_v8h>(hp, co, 64 * kk);
+                cl[kk] = ssm_at<const ssm_v8h>(lp, co, 64 * kk);
             }
+            const float * cb = q.cb + (sg * q.chunks + c) * kSsmL * kSsmL;
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++) {
+                *(float4 *) &cbv[kk][0] = ssm_at<const float4>(cb, cbo, 128 * kk);
+                *(float4 *) &cbv[kk][4] = ssm_at<const float4>(cb, cbo, 128 * kk + 16);
+            }
+            *(float4 *) cs = ssm_at<const float4>(q.c_s + (sg * tp + t0), cso);
+            *(float4 *) cbs = ssm_at<const float4>(q.cb_s + (sg * tp + t0), cso);
         }
-        // lane's channel's exponents, then those of the accumulators' columns
-        const int ku = ssm_scale(mu), ks = ssm_scale(ms);
-        // (terms under 2^-30 of the state need no bits of their own: keeps
-        // the state in their units far from f32's ends)
-        const int kv = ms ? min(ssm_scale(mv), ks + 30) : ssm_scale(mv);
-        int kup[4], ksp[4], kvp[4];
+        mx = max(max(L.mag[0][0][lane], L.mag[0][1][lane]), max(L.mag[0][2][lane], L.mag[0][3][lane]));
+        const uint32_t ms = max(max(L.mag[1][0][lane], L.mag[1][1][lane]), max(L.mag[1][2][lane], L.mag[1][3][lane]));
+        first = L.mag[2][0][lane] ? L.mag[2][0][lane] : L.mag[2][1][lane] ? L.mag[2][1][lane]
+                : L.mag[2][2][lane] ? L.mag[2][2][lane] : L.mag[2][3][lane];
+        // one step of the exponent is 2^23 in a float's bits
+        const bool rising = (mx >> 23) > (first >> 23) + 24;
+        decayed += total;
+        // the same for every wave: they see the same magnitudes
+        if (bad || odd || __any(rising || !ssm_finite(mx) || !ssm_finite(ms))) {
+            float * sl = (float *) &L.st[0][0][0];
+            static_assert(sizeof(L.st) == sizeof(float) * 64 * (NP + 8), "the state fits in place of its halves");
+#pragma unroll
+            for (int k = 0; k < NT; k++)
+#pragma unroll
+                for (int pt = 0; pt < 4; pt++)
+                    *(ssm_v4f *) (sl + (16 * pt + r) * (NP + 8) + nbase + 16 * k + 4 * gq) = st[k][pt] * ldexpf(1.0f, -ks[pt]);
+            __syncthreads();
+            ssm_chunk_slow<NP, OUT>(a, L, s, h, p0, t0, nt, A);
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < NT; k++)
+#pragma unroll
+                for (int pt = 0; pt < 4; pt++)
+                    st[k][pt] = *(const ssm_v4f *) (sl + (16 * pt + r) * (NP + 8) + nbase + 16 * k + 4 * gq);
+#pragma unroll
+            for (int pt = 0; pt < 4; pt++) ks[pt] = 0;
+            kst = 0;
+            __syncthreads();
+            if (c + 1 < c1) load_next(c + 1, lane);
+            continue;
+        }
+        // Channel lane's exponents: x 2^kx below 2^14, so u below 2^15 over the
+        // steps' exponent; the state, in its units, 2^km below 2^14. The
+        // state's next units are those its new terms are staged in, 2^kv (at
+        // most 2^30 finer than it needs: far from f32's ends).
+        const int kx = ssm_scale(mx), km = ssm_scale(ms);
+        int kv = min(kx - e_left + kb, 120);
+        if (ms) kv = min(kv, kst + km + 30);
+        int kxp[4], kmp[4], kvp[4];  // of the accumulators' channels
 #pragma unroll
         for (int pt = 0; pt < 4; pt++) {
-            kup[pt] = __shfl(ku, 16 * pt + r);
-            ksp[pt] = __shfl(ks, 16 * pt + r);
+            kxp[pt] = __shfl(kx, 16 * pt + r);
+            kmp[pt] = __shfl(km, 16 * pt + r);
             kvp[pt] = __shfl(kv, 16 * pt + r);
         }
+        kst = kv;
         {
-            const float fu = ssm_pow2(ku), fv = ssm_pow2(kv);
+            const float fx = ssm_pow2(kx), fv = ldexpf(1.0f, kv + e_left - kb);
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-                ssm_v8h uh, ul, vh, vl;
+                float u[8], v[8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float x = u[8 * half + e] * fu, y = v[8 * half + e] * fv;
-                    uh[e] = (_Float16) x;
-                    ul[e] = (_Float16) (x - (float) uh[e]);
-                    vh[e] = (_Float16) y;
-                    vl[e] = (_Float16) (y - (float) vh[e]);
+                    u[e] = x[8 * half + e] * fx * dts[8 * half + e];
+                    v[e] = x[8 * half + e] * fv * lefts[8 * half + e];
                 }
+                ssm_v8h hi, lo;
                 const int at = 16 * wave + 8 * half;
                 if constexpr (OUT) {
-                    *(ssm_v8h *) &L.x[0][lane][at] = uh;
-                    *(ssm_v8h *) &L.x[1][lane][at] = ul;
+                    ssm_halves(u, hi, lo);
+                    *(ssm_v8h *) &L.x[0][lane][at] = hi;
+                    *(ssm_v8h *) &L.x[1][lane][at] = lo;
                 }
-                *(ssm_v8h *) &L.x[2][lane][at] = vh;
-                *(ssm_v8h *) &L.x[3][lane][at] = vl;
-            }
-            if constexpr (OUT) {
-#pragma unroll
-                for (int k = 0; k < NT; k++)
-#pragma unroll
-                    for (int pt = 0; pt < 4; pt++) {
-                        const float fs = ssm_pow2(ksp[pt]);
-                        ssm_v4h hi, lo;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float x = st[k][pt][i] * fs;
-                            hi[i] = (_Float16) x;
-                            lo[i] = (_Float16) (x - (float) hi[i]);
-                        }
-                        const int n = nbase + 16 * k + 4 * gq;
-                        *(ssm_v4h *) &L.st[0][16 * pt + r][n] = hi;
-                        *(ssm_v4h *) &L.st[1][16 * pt + r][n] = lo;
-                    }
-                if (wave == 0) {
-                    L.whole[lane] = (float) whole;
-                    L.frac[lane] = (float) (cum - whole);
-                }
+                ssm_halves(v, hi, lo);
+                *(ssm_v8h *) &L.x[2][lane][at] = hi;
+                *(ssm_v8h *) &L.x[3][lane][at] = lo;
             }
         }
+        if constexpr (OUT) {
+#pragma unroll
+            for (int k = 0; k < NT; k++)
+#pragma unroll
+                for (int pt = 0; pt < 4; pt++) {
+                    const float fs = ssm_pow2(kmp[pt]);
+                    float v[4];
+                    ssm_v4h hi, lo;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[i] = st[k][pt][i] * fs;
+                    ssm_halves(v, hi, lo);
+                    const int n = nbase + 16 * k + 4 * gq;
+                    *(ssm_v4h *) &L.st[0][16 * pt + r][n] = hi;
+                    *(ssm_v4h *) &L.st[1][16 * pt + r][n] = lo;
+                }
+            if (wave == 0) {
+                L.whole[lane] = whole;
+                L.frac[lane] = frac;
+            }
+        }
+        ssm_v8h bh[2][NT], bl[2][NT];
+        auto load_b = [&] {
+            const _Float16 * hp = q.b_hi + (sg * q.chunks + c) * NP * kSsmL;
+            const _Float16 * lp = q.b_lo + (sg * q.chunks + c) * NP * kSsmL;
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+                for (int k = 0; k < NT; k++) {
+                    bh[kk][k] = ssm_at<const ssm_v8h>(hp, bo, 32 * k * kSsmL + 64 * kk);
+                    bl[kk][k] = ssm_at<const ssm_v8h>(lp, bo, 32 * k * kSsmL + 64 * kk);
+                }
+            if (c + 1 < c1) load_next(c + 1, lane);
+        };
+        if constexpr (!OUT) load_b();
         __syncthreads();
         if constexpr (OUT) {
-            const int t = 16 * wave + r;  // the token of this lane's operand rows
             ssm_v4f yh[4], yx[4];
 #pragma unroll
             for (int pt = 0; pt < 4; pt++) yh[pt] = yx[pt] = ssm_v4f{0, 0, 0, 0};
             // H C_t
-            const _Float16 * ch = q.c_hi + (sg * tp + t0 + t) * NP + 8 * gq;
-            const _Float16 * cl = q.c_lo + (sg * tp + t0 + t) * NP + 8 * gq;
 #pragma unroll
             for (int kk = 0; kk < NP / 32; kk++) {
-                const ssm_v8h ah = *(const ssm_v8h *) (ch + 32 * kk), al = *(const ssm_v8h *) (cl + 32 * kk);
 #pragma unroll
                 for (int pt = 0; pt < 4; pt++) {
-                    const ssm_v8h bh = *(const ssm_v8h *) &L.st[0][16 * pt + r][32 * kk + 8 * gq];
-                    const ssm_v8h bl = *(const ssm_v8h *) &L.st[1][16 * pt + r][32 * kk + 8 * gq];
-                    yh[pt] = ssm_mfma(ah, bh, yh[pt]);
-                    yh[pt] = ssm_mfma(ah, bl, yh[pt]);
-                    yh[pt] = ssm_mfma(al, bh, yh[pt]);
+                    const ssm_v8h sh8 = *(const ssm_v8h *) &L.st[0][16 * pt + r][32 * kk + 8 * gq];
+                    const ssm_v8h sl8 = *(const ssm_v8h *) &L.st[1][16 * pt + r][32 * kk + 8 * gq];
+                    yh[pt] = ssm_mfma(ch[kk], sh8, yh[pt]);
+                    yh[pt] = ssm_mfma(ch[kk], sl8, yh[pt]);
+                    yh[pt] = ssm_mfma(cl[kk], sh8, yh[pt]);
                 }
+                // (one K step's operands at a time: more in flight spill)
+                __builtin_amdgcn_sched_barrier(0);
             }
-            // the chunk's own tokens: the decayed C . B of this lane's row
-            const float tw = L.whole[t], tf = L.frac[t];
-            const float * cb = q.cb + ((sg * q.chunks + c) * kSsmL + t) * kSsmL + 8 * gq;
-            float m[2][8];
-            uint32_t mm = 0;
+            load_b();  // (in the registers that held C)
+            __builtin_amdgcn_sched_barrier(0);
+            // the chunk's own tokens: the decayed C . B of this lane's row (the
+            // 16-blocks past the wave's tokens are zeros; a decay is at most one)
+            const float tw = L.whole[16 * wave + r], tf = L.frac[16 * wave + r];
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
                 if (kk == 1 && wave < 2) continue;
-                float gv[8], jw[8], jf[8];
-                *(float4 *) &gv[0] = *(const float4 *) (cb + 32 * kk);
-                *(float4 *) &gv[4] = *(const float4 *) (cb + 32 * kk + 4);
+                float jw[8], jf[8], m[8];
                 *(float4 *) &jw[0] = *(const float4 *) &L.whole[32 * kk + 8 * gq];
                 *(float4 *) &jw[4] = *(const float4 *) &L.whole[32 * kk + 8 * gq + 4];
                 *(float4 *) &jf[0] = *(const float4 *) &L.frac[32 * kk + 8 * gq];
                 *(float4 *) &jf[4] = *(const float4 *) &L.frac[32 * kk + 8 * gq + 4];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float dec = __builtin_amdgcn_exp2f((tw - jw[e]) + (tf - jf[e]));
-                    m[kk][e] = 32 * kk + 8 * gq + e <= t ? gv[e] * dec : 0.0f;
-                    mm = max(mm, ssm_mag(m[kk][e]));
-                }
-            }
-            mm = max(mm, (uint32_t) __shfl_xor((int) mm, 16));
-            mm = max(mm, (uint32_t) __shfl_xor((int) mm, 32));
-            const int km = ssm_scale(mm);  // of the lane's row
-            const float fm = ssm_pow2(km);
-#pragma unroll
-            for (int kk = 0; kk < 2; kk++) {
-                if (kk == 1 && wave < 2) continue;
+                for (int e = 0; e < 8; e++)
+                    m[e] = cbv[kk][e] * __builtin_amdgcn_exp2f(fminf((tw - jw[e]) + (tf - jf[e]), 0.0f));
                 ssm_v8h ah, al;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float x = m[kk][e] * fm;
-                    ah[e] = (_Float16) x;
-                    al[e] = (_Float16) (x - (float) ah[e]);
-                }
+                ssm_halves(m, ah, al);
 #pragma unroll
                 for (int pt = 0; pt < 4; pt++) {
-                    const ssm_v8h bh = *(const ssm_v8h *) &L.x[0][16 * pt + r][32 * kk + 8 * gq];
-                    const ssm_v8h bl = *(const ssm_v8h *) &L.x[1][16 * pt + r][32 * kk + 8 * gq];
-                    yx[pt] = ssm_mfma(ah, bh, yx[pt]);
-                    yx[pt] = ssm_mfma(ah, bl, yx[pt]);
-                    yx[pt] = ssm_mfma(al, bh, yx[pt]);
+                    const ssm_v8h xh = *(const ssm_v8h *) &L.x[0][16 * pt + r][32 * kk + 8 * gq];
+                    const ssm_v8h xl = *(const ssm_v8h *) &L.x[1][16 * pt + r][32 * kk + 8 * gq];
+                    yx[pt] = ssm_mfma(ah, xh, yx[pt]);
+                    yx[pt] = ssm_mfma(ah, xl, yx[pt]);
+                    yx[pt] = ssm_mfma(al, xh, yx[pt]);
                 }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            float fh[4], fxr[4], fk[4], fu[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {  // rows: the tokens 16 wave + 4 gq + i
+                const int tr = 16 * wave + 4 * gq + i;
+                fh[i] = __builtin_amdgcn_exp2f(L.whole[tr] + L.frac[tr]) * cs[i];
+                fxr[i] = cbs[i] * ssm_pow2(e_dt);
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int tr = 16 * wave + 4 * gq + i;  // the token of the accumulators' row i
-                const float fx = ssm_pow2(-__shfl(km, 4 * gq + i));
-                const float fh = __builtin_amdgcn_exp2f(L.whole[tr] + L.frac[tr]) * q.c_s[sg * tp + t0 + tr];
-                if (tr >= nt) continue;
-                float * y = a.y + ((s * a.tokens + t0 + tr) * a.heads + h) * a.dim + p0;
-#pragma unroll
-                for (int pt = 0; pt < 4; pt++)
-                    if (p0 + 16 * pt + r < a.dim)
-                        y[16 * pt + r] = fmaf(yh[pt][i], fh * ssm_pow2(-ksp[pt]), yx[pt][i] * (fx * ssm_pow2(-kup[pt])));
+            for (int pt = 0; pt < 4; pt++) {
+                fk[pt] = ldexpf(1.0f, -ks[pt] - kmp[pt]);
+                fu[pt] = ssm_pow2(-kxp[pt]);
             }
+            float * yp = a.y + (((s * a.tokens + t0) * a.heads + h) * a.dim + p0);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int pt = 0; pt < 4; pt++) {
+                    const float y = fmaf(yh[pt][i], fk[pt] * fh[i], yx[pt][i] * (fu[pt] * fxr[i]));
+                    if (inside || (16 * wave + 4 * gq + i < nt && p0 + 16 * pt + r < a.dim))
+                        ssm_at<float>(yp + i * yrow, yo, 64 * pt) = y;
+                }
         }
-        // the state after the chunk, in the staged operand's units meanwhile
+        // the state after the chunk
         {
             const float fd = __builtin_amdgcn_exp2f((float) total);
-            const _Float16 * bh = q.b_hi + ((sg * q.chunks + c) * NP + nbase + r) * kSsmL + 8 * gq;
-            const _Float16 * bl = q.b_lo + ((sg * q.chunks + c) * NP + nbase + r) * kSsmL + 8 * gq;
 #pragma unroll
-            for (int k = 0; k < NT; k++)
+            for (int pt = 0; pt < 4; pt++) {
+                const float f = fd * ssm_pow2(max(min(kvp[pt] - ks[pt], 126), -126));
 #pragma unroll
-                for (int pt = 0; pt < 4; pt++) st[k][pt] *= fd * ssm_pow2(kvp[pt]);
+                for (int k = 0; k < NT; k++) st[k][pt] *= f;
+                ks[pt] = kvp[pt];
+            }
+        }
 #pragma unroll
-            for (int kk = 0; kk < 2; kk++) {
-                ssm_v8h xh[4], xl[4];
+        for (int kk = 0; kk < 2; kk++) {
+            ssm_v8h xh[4], xl[4];
 #pragma unroll
-                for (int pt = 0; pt < 4; pt++) {
-                    xh[pt] = *(const ssm_v8h *) &L.x[2][16 * pt + r][32 * kk + 8 * gq];
-                    xl[pt] = *(const ssm_v8h *) &L.x[3][16 * pt + r][32 * kk + 8 * gq];
-                }
-#pragma unroll
-                for (int k = 0; k < NT; k++) {
-                    const ssm_v8h ah = *(const ssm_v8h *) (bh + 16 * k * kSsmL + 32 * kk);
-                    const ssm_v8h al = *(const ssm_v8h *) (bl + 16 * k * kSsmL + 32 * kk);
-#pragma unroll
-                    for (int pt = 0; pt < 4; pt++) {
-                        st[k][pt] = ssm_mfma(ah, xh[pt], st[k][pt]);
-                        st[k][pt] = ssm_mfma(ah, xl[pt], st[k][pt]);
-                        st[k][pt] = ssm_mfma(al, xh[pt], st[k][pt]);
-                    }
-                }
+            for (int pt = 0; pt < 4; pt++) {
+                xh[pt] = *(const ssm_v8h *) &L.x[2][16 * pt + r][32 * kk + 8 * gq];
+                xl[pt] = *(const ssm_v8h *) &L.x[3][16 * pt + r][32 * kk + 8 * gq];
             }
 #pragma unroll
             for (int k = 0; k < NT; k++)
 #pragma unroll
-                for (int pt = 0; pt < 4; pt++) st[k][pt] *= ssm_pow2(-kvp[pt]);
+                for (int pt = 0; pt < 4; pt++) {
+                    st[k][pt] = ssm_mfma(bh[kk][k], xh[pt], st[k][pt]);
+                    st[k][pt] = ssm_mfma(bh[kk][k], xl[pt], st[k][pt]);
+                    st[k][pt] = ssm_mfma(bl[kk][k], xh[pt], st[k][pt]);
+                }
         }
     }
+    float back[4];
+#pragma unroll
+    for (int pt = 0; pt < 4; pt++) back[pt] = ldexpf(1.0f, -ks[pt]);
     if constexpr (OUT) {
         if (seg != q.segs - 1) return;
-        float * o = a.out + ((int64_t) s * a.heads + h) * a.dim * a.n;
+        float * o = a.out + sh * a.dim * a.n;
 #pragma unroll
         for (int k = 0; k < NT; k++)
 #pragma unroll
@@ -621,17 +769,18 @@ __global__ __launch_bounds__(256, 2) void k_ssm_chunks(ssm_chunk_args q) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int n = nbase + 16 * k + 4 * gq + i, p = p0 + 16 * pt + r;
-                    if (n < a.n && p < a.dim) o[(int64_t) p * a.n + n] = st[k][pt][i];
+                    if (n < a.n && p < a.dim) o[(int64_t) p * a.n + n] = st[k][pt][i] * back[pt];
                 }
     } else {
-        if (pb == 0 && threadIdx.x == 0) q.seg_decay[((int64_t) s * a.heads + h) * q.segs + seg] = decayed;
+        if (pb == 0 && threadIdx.x == 0) q.seg_decay[sh * q.segs + seg] = decayed;
         float * o = q.seg_state + ((int64_t) unit * q.segs + seg) * 64 * NP;
 #pragma unroll
         for (int k = 0; k < NT; k++)
 #pragma unroll
             for (int pt = 0; pt < 4; pt++)
                 *(float4 *) (o + (16 * pt + r) * NP + nbase + 16 * k + 4 * gq) =
-                    make_float4(st[k][pt][0], st[k][pt][1], st[k][pt][2], st[k][pt][3]);
+                    make_float4(st[k][pt][0] * back[pt], st[k][pt][1] * back[pt], st[k][pt][2] * back[pt],
+                                st[k][pt][3] * back[pt]);
     }
 }
 
@@ -643,23 +792,33 @@ static size_t ssm_al(size_t v) { return (v + 255) / 256 * 256; }
 
 // the chunked form takes a decay a head over enough tokens, channels and
 // state elements to fill its tiles
-static bool ssm_chunked(const ssm_scan_args & a) { return !a.a_elem && a.tokens >= 16 && a.dim >= 16 && a.n >= 16; }
+static bool ssm_chunked(const ssm_scan_args & a) {
+    return !a.a_elem && a.tokens >= 16 && a.dim >= 16 && a.n >= 16 &&
+           (int64_t) a.heads * a.dim < 1 << 22;  // (a chunk's rows of y in 32-bit offsets)
+}
 
 static int ssm_np(const ssm_scan_args & a) { return a.n <= 64 ? 64 : a.n <= 128 ? 128 : 256; }
 
-// segments of a chunked scan: workgroups for every CU where the heads alone
-// are too few, each of four chunks at least
+// Segments of a chunked scan. Two workgroups a CU run at a time, so n segments
+// take the rounds of their workgroups times a segment's chunks and what it
+// reads of the segments before it; the first pass, which forms no outputs,
+// about half of that for all segments but the last, and a launch. In quarters
+// of a chunk's time.
 static void ssm_segments(const ssm_scan_args & a, int n_cu, ssm_chunk_args & q) {
     q.a = a;
     q.chunks = (a.tokens + kSsmL - 1) / kSsmL;
     q.pblocks = (a.dim + 63) / 64;
     const int64_t units = (int64_t) a.seqs * a.heads * q.pblocks;
-    int64_t segs = (2 * n_cu + units - 1) / units;
-    segs = segs < 1 ? 1 : segs;
-    const int64_t most = (q.chunks + 3) / 4;
-    segs = segs < most ? segs : most;
-    q.seg_chunks = (int) ((q.chunks + segs - 1) / segs);
-    q.segs = (int) ((q.chunks + q.seg_chunks - 1) / q.seg_chunks);
+    auto rounds = [&](int64_t wgs) { return (wgs + 2 * n_cu - 1) / (2 * n_cu); };
+    int64_t best = 0, best_cost = INT64_MAX;
+    for (int64_t n = 1; n <= 32 && n <= q.chunks; n++) {
+        const int64_t each = (q.chunks + n - 1) / n, segs = (q.chunks + each - 1) / each;
+        const int64_t cost = rounds(units * segs) * (4 * each + segs / 2 + 2) +
+                             (segs > 1 ? rounds(units * (segs - 1)) * (2 * each + 2) + 8 : 0);
+        if (cost < best_cost) best = each, best_cost = cost;
+    }
+    q.seg_chunks = (int) best;
+    q.segs = (int) ((q.chunks + best - 1) / best);
 }
 
 // the scratch's parts, in order; base null: their total size only
@@ -676,9 +835,15 @@ static size_t ssm_carve(ssm_chunk_args & q, char * base) {
     take(q.b_hi, sg * tp * np * 2);
     take(q.b_lo, sg * tp * np * 2);
     take(q.c_s, sg * tp * 4);
-    take(q.b_s, sg * tp * 4);
+    take(q.cb_s, sg * tp * 4);
     take(q.cb, sg * tp * kSsmL * 4);
-    take(q.bad, sg * (size_t) q.chunks * 16);
+    take(q.flags, sg * (size_t) q.chunks * sizeof(ssm_flags));
+    const size_t sh = (size_t) a.seqs * a.heads;
+    take(q.dt, sh * tp * 4);
+    take(q.left, sh * tp * 4);
+    take(q.whole, sh * tp * 4);
+    take(q.frac, sh * tp * 4);
+    take(q.decay, sh * (size_t) q.chunks * sizeof(ssm_decay));
     const size_t segs = q.segs > 1 ? (size_t) q.segs : 0;
     take(q.seg_state, (size_t) a.seqs * a.heads * q.pblocks * segs * 64 * np * 4);
     take(q.seg_decay, (size_t) a.seqs * a.heads * segs * 8);
@@ -699,7 +864,9 @@ static void launch_ssm_chunks(const ssm_scan_args & a, void * scratch, hipStream
     auto go = [&](auto np) {
         constexpr int NP = decltype(np)::value;
         const unsigned units = (unsigned) (a.seqs * a.heads * q.pblocks);
-        hipLaunchKernelGGL(k_ssm_split<NP>, dim3((unsigned) (4 * q.chunks * a.seqs * a.groups)), dim3(256), 0, s, q);
+        q.split_blocks = (uint32_t) (4 * q.chunks * a.seqs * a.groups);
+        const uint32_t decay_blocks = (uint32_t) ((q.chunks * a.seqs * a.heads + 3) / 4);
+        hipLaunchKernelGGL(k_ssm_split<NP>, dim3(q.split_blocks + decay_blocks), dim3(256), 0, s, q);
         if (q.segs > 1)
             hipLaunchKernelGGL((k_ssm_chunks<NP, false>), dim3(units, (unsigned) (q.segs - 1)), dim3(256), 0, s, q);
         hipLaunchKernelGGL((k_ssm_chunks<NP, true>), dim3(units, (unsigned) q.segs), dim3(256), 0, s, q);
