@@ -122,6 +122,17 @@ constexpr float kLog2e = 1.44269504088896340736f;
 __device__ __forceinline__ ssm_v4f ssm_mfma(ssm_v8h a, ssm_v8h b, ssm_v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
+// a b of split halves for four b's: the three products of one accumulator
+// apart, since each waits for the one before
+__device__ __forceinline__ void ssm_products(ssm_v8h ah, ssm_v8h al, const ssm_v8h (&bh)[4], const ssm_v8h (&bl)[4],
+                                             ssm_v4f (&c)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) c[i] = ssm_mfma(ah, bh[i], c[i]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) c[i] = ssm_mfma(ah, bl[i], c[i]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) c[i] = ssm_mfma(al, bh[i], c[i]);
+}
 // 2^e, e a whole number in f32's normal range
 __device__ __forceinline__ float ssm_pow2(int e) { return __uint_as_float((uint32_t) (e + 127) << 23); }
 // the exponent k that brings a largest magnitude (its bits) into [2^13, 2^14);
@@ -145,14 +156,14 @@ __device__ __forceinline__ uint32_t ssm_group_max(uint32_t v) {
 }
 __device__ __forceinline__ bool ssm_finite(uint32_t mag) { return mag < 0x7F800000u; }
 
-// f16 hi + lo of N scaled f32 values
-template <int N, typename V>
-__device__ __forceinline__ void ssm_halves(const float (&x)[N], V & hi, V & lo) {
+// f16 hi + lo of N products x f (the lo part by a fused multiply-add)
+template <int N, typename V, typename F>
+__device__ __forceinline__ void ssm_halves(const float (&x)[N], F f, V & hi, V & lo) {
 #pragma unroll
     for (int e = 0; e < N; e += 2) {
-        const ssm_v2f v = {x[e], x[e + 1]};
+        const ssm_v2f v = {x[e] * f(e), x[e + 1] * f(e + 1)};
         const ssm_v2h h = __builtin_convertvector(v, ssm_v2h);
-        const ssm_v2f d = {fmaf(x[e], 1.0f, -(float) h.x), fmaf(x[e + 1], 1.0f, -(float) h.y)};
+        const ssm_v2f d = {fmaf(x[e], f(e), -(float) h.x), fmaf(x[e + 1], f(e + 1), -(float) h.y)};
         const ssm_v2h l = __builtin_convertvector(d, ssm_v2h);
         hi[e] = h.x, hi[e + 1] = h.y;
         lo[e] = l.x, lo[e + 1] = l.y;
@@ -171,21 +182,33 @@ struct ssm_flags {
     int pad[3];
 };
 
-// the operands' places in scratch, for NP = the padded state size
+// The operands in scratch: a record a (sequence, group, chunk) and one a
+// (sequence, head, chunk), byte offsets of their parts, NP the padded state size
+template <int NP>
+struct ssm_shared_at {
+    static constexpr int c_hi = 0;              // [64 tokens][NP] f16, each token's row scaled
+    static constexpr int c_lo = 128 * NP;
+    static constexpr int b_hi = 256 * NP;       // [NP][64 tokens] f16, scaled
+    static constexpr int b_lo = 384 * NP;
+    static constexpr int cb = 512 * NP;         // [64][64] f32: C_t . B_j for j <= t (zeros past it), rows scaled
+    static constexpr int c_s = cb + 16384;      // [64] f32: a row of C is its operand times this
+    static constexpr int cb_s = c_s + 256;      // [64] f32: a row of C . B is its operand times this
+    static constexpr int flags = cb_s + 256;    // ssm_flags
+    static constexpr int size = flags + 256;
+};
+struct ssm_head_at {  // c_t: the sum of the log2 decays from the chunk's start to token t
+    static constexpr int dt = 0;        // [64] f32: the step over 2^e_dt
+    static constexpr int left = 256;    // [64] f32: the step times 2^(c_L - c_t), over 2^e_left
+    static constexpr int whole = 512;   // [64] f32: c_t's whole and fractional part
+    static constexpr int frac = 768;
+    static constexpr int decay = 1024;  // ssm_decay
+    static constexpr int size = 1280;
+};
 struct ssm_chunk_args {
     ssm_scan_args a;
-    _Float16 *c_hi, *c_lo;  // [seq, group][token][NP], each token's row scaled
-    _Float16 *b_hi, *b_lo;  // [seq, group][chunk][NP][64 tokens], each chunk scaled
-    float * c_s;            // [seq, group][token]: a row of C is its operand times this
-    float * cb;             // [seq, group][chunk][64][64]: C_t . B_j for j <= t (zeros in the 16-blocks past t's), rows scaled
-    float * cb_s;           // [seq, group][token]: a row of it is its operand times this
-    ssm_flags * flags;      // [seq, group][chunk]
-    // the heads' decays, c_t the sum of the log2 decays from the chunk's start
-    float *dt, *left;       // [seq, head][token]: the step and the step times 2^(c_L - c_t), over 2^(exponents)
-    float *whole, *frac;    // [seq, head][token]: c_t's whole and fractional part
-    ssm_decay * decay;      // [seq, head][chunk]
-    float * seg_state;      // [seq, head, channel block][segment][64][NP]
-    double * seg_decay;     // [seq, head][segment]: its log2 decay
+    char *shared, *heads;
+    float * seg_state;   // [seq, head, channel block][segment][64][NP]
+    double * seg_decay;  // [seq, head][segment]: its log2 decay
     int64_t chunks;
     int segs, seg_chunks, pblocks;
     uint32_t split_blocks;
@@ -198,7 +221,8 @@ __device__ __forceinline__ void ssm_decays(const ssm_chunk_args & q, int64_t uni
     const int64_t c = unit % q.chunks, sh = unit / q.chunks;
     if (sh >= (int64_t) a.seqs * a.heads) return;
     const int h = (int) (sh % a.heads), s = (int) (sh / a.heads);
-    const int64_t t = c * kSsmL + lane, at = sh * q.chunks * kSsmL + t;
+    const int64_t t = c * kSsmL + lane;
+    char * rec = q.heads + unit * ssm_head_at::size;
     const float A = *(const float *) (a.A + h * a.A_nb1);
     const float dt = t < a.tokens ? ssm_softplus(*(const float *) (a.dt + 4 * h + t * a.dt_nb1 + s * a.dt_nb2)) : 0.0f;
     double cum = (double) dt * (double) A * 1.4426950408889634074;
@@ -217,11 +241,11 @@ __device__ __forceinline__ void ssm_decays(const ssm_chunk_args & q, int64_t uni
     d.e_left = max((int) (ml >> 23) - 127, -60);
     // A positive, or decays whose whole parts leave f32's exact range
     d.odd = !(total <= 0.0 && total > -8388608.0) || !ssm_finite(md);
-    q.dt[at] = dt * ssm_pow2(-d.e_dt);
-    q.left[at] = left * ssm_pow2(-d.e_left);
-    q.whole[at] = (float) whole;
-    q.frac[at] = (float) (cum - whole);
-    if (lane == 0) q.decay[sh * q.chunks + c] = d;
+    ((float *) (rec + ssm_head_at::dt))[lane] = dt * ssm_pow2(-d.e_dt);
+    ((float *) (rec + ssm_head_at::left))[lane] = left * ssm_pow2(-d.e_left);
+    ((float *) (rec + ssm_head_at::whole))[lane] = (float) whole;
+    ((float *) (rec + ssm_head_at::frac))[lane] = (float) (cum - whole);
+    if (lane == 0) *(ssm_decay *) (rec + ssm_head_at::decay) = d;
 }
 
 // the first blocks the shared operands, a quarter of a chunk's rows each; the
@@ -290,7 +314,8 @@ __global__ __launch_bounds__(256) void k_ssm_split(ssm_chunk_args q) {
     if (lane == 0) s_mb[wave] = mb;
     __syncthreads();
     mb = max(max(s_mb[0], s_mb[1]), max(s_mb[2], s_mb[3]));
-    const int64_t tp = q.chunks * kSsmL;
+    using at = ssm_shared_at<NP>;
+    char * rec = q.shared + (sg * q.chunks + chunk) * at::size;
     // C's rows: 16 threads each
     const int row = tid / 16, sub = tid % 16;
     uint32_t mc = 0;
@@ -299,32 +324,33 @@ __global__ __launch_bounds__(256) void k_ssm_split(ssm_chunk_args q) {
     const int kb = ssm_finite(mb) ? ssm_scale(mb) : 0, kc = ssm_finite(mc) ? ssm_scale(mc) : 0;
     const int any = __syncthreads_or(!ssm_finite(mb) || !ssm_finite(mc));
     if (tid == 0) {
-        q.flags[sg * q.chunks + chunk].bad[part] = any;
-        if (part == 0) q.flags[sg * q.chunks + chunk].kb = kb;
+        ssm_flags * fl = (ssm_flags *) (rec + at::flags);
+        fl->bad[part] = any;
+        if (part == 0) fl->kb = kb;
     }
-    const int64_t t = t0 + 16 * part + row;
-    if (sub == 0) q.c_s[sg * tp + t] = ssm_pow2(-kc);
+    const int t = 16 * part + row;
+    if (sub == 0) ((float *) (rec + at::c_s))[t] = ssm_pow2(-kc);
     const float fc = ssm_pow2(kc), fb = ssm_pow2(kb);
     for (int n = 8 * sub; n < NP; n += 128) {
         float v[8];
         ssm_v8h hi, lo;
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = sc[row][n + e] * fc;
-        ssm_halves(v, hi, lo);
-        *(ssm_v8h *) (q.c_hi + (sg * tp + t) * NP + n) = hi;
-        *(ssm_v8h *) (q.c_lo + (sg * tp + t) * NP + n) = lo;
+        for (int e = 0; e < 8; e++) v[e] = sc[row][n + e];
+        ssm_halves(v, [&](int) { return fc; }, hi, lo);
+        *(ssm_v8h *) (rec + at::c_hi + 2 * (t * NP + n)) = hi;
+        *(ssm_v8h *) (rec + at::c_lo + 2 * (t * NP + n)) = lo;
     }
     // B's columns: 16 tokens of one a thread
     if (tid < NP) {
-        _Float16 * oh = q.b_hi + ((sg * q.chunks + chunk) * NP + tid) * kSsmL + 16 * part;
-        _Float16 * ol = q.b_lo + ((sg * q.chunks + chunk) * NP + tid) * kSsmL + 16 * part;
+        _Float16 * oh = (_Float16 *) (rec + at::b_hi) + tid * kSsmL + 16 * part;
+        _Float16 * ol = (_Float16 *) (rec + at::b_lo) + tid * kSsmL + 16 * part;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             float v[8];
             ssm_v8h hi, lo;
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = sb[16 * part + 8 * h + e][tid] * fb;
-            ssm_halves(v, hi, lo);
+            for (int e = 0; e < 8; e++) v[e] = sb[16 * part + 8 * h + e][tid];
+            ssm_halves(v, [&](int) { return fb; }, hi, lo);
             *(ssm_v8h *) (oh + 8 * h) = hi;
             *(ssm_v8h *) (ol + 8 * h) = lo;
         }
@@ -353,13 +379,13 @@ __global__ __launch_bounds__(256) void k_ssm_split(ssm_chunk_args q) {
         if (r == 0) s_row[wave][4 * gq + i] = m;
     }
     __syncthreads();
-    float * cb = q.cb + ((sg * q.chunks + chunk) * kSsmL + 16 * part) * kSsmL + 16 * wave;
+    float * cb = (float *) (rec + at::cb) + 16 * part * kSsmL + 16 * wave;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int at = 4 * gq + i;
-        const int k = ssm_scale(max(max(s_row[0][at], s_row[1][at]), max(s_row[2][at], s_row[3][at])));
-        cb[at * kSsmL + r] = acc[i] * ssm_pow2(k);
-        if (wave == 0 && r == 0) q.cb_s[sg * tp + t0 + 16 * part + at] = ssm_pow2(-k);
+        const int m = 4 * gq + i;
+        const int k = ssm_scale(max(max(s_row[0][m], s_row[1][m]), max(s_row[2][m], s_row[3][m])));
+        cb[m * kSsmL + r] = acc[i] * ssm_pow2(k);
+        if (wave == 0 && r == 0) ((float *) (rec + at::cb_s))[16 * part + m] = ssm_pow2(-k);
     }
 }
 
@@ -372,6 +398,7 @@ struct ssm_lds {
     float whole[kSsmL], frac[kSsmL];  // c_t
     uint32_t mag[3][4][64];       // a channel's largest x, state, and its first x but 0, by wave
     float red[4][64];
+    float steps[4][32];           // a wave's tokens' dt, then left (read by their wave only)
 };
 
 // token by token: the chunk's nt tokens from t0 on, for chunks the matrix
@@ -424,7 +451,7 @@ __global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk
     const int unit = blockIdx.x, seg = blockIdx.y;
     const int pb = unit % q.pblocks, h = unit / q.pblocks % a.heads, s = unit / (q.pblocks * a.heads);
     const int g = h / (a.heads / a.groups), p0 = 64 * pb;
-    const int64_t sg = (int64_t) s * a.groups + g, sh = (int64_t) s * a.heads + h, tp = q.chunks * kSsmL;
+    const int64_t sg = (int64_t) s * a.groups + g, sh = (int64_t) s * a.heads + h;
     const float A = *(const float *) (a.A + h * a.A_nb1);
     const int nbase = wave * (NP / 4);
 
@@ -473,25 +500,33 @@ __global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk
     const int64_t c0 = (int64_t) seg * q.seg_chunks, c1 = min(c0 + q.seg_chunks, q.chunks);
     const int64_t yrow = (int64_t) a.heads * a.dim;
     const char * const xbase = a.x + h * a.x_nb1 + s * a.x_nb3;
+    using at = ssm_shared_at<NP>;
+    const char * gp = q.shared + (sg * q.chunks + c0) * at::size;              // the chunk's records
+    const char * hp = q.heads + (sh * q.chunks + c0) * ssm_head_at::size;
     // the next chunk's x and c_t, in flight under this one's products
-    float xn[16], wholen = 0.0f, fracn = 0.0f;
+    float xn[16], stepn = 0.0f, wholen = 0.0f, fracn = 0.0f;
     // (a lane's part of an address in 32 bits, the rest uniform)
-    auto load_next = [&](int64_t c, int lane) {
-        const int64_t at = sh * tp + c * kSsmL;
+    auto load_next = [&](int64_t c, const char * hp, int lane) {
         const uint32_t xo = 4u * (uint32_t) (p0 + lane < a.dim ? p0 + lane : 0), lo4 = 4u * (uint32_t) lane;
+        // lanes 0 .. 15 the wave's dt, 16 .. 31 its left
+        stepn = ssm_at<const float>(hp + 64 * wave, 4u * (uint32_t) ((lane & 15) + 4 * (lane & 16)));
         if (OUT && wave == 0) {
-            wholen = ssm_at<const float>(q.whole + at, lo4);
-            fracn = ssm_at<const float>(q.frac + at, lo4);
+            wholen = ssm_at<const float>(hp, lo4, ssm_head_at::whole);
+            fracn = ssm_at<const float>(hp, lo4, ssm_head_at::frac);
         }
+        // rows from the wave's first token on, the last token's again past it
+        const int64_t t = min(c * kSsmL + 16 * wave, a.tokens - 1);
+        const char * row = xbase + t * a.x_nb2;
+        const int left = (int) min((int64_t) 16, a.tokens - 1 - t);
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const int64_t t = c * kSsmL + 16 * wave + i;  // uniform, as the row's address
-            xn[i] = ssm_at<const float>(xbase + (t < a.tokens ? t : 0) * a.x_nb2, xo);
+            xn[i] = ssm_at<const float>(row, xo);
+            row += i < left ? a.x_nb2 : 0;
         }
     };
-    if (c0 < c1) load_next(c0, lane);
+    if (c0 < c1) load_next(c0, hp, lane);
     double decayed = 0.0;
-    for (int64_t c = c0; c < c1; c++) {
+    for (int64_t c = c0; c < c1; c++, gp += at::size, hp += ssm_head_at::size) {
         // The lane is unknown to the compiler anew in every iteration: the
         // addresses that follow from it, kept over the loop, would spill, and
         // a spill's reload waits for every load in flight.
@@ -505,10 +540,10 @@ __global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk
         const int64_t t0 = c * kSsmL;
         const int nt = (int) min((int64_t) kSsmL, a.tokens - t0);
         const bool inside = nt == kSsmL && p0 + 64 <= a.dim;
-        SSM_UNIFORM ssm_decay * dec = (SSM_UNIFORM ssm_decay *) (q.decay + sh * q.chunks + c);
-        SSM_UNIFORM ssm_flags * fl = (SSM_UNIFORM ssm_flags *) (q.flags + sg * q.chunks + c);
-        SSM_UNIFORM float * dts = (SSM_UNIFORM float *) (q.dt + sh * tp + t0 + 16 * wave);
-        SSM_UNIFORM float * lefts = (SSM_UNIFORM float *) (q.left + sh * tp + t0 + 16 * wave);
+        SSM_UNIFORM ssm_decay * dec = (SSM_UNIFORM ssm_decay *) (hp + ssm_head_at::decay);
+        SSM_UNIFORM ssm_flags * fl = (SSM_UNIFORM ssm_flags *) (gp + at::flags);
+        static_assert(ssm_head_at::left == 256 && ssm_head_at::dt == 0, "the lanes' offsets of dt and left");
+        if (lane < 32) L.steps[wave][lane] = stepn;
         const double total = dec->total;
         const int e_dt = dec->e_dt, e_left = dec->e_left, odd = dec->odd;
         const int bad = fl->bad[0] | fl->bad[1] | fl->bad[2] | fl->bad[3], kb = fl->kb;
@@ -516,8 +551,14 @@ __global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk
         float x[16];
         uint32_t mx = 0, first = 0;
 #pragma unroll
+        for (int i = 0; i < 16; i++) x[i] = xn[i];
+        if (!inside) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i] = px < a.dim && 16 * wave + i < nt ? x[i] : 0.0f;
+        }
+        if (!OUT && c + 1 < c1) load_next(c + 1, hp + ssm_head_at::size, lane);
+#pragma unroll
         for (int i = 0; i < 16; i++) {
-            x[i] = inside || (px < a.dim && 16 * wave + i < nt) ? xn[i] : 0.0f;
             mx = max(mx, ssm_mag(x[i]));
             first = first ? first : mx;
         }
@@ -541,20 +582,18 @@ __global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk
         ssm_v8h ch[OUT ? NP / 32 : 1], cl[OUT ? NP / 32 : 1];
         float cbv[2][8], cs[4], cbs[4];
         if constexpr (OUT) {
-            const _Float16 *hp = q.c_hi + (sg * tp + t0) * NP, *lp = q.c_lo + (sg * tp + t0) * NP;
 #pragma unroll
             for (int kk = 0; kk < NP / 32; kk++) {
-                ch[kk] = ssm_at<const ssm_v8h>(hp, co, 64 * kk);
-                cl[kk] = ssm_at<const ssm_v8h>(lp, co, 64 * kk);
+                ch[kk] = ssm_at<const ssm_v8h>(gp + at::c_hi, co, 64 * kk);
+                cl[kk] = ssm_at<const ssm_v8h>(gp + at::c_lo, co, 64 * kk);
             }
-            const float * cb = q.cb + (sg * q.chunks + c) * kSsmL * kSsmL;
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
-                *(float4 *) &cbv[kk][0] = ssm_at<const float4>(cb, cbo, 128 * kk);
-                *(float4 *) &cbv[kk][4] = ssm_at<const float4>(cb, cbo, 128 * kk + 16);
+                *(float4 *) &cbv[kk][0] = ssm_at<const float4>(gp + at::cb, cbo, 128 * kk);
+                *(float4 *) &cbv[kk][4] = ssm_at<const float4>(gp + at::cb, cbo, 128 * kk + 16);
             }
-            *(float4 *) cs = ssm_at<const float4>(q.c_s + (sg * tp + t0), cso);
-            *(float4 *) cbs = ssm_at<const float4>(q.cb_s + (sg * tp + t0), cso);
+            *(float4 *) cs = ssm_at<const float4>(gp + at::c_s, cso);
+            *(float4 *) cbs = ssm_at<const float4>(gp + at::cb_s, cso);
         }
         mx = max(max(L.mag[0][0][lane], L.mag[0][1][lane]), max(L.mag[0][2][lane], L.mag[0][3][lane]));
         const uint32_t ms = max(max(L.mag[1][0][lane], L.mag[1][1][lane]), max(L.mag[1][2][lane], L.mag[1][3][lane]));
@@ -584,7 +623,7 @@ __global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk
             for (int pt = 0; pt < 4; pt++) ks[pt] = 0;
             kst = 0;
             __syncthreads();
-            if (c + 1 < c1) load_next(c + 1, lane);
+            if (OUT && c + 1 < c1) load_next(c + 1, hp + ssm_head_at::size, lane);
             continue;
         }
         // Channel lane's exponents: x 2^kx below 2^14, so u below 2^15 over the
@@ -604,26 +643,27 @@ __global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk
         kst = kv;
         {
             const float fx = ssm_pow2(kx), fv = ldexpf(1.0f, kv + e_left - kb);
+            const float *dts = L.steps[wave], *lefts = L.steps[wave] + 16;
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-                float u[8], v[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    u[e] = x[8 * half + e] * fx * dts[8 * half + e];
-                    v[e] = x[8 * half + e] * fv * lefts[8 * half + e];
-                }
+                float xs[8];
                 ssm_v8h hi, lo;
-                const int at = 16 * wave + 8 * half;
+                const int to = 16 * wave + 8 * half;
                 if constexpr (OUT) {
-                    ssm_halves(u, hi, lo);
-                    *(ssm_v8h *) &L.x[0][lane][at] = hi;
-                    *(ssm_v8h *) &L.x[1][lane][at] = lo;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) xs[e] = x[8 * half + e] * fx;
+                    ssm_halves(xs, [&](int e) { return dts[8 * half + e]; }, hi, lo);
+                    *(ssm_v8h *) &L.x[0][lane][to] = hi;
+                    *(ssm_v8h *) &L.x[1][lane][to] = lo;
                 }
-                ssm_halves(v, hi, lo);
-                *(ssm_v8h *) &L.x[2][lane][at] = hi;
-                *(ssm_v8h *) &L.x[3][lane][at] = lo;
+#pragma unroll
+                for (int e = 0; e < 8; e++) xs[e] = x[8 * half + e] * fv;
+                ssm_halves(xs, [&](int e) { return lefts[8 * half + e]; }, hi, lo);
+                *(ssm_v8h *) &L.x[2][lane][to] = hi;
+                *(ssm_v8h *) &L.x[3][lane][to] = lo;
             }
         }
+        if (OUT && c + 1 < c1) load_next(c + 1, hp + ssm_head_at::size, lane);
         if constexpr (OUT) {
 #pragma unroll
             for (int k = 0; k < NT; k++)
@@ -633,8 +673,8 @@ __global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk
                     float v[4];
                     ssm_v4h hi, lo;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) v[i] = st[k][pt][i] * fs;
-                    ssm_halves(v, hi, lo);
+                    for (int i = 0; i < 4; i++) v[i] = st[k][pt][i];
+                    ssm_halves(v, [&](int) { return fs; }, hi, lo);
                     const int n = nbase + 16 * k + 4 * gq;
                     *(ssm_v4h *) &L.st[0][16 * pt + r][n] = hi;
                     *(ssm_v4h *) &L.st[1][16 * pt + r][n] = lo;
@@ -646,16 +686,13 @@ __global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk
         }
         ssm_v8h bh[2][NT], bl[2][NT];
         auto load_b = [&] {
-            const _Float16 * hp = q.b_hi + (sg * q.chunks + c) * NP * kSsmL;
-            const _Float16 * lp = q.b_lo + (sg * q.chunks + c) * NP * kSsmL;
 #pragma unroll
             for (int kk = 0; kk < 2; kk++)
 #pragma unroll
                 for (int k = 0; k < NT; k++) {
-                    bh[kk][k] = ssm_at<const ssm_v8h>(hp, bo, 32 * k * kSsmL + 64 * kk);
-                    bl[kk][k] = ssm_at<const ssm_v8h>(lp, bo, 32 * k * kSsmL + 64 * kk);
+                    bh[kk][k] = ssm_at<const ssm_v8h>(gp + at::b_hi, bo, 32 * k * kSsmL + 64 * kk);
+                    bl[kk][k] = ssm_at<const ssm_v8h>(gp + at::b_lo, bo, 32 * k * kSsmL + 64 * kk);
                 }
-            if (c + 1 < c1) load_next(c + 1, lane);
         };
         if constexpr (!OUT) load_b();
         __syncthreads();
@@ -663,17 +700,16 @@ __global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk
             ssm_v4f yh[4], yx[4];
 #pragma unroll
             for (int pt = 0; pt < 4; pt++) yh[pt] = yx[pt] = ssm_v4f{0, 0, 0, 0};
+            ssm_v8h oh[4], ol[4];
             // H C_t
 #pragma unroll
             for (int kk = 0; kk < NP / 32; kk++) {
 #pragma unroll
                 for (int pt = 0; pt < 4; pt++) {
-                    const ssm_v8h sh8 = *(const ssm_v8h *) &L.st[0][16 * pt + r][32 * kk + 8 * gq];
-                    const ssm_v8h sl8 = *(const ssm_v8h *) &L.st[1][16 * pt + r][32 * kk + 8 * gq];
-                    yh[pt] = ssm_mfma(ch[kk], sh8, yh[pt]);
-                    yh[pt] = ssm_mfma(ch[kk], sl8, yh[pt]);
-                    yh[pt] = ssm_mfma(cl[kk], sh8, yh[pt]);
+                    oh[pt] = *(const ssm_v8h *) &L.st[0][16 * pt + r][32 * kk + 8 * gq];
+                    ol[pt] = *(const ssm_v8h *) &L.st[1][16 * pt + r][32 * kk + 8 * gq];
                 }
+                ssm_products(ch[kk], cl[kk], oh, ol, yh);
                 // (one K step's operands at a time: more in flight spill)
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -692,17 +728,15 @@ __global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk
                 *(float4 *) &jf[4] = *(const float4 *) &L.frac[32 * kk + 8 * gq + 4];
 #pragma unroll
                 for (int e = 0; e < 8; e++)
-                    m[e] = cbv[kk][e] * __builtin_amdgcn_exp2f(fminf((tw - jw[e]) + (tf - jf[e]), 0.0f));
+                    m[e] = __builtin_amdgcn_exp2f(fminf((tw - jw[e]) + (tf - jf[e]), 0.0f));
                 ssm_v8h ah, al;
-                ssm_halves(m, ah, al);
+                ssm_halves(m, [&](int e) { return cbv[kk][e]; }, ah, al);
 #pragma unroll
                 for (int pt = 0; pt < 4; pt++) {
-                    const ssm_v8h xh = *(const ssm_v8h *) &L.x[0][16 * pt + r][32 * kk + 8 * gq];
-                    const ssm_v8h xl = *(const ssm_v8h *) &L.x[1][16 * pt + r][32 * kk + 8 * gq];
-                    yx[pt] = ssm_mfma(ah, xh, yx[pt]);
-                    yx[pt] = ssm_mfma(ah, xl, yx[pt]);
-                    yx[pt] = ssm_mfma(al, xh, yx[pt]);
+                    oh[pt] = *(const ssm_v8h *) &L.x[0][16 * pt + r][32 * kk + 8 * gq];
+                    ol[pt] = *(const ssm_v8h *) &L.x[1][16 * pt + r][32 * kk + 8 * gq];
                 }
+                ssm_products(ah, al, oh, ol, yx);
                 __builtin_amdgcn_sched_barrier(0);
             }
             float fh[4], fxr[4], fk[4], fu[4];
@@ -721,11 +755,21 @@ __global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int pt = 0; pt < 4; pt++) {
-                    const float y = fmaf(yh[pt][i], fk[pt] * fh[i], yx[pt][i] * (fu[pt] * fxr[i]));
-                    if (inside || (16 * wave + 4 * gq + i < nt && p0 + 16 * pt + r < a.dim))
-                        ssm_at<float>(yp + i * yrow, yo, 64 * pt) = y;
-                }
+                for (int pt = 0; pt < 4; pt++)
+                    yh[pt][i] = fmaf(yh[pt][i], fk[pt] * fh[i], yx[pt][i] * (fu[pt] * fxr[i]));
+            if (inside) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int pt = 0; pt < 4; pt++) ssm_at<float>(yp + i * yrow, yo, 64 * pt) = yh[pt][i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int pt = 0; pt < 4; pt++)
+                        if (16 * wave + 4 * gq + i < nt && p0 + 16 * pt + r < a.dim)
+                            ssm_at<float>(yp + i * yrow, yo, 64 * pt) = yh[pt][i];
+            }
         }
         // the state after the chunk
         {
@@ -747,13 +791,7 @@ __global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk
                 xl[pt] = *(const ssm_v8h *) &L.x[3][16 * pt + r][32 * kk + 8 * gq];
             }
 #pragma unroll
-            for (int k = 0; k < NT; k++)
-#pragma unroll
-                for (int pt = 0; pt < 4; pt++) {
-                    st[k][pt] = ssm_mfma(bh[kk][k], xh[pt], st[k][pt]);
-                    st[k][pt] = ssm_mfma(bh[kk][k], xl[pt], st[k][pt]);
-                    st[k][pt] = ssm_mfma(bl[kk][k], xh[pt], st[k][pt]);
-                }
+            for (int k = 0; k < NT; k++) ssm_products(bh[kk][k], bl[kk][k], xh, xl, st[k]);
         }
     }
     float back[4];
@@ -824,26 +862,15 @@ static void ssm_segments(const ssm_scan_args & a, int n_cu, ssm_chunk_args & q) 
 // the scratch's parts, in order; base null: their total size only
 static size_t ssm_carve(ssm_chunk_args & q, char * base) {
     const ssm_scan_args & a = q.a;
-    const size_t np = (size_t) ssm_np(a), sg = (size_t) a.seqs * a.groups, tp = (size_t) q.chunks * kSsmL;
+    const size_t np = (size_t) ssm_np(a);
     size_t at = 0;
     auto take = [&](auto *& p, size_t bytes) {
         p = (typename std::remove_reference<decltype(p)>::type) (base + at);
         at += ssm_al(bytes);
     };
-    take(q.c_hi, sg * tp * np * 2);
-    take(q.c_lo, sg * tp * np * 2);
-    take(q.b_hi, sg * tp * np * 2);
-    take(q.b_lo, sg * tp * np * 2);
-    take(q.c_s, sg * tp * 4);
-    take(q.cb_s, sg * tp * 4);
-    take(q.cb, sg * tp * kSsmL * 4);
-    take(q.flags, sg * (size_t) q.chunks * sizeof(ssm_flags));
-    const size_t sh = (size_t) a.seqs * a.heads;
-    take(q.dt, sh * tp * 4);
-    take(q.left, sh * tp * 4);
-    take(q.whole, sh * tp * 4);
-    take(q.frac, sh * tp * 4);
-    take(q.decay, sh * (size_t) q.chunks * sizeof(ssm_decay));
+    const size_t rec = (size_t) (np == 64 ? ssm_shared_at<64>::size : np == 128 ? ssm_shared_at<128>::size : ssm_shared_at<256>::size);
+    take(q.shared, (size_t) a.seqs * a.groups * q.chunks * rec);
+    take(q.heads, (size_t) a.seqs * a.heads * q.chunks * ssm_head_at::size);
     const size_t segs = q.segs > 1 ? (size_t) q.segs : 0;
     take(q.seg_state, (size_t) a.seqs * a.heads * q.pblocks * segs * 64 * np * 4);
     take(q.seg_decay, (size_t) a.seqs * a.heads * segs * 8);
