@@ -1,8 +1,12 @@
 // k_moe.hip -- the mixture-of-experts operators: GGML_OP_MUL_MAT_ID (each
 // column by the matrix of its own expert) and the router's GGML_OP_ARGSORT
 // and GGML_OP_SUM_ROWS.
+#include <type_traits>
+
+#include "../mfma_units.h"
 #include "../mi355x_common.h"
 #include "../ops.h"
+#include "../quant_dev.h"
 
 namespace mi355x {
 
@@ -59,8 +63,688 @@ __global__ __launch_bounds__(256) void k_mul_mat_id_rows(mul_mat_id_args a) {
     }
 }
 
-void launch_mul_mat_id(int wtype, const mul_mat_id_args & a, hipStream_t s) {
+// ------------------------------------------------- few columns: streaming ---
+//
+// A workgroup takes 16 rows of one expert (PAIR: of both its matrices, whose
+// SwiGLU it stores) and the columns routed to it, 16 at a time; its waves
+// split K, their sums added through LDS in order. Bound by the weights'
+// stream: each wave reads its own, straight into the matrix cores' operand
+// layout (activations A, weights B: lane l ends with weight row l % 16 of the
+// columns 4 (l / 16) + i). The routing is done in place: workgroup y serves
+// the expert of pair y if no earlier pair has it.
+constexpr int kMoeFew = 256;  // pairs a workgroup's threads hold
+
+typedef _Float16 moe_v8h __attribute__((ext_vector_type(8)));
+typedef float moe_v4f __attribute__((ext_vector_type(4)));
+
+// eight f32 values at p as f16 (rounded to nearest even)
+__device__ __forceinline__ moe_v8h moe_round8(const float * p) {
+    const float4 a = *(const float4 *) p, b = *(const float4 *) (p + 4);
+    return moe_v8h{(_Float16) a.x, (_Float16) a.y, (_Float16) a.z, (_Float16) a.w,
+                   (_Float16) b.x, (_Float16) b.y, (_Float16) b.z, (_Float16) b.w};
+}
+
+// The 16 x 16 sums of one matrix's rows and 16 columns over wave w's share of
+// K, acc[i]: row r, column 4 g + i. bcol: the lane's own column (r) in b's
+// order, bc4: the columns 4 g + i.
+template <int WT>
+struct moe_tile;
+
+template <>
+struct moe_tile<GGML_TYPE_F16> {
+    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * wrow, int64_t bcol, const int (&)[4],
+                                               int wave, int waves, int g, double (&out)[4]) {
+        const float * x = (const float *) (a.b + (bcol % a.b_ne1) * a.b_nb1 + (bcol / a.b_ne1) * a.b_nb2);
+        const int64_t steps = (a.K + 31) / 32;
+        moe_v4f acc = {0, 0, 0, 0};
+        constexpr int U = 4;  // steps in flight
+        for (int64_t s0 = wave; s0 < steps; s0 += (int64_t) U * waves) {
+            uint4 w[U];
+            moe_v8h xv[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int64_t k = (s0 + (int64_t) u * waves) * 32 + 8 * g;
+                const bool ok = k < a.K;  // K % 8 == 0: eight at a time
+                w[u] = *(const uint4 *) (wrow + 2 * (ok ? k : 0));
+                xv[u] = moe_round8(x + (ok ? k : 0));
+                if (!ok) {
+                    w[u] = make_uint4(0, 0, 0, 0);
+                    xv[u] = moe_v8h{0, 0, 0, 0, 0, 0, 0, 0};
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(xv[u], __builtin_bit_cast(moe_v8h, w[u]), acc, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[i] = acc[i];
+    }
+};
+
+template <>
+struct moe_tile<GGML_TYPE_Q8_0> {
+    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * wrow, int64_t bcol, const int (&bc4)[4],
+                                               int wave, int waves, int g, double (&out)[4]) {
+        const int64_t nblk = a.K / 32;
+        const uint16_t * ds = (const uint16_t *) (wrow + a.K);
+        const int8_t * aq = a.act.q + bcol * a.K;
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[i] = 0.0;
+        constexpr int U = 4;
+        for (int64_t b0 = wave; b0 < nblk; b0 += (int64_t) U * waves) {
+            long q[U], af[U];
+            uint16_t d[U];
+            float da[U][4];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int64_t b = min(b0 + (int64_t) u * waves, nblk - 1);
+                q[u] = *(const long *) (wrow + 32 * b + 8 * g);
+                af[u] = *(const long *) (aq + 32 * b + 8 * g);
+                d[u] = ds[b];
+#pragma unroll
+                for (int i = 0; i < 4; i++) da[u][i] = a.act.d[bc4[i] * nblk + b];
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (b0 + (int64_t) u * waves < nblk) q8_0_block(af[u], q[u], d[u], da[u], out);
+        }
+    }
+};
+
+template <>
+struct moe_tile<GGML_TYPE_Q4_K> {
+    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * wrow, int64_t bcol, const int (&bc4)[4],
+                                               int wave, int waves, int g, double (&out)[4]) {
+        const int64_t nsb = a.K / 256;
+        const int8_t * aq = a.act.q + bcol * a.K;
+        const int16_t * ass = a.act.ssum + bcol * (a.K / 32);
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[i] = 0.0;
+        for (int64_t b = wave; b < nsb; b += waves) {
+            const char * blk = wrow + b * 144;
+            const uint4 hdr = *(const uint4 *) blk;
+            long q[4], af[8];
+#pragma unroll
+            for (int c = 0; c < 4; c++) q[c] = *(const long *) (blk + 16 + 32 * c + 8 * g);
+#pragma unroll
+            for (int j = 0; j < 8; j++) af[j] = *(const long *) (aq + 256 * b + 32 * j + 8 * g);
+            float ad[4], ssa[2];
+#pragma unroll
+            for (int i = 0; i < 4; i++) ad[i] = a.act.d[bc4[i] * nsb + b];
+            q4k_ssum_operand(ass + 8 * b, true, g, ssa);
+            q4k_unit(hdr, q, af, ad, ssa, out);
+        }
+    }
+};
+
+__device__ __forceinline__ float moe_swiglu(float g, float u) { return (g / (1.0f + expf_det(-g))) * u; }
+
+template <int WT, bool PAIR>
+__global__ __launch_bounds__(256) void k_moe_few(mul_mat_id_args a) {
+    __shared__ int s_id[kMoeFew];
+    __shared__ int s_list[kMoeFew];
+    __shared__ int s_n[4];
+    __shared__ double s_acc[2][3][4][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
+    const int me = blockIdx.y;
+    const int64_t m0 = (int64_t) blockIdx.x * 16;
+    int id = -1;
+    if (tid < a.pairs) id = *(const int32_t *) (a.ids + (tid % a.used) * a.ids_nb0 + (tid / a.used) * a.ids_nb1);
+    s_id[tid] = id;
+    __syncthreads();
+    const int e = s_id[me];
+    if (e < 0 || e >= a.experts) {  // no expert: the pair's column is zero
+        if (tid < 16 && m0 + tid < a.M) a.out[(int64_t) me * a.M + m0 + tid] = 0.0f;
+        return;
+    }
+    const bool mine = tid < a.pairs && id == e;
+    const uint64_t have = __ballot(mine);
+    if (lane == 0) s_n[wave] = __popcll(have);
+    if (__syncthreads_or(mine && tid < me)) return;  // an earlier pair's workgroup serves this expert
+    int at = 0, n = 0;
+    for (int w = 0; w < 4; w++) {
+        at += w < wave ? s_n[w] : 0;
+        n += s_n[w];
+    }
+    if (mine) s_list[at + __popcll(have & ((1ull << lane) - 1))] = tid;
+    __syncthreads();
+    const int64_t row = min(m0 + r, a.M - 1);
+    const char * w1 = a.W + e * a.W_nb2 + row * a.W_nb1;
+    const char * w2 = PAIR ? a.W2 + e * a.W_nb2 + row * a.W_nb1 : nullptr;
+    auto column = [&](int p) { return (int) (p / a.used * a.b_ne1 + p % a.used % a.b_ne1); };
+    for (int c0 = 0; c0 < n; c0 += 16) {
+        const int64_t bcol = column(s_list[min(c0 + r, n - 1)]);
+        int bc4[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) bc4[i] = column(s_list[min(c0 + 4 * g + i, n - 1)]);
+        double acc[2][4];
+        moe_tile<WT>::run(a, w1, bcol, bc4, wave, 4, g, acc[0]);
+        if constexpr (PAIR) moe_tile<WT>::run(a, w2, bcol, bc4, wave, 4, g, acc[1]);
+        if (wave > 0) {
+#pragma unroll
+            for (int m = 0; m < (PAIR ? 2 : 1); m++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) s_acc[m][wave - 1][i][lane] = acc[m][i];
+        }
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+#pragma unroll
+                for (int m = 0; m < (PAIR ? 2 : 1); m++)
+#pragma unroll
+                    for (int w = 0; w < 3; w++) acc[m][i] += s_acc[m][w][i][lane];
+                const int c = c0 + 4 * g + i;
+                if (c < n && m0 + r < a.M)
+                    a.out[(int64_t) s_list[c] * a.M + m0 + r] =
+                        PAIR ? moe_swiglu((float) acc[0][i], (float) acc[1][i]) : (float) acc[0][i];
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------ many columns: tile GEMM ---
+//
+// k_moe_route sorts the pairs by expert (a counting sort of one workgroup,
+// each expert's pairs in their order) and cuts every expert's run into tiles
+// of BN columns. k_moe_act makes the columns' f16 operands: the rounded
+// values of F16 weights, the whole numbers of the quantized blocks otherwise
+// (with their scales beside them). k_moe_gemm takes 128 weight rows (PAIR: 64
+// of each matrix) by BN columns of one expert, K in steps of 64 through two
+// LDS buffers (16-byte pieces swizzled by row), the next step's loads in
+// flight under the current one's products.
+//
+// Quantized weights are staged as the whole numbers of their blocks too:
+// a block's sum of 32 products is exact on the f16 matrix cores, and a block
+// then costs a multiply and a fused multiply-add an output for its scales
+// (Q4_K's minimum: another). The sums are f32: within the roundings of K / 32
+// terms of the exact block sums.
+constexpr int kMoeK = 64;
+constexpr int kMoeRows = 128;
+
+struct moe_wide_args {
+    mul_mat_id_args a;
+    int * head;     // [0]: the number of tiles
+    int4 * tiles;   // expert (-1: none), first place, columns
+    int * sorted;   // place -> pair
+    _Float16 * x;   // [b column][Kp]
+    float * xd;     // quantized: the blocks' scales, [b column][Kp / 32 or Kp / 256]
+    float * xs;     // Q4_K: scale times sum of 32 elements, [b column][Kp / 32]
+    int64_t kp, bcols, row_tiles;
+    int bn, max_tiles;
+};
+
+__global__ __launch_bounds__(1024) void k_moe_route(moe_wide_args q) {
+    extern __shared__ int s_hist[];  // [16][bins], bins = experts + 1 (no expert)
+    const mul_mat_id_args & a = q.a;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int bins = (int) a.experts + 1, pairs = (int) a.pairs;
+    for (int i = tid; i < 16 * bins; i += 1024) s_hist[i] = 0;
+    __syncthreads();
+    // wave w's share: consecutive groups of 64 pairs
+    const int groups = (pairs + 63) / 64, per = (groups + 15) / 16;
+    auto expert_of = [&](int p) {
+        const int e = *(const int32_t *) (a.ids + (p % (int) a.used) * a.ids_nb0 + (int64_t) (p / (int) a.used) * a.ids_nb1);
+        return e < 0 || e >= a.experts ? (int) a.experts : e;
+    };
+    for (int k = 0; k < per; k++) {
+        const int p = ((wave * per + k) * 64) + lane;
+        if (p < pairs) atomicAdd(&s_hist[wave * bins + expert_of(p)], 1);
+    }
+    __syncthreads();
+    // the bins' totals, their exclusive sums (places and tiles) over bins in order
+    __shared__ int s_sum[2][16];
+    int base = 0, tbase = 0;
+    for (int b0 = 0; b0 < bins; b0 += 1024) {
+        const int b = b0 + tid;
+        int total = 0;
+        if (b < bins)
+            for (int w = 0; w < 16; w++) total += s_hist[w * bins + b];
+        const int nt = (total + q.bn - 1) / q.bn;
+        int sum = total, tsum = nt;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(sum, o), tv = __shfl_up(tsum, o);
+            if (lane >= o) sum += v, tsum += tv;
+        }
+        if (lane == 63) s_sum[0][wave] = sum, s_sum[1][wave] = tsum;
+        __syncthreads();
+        int before = base, tbefore = tbase;
+        for (int w = 0; w < 16; w++) {
+            before += w < wave ? s_sum[0][w] : 0;
+            tbefore += w < wave ? s_sum[1][w] : 0;
+            base += s_sum[0][w];
+            tbase += s_sum[1][w];
+        }
+        if (b < bins) {
+            int at = before + sum - total;
+            const int t0 = tbefore + tsum - nt;
+            for (int t = 0; t < nt; t++)
+                q.tiles[t0 + t] = make_int4(b < a.experts ? b : -1, at + t * q.bn, min(q.bn, total - t * q.bn), 0);
+            for (int w = 0; w < 16; w++) {  // the waves' first places
+                const int c = s_hist[w * bins + b];
+                s_hist[w * bins + b] = at;
+                at += c;
+            }
+        }
+        __syncthreads();
+    }
+    if (tid == 0) q.head[0] = tbase;
+    // places: within a group of 64, pairs of one expert in lane order
+    for (int k = 0; k < per; k++) {
+        const int p = ((wave * per + k) * 64) + lane;
+        const bool ok = p < pairs;
+        const int e = ok ? expert_of(p) : -1;
+        uint64_t same = __ballot(ok);
+        for (int bit = 1; bit < 2 * bins; bit <<= 1) {
+            const uint64_t set = __ballot(ok && (e & bit));
+            same &= (e & bit) ? set : ~set;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        if (ok) q.sorted[s_hist[wave * bins + e] + rank] = p;
+        __builtin_amdgcn_wave_barrier();
+        if (ok && rank == 0) s_hist[wave * bins + e] += __popcll(same);
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// one wave 256 elements of a column
+template <int WT>
+__global__ __launch_bounds__(256) void k_moe_act(moe_wide_args q) {
+    const mul_mat_id_args & a = q.a;
+    const int lane = threadIdx.x & 63;
+    const int64_t chunks = (q.kp + 255) / 256, w = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t col = w / chunks, k = w % chunks * 256 + 4 * lane;
+    if (col >= q.bcols) return;
+    const float * x = (const float *) (a.b + (col % a.b_ne1) * a.b_nb1 + (col / a.b_ne1) * a.b_nb2);
+    float4 v = make_float4(0, 0, 0, 0);
+    if (k < a.K) v = *(const float4 *) (x + k);  // K % 4 == 0
+    typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+    v4h o = {(_Float16) v.x, (_Float16) v.y, (_Float16) v.z, (_Float16) v.w};
+    if constexpr (WT == GGML_TYPE_Q8_0) {
+        const q8_0_lane l = quantize_q8_0_group(v);
+        o = v4h{(_Float16) (float) l.q.x, (_Float16) (float) l.q.y, (_Float16) (float) l.q.z, (_Float16) (float) l.q.w};
+        if ((lane & 7) == 0 && k < q.kp) q.xd[col * (q.kp / 32) + k / 32] = l.d;
+    } else if constexpr (WT == GGML_TYPE_Q4_K) {
+        const q8_K_lane l = quantize_q8_K_wave(v, lane);
+        o = v4h{(_Float16) (float) l.q.x, (_Float16) (float) l.q.y, (_Float16) (float) l.q.z, (_Float16) (float) l.q.w};
+        if ((lane & 7) == 0) q.xs[col * (q.kp / 32) + k / 32] = l.d * (float) l.ssum;
+        if (lane == 0) q.xd[col * (q.kp / 256) + k / 256] = l.d;
+    }
+    if (k < q.kp) *(v4h *) (q.x + col * q.kp + k) = o;
+}
+
+// the staged row's 16-byte piece p at slot p ^ (row % 8): fragment reads (16
+// rows, one piece each) spread over the banks
+__device__ __forceinline__ uint4 * moe_slot(_Float16 (*s)[kMoeK], int row, int piece) {
+    return (uint4 *) &s[row][8 * (piece ^ (row & 7))];
+}
+
+// eight bytes' values as f16, less `bias`: the byte in the mantissa under the
+// exponent of 1024
+__device__ __forceinline__ uint4 moe_bytes(uint32_t w0, uint32_t w1, float bias) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 k = {(_Float16) (1024.0f + bias), (_Float16) (1024.0f + bias)};
+    const h2 a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u)) - k;
+    const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u)) - k;
+    const h2 c = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u)) - k;
+    const h2 d = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u)) - k;
+    return make_uint4(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c),
+                      __builtin_bit_cast(uint32_t, d));
+}
+
+// a thread's share of a step's weights: row t / 2, 32 of its 64 elements
+// (Q4_K: 16 elements of each of the step's two blocks)
+template <int WT>
+struct moe_w;
+template <>
+struct moe_w<GGML_TYPE_F16> {
+    uint4 v[4];
+};
+template <>
+struct moe_w<GGML_TYPE_Q8_0> {
+    uint4 v[2];
+    uint16_t d;
+};
+template <>
+struct moe_w<GGML_TYPE_Q4_K> {
+    uint4 hdr, v;
+};
+
+// and of its columns: 16-byte pieces and their places (in halfs)
+typedef uint32_t moe_u4 __attribute__((ext_vector_type(4)));  // (an array of uint4 stayed in memory)
+template <int XP>
+struct moe_x {
+    moe_u4 v[XP];
+    uint32_t at[XP];
+};
+
+template <int XP>
+__device__ __forceinline__ void moe_x_load(moe_x<XP> & x, const _Float16 * base) {
+#pragma unroll
+    for (int u = 0; u < XP; u++) x.v[u] = *(const moe_u4 *) (base + x.at[u]);
+}
+template <int XP>
+__device__ __forceinline__ void moe_x_store(const moe_x<XP> & x, _Float16 (*s)[kMoeK]) {
+#pragma unroll
+    for (int u = 0; u < XP; u++) *(moe_u4 *) moe_slot(s, (threadIdx.x + 256 * u) / 8, threadIdx.x % 8) = x.v[u];
+}
+
+template <int BN>
+struct moe_lds {
+    _Float16 w[2][kMoeRows][kMoeK];
+    _Float16 x[2][BN][kMoeK];
+    float wd[2][2][kMoeRows];  // a block's scale by [buffer][block of the step][row]
+    float wm[2][2][kMoeRows];  // Q4_K: its minimum
+    float xd[2][2][BN];        // the columns' scales
+    float xs[2][2][BN];        // Q4_K: scale times sum
+    int col[BN];               // the columns' places in b
+    int pair[BN];              // and in the result
+};
+
+template <int WT, bool PAIR, int BN>
+__global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
+    constexpr int kQ = WT != GGML_TYPE_F16;
+    constexpr int NR = 4, NC = BN / 32;  // a wave's 16-tiles of rows and columns: 64 rows, BN / 2 columns
+    __shared__ __align__(16) moe_lds<BN> L;
+    const mul_mat_id_args & a = q.a;
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave & 1, wc = wave >> 1;
+    // contiguous runs of tiles an XCD (workgroup i on XCD i % 8), row tiles of a column tile in turn
+    const int64_t total = q.head[0] * q.row_tiles, per = (total + 7) / 8;
+    const int64_t id = blockIdx.x, t = id % 8 * per + id / 8;
+    if (id / 8 >= per || t >= total) return;
+    const int4 tile = q.tiles[t / q.row_tiles];
+    const int64_t m0 = t % q.row_tiles * (PAIR ? 64 : 128);
+    const int n = tile.z;
+    if (tid < BN) {
+        const int p = q.sorted[tile.y + min(tid, n - 1)];
+        L.pair[tid] = p;
+        L.col[tid] = (int) (p / a.used * a.b_ne1 + p % a.used % a.b_ne1);
+    }
+    __syncthreads();
+    if (tile.x < 0) {  // no expert: zeros
+        const int rows = (int) min((int64_t) (PAIR ? 64 : 128), a.M - m0);
+        for (int i = tid; i < n * rows; i += 256) a.out[(int64_t) L.pair[i / rows] * a.M + m0 + i % rows] = 0.0f;
+        return;
+    }
+    // staging: thread t row t / 2 of the tile, half t % 2; PAIR: rows 0 .. 63 of
+    // W, then the same of W2
+    const int srow = tid >> 1, half = tid & 1;
+    const int64_t mrow = min(PAIR ? m0 + (srow & 63) : m0 + srow, a.M - 1);
+    const char * wrow = (PAIR && srow >= 64 ? a.W2 : a.W) + tile.x * a.W_nb2 + mrow * a.W_nb1;
+    const int64_t steps = (a.K + kMoeK - 1) / kMoeK;
+    constexpr int XP = BN * 8 / 256;  // 16-byte pieces of the columns a thread stages
+    moe_x<XP> x;  // (places in 32 bits: mul_mat_id_wide)
+#pragma unroll
+    for (int u = 0; u < XP; u++) x.at[u] = (uint32_t) L.col[(tid + 256 * u) / 8] * (uint32_t) q.kp + 8 * (tid % 8);
+    moe_w<WT> w;
+    float xd = 0.0f, xs = 0.0f;
+    const int scol = tid % BN, sblk = tid / BN;  // the scale this thread stages (sblk < 2)
+    auto load = [&](int64_t s) {
+        const int64_t k0 = s * kMoeK;
+        if constexpr (WT == GGML_TYPE_F16) {
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int64_t k = k0 + 32 * half + 8 * u;
+                w.v[u] = *(const uint4 *) (wrow + 2 * (k < a.K ? k : 0));
+                if (k >= a.K) w.v[u] = make_uint4(0, 0, 0, 0);
+            }
+        } else if constexpr (WT == GGML_TYPE_Q8_0) {
+            const int64_t b = 2 * s + half;
+            const bool ok = 32 * b < a.K;
+            const uint4 * p = (const uint4 *) (wrow + (ok ? 32 * b : 0));
+            w.v[0] = p[0];
+            w.v[1] = p[1];
+            w.d = ok ? *(const uint16_t *) (wrow + a.K + 2 * b) : (uint16_t) 0;
+        } else {
+            const char * blk = wrow + s / 4 * 144;
+            w.hdr = *(const uint4 *) blk;
+            w.v = *(const uint4 *) (blk + 16 + 32 * (s % 4) + 16 * half);
+        }
+        moe_x_load<XP>(x, q.x + k0);
+        if constexpr (kQ) {
+            if (sblk < 2) {
+                const int64_t c = L.col[scol];
+                if constexpr (WT == GGML_TYPE_Q8_0) xd = q.xd[c * (q.kp / 32) + 2 * s + sblk];
+                else {
+                    xd = q.xd[c * (q.kp / 256) + s / 4];
+                    xs = q.xs[c * (q.kp / 32) + 2 * s + sblk];
+                }
+            }
+        }
+    };
+    auto store = [&](int64_t s) {
+        const int b = (int) (s & 1);
+        if constexpr (WT == GGML_TYPE_F16) {
+#pragma unroll
+            for (int u = 0; u < 4; u++) *moe_slot(L.w[b], srow, 4 * half + u) = w.v[u];
+        } else if constexpr (WT == GGML_TYPE_Q8_0) {
+            const uint32_t z = 0x80808080u;
+            const uint32_t v[8] = {w.v[0].x, w.v[0].y, w.v[0].z, w.v[0].w, w.v[1].x, w.v[1].y, w.v[1].z, w.v[1].w};
+#pragma unroll
+            for (int u = 0; u < 4; u++) *moe_slot(L.w[b], srow, 4 * half + u) = moe_bytes(v[2 * u] ^ z, v[2 * u + 1] ^ z, 128.0f);
+            L.wd[b][half][srow] = half_bits_to_float(w.d);
+        } else {
+            const uint32_t lo = 0x0F0F0F0Fu;
+            const uint32_t v[4] = {w.v.x, w.v.y, w.v.z, w.v.w};
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                *moe_slot(L.w[b], srow, 2 * half + u) = moe_bytes(v[2 * u] & lo, v[2 * u + 1] & lo, 0.0f);
+                *moe_slot(L.w[b], srow, 4 + 2 * half + u) = moe_bytes(v[2 * u] >> 4 & lo, v[2 * u + 1] >> 4 & lo, 0.0f);
+            }
+            // block j's 6-bit scale and minimum of the packed 12 bytes
+            const int j = (int) (2 * (s % 4)) + half;
+            const uint32_t lowj = j < 4 ? w.hdr.y >> (8 * j) : w.hdr.w >> (8 * (j - 4));
+            const uint32_t minj = j < 4 ? w.hdr.z >> (8 * j) : w.hdr.w >> (8 * (j - 4) + 4);
+            const uint32_t hs = j < 4 ? 0 : w.hdr.y >> (8 * (j - 4) + 6) & 3, hm = j < 4 ? 0 : w.hdr.z >> (8 * (j - 4) + 6) & 3;
+            const uint32_t sc = j < 4 ? lowj & 63 : (lowj & 15) | hs << 4, mn = j < 4 ? minj & 63 : (minj & 15) | hm << 4;
+            L.wd[b][half][srow] = half_bits_to_float((uint16_t) w.hdr.x) * (float) sc;
+            L.wm[b][half][srow] = -half_bits_to_float((uint16_t) (w.hdr.x >> 16)) * (float) mn;
+        }
+        moe_x_store<XP>(x, L.x[b]);
+        if constexpr (kQ) {
+            if (sblk < 2) {
+                L.xd[b][sblk][scol] = xd;
+                if constexpr (WT == GGML_TYPE_Q4_K) L.xs[b][sblk][scol] = xs;
+            }
+        }
+    };
+    // wave (wr, wc): columns BN / 2 wc ..; rows 64 wr .., or 32 wr .. of both matrices
+    auto tile_row = [&](int i) { return PAIR ? 64 * (i >> 1) + 32 * wr + 16 * (i & 1) : 64 * wr + 16 * i; };
+    moe_v4f acc[NR][NC];
+#pragma unroll
+    for (int i = 0; i < NR; i++)
+#pragma unroll
+        for (int j = 0; j < NC; j++) acc[i][j] = moe_v4f{0, 0, 0, 0};
+    const moe_v4f zero = {0, 0, 0, 0};
+    load(0);
+    for (int64_t s = 0; s < steps; s++) {
+        const int b = (int) (s & 1);
+        store(s);
+        __syncthreads();  // the step is staged; the buffer of the step before is free
+        if (s + 1 < steps) load(s + 1);
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+            moe_v8h wf[NR], xf[NC];
+#pragma unroll
+            for (int i = 0; i < NR; i++)
+                wf[i] = __builtin_bit_cast(moe_v8h, *moe_slot(L.w[b], tile_row(i) + r, 4 * kk + g));
+#pragma unroll
+            for (int j = 0; j < NC; j++)
+                xf[j] = __builtin_bit_cast(moe_v8h, *moe_slot(L.x[b], BN / 2 * wc + 16 * j + r, 4 * kk + g));
+            if constexpr (!kQ) {
+#pragma unroll
+                for (int i = 0; i < NR; i++)
+#pragma unroll
+                    for (int j = 0; j < NC; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[j], wf[i], acc[i][j], 0, 0, 0);
+            } else {
+                float dw[NR], mw[NR];
+#pragma unroll
+                for (int i = 0; i < NR; i++) {
+                    dw[i] = L.wd[b][kk][tile_row(i) + r];
+                    if constexpr (WT == GGML_TYPE_Q4_K) mw[i] = L.wm[b][kk][tile_row(i) + r];
+                }
+#pragma unroll
+                for (int j = 0; j < NC; j++) {
+                    const float4 dx = *(const float4 *) &L.xd[b][kk][BN / 2 * wc + 16 * j + 4 * g];
+                    const float d4[4] = {dx.x, dx.y, dx.z, dx.w};
+                    float s4[4];
+                    if constexpr (WT == GGML_TYPE_Q4_K) *(float4 *) s4 = *(const float4 *) &L.xs[b][kk][BN / 2 * wc + 16 * j + 4 * g];
+#pragma unroll
+                    for (int i = 0; i < NR; i++) {
+                        const moe_v4f p = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[j], wf[i], zero, 0, 0, 0);
+#pragma unroll
+                        for (int v = 0; v < 4; v++) {
+                            acc[i][j][v] = fmaf(p[v], dw[i] * d4[v], acc[i][j][v]);
+                            if constexpr (WT == GGML_TYPE_Q4_K) acc[i][j][v] = fmaf(mw[i], s4[v], acc[i][j][v]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NC; j++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const int c = BN / 2 * wc + 16 * j + 4 * g + v;
+            if (c >= n) continue;
+            float * o = a.out + (int64_t) L.pair[c] * a.M;
+            if constexpr (PAIR) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int64_t m = m0 + 32 * wr + 16 * i + r;
+                    if (m < a.M) o[m] = moe_swiglu(acc[i][j][v], acc[i + 2][j][v]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NR; i++) {
+                    const int64_t m = m0 + 64 * wr + 16 * i + r;
+                    if (m < a.M) o[m] = acc[i][j][v];
+                }
+            }
+        }
+}
+
+// ------------------------------------------------------ the slots' sum ---
+
+// out[m, t] = sum over a token's slots, in order, of w[slot, t] y[m, slot, t]
+__global__ __launch_bounds__(256) void k_moe_sum(moe_sum_args a) {
+    const int64_t per = (a.M + 3) / 4, n = per * a.tokens;
+    for (int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t) gridDim.x * 256) {
+        const int64_t t = i / per, m = i % per * 4;
+        const float * y = a.y + t * a.used * a.M + m;
+        float * o = a.out + t * a.M + m;
+        const int left = (int) min((int64_t) 4, a.M - m);
+        float s[4] = {0, 0, 0, 0};
+        for (int64_t k = 0; k < a.used; k++, y += a.M) {
+            const float w = a.w ? *(const float *) (a.w + k * a.w_nb1 + t * a.w_nb2) : 1.0f;
+            float v[4] = {0, 0, 0, 0};
+            if (a.vec) *(float4 *) v = *(const float4 *) y;
+            else
+                for (int e = 0; e < left; e++) v[e] = y[e];
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[e] = k ? s[e] + v[e] * w : v[e] * w;
+        }
+        if (a.vec) *(float4 *) o = *(const float4 *) s;
+        else
+            for (int e = 0; e < left; e++) o[e] = s[e];
+    }
+}
+
+void launch_moe_sum(const moe_sum_args & in, hipStream_t s, int n_cu) {
+    moe_sum_args a = in;
+    if (a.M == 0 || a.tokens == 0) return;
+    a.vec = a.M % 4 == 0 && (((uintptr_t) a.y | (uintptr_t) a.out) & 15) == 0;
+    const int64_t blocks = ((a.M + 3) / 4 * a.tokens + 255) / 256;
+    hipLaunchKernelGGL(k_moe_sum, dim3((unsigned) (blocks < 16 * n_cu ? blocks : 16 * n_cu)), dim3(256), 0, s, a);
+}
+
+// ------------------------------------------------------------- launches ---
+
+// whether the matrix-core forms read these operands: 16-byte pieces of rows
+static bool moe_aligned(int wtype, const mul_mat_id_args & a) {
+    const uintptr_t w = (uintptr_t) a.W | (uintptr_t) a.W2 | (uintptr_t) a.W_nb2;
+    if (((uintptr_t) a.b | (uintptr_t) a.b_nb1 | (uintptr_t) a.b_nb2) & 15) return false;
+    if (wtype == GGML_TYPE_F16) return a.K % 8 == 0 && ((w | (uintptr_t) a.W_nb1) & 15) == 0;
+    return wtype == GGML_TYPE_Q8_0 || (wtype == GGML_TYPE_Q4_K && (w & 15) == 0);
+}
+
+bool mul_mat_id_wide(int wtype, const mul_mat_id_args & a) {
+    return moe_aligned(wtype, a) && a.pairs > kMoeFew && a.experts <= 960 && a.pairs < 1 << 30 &&
+           (a.K + 63) / 64 * 64 * a.b_ne1 * (a.pairs / a.used) < 1ll << 32;
+}
+
+bool mul_mat_id_pairs(int wtype, const mul_mat_id_args & a) {
+    return moe_aligned(wtype, a) && (a.pairs <= kMoeFew || mul_mat_id_wide(wtype, a));
+}
+
+static size_t moe_carve(int wtype, const mul_mat_id_args & a, moe_wide_args & q, char * base) {
+    q.a = a;
+    q.bn = a.pairs >= 24 * a.experts ? 128 : 32;
+    q.kp = (a.K + 63) / 64 * 64;
+    q.bcols = a.b_ne1 * (a.pairs / a.used);
+    q.row_tiles = (a.M + (a.W2 ? 64 : 128) - 1) / (a.W2 ? 64 : 128);
+    const int64_t runs = a.experts + 1 < a.pairs ? a.experts + 1 : a.pairs;
+    q.max_tiles = (int) (a.pairs / q.bn + runs);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        char * p = base + at;
+        at += (bytes + 255) / 256 * 256;
+        return p;
+    };
+    q.head = (int *) take(256);
+    q.tiles = (int4 *) take((size_t) q.max_tiles * 16);
+    q.sorted = (int *) take((size_t) a.pairs * 4);
+    q.x = (_Float16 *) take((size_t) (q.bcols * q.kp) * 2);
+    if (wtype == GGML_TYPE_Q8_0) q.xd = (float *) take((size_t) (q.bcols * (q.kp / 32)) * 4);
+    if (wtype == GGML_TYPE_Q4_K) {
+        q.xd = (float *) take((size_t) (q.bcols * (q.kp / 256)) * 4);
+        q.xs = (float *) take((size_t) (q.bcols * (q.kp / 32)) * 4);
+    }
+    return at;
+}
+
+size_t mul_mat_id_scratch_bytes(int wtype, const mul_mat_id_args & a) {
+    moe_wide_args q{};
+    return mul_mat_id_wide(wtype, a) ? moe_carve(wtype, a, q, nullptr) : 0;
+}
+
+template <int WT>
+static void launch_moe_wide(const mul_mat_id_args & a, char * scratch, hipStream_t s) {
+    moe_wide_args q{};
+    moe_carve(WT, a, q, scratch);
+    hipLaunchKernelGGL(k_moe_route, dim3(1), dim3(1024), (size_t) (16 * (a.experts + 1)) * 4, s, q);
+    const int64_t waves = (q.kp + 255) / 256 * q.bcols;
+    hipLaunchKernelGGL(k_moe_act<WT>, dim3((unsigned) ((waves + 3) / 4)), dim3(256), 0, s, q);
+    const unsigned grid = (unsigned) ((q.max_tiles * q.row_tiles + 7) / 8 * 8);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, q); };
+    if (q.bn == 128) a.W2 ? go(k_moe_gemm<WT, true, 128>) : go(k_moe_gemm<WT, false, 128>);
+    else a.W2 ? go(k_moe_gemm<WT, true, 32>) : go(k_moe_gemm<WT, false, 32>);
+}
+
+void launch_mul_mat_id(int wtype, const mul_mat_id_args & a, void * scratch, hipStream_t s) {
     if (a.M == 0 || a.pairs == 0) return;
+    if (mul_mat_id_wide(wtype, a)) {
+        if (wtype == GGML_TYPE_Q8_0) launch_moe_wide<GGML_TYPE_Q8_0>(a, (char *) scratch, s);
+        else if (wtype == GGML_TYPE_Q4_K) launch_moe_wide<GGML_TYPE_Q4_K>(a, (char *) scratch, s);
+        else launch_moe_wide<GGML_TYPE_F16>(a, (char *) scratch, s);
+        return;
+    }
+    if (moe_aligned(wtype, a) && a.pairs <= kMoeFew) {
+        const dim3 grid((unsigned) ((a.M + 15) / 16), (unsigned) a.pairs);
+        auto go = [&](auto one, auto pair) {
+            if (a.W2) hipLaunchKernelGGL(pair, grid, dim3(256), 0, s, a);
+            else hipLaunchKernelGGL(one, grid, dim3(256), 0, s, a);
+        };
+        if (wtype == GGML_TYPE_Q8_0) go(k_moe_few<GGML_TYPE_Q8_0, false>, k_moe_few<GGML_TYPE_Q8_0, true>);
+        else if (wtype == GGML_TYPE_Q4_K) go(k_moe_few<GGML_TYPE_Q4_K, false>, k_moe_few<GGML_TYPE_Q4_K, true>);
+        else go(k_moe_few<GGML_TYPE_F16, false>, k_moe_few<GGML_TYPE_F16, true>);
+        return;
+    }
+    // F32 weights, and rows without 16-byte pieces
     const dim3 grid((unsigned) ((a.M + 3) / 4), (unsigned) (a.pairs < 32768 ? a.pairs : 32768));
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
     if (wtype == GGML_TYPE_Q8_0) go(k_mul_mat_id_rows<GGML_TYPE_Q8_0>);

@@ -520,7 +520,7 @@ struct planner {
     bool fattn_kv32(const ggml_tensor * t, const fattn_args & a) const;
     void fattn_quant_out(int i, const ggml_tensor * t, fattn_args & a, const ggml_tensor *& view);
     bool plan_attn_step(int i, const ggml_tensor * t);
-    bool plan_mul_mat_id(const ggml_tensor * t);
+    bool plan_mul_mat_id(int i, const ggml_tensor * t);
     void plan_ssm_conv(const ggml_tensor * t);
     bool plan_ssm_scan(const ggml_tensor * t);
 };
@@ -1921,7 +1921,13 @@ static bool overlaps_operand(const ggml_tensor * t) {
     return false;
 }
 
-bool planner::plan_mul_mat_id(const ggml_tensor * t) {
+static bool same_shape(const ggml_tensor * a, const ggml_tensor * b) {
+    for (int d = 0; d < 4; d++)
+        if (a->ne[d] != b->ne[d]) return false;
+    return true;
+}
+
+bool planner::plan_mul_mat_id(int i, const ggml_tensor * t) {
     const ggml_tensor *w = t->src[0], *x = t->src[1], *ids = t->src[2];
     if (overlaps_operand(t)) return fail(t, "MUL_MAT_ID output overlaps its own input");
     const int wtype = w->type;
@@ -1932,8 +1938,48 @@ bool planner::plan_mul_mat_id(const ggml_tensor * t) {
     a.ids = (const char *) ids->data, a.ids_nb0 = (int64_t) ids->nb[0], a.ids_nb1 = (int64_t) ids->nb[1];
     a.used = ids->ne[0], a.pairs = ids->ne[0] * ids->ne[1];
     a.out = (float *) t->data;
+    const ggml_tensor * produced = t;
+    // SwiGLU: SILU(this) * another MUL_MAT_ID of the same columns and ids,
+    // whichever of the two comes first, in one launch here
+    auto silu_of = [&](const ggml_tensor * m) -> const ggml_tensor * {
+        const ggml_tensor * u = sole_consumer(m, index.at(m) + 1);
+        return u && u->op == GGML_OP_UNARY && u->op_params[0] == GGML_UNARY_OP_SILU && u->src[0] == m ? u : nullptr;
+    };
+    const ggml_tensor * silu = silu_of(t);
+    const ggml_tensor * hm = sole_consumer(silu ? silu : t, i + 1);
+    if (hm && hm->op == GGML_OP_MUL && same_shape(hm, t) && is_contiguous(hm) && hm->type == GGML_TYPE_F32) {
+        const ggml_tensor * o = hm->src[0] == (silu ? silu : t) ? hm->src[1] : hm->src[0];
+        const ggml_tensor * other = silu ? o : o->op == GGML_OP_UNARY ? o->src[0] : nullptr;  // the partner product
+        const ggml_tensor * act = silu ? silu : o;
+        bool ok = other && other != t && other->op == GGML_OP_MUL_MAT_ID && index.count(other) && index.at(other) > i &&
+                  other->src[1] == x && other->src[2] == ids && other->src[0]->type == wtype &&
+                  same_shape(other->src[0], w) && same_shape(other, t) && supports_op(be->dev, other) &&
+                  ready_before(other->src[0], i);
+        for (int d = 0; d < 4 && ok; d++) ok = other->src[0]->nb[d] == w->nb[d];
+        if (ok) ok = silu ? sole_consumer(other, index.at(other) + 1) == hm
+                          : silu_of(other) == act && sole_consumer(act, index.at(act) + 1) == hm;
+        if (ok) {
+            mul_mat_id_args p = a;
+            const char * ow = (const char *) other->src[0]->data;
+            p.W = silu ? a.W : ow;
+            p.W2 = silu ? ow : a.W;
+            p.out = (float *) hm->data;
+            hoist h;
+            h.nodes = {other, act, hm};
+            h.reads = {span_of(w), span_of(other->src[0]), span_of(x), span_of(ids)};
+            h.writes = {span_of(hm)};
+            if (mul_mat_id_pairs(wtype, p) && hoist_ok(i, h)) {
+                a = p;
+                produced = hm;
+                deferred[other] = other;
+                deferred[act] = act;
+                deferred[hm] = hm;
+            }
+        }
+    }
     backend_state * b = be;
-    if (wtype == GGML_TYPE_Q8_0 || wtype == GGML_TYPE_Q4_K) {
+    gen_need = std::max(gen_need, mul_mat_id_scratch_bytes(wtype, a));
+    if ((wtype == GGML_TYPE_Q8_0 || wtype == GGML_TYPE_Q4_K) && !mul_mat_id_wide(wtype, a)) {
         const tview xv = make_view(x);
         const int64_t N = x->ne[1] * x->ne[2];
         act_need = std::max(act_need, act_bytes(wtype, a.K, N));
@@ -1948,12 +1994,13 @@ bool planner::plan_mul_mat_id(const ggml_tensor * t) {
             [=](hipStream_t s) {
                 mul_mat_id_args r = a;
                 r.act = act_carve(wtype, act_base(b), K, N);
-                launch_mul_mat_id(wtype, r, s);
+                launch_mul_mat_id(wtype, r, gen_base(b), s);
             },
-            t, "mul_mat_id");
+            produced, produced == t ? "mul_mat_id" : "mul_mat_id_swiglu");
         return true;
     }
-    add_step([=](hipStream_t s) { launch_mul_mat_id(wtype, a, s); }, t, "mul_mat_id");
+    add_step([=](hipStream_t s) { launch_mul_mat_id(wtype, a, gen_base(b), s); }, produced,
+             produced == t ? "mul_mat_id" : "mul_mat_id_swiglu");
     return true;
 }
 
@@ -2238,7 +2285,7 @@ bool planner::plan() {
                 if (!plan_fattn(i, t)) return false;
                 continue;
             case GGML_OP_MUL_MAT_ID:
-                if (!plan_mul_mat_id(t)) return false;
+                if (!plan_mul_mat_id(i, t)) return false;
                 continue;
             case GGML_OP_ARGSORT: {
                 const tview dv = make_view(t), av = make_view(t->src[0]);

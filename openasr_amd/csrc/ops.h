@@ -427,10 +427,30 @@ struct mul_mat_id_args {
     int64_t b_ne1, b_nb1, b_nb2;
     const char * ids;
     int64_t ids_nb0, ids_nb1, used, pairs;
-    act_buffers act;
+    act_buffers act;  // quantized weights, where the launch is not wide
     float * out;
+    // the SwiGLU pair (mul_mat_id_pairs): out = silu(W x) * (W2 x), W2 laid
+    // out as W
+    const char * W2;
 };
-void launch_mul_mat_id(int wtype, const mul_mat_id_args & a, hipStream_t s);
+// whether the launch takes its columns by expert from f32 (it quantizes them
+// itself, into scratch); whether it can take a SwiGLU pair
+bool mul_mat_id_wide(int wtype, const mul_mat_id_args & a);
+bool mul_mat_id_pairs(int wtype, const mul_mat_id_args & a);
+size_t mul_mat_id_scratch_bytes(int wtype, const mul_mat_id_args & a);
+void launch_mul_mat_id(int wtype, const mul_mat_id_args & a, void * scratch, hipStream_t s);
+
+// the weighted sum over a token's slots of y [M, used, tokens] (contiguous):
+// out[m, t] = sum of w[slot, t] y[m, slot, t] in slot order (w null: of y)
+struct moe_sum_args {
+    const float * y;
+    const char * w;
+    int64_t w_nb1, w_nb2;
+    float * out;
+    int64_t M, used, tokens;
+    bool vec;  // set by the launcher
+};
+void launch_moe_sum(const moe_sum_args & a, hipStream_t s, int n_cu);
 
 // GGML_OP_ARGSORT: the indices that sort each row, equal elements in their
 // order, NaN the largest; GGML_OP_SUM_ROWS
