@@ -288,9 +288,21 @@ __global__ __launch_bounds__(1024) void k_moe_route(moe_wide_args q) {
         const int e = *(const int32_t *) (a.ids + (p % (int) a.used) * a.ids_nb0 + (int64_t) (p / (int) a.used) * a.ids_nb1);
         return e < 0 || e >= a.experts ? (int) a.experts : e;
     };
-    for (int k = 0; k < per; k++) {
-        const int p = ((wave * per + k) * 64) + lane;
-        if (p < pairs) atomicAdd(&s_hist[wave * bins + expert_of(p)], 1);
+    // a batch of groups' ids in flight at once (one by one, each waits for its load)
+    constexpr int kBatch = 8;
+    int e[kBatch];
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int k = 0; k < kBatch; k++) {
+            const int p = (wave * per + k0 + k) * 64 + lane;
+            e[k] = k0 + k < per && p < pairs ? expert_of(p) : -1;
+        }
+    };
+    for (int k0 = 0; k0 < per; k0 += kBatch) {
+        load(k0);
+#pragma unroll
+        for (int k = 0; k < kBatch; k++)
+            if (e[k] >= 0) atomicAdd(&s_hist[wave * bins + e[k]], 1);
     }
     __syncthreads();
     // the bins' totals, their exclusive sums (places and tiles) over bins in order
@@ -332,20 +344,23 @@ __global__ __launch_bounds__(1024) void k_moe_route(moe_wide_args q) {
     }
     if (tid == 0) q.head[0] = tbase;
     // places: within a group of 64, pairs of one expert in lane order
-    for (int k = 0; k < per; k++) {
-        const int p = ((wave * per + k) * 64) + lane;
-        const bool ok = p < pairs;
-        const int e = ok ? expert_of(p) : -1;
-        uint64_t same = __ballot(ok);
-        for (int bit = 1; bit < 2 * bins; bit <<= 1) {
-            const uint64_t set = __ballot(ok && (e & bit));
-            same &= (e & bit) ? set : ~set;
+    for (int k0 = 0; k0 < per; k0 += kBatch) {
+        if (per > kBatch) load(k0);
+#pragma unroll
+        for (int k = 0; k < kBatch; k++) {
+            if (k0 + k >= per) break;
+            const bool ok = e[k] >= 0;
+            uint64_t same = __ballot(ok);
+            for (int bit = 1; bit < bins; bit <<= 1) {
+                const uint64_t set = __ballot(ok && (e[k] & bit));
+                same &= (e[k] & bit) ? set : ~set;
+            }
+            const int rank = __popcll(same & ((1ull << lane) - 1));
+            if (ok) q.sorted[s_hist[wave * bins + e[k]] + rank] = (wave * per + k0 + k) * 64 + lane;
+            __builtin_amdgcn_wave_barrier();
+            if (ok && rank == 0) s_hist[wave * bins + e[k]] += __popcll(same);
+            __builtin_amdgcn_wave_barrier();
         }
-        const int rank = __popcll(same & ((1ull << lane) - 1));
-        if (ok) q.sorted[s_hist[wave * bins + e] + rank] = p;
-        __builtin_amdgcn_wave_barrier();
-        if (ok && rank == 0) s_hist[wave * bins + e] += __popcll(same);
-        __builtin_amdgcn_wave_barrier();
     }
 }
 

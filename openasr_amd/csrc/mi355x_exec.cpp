@@ -205,7 +205,7 @@ struct hoist {
 // fusions a previous planning pass found unsafe under the graph's
 // allocation, or that a reader could not take (see validate and replan)
 struct plan_exclusions {
-    std::unordered_set<const ggml_tensor *> no_bypass, no_defer, no_divert, no_fold, no_naive;
+    std::unordered_set<const ggml_tensor *> no_bypass, no_defer, no_divert, no_fold, no_naive, no_sum;
 };
 
 struct planner {
@@ -233,8 +233,10 @@ struct planner {
     std::unordered_set<const ggml_tensor *> no_divert;
     // REPEATs to materialise, unfused attention chains to run op by op
     std::unordered_set<const ggml_tensor *> no_fold, no_naive;
+    // MUL_MAT_IDs whose slots are summed op by op
+    std::unordered_set<const ggml_tensor *> no_sum;
     bool replan = false;
-    plan_exclusions exclusions() const { return {no_bypass, no_defer, no_divert, no_fold, no_naive}; }
+    plan_exclusions exclusions() const { return {no_bypass, no_defer, no_divert, no_fold, no_naive, no_sum}; }
 
     // GQA expansions (match_gqa) every reader of which reads the source's kv
     // heads instead: the REPEAT is not launched
@@ -279,7 +281,7 @@ struct planner {
 
     planner(backend_state * b, const ggml_cgraph * g, const plan_exclusions & x = {})
         : be(b), cg(g), n_cu(b->dev->n_cu), no_bypass(x.no_bypass), no_defer(x.no_defer), no_divert(x.no_divert),
-          no_fold(x.no_fold), no_naive(x.no_naive) {}
+          no_fold(x.no_fold), no_naive(x.no_naive), no_sum(x.no_sum) {}
 
     std::unordered_map<const ggml_tensor *, int> index;  // node -> position in the graph
     // CONT nodes whose copy is skipped: consumers read the CONT's strided
@@ -521,6 +523,13 @@ struct planner {
     void fattn_quant_out(int i, const ggml_tensor * t, fattn_args & a, const ggml_tensor *& view);
     bool plan_attn_step(int i, const ggml_tensor * t);
     bool plan_mul_mat_id(int i, const ggml_tensor * t);
+    // the weighted sums over a token's experts (find_slot_sums), by their last ADD
+    struct slot_sum {
+        const ggml_tensor *y = nullptr, *mul = nullptr, *w = nullptr, *out = nullptr;
+        std::vector<const ggml_tensor *> adds;
+    };
+    std::unordered_map<const ggml_tensor *, slot_sum> slot_sums;
+    void find_slot_sums();
     void plan_ssm_conv(const ggml_tensor * t);
     bool plan_ssm_scan(const ggml_tensor * t);
 };
@@ -2004,6 +2013,67 @@ bool planner::plan_mul_mat_id(int i, const ggml_tensor * t) {
     return true;
 }
 
+// The weighted sum over a token's experts as hosts write it: y [M, used,
+// tokens], read only by its MUL with w [1, used, tokens] (optional), the
+// result's slots read as `used` 2-D views, slot by slot, by a chain of ADDs.
+// One launch at the last ADD, from y, in the chain's order.
+void planner::find_slot_sums() {
+    for (int i = 0; i < cg->n_nodes; i++) {
+        const ggml_tensor * y = cg->nodes[i];
+        if (y->op != GGML_OP_MUL_MAT_ID || (y->flags & GGML_TENSOR_FLAG_OUTPUT) || no_sum.count(y)) continue;
+        const int64_t M = y->ne[0], used = y->ne[1], T = y->ne[2];
+        if (used < 2 || used > 64) continue;
+        slot_sum j;
+        j.y = y;
+        const ggml_tensor * base = y;  // whose views the chain reads
+        const ggml_tensor * mul = sole_consumer(y, i + 1);
+        if (mul && mul->op == GGML_OP_MUL && mul->src[0] == y && same_shape(mul, y) && is_contiguous(mul) &&
+            !(mul->flags & GGML_TENSOR_FLAG_OUTPUT)) {
+            const ggml_tensor * w = mul->src[1];
+            if (w == y || w->type != GGML_TYPE_F32 || bypass.count(root_of(w)) || w->ne[0] != 1 || w->ne[1] != used || w->ne[2] != T || w->ne[3] != 1) continue;
+            j.mul = mul;
+            j.w = w;
+            base = mul;
+        }
+        // the views: every reader of base
+        std::vector<const ggml_tensor *> views((size_t) used, nullptr);
+        int readers = 0;
+        bool ok = true;
+        for (int k = index.at(base) + 1; k < cg->n_nodes && ok; k++) {
+            const ggml_tensor * v = cg->nodes[k];
+            for (int s = 0; s < GGML_MAX_SRC && ok; s++) ok = v->src[s] != base || (v->op == GGML_OP_VIEW && s == 0);
+            if (v->view_src != base) continue;
+            readers++;
+            const size_t at = (size_t) ((const char *) v->data - (const char *) base->data);
+            ok = ok && v->op == GGML_OP_VIEW && v->ne[0] == M && v->ne[1] == T && v->ne[2] == 1 && v->ne[3] == 1 &&
+                 v->nb[0] == 4 && (T == 1 || v->nb[1] == base->nb[2]) && at % base->nb[1] == 0 &&
+                 (int64_t) (at / base->nb[1]) < used && !views[at / base->nb[1]] && single_use(v);
+            if (ok) views[at / base->nb[1]] = v;
+        }
+        if (!ok || readers != (int) used || (base == y && uses[y] != (int) used)) continue;
+        if (base != y && uses[base] != (int) used) continue;
+        // the chain ((slot 0 + slot 1) + slot 2) + ...
+        const ggml_tensor * sum = views[0];
+        for (int64_t k = 1; k < used && ok; k++) {
+            const ggml_tensor * add = sole_consumer(views[(size_t) k], index.at(views[(size_t) k]) + 1);
+            ok = add && add->op == GGML_OP_ADD && add->src[0] == sum && add->src[1] == views[(size_t) k] &&
+                 add->type == GGML_TYPE_F32 && is_contiguous(add) && add->ne[0] == M && add->ne[1] == T && add->ne[2] == 1 &&
+                 add->ne[3] == 1 && (k == 1 || single_use(sum));
+            if (!ok) break;
+            j.adds.push_back(add);
+            sum = add;
+        }
+        if (!ok) continue;
+        const span out = span_of(sum);
+        if (overlap(out, span_of(y)) || (j.w && overlap(out, span_of(j.w)))) continue;
+        j.out = sum;
+        if (j.mul) deferred[j.mul] = sum;
+        for (const ggml_tensor * a : j.adds)
+            if (a != sum) deferred[a] = sum;
+        slot_sums[sum] = j;
+    }
+}
+
 void planner::plan_ssm_conv(const ggml_tensor * t) {
     const ggml_tensor *sx = t->src[0], *w = t->src[1];
     ssm_conv_args a{};
@@ -2075,6 +2145,16 @@ bool planner::validate() {
             ok = false;
         }
     }
+    // a slots' sum reads the products, and the weights, at its last ADD
+    for (const auto & ss : slot_sums) {
+        const int at = index.at(ss.first);
+        const ggml_tensor *y = ss.second.y, *w = ss.second.w;
+        if (written_between(span_of(y), index.at(y), at - 1, false) ||
+            (w && written_between(span_of(w), index.at(ss.second.mul), at - 1, false))) {
+            no_sum.insert(y);
+            ok = false;
+        }
+    }
     // a fused attention chain reads its operands at its output's position
     for (const auto & nj : naive_jobs) {
         const int at = index.at(nj.first);
@@ -2093,6 +2173,7 @@ bool planner::plan() {
     count_uses();
     find_bypass();
     find_naive();
+    find_slot_sums();
     find_gqa_skip();
     if (naive_dropped) {
         // a chain dropped after the expansions were decided: decide again without it
@@ -2153,9 +2234,22 @@ bool planner::plan() {
             case GGML_OP_ADD:
             case GGML_OP_SUB:
             case GGML_OP_MUL:
-            case GGML_OP_DIV:
+            case GGML_OP_DIV: {
+                auto ss = slot_sums.find(t);
+                if (ss != slot_sums.end()) {
+                    const slot_sum & j = ss->second;
+                    if (j.w && reads_unwritten(t, j.w)) return false;
+                    moe_sum_args a{};
+                    a.y = (const float *) j.y->data;
+                    if (j.w) a.w = (const char *) j.w->data, a.w_nb1 = (int64_t) j.w->nb[1], a.w_nb2 = (int64_t) j.w->nb[2];
+                    a.out = (float *) t->data;
+                    a.M = j.y->ne[0], a.used = j.y->ne[1], a.tokens = j.y->ne[2];
+                    add_step([=](hipStream_t s) { launch_moe_sum(a, s, ncu); }, t, "slot_sum");
+                    break;
+                }
                 plan_binary(t);
                 break;
+            }
             case GGML_OP_SCALE: {
                 const tview dv = make_view(t), av = make_view(t->src[0]);
                 const float sc = op_f32(t, 0), bias = op_f32(t, 1);
