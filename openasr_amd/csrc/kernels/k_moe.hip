@@ -246,11 +246,11 @@ __global__ __launch_bounds__(256) void k_moe_few(mul_mat_id_args a) {
 
 // ------------------------------------------------ many columns: tile GEMM ---
 //
-// k_moe_route sorts the pairs by expert (a counting sort of one workgroup,
+// k_moe_prepare sorts the pairs by expert (a counting sort of one workgroup,
 // each expert's pairs in their order) and cuts every expert's run into tiles
-// of BN columns. k_moe_act makes the columns' f16 operands: the rounded
-// values of F16 weights, the whole numbers of the quantized blocks otherwise
-// (with their scales beside them). k_moe_gemm takes 128 weight rows (PAIR: 64
+// of BN columns; its other workgroups make the columns' f16 operands: the
+// rounded values of F16 weights, the whole numbers of the quantized blocks
+// otherwise (with their scales beside them). k_moe_gemm takes 128 weight rows (PAIR: 64
 // of each matrix) by BN columns of one expert, K in steps of 64 through two
 // LDS buffers (16-byte pieces swizzled by row), the next step's loads in
 // flight under the current one's products.
@@ -275,7 +275,7 @@ struct moe_wide_args {
     int bn, max_tiles;
 };
 
-__global__ __launch_bounds__(1024) void k_moe_route(moe_wide_args q) {
+__device__ __forceinline__ void moe_route(const moe_wide_args & q) {
     extern __shared__ int s_hist[];  // [16][bins], bins = experts + 1 (no expert)
     const mul_mat_id_args & a = q.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -364,12 +364,17 @@ __global__ __launch_bounds__(1024) void k_moe_route(moe_wide_args q) {
     }
 }
 
-// one wave 256 elements of a column
+// the first workgroup sorts, the others make the operands, one wave 256
+// elements of a column
 template <int WT>
-__global__ __launch_bounds__(256) void k_moe_act(moe_wide_args q) {
+__global__ __launch_bounds__(1024) void k_moe_prepare(moe_wide_args q) {
+    if (blockIdx.x == 0) {
+        moe_route(q);
+        return;
+    }
     const mul_mat_id_args & a = q.a;
     const int lane = threadIdx.x & 63;
-    const int64_t chunks = (q.kp + 255) / 256, w = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t chunks = (q.kp + 255) / 256, w = (int64_t) (blockIdx.x - 1) * 16 + (threadIdx.x >> 6);
     const int64_t col = w / chunks, k = w % chunks * 256 + 4 * lane;
     if (col >= q.bcols) return;
     const float * x = (const float *) (a.b + (col % a.b_ne1) * a.b_nb1 + (col / a.b_ne1) * a.b_nb2);
@@ -413,32 +418,31 @@ __device__ __forceinline__ uint4 moe_bytes(uint32_t w0, uint32_t w1, float bias)
 // (Q4_K: 16 elements of each of the step's two blocks)
 template <int WT>
 struct moe_w;
+typedef uint32_t moe_u4 __attribute__((ext_vector_type(4)));  // (an array of uint4 stayed in memory)
 template <>
 struct moe_w<GGML_TYPE_F16> {
-    uint4 v[4];
+    moe_u4 v[4];
 };
 template <>
 struct moe_w<GGML_TYPE_Q8_0> {
-    uint4 v[2];
+    moe_u4 v[2];
     uint16_t d;
 };
 template <>
 struct moe_w<GGML_TYPE_Q4_K> {
-    uint4 hdr, v;
+    moe_u4 hdr, v;
 };
 
-// and of its columns: 16-byte pieces and their places (in halfs)
-typedef uint32_t moe_u4 __attribute__((ext_vector_type(4)));  // (an array of uint4 stayed in memory)
+// and of its columns, 16-byte pieces
 template <int XP>
 struct moe_x {
     moe_u4 v[XP];
-    uint32_t at[XP];
 };
 
 template <int XP>
-__device__ __forceinline__ void moe_x_load(moe_x<XP> & x, const _Float16 * base) {
+__device__ __forceinline__ void moe_x_load(moe_x<XP> & x, const _Float16 * base, const uint32_t (&at)[XP]) {
 #pragma unroll
-    for (int u = 0; u < XP; u++) x.v[u] = *(const moe_u4 *) (base + x.at[u]);
+    for (int u = 0; u < XP; u++) x.v[u] = *(const moe_u4 *) (base + at[u]);
 }
 template <int XP>
 __device__ __forceinline__ void moe_x_store(const moe_x<XP> & x, _Float16 (*s)[kMoeK]) {
@@ -491,50 +495,57 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
     const char * wrow = (PAIR && srow >= 64 ? a.W2 : a.W) + tile.x * a.W_nb2 + mrow * a.W_nb1;
     const int64_t steps = (a.K + kMoeK - 1) / kMoeK;
     constexpr int XP = BN * 8 / 256;  // 16-byte pieces of the columns a thread stages
-    moe_x<XP> x;  // (places in 32 bits: mul_mat_id_wide)
+    uint32_t xat[XP];  // the columns' pieces (places in 32 bits: mul_mat_id_wide)
 #pragma unroll
-    for (int u = 0; u < XP; u++) x.at[u] = (uint32_t) L.col[(tid + 256 * u) / 8] * (uint32_t) q.kp + 8 * (tid % 8);
-    moe_w<WT> w;
-    float xd = 0.0f, xs = 0.0f;
+    for (int u = 0; u < XP; u++) xat[u] = (uint32_t) L.col[(tid + 256 * u) / 8] * (uint32_t) q.kp + 8 * (tid % 8);
     const int scol = tid % BN, sblk = tid / BN;  // the scale this thread stages (sblk < 2)
-    auto load = [&](int64_t s) {
+    struct stage {
+        moe_w<WT> w;
+        moe_x<XP> x;
+        float xd, xs;
+    };
+    auto load = [&](int64_t s, stage & st) {
+        moe_w<WT> & w = st.w;
         const int64_t k0 = s * kMoeK;
         if constexpr (WT == GGML_TYPE_F16) {
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 const int64_t k = k0 + 32 * half + 8 * u;
-                w.v[u] = *(const uint4 *) (wrow + 2 * (k < a.K ? k : 0));
-                if (k >= a.K) w.v[u] = make_uint4(0, 0, 0, 0);
+                w.v[u] = *(const moe_u4 *) (wrow + 2 * (k < a.K ? k : 0));  // past K: masked when stored
             }
         } else if constexpr (WT == GGML_TYPE_Q8_0) {
             const int64_t b = 2 * s + half;
-            const bool ok = 32 * b < a.K;
-            const uint4 * p = (const uint4 *) (wrow + (ok ? 32 * b : 0));
+            const int64_t bc = 32 * b < a.K ? b : 0;  // past K: the columns' scale is zero
+            const moe_u4 * p = (const moe_u4 *) (wrow + 32 * bc);
             w.v[0] = p[0];
             w.v[1] = p[1];
-            w.d = ok ? *(const uint16_t *) (wrow + a.K + 2 * b) : (uint16_t) 0;
+            w.d = *(const uint16_t *) (wrow + a.K + 2 * bc);
         } else {
             const char * blk = wrow + s / 4 * 144;
-            w.hdr = *(const uint4 *) blk;
-            w.v = *(const uint4 *) (blk + 16 + 32 * (s % 4) + 16 * half);
+            w.hdr = *(const moe_u4 *) blk;
+            w.v = *(const moe_u4 *) (blk + 16 + 32 * (s % 4) + 16 * half);
         }
-        moe_x_load<XP>(x, q.x + k0);
+        moe_x_load<XP>(st.x, q.x + k0, xat);
         if constexpr (kQ) {
             if (sblk < 2) {
                 const int64_t c = L.col[scol];
-                if constexpr (WT == GGML_TYPE_Q8_0) xd = q.xd[c * (q.kp / 32) + 2 * s + sblk];
+                if constexpr (WT == GGML_TYPE_Q8_0) st.xd = q.xd[c * (q.kp / 32) + 2 * s + sblk];
                 else {
-                    xd = q.xd[c * (q.kp / 256) + s / 4];
-                    xs = q.xs[c * (q.kp / 32) + 2 * s + sblk];
+                    st.xd = q.xd[c * (q.kp / 256) + s / 4];
+                    st.xs = q.xs[c * (q.kp / 32) + 2 * s + sblk];
                 }
             }
         }
     };
-    auto store = [&](int64_t s) {
+    auto store = [&](int64_t s, const stage & st) {
+        const moe_w<WT> & w = st.w;
         const int b = (int) (s & 1);
         if constexpr (WT == GGML_TYPE_F16) {
 #pragma unroll
-            for (int u = 0; u < 4; u++) *moe_slot(L.w[b], srow, 4 * half + u) = w.v[u];
+            for (int u = 0; u < 4; u++) {
+                const uint32_t in = s * kMoeK + 32 * half + 8 * u < a.K ? 0xFFFFFFFFu : 0u;
+                *(moe_u4 *) moe_slot(L.w[b], srow, 4 * half + u) = w.v[u] & in;
+            }
         } else if constexpr (WT == GGML_TYPE_Q8_0) {
             const uint32_t z = 0x80808080u;
             const uint32_t v[8] = {w.v[0].x, w.v[0].y, w.v[0].z, w.v[0].w, w.v[1].x, w.v[1].y, w.v[1].z, w.v[1].w};
@@ -558,11 +569,11 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
             L.wd[b][half][srow] = half_bits_to_float((uint16_t) w.hdr.x) * (float) sc;
             L.wm[b][half][srow] = -half_bits_to_float((uint16_t) (w.hdr.x >> 16)) * (float) mn;
         }
-        moe_x_store<XP>(x, L.x[b]);
+        moe_x_store<XP>(st.x, L.x[b]);
         if constexpr (kQ) {
             if (sblk < 2) {
-                L.xd[b][sblk][scol] = xd;
-                if constexpr (WT == GGML_TYPE_Q4_K) L.xs[b][sblk][scol] = xs;
+                L.xd[b][sblk][scol] = st.xd;
+                if constexpr (WT == GGML_TYPE_Q4_K) L.xs[b][sblk][scol] = st.xs;
             }
         }
     };
@@ -574,14 +585,10 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
 #pragma unroll
         for (int j = 0; j < NC; j++) acc[i][j] = moe_v4f{0, 0, 0, 0};
     const moe_v4f zero = {0, 0, 0, 0};
-    load(0);
-    for (int64_t s = 0; s < steps; s++) {
-        const int b = (int) (s & 1);
-        store(s);
-        __syncthreads();  // the step is staged; the buffer of the step before is free
-        if (s + 1 < steps) load(s + 1);
+    auto multiply = [&](int b) {
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
+            __builtin_amdgcn_sched_barrier(0);  // (one block's operands at a time: more in flight spill)
             moe_v8h wf[NR], xf[NC];
 #pragma unroll
             for (int i = 0; i < NR; i++)
@@ -619,6 +626,14 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
                 }
             }
         }
+    };
+    stage st;
+    load(0, st);
+    for (int64_t s = 0; s < steps; s++) {
+        store(s, st);
+        __syncthreads();  // the step is staged; the buffer of the step before is free
+        if (s + 1 < steps) load(s + 1, st);
+        multiply((int) (s & 1));
     }
 #pragma unroll
     for (int j = 0; j < NC; j++)
@@ -645,36 +660,47 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
 
 // ------------------------------------------------------ the slots' sum ---
 
-// out[m, t] = sum over a token's slots, in order, of w[slot, t] y[m, slot, t]
+// out[m, t] = sum over a token's slots, in order, of w[slot, t] y[m, slot, t];
+// four rows a thread, four slots' loads in flight
+template <bool VEC>
 __global__ __launch_bounds__(256) void k_moe_sum(moe_sum_args a) {
-    const int64_t per = (a.M + 3) / 4, n = per * a.tokens;
-    for (int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t) gridDim.x * 256) {
-        const int64_t t = i / per, m = i % per * 4;
+    const int64_t m = ((int64_t) blockIdx.x * 256 + threadIdx.x) * 4;
+    if (m >= a.M) return;
+    const int left = (int) min((int64_t) 4, a.M - m);
+    for (int64_t t = blockIdx.y; t < a.tokens; t += gridDim.y) {
         const float * y = a.y + t * a.used * a.M + m;
-        float * o = a.out + t * a.M + m;
-        const int left = (int) min((int64_t) 4, a.M - m);
+        const char * wp = a.w + t * a.w_nb2;
         float s[4] = {0, 0, 0, 0};
-        for (int64_t k = 0; k < a.used; k++, y += a.M) {
-            const float w = a.w ? *(const float *) (a.w + k * a.w_nb1 + t * a.w_nb2) : 1.0f;
-            float v[4] = {0, 0, 0, 0};
-            if (a.vec) *(float4 *) v = *(const float4 *) y;
-            else
-                for (int e = 0; e < left; e++) v[e] = y[e];
+        for (int64_t k0 = 0; k0 < a.used; k0 += 4) {
+            float v[4][4], w[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[e] = k ? s[e] + v[e] * w : v[e] * w;
+            for (int u = 0; u < 4; u++) {
+                const int64_t k = k0 + u < a.used ? k0 + u : k0;
+                w[u] = a.w ? *(const float *) (wp + k * a.w_nb1) : 1.0f;
+                if constexpr (VEC) *(float4 *) v[u] = *(const float4 *) (y + k * a.M);
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[u][e] = y[k * a.M + min(e, left - 1)];
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (k0 + u < a.used)  // (the first slot's product as it is: 0 + -0 would be 0)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[e] = k0 + u == 0 ? v[u][e] * w[u] : s[e] + v[u][e] * w[u];
         }
-        if (a.vec) *(float4 *) o = *(const float4 *) s;
+        float * o = a.out + t * a.M + m;
+        if constexpr (VEC) *(float4 *) o = *(const float4 *) s;
         else
             for (int e = 0; e < left; e++) o[e] = s[e];
     }
 }
 
-void launch_moe_sum(const moe_sum_args & in, hipStream_t s, int n_cu) {
-    moe_sum_args a = in;
+void launch_moe_sum(const moe_sum_args & a, hipStream_t s) {
     if (a.M == 0 || a.tokens == 0) return;
-    a.vec = a.M % 4 == 0 && (((uintptr_t) a.y | (uintptr_t) a.out) & 15) == 0;
-    const int64_t blocks = ((a.M + 3) / 4 * a.tokens + 255) / 256;
-    hipLaunchKernelGGL(k_moe_sum, dim3((unsigned) (blocks < 16 * n_cu ? blocks : 16 * n_cu)), dim3(256), 0, s, a);
+    const bool vec = a.M % 4 == 0 && (((uintptr_t) a.y | (uintptr_t) a.out) & 15) == 0;
+    const dim3 grid((unsigned) ((a.M + 1023) / 1024), (unsigned) (a.tokens < 65535 ? a.tokens : 65535));
+    if (vec) hipLaunchKernelGGL(k_moe_sum<true>, grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(k_moe_sum<false>, grid, dim3(256), 0, s, a);
 }
 
 // ------------------------------------------------------------- launches ---
@@ -731,9 +757,9 @@ template <int WT>
 static void launch_moe_wide(const mul_mat_id_args & a, char * scratch, hipStream_t s) {
     moe_wide_args q{};
     moe_carve(WT, a, q, scratch);
-    hipLaunchKernelGGL(k_moe_route, dim3(1), dim3(1024), (size_t) (16 * (a.experts + 1)) * 4, s, q);
     const int64_t waves = (q.kp + 255) / 256 * q.bcols;
-    hipLaunchKernelGGL(k_moe_act<WT>, dim3((unsigned) ((waves + 3) / 4)), dim3(256), 0, s, q);
+    hipLaunchKernelGGL(k_moe_prepare<WT>, dim3((unsigned) ((waves + 15) / 16 + 1)), dim3(1024),
+                       (size_t) (16 * (a.experts + 1)) * 4, s, q);
     const unsigned grid = (unsigned) ((q.max_tiles * q.row_tiles + 7) / 8 * 8);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, q); };
     if (q.bn == 128) a.W2 ? go(k_moe_gemm<WT, true, 128>) : go(k_moe_gemm<WT, false, 128>);

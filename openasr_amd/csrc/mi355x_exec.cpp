@@ -2244,7 +2244,7 @@ bool planner::plan() {
                     if (j.w) a.w = (const char *) j.w->data, a.w_nb1 = (int64_t) j.w->nb[1], a.w_nb2 = (int64_t) j.w->nb[2];
                     a.out = (float *) t->data;
                     a.M = j.y->ne[0], a.used = j.y->ne[1], a.tokens = j.y->ne[2];
-                    add_step([=](hipStream_t s) { launch_moe_sum(a, s, ncu); }, t, "slot_sum");
+                    add_step([=](hipStream_t s) { launch_moe_sum(a, s); }, t, "slot_sum");
                     break;
                 }
                 plan_binary(t);

@@ -448,9 +448,8 @@ struct moe_sum_args {
     int64_t w_nb1, w_nb2;
     float * out;
     int64_t M, used, tokens;
-    bool vec;  // set by the launcher
 };
-void launch_moe_sum(const moe_sum_args & a, hipStream_t s, int n_cu);
+void launch_moe_sum(const moe_sum_args & a, hipStream_t s);
 
 // GGML_OP_ARGSORT: the indices that sort each row, equal elements in their
 // order, NaN the largest; GGML_OP_SUM_ROWS
