@@ -252,8 +252,8 @@ __global__ __launch_bounds__(256) void k_moe_few(mul_mat_id_args a) {
 // rounded values of F16 weights, the whole numbers of the quantized blocks
 // otherwise (with their scales beside them). k_moe_gemm takes 128 weight rows (PAIR: 64
 // of each matrix) by BN columns of one expert, K in steps of 64 through two
-// LDS buffers (16-byte pieces swizzled by row), the next step's loads in
-// flight under the current one's products.
+// LDS buffers (16-byte pieces swizzled by row), the loads of two steps in
+// flight.
 //
 // Quantized weights are staged as the whole numbers of their blocks too:
 // a block's sum of 32 products is exact on the f16 matrix cores, and a block
@@ -266,7 +266,8 @@ constexpr int kMoeRows = 128;
 struct moe_wide_args {
     mul_mat_id_args a;
     int * head;     // [0]: the number of tiles
-    int4 * tiles;   // expert (-1: none), first place, columns
+    int4 * tiles;   // expert (-1: none), first place, columns, the expert's first tile
+    int * runs;     // by tile: the tiles of its expert
     int * sorted;   // place -> pair
     _Float16 * x;   // [b column][Kp]
     float * xd;     // quantized: the blocks' scales, [b column][Kp / 32 or Kp / 256]
@@ -332,8 +333,10 @@ __device__ __forceinline__ void moe_route(const moe_wide_args & q) {
         if (b < bins) {
             int at = before + sum - total;
             const int t0 = tbefore + tsum - nt;
-            for (int t = 0; t < nt; t++)
-                q.tiles[t0 + t] = make_int4(b < a.experts ? b : -1, at + t * q.bn, min(q.bn, total - t * q.bn), 0);
+            for (int t = 0; t < nt; t++) {
+                q.tiles[t0 + t] = make_int4(b < a.experts ? b : -1, at + t * q.bn, min(q.bn, total - t * q.bn), t0);
+                q.runs[t0 + t] = nt;
+            }
             for (int w = 0; w < 16; w++) {  // the waves' first places
                 const int c = s_hist[w * bins + b];
                 s_hist[w * bins + b] = at;
@@ -442,7 +445,7 @@ struct moe_x {
 template <int XP>
 __device__ __forceinline__ void moe_x_load(moe_x<XP> & x, const _Float16 * base, const uint32_t (&at)[XP]) {
 #pragma unroll
-    for (int u = 0; u < XP; u++) x.v[u] = *(const moe_u4 *) (base + at[u]);
+    for (int u = 0; u < XP; u++) x.v[u] = *(const moe_u4 *) ((const char *) base + at[u]);
 }
 template <int XP>
 __device__ __forceinline__ void moe_x_store(const moe_x<XP> & x, _Float16 (*s)[kMoeK]) {
@@ -470,12 +473,17 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
     const mul_mat_id_args & a = q.a;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave & 1, wc = wave >> 1;
-    // contiguous runs of tiles an XCD (workgroup i on XCD i % 8), row tiles of a column tile in turn
-    const int64_t total = q.head[0] * q.row_tiles, per = (total + 7) / 8;
-    const int64_t id = blockIdx.x, t = id % 8 * per + id / 8;
-    if (id / 8 >= per || t >= total) return;
-    const int4 tile = q.tiles[t / q.row_tiles];
-    const int64_t m0 = t % q.row_tiles * (PAIR ? 64 : 128);
+    // Contiguous runs of tiles an XCD (workgroup i on XCD i % 8), an expert's
+    // row tiles in turn with its column tiles adjacent: they read the same
+    // weights at the same time, once beyond their XCD's L2. (A column tile's
+    // row tiles in turn: a weight tile came in 1.5 times.)
+    const uint32_t rows = (uint32_t) q.row_tiles, total = (uint32_t) q.head[0] * rows, per = (total + 7) / 8;
+    const uint32_t t = blockIdx.x % 8 * per + blockIdx.x / 8;
+    if (blockIdx.x / 8 >= per || t >= total) return;
+    const int first = q.tiles[t / rows].w;
+    const uint32_t in = t - (uint32_t) first * rows, run = (uint32_t) q.runs[first], rt = in / run;
+    const int4 tile = q.tiles[first + (int) (in - rt * run)];
+    const int64_t m0 = (int64_t) rt * (PAIR ? 64 : 128);
     const int n = tile.z;
     if (tid < BN) {
         const int p = q.sorted[tile.y + min(tid, n - 1)];
@@ -493,11 +501,20 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
     const int srow = tid >> 1, half = tid & 1;
     const int64_t mrow = min(PAIR ? m0 + (srow & 63) : m0 + srow, a.M - 1);
     const char * wrow = (PAIR && srow >= 64 ? a.W2 : a.W) + tile.x * a.W_nb2 + mrow * a.W_nb1;
+    // (F16: pieces t % 8 of the rows t / 8 + 32 u, whole lines a load)
+    const char * wp[WT == GGML_TYPE_F16 ? 4 : 1];
+    if constexpr (WT == GGML_TYPE_F16) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int64_t m = min(m0 + (PAIR ? (tid / 8 + 32 * u) & 63 : tid / 8 + 32 * u), a.M - 1);
+            wp[u] = (PAIR && u >= 2 ? a.W2 : a.W) + tile.x * a.W_nb2 + m * a.W_nb1 + 16 * (tid % 8);
+        }
+    }
     const int64_t steps = (a.K + kMoeK - 1) / kMoeK;
     constexpr int XP = BN * 8 / 256;  // 16-byte pieces of the columns a thread stages
-    uint32_t xat[XP];  // the columns' pieces (places in 32 bits: mul_mat_id_wide)
+    uint32_t xat[XP];  // the columns' pieces (byte offsets in 32 bits: mul_mat_id_wide)
 #pragma unroll
-    for (int u = 0; u < XP; u++) xat[u] = (uint32_t) L.col[(tid + 256 * u) / 8] * (uint32_t) q.kp + 8 * (tid % 8);
+    for (int u = 0; u < XP; u++) xat[u] = 2 * ((uint32_t) L.col[(tid + 256 * u) / 8] * (uint32_t) q.kp + 8 * (tid % 8));
     const int scol = tid % BN, sblk = tid / BN;  // the scale this thread stages (sblk < 2)
     struct stage {
         moe_w<WT> w;
@@ -508,10 +525,12 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
         moe_w<WT> & w = st.w;
         const int64_t k0 = s * kMoeK;
         if constexpr (WT == GGML_TYPE_F16) {
+            if (k0 + kMoeK <= a.K) {
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int64_t k = k0 + 32 * half + 8 * u;
-                w.v[u] = *(const moe_u4 *) (wrow + 2 * (k < a.K ? k : 0));  // past K: masked when stored
+                for (int u = 0; u < 4; u++) w.v[u] = *(const moe_u4 *) (wp[u] + 2 * k0);
+            } else {  // past K: the row's first piece, masked when stored
+#pragma unroll
+                for (int u = 0; u < 4; u++) w.v[u] = *(const moe_u4 *) (wp[u] + (k0 + 8 * (tid % 8) < a.K ? 2 * k0 : -16 * (tid % 8)));
             }
         } else if constexpr (WT == GGML_TYPE_Q8_0) {
             const int64_t b = 2 * s + half;
@@ -537,14 +556,13 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
             }
         }
     };
-    auto store = [&](int64_t s, const stage & st) {
+    auto store = [&](int b, int64_t s, const stage & st) {
         const moe_w<WT> & w = st.w;
-        const int b = (int) (s & 1);
         if constexpr (WT == GGML_TYPE_F16) {
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const uint32_t in = s * kMoeK + 32 * half + 8 * u < a.K ? 0xFFFFFFFFu : 0u;
-                *(moe_u4 *) moe_slot(L.w[b], srow, 4 * half + u) = w.v[u] & in;
+                const uint32_t in = s * kMoeK + 8 * (tid % 8) < a.K ? 0xFFFFFFFFu : 0u;
+                *(moe_u4 *) moe_slot(L.w[b], tid / 8 + 32 * u, tid % 8) = w.v[u] & in;
             }
         } else if constexpr (WT == GGML_TYPE_Q8_0) {
             const uint32_t z = 0x80808080u;
@@ -596,12 +614,7 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
 #pragma unroll
             for (int j = 0; j < NC; j++)
                 xf[j] = __builtin_bit_cast(moe_v8h, *moe_slot(L.x[b], BN / 2 * wc + 16 * j + r, 4 * kk + g));
-            if constexpr (!kQ) {
-#pragma unroll
-                for (int i = 0; i < NR; i++)
-#pragma unroll
-                    for (int j = 0; j < NC; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[j], wf[i], acc[i][j], 0, 0, 0);
-            } else {
+            if constexpr (kQ) {
                 float dw[NR], mw[NR];
 #pragma unroll
                 for (int i = 0; i < NR; i++) {
@@ -627,13 +640,78 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
             }
         }
     };
-    stage st;
-    load(0, st);
-    for (int64_t s = 0; s < steps; s++) {
-        store(s, st);
-        __syncthreads();  // the step is staged; the buffer of the step before is free
-        if (s + 1 < steps) load(s + 1, st);
-        multiply((int) (s & 1));
+    // Two steps in flight: a step's products take a fraction of a load's way.
+    // (The loads past the last step are the last step's again: one that may
+    // not have been made would be waited for with all later ones. Q4_K at 128
+    // columns has the registers for one: a second one spilled 34 of them.)
+    constexpr int kAhead = WT == GGML_TYPE_Q4_K && BN == 128 ? 1 : 2;
+    stage s0, s1;
+    load(0, s0);
+    if constexpr (kAhead == 2) load(min((int64_t) 1, steps - 1), s1);
+    if constexpr (!kQ) {
+        // A half step's operands are read under the products of the one
+        // before: the second half's at the step's start, the next step's first
+        // half's after the barrier in its middle, by which that step is staged.
+        struct half_step {
+            moe_v8h w[NR], x[NC];
+        };
+        auto read = [&](int b, int kk, half_step & f) {
+#pragma unroll
+            for (int j = 0; j < NC; j++)
+                f.x[j] = __builtin_bit_cast(moe_v8h, *moe_slot(L.x[b], BN / 2 * wc + 16 * j + r, 4 * kk + g));
+#pragma unroll
+            for (int i = 0; i < NR; i++)
+                f.w[i] = __builtin_bit_cast(moe_v8h, *moe_slot(L.w[b], tile_row(i) + r, 4 * kk + g));
+        };
+        auto products = [&](const half_step & f) {
+#pragma unroll
+            for (int i = 0; i < NR; i++)
+#pragma unroll
+                for (int j = 0; j < NC; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.x[j], f.w[i], acc[i][j], 0, 0, 0);
+        };
+        half_step f0, f1;
+        store(0, 0, s0);
+        __syncthreads();
+        load(min((int64_t) 2, steps - 1), s0);
+        read(0, 0, f0);
+        // step s of buffer b; `next` holds step s + 1
+        auto step = [&](int64_t s, int b, stage & next) {
+            read(b, 1, f1);
+            store(b ^ 1, min(s + 1, steps - 1), next);
+            products(f0);
+            __syncthreads();
+            load(min(s + 3, steps - 1), next);
+            read(b ^ 1, 0, f0);
+            products(f1);
+        };
+        for (int64_t s = 0;;) {
+            step(s, 0, s1);
+            if (++s >= steps) break;
+            step(s, 1, s0);
+            if (++s >= steps) break;
+        }
+    } else if constexpr (kAhead == 1) {
+        for (int64_t s = 0; s < steps; s++) {
+            const int b = (int) (s & 1);
+            store(b, s, s0);
+            __syncthreads();  // the step is staged; the buffer of the step before is free
+            load(min(s + 1, steps - 1), s0);
+            multiply(b);
+        }
+    } else {
+        for (int64_t s = 0;;) {
+            store(0, s, s0);
+            __syncthreads();  // the step is staged; the buffer of the step before is free
+            load(min(s + 2, steps - 1), s0);
+            multiply(0);
+            if (++s >= steps) break;
+            store(1, s, s1);
+            __syncthreads();
+            load(min(s + 2, steps - 1), s1);
+            multiply(1);
+            if (++s >= steps) break;
+        }
     }
 #pragma unroll
     for (int j = 0; j < NC; j++)
@@ -715,7 +793,7 @@ static bool moe_aligned(int wtype, const mul_mat_id_args & a) {
 
 bool mul_mat_id_wide(int wtype, const mul_mat_id_args & a) {
     return moe_aligned(wtype, a) && a.pairs > kMoeFew && a.experts <= 960 && a.pairs < 1 << 30 &&
-           (a.K + 63) / 64 * 64 * a.b_ne1 * (a.pairs / a.used) < 1ll << 32;
+           (a.K + 63) / 64 * 64 * a.b_ne1 * (a.pairs / a.used) < 1ll << 31;
 }
 
 bool mul_mat_id_pairs(int wtype, const mul_mat_id_args & a) {
@@ -738,6 +816,7 @@ static size_t moe_carve(int wtype, const mul_mat_id_args & a, moe_wide_args & q,
     };
     q.head = (int *) take(256);
     q.tiles = (int4 *) take((size_t) q.max_tiles * 16);
+    q.runs = (int *) take((size_t) q.max_tiles * 4);
     q.sorted = (int *) take((size_t) a.pairs * 4);
     q.x = (_Float16 *) take((size_t) (q.bcols * q.kp) * 2);
     if (wtype == GGML_TYPE_Q8_0) q.xd = (float *) take((size_t) (q.bcols * (q.kp / 32)) * 4);
