@@ -1,6 +1,7 @@
 // k_ssm.hip -- the state-space mixer's operators: GGML_OP_SSM_CONV (the short
 // depthwise causal convolution over the carried and the step's columns) and
 // GGML_OP_SSM_SCAN (the selective scan).
+#include <algorithm>
 #include <type_traits>
 
 #include "../mi355x_common.h"
@@ -10,24 +11,176 @@ namespace mi355x {
 
 // ---------------------------------------------------------------- conv ---
 
-// y[c, t, s] = sum_j w[j, c] sx[t + j, c, s]
-__global__ __launch_bounds__(256) void k_ssm_conv(ssm_conv_args a) {
-    const int64_t n = a.channels * a.tokens * a.seqs;
-    for (int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t) gridDim.x * 256) {
-        const int64_t c = i % a.channels, t = i / a.channels % a.tokens, s = i / (a.channels * a.tokens);
-        const char * row = a.sx + c * a.sx_nb1 + s * a.sx_nb2;
-        const float * w = (const float *) (a.w + c * a.w_nb1);
-        float y = 0.0f;
-        for (int j = 0; j < a.taps; j++) y = fmaf(w[j], *(const float *) (row + (t + j) * a.sx_nb0), y);
-        a.out[i] = y;
+// y[c, t, s] = silu(bias[c] + sum_j w[j, c] col[t + j, c, s]): every column is
+// read once and every result written once, so memory bounds it. (The SILU's
+// exponential is the library's one in doubles, the same bits as the operator
+// on its own.)
+__device__ __forceinline__ float ssm_conv_end(const ssm_conv_args & a, float v, float bias) {
+    if (a.bias) v = v + bias;
+    return a.silu ? v / (1.0f + expf_det(-v)) : v;
+}
+
+// Channels adjacent: a lane takes NC channels and a run of tokens, the window
+// of TAPS - 1 columns in registers, U columns' loads ahead of their products.
+// The lane with a channel's first token alone reads its carried columns, so it
+// may write the ones carried on over them.
+template <int TAPS, int NC, int U>
+__global__ __launch_bounds__(256) void k_ssm_conv_rows(ssm_conv_args a, int run) {
+    const int lane = threadIdx.x & 63;
+    const int64_t cgroups = (a.channels + 64 * NC - 1) / (64 * NC), runs = (a.tokens + run - 1) / run;
+    const int64_t units = cgroups * runs * a.seqs;
+    for (int64_t u = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6); u < units; u += (int64_t) gridDim.x * 4) {
+        const int64_t c = (u % cgroups * 64 + lane) * NC, s = u / (cgroups * runs);
+        const int64_t t0 = u / cgroups % runs * run, t1 = min(t0 + run, a.tokens);
+        if (c >= a.channels) continue;
+        typedef float vec __attribute__((ext_vector_type(NC)));
+        float w[TAPS][NC], bias[NC];
+#pragma unroll
+        for (int e = 0; e < NC; e++) {
+            const float * wc = (const float *) (a.w + (c + e) * a.w_nb1);
+#pragma unroll
+            for (int j = 0; j < TAPS; j++) w[j][e] = wc[j];
+            bias[e] = a.bias ? a.bias[c + e] : 0.0f;
+        }
+        const char * x = a.x + c * a.x_nb1 + s * a.x_nb2;
+        const char * st = a.st + c * a.st_nb1 + s * a.st_nb2;
+        auto column = [&](int64_t i) {  // of x
+            vec v;
+            if constexpr (NC == 1) v[0] = *(const float *) (x + i * a.x_nb0);
+            else v = *(const vec *) (x + i * a.x_nb0);
+            return v;
+        };
+        vec win[TAPS - 1];
+#pragma unroll
+        for (int j = 0; j < TAPS - 1; j++) {
+            const int64_t i = t0 + j;
+            if (i < a.lead) {
+#pragma unroll
+                for (int e = 0; e < NC; e++) win[j][e] = *(const float *) (st + e * a.st_nb1 + i * a.st_nb0);
+            } else win[j] = column(i - a.lead);
+        }
+        const int64_t in = TAPS - 1 - a.lead;  // token t's newest column is x's t + in
+        if (a.carry && t0 == 0) {
+            vec on[TAPS - 1];
+#pragma unroll
+            for (int j = 0; j < TAPS - 1; j++) {
+                const int64_t i = a.tokens + j - (TAPS - 1);
+                if (i >= 0) on[j] = column(i);
+                else
+#pragma unroll
+                    for (int k = 1; k < TAPS - 1; k++)
+                        if (a.tokens + j == k) on[j] = win[k];
+            }
+#pragma unroll
+            for (int j = 0; j < TAPS - 1; j++)
+#pragma unroll
+                for (int e = 0; e < NC; e++)
+                    *(float *) (a.carry + (c + e) * a.c_nb1 + j * a.c_nb0 + s * a.c_nb2) = on[j][e];
+        }
+        float * out = a.out + (s * a.tokens) * a.channels + c;
+        vec next[U];
+#pragma unroll
+        for (int k = 0; k < U; k++) next[k] = column(min(t0 + k, t1 - 1) + in);
+        for (int64_t t = t0; t < t1; t += U) {
+            vec cur[U];
+#pragma unroll
+            for (int k = 0; k < U; k++) cur[k] = next[k];
+            if (U > 1 && t + U < t1) {
+#pragma unroll
+                for (int k = 0; k < U; k++) next[k] = column(min(t + U + k, t1 - 1) + in);
+            }
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                if (U > 1 && t + k >= t1) break;
+                vec y;
+#pragma unroll
+                for (int e = 0; e < NC; e++) {
+                    float v = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < TAPS - 1; j++) v = fmaf(w[j][e], win[j][e], v);
+                    y[e] = ssm_conv_end(a, fmaf(w[TAPS - 1][e], cur[k][e], v), bias[e]);
+                }
+#pragma unroll
+                for (int j = 0; j < TAPS - 2; j++) win[j] = win[j + 1];
+                win[TAPS - 2] = cur[k];
+                if constexpr (NC == 1) out[(t + k) * a.channels] = y[0];
+                else *(vec *) (out + (t + k) * a.channels) = y;
+            }
+            if (U == 1 && t + 1 < t1) next[0] = column(t + 1 + in);
+        }
     }
 }
 
-void launch_ssm_conv(const ssm_conv_args & a, hipStream_t s, int n_cu) {
+// Columns adjacent, one tensor: 64 channels' columns of 64 tokens through LDS,
+// read along the columns and written along the channels, whole lines both
+constexpr int kConvTaps = 33;  // the most of this form
+__global__ __launch_bounds__(256) void k_ssm_conv_cols(ssm_conv_args a) {
+    __shared__ float tile[64][64 + kConvTaps];  // (odd rows: a column's reads on distinct banks)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t cgroups = (a.channels + 63) / 64, tgroups = (a.tokens + 63) / 64, n = cgroups * tgroups * a.seqs;
+    for (int64_t u = blockIdx.x; u < n; u += gridDim.x) {
+        const int64_t t0 = u % tgroups * 64, c0 = u / tgroups % cgroups * 64, s = u / (tgroups * cgroups);
+        const int cols = (int) min((int64_t) 64, a.tokens - t0) + a.taps - 1;
+        for (int r = wave; r < 64; r += 4) {
+            const char * row = a.x + min(c0 + r, a.channels - 1) * a.x_nb1 + s * a.x_nb2 + t0 * a.x_nb0;
+            for (int i = lane; i < cols; i += 64) tile[r][i] = *(const float *) (row + i * a.x_nb0);
+        }
+        __syncthreads();
+        const int64_t c = c0 + lane;
+        if (c < a.channels) {
+            const float * w = (const float *) (a.w + c * a.w_nb1);
+            const float bias = a.bias ? a.bias[c] : 0.0f;
+            const int t1 = cols - (a.taps - 1);
+            for (int t = 16 * wave; t < min(16 * wave + 16, t1); t++) {
+                float v = 0.0f;
+                for (int j = 0; j < a.taps; j++) v = fmaf(w[j], tile[lane][t + j], v);
+                a.out[(s * a.tokens + t0 + t) * a.channels + c] = ssm_conv_end(a, v, bias);
+            }
+        }
+        __syncthreads();  // the tile is read
+    }
+}
+
+// any taps and strides
+__global__ __launch_bounds__(256) void k_ssm_conv_any(ssm_conv_args a) {
+    const int64_t n = a.channels * a.tokens * a.seqs;
+    for (int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t) gridDim.x * 256) {
+        const int64_t c = i % a.channels, t = i / a.channels % a.tokens, s = i / (a.channels * a.tokens);
+        const char * row = a.x + c * a.x_nb1 + s * a.x_nb2;
+        const float * w = (const float *) (a.w + c * a.w_nb1);
+        float y = 0.0f;
+        for (int j = 0; j < a.taps; j++) y = fmaf(w[j], *(const float *) (row + (t + j) * a.x_nb0), y);
+        a.out[i] = ssm_conv_end(a, y, a.bias ? a.bias[c] : 0.0f);
+    }
+}
+
+bool ssm_conv_rows(const ssm_conv_args & a) { return a.taps >= 2 && a.taps <= 4 && (a.x_nb1 == 4 || a.tokens == 1); }
+
+template <int TAPS>
+static void launch_conv_rows(const ssm_conv_args & a, hipStream_t s) {
+    const bool vec = a.channels % 4 == 0 && a.x_nb1 == 4 && a.x_nb0 % 16 == 0 && a.x_nb2 % 16 == 0 &&
+                     (((uintptr_t) a.x | (uintptr_t) a.out) & 15) == 0;
+    const int nc = vec ? 4 : 1, run = 32;
+    const int64_t units = (a.channels + 64 * nc - 1) / (64 * nc) * ((a.tokens + run - 1) / run) * a.seqs;
+    const dim3 grid((unsigned) std::min<int64_t>((units + 3) / 4, 1 << 22));
+    auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(256), 0, s, a, run); };
+    if (a.tokens < 8) vec ? go(k_ssm_conv_rows<TAPS, 4, 1>) : go(k_ssm_conv_rows<TAPS, 1, 1>);
+    else vec ? go(k_ssm_conv_rows<TAPS, 4, 8>) : go(k_ssm_conv_rows<TAPS, 1, 8>);
+}
+
+void launch_ssm_conv(const ssm_conv_args & a, hipStream_t s) {
     const int64_t n = a.channels * a.tokens * a.seqs;
     if (n == 0) return;
-    const int64_t blocks = (n + 255) / 256;
-    hipLaunchKernelGGL(k_ssm_conv, dim3((unsigned) (blocks < 16 * n_cu ? blocks : 16 * n_cu)), dim3(256), 0, s, a);
+    if (ssm_conv_rows(a)) {
+        if (a.taps == 2) launch_conv_rows<2>(a, s);
+        else if (a.taps == 3) launch_conv_rows<3>(a, s);
+        else launch_conv_rows<4>(a, s);
+    } else if (a.x_nb0 == 4 && a.taps <= kConvTaps) {
+        const int64_t tiles = (a.channels + 63) / 64 * ((a.tokens + 63) / 64) * a.seqs;
+        hipLaunchKernelGGL(k_ssm_conv_cols, dim3((unsigned) std::min<int64_t>(tiles, 1 << 22)), dim3(256), 0, s, a);
+    } else {
+        hipLaunchKernelGGL(k_ssm_conv_any, dim3((unsigned) std::min<int64_t>((n + 255) / 256, 1 << 22)), dim3(256), 0, s, a);
+    }
 }
 
 // ---------------------------------------------------------------- scan ---

@@ -530,7 +530,9 @@ struct planner {
     };
     std::unordered_map<const ggml_tensor *, slot_sum> slot_sums;
     void find_slot_sums();
-    void plan_ssm_conv(const ggml_tensor * t);
+    std::vector<const ggml_tensor *> conv_tail(const ggml_tensor * conv, ssm_conv_args & a) const;
+    bool plan_carried_conv(int i, const ggml_tensor * t);
+    bool plan_ssm_conv(int i, const ggml_tensor * t);
     bool plan_ssm_scan(const ggml_tensor * t);
 };
 
@@ -2074,16 +2076,120 @@ void planner::find_slot_sums() {
     }
 }
 
-void planner::plan_ssm_conv(const ggml_tensor * t) {
-    const ggml_tensor *sx = t->src[0], *w = t->src[1];
+// the nodes after an SSM_CONV that its launch can do, in order: ADD of a bias
+// a channel, SILU
+std::vector<const ggml_tensor *> planner::conv_tail(const ggml_tensor * conv, ssm_conv_args & a) const {
+    std::vector<const ggml_tensor *> tail;
+    auto take = [&](const ggml_tensor * from) -> const ggml_tensor * {
+        const ggml_tensor * n = sole_consumer(from, index.at(from) + 1);
+        return n && n->src[0] == from && n->type == GGML_TYPE_F32 && same_shape(n, from) && is_contiguous(n) ? n : nullptr;
+    };
+    const ggml_tensor * n = take(conv);
+    if (n && n->op == GGML_OP_ADD) {
+        const ggml_tensor * b = n->src[1];
+        if (b == conv || b->type != GGML_TYPE_F32 || !is_contiguous(b) || b->ne[0] != conv->ne[0] || b->ne[1] != 1 || b->ne[2] != 1 ||
+            b->ne[3] != 1 || bypass.count(root_of(b)) || !ready_before(b, cur))
+            return tail;
+        a.bias = (const float *) b->data;
+        tail.push_back(n);
+        n = take(n);
+    }
+    if (n && n->op == GGML_OP_UNARY && n->op_params[0] == GGML_UNARY_OP_SILU) {
+        a.silu = 1;
+        tail.push_back(n);
+    }
+    return tail;
+}
+
+// CONCAT (the carried columns, the step's) read only by an SSM_CONV and by
+// the CPY or CONT of its last columns: one launch here reads both tensors, and
+// does the convolution, its bias and SILU, and the columns carried on (over
+// the carried ones, if they are written in place)
+bool planner::plan_carried_conv(int i, const ggml_tensor * t) {
+    if (t->op_params[0] != 0 || t->type != GGML_TYPE_F32 || !is_contiguous(t) || (t->flags & GGML_TENSOR_FLAG_OUTPUT)) return false;
+    const ggml_tensor *conv = nullptr, *last = nullptr;
+    int readers = 0;
+    for (int k = i + 1; k < cg->n_nodes; k++) {
+        const ggml_tensor * n = cg->nodes[k];
+        for (int q = 0; q < GGML_MAX_SRC; q++) {
+            if (n->src[q] != t) continue;
+            readers++;
+            if (n->op == GGML_OP_SSM_CONV && q == 0) conv = n;
+            if (n->op == GGML_OP_VIEW && q == 0) last = n;
+        }
+    }
+    if (!conv || readers != 1 + (last != nullptr) || uses.at(t) != readers || !supports_op(be->dev, conv)) return false;
+    const ggml_tensor * w = conv->src[1];
+    const int64_t C = t->ne[1], S = t->ne[2], lead = t->src[0]->ne[0], T = t->src[1]->ne[0];
+    if (T < 1 || C < 1 || S < 1 || w->ne[0] != lead + 1 || !ready_before(w, i) || bypass.count(root_of(w))) return false;
+    const tview sv = view_of(t->src[0]), xv = view_of(t->src[1]);
     ssm_conv_args a{};
-    a.sx = (const char *) sx->data;
-    a.sx_nb0 = (int64_t) sx->nb[0], a.sx_nb1 = (int64_t) sx->nb[1], a.sx_nb2 = (int64_t) sx->nb[2];
+    a.st = sv.data, a.st_nb0 = sv.nb[0], a.st_nb1 = sv.nb[1], a.st_nb2 = sv.nb[2];
+    a.x = xv.data, a.x_nb0 = xv.nb[0], a.x_nb1 = xv.nb[1], a.x_nb2 = xv.nb[2];
     a.w = (const char *) w->data, a.w_nb1 = (int64_t) w->nb[1];
-    a.out = (float *) t->data;
+    a.channels = C, a.tokens = T, a.seqs = S, a.taps = (int) w->ne[0], a.lead = (int) lead;
+    if (!ssm_conv_rows(a)) return false;
+    const std::vector<const ggml_tensor *> tail = conv_tail(conv, a);
+    const ggml_tensor * z = tail.empty() ? conv : tail.back();
+    a.out = (float *) z->data;
+    hoist h;
+    h.nodes = tail;
+    h.nodes.push_back(conv);
+    h.reads = {span_of(sv, 4), span_of(xv, 4), span_of(w)};
+    for (const ggml_tensor * n : tail)
+        if (n->op == GGML_OP_ADD) h.reads.push_back(span_of(n->src[1]));
+    h.writes = {span_of(z)};
+    const ggml_tensor * carry = nullptr;
+    if (last) {
+        carry = sole_consumer(last, index.at(last) + 1);
+        if (!carry || (carry->op != GGML_OP_CPY && carry->op != GGML_OP_CONT) || carry->src[0] != last || bypass.count(carry) ||
+            carry->type != GGML_TYPE_F32 || last->nb[0] != 4 || last->ne[0] != lead || last->ne[1] != C || last->ne[2] != S ||
+            last->ne[3] != 1 || last->nb[1] != t->nb[1] || last->nb[2] != t->nb[2] ||
+            (const char *) last->data - (const char *) t->data != 4 * T || deferred.count(carry))
+            return false;
+        if (carry->op == GGML_OP_CPY && !ready_before(carry->src[1], i)) return false;
+        if (!same_shape(carry, last) && !is_contiguous(carry)) return false;
+        a.carry = (char *) carry->data;
+        a.c_nb0 = 4, a.c_nb1 = 4 * lead, a.c_nb2 = 4 * lead * C;
+        if (same_shape(carry, last))
+            a.c_nb0 = (int64_t) carry->nb[0], a.c_nb1 = (int64_t) carry->nb[1], a.c_nb2 = (int64_t) carry->nb[2];
+        h.nodes.push_back(carry);
+        h.writes.push_back(span_of(carry));
+        if (a.c_nb0 == a.st_nb0 && a.c_nb1 == a.st_nb1 && a.c_nb2 == a.st_nb2) h.inplace.push_back({carry, t->src[0]});
+    }
+    if (!hoist_ok(i, h)) return false;
+    for (const ggml_tensor * n : h.nodes) deferred[n] = n;
+    add_step([=](hipStream_t s) { launch_ssm_conv(a, s); }, t, "carried_conv",
+             carry ? std::vector<const ggml_tensor *>{z, carry} : std::vector<const ggml_tensor *>{z});
+    return true;
+}
+
+bool planner::plan_ssm_conv(int i, const ggml_tensor * t) {
+    const ggml_tensor *sx = t->src[0], *w = t->src[1];
+    if (overlaps_operand(t)) return fail(t, "SSM_CONV output overlaps its own input");
+    ssm_conv_args a{};
+    a.x = (const char *) sx->data;
+    a.x_nb0 = (int64_t) sx->nb[0], a.x_nb1 = (int64_t) sx->nb[1], a.x_nb2 = (int64_t) sx->nb[2];
+    a.w = (const char *) w->data, a.w_nb1 = (int64_t) w->nb[1];
     a.channels = t->ne[0], a.tokens = t->ne[1], a.seqs = t->ne[2], a.taps = (int) w->ne[0];
-    const int ncu = n_cu;
-    add_step([=](hipStream_t s) { launch_ssm_conv(a, s, ncu); }, t, "ssm_conv");
+    ssm_conv_args f = a;
+    const std::vector<const ggml_tensor *> tail = conv_tail(t, f);
+    const ggml_tensor * z = t;
+    if (!tail.empty()) {
+        hoist h;
+        h.nodes = tail;
+        h.reads = {span_of(sx), span_of(w)};
+        if (f.bias) h.reads.push_back(span_of(tail[0]->src[1]));
+        h.writes = {span_of(tail.back())};
+        if (hoist_ok(i, h)) {
+            for (const ggml_tensor * n : tail) deferred[n] = n;
+            a = f;
+            z = tail.back();
+        }
+    }
+    a.out = (float *) z->data;
+    add_step([=](hipStream_t s) { launch_ssm_conv(a, s); }, t, "ssm_conv", {z});
+    return true;
 }
 
 bool planner::plan_ssm_scan(const ggml_tensor * t) {
@@ -2226,6 +2332,7 @@ bool planner::plan() {
                 break;
             }
             case GGML_OP_CONCAT: {
+                if (plan_carried_conv(i, t)) break;
                 const tview dv = make_view(t), av = view_of(t->src[0]), bv = view_of(t->src[1]);
                 const int dim = t->op_params[0], es = t->type == GGML_TYPE_F16 ? 2 : 4;
                 add_step([=](hipStream_t s) { launch_concat(dv, av, bv, dim, es, s, ncu); }, t, "concat");
@@ -2393,7 +2500,7 @@ bool planner::plan() {
                 break;
             }
             case GGML_OP_SSM_CONV:
-                plan_ssm_conv(t);
+                if (!plan_ssm_conv(i, t)) return false;
                 break;
             case GGML_OP_SSM_SCAN:
                 if (!plan_ssm_scan(t)) return false;

@@ -385,18 +385,25 @@ struct im2col_args {
 void launch_im2col(void * dst, int dst_f16, const char * src, const im2col_args & a, hipStream_t s);
 bool norm_supported(int64_t ne0);
 
-// GGML_OP_SSM_CONV: sx [taps - 1 + tokens, channels, seqs] f32 (byte strides),
-// w [taps, channels] (taps contiguous) -> out [channels, tokens, seqs]
+// GGML_OP_SSM_CONV: channel c's columns are the `lead` of st (the carried
+// ones, or none), then those of x, element strides in bytes [column, channel,
+// sequence]; w [taps, channels] (taps contiguous), y = conv (+ bias[c]), then
+// SILU if asked -> out [channels, tokens, seqs]. `carry` (lead == taps - 1,
+// may be st itself) takes each channel's last taps - 1 columns.
 struct ssm_conv_args {
-    const char * sx;
-    int64_t sx_nb0, sx_nb1, sx_nb2;
+    const char *st, *x;
+    int64_t st_nb0, st_nb1, st_nb2, x_nb0, x_nb1, x_nb2;
     const char * w;
     int64_t w_nb1;
+    const float * bias;
+    char * carry;
+    int64_t c_nb0, c_nb1, c_nb2;
     float * out;
     int64_t channels, tokens, seqs;
-    int taps;
+    int taps, lead, silu;
 };
-void launch_ssm_conv(const ssm_conv_args & a, hipStream_t s, int n_cu);
+bool ssm_conv_rows(const ssm_conv_args & a);  // the form that takes st and carry: adjacent channels, 2 .. 4 taps
+void launch_ssm_conv(const ssm_conv_args & a, hipStream_t s);
 
 // GGML_OP_SSM_SCAN: states s [n, dim, heads] a slot (contiguous, s_nb3 bytes
 // apart), x [dim, heads, tokens, seqs], dt [heads, tokens, seqs], B and C [n,

@@ -120,6 +120,85 @@ def test_mixer_convolution(ggml, gpu, C, taps, T, S, bias, inplace):
     G.free()
 
 
+@pytest.mark.parametrize("C,taps,T,S", [(64, 4, 1, 1), (100, 4, 70, 2), (61, 3, 33, 1), (128, 2, 8, 3), (40, 6, 20, 1),
+                                        (256, 40, 70, 1)])
+@pytest.mark.parametrize("silu", [False, True])
+def test_conv_of_adjacent_channels(ggml, gpu, C, taps, T, S, silu):
+    """the columns as a transposed tensor: channels adjacent in memory"""
+    print(f"adjacent channels C={C} taps={taps} T={T} S={S} silu={silu}", flush=True)
+    rng = np.random.default_rng(C + T)
+    sx = rng.standard_normal((S, taps - 1 + T, C)).astype(np.float32)
+    w = rng.standard_normal((C, taps)).astype(np.float32)
+    G = ggml.Graph(64, 64)
+    X, W = G.new(ggml.F32, C, taps - 1 + T, S), G.new(ggml.F32, taps, C)
+    y = G.lib.ggml_ssm_conv(G.ctx, G.lib.ggml_transpose(G.ctx, X), W)
+    if silu:
+        y = G.lib.ggml_silu(G.ctx, y)
+    G.build(y)
+    G.allocate(gpu.buft)
+    G.set(X, sx)
+    G.set(W, w)
+    compute(gpu, G)
+    want, m = conv64(sx.transpose(0, 2, 1).astype(np.float64), w.astype(np.float64))
+    bound = taps * U * m
+    if silu:
+        want = want / (1 + np.exp(-want))
+        bound = 1.1 * bound + 4 * U * np.abs(want) + 1e-37
+    within(G.get(y).reshape(S, T, C), want, bound)
+    G.free()
+
+
+@pytest.mark.parametrize("case", ["carried first", "columns read too", "bias is an output", "two carried", "x over its cache"])
+def test_mixer_convolution_variants(ggml, gpu, case):
+    """orders and readers with which the sequence may not, or may only partly,
+    run as one launch: the results are the same"""
+    print(f"mixer conv: {case}", flush=True)
+    C, taps, T, S = 96, 4, 21, 2
+    rng = np.random.default_rng(7)
+    x = rng.standard_normal((S, T, C)).astype(np.float32)
+    st = rng.standard_normal((S, C, taps - 1)).astype(np.float32)
+    w, b = rng.standard_normal((C, taps)).astype(np.float32), rng.standard_normal(C).astype(np.float32)
+    G = ggml.Graph(64, 64)
+    L, ctx = G.lib, G.ctx
+    W, B = G.new(ggml.F32, taps, C), G.new(ggml.F32, C)
+    X = G.new(ggml.F32, C, T, S, weight=True)
+    ST = G.new(ggml.F32, taps - 1, C, S, weight=True)
+    cols = L.ggml_concat(ctx, ST, L.ggml_transpose(ctx, X), 0)
+    conv = L.ggml_ssm_conv(ctx, cols, W)
+    pre = L.ggml_add(ctx, conv, B)
+    y = L.ggml_silu(ctx, pre)
+    row = 4 * (taps - 1 + T)
+    carried = L.ggml_cpy(ctx, L.ggml_view_3d(ctx, cols, taps - 1, C, S, row, row * C, 4 * T), ST)
+    outs = {"carried first": [carried, y], "columns read too": [y, carried, L.ggml_scale(ctx, cols, 2.0)],
+            "bias is an output": [pre, y, carried],
+            "two carried": [y, carried, L.ggml_cont(ctx, L.ggml_view_3d(ctx, cols, taps - 1, C, S, row, row * C, 0))],
+            # y's copy over x, which the sequence's launch would still be reading
+            "x over its cache": [carried, L.ggml_cpy(ctx, y, X)]}[case]
+    G.build(*outs)
+    G.allocate(gpu.buft)
+    for t, v in ((X, x), (ST, st), (W, w), (B, b)):
+        G.set(t, v)
+    for _ in range(3):
+        assert G.compute(gpu.backend) == 0
+        joined = np.concatenate([st, x.transpose(0, 2, 1)], 2)
+        want, m = conv64(joined.astype(np.float64), w.astype(np.float64))
+        want, m = want + b, m + np.abs(b)
+        if case == "bias is an output":
+            within(G.get(pre).reshape(S, T, C), want, (taps + 1) * U * m, "pre")
+        want = want / (1 + np.exp(-want))
+        got = G.get(X if case == "x over its cache" else y).reshape(S, T, C)
+        within(got, want, 1.1 * (taps + 1) * U * m + 4 * U * np.abs(want) + 1e-37, "y")
+        if case == "columns read too":
+            assert np.array_equal(G.get(outs[2]).reshape(joined.shape), 2 * joined)
+        if case == "two carried":
+            assert np.array_equal(G.get(outs[2]).reshape(st.shape), st)
+        if case == "x over its cache":
+            x = got
+        st = joined[:, :, T:]
+        assert np.array_equal(G.get(ST).reshape(st.shape), st)
+    G.free()
+
+
 # ---------------------------------------------------------------- scan ---
 
 def scan64(s, x, dt, A, B, C, ids):
