@@ -188,6 +188,8 @@ void launch_ssm_conv(const ssm_conv_args & a, hipStream_t s) {
 
 // ---------------------------------------------------------------- scan ---
 
+typedef float ssm_v4f __attribute__((ext_vector_type(4)));
+
 // softplus as the op defines it: the identity past 20
 __device__ __forceinline__ float ssm_softplus(float v) { return v <= 20.0f ? log1pf(expf(v)) : v; }
 
@@ -234,6 +236,202 @@ __global__ __launch_bounds__(256) void k_ssm_scan_rows(ssm_scan_args a) {
     }
 }
 
+// The same with 16-byte pieces: W lanes hold a row's state, four elements a
+// lane, and a wave 64 U / W rows of one head at once. One token reads and
+// writes every state once, which bounds it: all rows' loads are in flight
+// together, beside the token's operands.
+template <int W, int U>
+__global__ __launch_bounds__(256) void k_ssm_scan_pieces(ssm_scan_args a) {
+    constexpr int kRows = 64 / W;  // of one load
+    const int lane = threadIdx.x & 63, sub = lane / W, k = lane % W * 4;
+    const uint32_t pblocks = (uint32_t) ((a.dim + kRows * U - 1) / (kRows * U));
+    const int64_t unit = (int64_t) blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (unit >= (int64_t) pblocks * a.heads * a.seqs) return;
+    const int p0 = (int) (unit % pblocks) * kRows * U + sub, h = (int) (unit / pblocks % a.heads);
+    const int s = (int) (unit / ((int64_t) pblocks * a.heads)), g = h / (a.heads / a.groups);
+    const bool in = k < a.n;
+    const int kc = in ? k : 0;
+    const int64_t slot = a.ids[s];
+    const bool has = slot >= 0 && slot < a.slots;
+    const int64_t row0 = (int64_t) h * a.dim;
+    const float * s0 = (const float *) (a.s + (has ? slot : 0) * a.s_nb3) + kc;
+    struct token {
+        float dt, x[U];
+        ssm_v4f b, c;
+    };
+    auto load = [&](int64_t t, token & v) {
+        v.dt = *(const float *) (a.dt + 4 * h + t * a.dt_nb1 + s * a.dt_nb2);
+        v.b = *(const ssm_v4f *) (a.B + 4 * kc + g * a.B_nb1 + t * a.B_nb2 + s * a.B_nb3);
+        v.c = *(const ssm_v4f *) (a.C + 4 * kc + g * a.C_nb1 + t * a.C_nb2 + s * a.C_nb3);
+        const char * x = a.x + h * a.x_nb1 + t * a.x_nb2 + s * a.x_nb3;
+#pragma unroll
+        for (int u = 0; u < U; u++) v.x[u] = *(const float *) (x + 4 * min(p0 + kRows * u, a.dim - 1));
+    };
+    ssm_v4f st[U];
+    if (a.slots > 0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) st[u] = *(const ssm_v4f *) (s0 + (row0 + min(p0 + kRows * u, a.dim - 1)) * a.n);
+    }
+    float av[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) av[e] = *(const float *) (a.A + h * a.A_nb1 + (a.a_elem ? 4 * (kc + e) : 0));
+    token next;
+    if (a.tokens > 0) load(0, next);
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if (!has || !in) st[u] = ssm_v4f{0, 0, 0, 0};
+    for (int64_t t = 0; t < a.tokens; t++) {
+        token v = next;
+        if (t + 1 < a.tokens) load(t + 1, next);
+        const float dt = ssm_softplus(v.dt);
+        float d[4];
+        d[0] = expf(dt * av[0]);
+#pragma unroll
+        for (int e = 1; e < 4; e++) d[e] = a.a_elem ? expf(dt * av[e]) : d[0];
+        if (!in) v.b = v.c = ssm_v4f{0, 0, 0, 0};
+        float y[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const float xv = v.x[u] * dt;
+            y[u] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                st[u][e] = fmaf(st[u][e], d[e], in ? xv * v.b[e] : 0.0f);
+                y[u] = fmaf(st[u][e], v.c[e], y[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            y[u] = group_sum<W>(y[u]);
+            if (k == 0 && p0 + kRows * u < a.dim) a.y[(s * a.tokens + t) * a.heads * a.dim + row0 + p0 + kRows * u] = y[u];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if (in && p0 + kRows * u < a.dim)
+            *(ssm_v4f *) (a.out + ((int64_t) s * a.heads * a.dim + row0 + p0 + kRows * u) * a.n + k) = st[u];
+}
+
+// Short states (n <= 16): a lane a row, its state in registers, B and C of the
+// wave's group in scalar registers, no sums across lanes. An exponential a
+// state and token bounds it, so the tokens are cut into segments until there
+// are waves enough: the first pass (OUT false) makes each segment's own state
+// from zeros and its sum of steps D, and the second starts from the earlier
+// segments' states, each decayed by exp(A D) as a whole.
+struct ssm_lane_args {
+    ssm_scan_args a;
+    float * part;  // [segment][n states, D][row of (sequence, head, channel)]
+    int segs;
+    int64_t seg_tokens, blocks;  // blocks: of 64 rows, a group
+};
+constexpr int kSsmLane = 16;
+
+template <bool FULL, bool OUT>
+__global__ __launch_bounds__(256) void k_ssm_scan_lanes(ssm_lane_args q) {
+    const ssm_scan_args & a = q.a;
+    constexpr int N = kSsmLane;
+    constexpr float kLog2 = 1.44269504088896340736f;
+    typedef const __attribute__((address_space(4))) float * scalar_ptr;  // read-only here: scalar loads
+    const int lane = threadIdx.x & 63, n = FULL ? N : a.n;
+    const int64_t w = (int64_t) blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t units = q.blocks * a.groups * a.seqs;
+    const int seg = (int) (w / units);
+    if (seg >= q.segs - (OUT ? 0 : 1)) return;
+    const int64_t unit = w % units;
+    const int g = (int) (unit / q.blocks % a.groups), s = (int) (unit / (q.blocks * a.groups));
+    const int64_t per = (int64_t) a.heads / a.groups * a.dim, in = unit % q.blocks * 64 + lane;
+    const bool mine = in < per;
+    const int64_t row = g * per + (mine ? in : per - 1), all = (int64_t) a.seqs * a.heads * a.dim, at = s * per * a.groups + row;
+    const int64_t h = row / a.dim, p = row % a.dim;
+    float A[N], st[N], low = 0.0f;  // A log2(e); low: the least of them
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        A[k] = FULL || k < n ? kLog2 * *(const float *) (a.A + h * a.A_nb1 + (a.a_elem ? 4 * k : 0)) : 0.0f;
+        low = fminf(low, A[k]);
+        st[k] = 0.0f;
+    }
+    if constexpr (OUT) {
+        const int64_t slot = a.ids[s];
+        if (slot >= 0 && slot < a.slots) {
+            const float * s0 = (const float *) (a.s + slot * a.s_nb3) + row * n;
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                if (FULL || k < n) st[k] = s0[k];
+        }
+        for (int j = 0; j < seg; j++) {
+            const float * part = q.part + (int64_t) j * (n + 1) * all + at;
+            const float D = part[n * all];
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                if (!FULL && k >= n) break;
+                // 2^z in two parts: neither over- nor underflows before the product does
+                const float z = fminf(fmaxf(A[k] * D, -1000.0f), 1000.0f), zi = rintf(z);
+                st[k] = ldexpf(st[k] * exp2f(z - zi), (int) zi) + part[k * all];
+            }
+        }
+    }
+    const int64_t t0 = seg * q.seg_tokens, t1 = min(t0 + q.seg_tokens, a.tokens);
+    const char * dtp = a.dt + 4 * h + s * a.dt_nb2;
+    const char * xp = a.x + 4 * p + h * a.x_nb1 + s * a.x_nb3;
+    const char *bp = a.B + g * a.B_nb1 + s * a.B_nb3, *cp = a.C + g * a.C_nb1 + s * a.C_nb3;
+    constexpr int U = 4;  // tokens whose dt and x are loaded ahead
+    float dtn[U], xn[U];
+    auto load = [&](int64_t t) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t i = min(t + u, t1 - 1);
+            dtn[u] = *(const float *) (dtp + i * a.dt_nb1);
+            xn[u] = *(const float *) (xp + i * a.x_nb2);
+        }
+    };
+    double D = 0.0;
+    if (t0 < t1) load(t0);
+    for (int64_t t = t0; t < t1; t += U) {
+        float dts[U], xs[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) dts[u] = dtn[u], xs[u] = xn[u];
+        if (t + U < t1) load(t + U);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (t + u >= t1) break;
+            const scalar_ptr B = (scalar_ptr) (uintptr_t) (bp + (t + u) * a.B_nb2), C = (scalar_ptr) (uintptr_t) (cp + (t + u) * a.C_nb2);
+            const float dt = ssm_softplus(dts[u]), xv = xs[u] * dt;
+            if constexpr (!OUT) D += (double) dt;
+            float y = 0.0f;
+            if (__any(dt * low < -126.0f)) {  // decays below the instruction's range
+#pragma unroll
+                for (int k = 0; k < N; k++) {
+                    if (!FULL && k >= n) break;
+                    st[k] = fmaf(st[k], exp2f(dt * A[k]), xv * B[k]);
+                    if constexpr (OUT) y = fmaf(st[k], C[k], y);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < N; k++) {
+                    if (!FULL && k >= n) break;
+                    st[k] = fmaf(st[k], __builtin_amdgcn_exp2f(dt * A[k]), xv * B[k]);
+                    if constexpr (OUT) y = fmaf(st[k], C[k], y);
+                }
+            }
+            if constexpr (OUT)
+                if (mine) a.y[(s * a.tokens + t + u) * a.heads * a.dim + row] = y;
+        }
+    }
+    if (!mine) return;
+    if constexpr (!OUT) {
+        float * part = q.part + (int64_t) seg * (n + 1) * all + at;
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            if (FULL || k < n) part[k * all] = st[k];
+        part[n * all] = (float) D;
+    } else if (seg == q.segs - 1) {
+        float * o = a.out + at * n;
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            if (FULL || k < n) o[k] = st[k];
+    }
+}
+
 // ------------------------------------------------- scan, a decay a head ---
 //
 // Chunks of 64 tokens as matrix products. With c_t the sum of the log decays
@@ -266,7 +464,6 @@ __global__ __launch_bounds__(256) void k_ssm_scan_rows(ssm_scan_args a) {
 // and one whose decays leave the exact range, runs token by token
 // (ssm_chunk_slow), where a value reaches what the recurrence takes it to.
 
-typedef float ssm_v4f __attribute__((ext_vector_type(4)));
 typedef float ssm_v2f __attribute__((ext_vector_type(2)));
 typedef _Float16 ssm_v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 ssm_v4h __attribute__((ext_vector_type(4)));
@@ -1033,11 +1230,50 @@ static size_t ssm_carve(ssm_chunk_args & q, char * base) {
     return at;
 }
 
+// segments of the short states' form: about two waves a SIMD, of 16 tokens or
+// more (the earlier segments' states are read for each)
+static bool ssm_lanes(const ssm_scan_args & a) { return a.n <= kSsmLane; }
+static void ssm_lane_segments(const ssm_scan_args & a, int n_cu, ssm_lane_args & q) {
+    q.a = a;
+    q.blocks = ((int64_t) a.heads / a.groups * a.dim + 63) / 64;
+    const int64_t units = q.blocks * a.groups * a.seqs;
+    const int64_t segs = std::max<int64_t>(1, std::min<int64_t>({8 * n_cu / units, a.tokens / 16, 32}));
+    q.seg_tokens = (a.tokens + segs - 1) / segs;
+    q.segs = q.seg_tokens ? (int) ((a.tokens + q.seg_tokens - 1) / q.seg_tokens) : 1;
+}
+
 size_t ssm_scan_scratch_bytes(const ssm_scan_args & a, int n_cu) {
-    if (!ssm_chunked(a)) return 0;
-    ssm_chunk_args q{};
-    ssm_segments(a, n_cu, q);
-    return ssm_carve(q, nullptr);
+    if (a.seqs == 0) return 0;
+    if (ssm_chunked(a)) {
+        ssm_chunk_args q{};
+        ssm_segments(a, n_cu, q);
+        return ssm_carve(q, nullptr);
+    }
+    if (!ssm_lanes(a)) return 0;
+    ssm_lane_args q{};
+    ssm_lane_segments(a, n_cu, q);
+    return (size_t) (q.segs - 1) * (a.n + 1) * 4 * a.seqs * a.heads * a.dim;
+}
+
+static void launch_ssm_lanes(const ssm_scan_args & a, void * scratch, hipStream_t s, int n_cu) {
+    ssm_lane_args q{};
+    ssm_lane_segments(a, n_cu, q);
+    q.part = (float *) scratch;
+    const int64_t units = q.blocks * a.groups * a.seqs;
+    auto go = [&](auto k, int64_t segs) {
+        hipLaunchKernelGGL(k, dim3((unsigned) ((units * segs + 3) / 4)), dim3(256), 0, s, q);
+    };
+    const bool full = a.n == kSsmLane;
+    if (q.segs > 1) full ? go(k_ssm_scan_lanes<true, false>, q.segs - 1) : go(k_ssm_scan_lanes<false, false>, q.segs - 1);
+    full ? go(k_ssm_scan_lanes<true, true>, q.segs) : go(k_ssm_scan_lanes<false, true>, q.segs);
+}
+
+// whole 16-byte pieces of the states and the streams
+static bool ssm_pieces(const ssm_scan_args & a) {
+    const uintptr_t at = (uintptr_t) a.s | (uintptr_t) a.s_nb3 | (uintptr_t) a.B | (uintptr_t) a.C | (uintptr_t) a.out |
+                         (uintptr_t) a.B_nb1 | (uintptr_t) a.B_nb2 | (uintptr_t) a.B_nb3 | (uintptr_t) a.C_nb1 |
+                         (uintptr_t) a.C_nb2 | (uintptr_t) a.C_nb3;
+    return a.n % 4 == 0 && (at & 15) == 0;
 }
 
 static void launch_ssm_chunks(const ssm_scan_args & a, void * scratch, hipStream_t s, int n_cu) {
@@ -1064,11 +1300,21 @@ void launch_ssm_scan(const ssm_scan_args & a, void * scratch, hipStream_t s, int
     const int64_t rows = (int64_t) a.seqs * a.heads * a.dim;
     if (rows == 0) return;
     if (ssm_chunked(a)) return launch_ssm_chunks(a, scratch, s, n_cu);
+    if (ssm_lanes(a)) return launch_ssm_lanes(a, scratch, s, n_cu);
+    if (ssm_pieces(a)) {
+        auto go = [&](auto kernel, int per) {  // rows of a head a wave
+            const int64_t waves = (a.dim + per - 1) / per * (int64_t) a.heads * a.seqs;
+            hipLaunchKernelGGL(kernel, dim3((unsigned) ((waves + 3) / 4)), dim3(256), 0, s, a);
+        };
+        if (a.n <= 64) go(k_ssm_scan_pieces<16, 4>, 16);
+        else if (a.n <= 128) go(k_ssm_scan_pieces<32, 8>, 16);
+        else go(k_ssm_scan_pieces<64, 8>, 8);
+        return;
+    }
     auto go = [&](auto kernel, int w) {
         hipLaunchKernelGGL(kernel, dim3((unsigned) ((rows * w + 255) / 256)), dim3(256), 0, s, a);
     };
-    if (a.n <= 16) go(k_ssm_scan_rows<16, 1>, 16);
-    else if (a.n <= 64) go(k_ssm_scan_rows<64, 1>, 64);
+    if (a.n <= 64) go(k_ssm_scan_rows<64, 1>, 64);
     else if (a.n <= 128) go(k_ssm_scan_rows<64, 2>, 64);
     else go(k_ssm_scan_rows<64, 4>, 64);
 }

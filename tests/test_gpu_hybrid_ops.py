@@ -328,6 +328,57 @@ def test_ssm_scan_keeps_non_finite_values_where_they_are(ggml, gpu, T, what):
         within(got[fine], want[fine], bound[fine] + 1e-30, what)
 
 
+# short states cut into segments of tokens, the last rows of a group alone;
+# states in 16-byte pieces, rows left over
+PIECES = [(1, 1000, 130, 1, 2, 16, True), (2, 150, 33, 3, 1, 5, True), (1, 500, 64, 1, 1, 16, False), (1, 40, 5, 7, 1, 12, False),
+          (3, 97, 1, 1, 1, 1, True), (1, 31, 200, 1, 1, 16, True), (1, 32, 200, 1, 1, 16, True), (40, 64, 300, 1, 3, 16, True),
+          (2, 3, 5, 20, 1, 256, False), (1, 7, 3, 33, 1, 36, False), (1, 5, 2, 64, 1, 128, True), (2, 1, 3, 50, 3, 64, True),
+          (1, 1, 3, 9, 1, 192, False), (1, 40, 3, 12, 1, 24, False), (2, 2, 3, 17, 1, 131, False)]
+
+
+@pytest.mark.parametrize("S,T,H,P,Gr,n,elem", PIECES)
+def test_ssm_scan_segments_and_pieces(ggml, gpu, S, T, H, P, Gr, n, elem):
+    test_ssm_scan(ggml, gpu, S, T, H, P, Gr, n, elem)
+
+
+@pytest.mark.parametrize("T", [1, 70, 530])
+@pytest.mark.parametrize("what", ["x", "dt", "state", "long_dt", "rising", "zeros"])
+def test_ssm_scan_of_short_states_keeps_values_where_they_are(ggml, gpu, T, what):
+    """a NaN or an infinity in one channel, a step that forgets everything,
+    decays above one, states of zero under them"""
+    rng = np.random.default_rng(T)
+    S, H, P, n, at = 2, 70, 1, 16, T // 2
+    s, x, dt, A, B, C = scan_inputs(rng, S, T, H, P, 1, n, True, S)
+    if what == "x":
+        x[0, at, 5] = np.nan
+    elif what == "dt":
+        dt[1, at, 7] = np.nan
+    elif what == "state":
+        s[0, 5, 0, 3] = np.inf
+        dt[0, :, 5] = -4
+        A[5] = -1  # (an infinite state under a decay of zero would be a NaN)
+    elif what == "long_dt":
+        dt[0, at, 1] = 1e9
+    else:
+        A[3], A[4, ::2] = 2.0, 0.0
+        dt[:, :, 3:5] = -3.0  # 2 log1p(e^-3) T: e^51 at most
+        if what == "zeros":
+            s[:] = 0
+            x[:, :, 3] = 0
+            dt[:, :, 3] = 3.0  # without a state: no growth to see
+    y, h = run_scan(ggml, gpu, s, x, dt, A, B, C, range(S))
+    with np.errstate(all="ignore"):
+        wy, by, wh, bh = scan64(s, x, dt, A, B, C, range(S))
+        by, bh = np.nan_to_num(by, nan=0.0, posinf=3e38), np.nan_to_num(bh, nan=0.0, posinf=3e38)
+    if what == "zeros":  # in f64 too, 0 times a decay past its range
+        wy[:, :, 3], wh[:, 3] = 0.0, 0.0
+        by[:, :, 3], bh[:, 3] = 0.0, 0.0
+    for got, want, bound in ((y, wy, by), (h, wh, bh)):
+        fine = np.isfinite(want)
+        assert np.array_equal(np.isfinite(got), fine)
+        within(got[fine], want[fine], bound[fine] + 1e-30, what)
+
+
 @pytest.mark.parametrize("scale", [1e-20, 1e-6, 1e12])
 @pytest.mark.parametrize("T", [2, 130])
 def test_ssm_scan_scales(ggml, gpu, T, scale):
