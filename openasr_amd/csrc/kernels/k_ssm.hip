@@ -190,8 +190,26 @@ void launch_ssm_conv(const ssm_conv_args & a, hipStream_t s) {
 
 typedef float ssm_v4f __attribute__((ext_vector_type(4)));
 
-// softplus as the op defines it: the identity past 20
-__device__ __forceinline__ float ssm_softplus(float v) { return v <= 20.0f ? log1pf(expf(v)) : v; }
+// softplus as the op defines it, the identity past 20: max(v, 0) + log(1 + z),
+// z = exp(-|v|), and log(1 + z) = 2 atanh(s), s = z / (2 + z) <= 1/3, by its
+// series. Within 3.7 half steps of the value (the past-20 cut included: there
+// z is less than v's last place); log1pf(expf(v)) takes three times the
+// instructions.
+__device__ __forceinline__ float ssm_softplus(float v) {
+    const float z = expf(-fabsf(v)), d = 2.0f + z, r = __builtin_amdgcn_rcpf(d);
+    float s = z * r;
+    s = fmaf(fmaf(-s, d, z), r, s);
+    const float w = s * s;
+    float p = 1.0f / 15;
+    p = fmaf(p, w, 1.0f / 13);
+    p = fmaf(p, w, 1.0f / 11);
+    p = fmaf(p, w, 1.0f / 9);
+    p = fmaf(p, w, 1.0f / 7);
+    p = fmaf(p, w, 1.0f / 5);
+    p = fmaf(p, w, 1.0f / 3);
+    const float t = s + s;
+    return fmaxf(v, 0.0f) + fmaf(t, p * w, t);
+}
 
 // token by token: W lanes hold one (sequence, head, channel) row's state, R
 // elements a lane
@@ -343,11 +361,12 @@ __global__ __launch_bounds__(256) void k_ssm_scan_lanes(ssm_lane_args q) {
     const bool mine = in < per;
     const int64_t row = g * per + (mine ? in : per - 1), all = (int64_t) a.seqs * a.heads * a.dim, at = s * per * a.groups + row;
     const int64_t h = row / a.dim, p = row % a.dim;
-    float A[N], st[N], low = 0.0f;  // A log2(e); low: the least of them
+    float A[N], st[N], low = 0.0f, high = 0.0f;  // A log2(e); the least and the largest of them
 #pragma unroll
     for (int k = 0; k < N; k++) {
         A[k] = FULL || k < n ? kLog2 * *(const float *) (a.A + h * a.A_nb1 + (a.a_elem ? 4 * k : 0)) : 0.0f;
         low = fminf(low, A[k]);
+        high = fmaxf(high, A[k]);
         st[k] = 0.0f;
     }
     if constexpr (OUT) {
@@ -358,15 +377,30 @@ __global__ __launch_bounds__(256) void k_ssm_scan_lanes(ssm_lane_args q) {
             for (int k = 0; k < N; k++)
                 if (FULL || k < n) st[k] = s0[k];
         }
-        for (int j = 0; j < seg; j++) {
+        float own[N], D = 0.0f;  // the next segment's own state, a step ahead
+        auto fetch = [&](int j) {
             const float * part = q.part + (int64_t) j * (n + 1) * all + at;
-            const float D = part[n * all];
 #pragma unroll
-            for (int k = 0; k < N; k++) {
-                if (!FULL && k >= n) break;
-                // 2^z in two parts: neither over- nor underflows before the product does
-                const float z = fminf(fmaxf(A[k] * D, -1000.0f), 1000.0f), zi = rintf(z);
-                st[k] = ldexpf(st[k] * exp2f(z - zi), (int) zi) + part[k * all];
+            for (int k = 0; k < N; k++)
+                if (FULL || k < n) own[k] = part[k * all];
+            D = part[n * all];
+        };
+        if (seg > 0) fetch(0);
+        for (int j = 0; j < seg; j++) {
+            float add[N];
+            const float d = D;
+#pragma unroll
+            for (int k = 0; k < N; k++) add[k] = FULL || k < n ? own[k] : 0.0f;
+            fetch(min(j + 1, seg - 1));
+            if (__all(d * low >= -126.0f && d * high <= 0.0f)) {
+#pragma unroll
+                for (int k = 0; k < N; k++) st[k] = fmaf(st[k], __builtin_amdgcn_exp2f(A[k] * d), add[k]);
+            } else {  // 2^z in two parts: neither over- nor underflows before the product does
+#pragma unroll
+                for (int k = 0; k < N; k++) {
+                    const float z = fminf(fmaxf(A[k] * d, -1000.0f), 1000.0f), zi = rintf(z);
+                    st[k] = ldexpf(st[k] * exp2f(z - zi), (int) zi) + add[k];
+                }
             }
         }
     }
@@ -384,34 +418,52 @@ __global__ __launch_bounds__(256) void k_ssm_scan_lanes(ssm_lane_args q) {
             xn[u] = *(const float *) (xp + i * a.x_nb2);
         }
     };
+    // a token's B and C: a step ahead where they are whole
+    float B[N], C[N], Bn[N], Cn[N];
+    auto fetch = [&](int64_t t) {
+        const scalar_ptr b = (scalar_ptr) (uintptr_t) (bp + t * a.B_nb2), c = (scalar_ptr) (uintptr_t) (cp + t * a.C_nb2);
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            if (!FULL && k >= n) break;
+            Bn[k] = b[k];
+            if constexpr (OUT) Cn[k] = c[k];
+        }
+    };
     double D = 0.0;
-    if (t0 < t1) load(t0);
+    if (t0 < t1) {
+        load(t0);
+        fetch(t0);
+    }
     for (int64_t t = t0; t < t1; t += U) {
         float dts[U], xs[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) dts[u] = dtn[u], xs[u] = xn[u];
+        for (int u = 0; u < U; u++) dts[u] = ssm_softplus(dtn[u]), xs[u] = xn[u] * dts[u];
         if (t + U < t1) load(t + U);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (t + u >= t1) break;
-            const scalar_ptr B = (scalar_ptr) (uintptr_t) (bp + (t + u) * a.B_nb2), C = (scalar_ptr) (uintptr_t) (cp + (t + u) * a.C_nb2);
-            const float dt = ssm_softplus(dts[u]), xv = xs[u] * dt;
+            const float dt = dts[u], xv = xs[u];
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                if (!FULL && k >= n) break;
+                B[k] = Bn[k];
+                if constexpr (OUT) C[k] = Cn[k];
+            }
+            fetch(min(t + u + 1, t1 - 1));
+            __builtin_amdgcn_sched_barrier(0);
             if constexpr (!OUT) D += (double) dt;
-            float y = 0.0f;
-            if (__any(dt * low < -126.0f)) {  // decays below the instruction's range
+            float e[N], y = 0.0f;
 #pragma unroll
-                for (int k = 0; k < N; k++) {
-                    if (!FULL && k >= n) break;
-                    st[k] = fmaf(st[k], exp2f(dt * A[k]), xv * B[k]);
-                    if constexpr (OUT) y = fmaf(st[k], C[k], y);
-                }
-            } else {
+            for (int k = 0; k < N; k++) e[k] = __builtin_amdgcn_exp2f(dt * A[k]);
+            if (__any(dt * low < -126.0f)) {  // below the instruction's range
 #pragma unroll
-                for (int k = 0; k < N; k++) {
-                    if (!FULL && k >= n) break;
-                    st[k] = fmaf(st[k], __builtin_amdgcn_exp2f(dt * A[k]), xv * B[k]);
-                    if constexpr (OUT) y = fmaf(st[k], C[k], y);
-                }
+                for (int k = 0; k < N; k++) e[k] = exp2f(dt * A[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                if (!FULL && k >= n) break;
+                st[k] = fmaf(st[k], e[k], xv * B[k]);
+                if constexpr (OUT) y = fmaf(st[k], C[k], y);
             }
             if constexpr (OUT)
                 if (mine) a.y[(s * a.tokens + t + u) * a.heads * a.dim + row] = y;
