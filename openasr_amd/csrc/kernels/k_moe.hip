@@ -883,32 +883,161 @@ __device__ __forceinline__ uint32_t sort_key(float v) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// one wave a row: an element's place is the number of elements before it
-__global__ __launch_bounds__(256) void k_argsort_rank(tview d, tview a, int desc, int64_t rows) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
+// Sorted ascending by (key, index); descending turns the keys' bits.
+// Short rows, a wave each: an element's place is the number of elements
+// before it, all keys against all from LDS.
+constexpr int kArgsortRank = 256;
+__global__ __launch_bounds__(256) void k_argsort_rank(tview d, tview a, uint32_t flip, int64_t rows) {
+    __shared__ __align__(16) uint32_t keys[4][kArgsortRank];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t want = (int64_t) blockIdx.x * 4 + wave, row = min(want, rows - 1);
     const int64_t i1 = row % a.ne[1], i2 = row / a.ne[1] % a.ne[2], i3 = row / (a.ne[1] * a.ne[2]);
     const float * x = (const float *) (a.data + i1 * a.nb[1] + i2 * a.nb[2] + i3 * a.nb[3]);
     int32_t * o = (int32_t *) (d.data + i1 * d.nb[1] + i2 * d.nb[2] + i3 * d.nb[3]);
     const int n = (int) a.ne[0];
-    for (int i = lane; i < n; i += 64) {
-        const uint32_t k = sort_key(x[i]);
-        int at = 0;
-        for (int j = 0; j < n; j++) {
-            const uint32_t q = sort_key(x[j]);
-            at += (desc ? q > k : q < k) || (q == k && j < i);
-        }
-        o[at] = i;
+    constexpr int R = kArgsortRank / 64;
+    uint32_t key[R];
+    int at[R];
+#pragma unroll
+    for (int u = 0; u < R; u++) {
+        const int i = lane + 64 * u;
+        key[u] = i < n ? sort_key(x[i]) ^ flip : 0xFFFFFFFFu;  // (past the row: never before)
+        keys[wave][i] = key[u];
+        at[u] = 0;
     }
+    __syncthreads();
+    for (int j = 0; j < n; j += 4) {
+        const uint4 q4 = *(const uint4 *) &keys[wave][j];
+        const uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int u = 0; u < R; u++) at[u] += q[e] < key[u] || (q[e] == key[u] && j + e < lane + 64 * u);
+    }
+    if (want >= rows) return;
+#pragma unroll
+    for (int u = 0; u < R; u++)
+        if (lane + 64 * u < n) o[at[u]] = lane + 64 * u;
 }
 
-bool argsort_supported(int64_t n) { return n >= 0 && n <= 8192; }
+// longer rows, a workgroup each: a bitonic sort of 64-bit (key, index) in LDS
+constexpr int kArgsortMost = 8192;
+__global__ __launch_bounds__(1024) void k_argsort_bitonic(tview d, tview a, uint32_t flip, int size) {
+    __shared__ uint64_t k[kArgsortMost];
+    const int64_t row = blockIdx.x;
+    const int64_t i1 = row % a.ne[1], i2 = row / a.ne[1] % a.ne[2], i3 = row / (a.ne[1] * a.ne[2]);
+    const float * x = (const float *) (a.data + i1 * a.nb[1] + i2 * a.nb[2] + i3 * a.nb[3]);
+    int32_t * o = (int32_t *) (d.data + i1 * d.nb[1] + i2 * d.nb[2] + i3 * d.nb[3]);
+    const int n = (int) a.ne[0], tid = threadIdx.x;
+    for (int i = tid; i < size; i += 1024) k[i] = i < n ? (uint64_t) (sort_key(x[i]) ^ flip) << 32 | (uint32_t) i : ~0ull;
+    for (int run = 2; run <= size; run *= 2) {
+        for (int step = run / 2; step > 0; step /= 2) {
+            __syncthreads();
+            for (int i = tid; i < size / 2; i += 1024) {
+                const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+                const uint64_t u = k[lo], v = k[hi];
+                if ((u > v) == ((lo & run) == 0)) k[lo] = v, k[hi] = u;
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += 1024) o[i] = (int32_t) (uint32_t) k[i];
+}
+
+bool argsort_supported(int64_t n) { return n >= 0 && n <= kArgsortMost; }
 
 void launch_argsort(const tview & d, const tview & a, int desc, hipStream_t s) {
     const int64_t rows = a.ne[1] * a.ne[2] * a.ne[3];
     if (rows == 0 || a.ne[0] == 0) return;
-    hipLaunchKernelGGL(k_argsort_rank, dim3((unsigned) ((rows + 3) / 4)), dim3(256), 0, s, d, a, desc, rows);
+    const uint32_t flip = desc ? 0xFFFFFFFFu : 0;
+    if (a.ne[0] <= kArgsortRank) {
+        hipLaunchKernelGGL(k_argsort_rank, dim3((unsigned) ((rows + 3) / 4)), dim3(256), 0, s, d, a, flip, rows);
+        return;
+    }
+    int size = 2 * kArgsortRank;
+    while (size < a.ne[0]) size *= 2;
+    hipLaunchKernelGGL(k_argsort_bitonic, dim3((unsigned) rows), dim3(1024), 0, s, d, a, flip, size);
+}
+
+// ------------------------------------------------------------ a router ---
+
+// the largest of the wave's values, by adjacent lanes, rows of 16 and halves
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    auto with = [&](int got) { v = max(v, (uint32_t) got); };
+    with(__builtin_amdgcn_update_dpp(0, (int) v, 0x111, 0xf, 0xf, false));  // row_shr 1, 2, 4, 8
+    with(__builtin_amdgcn_update_dpp(0, (int) v, 0x112, 0xf, 0xf, false));
+    with(__builtin_amdgcn_update_dpp(0, (int) v, 0x114, 0xf, 0xf, false));
+    with(__builtin_amdgcn_update_dpp(0, (int) v, 0x118, 0xf, 0xf, false));
+    with(__builtin_amdgcn_update_dpp(0, (int) v, 0x142, 0xa, 0xf, false));  // row_bcast 15, 31
+    with(__builtin_amdgcn_update_dpp(0, (int) v, 0x143, 0xc, 0xf, false));
+    return (uint32_t) __builtin_amdgcn_readlane((int) v, 63);
+}
+
+// The first k places of a descending ARGSORT and what a router does with
+// them: the k values, their softmax, or their shares of their sum. A wave a
+// row, V adjacent values a lane: k times the largest key left, of the lowest
+// lane that holds it; then lane j has the j-th. The epilogues are SOFT_MAX's
+// and SUM_ROWS' and DIV's operations in their order.
+template <int V>
+__global__ __launch_bounds__(256) void k_top_k(top_k_args a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t) blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (row >= a.rows) return;
+    const float * x = (const float *) (a.x + row * a.x_nb1);
+    uint32_t key[V], most = 0;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const int i = lane * V + v;
+        key[v] = i < a.n ? sort_key(x[i]) : 0;  // (no value has the key 0)
+        most = max(most, key[v]);
+    }
+    int mine = 0;
+    for (int j = 0; j < a.k; j++) {
+        const uint32_t top = wave_max_u32(most);
+        const int from = __ffsll((unsigned long long) __ballot(most == top)) - 1;
+        int at = 0;
+        if (lane == from) {
+            most = 0;
+            bool taken = false;
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                if (!taken && key[v] == top) {
+                    taken = true;
+                    at = v;
+                    key[v] = 0;
+                }
+                most = max(most, key[v]);
+            }
+        }
+        at = __builtin_amdgcn_readlane(at, from);
+        if (lane == j) mine = from * V + at;
+    }
+    if (lane < a.k) *(int32_t *) (a.ids + row * a.ids_nb1 + 4 * lane) = mine;
+    if (!a.out) return;
+    const float w = lane < a.k ? x[mine] : 0.0f;
+    float y = w;
+    if (a.mode == kTopKSoftMax) {
+        const float z = w * a.scale + 0.0f, mx = wave_max(lane < a.k ? z : -INFINITY);
+        const float e = lane < a.k ? expf_det(z - mx) : 0.0f;
+        y = e * (float) (1.0 / wave_sum_d((double) e));
+    } else if (a.mode == kTopKShares) {
+        y = w / (float) wave_sum_d((double) w);
+    }
+    if (lane < a.k) a.out[row * a.k + lane] = y;
+}
+
+bool top_k_supported(int64_t n, int64_t k) { return n >= 1 && n <= 1024 && k >= 1 && k <= 32 && k <= n; }
+
+void launch_top_k(const top_k_args & a, hipStream_t s) {
+    if (a.rows == 0) return;
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned) ((a.rows + 3) / 4)), dim3(256), 0, s, a);
+    };
+    if (a.n <= 64) go(k_top_k<1>);
+    else if (a.n <= 128) go(k_top_k<2>);
+    else if (a.n <= 256) go(k_top_k<4>);
+    else if (a.n <= 512) go(k_top_k<8>);
+    else go(k_top_k<16>);
 }
 
 // one wave a row, the sum held in double

@@ -532,6 +532,7 @@ struct planner {
     void find_slot_sums();
     std::vector<const ggml_tensor *> conv_tail(const ggml_tensor * conv, ssm_conv_args & a) const;
     bool plan_carried_conv(int i, const ggml_tensor * t);
+    bool plan_top_k(int i, const ggml_tensor * t);
     bool plan_ssm_conv(int i, const ggml_tensor * t);
     bool plan_ssm_scan(const ggml_tensor * t);
 };
@@ -2076,6 +2077,80 @@ void planner::find_slot_sums() {
     }
 }
 
+// A descending ARGSORT read only through views of its first k columns (top_k):
+// only those are made; and where GET_ROWS takes the sorted values at them,
+// that, with the SOFT_MAX over the k of a row or their division by their
+// SUM_ROWS
+bool planner::plan_top_k(int i, const ggml_tensor * t) {
+    const ggml_tensor * x = t->src[0];
+    if (t->op_params[0] != GGML_SORT_ORDER_DESC || (t->flags & GGML_TENSOR_FLAG_OUTPUT) || bypass.count(root_of(x)) ||
+        t->ne[2] != 1 || t->ne[3] != 1 || t->ne[1] == 0)
+        return false;
+    int64_t k = 0;
+    int readers = 0;
+    const ggml_tensor * rows = nullptr;  // the GET_ROWS of the values
+    for (int j = i + 1; j < cg->n_nodes; j++) {
+        const ggml_tensor * n = cg->nodes[j];
+        for (int q = 0; q < GGML_MAX_SRC; q++) {
+            if (n->src[q] != t) continue;
+            readers++;
+            if (n->op != GGML_OP_VIEW || q != 0) return false;
+        }
+        if (n->view_src == t) {
+            if (n->data != t->data || n->nb[0] != 4 || n->ne[1] != t->ne[1] || (n->ne[1] > 1 && n->nb[1] != t->nb[1]) || n->ne[2] != 1 ||
+                n->ne[3] != 1)
+                return false;
+            k = std::max(k, n->ne[0]);
+        }
+    }
+    if (readers == 0 || uses.at(t) != readers || !top_k_supported(t->ne[0], k)) return false;
+    top_k_args a{};
+    a.x = (const char *) x->data, a.x_nb1 = (int64_t) x->nb[1], a.rows = t->ne[1];
+    a.ids = (char *) t->data, a.ids_nb1 = (int64_t) t->nb[1];
+    a.n = (int) t->ne[0], a.k = (int) k, a.scale = 1.0f;
+    for (int j = i + 1; j < cg->n_nodes && !rows; j++) {
+        const ggml_tensor * n = cg->nodes[j];
+        if (n->op != GGML_OP_GET_ROWS || n->src[1]->view_src != t || n->src[1]->ne[0] != k) continue;
+        const ggml_tensor * r = n->src[0];
+        if (r->type == GGML_TYPE_F32 && r->data == x->data && root_of(r) == root_of(x) && is_contiguous(r) && is_contiguous(x) &&
+            r->ne[0] == 1 && r->ne[1] == x->ne[0] && r->ne[2] == x->ne[1] && r->ne[3] == 1 && n->type == GGML_TYPE_F32 &&
+            is_contiguous(n) && !deferred.count(n) && !(n->flags & GGML_TENSOR_FLAG_OUTPUT))
+            rows = n;
+    }
+    std::vector<const ggml_tensor *> writes = {t};
+    auto take = [&](std::vector<const ggml_tensor *> nodes, int mode, float scale) {
+        const ggml_tensor * out = nodes.back();
+        hoist h;
+        h.reads = {span_of(x)};
+        h.writes = {span_of(t), span_of(out)};
+        h.nodes = nodes;
+        if (!hoist_ok(i, h)) return false;
+        for (const ggml_tensor * n : nodes) deferred[n] = n;
+        a.out = (float *) out->data;
+        a.mode = mode, a.scale = scale;
+        writes.push_back(out);
+        return true;
+    };
+    bool done = rows == nullptr;
+    const ggml_tensor * r = rows ? sole_consumer(rows, index.at(rows) + 1) : nullptr;
+    if (r && r->op == GGML_OP_RESHAPE && r->ne[0] == k && r->ne[1] == t->ne[1] && !(r->flags & GGML_TENSOR_FLAG_OUTPUT)) {
+        const ggml_tensor *sum = nullptr, *div = nullptr, *soft = sole_consumer(r, index.at(r) + 1);
+        for (int j = index.at(r) + 1; j < cg->n_nodes; j++) {
+            const ggml_tensor * n = cg->nodes[j];
+            if (n->op == GGML_OP_SUM_ROWS && n->src[0] == r && single_use(n)) sum = n;
+            if (n->op == GGML_OP_DIV && n->src[0] == r && sum && n->src[1] == sum) div = n;
+        }
+        if (soft && soft->op == GGML_OP_SOFT_MAX && soft->src[0] == r && !soft->src[1] && !soft->src[2] &&
+            op_f32(soft, 1) == 0.0f && is_contiguous(soft))
+            done = take({rows, soft}, kTopKSoftMax, op_f32(soft, 0));
+        else if (sum && div && uses.at(r) == 2 && same_shape(div, r) && is_contiguous(div) && div->type == GGML_TYPE_F32)
+            done = take({rows, sum, div}, kTopKShares, 1.0f);
+    }
+    if (!done) take({rows}, kTopKValues, 1.0f);
+    add_step([=](hipStream_t s) { launch_top_k(a, s); }, t, "top_k", writes);
+    return true;
+}
+
 // the nodes after an SSM_CONV that its launch can do, in order: ADD of a bias
 // a channel, SILU
 std::vector<const ggml_tensor *> planner::conv_tail(const ggml_tensor * conv, ssm_conv_args & a) const {
@@ -2489,6 +2564,8 @@ bool planner::plan() {
                 if (!plan_mul_mat_id(i, t)) return false;
                 continue;
             case GGML_OP_ARGSORT: {
+                if (overlaps_operand(t)) return fail(t, "ARGSORT output overlaps its own input");
+                if (plan_top_k(i, t)) break;
                 const tview dv = make_view(t), av = make_view(t->src[0]);
                 const int desc = t->op_params[0] == GGML_SORT_ORDER_DESC;
                 add_step([=](hipStream_t s) { launch_argsort(dv, av, desc, s); }, t, "argsort");

@@ -462,6 +462,21 @@ void launch_moe_sum(const moe_sum_args & a, hipStream_t s);
 // order, NaN the largest; GGML_OP_SUM_ROWS
 bool argsort_supported(int64_t n);
 void launch_argsort(const tview & d, const tview & a, int desc, hipStream_t s);
+// the first k places of a descending ARGSORT of x's rows (n f32, x_nb1 bytes
+// apart) into ids (ids_nb1 apart); out (if any) [k, rows] takes their values,
+// the values' softmax (of scale times them), or each over their sum
+enum top_k_mode { kTopKValues, kTopKSoftMax, kTopKShares };
+struct top_k_args {
+    const char * x;
+    int64_t x_nb1, rows;
+    char * ids;
+    int64_t ids_nb1;
+    float * out;
+    float scale;
+    int n, k, mode;
+};
+bool top_k_supported(int64_t n, int64_t k);
+void launch_top_k(const top_k_args & a, hipStream_t s);
 void launch_sum_rows(const tview & d, const tview & a, hipStream_t s);
 // a one-wave kernel that returns after `us` microseconds of device wall clock
 void launch_spin_us(double us, int wall_clock_khz, hipStream_t s);

@@ -719,6 +719,85 @@ def test_router(ggml, gpu, E, k, T, gating):
     G.free()
 
 
+@pytest.mark.parametrize("n,k", [(8, 1), (8, 8), (63, 5), (65, 32), (129, 3), (1000, 32), (1024, 7), (1025, 7), (200, 33)])
+@pytest.mark.parametrize("rows", [1, 6])
+def test_top_k_of_any_values(ggml, gpu, n, k, rows):
+    """equal values, both zeros, NaN (the largest), infinities; a second view of fewer columns"""
+    print(f"top_k n={n} k={k} rows={rows}", flush=True)
+    rng = np.random.default_rng(n)
+    a = (np.round(rng.standard_normal((rows, n)) * 2) / 2).astype(np.float32)
+    a[rng.random(a.shape) < 0.1] = -0.0
+    a[0, n // 2:], a[0, 0] = -np.inf, np.inf
+    a[-1, n // 3] = np.nan
+    a[rows // 2, :] = np.finfo(np.float32).min
+    G = ggml.Graph(64, 64)
+    L, ctx = G.lib, G.ctx
+    X = G.new(ggml.F32, n, rows)
+    ids = L.ggml_top_k(ctx, X, k)
+    fewer = L.ggml_view_2d(ctx, ids, (k + 1) // 2, rows, 4 * n, 0)
+    w = L.ggml_get_rows(ctx, L.ggml_reshape_3d(ctx, X, 1, n, rows), ids)
+    outs = [L.ggml_cont(ctx, ids), L.ggml_cont(ctx, fewer), w]
+    G.build(*outs)
+    G.allocate(gpu.buft)
+    G.set(X, a)
+    compute(gpu, G)
+    want = sorted64(a, 1)[:, :k]
+    assert np.array_equal(G.get(outs[0]).reshape(rows, k), want)
+    assert np.array_equal(G.get(outs[1]).reshape(rows, -1), want[:, :(k + 1) // 2])
+    assert np.array_equal(G.get(w).reshape(rows, k), np.take_along_axis(a, want, 1), equal_nan=True)
+    G.free()
+
+
+@pytest.mark.parametrize("case", ["all places read", "places are an output", "values are an output", "values read twice", "offset view"])
+def test_router_variants(ggml, gpu, case):
+    """readers with which the choice may not, or may only partly, run as one launch"""
+    E, k, T = 64, 6, 11
+    rng = np.random.default_rng(5)
+    a = rng.standard_normal((T, E)).astype(np.float32)
+    G = ggml.Graph(64, 64)
+    L, ctx = G.lib, G.ctx
+    X = G.new(ggml.F32, E, T)
+    order = L.ggml_argsort(ctx, X, 1)
+    at = 2 if case == "offset view" else 0
+    ids = L.ggml_view_2d(ctx, order, k, T, 4 * E, 4 * at)
+    g = L.ggml_get_rows(ctx, L.ggml_reshape_3d(ctx, X, 1, E, T), ids)
+    g2 = L.ggml_reshape_2d(ctx, g, k, T)
+    w = L.ggml_soft_max(ctx, g2)
+    outs = [w, L.ggml_cont(ctx, ids)]
+    if case == "all places read":
+        outs.append(L.ggml_cont(ctx, order))
+    if case == "places are an output":
+        outs.append(order)
+    if case == "values are an output":
+        outs.append(g)
+    if case == "values read twice":
+        outs.append(L.ggml_scale(ctx, g2, 2.0))
+    G.build(*outs)
+    G.allocate(gpu.buft)
+    G.set(X, a)
+    compute(gpu, G)
+    full = sorted64(a, 1)
+    want = full[:, at:at + k]
+    v = np.take_along_axis(a, want, 1)
+    p = np.exp(v.astype(np.float64) - v.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    within(G.get(w).reshape(T, k), p, (8 + k) * U * p)
+    assert np.array_equal(G.get(outs[1]).reshape(T, k), want)
+    if case in ("all places read", "places are an output"):
+        assert np.array_equal(G.get(outs[2]).reshape(T, E), full)
+    if case == "values are an output":
+        assert np.array_equal(G.get(g).reshape(T, k), v)
+    if case == "values read twice":
+        assert np.array_equal(G.get(outs[2]).reshape(T, k), 2 * v)
+    G.free()
+
+
+@pytest.mark.parametrize("n,rows", [(255, 7), (256, 3), (257, 3), (511, 2), (513, 2), (4096, 2), (4097, 1)])
+@pytest.mark.parametrize("desc", [0, 1])
+def test_argsort_lengths(ggml, gpu, n, rows, desc):
+    test_argsort(ggml, gpu, n, rows, desc)
+
+
 # ------------------------------------------------------ memory of others ---
 
 OVER = """
