@@ -442,15 +442,15 @@ struct moe_x {
     moe_u4 v[XP];
 };
 
-template <int XP>
-__device__ __forceinline__ void moe_x_load(moe_x<XP> & x, const _Float16 * base, const uint32_t (&at)[XP]) {
+template <int C, int XP>
+__device__ __forceinline__ void moe_x_load(moe_x<C> & x, const _Float16 * base, const uint32_t (&at)[XP]) {
 #pragma unroll
-    for (int u = 0; u < XP; u++) x.v[u] = *(const moe_u4 *) ((const char *) base + at[u]);
+    for (int u = 0; u < C; u++) x.v[u] = *(const moe_u4 *) ((const char *) base + at[u]);
 }
-template <int XP>
-__device__ __forceinline__ void moe_x_store(const moe_x<XP> & x, _Float16 (*s)[kMoeK]) {
+template <int C>
+__device__ __forceinline__ void moe_x_store(const moe_x<C> & x, _Float16 (*s)[kMoeK], int tid) {
 #pragma unroll
-    for (int u = 0; u < XP; u++) *(moe_u4 *) moe_slot(s, (threadIdx.x + 256 * u) / 8, threadIdx.x % 8) = x.v[u];
+    for (int u = 0; u < C; u++) *(moe_u4 *) moe_slot(s, (tid + 256 * u) / 8, tid % 8) = x.v[u];
 }
 
 template <int BN>
@@ -484,7 +484,7 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
     const uint32_t in = t - (uint32_t) first * rows, run = (uint32_t) q.runs[first], rt = in / run;
     const int4 tile = q.tiles[first + (int) (in - rt * run)];
     const int64_t m0 = (int64_t) rt * (PAIR ? 64 : 128);
-    const int n = tile.z;
+    const int n = __builtin_amdgcn_readfirstlane(tile.z);
     if (tid < BN) {
         const int p = q.sorted[tile.y + min(tid, n - 1)];
         L.pair[tid] = p;
@@ -511,91 +511,12 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
         }
     }
     const int64_t steps = (a.K + kMoeK - 1) / kMoeK;
-    constexpr int XP = BN * 8 / 256;  // 16-byte pieces of the columns a thread stages
-    uint32_t xat[XP];  // the columns' pieces (byte offsets in 32 bits: mul_mat_id_wide)
+    uint32_t xat[NC];  // the columns' pieces (byte offsets in 32 bits: mul_mat_id_wide)
 #pragma unroll
-    for (int u = 0; u < XP; u++) xat[u] = 2 * ((uint32_t) L.col[(tid + 256 * u) / 8] * (uint32_t) q.kp + 8 * (tid % 8));
-    const int scol = tid % BN, sblk = tid / BN;  // the scale this thread stages (sblk < 2)
-    struct stage {
-        moe_w<WT> w;
-        moe_x<XP> x;
-        float xd, xs;
-    };
-    auto load = [&](int64_t s, stage & st) {
-        moe_w<WT> & w = st.w;
-        const int64_t k0 = s * kMoeK;
-        if constexpr (WT == GGML_TYPE_F16) {
-            if (k0 + kMoeK <= a.K) {
-#pragma unroll
-                for (int u = 0; u < 4; u++) w.v[u] = *(const moe_u4 *) (wp[u] + 2 * k0);
-            } else {  // past K: the row's first piece, masked when stored
-#pragma unroll
-                for (int u = 0; u < 4; u++) w.v[u] = *(const moe_u4 *) (wp[u] + (k0 + 8 * (tid % 8) < a.K ? 2 * k0 : -16 * (tid % 8)));
-            }
-        } else if constexpr (WT == GGML_TYPE_Q8_0) {
-            const int64_t b = 2 * s + half;
-            const int64_t bc = 32 * b < a.K ? b : 0;  // past K: the columns' scale is zero
-            const moe_u4 * p = (const moe_u4 *) (wrow + 32 * bc);
-            w.v[0] = p[0];
-            w.v[1] = p[1];
-            w.d = *(const uint16_t *) (wrow + a.K + 2 * bc);
-        } else {
-            const char * blk = wrow + s / 4 * 144;
-            w.hdr = *(const moe_u4 *) blk;
-            w.v = *(const moe_u4 *) (blk + 16 + 32 * (s % 4) + 16 * half);
-        }
-        moe_x_load<XP>(st.x, q.x + k0, xat);
-        if constexpr (kQ) {
-            if (sblk < 2) {
-                const int64_t c = L.col[scol];
-                if constexpr (WT == GGML_TYPE_Q8_0) st.xd = q.xd[c * (q.kp / 32) + 2 * s + sblk];
-                else {
-                    st.xd = q.xd[c * (q.kp / 256) + s / 4];
-                    st.xs = q.xs[c * (q.kp / 32) + 2 * s + sblk];
-                }
-            }
-        }
-    };
-    auto store = [&](int b, int64_t s, const stage & st) {
-        const moe_w<WT> & w = st.w;
-        if constexpr (WT == GGML_TYPE_F16) {
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const uint32_t in = s * kMoeK + 8 * (tid % 8) < a.K ? 0xFFFFFFFFu : 0u;
-                *(moe_u4 *) moe_slot(L.w[b], tid / 8 + 32 * u, tid % 8) = w.v[u] & in;
-            }
-        } else if constexpr (WT == GGML_TYPE_Q8_0) {
-            const uint32_t z = 0x80808080u;
-            const uint32_t v[8] = {w.v[0].x, w.v[0].y, w.v[0].z, w.v[0].w, w.v[1].x, w.v[1].y, w.v[1].z, w.v[1].w};
-#pragma unroll
-            for (int u = 0; u < 4; u++) *moe_slot(L.w[b], srow, 4 * half + u) = moe_bytes(v[2 * u] ^ z, v[2 * u + 1] ^ z, 128.0f);
-            L.wd[b][half][srow] = half_bits_to_float(w.d);
-        } else {
-            const uint32_t lo = 0x0F0F0F0Fu;
-            const uint32_t v[4] = {w.v.x, w.v.y, w.v.z, w.v.w};
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                *moe_slot(L.w[b], srow, 2 * half + u) = moe_bytes(v[2 * u] & lo, v[2 * u + 1] & lo, 0.0f);
-                *moe_slot(L.w[b], srow, 4 + 2 * half + u) = moe_bytes(v[2 * u] >> 4 & lo, v[2 * u + 1] >> 4 & lo, 0.0f);
-            }
-            // block j's 6-bit scale and minimum of the packed 12 bytes
-            const int j = (int) (2 * (s % 4)) + half;
-            const uint32_t lowj = j < 4 ? w.hdr.y >> (8 * j) : w.hdr.w >> (8 * (j - 4));
-            const uint32_t minj = j < 4 ? w.hdr.z >> (8 * j) : w.hdr.w >> (8 * (j - 4) + 4);
-            const uint32_t hs = j < 4 ? 0 : w.hdr.y >> (8 * (j - 4) + 6) & 3, hm = j < 4 ? 0 : w.hdr.z >> (8 * (j - 4) + 6) & 3;
-            const uint32_t sc = j < 4 ? lowj & 63 : (lowj & 15) | hs << 4, mn = j < 4 ? minj & 63 : (minj & 15) | hm << 4;
-            L.wd[b][half][srow] = half_bits_to_float((uint16_t) w.hdr.x) * (float) sc;
-            L.wm[b][half][srow] = -half_bits_to_float((uint16_t) (w.hdr.x >> 16)) * (float) mn;
-        }
-        moe_x_store<XP>(st.x, L.x[b]);
-        if constexpr (kQ) {
-            if (sblk < 2) {
-                L.xd[b][sblk][scol] = st.xd;
-                if constexpr (WT == GGML_TYPE_Q4_K) L.xs[b][sblk][scol] = st.xs;
-            }
-        }
-    };
-    // wave (wr, wc): columns BN / 2 wc ..; rows 64 wr .., or 32 wr .. of both matrices
+    for (int u = 0; u < NC; u++) xat[u] = 2 * ((uint32_t) L.col[(tid + 256 * u) / 8] * (uint32_t) q.kp + 8 * (tid % 8));
+    // wave (wr, wc): the 16-column tiles wc, wc + 2, ..; rows 64 wr .., or 32 wr .. of
+    // both matrices. Tiles past the last column are neither staged nor multiplied.
+    auto tile_col = [&](int j) { return 32 * j + 16 * wc; };
     auto tile_row = [&](int i) { return PAIR ? 64 * (i >> 1) + 32 * wr + 16 * (i & 1) : 64 * wr + 16 * i; };
     moe_v4f acc[NR][NC];
 #pragma unroll
@@ -603,121 +524,215 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
 #pragma unroll
         for (int j = 0; j < NC; j++) acc[i][j] = moe_v4f{0, 0, 0, 0};
     const moe_v4f zero = {0, 0, 0, 0};
-    auto multiply = [&](int b) {
+    // C: the tile's 32-column groups that hold columns (the workgroup's one value)
+    auto products_of = [&](auto groups) {
+        constexpr int C = decltype(groups)::value;
+        // (the values of the lane made anew for each C: shared ones were kept and spilled)
+        int tid = (int) threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        const int lane = tid & 63, r = lane & 15, g = lane >> 4, srow = tid >> 1, half = tid & 1;
+        const int scol = tid % BN, sblk = tid / BN;  // the scale this thread stages (sblk < 2)
+        struct stage {
+            moe_w<WT> w;
+            moe_x<C> x;
+            float xd, xs;
+        };
+        auto load = [&](int64_t s, stage & st) {
+            moe_w<WT> & w = st.w;
+            const int64_t k0 = s * kMoeK;
+            if constexpr (WT == GGML_TYPE_F16) {
+                if (k0 + kMoeK <= a.K) {
 #pragma unroll
-        for (int kk = 0; kk < 2; kk++) {
-            __builtin_amdgcn_sched_barrier(0);  // (one block's operands at a time: more in flight spill)
-            moe_v8h wf[NR], xf[NC];
+                    for (int u = 0; u < 4; u++) w.v[u] = *(const moe_u4 *) (wp[u] + 2 * k0);
+                } else {  // past K: the row's first piece, masked when stored
 #pragma unroll
-            for (int i = 0; i < NR; i++)
-                wf[i] = __builtin_bit_cast(moe_v8h, *moe_slot(L.w[b], tile_row(i) + r, 4 * kk + g));
-#pragma unroll
-            for (int j = 0; j < NC; j++)
-                xf[j] = __builtin_bit_cast(moe_v8h, *moe_slot(L.x[b], BN / 2 * wc + 16 * j + r, 4 * kk + g));
-            if constexpr (kQ) {
-                float dw[NR], mw[NR];
-#pragma unroll
-                for (int i = 0; i < NR; i++) {
-                    dw[i] = L.wd[b][kk][tile_row(i) + r];
-                    if constexpr (WT == GGML_TYPE_Q4_K) mw[i] = L.wm[b][kk][tile_row(i) + r];
+                    for (int u = 0; u < 4; u++) w.v[u] = *(const moe_u4 *) (wp[u] + (k0 + 8 * (tid % 8) < a.K ? 2 * k0 : -16 * (tid % 8)));
                 }
+            } else if constexpr (WT == GGML_TYPE_Q8_0) {
+                const int64_t b = 2 * s + half;
+                const int64_t bc = 32 * b < a.K ? b : 0;  // past K: the columns' scale is zero
+                const moe_u4 * p = (const moe_u4 *) (wrow + 32 * bc);
+                w.v[0] = p[0];
+                w.v[1] = p[1];
+                w.d = *(const uint16_t *) (wrow + a.K + 2 * bc);
+            } else {
+                const char * blk = wrow + s / 4 * 144;
+                w.hdr = *(const moe_u4 *) blk;
+                w.v = *(const moe_u4 *) (blk + 16 + 32 * (s % 4) + 16 * half);
+            }
+            moe_x_load<C>(st.x, q.x + k0, xat);
+            if constexpr (kQ) {
+                if (sblk < 2) {
+                    const int64_t c = L.col[scol];
+                    if constexpr (WT == GGML_TYPE_Q8_0) st.xd = q.xd[c * (q.kp / 32) + 2 * s + sblk];
+                    else {
+                        st.xd = q.xd[c * (q.kp / 256) + s / 4];
+                        st.xs = q.xs[c * (q.kp / 32) + 2 * s + sblk];
+                    }
+                }
+            }
+        };
+        auto store = [&](int b, int64_t s, const stage & st) {
+            const moe_w<WT> & w = st.w;
+            if constexpr (WT == GGML_TYPE_F16) {
 #pragma unroll
-                for (int j = 0; j < NC; j++) {
-                    const float4 dx = *(const float4 *) &L.xd[b][kk][BN / 2 * wc + 16 * j + 4 * g];
-                    const float d4[4] = {dx.x, dx.y, dx.z, dx.w};
-                    float s4[4];
-                    if constexpr (WT == GGML_TYPE_Q4_K) *(float4 *) s4 = *(const float4 *) &L.xs[b][kk][BN / 2 * wc + 16 * j + 4 * g];
+                for (int u = 0; u < 4; u++) {
+                    const uint32_t in = s * kMoeK + 8 * (tid % 8) < a.K ? 0xFFFFFFFFu : 0u;
+                    *(moe_u4 *) moe_slot(L.w[b], tid / 8 + 32 * u, tid % 8) = w.v[u] & in;
+                }
+            } else if constexpr (WT == GGML_TYPE_Q8_0) {
+                const uint32_t z = 0x80808080u;
+                const uint32_t v[8] = {w.v[0].x, w.v[0].y, w.v[0].z, w.v[0].w, w.v[1].x, w.v[1].y, w.v[1].z, w.v[1].w};
+#pragma unroll
+                for (int u = 0; u < 4; u++) *moe_slot(L.w[b], srow, 4 * half + u) = moe_bytes(v[2 * u] ^ z, v[2 * u + 1] ^ z, 128.0f);
+                L.wd[b][half][srow] = half_bits_to_float(w.d);
+            } else {
+                const uint32_t lo = 0x0F0F0F0Fu;
+                const uint32_t v[4] = {w.v.x, w.v.y, w.v.z, w.v.w};
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    *moe_slot(L.w[b], srow, 2 * half + u) = moe_bytes(v[2 * u] & lo, v[2 * u + 1] & lo, 0.0f);
+                    *moe_slot(L.w[b], srow, 4 + 2 * half + u) = moe_bytes(v[2 * u] >> 4 & lo, v[2 * u + 1] >> 4 & lo, 0.0f);
+                }
+                // block j's 6-bit scale and minimum of the packed 12 bytes
+                const int j = (int) (2 * (s % 4)) + half;
+                const uint32_t lowj = j < 4 ? w.hdr.y >> (8 * j) : w.hdr.w >> (8 * (j - 4));
+                const uint32_t minj = j < 4 ? w.hdr.z >> (8 * j) : w.hdr.w >> (8 * (j - 4) + 4);
+                const uint32_t hs = j < 4 ? 0 : w.hdr.y >> (8 * (j - 4) + 6) & 3, hm = j < 4 ? 0 : w.hdr.z >> (8 * (j - 4) + 6) & 3;
+                const uint32_t sc = j < 4 ? lowj & 63 : (lowj & 15) | hs << 4, mn = j < 4 ? minj & 63 : (minj & 15) | hm << 4;
+                L.wd[b][half][srow] = half_bits_to_float((uint16_t) w.hdr.x) * (float) sc;
+                L.wm[b][half][srow] = -half_bits_to_float((uint16_t) (w.hdr.x >> 16)) * (float) mn;
+            }
+            moe_x_store<C>(st.x, L.x[b], tid);
+            if constexpr (kQ) {
+                if (sblk < 2) {
+                    L.xd[b][sblk][scol] = st.xd;
+                    if constexpr (WT == GGML_TYPE_Q4_K) L.xs[b][sblk][scol] = st.xs;
+                }
+            }
+        };
+        auto multiply = [&](int b) {
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++) {
+                __builtin_amdgcn_sched_barrier(0);  // (one block's operands at a time: more in flight spill)
+                moe_v8h wf[NR], xf[C];
+#pragma unroll
+                for (int i = 0; i < NR; i++)
+                    wf[i] = __builtin_bit_cast(moe_v8h, *moe_slot(L.w[b], tile_row(i) + r, 4 * kk + g));
+#pragma unroll
+                for (int j = 0; j < C; j++)
+                    xf[j] = __builtin_bit_cast(moe_v8h, *moe_slot(L.x[b], tile_col(j) + r, 4 * kk + g));
+                if constexpr (kQ) {
+                    float dw[NR], mw[NR];
 #pragma unroll
                     for (int i = 0; i < NR; i++) {
-                        const moe_v4f p = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[j], wf[i], zero, 0, 0, 0);
+                        dw[i] = L.wd[b][kk][tile_row(i) + r];
+                        if constexpr (WT == GGML_TYPE_Q4_K) mw[i] = L.wm[b][kk][tile_row(i) + r];
+                    }
 #pragma unroll
-                        for (int v = 0; v < 4; v++) {
-                            acc[i][j][v] = fmaf(p[v], dw[i] * d4[v], acc[i][j][v]);
-                            if constexpr (WT == GGML_TYPE_Q4_K) acc[i][j][v] = fmaf(mw[i], s4[v], acc[i][j][v]);
+                    for (int j = 0; j < C; j++) {
+                        const float4 dx = *(const float4 *) &L.xd[b][kk][tile_col(j) + 4 * g];
+                        const float d4[4] = {dx.x, dx.y, dx.z, dx.w};
+                        float s4[4];
+                        if constexpr (WT == GGML_TYPE_Q4_K) *(float4 *) s4 = *(const float4 *) &L.xs[b][kk][tile_col(j) + 4 * g];
+#pragma unroll
+                        for (int i = 0; i < NR; i++) {
+                            const moe_v4f p = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[j], wf[i], zero, 0, 0, 0);
+#pragma unroll
+                            for (int v = 0; v < 4; v++) {
+                                acc[i][j][v] = fmaf(p[v], dw[i] * d4[v], acc[i][j][v]);
+                                if constexpr (WT == GGML_TYPE_Q4_K) acc[i][j][v] = fmaf(mw[i], s4[v], acc[i][j][v]);
+                            }
                         }
                     }
                 }
             }
+        };
+        // Two steps in flight: a step's products take a fraction of a load's way.
+        // (The loads past the last step are the last step's again: one that may
+        // not have been made would be waited for with all later ones. Q4_K at 128
+        // columns has the registers for one: a second one spilled 34 of them.)
+        constexpr int kAhead = kQ && BN == 128 ? 1 : 2;
+        stage s0, s1;
+        load(0, s0);
+        if constexpr (kAhead == 2) load(min((int64_t) 1, steps - 1), s1);
+        if constexpr (!kQ) {
+            // A half step's operands are read under the products of the one
+            // before: the second half's at the step's start, the next step's first
+            // half's after the barrier in its middle, by which that step is staged.
+            struct half_step {
+                moe_v8h w[NR], x[C];
+            };
+            auto read = [&](int b, int kk, half_step & f) {
+#pragma unroll
+                for (int j = 0; j < C; j++)
+                    f.x[j] = __builtin_bit_cast(moe_v8h, *moe_slot(L.x[b], tile_col(j) + r, 4 * kk + g));
+#pragma unroll
+                for (int i = 0; i < NR; i++)
+                    f.w[i] = __builtin_bit_cast(moe_v8h, *moe_slot(L.w[b], tile_row(i) + r, 4 * kk + g));
+            };
+            auto products = [&](const half_step & f) {
+#pragma unroll
+                for (int i = 0; i < NR; i++)
+#pragma unroll
+                    for (int j = 0; j < C; j++)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.x[j], f.w[i], acc[i][j], 0, 0, 0);
+            };
+            half_step f0, f1;
+            store(0, 0, s0);
+            __syncthreads();
+            load(min((int64_t) 2, steps - 1), s0);
+            read(0, 0, f0);
+            // step s of buffer b; `next` holds step s + 1
+            auto step = [&](int64_t s, int b, stage & next) {
+                read(b, 1, f1);
+                store(b ^ 1, min(s + 1, steps - 1), next);
+                products(f0);
+                __syncthreads();
+                load(min(s + 3, steps - 1), next);
+                read(b ^ 1, 0, f0);
+                products(f1);
+            };
+            for (int64_t s = 0;;) {
+                step(s, 0, s1);
+                if (++s >= steps) break;
+                step(s, 1, s0);
+                if (++s >= steps) break;
+            }
+        } else if constexpr (kAhead == 1) {
+            for (int64_t s = 0; s < steps; s++) {
+                const int b = (int) (s & 1);
+                store(b, s, s0);
+                __syncthreads();  // the step is staged; the buffer of the step before is free
+                load(min(s + 1, steps - 1), s0);
+                multiply(b);
+            }
+        } else {
+            for (int64_t s = 0;;) {
+                store(0, s, s0);
+                __syncthreads();  // the step is staged; the buffer of the step before is free
+                load(min(s + 2, steps - 1), s0);
+                multiply(0);
+                if (++s >= steps) break;
+                store(1, s, s1);
+                __syncthreads();
+                load(min(s + 2, steps - 1), s1);
+                multiply(1);
+                if (++s >= steps) break;
+            }
         }
     };
-    // Two steps in flight: a step's products take a fraction of a load's way.
-    // (The loads past the last step are the last step's again: one that may
-    // not have been made would be waited for with all later ones. Q4_K at 128
-    // columns has the registers for one: a second one spilled 34 of them.)
-    constexpr int kAhead = WT == GGML_TYPE_Q4_K && BN == 128 ? 1 : 2;
-    stage s0, s1;
-    load(0, s0);
-    if constexpr (kAhead == 2) load(min((int64_t) 1, steps - 1), s1);
-    if constexpr (!kQ) {
-        // A half step's operands are read under the products of the one
-        // before: the second half's at the step's start, the next step's first
-        // half's after the barrier in its middle, by which that step is staged.
-        struct half_step {
-            moe_v8h w[NR], x[NC];
-        };
-        auto read = [&](int b, int kk, half_step & f) {
-#pragma unroll
-            for (int j = 0; j < NC; j++)
-                f.x[j] = __builtin_bit_cast(moe_v8h, *moe_slot(L.x[b], BN / 2 * wc + 16 * j + r, 4 * kk + g));
-#pragma unroll
-            for (int i = 0; i < NR; i++)
-                f.w[i] = __builtin_bit_cast(moe_v8h, *moe_slot(L.w[b], tile_row(i) + r, 4 * kk + g));
-        };
-        auto products = [&](const half_step & f) {
-#pragma unroll
-            for (int i = 0; i < NR; i++)
-#pragma unroll
-                for (int j = 0; j < NC; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.x[j], f.w[i], acc[i][j], 0, 0, 0);
-        };
-        half_step f0, f1;
-        store(0, 0, s0);
-        __syncthreads();
-        load(min((int64_t) 2, steps - 1), s0);
-        read(0, 0, f0);
-        // step s of buffer b; `next` holds step s + 1
-        auto step = [&](int64_t s, int b, stage & next) {
-            read(b, 1, f1);
-            store(b ^ 1, min(s + 1, steps - 1), next);
-            products(f0);
-            __syncthreads();
-            load(min(s + 3, steps - 1), next);
-            read(b ^ 1, 0, f0);
-            products(f1);
-        };
-        for (int64_t s = 0;;) {
-            step(s, 0, s1);
-            if (++s >= steps) break;
-            step(s, 1, s0);
-            if (++s >= steps) break;
-        }
-    } else if constexpr (kAhead == 1) {
-        for (int64_t s = 0; s < steps; s++) {
-            const int b = (int) (s & 1);
-            store(b, s, s0);
-            __syncthreads();  // the step is staged; the buffer of the step before is free
-            load(min(s + 1, steps - 1), s0);
-            multiply(b);
-        }
-    } else {
-        for (int64_t s = 0;;) {
-            store(0, s, s0);
-            __syncthreads();  // the step is staged; the buffer of the step before is free
-            load(min(s + 2, steps - 1), s0);
-            multiply(0);
-            if (++s >= steps) break;
-            store(1, s, s1);
-            __syncthreads();
-            load(min(s + 2, steps - 1), s1);
-            multiply(1);
-            if (++s >= steps) break;
-        }
+    switch (kQ ? (n + 31) / 32 : NC) {
+        case 1: products_of(std::integral_constant<int, 1>{}); break;
+        case 2: products_of(std::integral_constant<int, NC < 2 ? NC : 2>{}); break;
+        case 3: products_of(std::integral_constant<int, NC < 3 ? NC : 3>{}); break;
+        default: products_of(std::integral_constant<int, NC>{}); break;
     }
 #pragma unroll
     for (int j = 0; j < NC; j++)
 #pragma unroll
         for (int v = 0; v < 4; v++) {
-            const int c = BN / 2 * wc + 16 * j + 4 * g + v;
+            const int c = tile_col(j) + 4 * g + v;
             if (c >= n) continue;
             float * o = a.out + (int64_t) L.pair[c] * a.M;
             if constexpr (PAIR) {
