@@ -266,8 +266,7 @@ constexpr int kMoeRows = 128;
 struct moe_wide_args {
     mul_mat_id_args a;
     int * head;     // [0]: the number of tiles
-    int4 * tiles;   // expert (-1: none), first place, columns, the expert's first tile
-    int * runs;     // by tile: the tiles of its expert
+    int4 * tiles;   // the expert (-1: none), its first place, its columns, its first tile
     int * sorted;   // place -> pair
     _Float16 * x;   // [b column][Kp]
     float * xd;     // quantized: the blocks' scales, [b column][Kp / 32 or Kp / 256]
@@ -333,10 +332,7 @@ __device__ __forceinline__ void moe_route(const moe_wide_args & q) {
         if (b < bins) {
             int at = before + sum - total;
             const int t0 = tbefore + tsum - nt;
-            for (int t = 0; t < nt; t++) {
-                q.tiles[t0 + t] = make_int4(b < a.experts ? b : -1, at + t * q.bn, min(q.bn, total - t * q.bn), t0);
-                q.runs[t0 + t] = nt;
-            }
+            for (int t = 0; t < nt; t++) q.tiles[t0 + t] = make_int4(b < a.experts ? b : -1, at, total, t0);
             for (int w = 0; w < 16; w++) {  // the waves' first places
                 const int c = s_hist[w * bins + b];
                 s_hist[w * bins + b] = at;
@@ -429,11 +425,23 @@ struct moe_w<GGML_TYPE_F16> {
 template <>
 struct moe_w<GGML_TYPE_Q8_0> {
     moe_u4 v[2];
-    uint16_t d;
 };
 template <>
 struct moe_w<GGML_TYPE_Q4_K> {
-    moe_u4 hdr, v;
+    moe_u4 v;
+};
+
+// and of the scales of four steps: a row's of four blocks (Q4_K: its
+// super-block's header), a column's of four
+template <int WT>
+struct moe_scales {
+    moe_u4 hdr;
+    float d, s[4];
+};
+template <>
+struct moe_scales<GGML_TYPE_Q8_0> {
+    uint16_t w[4];
+    float2 x[2];
 };
 
 // and of its columns, 16-byte pieces
@@ -453,45 +461,46 @@ __device__ __forceinline__ void moe_x_store(const moe_x<C> & x, _Float16 (*s)[kM
     for (int u = 0; u < C; u++) *(moe_u4 *) moe_slot(s, (tid + 256 * u) / 8, tid % 8) = x.v[u];
 }
 
-template <int BN>
+template <int WT, int BN, int NB>
 struct moe_lds {
-    _Float16 w[2][kMoeRows][kMoeK];
-    _Float16 x[2][BN][kMoeK];
-    float wd[2][2][kMoeRows];  // a block's scale by [buffer][block of the step][row]
-    float wm[2][2][kMoeRows];  // Q4_K: its minimum
-    float xd[2][2][BN];        // the columns' scales
-    float xs[2][2][BN];        // Q4_K: scale times sum
+    static constexpr int kS = WT == GGML_TYPE_F16 ? 1 : 8, kM = WT == GGML_TYPE_Q4_K ? 8 : 1;
+    _Float16 w[NB][kMoeRows][kMoeK];
+    _Float16 x[NB][BN][kMoeK];
+    float wd[NB][kS][kMoeRows];  // a block's scale by [buffer][block of four steps][row]
+    float wm[NB][kM][kMoeRows];  // Q4_K: its minimum
+    float xd[NB][kS][BN];        // the columns' scales (Q4_K: one)
+    float xs[NB][kM][BN];        // Q4_K: scale times sum
     int col[BN];               // the columns' places in b
     int pair[BN];              // and in the result
 };
 
 template <int WT, bool PAIR, int BN>
 __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
-    constexpr int kQ = WT != GGML_TYPE_F16;
+    constexpr int kQ = WT != GGML_TYPE_F16, NB = kQ && BN == 128 ? 1 : 2;
     constexpr int NR = 4, NC = BN / 32;  // a wave's 16-tiles of rows and columns: 64 rows, BN / 2 columns
-    __shared__ __align__(16) moe_lds<BN> L;
+    __shared__ __align__(16) moe_lds<WT, BN, NB> L;
     const mul_mat_id_args & a = q.a;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave & 1, wc = wave >> 1;
-    // Contiguous runs of tiles an XCD (workgroup i on XCD i % 8), an expert's
-    // row tiles in turn with its column tiles adjacent: they read the same
-    // weights at the same time, once beyond their XCD's L2. (A column tile's
-    // row tiles in turn: a weight tile came in 1.5 times.)
-    const uint32_t rows = (uint32_t) q.row_tiles, total = (uint32_t) q.head[0] * rows, per = (total + 7) / 8;
-    const uint32_t t = blockIdx.x % 8 * per + blockIdx.x / 8;
-    if (blockIdx.x / 8 >= per || t >= total) return;
-    const int first = q.tiles[t / rows].w;
-    const uint32_t in = t - (uint32_t) first * rows, run = (uint32_t) q.runs[first], rt = in / run;
-    const int4 tile = q.tiles[first + (int) (in - rt * run)];
+    // Workgroup i is on XCD i % 8. Each expert's row tiles go to the XCDs in
+    // turn, so that a much used expert's work is spread; a row tile's column
+    // tiles are adjacent: they read the same weights at the same time, once
+    // beyond their XCD's L2.
+    const uint32_t rows = (uint32_t) q.row_tiles, each = (rows + 7) / 8, t = blockIdx.x / 8;
+    if (t >= (uint32_t) q.head[0] * each) return;
+    const int4 of = q.tiles[t / each];  // its expert's columns and first tile
+    const uint32_t in = t - (uint32_t) of.w * each, run = (uint32_t) (of.z + BN - 1) / BN, nth = in / run, ct = in - nth * run;
+    const uint32_t rt = 8 * nth + (blockIdx.x + (uint32_t) of.w) % 8;
+    if (rt >= rows) return;
     const int64_t m0 = (int64_t) rt * (PAIR ? 64 : 128);
-    const int n = __builtin_amdgcn_readfirstlane(tile.z);
+    const int n = __builtin_amdgcn_readfirstlane(min(BN, of.z - (int) ct * BN)), at = of.y + (int) ct * BN;
     if (tid < BN) {
-        const int p = q.sorted[tile.y + min(tid, n - 1)];
+        const int p = q.sorted[at + min(tid, n - 1)];
         L.pair[tid] = p;
         L.col[tid] = (int) (p / a.used * a.b_ne1 + p % a.used % a.b_ne1);
     }
     __syncthreads();
-    if (tile.x < 0) {  // no expert: zeros
+    if (of.x < 0) {  // no expert: zeros
         const int rows = (int) min((int64_t) (PAIR ? 64 : 128), a.M - m0);
         for (int i = tid; i < n * rows; i += 256) a.out[(int64_t) L.pair[i / rows] * a.M + m0 + i % rows] = 0.0f;
         return;
@@ -500,14 +509,14 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
     // W, then the same of W2
     const int srow = tid >> 1, half = tid & 1;
     const int64_t mrow = min(PAIR ? m0 + (srow & 63) : m0 + srow, a.M - 1);
-    const char * wrow = (PAIR && srow >= 64 ? a.W2 : a.W) + tile.x * a.W_nb2 + mrow * a.W_nb1;
+    const char * wrow = (PAIR && srow >= 64 ? a.W2 : a.W) + of.x * a.W_nb2 + mrow * a.W_nb1;
     // (F16: pieces t % 8 of the rows t / 8 + 32 u, whole lines a load)
     const char * wp[WT == GGML_TYPE_F16 ? 4 : 1];
     if constexpr (WT == GGML_TYPE_F16) {
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const int64_t m = min(m0 + (PAIR ? (tid / 8 + 32 * u) & 63 : tid / 8 + 32 * u), a.M - 1);
-            wp[u] = (PAIR && u >= 2 ? a.W2 : a.W) + tile.x * a.W_nb2 + m * a.W_nb1 + 16 * (tid % 8);
+            wp[u] = (PAIR && u >= 2 ? a.W2 : a.W) + of.x * a.W_nb2 + m * a.W_nb1 + 16 * (tid % 8);
         }
     }
     const int64_t steps = (a.K + kMoeK - 1) / kMoeK;
@@ -535,7 +544,52 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
         struct stage {
             moe_w<WT> w;
             moe_x<C> x;
-            float xd, xs;
+        };
+        // The scales are fetched and staged for four steps at once: a load a
+        // step touched a line of its own for each row and column, as much
+        // again as the weights.
+        auto load_scales = [&](int64_t s, moe_scales<WT> & sc) {
+            const int64_t c = L.col[scol];
+            if constexpr (WT == GGML_TYPE_Q8_0) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int64_t blk = 2 * s + 4 * half + i;
+                    sc.w[i] = *(const uint16_t *) (wrow + a.K + 2 * (32 * blk < a.K ? blk : 0));
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    sc.x[i] = *(const float2 *) (q.xd + c * (q.kp / 32) + 2 * min(s + 2 * (sblk & 1) + i, steps - 1));
+            } else if constexpr (WT == GGML_TYPE_Q4_K) {
+                sc.hdr = *(const moe_u4 *) (wrow + s / 4 * 144);
+                sc.d = q.xd[c * (q.kp / 256) + s / 4];
+                *(float4 *) sc.s = *(const float4 *) (q.xs + c * (q.kp / 32) + 2 * s + 4 * (sblk & 1));
+            }
+        };
+        auto store_scales = [&](int b, const moe_scales<WT> & sc) {
+            if constexpr (WT == GGML_TYPE_Q8_0) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) L.wd[b][4 * half + i][srow] = half_bits_to_float(sc.w[i]);
+                if (sblk < 2) {
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+                        L.xd[b][4 * sblk + 2 * i][scol] = sc.x[i].x, L.xd[b][4 * sblk + 2 * i + 1][scol] = sc.x[i].y;
+                }
+            } else if constexpr (WT == GGML_TYPE_Q4_K) {
+                // block j's 6-bit scale and minimum of the packed 12 bytes
+                const float d = half_bits_to_float((uint16_t) sc.hdr.x), m = -half_bits_to_float((uint16_t) (sc.hdr.x >> 16));
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t s6 = half ? (sc.hdr.w >> (8 * i) & 15) | (sc.hdr.y >> (8 * i + 6) & 3) << 4 : sc.hdr.y >> (8 * i) & 63;
+                    const uint32_t m6 = half ? (sc.hdr.w >> (8 * i + 4) & 15) | (sc.hdr.z >> (8 * i + 6) & 3) << 4 : sc.hdr.z >> (8 * i) & 63;
+                    L.wd[b][4 * half + i][srow] = d * (float) s6;
+                    L.wm[b][4 * half + i][srow] = m * (float) m6;
+                }
+                if (sblk < 2) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) L.xs[b][4 * sblk + i][scol] = sc.s[i];
+                    if (sblk == 0) L.xd[b][0][scol] = sc.d;
+                }
+            }
         };
         auto load = [&](int64_t s, stage & st) {
             moe_w<WT> & w = st.w;
@@ -554,23 +608,10 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
                 const moe_u4 * p = (const moe_u4 *) (wrow + 32 * bc);
                 w.v[0] = p[0];
                 w.v[1] = p[1];
-                w.d = *(const uint16_t *) (wrow + a.K + 2 * bc);
             } else {
-                const char * blk = wrow + s / 4 * 144;
-                w.hdr = *(const moe_u4 *) blk;
-                w.v = *(const moe_u4 *) (blk + 16 + 32 * (s % 4) + 16 * half);
+                w.v = *(const moe_u4 *) (wrow + s / 4 * 144 + 16 + 32 * (s % 4) + 16 * half);
             }
             moe_x_load<C>(st.x, q.x + k0, xat);
-            if constexpr (kQ) {
-                if (sblk < 2) {
-                    const int64_t c = L.col[scol];
-                    if constexpr (WT == GGML_TYPE_Q8_0) st.xd = q.xd[c * (q.kp / 32) + 2 * s + sblk];
-                    else {
-                        st.xd = q.xd[c * (q.kp / 256) + s / 4];
-                        st.xs = q.xs[c * (q.kp / 32) + 2 * s + sblk];
-                    }
-                }
-            }
         };
         auto store = [&](int b, int64_t s, const stage & st) {
             const moe_w<WT> & w = st.w;
@@ -585,7 +626,6 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
                 const uint32_t v[8] = {w.v[0].x, w.v[0].y, w.v[0].z, w.v[0].w, w.v[1].x, w.v[1].y, w.v[1].z, w.v[1].w};
 #pragma unroll
                 for (int u = 0; u < 4; u++) *moe_slot(L.w[b], srow, 4 * half + u) = moe_bytes(v[2 * u] ^ z, v[2 * u + 1] ^ z, 128.0f);
-                L.wd[b][half][srow] = half_bits_to_float(w.d);
             } else {
                 const uint32_t lo = 0x0F0F0F0Fu;
                 const uint32_t v[4] = {w.v.x, w.v.y, w.v.z, w.v.w};
@@ -594,24 +634,11 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
                     *moe_slot(L.w[b], srow, 2 * half + u) = moe_bytes(v[2 * u] & lo, v[2 * u + 1] & lo, 0.0f);
                     *moe_slot(L.w[b], srow, 4 + 2 * half + u) = moe_bytes(v[2 * u] >> 4 & lo, v[2 * u + 1] >> 4 & lo, 0.0f);
                 }
-                // block j's 6-bit scale and minimum of the packed 12 bytes
-                const int j = (int) (2 * (s % 4)) + half;
-                const uint32_t lowj = j < 4 ? w.hdr.y >> (8 * j) : w.hdr.w >> (8 * (j - 4));
-                const uint32_t minj = j < 4 ? w.hdr.z >> (8 * j) : w.hdr.w >> (8 * (j - 4) + 4);
-                const uint32_t hs = j < 4 ? 0 : w.hdr.y >> (8 * (j - 4) + 6) & 3, hm = j < 4 ? 0 : w.hdr.z >> (8 * (j - 4) + 6) & 3;
-                const uint32_t sc = j < 4 ? lowj & 63 : (lowj & 15) | hs << 4, mn = j < 4 ? minj & 63 : (minj & 15) | hm << 4;
-                L.wd[b][half][srow] = half_bits_to_float((uint16_t) w.hdr.x) * (float) sc;
-                L.wm[b][half][srow] = -half_bits_to_float((uint16_t) (w.hdr.x >> 16)) * (float) mn;
             }
             moe_x_store<C>(st.x, L.x[b], tid);
-            if constexpr (kQ) {
-                if (sblk < 2) {
-                    L.xd[b][sblk][scol] = st.xd;
-                    if constexpr (WT == GGML_TYPE_Q4_K) L.xs[b][sblk][scol] = st.xs;
-                }
-            }
         };
-        auto multiply = [&](int b) {
+        auto multiply = [&](int b, int64_t s) {
+            const int gb = NB == 2 ? (int) (s / 4 & 1) : 0;  // the scales' buffer
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
                 __builtin_amdgcn_sched_barrier(0);  // (one block's operands at a time: more in flight spill)
@@ -626,15 +653,15 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
                     float dw[NR], mw[NR];
 #pragma unroll
                     for (int i = 0; i < NR; i++) {
-                        dw[i] = L.wd[b][kk][tile_row(i) + r];
-                        if constexpr (WT == GGML_TYPE_Q4_K) mw[i] = L.wm[b][kk][tile_row(i) + r];
+                        dw[i] = L.wd[gb][2 * (s % 4) + kk][tile_row(i) + r];
+                        if constexpr (WT == GGML_TYPE_Q4_K) mw[i] = L.wm[gb][2 * (s % 4) + kk][tile_row(i) + r];
                     }
 #pragma unroll
                     for (int j = 0; j < C; j++) {
-                        const float4 dx = *(const float4 *) &L.xd[b][kk][tile_col(j) + 4 * g];
+                        const float4 dx = *(const float4 *) &L.xd[gb][WT == GGML_TYPE_Q4_K ? 0 : 2 * (s % 4) + kk][tile_col(j) + 4 * g];
                         const float d4[4] = {dx.x, dx.y, dx.z, dx.w};
                         float s4[4];
-                        if constexpr (WT == GGML_TYPE_Q4_K) *(float4 *) s4 = *(const float4 *) &L.xs[b][kk][tile_col(j) + 4 * g];
+                        if constexpr (WT == GGML_TYPE_Q4_K) *(float4 *) s4 = *(const float4 *) &L.xs[gb][2 * (s % 4) + kk][tile_col(j) + 4 * g];
 #pragma unroll
                         for (int i = 0; i < NR; i++) {
                             const moe_v4f p = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[j], wf[i], zero, 0, 0, 0);
@@ -699,26 +726,39 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
                 step(s, 1, s0);
                 if (++s >= steps) break;
             }
-        } else if constexpr (kAhead == 1) {
-            for (int64_t s = 0; s < steps; s++) {
-                const int b = (int) (s & 1);
-                store(b, s, s0);
-                __syncthreads();  // the step is staged; the buffer of the step before is free
-                load(min(s + 1, steps - 1), s0);
-                multiply(b);
-            }
         } else {
-            for (int64_t s = 0;;) {
-                store(0, s, s0);
-                __syncthreads();  // the step is staged; the buffer of the step before is free
-                load(min(s + 2, steps - 1), s0);
-                multiply(0);
-                if (++s >= steps) break;
-                store(1, s, s1);
-                __syncthreads();
-                load(min(s + 2, steps - 1), s1);
-                multiply(1);
-                if (++s >= steps) break;
+            moe_scales<WT> sc;
+            load_scales(0, sc);
+            // step s: its scales first, where four begin; the next four's loads
+            // then have four steps
+            auto scales = [&](int64_t s) {
+                if (s % 4 != 0) return;
+                store_scales(NB == 2 ? (int) (s / 4 & 1) : 0, sc);
+                load_scales(s + 4 < steps ? s + 4 : 0, sc);
+            };
+            if constexpr (kAhead == 1) {
+                for (int64_t s = 0; s < steps; s++) {
+                    scales(s);
+                    store(0, s, s0);
+                    __syncthreads();
+                    load(min(s + 1, steps - 1), s0);
+                    multiply(0, s);
+                    __syncthreads();  // the step's operands are read
+                }
+            } else {
+                for (int64_t s = 0;;) {
+                    scales(s);
+                    store(0, s, s0);
+                    __syncthreads();  // the step is staged; the buffer of the step before is free
+                    load(min(s + 2, steps - 1), s0);
+                    multiply(0, s);
+                    if (++s >= steps) break;
+                    store(1, s, s1);
+                    __syncthreads();
+                    load(min(s + 2, steps - 1), s1);
+                    multiply(1, s);
+                    if (++s >= steps) break;
+                }
             }
         }
     };
@@ -807,7 +847,7 @@ static bool moe_aligned(int wtype, const mul_mat_id_args & a) {
 }
 
 bool mul_mat_id_wide(int wtype, const mul_mat_id_args & a) {
-    return moe_aligned(wtype, a) && a.pairs > kMoeFew && a.experts <= 960 && a.pairs < 1 << 30 &&
+    return moe_aligned(wtype, a) && a.pairs > kMoeFew && a.experts <= 960 && a.pairs < 1 << 26 &&
            (a.K + 63) / 64 * 64 * a.b_ne1 * (a.pairs / a.used) < 1ll << 31;
 }
 
@@ -831,7 +871,6 @@ static size_t moe_carve(int wtype, const mul_mat_id_args & a, moe_wide_args & q,
     };
     q.head = (int *) take(256);
     q.tiles = (int4 *) take((size_t) q.max_tiles * 16);
-    q.runs = (int *) take((size_t) q.max_tiles * 4);
     q.sorted = (int *) take((size_t) a.pairs * 4);
     q.x = (_Float16 *) take((size_t) (q.bcols * q.kp) * 2);
     if (wtype == GGML_TYPE_Q8_0) q.xd = (float *) take((size_t) (q.bcols * (q.kp / 32)) * 4);
@@ -854,7 +893,7 @@ static void launch_moe_wide(const mul_mat_id_args & a, char * scratch, hipStream
     const int64_t waves = (q.kp + 255) / 256 * q.bcols;
     hipLaunchKernelGGL(k_moe_prepare<WT>, dim3((unsigned) ((waves + 15) / 16 + 1)), dim3(1024),
                        (size_t) (16 * (a.experts + 1)) * 4, s, q);
-    const unsigned grid = (unsigned) ((q.max_tiles * q.row_tiles + 7) / 8 * 8);
+    const unsigned grid = (unsigned) (q.max_tiles * ((q.row_tiles + 7) / 8 * 8));
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, q); };
     if (q.bn == 128) a.W2 ? go(k_moe_gemm<WT, true, 128>) : go(k_moe_gemm<WT, false, 128>);
     else a.W2 ? go(k_moe_gemm<WT, true, 32>) : go(k_moe_gemm<WT, false, 32>);
