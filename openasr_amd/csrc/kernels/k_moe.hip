@@ -69,8 +69,7 @@ __global__ __launch_bounds__(256) void k_mul_mat_id_rows(mul_mat_id_args a) {
 // SwiGLU it stores) and the columns routed to it, 16 at a time; its waves
 // split K, their sums added through LDS in order. Bound by the weights'
 // stream: each wave reads its own, straight into the matrix cores' operand
-// layout (activations A, weights B: lane l ends with weight row l % 16 of the
-// columns 4 (l / 16) + i). The routing is done in place: workgroup y serves
+// layout (activations A, weights B: lane l ends with weight row l % 16). The routing is done in place: workgroup y serves
 // the expert of pair y if no earlier pair has it.
 constexpr int kMoeFew = 256;  // pairs a workgroup's threads hold
 
@@ -84,95 +83,123 @@ __device__ __forceinline__ moe_v8h moe_round8(const float * p) {
                    (_Float16) b.x, (_Float16) b.y, (_Float16) b.z, (_Float16) b.w};
 }
 
-// The 16 x 16 sums of one matrix's rows and 16 columns over wave w's share of
-// K, acc[i]: row r, column 4 g + i. bcol: the lane's own column (r) in b's
-// order, bc4: the columns 4 g + i.
-template <int WT>
+// The 16 x 16 sums of NM matrices' rows and 16 columns over wave w's share of
+// K. The operand's row r holds column r / 4 + 4 (r % 4), so that lane group g
+// ends with the columns g + 4 i, and few columns need the first i only (NCL of
+// them: with 4 always, the scaling of absent columns was most of the
+// instructions). bcol: the lane's operand column in b's order, bc4: the
+// columns g + 4 i.
+template <int WT, int NM>
 struct moe_tile;
 
-template <>
-struct moe_tile<GGML_TYPE_F16> {
-    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * wrow, int64_t bcol, const int (&)[4],
-                                               int wave, int waves, int g, double (&out)[4]) {
+template <int NM>
+struct moe_tile<GGML_TYPE_F16, NM> {
+    template <int NCL>
+    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * const (&wrow)[NM], int64_t bcol,
+                                               const int (&)[4], int wave, int waves, int g, double (&out)[NM][4]) {
         const float * x = (const float *) (a.b + (bcol % a.b_ne1) * a.b_nb1 + (bcol / a.b_ne1) * a.b_nb2);
         const int64_t steps = (a.K + 31) / 32;
-        moe_v4f acc = {0, 0, 0, 0};
+        moe_v4f acc[NM];
+#pragma unroll
+        for (int m = 0; m < NM; m++) acc[m] = moe_v4f{0, 0, 0, 0};
         constexpr int U = 4;  // steps in flight
         for (int64_t s0 = wave; s0 < steps; s0 += (int64_t) U * waves) {
-            uint4 w[U];
+            uint4 w[NM][U];
             moe_v8h xv[U];
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int64_t k = (s0 + (int64_t) u * waves) * 32 + 8 * g;
                 const bool ok = k < a.K;  // K % 8 == 0: eight at a time
-                w[u] = *(const uint4 *) (wrow + 2 * (ok ? k : 0));
+#pragma unroll
+                for (int m = 0; m < NM; m++) w[m][u] = *(const uint4 *) (wrow[m] + 2 * (ok ? k : 0));
                 xv[u] = moe_round8(x + (ok ? k : 0));
                 if (!ok) {
-                    w[u] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int m = 0; m < NM; m++) w[m][u] = make_uint4(0, 0, 0, 0);
                     xv[u] = moe_v8h{0, 0, 0, 0, 0, 0, 0, 0};
                 }
             }
 #pragma unroll
             for (int u = 0; u < U; u++)
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(xv[u], __builtin_bit_cast(moe_v8h, w[u]), acc, 0, 0, 0);
+#pragma unroll
+                for (int m = 0; m < NM; m++)
+                    acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xv[u], __builtin_bit_cast(moe_v8h, w[m][u]), acc[m], 0, 0, 0);
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) out[i] = acc[i];
+        for (int m = 0; m < NM; m++)
+#pragma unroll
+            for (int i = 0; i < NCL; i++) out[m][i] = acc[m][i];
     }
 };
 
-template <>
-struct moe_tile<GGML_TYPE_Q8_0> {
-    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * wrow, int64_t bcol, const int (&bc4)[4],
-                                               int wave, int waves, int g, double (&out)[4]) {
+template <int NM>
+struct moe_tile<GGML_TYPE_Q8_0, NM> {
+    template <int NCL>
+    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * const (&wrow)[NM], int64_t bcol,
+                                               const int (&bc4)[4], int wave, int waves, int g, double (&out)[NM][4]) {
         const int64_t nblk = a.K / 32;
-        const uint16_t * ds = (const uint16_t *) (wrow + a.K);
         const int8_t * aq = a.act.q + bcol * a.K;
-#pragma unroll
-        for (int i = 0; i < 4; i++) out[i] = 0.0;
         constexpr int U = 4;
         for (int64_t b0 = wave; b0 < nblk; b0 += (int64_t) U * waves) {
-            long q[U], af[U];
-            uint16_t d[U];
+            long q[NM][U], af[U];
+            uint16_t d[NM][U];
             float da[U][4];
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int64_t b = min(b0 + (int64_t) u * waves, nblk - 1);
-                q[u] = *(const long *) (wrow + 32 * b + 8 * g);
-                af[u] = *(const long *) (aq + 32 * b + 8 * g);
-                d[u] = ds[b];
 #pragma unroll
-                for (int i = 0; i < 4; i++) da[u][i] = a.act.d[bc4[i] * nblk + b];
+                for (int m = 0; m < NM; m++) {
+                    q[m][u] = *(const long *) (wrow[m] + 32 * b + 8 * g);
+                    d[m][u] = *(const uint16_t *) (wrow[m] + a.K + 2 * b);
+                }
+                af[u] = *(const long *) (aq + 32 * b + 8 * g);
+#pragma unroll
+                for (int i = 0; i < NCL; i++) da[u][i] = a.act.d[bc4[i] * nblk + b];
             }
 #pragma unroll
             for (int u = 0; u < U; u++)
-                if (b0 + (int64_t) u * waves < nblk) q8_0_block(af[u], q[u], d[u], da[u], out);
+                if (b0 + (int64_t) u * waves < nblk)
+#pragma unroll
+                    for (int m = 0; m < NM; m++) q8_0_block<NCL>(af[u], q[m][u], d[m][u], da[u], out[m]);
         }
     }
 };
 
-template <>
-struct moe_tile<GGML_TYPE_Q4_K> {
-    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * wrow, int64_t bcol, const int (&bc4)[4],
-                                               int wave, int waves, int g, double (&out)[4]) {
+template <int NM>
+struct moe_tile<GGML_TYPE_Q4_K, NM> {
+    template <int NCL>
+    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * const (&wrow)[NM], int64_t bcol,
+                                               const int (&bc4)[4], int wave, int waves, int g, double (&out)[NM][4]) {
         const int64_t nsb = a.K / 256;
         const int8_t * aq = a.act.q + bcol * a.K;
         const int16_t * ass = a.act.ssum + bcol * (a.K / 32);
-#pragma unroll
-        for (int i = 0; i < 4; i++) out[i] = 0.0;
-        for (int64_t b = wave; b < nsb; b += waves) {
-            const char * blk = wrow + b * 144;
-            const uint4 hdr = *(const uint4 *) blk;
-            long q[4], af[8];
-#pragma unroll
-            for (int c = 0; c < 4; c++) q[c] = *(const long *) (blk + 16 + 32 * c + 8 * g);
-#pragma unroll
-            for (int j = 0; j < 8; j++) af[j] = *(const long *) (aq + 256 * b + 32 * j + 8 * g);
+        struct block {
+            uint4 hdr[NM];
+            long q[NM][4], af[8];
             float ad[4], ssa[2];
+        };
+        auto load = [&](int64_t b, block & v) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) ad[i] = a.act.d[bc4[i] * nsb + b];
-            q4k_ssum_operand(ass + 8 * b, true, g, ssa);
-            q4k_unit(hdr, q, af, ad, ssa, out);
+            for (int m = 0; m < NM; m++) {
+                const char * blk = wrow[m] + b * 144;
+                v.hdr[m] = *(const uint4 *) blk;
+#pragma unroll
+                for (int c = 0; c < 4; c++) v.q[m][c] = *(const long *) (blk + 16 + 32 * c + 8 * g);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) v.af[j] = *(const long *) (aq + 256 * b + 32 * j + 8 * g);
+#pragma unroll
+            for (int i = 0; i < NCL; i++) v.ad[i] = a.act.d[bc4[i] * nsb + b];
+            q4k_ssum_operand(ass + 8 * b, true, g, v.ssa);
+        };
+        if (wave >= nsb) return;
+        block cur, next;  // a block ahead
+        load(wave, cur);
+        for (int64_t b = wave; b < nsb; b += waves) {
+            load(min(b + waves, nsb - 1), next);
+#pragma unroll
+            for (int m = 0; m < NM; m++) q4k_unit<NCL>(cur.hdr[m], cur.q[m], cur.af, cur.ad, cur.ssa, out[m]);
+            cur = next;
         }
     }
 };
@@ -209,20 +236,24 @@ __global__ __launch_bounds__(256) void k_moe_few(mul_mat_id_args a) {
     if (mine) s_list[at + __popcll(have & ((1ull << lane) - 1))] = tid;
     __syncthreads();
     const int64_t row = min(m0 + r, a.M - 1);
-    const char * w1 = a.W + e * a.W_nb2 + row * a.W_nb1;
-    const char * w2 = PAIR ? a.W2 + e * a.W_nb2 + row * a.W_nb1 : nullptr;
+    constexpr int NM = PAIR ? 2 : 1;
+    const char * wrow[NM];
+    wrow[0] = a.W + e * a.W_nb2 + row * a.W_nb1;
+    if constexpr (PAIR) wrow[1] = a.W2 + e * a.W_nb2 + row * a.W_nb1;
     auto column = [&](int p) { return (int) (p / a.used * a.b_ne1 + p % a.used % a.b_ne1); };
     for (int c0 = 0; c0 < n; c0 += 16) {
-        const int64_t bcol = column(s_list[min(c0 + r, n - 1)]);
+        const int64_t bcol = column(s_list[min(c0 + (r >> 2) + 4 * (r & 3), n - 1)]);
         int bc4[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) bc4[i] = column(s_list[min(c0 + 4 * g + i, n - 1)]);
-        double acc[2][4];
-        moe_tile<WT>::run(a, w1, bcol, bc4, wave, 4, g, acc[0]);
-        if constexpr (PAIR) moe_tile<WT>::run(a, w2, bcol, bc4, wave, 4, g, acc[1]);
+        for (int i = 0; i < 4; i++) bc4[i] = column(s_list[min(c0 + g + 4 * i, n - 1)]);
+        double acc[NM][4] = {};
+        using tile = moe_tile<WT, NM>;
+        if (n - c0 <= 4) tile::template run<1>(a, wrow, bcol, bc4, wave, 4, g, acc);
+        else if (n - c0 <= 8) tile::template run<2>(a, wrow, bcol, bc4, wave, 4, g, acc);
+        else tile::template run<4>(a, wrow, bcol, bc4, wave, 4, g, acc);
         if (wave > 0) {
 #pragma unroll
-            for (int m = 0; m < (PAIR ? 2 : 1); m++)
+            for (int m = 0; m < NM; m++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) s_acc[m][wave - 1][i][lane] = acc[m][i];
         }
@@ -231,10 +262,10 @@ __global__ __launch_bounds__(256) void k_moe_few(mul_mat_id_args a) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
 #pragma unroll
-                for (int m = 0; m < (PAIR ? 2 : 1); m++)
+                for (int m = 0; m < NM; m++)
 #pragma unroll
                     for (int w = 0; w < 3; w++) acc[m][i] += s_acc[m][w][i][lane];
-                const int c = c0 + 4 * g + i;
+                const int c = c0 + g + 4 * i;
                 if (c < n && m0 + r < a.M)
                     a.out[(int64_t) s_list[c] * a.M + m0 + r] =
                         PAIR ? moe_swiglu((float) acc[0][i], (float) acc[1][i]) : (float) acc[0][i];
