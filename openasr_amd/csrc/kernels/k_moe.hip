@@ -1,6 +1,7 @@
 // k_moe.hip -- the mixture-of-experts operators: GGML_OP_MUL_MAT_ID (each
 // column by the matrix of its own expert) and the router's GGML_OP_ARGSORT
 // and GGML_OP_SUM_ROWS.
+#include <algorithm>
 #include <type_traits>
 
 #include "../mfma_units.h"
@@ -968,66 +969,38 @@ __device__ __forceinline__ uint32_t sort_key(float v) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sorted ascending by (key, index); descending turns the keys' bits.
-// Short rows, a wave each: an element's place is the number of elements
-// before it, all keys against all from LDS.
-constexpr int kArgsortRank = 256;
-__global__ __launch_bounds__(256) void k_argsort_rank(tview d, tview a, uint32_t flip, int64_t rows) {
-    __shared__ __align__(16) uint32_t keys[4][kArgsortRank];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t want = (int64_t) blockIdx.x * 4 + wave, row = min(want, rows - 1);
-    const int64_t i1 = row % a.ne[1], i2 = row / a.ne[1] % a.ne[2], i3 = row / (a.ne[1] * a.ne[2]);
-    const float * x = (const float *) (a.data + i1 * a.nb[1] + i2 * a.nb[2] + i3 * a.nb[3]);
-    int32_t * o = (int32_t *) (d.data + i1 * d.nb[1] + i2 * d.nb[2] + i3 * d.nb[3]);
-    const int n = (int) a.ne[0];
-    constexpr int R = kArgsortRank / 64;
-    uint32_t key[R];
-    int at[R];
-#pragma unroll
-    for (int u = 0; u < R; u++) {
-        const int i = lane + 64 * u;
-        key[u] = i < n ? sort_key(x[i]) ^ flip : 0xFFFFFFFFu;  // (past the row: never before)
-        keys[wave][i] = key[u];
-        at[u] = 0;
-    }
-    __syncthreads();
-    for (int j = 0; j < n; j += 4) {
-        const uint4 q4 = *(const uint4 *) &keys[wave][j];
-        const uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-#pragma unroll
-            for (int u = 0; u < R; u++) at[u] += q[e] < key[u] || (q[e] == key[u] && j + e < lane + 64 * u);
-    }
-    if (want >= rows) return;
-#pragma unroll
-    for (int u = 0; u < R; u++)
-        if (lane + 64 * u < n) o[at[u]] = lane + 64 * u;
-}
-
-// longer rows, a workgroup each: a bitonic sort of 64-bit (key, index) in LDS
+// Sorted ascending by (key, index), descending turns the keys' bits: a
+// workgroup a row, a bitonic sort of 64-bit (key, index) in LDS. 4096 rows of
+// 128 take 10 us; counting each element's predecessors from LDS instead, a wave a
+// row, took 13 us there and 38 us for rows of 256 (here 18 us).
 constexpr int kArgsortMost = 8192;
-__global__ __launch_bounds__(1024) void k_argsort_bitonic(tview d, tview a, uint32_t flip, int size) {
-    __shared__ uint64_t k[kArgsortMost];
-    const int64_t row = blockIdx.x;
-    const int64_t i1 = row % a.ne[1], i2 = row / a.ne[1] % a.ne[2], i3 = row / (a.ne[1] * a.ne[2]);
-    const float * x = (const float *) (a.data + i1 * a.nb[1] + i2 * a.nb[2] + i3 * a.nb[3]);
-    int32_t * o = (int32_t *) (d.data + i1 * d.nb[1] + i2 * d.nb[2] + i3 * d.nb[3]);
-    const int n = (int) a.ne[0], tid = threadIdx.x;
-    for (int i = tid; i < size; i += 1024) k[i] = i < n ? (uint64_t) (sort_key(x[i]) ^ flip) << 32 | (uint32_t) i : ~0ull;
-    for (int run = 2; run <= size; run *= 2) {
-        for (int step = run / 2; step > 0; step /= 2) {
-            __syncthreads();
-            for (int i = tid; i < size / 2; i += 1024) {
-                const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-                const uint64_t u = k[lo], v = k[hi];
-                if ((u > v) == ((lo & run) == 0)) k[lo] = v, k[hi] = u;
+__global__ __launch_bounds__(1024) void k_argsort(tview d, tview a, uint32_t flip, int size, int64_t rows) {
+    extern __shared__ uint64_t k[];  // [size]
+    const int threads = (int) blockDim.x;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const int64_t i1 = row % a.ne[1], i2 = row / a.ne[1] % a.ne[2], i3 = row / (a.ne[1] * a.ne[2]);
+        const float * x = (const float *) (a.data + i1 * a.nb[1] + i2 * a.nb[2] + i3 * a.nb[3]);
+        int32_t * o = (int32_t *) (d.data + i1 * d.nb[1] + i2 * d.nb[2] + i3 * d.nb[3]);
+        const int n = (int) a.ne[0], tid = threadIdx.x;
+        for (int i = tid; i < size; i += threads) k[i] = i < n ? (uint64_t) (sort_key(x[i]) ^ flip) << 32 | (uint32_t) i : ~0ull;
+        for (int run = 2; run <= size; run *= 2) {
+            for (int step = run / 2; step > 0; step /= 2) {
+                __syncthreads();
+                for (int i = tid; i < size / 2; i += threads) {
+                    const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+                    const uint64_t u = k[lo], v = k[hi];
+                    if ((u > v) == ((lo & run) == 0)) k[lo] = v, k[hi] = u;
+                }
             }
         }
+        __syncthreads();
+        for (int i = tid; i < n; i += threads) o[i] = (int32_t) (uint32_t) k[i];
+        __syncthreads();
     }
-    __syncthreads();
-    for (int i = tid; i < n; i += 1024) o[i] = (int32_t) (uint32_t) k[i];
 }
+
+// workgroups of four rows, each in turn where there are more
+static unsigned row_blocks(int64_t rows) { return (unsigned) std::min<int64_t>((rows + 3) / 4, 1 << 22); }
 
 bool argsort_supported(int64_t n) { return n >= 0 && n <= kArgsortMost; }
 
@@ -1035,13 +1008,10 @@ void launch_argsort(const tview & d, const tview & a, int desc, hipStream_t s) {
     const int64_t rows = a.ne[1] * a.ne[2] * a.ne[3];
     if (rows == 0 || a.ne[0] == 0) return;
     const uint32_t flip = desc ? 0xFFFFFFFFu : 0;
-    if (a.ne[0] <= kArgsortRank) {
-        hipLaunchKernelGGL(k_argsort_rank, dim3((unsigned) ((rows + 3) / 4)), dim3(256), 0, s, d, a, flip, rows);
-        return;
-    }
-    int size = 2 * kArgsortRank;
+    int size = 2;
     while (size < a.ne[0]) size *= 2;
-    hipLaunchKernelGGL(k_argsort_bitonic, dim3((unsigned) rows), dim3(1024), 0, s, d, a, flip, size);
+    hipLaunchKernelGGL(k_argsort, dim3((unsigned) std::min<int64_t>(rows, 1 << 20)), dim3(std::min(1024, std::max(64, size / 2))),
+                       (size_t) size * 8, s, d, a, flip, size, rows);
 }
 
 // ------------------------------------------------------------ a router ---
@@ -1066,49 +1036,50 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 template <int V>
 __global__ __launch_bounds__(256) void k_top_k(top_k_args a) {
     const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t) blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (row >= a.rows) return;
-    const float * x = (const float *) (a.x + row * a.x_nb1);
-    uint32_t key[V], most = 0;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int64_t row = (int64_t) blockIdx.x * 4 + wave; row < a.rows; row += (int64_t) gridDim.x * 4) {
+        const float * x = (const float *) (a.x + row * a.x_nb1);
+        uint32_t key[V], most = 0;
 #pragma unroll
-    for (int v = 0; v < V; v++) {
-        const int i = lane * V + v;
-        key[v] = i < a.n ? sort_key(x[i]) : 0;  // (no value has the key 0)
-        most = max(most, key[v]);
-    }
-    int mine = 0;
-    for (int j = 0; j < a.k; j++) {
-        const uint32_t top = wave_max_u32(most);
-        const int from = __ffsll((unsigned long long) __ballot(most == top)) - 1;
-        int at = 0;
-        if (lane == from) {
-            most = 0;
-            bool taken = false;
-#pragma unroll
-            for (int v = 0; v < V; v++) {
-                if (!taken && key[v] == top) {
-                    taken = true;
-                    at = v;
-                    key[v] = 0;
-                }
-                most = max(most, key[v]);
-            }
+        for (int v = 0; v < V; v++) {
+            const int i = lane * V + v;
+            key[v] = i < a.n ? sort_key(x[i]) : 0;  // (no value has the key 0)
+            most = max(most, key[v]);
         }
-        at = __builtin_amdgcn_readlane(at, from);
-        if (lane == j) mine = from * V + at;
+        int mine = 0;
+        for (int j = 0; j < a.k; j++) {
+            const uint32_t top = wave_max_u32(most);
+            const int from = __ffsll((unsigned long long) __ballot(most == top)) - 1;
+            int at = 0;
+            if (lane == from) {
+                most = 0;
+                bool taken = false;
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    if (!taken && key[v] == top) {
+                        taken = true;
+                        at = v;
+                        key[v] = 0;
+                    }
+                    most = max(most, key[v]);
+                }
+            }
+            at = __builtin_amdgcn_readlane(at, from);
+            if (lane == j) mine = from * V + at;
+        }
+        if (lane < a.k) *(int32_t *) (a.ids + row * a.ids_nb1 + 4 * lane) = mine;
+        if (!a.out) continue;
+        const float w = lane < a.k ? x[mine] : 0.0f;
+        float y = w;
+        if (a.mode == kTopKSoftMax) {
+            const float z = w * a.scale + 0.0f, mx = wave_max(lane < a.k ? z : -INFINITY);
+            const float e = lane < a.k ? expf_det(z - mx) : 0.0f;
+            y = e * (float) (1.0 / wave_sum_d((double) e));
+        } else if (a.mode == kTopKShares) {
+            y = w / (float) wave_sum_d((double) w);
+        }
+        if (lane < a.k) a.out[row * a.k + lane] = y;
     }
-    if (lane < a.k) *(int32_t *) (a.ids + row * a.ids_nb1 + 4 * lane) = mine;
-    if (!a.out) return;
-    const float w = lane < a.k ? x[mine] : 0.0f;
-    float y = w;
-    if (a.mode == kTopKSoftMax) {
-        const float z = w * a.scale + 0.0f, mx = wave_max(lane < a.k ? z : -INFINITY);
-        const float e = lane < a.k ? expf_det(z - mx) : 0.0f;
-        y = e * (float) (1.0 / wave_sum_d((double) e));
-    } else if (a.mode == kTopKShares) {
-        y = w / (float) wave_sum_d((double) w);
-    }
-    if (lane < a.k) a.out[row * a.k + lane] = y;
 }
 
 bool top_k_supported(int64_t n, int64_t k) { return n >= 1 && n <= 1024 && k >= 1 && k <= 32 && k <= n; }
@@ -1116,7 +1087,7 @@ bool top_k_supported(int64_t n, int64_t k) { return n >= 1 && n <= 1024 && k >= 
 void launch_top_k(const top_k_args & a, hipStream_t s) {
     if (a.rows == 0) return;
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned) ((a.rows + 3) / 4)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(kernel, dim3(row_blocks(a.rows)), dim3(256), 0, s, a);
     };
     if (a.n <= 64) go(k_top_k<1>);
     else if (a.n <= 128) go(k_top_k<2>);
@@ -1128,20 +1099,20 @@ void launch_top_k(const top_k_args & a, hipStream_t s) {
 // one wave a row, the sum held in double
 __global__ __launch_bounds__(256) void k_sum_rows(tview d, tview a, int64_t rows) {
     const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const int64_t i1 = row % a.ne[1], i2 = row / a.ne[1] % a.ne[2], i3 = row / (a.ne[1] * a.ne[2]);
-    const float * x = (const float *) (a.data + i1 * a.nb[1] + i2 * a.nb[2] + i3 * a.nb[3]);
-    double sum = 0.0;
-    for (int64_t i = lane; i < a.ne[0]; i += 64) sum += (double) x[i];
-    sum = wave_sum_d(sum);
-    if (lane == 0) *(float *) (d.data + i1 * d.nb[1] + i2 * d.nb[2] + i3 * d.nb[3]) = (float) sum;
+    for (int64_t row = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (int64_t) gridDim.x * 4) {
+        const int64_t i1 = row % a.ne[1], i2 = row / a.ne[1] % a.ne[2], i3 = row / (a.ne[1] * a.ne[2]);
+        const float * x = (const float *) (a.data + i1 * a.nb[1] + i2 * a.nb[2] + i3 * a.nb[3]);
+        double sum = 0.0;
+        for (int64_t i = lane; i < a.ne[0]; i += 64) sum += (double) x[i];
+        sum = wave_sum_d(sum);
+        if (lane == 0) *(float *) (d.data + i1 * d.nb[1] + i2 * d.nb[2] + i3 * d.nb[3]) = (float) sum;
+    }
 }
 
 void launch_sum_rows(const tview & d, const tview & a, hipStream_t s) {
     const int64_t rows = a.ne[1] * a.ne[2] * a.ne[3];
     if (rows == 0) return;
-    hipLaunchKernelGGL(k_sum_rows, dim3((unsigned) ((rows + 3) / 4)), dim3(256), 0, s, d, a, rows);
+    hipLaunchKernelGGL(k_sum_rows, dim3(row_blocks(rows)), dim3(256), 0, s, d, a, rows);
 }
 
 }  // namespace mi355x

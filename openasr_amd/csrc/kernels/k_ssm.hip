@@ -211,46 +211,46 @@ __device__ __forceinline__ float ssm_softplus(float v) {
     return fmaxf(v, 0.0f) + fmaf(t, p * w, t);
 }
 
-// token by token: W lanes hold one (sequence, head, channel) row's state, R
-// elements a lane
-template <int W, int R>
+// token by token: a wave holds one (sequence, head, channel) row's state, R
+// elements a lane (any n and alignment)
+template <int R>
 __global__ __launch_bounds__(256) void k_ssm_scan_rows(ssm_scan_args a) {
-    const int lane = threadIdx.x % W;
-    const int64_t row = ((int64_t) blockIdx.x * 256 + threadIdx.x) / W;
+    const int lane = threadIdx.x & 63;
     const int64_t rows = (int64_t) a.seqs * a.heads * a.dim;
-    if (row >= rows) return;  // whole groups of W lanes
-    const int p = (int) (row % a.dim), h = (int) (row / a.dim % a.heads), s = (int) (row / ((int64_t) a.dim * a.heads));
-    const int g = h / (a.heads / a.groups);
-    const int64_t slot = a.ids[s];
-    const bool has = slot >= 0 && slot < a.slots;
-    const float * s0 = (const float *) (a.s + (has ? slot : 0) * a.s_nb3) + ((int64_t) h * a.dim + p) * a.n;
-    float st[R], av[R];
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-        const int k = lane + W * r;
-        st[r] = has && k < a.n ? s0[k] : 0.0f;
-        av[r] = k < a.n ? *(const float *) (a.A + h * a.A_nb1 + (a.a_elem ? 4 * k : 0)) : 0.0f;
-    }
-    for (int64_t t = 0; t < a.tokens; t++) {
-        const float dt = ssm_softplus(*(const float *) (a.dt + 4 * h + t * a.dt_nb1 + s * a.dt_nb2));
-        const float xv = *(const float *) (a.x + 4 * p + h * a.x_nb1 + t * a.x_nb2 + s * a.x_nb3) * dt;
-        const float * b = (const float *) (a.B + g * a.B_nb1 + t * a.B_nb2 + s * a.B_nb3);
-        const float * c = (const float *) (a.C + g * a.C_nb1 + t * a.C_nb2 + s * a.C_nb3);
-        float y = 0.0f;
+    for (int64_t row = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (int64_t) gridDim.x * 4) {
+        const int p = (int) (row % a.dim), h = (int) (row / a.dim % a.heads), s = (int) (row / ((int64_t) a.dim * a.heads));
+        const int g = h / (a.heads / a.groups);
+        const int64_t slot = a.ids[s];
+        const bool has = slot >= 0 && slot < a.slots;
+        const float * s0 = (const float *) (a.s + (has ? slot : 0) * a.s_nb3) + ((int64_t) h * a.dim + p) * a.n;
+        float st[R], av[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const int k = lane + W * r;
-            const bool ok = k < a.n;
-            st[r] = fmaf(st[r], expf(dt * av[r]), ok ? xv * b[k] : 0.0f);
-            y = fmaf(st[r], ok ? c[k] : 0.0f, y);
+            const int k = lane + 64 * r;
+            st[r] = has && k < a.n ? s0[k] : 0.0f;
+            av[r] = k < a.n ? *(const float *) (a.A + h * a.A_nb1 + (a.a_elem ? 4 * k : 0)) : 0.0f;
         }
-        y = group_sum<W>(y);
-        if (lane == 0) a.y[((s * a.tokens + t) * a.heads + h) * a.dim + p] = y;
-    }
+        for (int64_t t = 0; t < a.tokens; t++) {
+            const float dt = ssm_softplus(*(const float *) (a.dt + 4 * h + t * a.dt_nb1 + s * a.dt_nb2));
+            const float xv = *(const float *) (a.x + 4 * p + h * a.x_nb1 + t * a.x_nb2 + s * a.x_nb3) * dt;
+            const float * b = (const float *) (a.B + g * a.B_nb1 + t * a.B_nb2 + s * a.B_nb3);
+            const float * c = (const float *) (a.C + g * a.C_nb1 + t * a.C_nb2 + s * a.C_nb3);
+            float y = 0.0f;
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        const int k = lane + W * r;
-        if (k < a.n) a.out[row * a.n + k] = st[r];
+            for (int r = 0; r < R; r++) {
+                const int k = lane + 64 * r;
+                const bool ok = k < a.n;
+                st[r] = fmaf(st[r], expf(dt * av[r]), ok ? xv * b[k] : 0.0f);
+                y = fmaf(st[r], ok ? c[k] : 0.0f, y);
+            }
+            y = wave_sum(y);
+            if (lane == 0) a.y[((s * a.tokens + t) * a.heads + h) * a.dim + p] = y;
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int k = lane + 64 * r;
+            if (k < a.n) a.out[row * a.n + k] = st[r];
+        }
     }
 }
 
@@ -1353,22 +1353,21 @@ void launch_ssm_scan(const ssm_scan_args & a, void * scratch, hipStream_t s, int
     if (rows == 0) return;
     if (ssm_chunked(a)) return launch_ssm_chunks(a, scratch, s, n_cu);
     if (ssm_lanes(a)) return launch_ssm_lanes(a, scratch, s, n_cu);
-    if (ssm_pieces(a)) {
-        auto go = [&](auto kernel, int per) {  // rows of a head a wave
-            const int64_t waves = (a.dim + per - 1) / per * (int64_t) a.heads * a.seqs;
-            hipLaunchKernelGGL(kernel, dim3((unsigned) ((waves + 3) / 4)), dim3(256), 0, s, a);
-        };
-        if (a.n <= 64) go(k_ssm_scan_pieces<16, 4>, 16);
-        else if (a.n <= 128) go(k_ssm_scan_pieces<32, 8>, 16);
-        else go(k_ssm_scan_pieces<64, 8>, 8);
+    const int per = a.n <= 128 ? 16 : 8;  // rows of a head a wave of k_ssm_scan_pieces takes
+    const int64_t waves = (a.dim + per - 1) / per * (int64_t) a.heads * a.seqs;
+    if (ssm_pieces(a) && waves <= 1 << 25) {  // (the other form's grid may be shorter than its rows)
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned) ((waves + 3) / 4)), dim3(256), 0, s, a); };
+        if (a.n <= 64) go(k_ssm_scan_pieces<16, 4>);
+        else if (a.n <= 128) go(k_ssm_scan_pieces<32, 8>);
+        else go(k_ssm_scan_pieces<64, 8>);
         return;
     }
-    auto go = [&](auto kernel, int w) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned) ((rows * w + 255) / 256)), dim3(256), 0, s, a);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned) std::min<int64_t>((rows + 3) / 4, 1 << 22)), dim3(256), 0, s, a);
     };
-    if (a.n <= 64) go(k_ssm_scan_rows<64, 1>, 64);
-    else if (a.n <= 128) go(k_ssm_scan_rows<64, 2>, 64);
-    else go(k_ssm_scan_rows<64, 4>, 64);
+    if (a.n <= 64) go(k_ssm_scan_rows<1>);
+    else if (a.n <= 128) go(k_ssm_scan_rows<2>);
+    else go(k_ssm_scan_rows<4>);
 }
 
 }  // namespace mi355x

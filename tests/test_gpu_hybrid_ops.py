@@ -533,6 +533,24 @@ def test_mul_mat_id(ggml, gpu, ref, wname, E, k, M, K, T, how, slots):
     G.free()
 
 
+# the borders between the forms: 256 pairs, 24 pairs an expert, K in part steps
+# and part groups of scales, more experts than the wide form sorts
+BORDERS = [(8, 4, 40, 96, 64), (8, 4, 40, 96, 65), (12, 4, 130, 160, 71), (12, 4, 130, 160, 72), (3, 1, 70, 1120, 300),
+           (1000, 2, 16, 64, 200), (960, 2, 16, 64, 200), (1, 1, 129, 320, 257), (5, 5, 65, 224, 120)]
+
+
+@pytest.mark.parametrize("wname", ["f16", "q8_0"])
+@pytest.mark.parametrize("E,k,M,K,T", BORDERS)
+@pytest.mark.parametrize("how", ["spread", "outside"])
+def test_mul_mat_id_borders(ggml, gpu, ref, wname, E, k, M, K, T, how):
+    test_mul_mat_id(ggml, gpu, ref, wname, E, k, M, K, T, how, how == "outside")
+
+
+@pytest.mark.parametrize("E,k,M,K,T", [(4, 2, 48, 768, 65), (3, 2, 200, 256, 300), (2, 1, 140, 1280, 290)])
+def test_mul_mat_id_borders_of_super_blocks(ggml, gpu, ref, E, k, M, K, T):
+    test_mul_mat_id(ggml, gpu, ref, "q4_K", E, k, M, K, T, "twice", True)
+
+
 @pytest.mark.parametrize("M,K", [(77, 100), (33, 7), (130, 1000), (64, 1)])
 @pytest.mark.parametrize("wname,T", [("f16", 2), ("f16", 90), ("f32", 90)])
 def test_mul_mat_id_odd_rows(ggml, gpu, ref, wname, M, K, T):
@@ -796,6 +814,43 @@ def test_router_variants(ggml, gpu, case):
 @pytest.mark.parametrize("desc", [0, 1])
 def test_argsort_lengths(ggml, gpu, n, rows, desc):
     test_argsort(ggml, gpu, n, rows, desc)
+
+
+def test_graphs_that_share_a_workspace(ggml, gpu, ref):
+    """a scan in segments and a wide experts' product, each in its own graph on
+    one backend, computed in turn until both are captured and replayed"""
+    rng = np.random.default_rng(11)
+    S, T, H, P, n = 1, 700, 3, 64, 128
+    a = scan_inputs(rng, S, T, H, P, 1, n, False, S)
+    E, k, M, K, N = 8, 2, 96, 256, 150
+    raw, w = expert_weights(ggml, ref, rng, ggml.F16, E, M, K)
+    x = rng.standard_normal((N, 1, K)).astype(np.float32)
+    ids = routes(rng, N, E, k, "spread")
+    G1, G2 = ggml.Graph(64, 64), ggml.Graph(64, 64)
+    arrays = [(a[0], (n, P, H, S)), (a[1], (P, H, T, S)), (a[2], (H, T, S)), (a[3], (1, H)), (a[4], (n, 1, T, S)),
+              (a[5], (n, 1, T, S)), (np.zeros(1, np.int32), (S,))]
+    t = [G1.new(ggml.I32 if v.dtype == np.int32 else ggml.F32, *ne) for v, ne in arrays]
+    y1 = G1.lib.ggml_ssm_scan(G1.ctx, *t)
+    G1.build(y1)
+    G1.allocate(gpu.buft)
+    for q, (v, _) in zip(t, arrays):
+        G1.set(q, v)
+    W, X, I = G2.new(ggml.F16, K, M, E, weight=True), G2.new(ggml.F32, K, 1, N), G2.new(ggml.I32, k, N)
+    y2 = G2.lib.ggml_mul_mat_id(G2.ctx, W, X, I)
+    G2.build(y2)
+    G2.allocate(gpu.buft)
+    for q, v in ((W, raw), (X, x), (I, ids)):
+        G2.set(q, v)
+    wy, by, wh, bh = scan64(*a, [0])
+    want, m = experts64(w, columns(ggml, ref, ggml.F16, x), ids)
+    for _ in range(4):
+        assert G1.compute(gpu.backend) == 0 and G2.compute(gpu.backend) == 0
+        out = G1.get(y1).reshape(-1)
+        within(out[:a[1].size].reshape(a[1].shape), wy, by, "y")
+        within(out[a[1].size:].reshape(wh.shape), wh, bh, "states")
+        within(G2.get(y2).reshape(N, k, M), want, roundings(K) * U * m + 1e-37, "experts")
+    G1.free()
+    G2.free()
 
 
 # ------------------------------------------------------ memory of others ---
