@@ -878,18 +878,28 @@ static bool moe_aligned(int wtype, const mul_mat_id_args & a) {
     return wtype == GGML_TYPE_Q8_0 || (wtype == GGML_TYPE_Q4_K && (w & 15) == 0);
 }
 
+// Up to how many pairs the streaming form is the faster one. 64 experts, 768 x
+// 1024 weights, SwiGLU pairs, with the call, streaming / wide: f16 128 pairs
+// 48 / 52 us, 256 55 / 54; Q4_K 32 pairs 26 / 38, 256 52 / 63; Q8_0 (whose
+// blocks' scales it applies one by one) 32 pairs 38 / 38, 48 41 / 39, 128 65 / 57.
+static int moe_few_pairs(int wtype) { return wtype == GGML_TYPE_Q8_0 ? 32 : kMoeFew; }
+
 bool mul_mat_id_wide(int wtype, const mul_mat_id_args & a) {
-    return moe_aligned(wtype, a) && a.pairs > kMoeFew && a.experts <= 960 && a.pairs < 1 << 26 &&
+    return moe_aligned(wtype, a) && a.pairs > moe_few_pairs(wtype) && a.experts <= 960 && a.pairs < 1 << 26 &&
            (a.K + 63) / 64 * 64 * a.b_ne1 * (a.pairs / a.used) < 1ll << 31;
 }
 
-bool mul_mat_id_pairs(int wtype, const mul_mat_id_args & a) {
-    return moe_aligned(wtype, a) && (a.pairs <= kMoeFew || mul_mat_id_wide(wtype, a));
+static bool moe_few(int wtype, const mul_mat_id_args & a) {
+    return moe_aligned(wtype, a) && a.pairs <= kMoeFew && !mul_mat_id_wide(wtype, a);
 }
+
+bool mul_mat_id_pairs(int wtype, const mul_mat_id_args & a) { return moe_few(wtype, a) || mul_mat_id_wide(wtype, a); }
 
 static size_t moe_carve(int wtype, const mul_mat_id_args & a, moe_wide_args & q, char * base) {
     q.a = a;
-    q.bn = a.pairs >= 24 * a.experts ? 128 : 32;
+    // (32 experts, 768 x 1024, pairs an expert: f16 16 28 / 32 us with 32 / 128
+    // columns; 32 of all types 1 or 2 us for 32; 48 Q4_K 56 / 50, the others even)
+    q.bn = a.pairs >= 40 * a.experts ? 128 : 32;
     q.kp = (a.K + 63) / 64 * 64;
     q.bcols = a.b_ne1 * (a.pairs / a.used);
     q.row_tiles = (a.M + (a.W2 ? 64 : 128) - 1) / (a.W2 ? 64 : 128);
@@ -939,7 +949,7 @@ void launch_mul_mat_id(int wtype, const mul_mat_id_args & a, void * scratch, hip
         else launch_moe_wide<GGML_TYPE_F16>(a, (char *) scratch, s);
         return;
     }
-    if (moe_aligned(wtype, a) && a.pairs <= kMoeFew) {
+    if (moe_few(wtype, a)) {
         const dim3 grid((unsigned) ((a.M + 15) / 16), (unsigned) a.pairs);
         auto go = [&](auto one, auto pair) {
             if (a.W2) hipLaunchKernelGGL(pair, grid, dim3(256), 0, s, a);

@@ -533,10 +533,11 @@ def test_mul_mat_id(ggml, gpu, ref, wname, E, k, M, K, T, how, slots):
     G.free()
 
 
-# the borders between the forms: 256 pairs, 24 pairs an expert, K in part steps
+# the borders between the forms: 32 and 256 pairs, 24 and 40 pairs an expert, K in part steps
 # and part groups of scales, more experts than the wide form sorts
 BORDERS = [(8, 4, 40, 96, 64), (8, 4, 40, 96, 65), (12, 4, 130, 160, 71), (12, 4, 130, 160, 72), (3, 1, 70, 1120, 300),
-           (1000, 2, 16, 64, 200), (960, 2, 16, 64, 200), (1, 1, 129, 320, 257), (5, 5, 65, 224, 120)]
+           (1000, 2, 16, 64, 200), (960, 2, 16, 64, 200), (1, 1, 129, 320, 257), (5, 5, 65, 224, 120),
+           (8, 4, 40, 96, 8), (8, 3, 40, 96, 11), (1000, 2, 16, 64, 50), (10, 4, 40, 128, 99), (10, 4, 40, 128, 100)]
 
 
 @pytest.mark.parametrize("wname", ["f16", "q8_0"])
