@@ -9,6 +9,8 @@
 
 namespace mi355x {
 
+typedef float ssm_v4f __attribute__((ext_vector_type(4)));
+
 // ---------------------------------------------------------------- conv ---
 
 // y[c, t, s] = silu(bias[c] + sum_j w[j, c] col[t + j, c, s]): every column is
@@ -27,7 +29,9 @@ __device__ __forceinline__ float ssm_conv_end(const ssm_conv_args & a, float v, 
 // half the waves, 40; 8 with 4, more columns read twice, 32.)
 // The lane with a channel's first token alone reads its carried columns, so it
 // may write the ones carried on over them.
-template <int TAPS, int NC, int U>
+// PACKED (NC 4): four channels' taps and carried columns come in whole 16-byte
+// pieces (one token of 32 streams: 5.3 us, element by element 7.3).
+template <int TAPS, int NC, int U, bool PACKED>
 __global__ __launch_bounds__(256) void k_ssm_conv_rows(ssm_conv_args a, int run) {
     const int lane = threadIdx.x & 63;
     const int64_t cgroups = (a.channels + 64 * NC - 1) / (64 * NC), runs = (a.tokens + run - 1) / run;
@@ -38,13 +42,20 @@ __global__ __launch_bounds__(256) void k_ssm_conv_rows(ssm_conv_args a, int run)
         if (c >= a.channels) continue;
         typedef float vec __attribute__((ext_vector_type(NC)));
         float w[TAPS][NC], bias[NC];
+        if constexpr (PACKED) {
+            ssm_v4f v[TAPS];
 #pragma unroll
-        for (int e = 0; e < NC; e++) {
-            const float * wc = (const float *) (a.w + (c + e) * a.w_nb1);
+            for (int j = 0; j < TAPS; j++) v[j] = ((const ssm_v4f *) (a.w + c * a.w_nb1))[j];
 #pragma unroll
-            for (int j = 0; j < TAPS; j++) w[j][e] = wc[j];
-            bias[e] = a.bias ? a.bias[c + e] : 0.0f;
+            for (int i = 0; i < NC * TAPS; i++) w[i % TAPS][i / TAPS] = v[i / 4][i % 4];
+        } else {
+#pragma unroll
+            for (int e = 0; e < NC; e++)
+#pragma unroll
+                for (int j = 0; j < TAPS; j++) w[j][e] = ((const float *) (a.w + (c + e) * a.w_nb1))[j];
         }
+#pragma unroll
+        for (int e = 0; e < NC; e++) bias[e] = a.bias ? a.bias[c + e] : 0.0f;
         const char * x = a.x + c * a.x_nb1 + s * a.x_nb2;
         const char * st = a.st + c * a.st_nb1 + s * a.st_nb2;
         auto column = [&](int64_t i) {  // of x
@@ -54,9 +65,18 @@ __global__ __launch_bounds__(256) void k_ssm_conv_rows(ssm_conv_args a, int run)
             return v;
         };
         vec win[TAPS - 1];
+        const bool packed = PACKED && a.lead > 0 && t0 == 0;
+        if (packed) {
+            ssm_v4f v[TAPS - 1];
+#pragma unroll
+            for (int j = 0; j < TAPS - 1; j++) v[j] = ((const ssm_v4f *) st)[j];
+#pragma unroll
+            for (int i = 0; i < NC * (TAPS - 1); i++) win[i % (TAPS - 1)][i / (TAPS - 1)] = v[i / 4][i % 4];
+        }
 #pragma unroll
         for (int j = 0; j < TAPS - 1; j++) {
             const int64_t i = t0 + j;
+            if (packed) continue;
             if (i < a.lead) {
 #pragma unroll
                 for (int e = 0; e < NC; e++) win[j][e] = *(const float *) (st + e * a.st_nb1 + i * a.st_nb0);
@@ -74,11 +94,19 @@ __global__ __launch_bounds__(256) void k_ssm_conv_rows(ssm_conv_args a, int run)
                     for (int k = 1; k < TAPS - 1; k++)
                         if (a.tokens + j == k) on[j] = win[k];
             }
+            if constexpr (PACKED) {
+                ssm_v4f v[TAPS - 1];
 #pragma unroll
-            for (int j = 0; j < TAPS - 1; j++)
+                for (int i = 0; i < NC * (TAPS - 1); i++) v[i / 4][i % 4] = on[i % (TAPS - 1)][i / (TAPS - 1)];
 #pragma unroll
-                for (int e = 0; e < NC; e++)
-                    *(float *) (a.carry + (c + e) * a.c_nb1 + j * a.c_nb0 + s * a.c_nb2) = on[j][e];
+                for (int j = 0; j < TAPS - 1; j++) ((ssm_v4f *) (a.carry + c * a.c_nb1 + s * a.c_nb2))[j] = v[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < TAPS - 1; j++)
+#pragma unroll
+                    for (int e = 0; e < NC; e++)
+                        *(float *) (a.carry + (c + e) * a.c_nb1 + j * a.c_nb0 + s * a.c_nb2) = on[j][e];
+            }
         }
         float * out = a.out + (s * a.tokens) * a.channels + c;
         vec next[U];
@@ -167,8 +195,13 @@ static void launch_conv_rows(const ssm_conv_args & a, hipStream_t s) {
     const int64_t units = (a.channels + 64 * nc - 1) / (64 * nc) * ((a.tokens + run - 1) / run) * a.seqs;
     const dim3 grid((unsigned) std::min<int64_t>((units + 3) / 4, 1 << 22));
     auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(256), 0, s, a, run); };
-    if (a.tokens < 4) vec ? go(k_ssm_conv_rows<TAPS, 4, 1>) : go(k_ssm_conv_rows<TAPS, 1, 1>);
-    else vec ? go(k_ssm_conv_rows<TAPS, 4, 4>) : go(k_ssm_conv_rows<TAPS, 1, 4>);
+    auto pieces = [](const char * p, int64_t nb0, int64_t nb1, int64_t nb2, int n) {  // rows of n, one after another
+        return p == nullptr || (nb0 == 4 && nb1 == 4 * n && nb2 % 16 == 0 && (uintptr_t) p % 16 == 0);
+    };
+    const bool packed = vec && pieces(a.w, 4, a.w_nb1, 0, TAPS) && pieces(a.st, a.st_nb0, a.st_nb1, a.st_nb2, TAPS - 1) &&
+                        pieces(a.carry, a.c_nb0, a.c_nb1, a.c_nb2, TAPS - 1);
+    if (a.tokens < 4) packed ? go(k_ssm_conv_rows<TAPS, 4, 1, true>) : vec ? go(k_ssm_conv_rows<TAPS, 4, 1, false>) : go(k_ssm_conv_rows<TAPS, 1, 1, false>);
+    else packed ? go(k_ssm_conv_rows<TAPS, 4, 4, true>) : vec ? go(k_ssm_conv_rows<TAPS, 4, 4, false>) : go(k_ssm_conv_rows<TAPS, 1, 4, false>);
 }
 
 void launch_ssm_conv(const ssm_conv_args & a, hipStream_t s) {
@@ -187,8 +220,6 @@ void launch_ssm_conv(const ssm_conv_args & a, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------- scan ---
-
-typedef float ssm_v4f __attribute__((ext_vector_type(4)));
 
 // softplus as the op defines it, the identity past 20: max(v, 0) + log(1 + z),
 // z = exp(-|v|), and log(1 + z) = 2 atanh(s), s = z / (2 + z) <= 1/3, by its
@@ -257,7 +288,8 @@ __global__ __launch_bounds__(256) void k_ssm_scan_rows(ssm_scan_args a) {
 // The same with 16-byte pieces: W lanes hold a row's state, four elements a
 // lane, and a wave 64 U / W rows of one head at once. One token reads and
 // writes every state once, which bounds it: all rows' loads are in flight
-// together, beside the token's operands.
+// together, beside the token's operands (48 sequences of 80 x 64 x 128 states,
+// 252 MB: 46 us, 5.5 TB/s; an element a lane, 145 us).
 template <int W, int U>
 __global__ __launch_bounds__(256) void k_ssm_scan_pieces(ssm_scan_args a) {
     constexpr int kRows = 64 / W;  // of one load
@@ -335,7 +367,9 @@ __global__ __launch_bounds__(256) void k_ssm_scan_pieces(ssm_scan_args a) {
 // state and token bounds it, so the tokens are cut into segments until there
 // are waves enough: the first pass (OUT false) makes each segment's own state
 // from zeros and its sum of steps D, and the second starts from the earlier
-// segments' states, each decayed by exp(A D) as a whole.
+// segments' states, each decayed by exp(A D) as a whole. (5120 channels of 16,
+// 1000 tokens: 32 + 49 us, of which the 82 M exponentials of a pass are 8 and
+// its other instructions 20; a row's 16 states on 16 lanes, unsegmented, 1040.)
 struct ssm_lane_args {
     ssm_scan_args a;
     float * part;  // [segment][n states, D][row of (sequence, head, channel)]
