@@ -537,6 +537,11 @@ __global__ __launch_bounds__(256) void k_ssm_scan_lanes(ssm_lane_args q) {
 // f32's own roundings; states, decays and sums are f32, the log decays f64
 // until they are split into whole and fractional powers of two.
 //
+// 2 x 2048 tokens of 80 heads of 64 x 128: 110 us and 41 for the first pass,
+// bound by the vector instructions around the products (965 a wave and chunk:
+// scales, halves, decays; the products, three for each, are 40 GFLOP: 37 us at
+// a large product's rate), and 11 for the shared operands. 333 tokens of 24 x 64 x 64: 14 + 6 + 7 us.
+//
 // k_ssm_split makes the operands that a group's heads share: C in rows and B
 // in columns, split, with their scales, and C_t . B_j. k_ssm_chunks gives a
 // workgroup a (sequence, head, 64 channels, segment of chunks): wave w owns
@@ -1267,10 +1272,12 @@ bool ssm_scan_supported(int64_t n) { return n >= 1 && n <= 256; }
 
 static size_t ssm_al(size_t v) { return (v + 255) / 256 * 256; }
 
-// the chunked form takes a decay a head over enough tokens, channels and
-// state elements to fill its tiles
+// The chunked form takes a decay a head over enough tokens, channels and state
+// elements to fill its tiles. 80 heads of 64 x 128, with the call, chunked /
+// token by token: one sequence 8 tokens 33 / 31 us, 12 33 / 40, 64 32 / 147;
+// 16 sequences 12 tokens 83 / 79 us, 16 83 / 97, 64 83 / 309.
 static bool ssm_chunked(const ssm_scan_args & a) {
-    return !a.a_elem && a.tokens >= 16 && a.dim >= 16 && a.n >= 16 &&
+    return !a.a_elem && a.tokens >= 12 && a.dim >= 16 && a.n >= 16 &&
            (int64_t) a.heads * a.dim < 1 << 22;  // (a chunk's rows of y in 32-bit offsets)
 }
 

@@ -333,7 +333,8 @@ def test_ssm_scan_keeps_non_finite_values_where_they_are(ggml, gpu, T, what):
 PIECES = [(1, 1000, 130, 1, 2, 16, True), (2, 150, 33, 3, 1, 5, True), (1, 500, 64, 1, 1, 16, False), (1, 40, 5, 7, 1, 12, False),
           (3, 97, 1, 1, 1, 1, True), (1, 31, 200, 1, 1, 16, True), (1, 32, 200, 1, 1, 16, True), (40, 64, 300, 1, 3, 16, True),
           (2, 3, 5, 20, 1, 256, False), (1, 7, 3, 33, 1, 36, False), (1, 5, 2, 64, 1, 128, True), (2, 1, 3, 50, 3, 64, True),
-          (1, 1, 3, 9, 1, 192, False), (1, 40, 3, 12, 1, 24, False), (2, 2, 3, 17, 1, 131, False)]
+          (1, 1, 3, 9, 1, 192, False), (1, 40, 3, 12, 1, 24, False), (2, 2, 3, 17, 1, 131, False), (2, 11, 3, 64, 1, 128, False), (2, 12, 3, 64, 1, 128, False),
+          (1, 13, 4, 40, 2, 72, False)]
 
 
 @pytest.mark.parametrize("S,T,H,P,Gr,n,elem", PIECES)
