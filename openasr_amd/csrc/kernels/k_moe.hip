@@ -719,8 +719,9 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
         };
         // Two steps in flight: a step's products take a fraction of a load's way.
         // (The loads past the last step are the last step's again: one that may
-        // not have been made would be waited for with all later ones. Q4_K at 128
-        // columns has the registers for one: a second one spilled 34 of them.)
+        // not have been made would be waited for with all later ones. Quantized
+        // weights at 128 columns have the registers for one: a second one spilled 34
+        // of them for Q4_K, 46 for Q8_0.)
         constexpr int kAhead = kQ && BN == 128 ? 1 : 2;
         stage s0, s1;
         load(0, s0);

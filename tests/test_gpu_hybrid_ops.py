@@ -148,7 +148,8 @@ def test_conv_of_adjacent_channels(ggml, gpu, C, taps, T, S, silu):
     G.free()
 
 
-@pytest.mark.parametrize("case", ["carried first", "columns read too", "bias is an output", "two carried", "x over its cache"])
+@pytest.mark.parametrize("case", ["carried first", "columns read too", "bias is an output", "two carried", "x over its cache",
+                                  "x is an intermediate", "y is an intermediate"])
 def test_mixer_convolution_variants(ggml, gpu, case):
     """orders and readers with which the sequence may not, or may only partly,
     run as one launch: the results are the same"""
@@ -163,7 +164,9 @@ def test_mixer_convolution_variants(ggml, gpu, case):
     W, B = G.new(ggml.F32, taps, C), G.new(ggml.F32, C)
     X = G.new(ggml.F32, C, T, S, weight=True)
     ST = G.new(ggml.F32, taps - 1, C, S, weight=True)
-    cols = L.ggml_concat(ctx, ST, L.ggml_transpose(ctx, X), 0)
+    # (an intermediate's memory is free once it is joined: the result may lie over it)
+    from_x = L.ggml_scale(ctx, X, 1.0) if case == "x is an intermediate" else X
+    cols = L.ggml_concat(ctx, ST, L.ggml_transpose(ctx, from_x), 0)
     conv = L.ggml_ssm_conv(ctx, cols, W)
     pre = L.ggml_add(ctx, conv, B)
     y = L.ggml_silu(ctx, pre)
@@ -172,6 +175,7 @@ def test_mixer_convolution_variants(ggml, gpu, case):
     outs = {"carried first": [carried, y], "columns read too": [y, carried, L.ggml_scale(ctx, cols, 2.0)],
             "bias is an output": [pre, y, carried],
             "two carried": [y, carried, L.ggml_cont(ctx, L.ggml_view_3d(ctx, cols, taps - 1, C, S, row, row * C, 0))],
+            "x is an intermediate": [y, carried], "y is an intermediate": [carried, L.ggml_scale(ctx, y, 1.0)],
             # y's copy over x, which the sequence's launch would still be reading
             "x over its cache": [carried, L.ggml_cpy(ctx, y, X)]}[case]
     G.build(*outs)
@@ -186,7 +190,7 @@ def test_mixer_convolution_variants(ggml, gpu, case):
         if case == "bias is an output":
             within(G.get(pre).reshape(S, T, C), want, (taps + 1) * U * m, "pre")
         want = want / (1 + np.exp(-want))
-        got = G.get(X if case == "x over its cache" else y).reshape(S, T, C)
+        got = G.get(X if case == "x over its cache" else outs[1] if case == "y is an intermediate" else y).reshape(S, T, C)
         within(got, want, 1.1 * (taps + 1) * U * m + 4 * U * np.abs(want) + 1e-37, "y")
         if case == "columns read too":
             assert np.array_equal(G.get(outs[2]).reshape(joined.shape), 2 * joined)
@@ -812,6 +816,42 @@ def test_router_variants(ggml, gpu, case):
     G.free()
 
 
+@pytest.mark.parametrize("gating", ["chosen", "normed"])
+def test_router_of_intermediates(ggml, gpu, gating):
+    """logits whose memory is free after their last reader, weights and places used by products"""
+    E, k, T, K, M = 16, 3, 37, 64, 48
+    rng = np.random.default_rng(9)
+    a = rng.standard_normal((T, E)).astype(np.float32)
+    raw = (0.1 * rng.standard_normal((E, M, K))).astype(np.float16)
+    x = rng.standard_normal((T, 1, K)).astype(np.float32)
+    G = ggml.Graph(64, 64)
+    L, ctx = G.lib, G.ctx
+    A, X, W = G.new(ggml.F32, E, T), G.new(ggml.F32, K, 1, T), G.new(ggml.F16, K, M, E, weight=True)
+    ids, w = router(ggml, G, L.ggml_scale(ctx, A, 1.0), E, k, T, gating)
+    y = L.ggml_mul_mat_id(ctx, W, L.ggml_scale(ctx, X, 1.0), ids)
+    y = L.ggml_mul(ctx, y, L.ggml_reshape_3d(ctx, w, 1, k, T))
+    total = None
+    for j in range(k):
+        v = L.ggml_view_2d(ctx, y, M, T, 4 * M * k, 4 * M * j)
+        total = v if total is None else L.ggml_add(ctx, total, v)
+    out = L.ggml_scale(ctx, total, 1.0)
+    G.build(out)
+    G.allocate(gpu.buft)
+    for t, v in ((A, a), (X, x), (W, raw.view(np.uint16))):
+        G.set(t, v)
+    want = sorted64(a, 1)[:, :k]
+    p = np.exp(np.take_along_axis(a, want, 1).astype(np.float64))
+    p /= p.sum(1, keepdims=True)
+    prod, m = experts64(raw.astype(np.float64), x.astype(np.float16).astype(np.float64), want)
+    # the weights (a softmax: 8 + k roundings, over all E for the shares), the product, the sum of k
+    bound = (roundings(K) + 8 + E + 2 * k + 2) * U
+    for _ in range(4):
+        assert G.compute(gpu.backend) == 0
+        got = G.get(out).reshape(T, M)
+        within(got, (prod * p[..., None]).sum(1), bound * (m * p[..., None]).sum(1) + 1e-37)
+    G.free()
+
+
 @pytest.mark.parametrize("n,rows", [(255, 7), (256, 3), (257, 3), (511, 2), (513, 2), (4096, 2), (4097, 1)])
 @pytest.mark.parametrize("desc", [0, 1])
 def test_argsort_lengths(ggml, gpu, n, rows, desc):
@@ -853,6 +893,39 @@ def test_graphs_that_share_a_workspace(ggml, gpu, ref):
         within(G2.get(y2).reshape(N, k, M), want, roundings(K) * U * m + 1e-37, "experts")
     G1.free()
     G2.free()
+
+
+def test_compute_without_allocations(ggml, gpu, ref):
+    """the same results from the static scratch as from the backend's own"""
+    import ctypes
+
+    lib = gpu.cdll
+    lib.ggml_backend_mi355x_graph_compute_static.restype = ctypes.c_int
+    lib.ggml_backend_mi355x_graph_compute_static.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    rng = np.random.default_rng(13)
+    H, T, n, E, k, M, K = 70, 300, 16, 8, 4, 96, 256
+    a = scan_inputs(rng, 1, T, H, 1, 1, n, True, 1)
+    raw, _ = expert_weights(ggml, ref, rng, ggml.Q8_0, E, M, K)
+    x, lg = rng.standard_normal((T, 1, K)).astype(np.float32), rng.standard_normal((T, E)).astype(np.float32)
+    G = ggml.Graph(64, 64)
+    arrays = [(a[0], (n, 1, H, 1)), (a[1], (1, H, T, 1)), (a[2], (H, T, 1)), (a[3], (n, H)), (a[4], (n, 1, T, 1)),
+              (a[5], (n, 1, T, 1)), (np.zeros(1, np.int32), (1,)), (lg, (E, T)), (x, (K, 1, T))]
+    t = [G.new(ggml.I32 if v.dtype == np.int32 else ggml.F32, *ne) for v, ne in arrays]
+    W = G.new(ggml.Q8_0, K, M, E, weight=True)
+    ids, w = router(ggml, G, t[7], E, k, T, "normed")
+    outs = [G.lib.ggml_ssm_scan(G.ctx, *t[:7]), w, G.lib.ggml_mul_mat_id(G.ctx, W, t[8], ids)]
+    G.build(*outs)
+    G.allocate(gpu.buft)
+    for q, (v, _) in zip(t, arrays):
+        G.set(q, v)
+    G.set(W, raw)
+    assert lib.ggml_backend_mi355x_graph_compute_static(gpu.backend, G.gf) == 0
+    got = [G.get(o).copy() for o in outs]
+    for _ in range(3):
+        assert G.compute(gpu.backend) == 0
+        for o, g in zip(outs, got):
+            assert np.isfinite(g).all() and np.array_equal(G.get(o), g)
+    G.free()
 
 
 # ------------------------------------------------------ memory of others ---
