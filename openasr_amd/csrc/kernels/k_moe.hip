@@ -314,8 +314,26 @@ struct moe_wide_args {
     float * xd;     // quantized: the blocks' scales, [b column][Kp / 32 or Kp / 256]
     float * xs;     // Q4_K: scale times sum of 32 elements, [b column][Kp / 32]
     int64_t kp, bcols, row_tiles;
+    uint32_t used_inv;  // floor(2^32 / used), 2^32 - 1 for one
     int bn, max_tiles;
 };
+
+// pair p's token and slot, without a division (p < 2^26: the product's high
+// half is the quotient or one less)
+__device__ __forceinline__ void moe_pair(const moe_wide_args & q, int p, int & token, int & slot) {
+    const int used = (int) q.a.used;
+    token = (int) __umulhi((uint32_t) p, q.used_inv);
+    slot = p - token * used;
+    if (slot >= used) token++, slot -= used;
+}
+// and its column of b
+__device__ __forceinline__ int moe_column(const moe_wide_args & q, int p) {
+    int token, slot;
+    moe_pair(q, p, token, slot);
+    const int per = (int) q.a.b_ne1;
+    if (per == 1) return token;
+    return token * per + (per == (int) q.a.used ? slot : slot % per);
+}
 
 __device__ __forceinline__ void moe_route(const moe_wide_args & q) {
     extern __shared__ int s_hist[];  // [16][bins], bins = experts + 1 (no expert)
@@ -327,7 +345,9 @@ __device__ __forceinline__ void moe_route(const moe_wide_args & q) {
     // wave w's share: consecutive groups of 64 pairs
     const int groups = (pairs + 63) / 64, per = (groups + 15) / 16;
     auto expert_of = [&](int p) {
-        const int e = *(const int32_t *) (a.ids + (p % (int) a.used) * a.ids_nb0 + (int64_t) (p / (int) a.used) * a.ids_nb1);
+        int token, slot;
+        moe_pair(q, p, token, slot);
+        const int e = *(const int32_t *) (a.ids + slot * a.ids_nb0 + token * a.ids_nb1);
         return e < 0 || e >= a.experts ? (int) a.experts : e;
     };
     // a batch of groups' ids in flight at once (one by one, each waits for its load)
@@ -336,8 +356,8 @@ __device__ __forceinline__ void moe_route(const moe_wide_args & q) {
     auto load = [&](int k0) {
 #pragma unroll
         for (int k = 0; k < kBatch; k++) {
-            const int p = (wave * per + k0 + k) * 64 + lane;
-            e[k] = k0 + k < per && p < pairs ? expert_of(p) : -1;
+            const int p = (wave * per + k0 + k) * 64 + lane, v = expert_of(min(p, pairs - 1));
+            e[k] = k0 + k < per && p < pairs ? v : -1;
         }
     };
     for (int k0 = 0; k0 < per; k0 += kBatch) {
@@ -375,10 +395,13 @@ __device__ __forceinline__ void moe_route(const moe_wide_args & q) {
             int at = before + sum - total;
             const int t0 = tbefore + tsum - nt;
             for (int t = 0; t < nt; t++) q.tiles[t0 + t] = make_int4(b < a.experts ? b : -1, at, total, t0);
-            for (int w = 0; w < 16; w++) {  // the waves' first places
-                const int c = s_hist[w * bins + b];
+            int count[16];  // the waves' first places
+#pragma unroll
+            for (int w = 0; w < 16; w++) count[w] = s_hist[w * bins + b];
+#pragma unroll
+            for (int w = 0; w < 16; w++) {
                 s_hist[w * bins + b] = at;
-                at += c;
+                at += count[w];
             }
         }
         __syncthreads();
@@ -415,10 +438,13 @@ __global__ __launch_bounds__(1024) void k_moe_prepare(moe_wide_args q) {
     }
     const mul_mat_id_args & a = q.a;
     const int lane = threadIdx.x & 63;
-    const int64_t chunks = (q.kp + 255) / 256, w = (int64_t) (blockIdx.x - 1) * 16 + (threadIdx.x >> 6);
-    const int64_t col = w / chunks, k = w % chunks * 256 + 4 * lane;
+    // (the wave's place in scalars of 32 bits: bcols * kp < 2^31)
+    const uint32_t chunks = (uint32_t) ((q.kp + 255) / 256);
+    const uint32_t w = (blockIdx.x - 1) * 16 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t wcol = w / chunks, per = (uint32_t) a.b_ne1, btoken = wcol / per;
+    const int64_t col = wcol, k = (int64_t) (w - wcol * chunks) * 256 + 4 * lane;
     if (col >= q.bcols) return;
-    const float * x = (const float *) (a.b + (col % a.b_ne1) * a.b_nb1 + (col / a.b_ne1) * a.b_nb2);
+    const float * x = (const float *) (a.b + (int64_t) (wcol - btoken * per) * a.b_nb1 + btoken * a.b_nb2);
     float4 v = make_float4(0, 0, 0, 0);
     if (k < a.K) v = *(const float4 *) (x + k);  // K % 4 == 0
     typedef _Float16 v4h __attribute__((ext_vector_type(4)));
@@ -539,7 +565,7 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
     if (tid < BN) {
         const int p = q.sorted[at + min(tid, n - 1)];
         L.pair[tid] = p;
-        L.col[tid] = (int) (p / a.used * a.b_ne1 + p % a.used % a.b_ne1);
+        L.col[tid] = moe_column(q, p);
     }
     __syncthreads();
     if (of.x < 0) {  // no expert: zeros
@@ -914,6 +940,7 @@ static size_t moe_carve(int wtype, const mul_mat_id_args & a, moe_wide_args & q,
     q.bn = a.pairs >= 40 * a.experts ? 128 : 32;
     q.kp = (a.K + 63) / 64 * 64;
     q.bcols = a.b_ne1 * (a.pairs / a.used);
+    q.used_inv = a.used == 1 ? 0xFFFFFFFFu : (uint32_t) ((1ull << 32) / (uint64_t) a.used);
     q.row_tiles = (a.M + (a.W2 ? 64 : 128) - 1) / (a.W2 ? 64 : 128);
     const int64_t runs = a.experts + 1 < a.pairs ? a.experts + 1 : a.pairs;
     q.max_tiles = (int) (a.pairs / q.bn + runs);
