@@ -86,6 +86,22 @@ __device__ __forceinline__ moe_v8h moe_round8(const float * p) {
                    (_Float16) b.x, (_Float16) b.y, (_Float16) b.z, (_Float16) b.w};
 }
 
+// pair p's token and slot, without a division (p < 2^26: the product's high
+// half is the quotient or one less)
+__device__ __forceinline__ void moe_pair(const mul_mat_id_args & a, int p, int & token, int & slot) {
+    const int used = (int) a.used;
+    token = (int) __umulhi((uint32_t) p, a.used_inv);
+    slot = p - token * used;
+    if (slot >= used) token++, slot -= used;
+}
+// its token, and which of the token's columns of b it takes
+__device__ __forceinline__ void moe_column(const mul_mat_id_args & a, int p, int & token, int & of) {
+    moe_pair(a, p, token, of);
+    const int per = (int) a.b_ne1;
+    if (per == 1) of = 0;
+    else if (per != (int) a.used) of %= per;
+}
+
 // The 16 x 16 sums of NM matrices' rows and 16 columns over wave w's share of
 // K. The operand's row r holds column r / 4 + 4 (r % 4), so that lane group g
 // ends with the columns g + 4 i, and few columns need the first i only (NCL of
@@ -98,9 +114,9 @@ struct moe_tile;
 template <int NM>
 struct moe_tile<GGML_TYPE_F16, NM> {
     template <int NCL>
-    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * const (&wrow)[NM], int64_t bcol,
+    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * const (&wrow)[NM], const char * xcol, int64_t bcol,
                                                const int (&)[4], int wave, int waves, int g, double (&out)[NM][4]) {
-        const float * x = (const float *) (a.b + (bcol % a.b_ne1) * a.b_nb1 + (bcol / a.b_ne1) * a.b_nb2);
+        const float * x = (const float *) xcol;
         const int64_t steps = (a.K + 31) / 32;
         moe_v4f acc[NM];
 #pragma unroll
@@ -138,7 +154,7 @@ struct moe_tile<GGML_TYPE_F16, NM> {
 template <int NM>
 struct moe_tile<GGML_TYPE_Q8_0, NM> {
     template <int NCL>
-    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * const (&wrow)[NM], int64_t bcol,
+    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * const (&wrow)[NM], const char * xcol, int64_t bcol,
                                                const int (&bc4)[4], int wave, int waves, int g, double (&out)[NM][4]) {
         const int64_t nblk = a.K / 32;
         const int8_t * aq = a.act.q + bcol * a.K;
@@ -171,7 +187,7 @@ struct moe_tile<GGML_TYPE_Q8_0, NM> {
 template <int NM>
 struct moe_tile<GGML_TYPE_Q4_K, NM> {
     template <int NCL>
-    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * const (&wrow)[NM], int64_t bcol,
+    static __device__ __forceinline__ void run(const mul_mat_id_args & a, const char * const (&wrow)[NM], const char * xcol, int64_t bcol,
                                                const int (&bc4)[4], int wave, int waves, int g, double (&out)[NM][4]) {
         const int64_t nsb = a.K / 256;
         const int8_t * aq = a.act.q + bcol * a.K;
@@ -219,7 +235,11 @@ __global__ __launch_bounds__(256) void k_moe_few(mul_mat_id_args a) {
     const int me = blockIdx.y;
     const int64_t m0 = (int64_t) blockIdx.x * 16;
     int id = -1;
-    if (tid < a.pairs) id = *(const int32_t *) (a.ids + (tid % a.used) * a.ids_nb0 + (tid / a.used) * a.ids_nb1);
+    if (tid < a.pairs) {
+        int token, slot;
+        moe_pair(a, tid, token, slot);
+        id = *(const int32_t *) (a.ids + slot * a.ids_nb0 + token * a.ids_nb1);
+    }
     s_id[tid] = id;
     __syncthreads();
     const int e = s_id[me];
@@ -243,17 +263,21 @@ __global__ __launch_bounds__(256) void k_moe_few(mul_mat_id_args a) {
     const char * wrow[NM];
     wrow[0] = a.W + e * a.W_nb2 + row * a.W_nb1;
     if constexpr (PAIR) wrow[1] = a.W2 + e * a.W_nb2 + row * a.W_nb1;
-    auto column = [&](int p) { return (int) (p / a.used * a.b_ne1 + p % a.used % a.b_ne1); };
     for (int c0 = 0; c0 < n; c0 += 16) {
-        const int64_t bcol = column(s_list[min(c0 + (r >> 2) + 4 * (r & 3), n - 1)]);
-        int bc4[4];
+        int token, of, bc4[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) bc4[i] = column(s_list[min(c0 + g + 4 * i, n - 1)]);
+        for (int i = 0; i < 4; i++) {
+            moe_column(a, s_list[min(c0 + g + 4 * i, n - 1)], token, of);
+            bc4[i] = token * (int) a.b_ne1 + of;
+        }
+        moe_column(a, s_list[min(c0 + (r >> 2) + 4 * (r & 3), n - 1)], token, of);
+        const int64_t bcol = token * a.b_ne1 + of;
+        const char * xcol = a.b + token * a.b_nb2 + of * a.b_nb1;
         double acc[NM][4] = {};
         using tile = moe_tile<WT, NM>;
-        if (n - c0 <= 4) tile::template run<1>(a, wrow, bcol, bc4, wave, 4, g, acc);
-        else if (n - c0 <= 8) tile::template run<2>(a, wrow, bcol, bc4, wave, 4, g, acc);
-        else tile::template run<4>(a, wrow, bcol, bc4, wave, 4, g, acc);
+        if (n - c0 <= 4) tile::template run<1>(a, wrow, xcol, bcol, bc4, wave, 4, g, acc);
+        else if (n - c0 <= 8) tile::template run<2>(a, wrow, xcol, bcol, bc4, wave, 4, g, acc);
+        else tile::template run<4>(a, wrow, xcol, bcol, bc4, wave, 4, g, acc);
         if (wave > 0) {
 #pragma unroll
             for (int m = 0; m < NM; m++)
@@ -314,26 +338,8 @@ struct moe_wide_args {
     float * xd;     // quantized: the blocks' scales, [b column][Kp / 32 or Kp / 256]
     float * xs;     // Q4_K: scale times sum of 32 elements, [b column][Kp / 32]
     int64_t kp, bcols, row_tiles;
-    uint32_t used_inv;  // floor(2^32 / used), 2^32 - 1 for one
     int bn, max_tiles;
 };
-
-// pair p's token and slot, without a division (p < 2^26: the product's high
-// half is the quotient or one less)
-__device__ __forceinline__ void moe_pair(const moe_wide_args & q, int p, int & token, int & slot) {
-    const int used = (int) q.a.used;
-    token = (int) __umulhi((uint32_t) p, q.used_inv);
-    slot = p - token * used;
-    if (slot >= used) token++, slot -= used;
-}
-// and its column of b
-__device__ __forceinline__ int moe_column(const moe_wide_args & q, int p) {
-    int token, slot;
-    moe_pair(q, p, token, slot);
-    const int per = (int) q.a.b_ne1;
-    if (per == 1) return token;
-    return token * per + (per == (int) q.a.used ? slot : slot % per);
-}
 
 __device__ __forceinline__ void moe_route(const moe_wide_args & q) {
     extern __shared__ int s_hist[];  // [16][bins], bins = experts + 1 (no expert)
@@ -346,7 +352,7 @@ __device__ __forceinline__ void moe_route(const moe_wide_args & q) {
     const int groups = (pairs + 63) / 64, per = (groups + 15) / 16;
     auto expert_of = [&](int p) {
         int token, slot;
-        moe_pair(q, p, token, slot);
+        moe_pair(a, p, token, slot);
         const int e = *(const int32_t *) (a.ids + slot * a.ids_nb0 + token * a.ids_nb1);
         return e < 0 || e >= a.experts ? (int) a.experts : e;
     };
@@ -565,7 +571,9 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(moe_wide_args q) {
     if (tid < BN) {
         const int p = q.sorted[at + min(tid, n - 1)];
         L.pair[tid] = p;
-        L.col[tid] = moe_column(q, p);
+        int token, of;
+        moe_column(a, p, token, of);
+        L.col[tid] = token * (int) a.b_ne1 + of;
     }
     __syncthreads();
     if (of.x < 0) {  // no expert: zeros
@@ -940,7 +948,6 @@ static size_t moe_carve(int wtype, const mul_mat_id_args & a, moe_wide_args & q,
     q.bn = a.pairs >= 40 * a.experts ? 128 : 32;
     q.kp = (a.K + 63) / 64 * 64;
     q.bcols = a.b_ne1 * (a.pairs / a.used);
-    q.used_inv = a.used == 1 ? 0xFFFFFFFFu : (uint32_t) ((1ull << 32) / (uint64_t) a.used);
     q.row_tiles = (a.M + (a.W2 ? 64 : 128) - 1) / (a.W2 ? 64 : 128);
     const int64_t runs = a.experts + 1 < a.pairs ? a.experts + 1 : a.pairs;
     q.max_tiles = (int) (a.pairs / q.bn + runs);
@@ -980,8 +987,10 @@ static void launch_moe_wide(const mul_mat_id_args & a, char * scratch, hipStream
     else a.W2 ? go(k_moe_gemm<WT, true, 32>) : go(k_moe_gemm<WT, false, 32>);
 }
 
-void launch_mul_mat_id(int wtype, const mul_mat_id_args & a, void * scratch, hipStream_t s) {
+void launch_mul_mat_id(int wtype, const mul_mat_id_args & args, void * scratch, hipStream_t s) {
+    mul_mat_id_args a = args;
     if (a.M == 0 || a.pairs == 0) return;
+    a.used_inv = a.used == 1 ? 0xFFFFFFFFu : (uint32_t) ((1ull << 32) / (uint64_t) a.used);
     if (mul_mat_id_wide(wtype, a)) {
         if (wtype == GGML_TYPE_Q8_0) launch_moe_wide<GGML_TYPE_Q8_0>(a, (char *) scratch, s);
         else if (wtype == GGML_TYPE_Q4_K) launch_moe_wide<GGML_TYPE_Q4_K>(a, (char *) scratch, s);

@@ -434,6 +434,7 @@ struct mul_mat_id_args {
     int64_t b_ne1, b_nb1, b_nb2;
     const char * ids;
     int64_t ids_nb0, ids_nb1, used, pairs;
+    uint32_t used_inv;  // floor(2^32 / used), 2^32 - 1 for one (launch_mul_mat_id sets it)
     act_buffers act;  // quantized weights, where the launch is not wide
     float * out;
     // the SwiGLU pair (mul_mat_id_pairs): out = silu(W x) * (W2 x), W2 laid
