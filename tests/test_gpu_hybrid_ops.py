@@ -552,6 +552,30 @@ def test_mul_mat_id_borders(ggml, gpu, ref, wname, E, k, M, K, T, how):
     test_mul_mat_id(ggml, gpu, ref, wname, E, k, M, K, T, how, how == "outside")
 
 
+@pytest.mark.parametrize("wname", ["f16", "q8_0", "q4_K", "f32"])
+@pytest.mark.parametrize("k,b,T", [(6, 2, 5), (6, 3, 90), (7, 1, 60), (12, 4, 21), (12, 4, 40)])
+def test_mul_mat_id_slots_share_columns(ggml, gpu, ref, wname, k, b, T):
+    """b columns a token, slot s takes column s % b"""
+    print(f"mul_mat_id shared columns {wname} k={k} b={b} T={T}", flush=True)
+    E, M, K = 14, 80, 256
+    wt = WT[wname]
+    rng = np.random.default_rng(k + T)
+    raw, w = expert_weights(ggml, ref, rng, wt, E, M, K)
+    x = rng.standard_normal((T, b, K)).astype(np.float32)
+    ids = routes(rng, T, E, k, "outside")
+    G = ggml.Graph(64, 64)
+    W, X, I = G.new(wt, K, M, E, weight=True), G.new(ggml.F32, K, b, T), G.new(ggml.I32, k, T)
+    y = G.lib.ggml_mul_mat_id(G.ctx, W, X, I)
+    G.build(y)
+    G.allocate(gpu.buft)
+    for t, v in ((W, raw), (X, x), (I, ids)):
+        G.set(t, v)
+    compute(gpu, G)
+    want, mag = experts64(w, columns(ggml, ref, wt, x), ids)
+    within(G.get(y).reshape(T, k, M), want, roundings(K) * U * mag, wname)
+    G.free()
+
+
 @pytest.mark.parametrize("E,k,M,K,T", [(4, 2, 48, 768, 65), (3, 2, 200, 256, 300), (2, 1, 140, 1280, 290)])
 def test_mul_mat_id_borders_of_super_blocks(ggml, gpu, ref, E, k, M, K, T):
     test_mul_mat_id(ggml, gpu, ref, "q4_K", E, k, M, K, T, "twice", True)
