@@ -2,6 +2,7 @@
 // depthwise causal convolution over the carried and the step's columns) and
 // GGML_OP_SSM_SCAN (the selective scan).
 #include <algorithm>
+#include <cstddef>
 #include <type_traits>
 
 #include "../mi355x_common.h"
@@ -527,135 +528,162 @@ __global__ __launch_bounds__(256) void k_ssm_scan_lanes(ssm_lane_args q) {
 // which takes 4 P N + O(64 P) multiply-adds a token on the matrix cores, where
 // the token by token form takes 3 P N vector operations and a sum over lanes.
 //
-// Products of f32 operands on the f16 matrix cores: every row (or column) that
-// a sum runs along is scaled by a power of two so that its largest element is
-// in [2^13, 2^14), and split into f16 hi + lo (22 bits down to 2^-17 of that
-// element, 2^-39 of it below); a product is hi hi + hi lo + lo hi, summed in
-// f32: a sum is off by some 2^-22 of its terms' magnitudes and 2^-38 of its
-// operands' largest elements' product. Against f32 MFMAs (an
-// eighth of the f16 rate after the three products) the sums are as good as
-// f32's own roundings; states, decays and sums are f32, the log decays f64
-// until they are split into whole and fractional powers of two.
+// Products of f32 operands on the bf16 matrix cores: an operand is the sum of
+// three bf16 (8 bits each: all 24 of an f32, in its range of exponents), and a
+// product the six of theirs that f32 can hold (what is left out is 2^-26 of it
+// and less), summed in f32. So an element keeps its bits however far it lies
+// under its neighbours, over tokens and over n alike, and the error is that of
+// f32 sums. The f32 matrix instructions need no parts, but take the vector
+// unit's time at 1/16 of the rate (a vector instruction beside one takes its
+// own again): 2 x 2048 tokens of 80 heads of 64 x 128 took 151 us, and 68 for
+// the first pass, where these take 110 and 50 (and 11 for the shared operands;
+// 333 tokens of 24 x 64 x 64: 13 + 8 + 5 us). Bound by reads of LDS (114 KB a
+// wave and chunk, 8 waves), the issue of loads after each barrier, and the
+// vector instructions around the products (some 800 a wave and chunk).
 //
-// 2 x 2048 tokens of 80 heads of 64 x 128: 110 us and 41 for the first pass,
-// bound by the vector instructions around the products (965 a wave and chunk:
-// scales, halves, decays; the products, three for each, are 40 GFLOP: 37 us at
-// a large product's rate), and 11 for the shared operands. 333 tokens of 24 x 64 x 64: 14 + 6 + 7 us.
+// The log decays are f64 until they are split into whole and fractional powers
+// of two; where they are deep, an operand takes its whole power by ldexp, so
+// that it underflows only where the product does.
 //
-// k_ssm_split makes the operands that a group's heads share: C in rows and B
-// in columns, split, with their scales, and C_t . B_j. k_ssm_chunks gives a
-// workgroup a (sequence, head, 64 channels, segment of chunks): wave w owns
-// the state's rows n in its quarter (in accumulators) and, for y, 16 tokens.
-// k_ssm_split also sums the heads' log decays. Where there are few heads the sequence is cut into segments: the
-// first pass (OUT false) makes each segment's own state from zeros, and the
-// second starts from the earlier segments' states, decayed and added.
+// k_ssm_split makes the operands that a group's heads share (the parts of C and
+// B, and C_t . B_j) and the heads' decays, in the matrix instructions' order:
+// 64 lanes' 16 bytes one after another. A workgroup of k_ssm_chunks takes two
+// blocks of (head, 64 channels) of a group, four waves each, and a segment of
+// chunks; only the shared operands and the decayed C . B go through LDS. Wave w
+// of a block keeps the state of its channels 16 w .. in its accumulators, which
+// are the products' operands as they lie: lane (g, r) holds n = 4 g .. 4 g + 3
+// of channel r, and K runs in that order for both sides (32 of K: the 4 g .. of
+// two blocks of 16). Where there are few heads the sequence is cut into
+// segments: the first pass (OUT false) makes each segment's own state from
+// zeros, and the second starts from the earlier segments' states, decayed and
+// added.
 //
-// Non-finite values would spread inside a chunk (0 * inf), and tokens far
-// larger than the ones before them would cost those their bits: such a chunk,
-// and one whose decays leave the exact range, runs token by token
-// (ssm_chunk_slow), where a value reaches what the recurrence takes it to.
+// Non-finite values would spread inside a chunk (0 * inf), and the products'
+// order could take large ones out of f32's range where the recurrence does not:
+// such a wave's chunk, and one whose decays leave the exact range, runs token
+// by token (ssm_tokens), where a value reaches what the recurrence takes it to.
 
+typedef uint32_t ssm_u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t ssm_u4 __attribute__((ext_vector_type(4)));
+typedef int ssm_i4 __attribute__((ext_vector_type(4)));
 typedef float ssm_v2f __attribute__((ext_vector_type(2)));
-typedef _Float16 ssm_v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 ssm_v4h __attribute__((ext_vector_type(4)));
-typedef _Float16 ssm_v2h __attribute__((ext_vector_type(2)));
+typedef __bf16 ssm_v2b __attribute__((ext_vector_type(2)));
+typedef __bf16 ssm_v8b __attribute__((ext_vector_type(8)));
+
+// (what the launch before wrote and all lanes read alike: scalar loads)
+#define SSM_UNIFORM const __attribute__((address_space(4)))
 
 constexpr int kSsmL = 64;
-constexpr float kLog2e = 1.44269504088896340736f;
 
-__device__ __forceinline__ ssm_v4f ssm_mfma(ssm_v8h a, ssm_v8h b, ssm_v4f c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+// two f32 as the sums of three bf16 each, rounded to nearest
+__device__ __forceinline__ void ssm_parts2(float a, float b, uint32_t & h, uint32_t & m, uint32_t & l) {
+    auto pack = [](float x, float y) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(ssm_v2f{x, y}, ssm_v2b)); };
+    auto less = [](float & x, float & y, uint32_t p) {
+        x -= __uint_as_float(p << 16);
+        y -= __uint_as_float(p & 0xFFFF0000u);
+    };
+    h = pack(a, b);
+    less(a, b, h);
+    m = pack(a, b);
+    less(a, b, m);
+    l = pack(a, b);
 }
-// a b of split halves for four b's: the three products of one accumulator
-// apart, since each waits for the one before
-__device__ __forceinline__ void ssm_products(ssm_v8h ah, ssm_v8h al, const ssm_v8h (&bh)[4], const ssm_v8h (&bl)[4],
-                                             ssm_v4f (&c)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) c[i] = ssm_mfma(ah, bh[i], c[i]);
-#pragma unroll
-    for (int i = 0; i < 4; i++) c[i] = ssm_mfma(ah, bl[i], c[i]);
-#pragma unroll
-    for (int i = 0; i < 4; i++) c[i] = ssm_mfma(al, bh[i], c[i]);
+struct ssm_parts {  // a lane's eight elements of K
+    ssm_u4 v[3];
+};
+__device__ __forceinline__ void ssm_parts8(ssm_v4f a, ssm_v4f b, ssm_parts & p) {
+    uint32_t h[4], m[4], l[4];
+    ssm_parts2(a[0], a[1], h[0], m[0], l[0]);
+    ssm_parts2(a[2], a[3], h[1], m[1], l[1]);
+    ssm_parts2(b[0], b[1], h[2], m[2], l[2]);
+    ssm_parts2(b[2], b[3], h[3], m[3], l[3]);
+    p.v[0] = ssm_u4{h[0], h[1], h[2], h[3]};
+    p.v[1] = ssm_u4{m[0], m[1], m[2], m[3]};
+    p.v[2] = ssm_u4{l[0], l[1], l[2], l[3]};
 }
-// 2^e, e a whole number in f32's normal range
-__device__ __forceinline__ float ssm_pow2(int e) { return __uint_as_float((uint32_t) (e + 127) << 23); }
-// the exponent k that brings a largest magnitude (its bits) into [2^13, 2^14);
-// 0 for zero, at most 74 (a magnitude under 2^-60 keeps fewer bits)
-__device__ __forceinline__ int ssm_scale(uint32_t bits) {
-    const int e = (int) (bits >> 23) - 127;  // floor(log2), -127 for zero and subnormals
-    return bits == 0 ? 0 : min(13 - e, 74);
+__device__ __forceinline__ ssm_v4f ssm_mfma(ssm_u4 a, ssm_u4 b, ssm_v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ssm_v8b, a), __builtin_bit_cast(ssm_v8b, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ uint32_t ssm_mag(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-// an element at a uniform base, a lane's byte offset and a constant one: the
-// address form a load takes without 64-bit vector arithmetic
+// the i-th of a product's six, the small ones first
+__device__ __forceinline__ ssm_v4f ssm_product(int i, const ssm_parts & a, const ssm_parts & b, ssm_v4f c) {
+    constexpr int of_a[6] = {2, 0, 1, 1, 0, 0}, of_b[6] = {0, 2, 1, 0, 1, 0};
+    return ssm_mfma(a.v[of_a[i]], b.v[of_b[i]], c);
+}
+// an element at a uniform base and a lane's byte offset
 template <typename T>
-__device__ __forceinline__ T & ssm_at(const void * base, uint32_t off, int fixed = 0) {
-    return *(T *) ((char *) base + off + fixed);
+__device__ __forceinline__ T & ssm_at(const void * base, uint32_t off) {
+    return *(T *) ((char *) base + off);
 }
-template <int W>
-__device__ __forceinline__ uint32_t ssm_group_max(uint32_t v) {
-#pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) v = max(v, (uint32_t) __shfl_xor((int) v, o, W));
-    return v;
-}
-__device__ __forceinline__ bool ssm_finite(uint32_t mag) { return mag < 0x7F800000u; }
-
-// f16 hi + lo of N products x f (the lo part by a fused multiply-add)
-template <int N, typename V, typename F>
-__device__ __forceinline__ void ssm_halves(const float (&x)[N], F f, V & hi, V & lo) {
-#pragma unroll
-    for (int e = 0; e < N; e += 2) {
-        const ssm_v2f v = {x[e] * f(e), x[e + 1] * f(e + 1)};
-        const ssm_v2h h = __builtin_convertvector(v, ssm_v2h);
-        const ssm_v2f d = {fmaf(x[e], f(e), -(float) h.x), fmaf(x[e + 1], f(e + 1), -(float) h.y)};
-        const ssm_v2h l = __builtin_convertvector(d, ssm_v2h);
-        hi[e] = h.x, hi[e + 1] = h.y;
-        lo[e] = l.x, lo[e + 1] = l.y;
+// The matrix form's operands are at most 2^30 (u, B and C). A chunk then adds at
+// most 2^66 to a state, so one that begins under 2^80 is under 2^87 after 2^20
+// chunks, its product with a row of C under 2^125.
+constexpr uint32_t kSsmLargest = (127u + 30) << 23, kSsmLargestState = (127u + 80) << 23;
+constexpr int64_t kSsmMostTokens = (int64_t) kSsmL << 20;
+// whether one of the values is larger, infinite or NaN: the largest of their bits
+// as signed numbers (among the positive ones), and as unsigned (the negative)
+struct ssm_most {
+    int pos = 0;
+    uint32_t neg = 0;
+    __device__ __forceinline__ void add(float a, float b) {
+        pos = max(max(pos, __float_as_int(a)), __float_as_int(b));
+        neg = max(max(neg, __float_as_uint(a)), __float_as_uint(b));
     }
+    __device__ __forceinline__ bool past(uint32_t limit) const { return pos > (int) limit || neg > (limit | 0x80000000u); }
+};
+// a power of two of any size: v times the fraction's power, then the whole one
+__device__ __forceinline__ float ssm_decayed(float v, float frac_pow2, float whole) { return ldexpf(v * frac_pow2, (int) whole); }
+struct ssm_power {
+    float frac, whole;
+};
+__device__ __forceinline__ ssm_power ssm_split_power(double z) {
+    const double whole = floor(fmin(fmax(z, -100000.0), 100000.0));
+    return {__builtin_amdgcn_exp2f((float) fmin(fmax(z - whole, 0.0), 1.0)), (float) whole};
 }
 
 // what a chunk's decays need besides the tokens' own
 struct ssm_decay {
-    double total;       // its log2 decay
-    int e_dt, e_left;   // the exponents of the largest step, and of the largest step times the decay after it
-    int odd, pad;       // outside what the matrix form takes
+    double total;  // its log2 decay
+    int kind;      // kSsmOdd: outside what the matrix form takes; kSsmDeep: powers that f32 may not hold
+    int pad;
 };
-struct ssm_flags {
-    int bad[4];  // a quarter's rows hold a non-finite value
-    int kb;      // B's operand is its value times 2^kb
-    int pad[3];
-};
+constexpr int kSsmOdd = 1, kSsmDeep = 2;
 
 // The operands in scratch: a record a (sequence, group, chunk) and one a
-// (sequence, head, chunk), byte offsets of their parts, NP the padded state size
+// (sequence, head, chunk), byte offsets of their arrays, NP the padded state
+// size. A fragment is 64 lanes' 16 bytes, lane (g, r).
 template <int NP>
 struct ssm_shared_at {
-    static constexpr int c_hi = 0;              // [64 tokens][NP] f16, each token's row scaled
-    static constexpr int c_lo = 128 * NP;
-    static constexpr int b_hi = 256 * NP;       // [NP][64 tokens] f16, scaled
-    static constexpr int b_lo = 384 * NP;
-    static constexpr int cb = 512 * NP;         // [64][64] f32: C_t . B_j for j <= t (zeros past it), rows scaled
-    static constexpr int c_s = cb + 16384;      // [64] f32: a row of C is its operand times this
-    static constexpr int cb_s = c_s + 256;      // [64] f32: a row of C . B is its operand times this
-    static constexpr int flags = cb_s + 256;    // ssm_flags
-    static constexpr int size = flags + 256;
+    static constexpr int KB = NP / 32, NK = NP / 16;
+    static constexpr int c = 0;                     // [4 tb][KB][part] bf16: token 16 tb + r, n 4 g .. of two blocks of 16
+    static constexpr int b = 12 * KB * 1024;        // [2 jb][NK][part] bf16: n r of 16, tokens 4 g .. of two blocks of 16
+    static constexpr int cb = b + 6 * NK * 1024;    // blocks (tb, jb) f32: token t r of 16, tokens j 4 g .. (zeros past t)
+    static constexpr int bad = cb + 12 * 1024;      // [4] bytes: a quarter's rows hold a value past 2^30
+    static constexpr int size = bad + 256;
 };
+// The blocks of C . B in turn: two for the first tokens' 16 and the second's,
+// four for the others' (pairs of blocks make a fragment)
+__device__ __forceinline__ int ssm_block(int tb, int jb) { return (tb < 2 ? 2 * tb : 4 * tb - 4) + jb; }
 struct ssm_head_at {  // c_t: the sum of the log2 decays from the chunk's start to token t
-    static constexpr int dt = 0;        // [64] f32: the step over 2^e_dt
-    static constexpr int left = 256;    // [64] f32: the step times 2^(c_L - c_t), over 2^e_left
-    static constexpr int whole = 512;   // [64] f32: c_t's whole and fractional part
-    static constexpr int frac = 768;
-    static constexpr int decay = 1024;  // ssm_decay
-    static constexpr int size = 1280;
+    static constexpr int dt = 0;          // [64] f32: the step
+    static constexpr int left = 256;      // [64] f32: 2^(c_L - c_t), deep: of its fraction
+    static constexpr int left_whole = 512;  // [64] i32: deep: its whole part (else 0)
+    static constexpr int in = 768;        // [64] f32: 2^c_t, deep: of its fraction
+    static constexpr int whole = 1024;    // c_t's whole part
+    static constexpr int frac = 1280;     // c_t's fractional part
+    static constexpr int decay = 1536;    // ssm_decay
+    static constexpr int size = 1792;
+    static constexpr int tokens = 6;      // arrays of 64
 };
 struct ssm_chunk_args {
     ssm_scan_args a;
     char *shared, *heads;
-    float * seg_state;   // [seq, head, channel block][segment][64][NP]
+    float * seg_state;   // [seq, head, channel block][segment][wave][NP / 16 fragments]
     double * seg_decay;  // [seq, head][segment]: its log2 decay
     int64_t chunks;
     int segs, seg_chunks, pblocks;
+    int pairs;             // workgroups a group: of two (head, channel block)s
     uint32_t split_blocks;
+    int xvec, yvec, svec;  // x, y and the states in 16-byte pieces
 };
 
 // the decays of one (sequence, head, chunk): a lane a token, the sums in f64
@@ -675,20 +703,21 @@ __device__ __forceinline__ void ssm_decays(const ssm_chunk_args & q, int64_t uni
         const double v = __shfl_up(cum, o);
         if (lane >= o) cum += v;
     }
-    const double total = __shfl(cum, 63), whole = floor(cum);
-    const float left = dt * __builtin_amdgcn_exp2f((float) (total - cum));
-    // the largest step's exponents: the operands' scales are bounded by them
-    const uint32_t md = ssm_group_max<64>(ssm_mag(dt)), ml = ssm_group_max<64>(ssm_mag(left));
+    const double total = __shfl(cum, 63);
     ssm_decay d{};
     d.total = total;
-    d.e_dt = max((int) (md >> 23) - 127, -60);
-    d.e_left = max((int) (ml >> 23) - 127, -60);
-    // A positive, or decays whose whole parts leave f32's exact range
-    d.odd = !(total <= 0.0 && total > -8388608.0) || !ssm_finite(md);
-    ((float *) (rec + ssm_head_at::dt))[lane] = dt * ssm_pow2(-d.e_dt);
-    ((float *) (rec + ssm_head_at::left))[lane] = left * ssm_pow2(-d.e_left);
-    ((float *) (rec + ssm_head_at::whole))[lane] = (float) whole;
-    ((float *) (rec + ssm_head_at::frac))[lane] = (float) (cum - whole);
+    // A positive, decays whose whole parts leave f32's exact range, steps that are not finite
+    const bool odd = !(total <= 0.0 && total > -8388608.0) || __any((__float_as_uint(dt) & 0x7FFFFFFFu) >= 0x7F800000u);
+    const bool deep = total < -120.0;  // else every power is one factor
+    d.kind = (odd ? kSsmOdd : 0) | (deep ? kSsmDeep : 0);
+    const ssm_power left = ssm_split_power(total - cum), in = ssm_split_power(cum);
+    auto put = [&](int at, float v) { ((float *) (rec + at))[lane] = v; };
+    put(ssm_head_at::dt, dt);
+    put(ssm_head_at::left, deep ? left.frac : ssm_decayed(1.0f, left.frac, left.whole));
+    ((int *) (rec + ssm_head_at::left_whole))[lane] = deep ? (int) left.whole : 0;
+    put(ssm_head_at::in, deep ? in.frac : ssm_decayed(1.0f, in.frac, in.whole));
+    put(ssm_head_at::whole, (float) floor(cum));
+    put(ssm_head_at::frac, (float) (cum - floor(cum)));
     if (lane == 0) *(ssm_decay *) (rec + ssm_head_at::decay) = d;
 }
 
@@ -711,558 +740,573 @@ __global__ __launch_bounds__(256) void k_ssm_split(ssm_chunk_args q) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const char * B = a.B + g * a.B_nb1 + s * a.B_nb3;
     const char * C = a.C + g * a.C_nb1 + s * a.C_nb3;
-    uint32_t mb = 0;
+    const int brows = 16 * part + 16;  // the rows of B up to this quarter's last
+    ssm_most most;
     const bool vec = a.n % 4 == 0 && (((uintptr_t) B | (uintptr_t) C | (uintptr_t) a.B_nb2 | (uintptr_t) a.C_nb2) & 15) == 0;
+    auto mags = [&](float4 v) { most.add(v.x, v.y), most.add(v.z, v.w); };
     if (vec) {
         float4 vb[kSsmL * NP / 1024], vc[16 * NP / 1024];
 #pragma unroll
         for (int k = 0; k < kSsmL * NP / 1024; k++) {
             const int i = tid + 256 * k, t = i / (NP / 4), n = i % (NP / 4) * 4;
-            const bool ok = t0 + t < a.tokens && n < a.n;
-            vb[k] = *(const float4 *) (B + (ok ? t0 + t : 0) * a.B_nb2 + (ok ? 4 * n : 0));
-            if (!ok) vb[k] = make_float4(0, 0, 0, 0);
+            const bool ok = t0 + t < a.tokens && n < a.n && t < brows;
+            vb[k] = make_float4(0, 0, 0, 0);
+            if (ok) vb[k] = *(const float4 *) (B + (t0 + t) * a.B_nb2 + 4 * n);
         }
 #pragma unroll
         for (int k = 0; k < 16 * NP / 1024; k++) {
             const int i = tid + 256 * k, t = 16 * part + i / (NP / 4), n = i % (NP / 4) * 4;
             const bool ok = t0 + t < a.tokens && n < a.n;
-            vc[k] = *(const float4 *) (C + (ok ? t0 + t : 0) * a.C_nb2 + (ok ? 4 * n : 0));
-            if (!ok) vc[k] = make_float4(0, 0, 0, 0);
+            vc[k] = make_float4(0, 0, 0, 0);
+            if (ok) vc[k] = *(const float4 *) (C + (t0 + t) * a.C_nb2 + 4 * n);
         }
 #pragma unroll
         for (int k = 0; k < kSsmL * NP / 1024; k++) {
             const int i = tid + 256 * k;
             *(float4 *) &sb[i / (NP / 4)][i % (NP / 4) * 4] = vb[k];
-            mb = max(max(mb, max(ssm_mag(vb[k].x), ssm_mag(vb[k].y))), max(ssm_mag(vb[k].z), ssm_mag(vb[k].w)));
+            mags(vb[k]);
         }
 #pragma unroll
         for (int k = 0; k < 16 * NP / 1024; k++) {
             const int i = tid + 256 * k;
             *(float4 *) &sc[i / (NP / 4)][i % (NP / 4) * 4] = vc[k];
+            mags(vc[k]);
         }
     } else {
-        for (int i = tid; i < kSsmL * NP; i += 256) {
+        for (int i = tid; i < brows * NP; i += 256) {
             const int t = i / NP, n = i % NP;
             const bool ok = t0 + t < a.tokens && n < a.n;
             sb[t][n] = ok ? ((const float *) (B + (t0 + t) * a.B_nb2))[n] : 0.0f;
-            mb = max(mb, ssm_mag(sb[t][n]));
+            most.add(sb[t][n], 0.0f);
         }
         for (int i = tid; i < 16 * NP; i += 256) {
             const int t = 16 * part + i / NP, n = i % NP;
             const bool ok = t0 + t < a.tokens && n < a.n;
             sc[i / NP][n] = ok ? ((const float *) (C + (t0 + t) * a.C_nb2))[n] : 0.0f;
+            most.add(sc[i / NP][n], 0.0f);
         }
     }
-    __shared__ uint32_t s_mb[4];
-    mb = ssm_group_max<64>(mb);
-    if (lane == 0) s_mb[wave] = mb;
-    __syncthreads();
-    mb = max(max(s_mb[0], s_mb[1]), max(s_mb[2], s_mb[3]));
+    const int bad = __syncthreads_or(most.past(kSsmLargest));  // (and the rows are staged)
     using at = ssm_shared_at<NP>;
     char * rec = q.shared + (sg * q.chunks + chunk) * at::size;
-    // C's rows: 16 threads each
-    const int row = tid / 16, sub = tid % 16;
-    uint32_t mc = 0;
-    for (int n = sub; n < NP; n += 16) mc = max(mc, ssm_mag(sc[row][n]));
-    mc = ssm_group_max<16>(mc);
-    const int kb = ssm_finite(mb) ? ssm_scale(mb) : 0, kc = ssm_finite(mc) ? ssm_scale(mc) : 0;
-    const int any = __syncthreads_or(!ssm_finite(mb) || !ssm_finite(mc));
-    if (tid == 0) {
-        ssm_flags * fl = (ssm_flags *) (rec + at::flags);
-        fl->bad[part] = any;
-        if (part == 0) fl->kb = kb;
-    }
-    const int t = 16 * part + row;
-    if (sub == 0) ((float *) (rec + at::c_s))[t] = ssm_pow2(-kc);
-    const float fc = ssm_pow2(kc), fb = ssm_pow2(kb);
-    for (int n = 8 * sub; n < NP; n += 128) {
-        float v[8];
-        ssm_v8h hi, lo;
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = sc[row][n + e];
-        ssm_halves(v, [&](int) { return fc; }, hi, lo);
-        *(ssm_v8h *) (rec + at::c_hi + 2 * (t * NP + n)) = hi;
-        *(ssm_v8h *) (rec + at::c_lo + 2 * (t * NP + n)) = lo;
-    }
-    // B's columns: 16 tokens of one a thread
-    if (tid < NP) {
-        _Float16 * oh = (_Float16 *) (rec + at::b_hi) + tid * kSsmL + 16 * part;
-        _Float16 * ol = (_Float16 *) (rec + at::b_lo) + tid * kSsmL + 16 * part;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float v[8];
-            ssm_v8h hi, lo;
-#pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = sb[16 * part + 8 * h + e][tid];
-            ssm_halves(v, [&](int) { return fb; }, hi, lo);
-            *(ssm_v8h *) (oh + 8 * h) = hi;
-            *(ssm_v8h *) (ol + 8 * h) = lo;
-        }
-    }
-    // C . B: wave w the 16-block of tokens j from 16 w on, K in an order both operands share
+    if (tid == 0) *(uint8_t *) (rec + at::bad + part) = bad != 0;
     const int r = lane & 15, gq = lane >> 4;
-    ssm_v4f acc = {0, 0, 0, 0};
+    for (int kb = wave; kb < at::KB; kb += 4) {
+        ssm_parts p;
+        ssm_parts8(*(const ssm_v4f *) &sc[r][32 * kb + 4 * gq], *(const ssm_v4f *) &sc[r][32 * kb + 16 + 4 * gq], p);
+#pragma unroll
+        for (int i = 0; i < 3; i++) ((ssm_u4 *) (rec + at::c))[((part * at::KB + kb) * 3 + i) * 64 + lane] = p.v[i];
+    }
+    for (int k = wave; k < at::NK; k += 4) {  // a half of each fragment: this quarter's tokens
+        const float * b = &sb[16 * part + 4 * gq][16 * k + r];
+        uint32_t h[2], m[2], l[2];
+        ssm_parts2(b[0], b[kRow], h[0], m[0], l[0]);
+        ssm_parts2(b[2 * kRow], b[3 * kRow], h[1], m[1], l[1]);
+        ssm_u2 * o = (ssm_u2 *) (rec + at::b) + ((part / 2 * at::NK + k) * 3 * 64 + lane) * 2 + part % 2;
+        o[0] = ssm_u2{h[0], h[1]}, o[128] = ssm_u2{m[0], m[1]}, o[256] = ssm_u2{l[0], l[1]};
+    }
+    // C . B: wave w the 16-block of tokens j from 16 w on (rows j, columns t: a
+    // lane ends with its elements), K in an order both operands share, in f32
+    if (wave > (part | 1)) return;
+    ssm_v4f acc = {0, 0, 0, 0}, acc2 = {0, 0, 0, 0};
     if (wave <= part) {
-        ssm_v4f acc2 = {0, 0, 0, 0};
 #pragma unroll 4
-        for (int n = 4 * gq; n < NP; n += 16) {
-            const float4 x = *(const float4 *) &sc[r][n], y = *(const float4 *) &sb[16 * wave + r][n];
+        for (int k = 0; k < at::NK; k++) {
+            const int n = 16 * k + 4 * gq;
+            const float4 x = *(const float4 *) &sb[16 * wave + r][n], y = *(const float4 *) &sc[r][n];
             acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, y.x, acc, 0, 0, 0);
             acc2 = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, y.y, acc2, 0, 0, 0);
             acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, y.z, acc, 0, 0, 0);
             acc2 = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, y.w, acc2, 0, 0, 0);
         }
         acc += acc2;
-    }
-    // rows 4 gq + i, column r: what is past the row's token is not seen
-    __shared__ uint32_t s_row[4][16];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (wave == part && r > 4 * gq + i) acc[i] = 0.0f;
-        const uint32_t m = ssm_group_max<16>(ssm_mag(acc[i]));
-        if (r == 0) s_row[wave][4 * gq + i] = m;
+        for (int i = 0; i < 4; i++)
+            if (wave == part && 4 * gq + i > r) acc[i] = 0.0f;  // past the row's token: not seen
     }
-    __syncthreads();
-    float * cb = (float *) (rec + at::cb) + 16 * part * kSsmL + 16 * wave;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int m = 4 * gq + i;
-        const int k = ssm_scale(max(max(s_row[0][m], s_row[1][m]), max(s_row[2][m], s_row[3][m])));
-        cb[m * kSsmL + r] = acc[i] * ssm_pow2(k);
-        if (wave == 0 && r == 0) ((float *) (rec + at::cb_s))[16 * part + m] = ssm_pow2(-k);
-    }
+    ((ssm_v4f *) (rec + at::cb))[ssm_block(part, wave) * 64 + lane] = acc;
 }
 
-constexpr int kSsmXRow = kSsmL + 8;  // halfs of a staged channel's tokens, padded
-
-template <int NP>
-struct ssm_lds {
-    _Float16 x[4][64][kSsmXRow];  // u for y (hi, lo), u 2^(c_L - c_j) for the state (hi, lo): [channel][token]
-    _Float16 st[2][64][NP + 8];   // the entering state (hi, lo): [channel][n]
-    float whole[kSsmL], frac[kSsmL];  // c_t
-    uint32_t mag[3][4][64];       // a channel's largest x, state, and its first x but 0, by wave
-    float red[4][64];
-    float steps[4][32];           // a wave's tokens' dt, then left (read by their wave only)
-};
-
-// token by token: the chunk's nt tokens from t0 on, for chunks the matrix
-// form cannot take. The state is in LDS (in the place of its split halves,
-// [channel][n]); wave w takes its quarter of n, a lane its channel.
+// token by token: the chunk's nt tokens from t0 on for a wave's 16 channels,
+// for chunks the matrix form cannot take. Lane (g, r) holds n = 16 k + 4 g + i
+// of channel p, as the matrix form does.
 template <int NP, bool OUT>
-__device__ __forceinline__ void ssm_chunk_slow(const ssm_scan_args & a, ssm_lds<NP> & L, int s, int h, int p0, int64_t t0,
-                                               int nt, float A) {
-    int lane = threadIdx.x & 63;
-    asm volatile("" : "+v"(lane));  // (nothing of this path is kept over the caller's loop)
-    const int wave = threadIdx.x >> 6;
-    const int g = h / (a.heads / a.groups), p = p0 + lane;
-    float * st = (float *) &L.st[0][0][0] + lane * (NP + 8);
-    const int n1 = min((wave + 1) * (NP / 4), a.n);
+__device__ __forceinline__ void ssm_tokens(ssm_v4f (&st)[NP / 16], int s, int h, int p, int64_t t0, int nt) {
+    // (the kernel's arguments, read here: kept over the caller's loop, they would spill)
+    SSM_UNIFORM ssm_scan_args * ap = (SSM_UNIFORM ssm_scan_args *) __builtin_amdgcn_kernarg_segment_ptr();
+    static_assert(offsetof(ssm_chunk_args, a) == 0, "the kernel's first argument");
+    asm volatile("" : "+s"(ap));
+    SSM_UNIFORM ssm_scan_args & a = *ap;
+    const float A = *(const float *) (a.A + h * a.A_nb1);
+    const int g = h / (a.heads / a.groups);
+    const bool mine = p < a.dim;
 #pragma unroll 1
     for (int t = 0; t < nt; t++) {
+        int gq = (threadIdx.x & 63) >> 4;
+        asm volatile("" : "+v"(gq));  // (what follows from the lane is made anew: kept, it would spill)
         const float d = ssm_softplus(*(const float *) (a.dt + 4 * h + (t0 + t) * a.dt_nb1 + s * a.dt_nb2));
-        const float ea = __builtin_amdgcn_exp2f(d * A * kLog2e);
+        const float ea = expf(d * A);
         const float * b = (const float *) (a.B + g * a.B_nb1 + (t0 + t) * a.B_nb2 + s * a.B_nb3);
         const float * c = (const float *) (a.C + g * a.C_nb1 + (t0 + t) * a.C_nb2 + s * a.C_nb3);
         const float * x = (const float *) (a.x + h * a.x_nb1 + (t0 + t) * a.x_nb2 + s * a.x_nb3);
-        const float u = p < a.dim ? x[p] * d : 0.0f;
+        const float u = mine ? x[p] * d : 0.0f;
         float y = 0.0f;
-#pragma unroll 1
-        for (int n = wave * (NP / 4); n < n1; n++) {
-            st[n] = fmaf(st[n], ea, u * b[n]);
-            y = fmaf(st[n], c[n], y);
+#pragma unroll
+        for (int k = 0; k < NP / 16; k++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int n = 16 * k + 4 * gq + i, at = min(n, a.n - 1);
+                const float v = fmaf(st[k][i], ea, u * b[at]);
+                st[k][i] = mine && n < a.n ? v : 0.0f;
+                if constexpr (OUT) y = n < a.n ? fmaf(v, c[at], y) : y;
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (one tile's loads at a time)
         }
         if constexpr (OUT) {
-            L.red[wave][lane] = y;
-            __syncthreads();
-            if (wave == 0 && p < a.dim)
-                a.y[((s * a.tokens + t0 + t) * a.heads + h) * a.dim + p] =
-                    (L.red[0][lane] + L.red[1][lane]) + (L.red[2][lane] + L.red[3][lane]);
-            __syncthreads();
+            y += __shfl_xor(y, 16);
+            y += __shfl_xor(y, 32);
+            if (gq == 0 && mine) a.y[((s * a.tokens + t0 + t) * a.heads + h) * a.dim + p] = y;
         }
     }
 }
 
-// (what the launch before wrote and all lanes read alike: scalar loads)
-#define SSM_UNIFORM const __attribute__((address_space(4)))
+// 16 bytes a lane of N KB from a record straight to LDS, wave w of eight its
+// share of them. What it writes is there after ssm_staged.
+template <int N>
+__device__ __forceinline__ void ssm_stage(const char * from, ssm_u4 * lds, int wave, uint32_t lane) {
+    static_assert(N % 8 == 0, "as much for every wave");
+#pragma unroll
+    for (int k = 0; k < N / 8; k++)
+        __builtin_amdgcn_global_load_lds(
+            (const void __attribute__((address_space(1))) *) &ssm_at<const char>(from, 16 * lane + 1024u * (uint32_t) wave + 8192u * k),
+            (void __attribute__((address_space(3))) *) (lds + 64 * (8 * k + wave)), 16, 0, 0);
+}
+// every wave's requests have arrived, and what they wrote to LDS is seen by all
+__device__ __forceinline__ void ssm_staged() {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0 (gfx9 encoding), the others as they are
+    __syncthreads();
+}
+
+// lane q of each four holds v[e] of row q, and is given v[q] of row e: across
+// neighbours, then across pairs
+__device__ __forceinline__ void ssm_turn(ssm_v4f & v, int lane) {
+    auto swap = [&](bool upper, auto ctrl, float & lo, float & hi) {
+        const int got = __builtin_amdgcn_update_dpp(0, __float_as_int(upper ? lo : hi), decltype(ctrl)::value, 0xf, 0xf, true);
+        if (upper) lo = __int_as_float(got);
+        else hi = __int_as_float(got);
+    };
+    float a = v[0], b = v[1], c = v[2], d = v[3];
+    const std::integral_constant<int, 0xB1> next;  // quad_perm 1, 0, 3, 2
+    const std::integral_constant<int, 0x4E> pair;  // quad_perm 2, 3, 0, 1
+    swap(lane & 1, next, a, b);
+    swap(lane & 1, next, c, d);
+    swap(lane & 2, pair, a, c);
+    swap(lane & 2, pair, b, d);
+    v = ssm_v4f{a, b, c, d};
+}
+
+// A step's instructions in order: 12 matrix ones with V vector ones under each,
+// R reads of LDS after the third. (While requests to LDS are in flight a wait
+// for the step before's reads is a wait for all there are: these come after it.)
+template <int R, int V>
+__device__ __forceinline__ void ssm_interleave() {
+#pragma unroll
+    for (int i = 0; i < 12; i++) {
+        if (i == 3) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
 
 template <int NP, bool OUT>
-__global__ __launch_bounds__(256, NP == 256 ? 1 : 2) void k_ssm_chunks(ssm_chunk_args q) {
-    constexpr int NT = NP / 64;  // 16-row tiles of the state a wave owns
-    __shared__ __align__(16) ssm_lds<NP> L;
+__global__ __launch_bounds__(512, 2) void k_ssm_chunks(ssm_chunk_args q) {
+    using at = ssm_shared_at<NP>;
+    constexpr int NK = at::NK, KB = at::KB;
+    // Room for C's fragments and B's (OUT false: B's of two chunks); for states
+    // of 256 for one of them at a time.
+    constexpr bool kOne = NP > 128;
+    __shared__ ssm_u4 s_c[12 * KB * 64];
+    __shared__ ssm_u4 s_other[kOne ? 1 : 6 * NK * 64];
+    static_assert(12 * KB == 6 * NK, "C and B are of one size");
+    __shared__ ssm_u4 s_m[OUT ? 2 * 6 * 3 * 64 : 1];  // a block's C . B times the decays between: [fragment][part]
+    __shared__ float s_dec[2][2][ssm_head_at::tokens][kSsmL];
     const ssm_scan_args & a = q.a;
-    const int lane = threadIdx.x & 63, r = lane & 15, gq = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
-    const int unit = blockIdx.x, seg = blockIdx.y;
-    const int pb = unit % q.pblocks, h = unit / q.pblocks % a.heads, s = unit / (q.pblocks * a.heads);
-    const int g = h / (a.heads / a.groups), p0 = 64 * pb;
+    const int tid = threadIdx.x;
+    // eight waves: four a block
+    const int first_wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = first_wave >> 2;
+    const int seg = blockIdx.y;
+    const int g = (int) (blockIdx.x / q.pairs % a.groups), s = (int) (blockIdx.x / q.pairs / a.groups);
+    const int per = a.heads / a.groups, blocks = per * q.pblocks;
+    const int of_group = 2 * (int) (blockIdx.x % q.pairs) + half, blk = min(of_group, blocks - 1);
+    const int h = g * per + blk / q.pblocks, pb = blk % q.pblocks, unit = (s * a.heads + h) * q.pblocks + pb;
+    const int first_p = 64 * pb + 16 * (first_wave & 3);
+    const bool idle = of_group >= blocks || first_p >= a.dim;  // the wave has no channel: it only stages
     const int64_t sg = (int64_t) s * a.groups + g, sh = (int64_t) s * a.heads + h;
-    const float A = *(const float *) (a.A + h * a.A_nb1);
-    const int nbase = wave * (NP / 4);
 
-    // the state: rows n = nbase + 16 k + 4 gq + i, channels 16 pt + r; its
-    // value times 2^ks[pt] (channel lane: 2^kst)
-    ssm_v4f st[NT][4];
-    int ks[4] = {0, 0, 0, 0}, kst = 0;
+    ssm_v4f st[NK];  // n = 16 k + 4 gq + i, channel p
     {
-        float carry = 1.0f;
+        const int lane = tid & 63, r = lane & 15, gq = lane >> 4, p = first_p + r;
+        ssm_power carry = {1.0f, 0.0f};
         if constexpr (OUT) {
             double d = 0.0;
             for (int m = 0; m < seg; m++) d += q.seg_decay[sh * q.segs + m];
-            carry = __builtin_amdgcn_exp2f((float) d);
+            carry = ssm_split_power(d);
         }
         const int64_t slot = a.ids[s];
-        const bool has = OUT && slot >= 0 && slot < a.slots;
-        const float * s0 = (const float *) (a.s + (has ? slot : 0) * a.s_nb3) + (int64_t) h * a.dim * a.n;
+        const bool has = OUT && slot >= 0 && slot < a.slots && p < a.dim;
+        const float * s0 = (const float *) (a.s + (has ? slot : 0) * a.s_nb3) + ((int64_t) h * a.dim + p) * a.n;
 #pragma unroll
-        for (int k = 0; k < NT; k++)
-#pragma unroll
-            for (int pt = 0; pt < 4; pt++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int n = nbase + 16 * k + 4 * gq + i, p = p0 + 16 * pt + r;
-                    st[k][pt][i] = has && n < a.n && p < a.dim ? s0[(int64_t) p * a.n + n] * carry : 0.0f;
-                }
-        if constexpr (OUT) {
-            for (int m = 0; m < seg; m++) {
-                double d = 0.0;
-                for (int e = m + 1; e < seg; e++) d += q.seg_decay[sh * q.segs + e];
-                const float f = __builtin_amdgcn_exp2f((float) d);
-                const float * o = q.seg_state + ((int64_t) unit * q.segs + m) * 64 * NP;
-#pragma unroll
-                for (int k = 0; k < NT; k++)
-#pragma unroll
-                    for (int pt = 0; pt < 4; pt++) {
-                        const float4 v = *(const float4 *) (o + (16 * pt + r) * NP + nbase + 16 * k + 4 * gq);
-                        st[k][pt][0] = fmaf(v.x, f, st[k][pt][0]);
-                        st[k][pt][1] = fmaf(v.y, f, st[k][pt][1]);
-                        st[k][pt][2] = fmaf(v.z, f, st[k][pt][2]);
-                        st[k][pt][3] = fmaf(v.w, f, st[k][pt][3]);
-                    }
-            }
-        }
-    }
-    const int64_t c0 = (int64_t) seg * q.seg_chunks, c1 = min(c0 + q.seg_chunks, q.chunks);
-    const int64_t yrow = (int64_t) a.heads * a.dim;
-    const char * const xbase = a.x + h * a.x_nb1 + s * a.x_nb3;
-    using at = ssm_shared_at<NP>;
-    const char * gp = q.shared + (sg * q.chunks + c0) * at::size;              // the chunk's records
-    const char * hp = q.heads + (sh * q.chunks + c0) * ssm_head_at::size;
-    // the next chunk's x and c_t, in flight under this one's products
-    float xn[16], stepn = 0.0f, wholen = 0.0f, fracn = 0.0f;
-    // (a lane's part of an address in 32 bits, the rest uniform)
-    auto load_next = [&](int64_t c, const char * hp, int lane) {
-        const uint32_t xo = 4u * (uint32_t) (p0 + lane < a.dim ? p0 + lane : 0), lo4 = 4u * (uint32_t) lane;
-        // lanes 0 .. 15 the wave's dt, 16 .. 31 its left
-        stepn = ssm_at<const float>(hp + 64 * wave, 4u * (uint32_t) ((lane & 15) + 4 * (lane & 16)));
-        if (OUT && wave == 0) {
-            wholen = ssm_at<const float>(hp, lo4, ssm_head_at::whole);
-            fracn = ssm_at<const float>(hp, lo4, ssm_head_at::frac);
-        }
-        // rows from the wave's first token on, the last token's again past it
-        const int64_t t = min(c * kSsmL + 16 * wave, a.tokens - 1);
-        const char * row = xbase + t * a.x_nb2;
-        const int left = (int) min((int64_t) 16, a.tokens - 1 - t);
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            xn[i] = ssm_at<const float>(row, xo);
-            row += i < left ? a.x_nb2 : 0;
-        }
-    };
-    if (c0 < c1) load_next(c0, hp, lane);
-    double decayed = 0.0;
-    for (int64_t c = c0; c < c1; c++, gp += at::size, hp += ssm_head_at::size) {
-        // The lane is unknown to the compiler anew in every iteration: the
-        // addresses that follow from it, kept over the loop, would spill, and
-        // a spill's reload waits for every load in flight.
-        int lane = threadIdx.x & 63;
-        asm volatile("" : "+v"(lane));
-        const int r = lane & 15, gq = lane >> 4, px = p0 + lane;  // px: the channel this lane stages
-        const uint32_t co = 2u * (uint32_t) ((16 * wave + r) * NP + 8 * gq);
-        const uint32_t bo = 2u * (uint32_t) ((nbase + r) * kSsmL + 8 * gq);
-        const uint32_t cbo = 4u * (uint32_t) ((16 * wave + r) * kSsmL + 8 * gq), cso = 4u * (uint32_t) (16 * wave + 4 * gq);
-        const uint32_t yo = 4u * ((uint32_t) (16 * wave + 4 * gq) * (uint32_t) yrow + (uint32_t) r);
-        const int64_t t0 = c * kSsmL;
-        const int nt = (int) min((int64_t) kSsmL, a.tokens - t0);
-        const bool inside = nt == kSsmL && p0 + 64 <= a.dim;
-        SSM_UNIFORM ssm_decay * dec = (SSM_UNIFORM ssm_decay *) (hp + ssm_head_at::decay);
-        SSM_UNIFORM ssm_flags * fl = (SSM_UNIFORM ssm_flags *) (gp + at::flags);
-        static_assert(ssm_head_at::left == 256 && ssm_head_at::dt == 0, "the lanes' offsets of dt and left");
-        if (lane < 32) L.steps[wave][lane] = stepn;
-        const double total = dec->total;
-        const int e_dt = dec->e_dt, e_left = dec->e_left, odd = dec->odd;
-        const int bad = fl->bad[0] | fl->bad[1] | fl->bad[2] | fl->bad[3], kb = fl->kb;
-        const float whole = wholen, frac = fracn;
-        float x[16];
-        uint32_t mx = 0, first = 0;
-#pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = xn[i];
-        if (!inside) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) x[i] = px < a.dim && 16 * wave + i < nt ? x[i] : 0.0f;
-        }
-        if (!OUT && c + 1 < c1) load_next(c + 1, hp + ssm_head_at::size, lane);
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            mx = max(mx, ssm_mag(x[i]));
-            first = first ? first : mx;
-        }
-#pragma unroll
-        for (int pt = 0; pt < 4; pt++) {
-            uint32_t m = 0;
-#pragma unroll
-            for (int k = 0; k < NT; k++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) m = max(m, ssm_mag(st[k][pt][i]));
-            m = max(m, (uint32_t) __shfl_xor((int) m, 16));
-            m = max(m, (uint32_t) __shfl_xor((int) m, 32));
-            if (gq == 0) L.mag[1][wave][16 * pt + r] = m;
-        }
-        L.mag[0][wave][lane] = mx;
-        L.mag[2][wave][lane] = first;
-        __syncthreads();  // the magnitudes; every wave is done with the chunk before
-        // The chunk's operands, requested where the arithmetic up to their use
-        // covers their latency, and ahead of the next chunk's x: loads return
-        // in order, and x comes from HBM.
-        ssm_v8h ch[OUT ? NP / 32 : 1], cl[OUT ? NP / 32 : 1];
-        float cbv[2][8], cs[4], cbs[4];
-        if constexpr (OUT) {
-#pragma unroll
-            for (int kk = 0; kk < NP / 32; kk++) {
-                ch[kk] = ssm_at<const ssm_v8h>(gp + at::c_hi, co, 64 * kk);
-                cl[kk] = ssm_at<const ssm_v8h>(gp + at::c_lo, co, 64 * kk);
-            }
-#pragma unroll
-            for (int kk = 0; kk < 2; kk++) {
-                *(float4 *) &cbv[kk][0] = ssm_at<const float4>(gp + at::cb, cbo, 128 * kk);
-                *(float4 *) &cbv[kk][4] = ssm_at<const float4>(gp + at::cb, cbo, 128 * kk + 16);
-            }
-            *(float4 *) cs = ssm_at<const float4>(gp + at::c_s, cso);
-            *(float4 *) cbs = ssm_at<const float4>(gp + at::cb_s, cso);
-        }
-        mx = max(max(L.mag[0][0][lane], L.mag[0][1][lane]), max(L.mag[0][2][lane], L.mag[0][3][lane]));
-        const uint32_t ms = max(max(L.mag[1][0][lane], L.mag[1][1][lane]), max(L.mag[1][2][lane], L.mag[1][3][lane]));
-        first = L.mag[2][0][lane] ? L.mag[2][0][lane] : L.mag[2][1][lane] ? L.mag[2][1][lane]
-                : L.mag[2][2][lane] ? L.mag[2][2][lane] : L.mag[2][3][lane];
-        // one step of the exponent is 2^23 in a float's bits
-        const bool rising = (mx >> 23) > (first >> 23) + 24;
-        decayed += total;
-        // the same for every wave: they see the same magnitudes
-        if (bad || odd || __any(rising || !ssm_finite(mx) || !ssm_finite(ms))) {
-            float * sl = (float *) &L.st[0][0][0];
-            static_assert(sizeof(L.st) == sizeof(float) * 64 * (NP + 8), "the state fits in place of its halves");
-#pragma unroll
-            for (int k = 0; k < NT; k++)
-#pragma unroll
-                for (int pt = 0; pt < 4; pt++)
-                    *(ssm_v4f *) (sl + (16 * pt + r) * (NP + 8) + nbase + 16 * k + 4 * gq) = st[k][pt] * ldexpf(1.0f, -ks[pt]);
-            __syncthreads();
-            ssm_chunk_slow<NP, OUT>(a, L, s, h, p0, t0, nt, A);
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < NT; k++)
-#pragma unroll
-                for (int pt = 0; pt < 4; pt++)
-                    st[k][pt] = *(const ssm_v4f *) (sl + (16 * pt + r) * (NP + 8) + nbase + 16 * k + 4 * gq);
-#pragma unroll
-            for (int pt = 0; pt < 4; pt++) ks[pt] = 0;
-            kst = 0;
-            __syncthreads();
-            if (OUT && c + 1 < c1) load_next(c + 1, hp + ssm_head_at::size, lane);
-            continue;
-        }
-        // Channel lane's exponents: x 2^kx below 2^14, so u below 2^15 over the
-        // steps' exponent; the state, in its units, 2^km below 2^14. The
-        // state's next units are those its new terms are staged in, 2^kv (at
-        // most 2^30 finer than it needs: far from f32's ends).
-        const int kx = ssm_scale(mx), km = ssm_scale(ms);
-        int kv = min(kx - e_left + kb, 120);
-        if (ms) kv = min(kv, kst + km + 30);
-        int kxp[4], kmp[4], kvp[4];  // of the accumulators' channels
-#pragma unroll
-        for (int pt = 0; pt < 4; pt++) {
-            kxp[pt] = __shfl(kx, 16 * pt + r);
-            kmp[pt] = __shfl(km, 16 * pt + r);
-            kvp[pt] = __shfl(kv, 16 * pt + r);
-        }
-        kst = kv;
-        {
-            const float fx = ssm_pow2(kx), fv = ldexpf(1.0f, kv + e_left - kb);
-            const float *dts = L.steps[wave], *lefts = L.steps[wave] + 16;
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                float xs[8];
-                ssm_v8h hi, lo;
-                const int to = 16 * wave + 8 * half;
-                if constexpr (OUT) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) xs[e] = x[8 * half + e] * fx;
-                    ssm_halves(xs, [&](int e) { return dts[8 * half + e]; }, hi, lo);
-                    *(ssm_v8h *) &L.x[0][lane][to] = hi;
-                    *(ssm_v8h *) &L.x[1][lane][to] = lo;
-                }
-#pragma unroll
-                for (int e = 0; e < 8; e++) xs[e] = x[8 * half + e] * fv;
-                ssm_halves(xs, [&](int e) { return lefts[8 * half + e]; }, hi, lo);
-                *(ssm_v8h *) &L.x[2][lane][to] = hi;
-                *(ssm_v8h *) &L.x[3][lane][to] = lo;
-            }
-        }
-        if (OUT && c + 1 < c1) load_next(c + 1, hp + ssm_head_at::size, lane);
-        if constexpr (OUT) {
-#pragma unroll
-            for (int k = 0; k < NT; k++)
-#pragma unroll
-                for (int pt = 0; pt < 4; pt++) {
-                    const float fs = ssm_pow2(kmp[pt]);
-                    float v[4];
-                    ssm_v4h hi, lo;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) v[i] = st[k][pt][i];
-                    ssm_halves(v, [&](int) { return fs; }, hi, lo);
-                    const int n = nbase + 16 * k + 4 * gq;
-                    *(ssm_v4h *) &L.st[0][16 * pt + r][n] = hi;
-                    *(ssm_v4h *) &L.st[1][16 * pt + r][n] = lo;
-                }
-            if (wave == 0) {
-                L.whole[lane] = whole;
-                L.frac[lane] = frac;
-            }
-        }
-        ssm_v8h bh[2][NT], bl[2][NT];
-        auto load_b = [&] {
-#pragma unroll
-            for (int kk = 0; kk < 2; kk++)
-#pragma unroll
-                for (int k = 0; k < NT; k++) {
-                    bh[kk][k] = ssm_at<const ssm_v8h>(gp + at::b_hi, bo, 32 * k * kSsmL + 64 * kk);
-                    bl[kk][k] = ssm_at<const ssm_v8h>(gp + at::b_lo, bo, 32 * k * kSsmL + 64 * kk);
-                }
-        };
-        if constexpr (!OUT) load_b();
-        __syncthreads();
-        if constexpr (OUT) {
-            ssm_v4f yh[4], yx[4];
-#pragma unroll
-            for (int pt = 0; pt < 4; pt++) yh[pt] = yx[pt] = ssm_v4f{0, 0, 0, 0};
-            ssm_v8h oh[4], ol[4];
-            // H C_t
-#pragma unroll
-            for (int kk = 0; kk < NP / 32; kk++) {
-#pragma unroll
-                for (int pt = 0; pt < 4; pt++) {
-                    oh[pt] = *(const ssm_v8h *) &L.st[0][16 * pt + r][32 * kk + 8 * gq];
-                    ol[pt] = *(const ssm_v8h *) &L.st[1][16 * pt + r][32 * kk + 8 * gq];
-                }
-                ssm_products(ch[kk], cl[kk], oh, ol, yh);
-                // (one K step's operands at a time: more in flight spill)
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            load_b();  // (in the registers that held C)
-            __builtin_amdgcn_sched_barrier(0);
-            // the chunk's own tokens: the decayed C . B of this lane's row (the
-            // 16-blocks past the wave's tokens are zeros; a decay is at most one)
-            const float tw = L.whole[16 * wave + r], tf = L.frac[16 * wave + r];
-#pragma unroll
-            for (int kk = 0; kk < 2; kk++) {
-                if (kk == 1 && wave < 2) continue;
-                float jw[8], jf[8], m[8];
-                *(float4 *) &jw[0] = *(const float4 *) &L.whole[32 * kk + 8 * gq];
-                *(float4 *) &jw[4] = *(const float4 *) &L.whole[32 * kk + 8 * gq + 4];
-                *(float4 *) &jf[0] = *(const float4 *) &L.frac[32 * kk + 8 * gq];
-                *(float4 *) &jf[4] = *(const float4 *) &L.frac[32 * kk + 8 * gq + 4];
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    m[e] = __builtin_amdgcn_exp2f(fminf((tw - jw[e]) + (tf - jf[e]), 0.0f));
-                ssm_v8h ah, al;
-                ssm_halves(m, [&](int e) { return cbv[kk][e]; }, ah, al);
-#pragma unroll
-                for (int pt = 0; pt < 4; pt++) {
-                    oh[pt] = *(const ssm_v8h *) &L.x[0][16 * pt + r][32 * kk + 8 * gq];
-                    ol[pt] = *(const ssm_v8h *) &L.x[1][16 * pt + r][32 * kk + 8 * gq];
-                }
-                ssm_products(ah, al, oh, ol, yx);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            float fh[4], fxr[4], fk[4], fu[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {  // rows: the tokens 16 wave + 4 gq + i
-                const int tr = 16 * wave + 4 * gq + i;
-                fh[i] = __builtin_amdgcn_exp2f(L.whole[tr] + L.frac[tr]) * cs[i];
-                fxr[i] = cbs[i] * ssm_pow2(e_dt);
-            }
-#pragma unroll
-            for (int pt = 0; pt < 4; pt++) {
-                fk[pt] = ldexpf(1.0f, -ks[pt] - kmp[pt]);
-                fu[pt] = ssm_pow2(-kxp[pt]);
-            }
-            float * yp = a.y + (((s * a.tokens + t0) * a.heads + h) * a.dim + p0);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int pt = 0; pt < 4; pt++)
-                    yh[pt][i] = fmaf(yh[pt][i], fk[pt] * fh[i], yx[pt][i] * (fu[pt] * fxr[i]));
-            if (inside) {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int pt = 0; pt < 4; pt++) ssm_at<float>(yp + i * yrow, yo, 64 * pt) = yh[pt][i];
+        for (int k = 0; k < NK; k++) {
+            const int n = 16 * k + 4 * gq;
+            st[k] = ssm_v4f{0, 0, 0, 0};
+            if (q.svec) {
+                if (has && n < a.n) st[k] = *(const ssm_v4f *) (s0 + n);
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; i++)
+                    if (has && n + i < a.n) st[k][i] = s0[n + i];
+            }
+        }
+        if constexpr (OUT) {
 #pragma unroll
-                    for (int pt = 0; pt < 4; pt++)
-                        if (16 * wave + 4 * gq + i < nt && p0 + 16 * pt + r < a.dim)
-                            ssm_at<float>(yp + i * yrow, yo, 64 * pt) = yh[pt][i];
+            for (int k = 0; k < NK; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) st[k][i] = ssm_decayed(st[k][i], carry.frac, carry.whole);
+            for (int m = 0; m < seg; m++) {
+                double d = 0.0;
+                for (int e = m + 1; e < seg; e++) d += q.seg_decay[sh * q.segs + e];
+                const ssm_power f = ssm_split_power(d);
+                const ssm_v4f * o = (const ssm_v4f *) q.seg_state + (((int64_t) unit * q.segs + m) * 4 + (first_wave & 3)) * NK * 64 + lane;
+#pragma unroll
+                for (int k = 0; k < NK; k++) {
+                    const ssm_v4f v = o[64 * k];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) st[k][i] += ssm_decayed(v[i], f.frac, f.whole);
+                }
+            }
+        }
+    }
+    const int c0 = seg * q.seg_chunks, c1 = (int) min((int64_t) c0 + q.seg_chunks, q.chunks);
+    // (a lane's part of an address in 32 bits, the rest uniform)
+    const uint32_t yrow = (uint32_t) (a.heads * a.dim);
+    char * ybase = (char *) (a.y + ((s * a.tokens + (int64_t) c0 * kSsmL) * a.heads + h) * a.dim);
+    const char * const xbase = a.x + h * a.x_nb1 + s * a.x_nb3;
+    const char * gp = q.shared + (sg * q.chunks + c0) * at::size;              // the chunk's records
+    const char * hp = q.heads + (sh * q.chunks + c0) * ssm_head_at::size;
+    // A chunk's C, C . B, x and decays (OUT false: B for C) are in flight under
+    // the products before, its B under those of its own C.
+    ssm_v4f cbn[OUT ? 3 : 1], xn[4], dtn[4];
+    float dn[2];
+    int next_kind = 0, next_bad = 0;
+    auto load_next = [&](int c, bool more, const char * gp, const char * hp, int tid, int wave, auto to_other) {
+        const uint32_t lane = tid & 63, gq = lane >> 4, nb = (uint32_t) a.x_nb2;
+        // token 4 gq + r % 4, channels r / 4 * 4 ..: make_u turns them over (rows
+        // past the last token: that one again)
+        const char * row = xbase + (int64_t) c * kSsmL * a.x_nb2;
+        const uint32_t last = (uint32_t) min((int64_t) kSsmL, a.tokens - (int64_t) c * kSsmL) - 1;
+        const int p = 64 * pb + 16 * (wave & 3) + (tid & 12);
+        if (q.xvec) {
+#pragma unroll
+            for (int b = 0; b < 4; b++)
+                xn[b] = ssm_at<const ssm_v4f>(row, 4u * (uint32_t) min(p, a.dim - 4) + min(16u * b + 4 * gq + (tid & 3), last) * nb);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; k++)
+                xn[k / 4][k % 4] = ssm_at<const float>(row, 4u * (uint32_t) min(p + k % 4, a.dim - 1) +
+                                                                min(16u * (k / 4) + 4 * gq + (tid & 3), last) * nb);
+        }
+        next_kind = *(SSM_UNIFORM int *) (hp + ssm_head_at::decay + offsetof(ssm_decay, kind));
+        next_bad = *(SSM_UNIFORM int *) (gp + at::bad);
+        dn[0] = ssm_at<const float>(hp, 4u * (uint32_t) (tid & 255));
+        dn[1] = ssm_at<const float>(hp + 1024, 4u * (uint32_t) (tid & 127));
+#pragma unroll
+        for (int b = 0; b < 4; b++) dtn[b] = ssm_at<const ssm_v4f>(hp, 16 * gq + 64 * b);
+        // (behind the others: a wait for those does not wait for it)
+        if (!kOne && more) ssm_stage<12 * KB>(gp + (OUT ? at::c : at::b), decltype(to_other)::value ? s_other : s_c, wave, lane);
+    };
+    auto load_cb = [&](const char * gp, int tid, int wave) {
+        const uint32_t lane = tid & 63;
+        if constexpr (OUT) {
+#pragma unroll
+            for (int k = 0; k < 3; k++) cbn[k] = ssm_at<const ssm_v4f>(gp + at::cb, 1024u * (uint32_t) ((wave & 3) + 4 * k) + 16 * lane);
+        }
+    };
+    // that chunk's u: channel p, tokens 16 b + 4 gq + i. (A token past the last
+    // has a step of zero; channels past the last are never stored.)
+    auto make_u = [&](int b, int tid, ssm_v4f & u) {
+        u = xn[b];
+        ssm_turn(u, tid);
+        u *= dtn[b];
+    };
+    static_assert(ssm_head_at::tokens * kSsmL == 384 && ssm_head_at::decay == 4 * 384, "the threads' share of the decays");
+    enum { kDt, kLeft, kLeftWhole, kIn, kWhole, kFrac };
+    // whether the wave's states are past what the matrix form takes: at the
+    // start, and after chunks it did not
+    auto large_state = [&] {
+        ssm_most most;
+#pragma unroll
+        for (int k = 0; k < NK; k++) most.add(st[k][0], st[k][1]), most.add(st[k][2], st[k][3]);
+        return (bool) __any(most.past(kSsmLargestState));
+    };
+    bool large = large_state();
+    ssm_v4f u[4];
+    if (c0 < c1) {
+        load_next(c0, true, gp, hp, tid, first_wave, std::false_type{});
+        load_cb(gp, tid, first_wave);
+#pragma unroll
+        for (int b = 0; b < 4; b++) make_u(b, tid, u[b]);
+    }
+    auto next = [&] { gp += at::size, hp += ssm_head_at::size, ybase += 4 * kSsmL * (int64_t) yrow; };
+    // OUT false: odd chunks' B is in the other room (as types: reads of one room
+    // do not wait for requests to the other)
+    auto chunk = [&](int c, auto odd) {
+        constexpr bool kOdd = decltype(odd)::value;
+        // The lane and the wave are unknown to the compiler anew in every
+        // iteration: what follows from them, kept over the loop, would spill.
+        int tid = threadIdx.x, wave = first_wave;
+        asm volatile("" : "+v"(tid), "+s"(wave));
+        const int lane = tid & 63, r = lane & 15, gq = lane >> 4, w = wave & 3;
+        const int64_t t0 = (int64_t) c * kSsmL;
+        const int nt = (int) min((int64_t) kSsmL, a.tokens - t0);
+        float (&dec)[ssm_head_at::tokens][kSsmL] = s_dec[c & 1][wave >> 2];
+        const bool deep = next_kind & kSsmDeep, apart = (next_kind & kSsmOdd) || next_bad;
+        (&dec[0][0])[tid & 255] = dn[0];
+        if ((tid & 255) < 128) (&dec[0][0])[256 + (tid & 127)] = dn[1];
+        ssm_most most;
+#pragma unroll
+        for (int b = 0; b < 4; b++) most.add(u[b][0], u[b][1]), most.add(u[b][2], u[b][3]);
+        const bool by_token = apart || large || __any(most.past(kSsmLargest));
+        if constexpr (kOne) {
+            __syncthreads();  // the products of the chunk before have read B
+            ssm_stage<12 * KB>(gp + (OUT ? at::c : at::b), s_c, wave, lane);
+        }
+        ssm_staged();  // C (OUT false: B) and the decays; the products of the chunk before have read B and the decayed C . B
+        ssm_v4f y[4];  // token 16 tb + r, channels 16 w + 4 gq + i
+        ssm_parts us[2];
+        ssm_u4 * const sm = s_m + (OUT ? (wave >> 2) * 6 * 3 * 64 : 0);
+        if constexpr (OUT) {
+            // (reads of the decays before requests to LDS: behind them they would wait)
+            float tw[3], tf[3], e[4];
+            ssm_v4f jw[3], jf[3];
+#pragma unroll
+            for (int k = 0; k < 3; k++) {
+                const int tb = k == 0 ? w >> 1 : 1 + k, jb = k == 0 ? w & 1 : w;
+                tw[k] = dec[kWhole][16 * tb + r], tf[k] = dec[kFrac][16 * tb + r];
+                jw[k] = *(const ssm_v4f *) &dec[kWhole][16 * jb + 4 * gq], jf[k] = *(const ssm_v4f *) &dec[kFrac][16 * jb + 4 * gq];
+            }
+#pragma unroll
+            for (int tb = 0; tb < 4; tb++) e[tb] = dec[kIn][16 * tb + r];
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (!kOne) ssm_stage<6 * NK>(gp + at::b, s_other, wave, lane);
+            // the decayed C . B: three blocks a wave, half a fragment each
+#pragma unroll
+            for (int k = 0; k < 3; k++) {
+                const int i = w + 4 * k;
+#pragma unroll
+                for (int v = 0; v < 4; v++) cbn[k][v] = ssm_decayed(cbn[k][v], __builtin_amdgcn_exp2f(tf[k] - jf[k][v]), tw[k] - jw[k][v]);
+                uint32_t h[2], m[2], l[2];
+                ssm_parts2(cbn[k][0], cbn[k][1], h[0], m[0], l[0]);
+                ssm_parts2(cbn[k][2], cbn[k][3], h[1], m[1], l[1]);
+                ssm_u2 * o = (ssm_u2 *) sm + ((i / 2) * 3 * 64 + lane) * 2 + i % 2;
+                o[0] = ssm_u2{h[0], h[1]}, o[128] = ssm_u2{m[0], m[1]}, o[256] = ssm_u2{l[0], l[1]};
+            }
+            if (!idle && !by_token) {
+                // H C_t: a step takes 32 n and 32 tokens. The next step's fragments
+                // are read under its products, with a share of the vector work
+                // beside them: the state's next parts, then those of u.
+                ssm_parts f[2][2], hs[2];
+                auto read = [&](int m, ssm_parts (&v)[2]) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+#pragma unroll
+                        for (int i = 0; i < 3; i++) v[e].v[i] = s_c[(((2 * (m & 1) + e) * KB + m / 2) * 3 + i) * 64 + lane];
+                };
+#pragma unroll
+                for (int tb = 0; tb < 4; tb++) y[tb] = ssm_v4f{0, 0, 0, 0};
+                if constexpr (!kOne) read(0, f[0]);
+                ssm_parts8(st[0], st[1], hs[0]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int m = 0; m < 2 * KB; m++) {
+                    if constexpr (kOne) read(m, f[m & 1]);
+                    else if (m + 1 < 2 * KB) read(m + 1, f[(m + 1) & 1]);
+                    if ((m & 1) && m + 1 < 2 * KB) ssm_parts8(st[m + 1], st[m + 2], hs[(m / 2 + 1) & 1]);
+                    if (m == 2 * KB - 1) ssm_parts8(u[0], u[1], us[0]);
+#pragma unroll
+                    for (int i = 0; i < 6; i++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) y[2 * (m & 1) + e] = ssm_product(i, hs[m / 2 & 1], f[m & 1][e], y[2 * (m & 1) + e]);
+                    ssm_interleave<6, 4>();
+                }
+#pragma unroll
+                for (int tb = 0; tb < 4; tb++) y[tb] *= e[tb];
+                if (deep)
+#pragma unroll
+                    for (int tb = 0; tb < 4; tb++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) y[tb][i] = ldexpf(y[tb][i], (int) dec[kWhole][16 * tb + r]);
+            }
+        }
+        if constexpr (OUT && kOne) {
+            __syncthreads();  // the products have read C
+            ssm_stage<6 * NK>(gp + at::b, s_c, wave, lane);
+        }
+        const ssm_u4 * const s_b = OUT ? (kOne ? s_c : s_other) : (!kOne && kOdd ? s_other : s_c);
+        if constexpr (OUT) ssm_staged();  // B and the decayed C . B; the products have read C
+        tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        const int lane2 = tid & 63, r2 = lane2 & 15, gq2 = lane2 >> 4;
+        const float ef = dec[kIn][63];
+        __builtin_amdgcn_sched_barrier(0);
+        const bool more = c + 1 < c1;
+        // (at the end the last chunk's loads again, unused: no branch around what a
+        // register waits for. But no request to LDS: none may outlive the kernel.)
+        const char *const gn = more ? gp + at::size : gp, *const hn = more ? hp + ssm_head_at::size : hp;
+        load_next(more ? c + 1 : c, more, gn, hn, tid, wave, std::integral_constant<bool, !OUT && !kOdd>{});
+        if (idle) {
+            load_cb(gn, tid, wave);
+            return next();
+        }
+        if (by_token) {
+            load_cb(gn, tid, wave);
+            ssm_tokens<NP, OUT>(st, s, h, 64 * pb + 16 * w + r2, t0, nt);
+            large = large_state();
+#pragma unroll
+            for (int b = 0; b < 4; b++) make_u(b, tid, u[b]);
+            return next();
+        }
+        ssm_parts f[2][2], left_us[2];
+        // the parts of 32 tokens' u, decayed to the chunk's end
+        ssm_v4f left[2];
+        ssm_i4 left_whole[2];
+        auto read_left = [&](int m) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                left[e] = *(const ssm_v4f *) &dec[kLeft][32 * m + 16 * e + 4 * gq2];
+                left_whole[e] = *(const ssm_i4 *) &dec[kLeftWhole][32 * m + 16 * e + 4 * gq2];
+            }
+        };
+        auto make_left = [&](int m) {
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) left[e][i] = ldexpf(u[2 * m + e][i] * left[e][i], left_whole[e][i]);
+            ssm_parts8(left[0], left[1], left_us[m]);
+        };
+        auto read_b = [&](int m, ssm_parts (&v)[2]) {  // step m of the state's: 32 tokens, 32 n
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int i = 0; i < 3; i++) v[e].v[i] = s_b[((m / KB * NK + 2 * (m % KB) + e) * 3 + i) * 64 + lane2];
+        };
+        if constexpr (OUT) {
+            // the chunk's own tokens: fragments 0 .. 3 of the first 32, 3 and 5 of the others
+            auto read_m = [&](int m, ssm_parts (&v)[2]) {
+                constexpr int frag[3][2] = {{0, 1}, {2, 4}, {3, 5}};
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int i = 0; i < 3; i++) v[e].v[i] = sm[(frag[m][e] * 3 + i) * 64 + lane2];
+            };
+            read_m(0, f[0]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int m = 0; m < 3; m++) {  // tokens t 0 .. 31, 32 .. of the first 32; 32 .. of the others
+                if (m + 1 < 3) read_m(m + 1, f[(m + 1) & 1]);
+                else read_b(0, f[(m + 1) & 1]);
+                if (m == 0) ssm_parts8(u[2], u[3], us[1]);
+                else make_left(m - 1);
+                if (m < 2) read_left(m);
+#pragma unroll
+                for (int i = 0; i < 6; i++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) y[2 * (m > 0) + e] = ssm_product(i, us[m / 2], f[m & 1][e], y[2 * (m > 0) + e]);
+                if (m < 2) ssm_interleave<10, 4>();
+                else ssm_interleave<6, 4>();
+            }
+            const int py = 64 * pb + 16 * w + 4 * gq2;
+#pragma unroll
+            for (int tb = 0; tb < 4; tb++) {
+                const uint32_t at32 = 4u * ((uint32_t) (16 * tb + r2) * yrow + (uint32_t) py);
+                if (q.yvec) {
+                    if (py < a.dim && 16 * tb + r2 < nt) ssm_at<ssm_v4f>(ybase, at32) = y[tb];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (py + i < a.dim && 16 * tb + r2 < nt) ssm_at<float>(ybase, at32 + 4 * i) = y[tb][i];
+                }
+            }
+        } else {
+            read_b(0, f[1]);
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                read_left(m);
+                make_left(m);
             }
         }
         // the state after the chunk
-        {
-            const float fd = __builtin_amdgcn_exp2f((float) total);
 #pragma unroll
-            for (int pt = 0; pt < 4; pt++) {
-                const float f = fd * ssm_pow2(max(min(kvp[pt] - ks[pt], 126), -126));
+        for (int k = 0; k < NK; k++) st[k] *= ef;
+        if (deep) {
+            const int ew = (int) dec[kWhole][63];
 #pragma unroll
-                for (int k = 0; k < NT; k++) st[k][pt] *= f;
-                ks[pt] = kvp[pt];
+            for (int k = 0; k < NK; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) st[k][i] = ldexpf(st[k][i], ew);
+        }
+        // step m: tokens 32 (m / KB) .., the state's tiles 2 (m % KB) ..; beside
+        // them the next chunk's u
+#pragma unroll
+        for (int m = 0; m < 2 * KB; m++) {
+            if constexpr (kOne) read_b(m, f[(m + 1) & 1]);
+            else if (m + 1 < 2 * KB) read_b(m + 1, f[m & 1]);
+            if (m >= KB) {
+#pragma unroll
+                for (int b = 4 * (m - KB) / KB; b < 4 * (m - KB + 1) / KB; b++) make_u(b, tid, xn[b]);
             }
+#pragma unroll
+            for (int i = 0; i < 6; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    st[2 * (m % KB) + e] = ssm_product(i, f[(m + 1) & 1][e], left_us[m / KB], st[2 * (m % KB) + e]);
+            ssm_interleave<6, 4>();
         }
 #pragma unroll
-        for (int kk = 0; kk < 2; kk++) {
-            ssm_v8h xh[4], xl[4];
-#pragma unroll
-            for (int pt = 0; pt < 4; pt++) {
-                xh[pt] = *(const ssm_v8h *) &L.x[2][16 * pt + r][32 * kk + 8 * gq];
-                xl[pt] = *(const ssm_v8h *) &L.x[3][16 * pt + r][32 * kk + 8 * gq];
-            }
-#pragma unroll
-            for (int k = 0; k < NT; k++) ssm_products(bh[kk][k], bl[kk][k], xh, xl, st[k]);
-        }
+        for (int b = 0; b < 4; b++) u[b] = xn[b];
+        load_cb(gn, tid, wave);
+        next();
+    };
+    for (int c = c0; c < c1; c++) {
+        chunk(c, std::false_type{});
+        if (!OUT && !kOne && ++c < c1) chunk(c, std::true_type{});
     }
-    float back[4];
-#pragma unroll
-    for (int pt = 0; pt < 4; pt++) back[pt] = ldexpf(1.0f, -ks[pt]);
+    if (of_group >= blocks) return;
+    const int lane = tid & 63, gq = lane >> 4, p = first_p + (lane & 15);
     if constexpr (OUT) {
-        if (seg != q.segs - 1) return;
-        float * o = a.out + sh * a.dim * a.n;
+        if (seg != q.segs - 1 || p >= a.dim) return;
+        float * o = a.out + (sh * a.dim + p) * a.n;
 #pragma unroll
-        for (int k = 0; k < NT; k++)
+        for (int k = 0; k < NK; k++) {
+            const int n = 16 * k + 4 * gq;
+            if (q.svec) {
+                if (n < a.n) *(ssm_v4f *) (o + n) = st[k];
+            } else {
 #pragma unroll
-            for (int pt = 0; pt < 4; pt++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int n = nbase + 16 * k + 4 * gq + i, p = p0 + 16 * pt + r;
-                    if (n < a.n && p < a.dim) o[(int64_t) p * a.n + n] = st[k][pt][i] * back[pt];
-                }
+                for (int i = 0; i < 4; i++)
+                    if (n + i < a.n) o[n + i] = st[k][i];
+            }
+        }
     } else {
-        if (pb == 0 && threadIdx.x == 0) q.seg_decay[sh * q.segs + seg] = decayed;
-        float * o = q.seg_state + ((int64_t) unit * q.segs + seg) * 64 * NP;
+        if (pb == 0 && (tid & 255) == 0) {
+            double decayed = 0.0;
+            hp = q.heads + (sh * q.chunks + c0) * ssm_head_at::size;
+            for (int c = c0; c < c1; c++) decayed += ((const ssm_decay *) (hp + (c - c0) * ssm_head_at::size + ssm_head_at::decay))->total;
+            q.seg_decay[sh * q.segs + seg] = decayed;
+        }
+        ssm_v4f * o = (ssm_v4f *) q.seg_state + (((int64_t) unit * q.segs + seg) * 4 + (first_wave & 3)) * NK * 64 + lane;
 #pragma unroll
-        for (int k = 0; k < NT; k++)
-#pragma unroll
-            for (int pt = 0; pt < 4; pt++)
-                *(float4 *) (o + (16 * pt + r) * NP + nbase + 16 * k + 4 * gq) =
-                    make_float4(st[k][pt][0] * back[pt], st[k][pt][1] * back[pt], st[k][pt][2] * back[pt],
-                                st[k][pt][3] * back[pt]);
+        for (int k = 0; k < NK; k++) o[64 * k] = st[k];
     }
 }
 
@@ -1273,17 +1317,20 @@ bool ssm_scan_supported(int64_t n) { return n >= 1 && n <= 256; }
 static size_t ssm_al(size_t v) { return (v + 255) / 256 * 256; }
 
 // The chunked form takes a decay a head over enough tokens, channels and state
-// elements to fill its tiles. 80 heads of 64 x 128, with the call, chunked /
-// token by token: one sequence 8 tokens 33 / 31 us, 12 33 / 40, 64 32 / 147;
-// 16 sequences 12 tokens 83 / 79 us, 16 83 / 97, 64 83 / 309.
+// elements to fill its tiles. Chunked / token by token, us: 80 heads of 64 x 128,
+// one sequence 8 tokens 19 / 22, 12 19 / 30; 16 sequences 8 51 / 51, 12 51 / 67; 48
+// sequences 8 128 / 122, 12 128 / 164; 24 heads of 64 x 32 8 tokens 14 / 13, 12 14 /
+// 17, 64 15 / 74; 8 heads of 16 x 20 8 tokens 14 / 13, 12 14 / 17; 4 sequences of 40
+// heads of 64 x 256 12 tokens 38 / 36, 24 39 / 64.
 static bool ssm_chunked(const ssm_scan_args & a) {
     return !a.a_elem && a.tokens >= 12 && a.dim >= 16 && a.n >= 16 &&
-           (int64_t) a.heads * a.dim < 1 << 22;  // (a chunk's rows of y in 32-bit offsets)
+           (int64_t) a.heads * a.dim < 1 << 22 && a.x_nb2 < 1 << 25 &&  // (a lane's rows of y and x in 32-bit offsets)
+           a.tokens <= kSsmMostTokens;
 }
 
 static int ssm_np(const ssm_scan_args & a) { return a.n <= 64 ? 64 : a.n <= 128 ? 128 : 256; }
 
-// Segments of a chunked scan. Two workgroups a CU run at a time, so n segments
+// Segments of a chunked scan. A workgroup a CU runs at a time, so n segments
 // take the rounds of their workgroups times a segment's chunks and what it
 // reads of the segments before it; the first pass, which forms no outputs,
 // about half of that for all segments but the last, and a launch. In quarters
@@ -1292,8 +1339,9 @@ static void ssm_segments(const ssm_scan_args & a, int n_cu, ssm_chunk_args & q) 
     q.a = a;
     q.chunks = (a.tokens + kSsmL - 1) / kSsmL;
     q.pblocks = (a.dim + 63) / 64;
-    const int64_t units = (int64_t) a.seqs * a.heads * q.pblocks;
-    auto rounds = [&](int64_t wgs) { return (wgs + 2 * n_cu - 1) / (2 * n_cu); };
+    q.pairs = (a.heads / a.groups * q.pblocks + 1) / 2;
+    const int64_t units = (int64_t) a.seqs * a.groups * q.pairs;
+    auto rounds = [&](int64_t wgs) { return (wgs + n_cu - 1) / n_cu; };
     int64_t best = 0, best_cost = INT64_MAX;
     for (int64_t n = 1; n <= 32 && n <= q.chunks; n++) {
         const int64_t each = (q.chunks + n - 1) / n, segs = (q.chunks + each - 1) / each;
@@ -1376,13 +1424,17 @@ static void launch_ssm_chunks(const ssm_scan_args & a, void * scratch, hipStream
     ssm_carve(q, (char *) scratch);
     auto go = [&](auto np) {
         constexpr int NP = decltype(np)::value;
-        const unsigned units = (unsigned) (a.seqs * a.heads * q.pblocks);
+        const unsigned units = (unsigned) (a.seqs * a.groups * q.pairs);
+        const auto whole = [](uintptr_t bits) { return (bits & 15) == 0; };
+        q.xvec = a.dim % 4 == 0 && whole((uintptr_t) a.x | (uintptr_t) a.x_nb1 | (uintptr_t) a.x_nb2 | (uintptr_t) a.x_nb3);
+        q.yvec = a.dim % 4 == 0 && whole((uintptr_t) a.y);
+        q.svec = a.n % 4 == 0 && whole((uintptr_t) a.s | (uintptr_t) a.s_nb3 | (uintptr_t) a.out);
         q.split_blocks = (uint32_t) (4 * q.chunks * a.seqs * a.groups);
         const uint32_t decay_blocks = (uint32_t) ((q.chunks * a.seqs * a.heads + 3) / 4);
         hipLaunchKernelGGL(k_ssm_split<NP>, dim3(q.split_blocks + decay_blocks), dim3(256), 0, s, q);
         if (q.segs > 1)
-            hipLaunchKernelGGL((k_ssm_chunks<NP, false>), dim3(units, (unsigned) (q.segs - 1)), dim3(256), 0, s, q);
-        hipLaunchKernelGGL((k_ssm_chunks<NP, true>), dim3(units, (unsigned) q.segs), dim3(256), 0, s, q);
+            hipLaunchKernelGGL((k_ssm_chunks<NP, false>), dim3(units, (unsigned) (q.segs - 1)), dim3(512), 0, s, q);
+        hipLaunchKernelGGL((k_ssm_chunks<NP, true>), dim3(units, (unsigned) q.segs), dim3(512), 0, s, q);
     };
     const int np = ssm_np(a);
     if (np == 64) go(std::integral_constant<int, 64>{});

@@ -448,6 +448,104 @@ def test_ssm_scan_step_by_step_is_the_prompt(ggml, gpu):
     within(st, wh, 2 * bh, "states")
 
 
+# What of a chunk lies far under or over the rest: dt, x, B, C and the states, over tokens and over the states' elements
+WIDE = [("dt", -20), ("dt", -25), ("dt", -30), ("x up", 16), ("x up", 20), ("x up", 23), ("x up", 30), ("x down", 16), ("x down", 24),
+        ("x down", 40), ("x outlier", 20), ("x outlier", 23), ("n", 12), ("n", 20), ("n", 40), ("B row", 24), ("C row", 24),
+        ("B column", -27), ("B column", -40), ("state", 20), ("state", 40)]
+
+
+@pytest.mark.parametrize("T", [11, 64, 150])
+@pytest.mark.parametrize("what,e", WIDE)
+def test_ssm_scan_of_wide_ranges(ggml, gpu, T, what, e):
+    """every element keeps its bits, whatever the tokens and elements beside
+    it: the recurrence's bound holds element by element"""
+    print(f"wide ranges T={T} {what} {e}", flush=True)
+    rng = np.random.default_rng(T + abs(e))
+    S, H, P, n, Gr = 2, 3, 64, 128, 1
+    s, x, dt, A, B, C = scan_inputs(rng, S, T, H, P, Gr, n, False, S)
+    half, k = T // 2, np.float32(2.0 ** e)
+    if what == "dt":  # short steps first, from a state of zeros
+        s[:] = 0
+        dt[:, :half], dt[:, half:] = e, np.log(np.expm1(1.0))
+    elif what == "x up":
+        s[:] = 0
+        x[:, half:] *= k
+    elif what == "x down":  # a large token, decayed away before the chunk's end
+        A[:] = -16
+        dt[:] = np.log(np.expm1(0.1))
+        for t in range(0, T, 64):
+            x[:, t] *= k
+    elif what == "x outlier":
+        s[:] = 0
+        x[:, half] *= k
+    elif what == "n":  # y is the same, the states are not
+        v = np.exp2(rng.uniform(-e, e, n)).astype(np.float32)
+        B, C, s = B * v, C / v, s * v
+    elif what == "B row":
+        B[:, ::3] *= k
+        B[:, 1::3] /= k
+    elif what == "C row":
+        C[:, ::3] *= k
+        C[:, 1::3] /= k
+    elif what == "B column":
+        B[..., ::5] *= k
+        s[..., ::5] *= k
+    else:
+        s[..., ::7] *= k
+        s[..., 1::7] /= k
+    a = (s, x, dt, A, B, C, range(S))
+    y, h = run_scan(ggml, gpu, *a)
+    wy, by, wh, bh = scan64(*a)
+    within(h, wh, bh + 1e-30, "states")
+    within(y, wy, by + 1e-30, "y")
+
+
+# rows of x, y and states without 16-byte pieces, an odd number of blocks a group, several blocks a head, the
+# largest states over several segments of chunks
+FORMS = [(1, 700, 3, 64, 1, 256, False), (2, 300, 3, 30, 1, 30, False), (1, 200, 5, 64, 5, 130, False), (1, 1500, 7, 200, 7, 64, False),
+         (1, 2200, 1, 64, 1, 128, False), (2, 129, 2, 18, 2, 253, False), (5, 12, 3, 16, 1, 16, False), (1, 128, 3, 65, 1, 129, False)]
+
+
+@pytest.mark.parametrize("S,T,H,P,Gr,n,elem", FORMS)
+def test_ssm_scan_forms_of_chunks(ggml, gpu, S, T, H, P, Gr, n, elem):
+    test_ssm_scan(ggml, gpu, S, T, H, P, Gr, n, elem)
+
+
+@pytest.mark.parametrize("n", [24, 128, 200])
+def test_ssm_scan_by_token_beside_chunks(ggml, gpu, n):
+    """one channel's NaN, one head's step past every number and one token's
+    huge B each send their own part token by token, the rest stays as it is"""
+    rng = np.random.default_rng(n)
+    S, T, H, P, Gr = 2, 330, 4, 64, 2
+    s, x, dt, A, B, C = scan_inputs(rng, S, T, H, P, Gr, n, False, S)
+    x[0, 100, 0, 37] = np.nan
+    dt[0, 200, 1] = 1e9
+    B[1, 70, 1] *= np.float32(2.0 ** 40)
+    s[1, 0, 3] *= np.float32(2.0 ** 90)
+    y, h = run_scan(ggml, gpu, s, x, dt, A, B, C, range(S))
+    with np.errstate(all="ignore"):
+        wy, by, wh, bh = scan64(s, x, dt, A, B, C, range(S))
+    for got, want, bound in ((y, wy, by), (h, wh, bh)):
+        fine = np.isfinite(want)
+        assert np.array_equal(np.isfinite(got), fine)
+        within(got[fine], want[fine], bound[fine] + 1e-30)
+
+
+def test_ssm_scan_does_not_look_ahead(ggml, gpu):
+    """a token's y has the same bits whatever comes after it in its chunk"""
+    rng = np.random.default_rng(2)
+    S, T, H, P, n = 1, 64, 2, 64, 128
+    s, x, dt, A, B, C = scan_inputs(rng, S, T, H, P, 1, n, False, S)
+    y, _ = run_scan(ggml, gpu, s, x, dt, A, B, C, range(S))
+    x2, dt2, B2, C2 = (v.copy() for v in (x, dt, B, C))
+    x2[:, 40:] *= np.float32(2.0 ** 22)
+    dt2[:, 40:] += 4
+    B2[:, 40:] *= np.float32(2.0 ** 10)
+    C2[:, 40:] *= np.float32(2.0 ** 10)
+    y2, _ = run_scan(ggml, gpu, s, x2, dt2, A, B2, C2, range(S))
+    assert np.array_equal(y[:, :40], y2[:, :40])
+
+
 # -------------------------------------------------------------- experts ---
 
 WT = {"f16": 1, "f32": 0, "q8_0": 8, "q4_K": 12}
