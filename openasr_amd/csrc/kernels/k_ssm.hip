@@ -272,7 +272,7 @@ __global__ __launch_bounds__(256) void k_ssm_scan_rows(ssm_scan_args a) {
             for (int r = 0; r < R; r++) {
                 const int k = lane + 64 * r;
                 const bool ok = k < a.n;
-                st[r] = fmaf(st[r], expf(dt * av[r]), ok ? xv * b[k] : 0.0f);
+                st[r] = ok ? fmaf(st[r], expf(dt * av[r]), xv * b[k]) : 0.0f;  // (past n nothing, an infinite step neither)
                 y = fmaf(st[r], ok ? c[k] : 0.0f, y);
             }
             y = wave_sum(y);
@@ -330,7 +330,7 @@ __global__ __launch_bounds__(256) void k_ssm_scan_pieces(ssm_scan_args a) {
     if (a.tokens > 0) load(0, next);
 #pragma unroll
     for (int u = 0; u < U; u++)
-        if (!has || !in) st[u] = ssm_v4f{0, 0, 0, 0};
+        if (!has) st[u] = ssm_v4f{0, 0, 0, 0};
     for (int64_t t = 0; t < a.tokens; t++) {
         token v = next;
         if (t + 1 < a.tokens) load(t + 1, next);
@@ -339,7 +339,6 @@ __global__ __launch_bounds__(256) void k_ssm_scan_pieces(ssm_scan_args a) {
         d[0] = expf(dt * av[0]);
 #pragma unroll
         for (int e = 1; e < 4; e++) d[e] = a.a_elem ? expf(dt * av[e]) : d[0];
-        if (!in) v.b = v.c = ssm_v4f{0, 0, 0, 0};
         float y[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -347,13 +346,13 @@ __global__ __launch_bounds__(256) void k_ssm_scan_pieces(ssm_scan_args a) {
             y[u] = 0.0f;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                st[u][e] = fmaf(st[u][e], d[e], in ? xv * v.b[e] : 0.0f);
+                st[u][e] = fmaf(st[u][e], d[e], xv * v.b[e]);
                 y[u] = fmaf(st[u][e], v.c[e], y[u]);
             }
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            y[u] = group_sum<W>(y[u]);
+            y[u] = group_sum<W>(in ? y[u] : 0.0f);  // (past n the state's first elements again)
             if (k == 0 && p0 + kRows * u < a.dim) a.y[(s * a.tokens + t) * a.heads * a.dim + row0 + p0 + kRows * u] = y[u];
         }
     }
@@ -490,9 +489,13 @@ __global__ __launch_bounds__(256) void k_ssm_scan_lanes(ssm_lane_args q) {
             float e[N], y = 0.0f;
 #pragma unroll
             for (int k = 0; k < N; k++) e[k] = __builtin_amdgcn_exp2f(dt * A[k]);
-            if (__any(dt * low < -126.0f)) {  // below the instruction's range
+            if (__any(dt * low < -126.0f || dt * high > 127.0f)) {  // at the ends of the instruction's range
 #pragma unroll
-                for (int k = 0; k < N; k++) e[k] = exp2f(dt * A[k]);
+                for (int k = 0; k < N; k++) {
+                    e[k] = exp2f(dt * A[k]);
+                    // (a segment's own zero is none of the state's: it has no growth to be spoilt by)
+                    if (!OUT && st[k] == 0.0f) e[k] = 0.0f;
+                }
             }
 #pragma unroll
             for (int k = 0; k < N; k++) {
@@ -856,7 +859,8 @@ __device__ __forceinline__ void ssm_tokens(ssm_v4f (&st)[NP / 16], int s, int h,
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int n = 16 * k + 4 * gq + i, at = min(n, a.n - 1);
-                const float v = fmaf(st[k][i], ea, u * b[at]);
+                // (a segment's own zero is none of the state's: no growth spoils it)
+                const float v = !OUT && st[k][i] == 0.0f ? u * b[at] : fmaf(st[k][i], ea, u * b[at]);
                 st[k][i] = mine && n < a.n ? v : 0.0f;
                 if constexpr (OUT) y = n < a.n ? fmaf(v, c[at], y) : y;
             }

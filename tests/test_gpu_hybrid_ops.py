@@ -546,6 +546,32 @@ def test_ssm_scan_does_not_look_ahead(ggml, gpu):
     assert np.array_equal(y[:, :40], y2[:, :40])
 
 
+@pytest.mark.parametrize("S,T,H,P,Gr,n,elem", [(2, 1, 3, 16, 1, 20, False), (1, 1, 3, 5, 1, 21, False), (1, 1, 2, 16, 1, 100, True),
+                                               (1, 5, 2, 16, 1, 36, False), (1, 70, 2, 24, 1, 20, False), (1, 70, 3, 5, 1, 5, True),
+                                               (1, 3, 2, 8, 1, 65, True)])
+@pytest.mark.parametrize("what", ["dt", "growth"])
+def test_ssm_scan_infinities_with_part_rows(ggml, gpu, S, T, H, P, Gr, n, elem, what):
+    """a step or a decay past every number makes infinities, not NaN: states
+    shorter than a row of lanes have nothing beside them that could"""
+    print(f"infinities {what} S={S} T={T} H={H} P={P} n={n} elem={elem}", flush=True)
+    rng = np.random.default_rng(n)
+    s, x, dt, A, B, C = scan_inputs(rng, S, T, H, P, Gr, n, elem, S)
+    s, x, B, C = (np.abs(v) + 0.5 for v in (s, x, B, C))
+    if what == "dt":
+        dt[:, 0, 1] = np.inf
+    else:
+        dt[:, 0, 1], A[1] = 1e3, 2.0  # e^2000
+        dt[:, 1:, 1] = -30
+    y, h = run_scan(ggml, gpu, s, x, dt, A, B, C, range(S))
+    with np.errstate(all="ignore"):
+        wy, by, wh, bh = scan64(s, x, dt, A, B, C, range(S))
+    assert np.isinf(wy[:, :, 1]).all() and np.isfinite(wy[:, :, 0]).all()
+    for got, want, bound in ((y, wy, by), (h, wh, bh)):
+        fine = np.isfinite(want)
+        assert np.array_equal(got[~fine], want[~fine]) and np.isfinite(got[fine]).all()
+        within(got[fine], want[fine], bound[fine] + 1e-30, what)
+
+
 # -------------------------------------------------------------- experts ---
 
 WT = {"f16": 1, "f32": 0, "q8_0": 8, "q4_K": 12}
