@@ -168,6 +168,12 @@ span span_of(const tview & v, int64_t elem) {
     return s;
 }
 
+bool same_shape(const ggml_tensor * a, const ggml_tensor * b) {
+    for (int d = 0; d < 4; d++)
+        if (a->ne[d] != b->ne[d]) return false;
+    return true;
+}
+
 bool overlap(span a, span b) { return a.lo < a.hi && b.lo < b.hi && a.lo < b.hi && b.lo < a.hi; }
 
 // The GQA expansion of expand_attention_kv (nn/decoder.rs:1799-1841): x is
@@ -1495,9 +1501,9 @@ bool planner::plan_unary(int i, const ggml_tensor * t) {
         const ggml_tensor * mul = sole_consumer(t, i + 1);
         if (mul && mul->op == GGML_OP_MUL && (mul->src[0] == t || mul->src[1] == t)) {
             const ggml_tensor * other = mul->src[0] == t ? mul->src[1] : mul->src[0];
-            bool same_shape = true;
-            for (int d = 0; d < 4; d++) same_shape = same_shape && other->ne[d] == mul->ne[d];
-            if (same_shape) {
+            // both of its shape; and a multiply that is itself another launch's
+            // (a sum over experts' slots) evaluates nothing
+            if (same_shape(other, mul) && same_shape(t, mul) && !deferred.count(mul)) {
                 // the SiLU is evaluated inside the multiply, at the multiply's position
                 deferred[t] = mul;
                 deferred_unary.push_back({t, index.at(mul)});
@@ -1931,12 +1937,6 @@ static bool overlaps_operand(const ggml_tensor * t) {
     for (int k = 0; k < GGML_MAX_SRC; k++)
         if (t->src[k] && overlap(span_of(t), span_of(t->src[k]))) return true;
     return false;
-}
-
-static bool same_shape(const ggml_tensor * a, const ggml_tensor * b) {
-    for (int d = 0; d < 4; d++)
-        if (a->ne[d] != b->ne[d]) return false;
-    return true;
 }
 
 bool planner::plan_mul_mat_id(int i, const ggml_tensor * t) {

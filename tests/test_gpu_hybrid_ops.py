@@ -794,6 +794,62 @@ def test_experts_down(ggml, gpu, ref, wname, E, k, M, F, T, weighted):
     G.free()
 
 
+@pytest.mark.parametrize("k", [2, 3])
+@pytest.mark.parametrize("last", ["silu", "scale"])
+def test_experts_down_by_weights_made_in_place(ggml, gpu, ref, k, last):
+    """the slots' weights come from an operator right before the product with
+    them: they are there when the sum reads them"""
+    print(f"experts down by {last} weights k={k}", flush=True)
+    E, M, F, T = 8, 96, 256, 5
+    rng = np.random.default_rng(k)
+    raw, w = expert_weights(ggml, ref, rng, ggml.F16, E, M, F)
+    h = rng.standard_normal((T, k, F)).astype(np.float32)
+    gate = rng.standard_normal((T, k)).astype(np.float32)
+    ids = routes(rng, T, E, k, "twice")
+    G = ggml.Graph(64, 64)
+    L, ctx = G.lib, G.ctx
+    W, H, I, P = G.new(ggml.F16, F, M, E, weight=True), G.new(ggml.F32, F, k, T), G.new(ggml.I32, k, T), G.new(ggml.F32, 1, k, T)
+    p = L.ggml_silu(ctx, P) if last == "silu" else L.ggml_scale(ctx, P, 0.5)
+    y = L.ggml_mul(ctx, L.ggml_mul_mat_id(ctx, W, H, I), p)
+    parts = [L.ggml_view_2d(ctx, y, M, T, 4 * M * k, 4 * M * i) for i in range(k)]
+    out = parts[0]
+    for q in parts[1:]:
+        out = L.ggml_add(ctx, out, q)
+    G.build(out)
+    G.allocate(gpu.buft)
+    y64, mag = experts64(w, columns(ggml, ref, ggml.F16, h), ids)
+    for t, v in ((W, raw), (H, h), (I, ids)):
+        G.set(t, v)
+    for _ in range(4):  # other weights each time: none from the pass before
+        gate = rng.standard_normal((T, k)).astype(np.float32)
+        G.set(P, gate)
+        assert G.compute(gpu.backend) == 0
+        g = gate.astype(np.float64)
+        g = (g / (1 + np.exp(-g)) if last == "silu" else 0.5 * g)[:, :, None]
+        # the weight's own roundings: four of the SILU's
+        within(G.get(out).reshape(T, M), (y64 * g).sum(1), ((roundings(F) + k + 5) * U * mag * np.abs(g)).sum(1))
+    G.free()
+
+
+@pytest.mark.parametrize("shape", [(1, 6, 5), (64, 1, 5), (1, 1, 1), (64, 6, 5)])
+def test_product_with_a_broadcast_silu(ggml, gpu, shape):
+    """MUL with a SILU of fewer elements than the product has"""
+    print(f"broadcast silu {shape}", flush=True)
+    rng = np.random.default_rng(1)
+    a, b = rng.standard_normal((5, 6, 64)).astype(np.float32), rng.standard_normal(shape[::-1]).astype(np.float32)
+    G = ggml.Graph(64, 64)
+    A, B = G.new(ggml.F32, 64, 6, 5), G.new(ggml.F32, *shape)
+    y = G.lib.ggml_mul(G.ctx, A, G.lib.ggml_silu(G.ctx, B))
+    G.build(y)
+    G.allocate(gpu.buft)
+    G.set(A, a)
+    G.set(B, b)
+    compute(gpu, G)
+    want = a * (b / (1 + np.exp(-b.astype(np.float64))))
+    within(G.get(y).reshape(5, 6, 64), want, 6 * U * np.abs(want))
+    G.free()
+
+
 # --------------------------------------------------------------- router ---
 
 def sorted64(a, desc):
