@@ -1959,7 +1959,7 @@ bool planner::plan_mul_mat_id(int i, const ggml_tensor * t) {
     };
     const ggml_tensor * silu = silu_of(t);
     const ggml_tensor * hm = sole_consumer(silu ? silu : t, i + 1);
-    if (hm && hm->op == GGML_OP_MUL && same_shape(hm, t) && is_contiguous(hm) && hm->type == GGML_TYPE_F32) {
+    if (hm && hm->op == GGML_OP_MUL && same_shape(hm, t) && is_contiguous(hm) && hm->type == GGML_TYPE_F32 && !deferred.count(hm)) {
         const ggml_tensor * o = hm->src[0] == (silu ? silu : t) ? hm->src[1] : hm->src[0];
         const ggml_tensor * other = silu ? o : o->op == GGML_OP_UNARY ? o->src[0] : nullptr;  // the partner product
         const ggml_tensor * act = silu ? silu : o;

@@ -831,6 +831,40 @@ def test_experts_down_by_weights_made_in_place(ggml, gpu, ref, k, last):
     G.free()
 
 
+@pytest.mark.parametrize("k,T", [(2, 5), (4, 130)])
+def test_experts_of_one_row(ggml, gpu, ref, k, T):
+    """SILU(gate) * up of experts with one row each, summed over the slots: a
+    row of weights and one of products look alike"""
+    print(f"experts of one row k={k} T={T}", flush=True)
+    E, K = 6, 256
+    rng = np.random.default_rng(T)
+    (rg, wg), (ru, wu) = (expert_weights(ggml, ref, rng, ggml.F16, E, 1, K) for _ in range(2))
+    x = rng.standard_normal((T, 1, K)).astype(np.float32)
+    ids = routes(rng, T, E, k, "twice")
+    G = ggml.Graph(64, 64)
+    L, ctx = G.lib, G.ctx
+    WG, WU = (G.new(ggml.F16, K, 1, E, weight=True) for _ in range(2))
+    X, I = G.new(ggml.F32, K, 1, T), G.new(ggml.I32, k, T)
+    g = L.ggml_silu(ctx, L.ggml_mul_mat_id(ctx, WG, X, I))
+    y = L.ggml_mul(ctx, L.ggml_mul_mat_id(ctx, WU, X, I), g)
+    parts = [L.ggml_view_2d(ctx, y, 1, T, 4 * k, 4 * i) for i in range(k)]
+    out = parts[0]
+    for q in parts[1:]:
+        out = L.ggml_add(ctx, out, q)
+    G.build(out)
+    G.allocate(gpu.buft)
+    for t, v in ((WG, rg), (WU, ru), (X, x), (I, ids)):
+        G.set(t, v)
+    compute(gpu, G)
+    xc = columns(ggml, ref, ggml.F16, x)
+    (a, am), (b, bm) = experts64(wg, xc, ids), experts64(wu, xc, ids)
+    act = a / (1 + np.exp(-a))
+    # the gate's error grows by SILU's slope, 1.1 at most; SILU's own and the product's roundings
+    bound = roundings(K) * U * (1.1 * am * np.abs(b) + np.abs(act) * bm) + 6 * U * np.abs(act * b)
+    within(G.get(out).reshape(T), (act * b).sum((1, 2)), (bound + k * U * np.abs(act * b)).sum((1, 2)))
+    G.free()
+
+
 @pytest.mark.parametrize("shape", [(1, 6, 5), (64, 1, 5), (1, 1, 1), (64, 6, 5)])
 def test_product_with_a_broadcast_silu(ggml, gpu, shape):
     """MUL with a SILU of fewer elements than the product has"""
