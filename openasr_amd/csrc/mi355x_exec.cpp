@@ -138,6 +138,7 @@ uint64_t graph_key(const ggml_cgraph * cg) {
     for (int i = 0; i < cg->n_nodes; i++) {
         const ggml_tensor * t = cg->nodes[i];
         h = tensor_sig(h, t);
+        h = mix(h, (uint64_t) (t->flags & GGML_TENSOR_FLAG_OUTPUT));  // decides which results a plan makes
         for (int p = 0; p < 16; p++) h = mix(h, (uint64_t) (uint32_t) t->op_params[p]);
         for (int s = 0; s < GGML_MAX_SRC; s++) {
             if (t->src[s]) h = tensor_sig(h, t->src[s]);

@@ -1090,6 +1090,34 @@ def test_router_of_intermediates(ggml, gpu, gating):
     G.free()
 
 
+def test_an_output_flag_is_part_of_a_captured_graph(ggml, gpu):
+    """the same nodes in the same memory, one more of them an output: its
+    launches are planned anew, not replayed from the graph without it"""
+    E, k, T = 64, 6, 11
+    rng = np.random.default_rng(6)
+    G = ggml.Graph(64, 64)
+    L, ctx = G.lib, G.ctx
+    X = G.new(ggml.F32, E, T)
+    order = L.ggml_argsort(ctx, X, 1)
+    w = L.ggml_get_rows(ctx, L.ggml_reshape_3d(ctx, X, 1, E, T), L.ggml_view_2d(ctx, order, k, T, 4 * E, 0))
+    G.build(w, order)  # (both have memory of their own)
+    G.allocate(gpu.buft)
+    t = ggml.tensor(order)
+    flagged = t.flags
+    plain = flagged & ~2  # GGML_TENSOR_FLAG_OUTPUT
+    assert plain != flagged
+    for flags in (plain, flagged, plain, flagged):
+        t.flags = flags
+        a = rng.standard_normal((T, E)).astype(np.float32)
+        G.set(X, a)
+        compute(gpu, G, 4)
+        full = sorted64(a, 1)
+        assert np.array_equal(G.get(w).reshape(T, k), np.take_along_axis(a, full[:, :k], 1))
+        if flags == flagged:
+            assert np.array_equal(G.get(order).reshape(T, E), full)
+    G.free()
+
+
 @pytest.mark.parametrize("n,rows", [(255, 7), (256, 3), (257, 3), (511, 2), (513, 2), (4096, 2), (4097, 1)])
 @pytest.mark.parametrize("desc", [0, 1])
 def test_argsort_lengths(ggml, gpu, n, rows, desc):
