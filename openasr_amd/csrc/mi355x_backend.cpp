@@ -103,6 +103,12 @@ static void buf_free(ggml_backend_buffer_t buffer) {
     delete c;
 }
 
+// What a fill or copy on the null stream writes into memory of others is there
+// when the call returns: their streams are not ordered after it.
+static void finish_borrowed(const buffer_ctx * c) {
+    if (c->borrowed) MI_CHECK(hipStreamSynchronize(nullptr));
+}
+
 static void * buf_get_base(ggml_backend_buffer_t buffer) { return ((buffer_ctx *) buffer->context)->base; }
 
 static enum ggml_status buf_init_tensor(ggml_backend_buffer_t buffer, struct ggml_tensor * t) {
@@ -128,6 +134,7 @@ static void buf_memset_tensor(ggml_backend_buffer_t buffer, struct ggml_tensor *
         return;
     }
     MI_CHECK(hipMemset((char *) t->data + offset, value, size));
+    finish_borrowed(c);
 }
 
 // Q8_0 transfers work on whole rows; a partial-row range is widened to the
@@ -146,10 +153,12 @@ static void buf_set_tensor(ggml_backend_buffer_t buffer, struct ggml_tensor * t,
     error_scope scope(&c->dev->transfer_error);
     MI_CHECK(hipSetDevice(c->dev->hip_id));
     if (t->type != GGML_TYPE_Q8_0) {
-        // small writes wait in pinned memory for the next device use
-        if (stage_upload(c->dev, (char *) t->data + offset, data, size)) return;
+        // small writes wait in pinned memory for the next device use (the
+        // plugin's: memory of others is written now)
+        if (!c->borrowed && stage_upload(c->dev, (char *) t->data + offset, data, size)) return;
         flush_uploads(c->dev, nullptr, true);
         MI_CHECK(hipMemcpy((char *) t->data + offset, data, size, hipMemcpyHostToDevice));
+        finish_borrowed(c);
         return;
     }
     flush_uploads(c->dev, nullptr, true);
@@ -170,6 +179,7 @@ static void buf_set_tensor(ggml_backend_buffer_t buffer, struct ggml_tensor * t,
     std::memcpy(ggml_rows.data() + (offset - (size_t) r0 * rb), data, size);
     q8_0_to_split_rows(ggml_rows.data(), split.data(), r1 - r0, t->ne[0]);
     MI_CHECK(hipMemcpy(dev_rows, split.data(), span, hipMemcpyHostToDevice));
+    finish_borrowed(c);
 }
 
 static void buf_get_tensor(ggml_backend_buffer_t buffer, const struct ggml_tensor * t, void * data, size_t offset,
@@ -206,6 +216,7 @@ static bool buf_cpy_tensor(ggml_backend_buffer_t buffer, const struct ggml_tenso
     MI_CHECK(hipSetDevice(c->dev->hip_id));
     flush_uploads(c->dev, nullptr, true);
     MI_CHECK(hipMemcpy(dst->data, src->data, ggml_nbytes(src), hipMemcpyDeviceToDevice));
+    finish_borrowed(c);
     return true;
 }
 
@@ -215,6 +226,7 @@ static void buf_clear(ggml_backend_buffer_t buffer, uint8_t value) {
     MI_CHECK(hipSetDevice(c->dev->hip_id));
     flush_uploads(c->dev, nullptr, true);
     MI_CHECK(hipMemset(c->base, value, c->size));
+    finish_borrowed(c);
 }
 
 static const ggml_backend_buffer_i kBufferIface = {

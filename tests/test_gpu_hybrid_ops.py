@@ -1244,6 +1244,47 @@ def test_graph_over_memory_of_another_runtime():
     assert r.returncode == 0 and "over: done" in r.stdout, r.stdout + r.stderr
 
 
+WRITES = """
+import numpy as np, torch
+x = torch.zeros(1 << 16, device="cuda")
+y = torch.zeros(1 << 16, device="cuda")
+from openasr_amd import ggml
+gpu = ggml.plugin()
+G = ggml.Graph(64, 64)
+a, b = (G.over(ggml.F32, 1 << 16, memory=m) for m in (x, y))
+side = torch.cuda.Stream()
+rng = np.random.default_rng(1)
+for n in (4, 64, 1 << 16):
+    v = rng.standard_normal(1 << 16).astype(np.float32)
+    with torch.cuda.stream(side):
+        x.fill_(-1)
+    side.synchronize()
+    assert G.lib.ggml_backend_tensor_set(a, v.ctypes.data, 16, 4 * n - 16 if n == 1 << 16 else 4 * n) == 0
+    m = n - 4 if n == 1 << 16 else n
+    with torch.cuda.stream(side):  # written when the call returns, for any stream
+        got = x.cpu().numpy()
+    assert np.array_equal(got[4:4 + m], v[:m]) and (got[:4] == -1).all() and (got[4 + m:] == -1).all(), n
+for _ in range(20):
+    with torch.cuda.stream(side):
+        x.fill_(-1)
+    side.synchronize()
+    assert G.lib.ggml_backend_tensor_memset(a, 0, 64, 4 << 14) == 0
+    with torch.cuda.stream(side):
+        got = x.cpu().numpy()
+    assert (got[16:16 + (1 << 14)] == 0).all() and (got[:16] == -1).all() and (got[16 + (1 << 14):] == -1).all()
+G.free()
+print("writes: done", flush=True)
+"""
+
+
+def test_transfers_to_memory_of_another_runtime_are_finished():
+    """what ggml_backend_tensor_set and memset write is there for the memory's
+    owner when they return"""
+    root = Path(__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", WRITES], cwd=root, capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0 and "writes: done" in r.stdout, r.stdout + r.stderr
+
+
 # ----------------------------------------------------------- a whole layer ---
 
 @pytest.mark.parametrize("T,S", [(1, 1), (1, 4), (70, 2)])
