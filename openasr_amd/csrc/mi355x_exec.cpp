@@ -2026,7 +2026,7 @@ void planner::find_slot_sums() {
         const ggml_tensor * y = cg->nodes[i];
         if (y->op != GGML_OP_MUL_MAT_ID || (y->flags & GGML_TENSOR_FLAG_OUTPUT) || no_sum.count(y)) continue;
         const int64_t M = y->ne[0], used = y->ne[1], T = y->ne[2];
-        if (used < 2 || used > 64) continue;
+        if (used < 2 || used > 64 || M < 1) continue;  // (no rows: strides of zero)
         slot_sum j;
         j.y = y;
         const ggml_tensor * base = y;  // whose views the chain reads

@@ -884,6 +884,24 @@ def test_product_with_a_broadcast_silu(ggml, gpu, shape):
     G.free()
 
 
+def test_experts_down_without_rows(ggml, gpu):
+    """experts of no rows: nothing to sum, nothing done"""
+    E, k, K, T = 4, 3, 32, 2
+    G = ggml.Graph(64, 64)
+    L, ctx = G.lib, G.ctx
+    W, H, I, P = G.new(ggml.F16, K, 0, E), G.new(ggml.F32, K, k, T), G.new(ggml.I32, k, T), G.new(ggml.F32, 1, k, T)
+    y = L.ggml_mul(ctx, L.ggml_mul_mat_id(ctx, W, H, I), P)
+    parts = [L.ggml_view_2d(ctx, y, 0, T, 0, 0) for i in range(k)]
+    out = parts[0]
+    for q in parts[1:]:
+        out = L.ggml_add(ctx, out, q)
+    G.build(out)
+    G.allocate(gpu.buft)
+    G.set(I, np.zeros((T, k), np.int32))
+    compute(gpu, G)
+    G.free()
+
+
 # --------------------------------------------------------------- router ---
 
 def sorted64(a, desc):
