@@ -3111,7 +3111,8 @@ bool supports_op(const device_state * dev, const ggml_tensor * t) {
         case GGML_OP_MUL_MAT_ID: {
             const ggml_tensor *w = t->src[0], *x = t->src[1], *ids = t->src[2];
             if (!w || !f32(x) || !ids || !f32(t) || !is_contiguous(t)) return false;
-            if (ids->type != GGML_TYPE_I32 || w->ne[3] != 1 || x->nb[0] != 4) return false;
+            if (ids->type != GGML_TYPE_I32 || x->nb[0] != 4) return false;
+            if (w->ne[3] != 1 || x->ne[3] != 1 || t->ne[3] != 1 || ids->ne[2] != 1 || ids->ne[3] != 1) return false;
             if (w->ne[0] != x->ne[0] || t->ne[0] != w->ne[1] || t->ne[1] != ids->ne[0] || t->ne[2] != ids->ne[1] ||
                 x->ne[2] != ids->ne[1] || x->ne[1] < 1 || ids->ne[0] % x->ne[1] != 0 || w->ne[0] < 1)
                 return false;
@@ -3122,15 +3123,18 @@ bool supports_op(const device_state * dev, const ggml_tensor * t) {
                    rows_contiguous(w, w->type == GGML_TYPE_F16 ? 2 : 4);
         }
         case GGML_OP_ARGSORT:
-            return t->type == GGML_TYPE_I32 && f32(t->src[0]) && rows_contiguous(t->src[0], 4) &&
+            return t->type == GGML_TYPE_I32 && f32(t->src[0]) && same_shape(t, t->src[0]) && rows_contiguous(t->src[0], 4) &&
                    rows_contiguous(t, 4) && argsort_supported(t->ne[0]) &&
                    (t->op_params[0] == GGML_SORT_ORDER_ASC || t->op_params[0] == GGML_SORT_ORDER_DESC);
         case GGML_OP_SUM_ROWS:
-            return f32(t) && f32(t->src[0]) && rows_contiguous(t->src[0], 4);
+            if (!f32(t) || !f32(t->src[0]) || t->ne[0] != 1) return false;
+            for (int d = 1; d < 4; d++)
+                if (t->ne[d] != t->src[0]->ne[d]) return false;
+            return rows_contiguous(t->src[0], 4);
         case GGML_OP_SSM_CONV: {
             const ggml_tensor *sx = t->src[0], *w = t->src[1];
             return f32(t) && f32(sx) && f32(w) && is_contiguous(t) && rows_contiguous(w, 4) && sx->ne[3] == 1 &&
-                   w->ne[1] == sx->ne[1] && w->ne[0] >= 1 && w->ne[0] <= INT32_MAX && t->ne[0] == sx->ne[1] &&
+                   t->ne[3] == 1 && w->ne[2] == 1 && w->ne[3] == 1 && w->ne[1] == sx->ne[1] && w->ne[0] >= 1 && w->ne[0] <= INT32_MAX && t->ne[0] == sx->ne[1] &&
                    t->ne[1] == sx->ne[0] - (w->ne[0] - 1) && t->ne[2] == sx->ne[2];
         }
         case GGML_OP_SSM_SCAN: {
@@ -3151,7 +3155,7 @@ bool supports_op(const device_state * dev, const ggml_tensor * t) {
                 if (y->ne[0] != n || y->ne[1] < 1 || h % y->ne[1] != 0 || y->ne[1] != B->ne[1] ||
                     y->ne[2] != x->ne[2] || y->ne[3] != x->ne[3])
                     return false;
-            if (ids->ne[0] != x->ne[3] || t->ne[0] != nelem(x) + n * p * h * x->ne[3]) return false;
+            if (nelem(ids) != ids->ne[0] || ids->ne[0] != x->ne[3] || nelem(t) != nelem(x) + n * p * h * x->ne[3]) return false;
             return p <= INT32_MAX && h <= INT32_MAX && x->ne[3] <= INT32_MAX && ssm_scan_supported(n);
         }
         case GGML_OP_CPY:

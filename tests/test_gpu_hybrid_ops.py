@@ -1212,6 +1212,31 @@ def test_compute_without_allocations(ggml, gpu, ref):
     G.free()
 
 
+@pytest.mark.parametrize("what", ["w3", "x3", "ids2", "ids3", "y3", "sort", "sum", "taps2", "conv3", "scan_ids", "nothing"])
+def test_supports_only_whole_shapes(ggml, gpu, what):
+    """an outer dimension that an operator would leave out is refused (nodes
+    as other hosts may make them; the constructors here do not)"""
+    G = ggml.Graph(64, 64)
+    L, ctx = G.lib, G.ctx
+    W, X, I = G.new(ggml.F16, 64, 24, 5), G.new(ggml.F32, 64, 1, 7), G.new(ggml.I32, 3, 7)
+    y = L.ggml_mul_mat_id(ctx, W, X, I)
+    A = G.new(ggml.F32, 40, 6)
+    srt, sm = L.ggml_argsort(ctx, A, 1), L.ggml_sum_rows(ctx, A)
+    TW = G.new(ggml.F32, 4, 6)
+    conv = L.ggml_ssm_conv(ctx, G.new(ggml.F32, 11, 6, 2), TW)
+    S = G.new(ggml.I32, 2)
+    scan = L.ggml_ssm_scan(ctx, G.new(ggml.F32, 16, 8, 4, 3), G.new(ggml.F32, 8, 4, 5, 2), G.new(ggml.F32, 4, 5, 2), G.new(ggml.F32, 1, 4),
+                           G.new(ggml.F32, 16, 1, 5, 2), G.new(ggml.F32, 16, 1, 5, 2), S)
+    node, of, dim = {"w3": (y, W, 3), "x3": (y, X, 3), "ids2": (y, I, 2), "ids3": (y, I, 3), "y3": (y, y, 3), "sort": (srt, srt, 2),
+                     "sum": (sm, sm, 3), "taps2": (conv, TW, 2), "conv3": (conv, conv, 3), "scan_ids": (scan, S, 1), "nothing": (y, W, 3)}[what]
+    for n in (y, srt, sm, conv, scan):
+        assert L.ggml_backend_supports_op(gpu.backend, n)
+    if what != "nothing":
+        ggml.tensor(of).ne[dim] = 2
+        assert not L.ggml_backend_supports_op(gpu.backend, node)
+    G.free()
+
+
 # ------------------------------------------------------ memory of others ---
 
 OVER = """
