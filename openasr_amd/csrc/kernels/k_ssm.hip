@@ -1389,7 +1389,7 @@ static void ssm_lane_segments(const ssm_scan_args & a, int n_cu, ssm_lane_args &
 }
 
 size_t ssm_scan_scratch_bytes(const ssm_scan_args & a, int n_cu) {
-    if (a.seqs == 0) return 0;
+    if ((int64_t) a.seqs * a.heads * a.dim == 0) return 0;
     if (ssm_chunked(a)) {
         ssm_chunk_args q{};
         ssm_segments(a, n_cu, q);

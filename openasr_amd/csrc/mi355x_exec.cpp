@@ -1926,12 +1926,6 @@ bool planner::plan_naive(int i, const ggml_tensor * t) {
     return true;
 }
 
-// The plan moves reads later than the graph has them in two places: a
-// bypassed CONT's readers read its source at their own positions, and a
-// deferred unary node reads its source at its consumer's position. Under an
-// allocator that reuses dead blocks, a launch between may already have
-// written those bytes. Such a fusion is recorded in no_bypass / no_defer and
-// validate returns false, and the caller plans again without it.
 // whether a node's result overlaps one of its operands (an allocation that a
 // launch reading and writing in no particular order cannot take)
 static bool overlaps_operand(const ggml_tensor * t) {
@@ -2291,6 +2285,14 @@ bool planner::plan_ssm_scan(const ggml_tensor * t) {
     return true;
 }
 
+// The plan moves reads later than the graph has them: a bypassed CONT's
+// readers read its source at their own positions, a deferred unary node its
+// source at its consumer's, an expansion's readers its source, a slots' sum the
+// products and weights at its last ADD, a fused attention chain its operands at
+// its output. Under an allocator that reuses dead blocks, a launch between may
+// already have written those bytes. Such a fusion is recorded in no_bypass,
+// no_defer, no_fold, no_sum or no_naive and validate returns false, and the
+// caller plans again without it.
 bool planner::validate() {
     bool ok = true;
     auto written_between = [&](span src, int from, int to, bool allow_exact_at_to) {

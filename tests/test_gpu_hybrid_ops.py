@@ -794,6 +794,36 @@ def test_experts_down(ggml, gpu, ref, wname, E, k, M, F, T, weighted):
     G.free()
 
 
+@pytest.mark.parametrize("wname", ["f16", "q8_0", "q4_K", "f32"])
+@pytest.mark.parametrize("E,k,M,K,T", [(8, 2, 40, 256, 1), (8, 2, 40, 256, 9), (8, 4, 140, 512, 100)])
+def test_mul_mat_id_keeps_non_finite_columns_apart(ggml, gpu, ref, wname, E, k, M, K, T):
+    """a column with a NaN or an infinity spoils its own results only"""
+    print(f"mul_mat_id non-finite columns {wname} E={E} k={k} M={M} K={K} T={T}", flush=True)
+    wt = WT[wname]
+    rng = np.random.default_rng(M + T)
+    raw, w = expert_weights(ggml, ref, rng, wt, E, M, K)
+    x = rng.standard_normal((T, k, K)).astype(np.float32)
+    bad = np.zeros((T, k), bool)
+    bad[::3, 0] = True
+    x[bad, 5] = np.where(np.arange(bad.sum()) % 2, np.nan, np.inf)
+    ids = routes(rng, T, E, k, "twice")
+    G = ggml.Graph(64, 64)
+    W, X, I = G.new(wt, K, M, E, weight=True), G.new(ggml.F32, K, k, T), G.new(ggml.I32, k, T)
+    y = G.lib.ggml_mul_mat_id(G.ctx, W, X, I)
+    G.build(y)
+    G.allocate(gpu.buft)
+    for t, v in ((W, raw), (X, x), (I, ids)):
+        G.set(t, v)
+    compute(gpu, G)
+    got = G.get(y).reshape(T, k, M)
+    clean = np.where(bad[:, :, None], np.float32(0), x)
+    want, mag = experts64(w, columns(ggml, ref, wt, clean), ids)
+    within(got[~bad], want[~bad], roundings(K) * U * mag[~bad], wname)
+    if wname in ("f16", "f32"):
+        assert not np.isfinite(got[bad]).any()
+    G.free()
+
+
 @pytest.mark.parametrize("k", [2, 3])
 @pytest.mark.parametrize("last", ["silu", "scale"])
 def test_experts_down_by_weights_made_in_place(ggml, gpu, ref, k, last):
