@@ -99,7 +99,9 @@ void ggml_mul_mat_set_prec(struct ggml_tensor * a, enum ggml_prec prec);
 /* as [K, M, n_expert], b [K, 1 | n_used, n_tokens] f32, ids [n_used, n_tokens]
  * i32 (rows may be strided) -> [M, n_used, n_tokens]: column (slot, token) is
  * as[ids[slot, token]] times b's column (slot % b.ne[1], token); zeros where
- * the id is outside [0, n_expert) */
+ * the id is outside [0, n_expert). Quantized weights' sums over K are f64 for few
+ * columns (slots times tokens) and f32 of exact block sums for many: the last
+ * bits of a column may depend on how many there are. */
 struct ggml_tensor * ggml_mul_mat_id(struct ggml_context * ctx, struct ggml_tensor * as, struct ggml_tensor * b,
                                      struct ggml_tensor * ids);
 /* the indices that sort each row of a; equal elements keep their order, NaN

@@ -317,9 +317,10 @@ __global__ __launch_bounds__(256) void k_moe_few(mul_mat_id_args a) {
 // of the columns there are. Loads, LDS stores and barriers alone take 105, the
 // rest without loads 89: bound by 1.07 GB through the L2s (268 MB of weights
 // twice, columns for each row tile) with the matrix cores waiting. Q8_0 (700
-// tokens of 8, 64 experts of 2048 x 768): 84 us; 38 % of the cycles issue vector
-// instructions (8 for the scales of each product of 16 x 16 x 32, 7 others), the
-// matrix cores are busy 10 %, and the tiles' last round leaves CUs idle.
+// tokens of 8, 64 experts of 2048 x 768): 84 us, most of it waiting (35 % of the
+// waves' cycles on memory and barriers, 25 % on issue); 38 % of the cycles issue
+// vector instructions (8 for the scales of each product of 16 x 16 x 32, 7 others),
+// the matrix cores are busy 10 %, and the tiles' last round leaves CUs idle.
 //
 // Quantized weights are staged as the whole numbers of their blocks too:
 // a block's sum of 32 products is exact on the f16 matrix cores, and a block

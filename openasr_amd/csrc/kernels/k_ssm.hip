@@ -1376,8 +1376,10 @@ static size_t ssm_carve(ssm_chunk_args & q, char * base) {
 }
 
 // Segments of the short states' form: about two waves a SIMD, of 16 tokens or
-// more, since each reads the earlier segments' states (5120 channels, 1000
-// tokens, both passes: 8 waves a CU 83 us, 4 107, 6 97, 12 89, 16 100).
+// more, since each reads the earlier segments' states. At 4 / 8 / 16 waves a CU,
+// us, states of 16: 5120 channels, 1000 tokens 105 / 81 / 89, two sequences of
+// them 185 / 133 / 120; 4096 channels, 2000 tokens 151 / 123 / 123; 4 x 200 tokens
+// of 2048 38 / 43 / 42; 1024 channels, 300 or 1000 tokens alike.
 static bool ssm_lanes(const ssm_scan_args & a) { return a.n <= kSsmLane; }
 static void ssm_lane_segments(const ssm_scan_args & a, int n_cu, ssm_lane_args & q) {
     q.a = a;
