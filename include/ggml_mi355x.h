@@ -88,7 +88,8 @@ size_t ggml_backend_mi355x_static_scratch_bytes(void);
  * where they are. The memory must stay allocated until the buffer is freed
  * (ggml_backend_buffer_free leaves it alone), and writes that other streams
  * have pending must be finished before a compute or transfer reads it;
- * computes and transfers here are finished when they return. NULL, with a
+ * computes and transfers here are finished when they return (and leave the
+ * plugin's device the calling thread's current one). NULL, with a
  * message, unless ptr is 16-byte aligned and [ptr, ptr + size) lies in one
  * allocation on the device. Q8_0 tensors hold the device's row layout (ggml_backend_tensor_set
  * converts); other types are as ggml lays them out. Not counted in the memory

@@ -1158,7 +1158,7 @@ __global__ __launch_bounds__(512, 2) void k_ssm_chunks(ssm_chunk_args q) {
         }
         const ssm_u4 * const s_b = OUT ? (kOne ? s_c : s_other) : (!kOne && kOdd ? s_other : s_c);
         if constexpr (OUT) ssm_staged();  // B and the decayed C . B; the products have read C
-        tid = threadIdx.x;
+        tid = threadIdx.x;  // (anew again: the addresses of the first products would stay)
         asm volatile("" : "+v"(tid));
         const int lane2 = tid & 63, r2 = lane2 & 15, gq2 = lane2 >> 4;
         const float ef = dec[kIn][63];
