@@ -539,8 +539,8 @@ __global__ __launch_bounds__(256) void k_ssm_scan_lanes(ssm_lane_args q) {
 // f32 sums. The f32 matrix instructions need no parts, but take the vector
 // unit's time at 1/16 of the rate (a vector instruction beside one takes its
 // own again): 2 x 2048 tokens of 80 heads of 64 x 128 took 151 us, and 68 for
-// the first pass, where these take 110 and 50 (and 11 for the shared operands;
-// 333 tokens of 24 x 64 x 64: 13 + 8 + 5 us). Bound by reads of LDS (114 KB a
+// the first pass, where these take 104 and 46 (and 11 for the shared operands;
+// 333 tokens of 24 x 64 x 64: 12 + 7 + 5 us). Bound by reads of LDS (114 KB a
 // wave and chunk, 8 waves), the issue of loads after each barrier, and the
 // vector instructions around the products (some 800 a wave and chunk).
 //
@@ -1000,12 +1000,12 @@ __global__ __launch_bounds__(512, 2) void k_ssm_chunks(ssm_chunk_args q) {
     const char * hp = q.heads + (sh * q.chunks + c0) * ssm_head_at::size;
     // A chunk's C, C . B, x and decays (OUT false: B for C) are in flight under
     // the products before, its B under those of its own C.
-    ssm_v4f cbn[OUT ? 3 : 1], xn[4], dtn[4];
+    ssm_v4f cbn[OUT ? 3 : 1], xn[4];
     float dn[2];
     int next_kind = 0, next_bad = 0;
     auto load_next = [&](int c, bool more, const char * gp, const char * hp, int tid, int wave, auto to_other) {
         const uint32_t lane = tid & 63, gq = lane >> 4, nb = (uint32_t) a.x_nb2;
-        // token 4 gq + r % 4, channels r / 4 * 4 ..: make_u turns them over (rows
+        // token 4 gq + r % 4, channels r / 4 * 4 ..: ssm_turn makes u's of them (rows
         // past the last token: that one again)
         const char * row = xbase + (int64_t) c * kSsmL * a.x_nb2;
         const uint32_t last = (uint32_t) min((int64_t) kSsmL, a.tokens - (int64_t) c * kSsmL) - 1;
@@ -1024,8 +1024,6 @@ __global__ __launch_bounds__(512, 2) void k_ssm_chunks(ssm_chunk_args q) {
         next_bad = *(SSM_UNIFORM int *) (gp + at::bad);
         dn[0] = ssm_at<const float>(hp, 4u * (uint32_t) (tid & 255));
         dn[1] = ssm_at<const float>(hp + 1024, 4u * (uint32_t) (tid & 127));
-#pragma unroll
-        for (int b = 0; b < 4; b++) dtn[b] = ssm_at<const ssm_v4f>(hp, 16 * gq + 64 * b);
         // (behind the others: a wait for those does not wait for it)
         if (!kOne && more) ssm_stage<12 * KB>(gp + (OUT ? at::c : at::b), decltype(to_other)::value ? s_other : s_c, wave, lane);
     };
@@ -1035,13 +1033,6 @@ __global__ __launch_bounds__(512, 2) void k_ssm_chunks(ssm_chunk_args q) {
 #pragma unroll
             for (int k = 0; k < 3; k++) cbn[k] = ssm_at<const ssm_v4f>(gp + at::cb, 1024u * (uint32_t) ((wave & 3) + 4 * k) + 16 * lane);
         }
-    };
-    // that chunk's u: channel p, tokens 16 b + 4 gq + i. (A token past the last
-    // has a step of zero; channels past the last are never stored.)
-    auto make_u = [&](int b, int tid, ssm_v4f & u) {
-        u = xn[b];
-        ssm_turn(u, tid);
-        u *= dtn[b];
     };
     static_assert(ssm_head_at::tokens * kSsmL == 384 && ssm_head_at::decay == 4 * 384, "the threads' share of the decays");
     enum { kDt, kLeft, kLeftWhole, kIn, kWhole, kFrac };
@@ -1054,12 +1045,9 @@ __global__ __launch_bounds__(512, 2) void k_ssm_chunks(ssm_chunk_args q) {
         return (bool) __any(most.past(kSsmLargestState));
     };
     bool large = large_state();
-    ssm_v4f u[4];
     if (c0 < c1) {
         load_next(c0, true, gp, hp, tid, first_wave, std::false_type{});
         load_cb(gp, tid, first_wave);
-#pragma unroll
-        for (int b = 0; b < 4; b++) make_u(b, tid, u[b]);
     }
     auto next = [&] { gp += at::size, hp += ssm_head_at::size, ybase += 4 * kSsmL * (int64_t) yrow; };
     // OUT false: odd chunks' B is in the other room (as types: reads of one room
@@ -1077,15 +1065,23 @@ __global__ __launch_bounds__(512, 2) void k_ssm_chunks(ssm_chunk_args q) {
         const bool deep = next_kind & kSsmDeep, apart = (next_kind & kSsmOdd) || next_bad;
         (&dec[0][0])[tid & 255] = dn[0];
         if ((tid & 255) < 128) (&dec[0][0])[256 + (tid & 127)] = dn[1];
-        ssm_most most;
-#pragma unroll
-        for (int b = 0; b < 4; b++) most.add(u[b][0], u[b][1]), most.add(u[b][2], u[b][3]);
-        const bool by_token = apart || large || __any(most.past(kSsmLargest));
         if constexpr (kOne) {
             __syncthreads();  // the products of the chunk before have read B
             ssm_stage<12 * KB>(gp + (OUT ? at::c : at::b), s_c, wave, lane);
         }
         ssm_staged();  // C (OUT false: B) and the decays; the products of the chunk before have read B and the decayed C . B
+        // u: channel r, tokens 16 b + 4 gq + i. (A token past the last has a step of
+        // zero; channels past the last are never stored.)
+        ssm_v4f u[4];
+        ssm_most most;
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            u[b] = xn[b];
+            ssm_turn(u[b], lane);
+            u[b] *= *(const ssm_v4f *) &dec[kDt][16 * b + 4 * gq];
+            most.add(u[b][0], u[b][1]), most.add(u[b][2], u[b][3]);
+        }
+        const bool by_token = apart || large || __any(most.past(kSsmLargest));
         ssm_v4f y[4];  // token 16 tb + r, channels 16 w + 4 gq + i
         ssm_parts us[2];
         ssm_u4 * const sm = s_m + (OUT ? (wave >> 2) * 6 * 3 * 64 : 0);
@@ -1176,8 +1172,6 @@ __global__ __launch_bounds__(512, 2) void k_ssm_chunks(ssm_chunk_args q) {
             load_cb(gn, tid, wave);
             ssm_tokens<NP, OUT>(st, s, h, 64 * pb + 16 * w + r2, t0, nt);
             large = large_state();
-#pragma unroll
-            for (int b = 0; b < 4; b++) make_u(b, tid, u[b]);
             return next();
         }
         ssm_parts f[2][2], left_us[2];
@@ -1259,16 +1253,11 @@ __global__ __launch_bounds__(512, 2) void k_ssm_chunks(ssm_chunk_args q) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) st[k][i] = ldexpf(st[k][i], ew);
         }
-        // step m: tokens 32 (m / KB) .., the state's tiles 2 (m % KB) ..; beside
-        // them the next chunk's u
+        // step m: tokens 32 (m / KB) .., the state's tiles 2 (m % KB) ..
 #pragma unroll
         for (int m = 0; m < 2 * KB; m++) {
             if constexpr (kOne) read_b(m, f[(m + 1) & 1]);
             else if (m + 1 < 2 * KB) read_b(m + 1, f[m & 1]);
-            if (m >= KB) {
-#pragma unroll
-                for (int b = 4 * (m - KB) / KB; b < 4 * (m - KB + 1) / KB; b++) make_u(b, tid, xn[b]);
-            }
 #pragma unroll
             for (int i = 0; i < 6; i++)
 #pragma unroll
@@ -1276,8 +1265,6 @@ __global__ __launch_bounds__(512, 2) void k_ssm_chunks(ssm_chunk_args q) {
                     st[2 * (m % KB) + e] = ssm_product(i, f[(m + 1) & 1][e], left_us[m / KB], st[2 * (m % KB) + e]);
             ssm_interleave<6, 4>();
         }
-#pragma unroll
-        for (int b = 0; b < 4; b++) u[b] = xn[b];
         load_cb(gn, tid, wave);
         next();
     };
@@ -1322,7 +1309,7 @@ static size_t ssm_al(size_t v) { return (v + 255) / 256 * 256; }
 
 // The chunked form takes a decay a head over enough tokens, channels and state
 // elements to fill its tiles. Chunked / token by token, us: 80 heads of 64 x 128,
-// one sequence 8 tokens 19 / 22, 12 19 / 30; 16 sequences 8 51 / 51, 12 51 / 67; 48
+// one sequence 8 tokens 19 / 21, 12 19 / 30; 16 sequences 8 51 / 51, 12 51 / 67; 48
 // sequences 8 128 / 122, 12 128 / 164; 24 heads of 64 x 32 8 tokens 14 / 13, 12 14 /
 // 17, 64 15 / 74; 8 heads of 16 x 20 8 tokens 14 / 13, 12 14 / 17; 4 sequences of 40
 // heads of 64 x 256 12 tokens 38 / 36, 24 39 / 64.
