@@ -173,6 +173,9 @@ enum ggml_op {
     GGML_OP_GLU,
     /* fork-local: lowest-index argmax (ffi.rs:786, cpu_graph.rs:3749-3768) */
     GGML_OP_ARGMAX_FIRST,
+    /* the gated delta rule (ggml_gated_delta_net). Upstream versions that have
+     * the op number it before UNARY; this list keeps the numbers above */
+    GGML_OP_GATED_DELTA_NET,
     GGML_OP_COUNT
 };
 

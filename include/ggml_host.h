@@ -93,7 +93,7 @@ struct ggml_tensor * ggml_gelu_erf(struct ggml_context * ctx, struct ggml_tensor
 struct ggml_tensor * ggml_relu(struct ggml_context * ctx, struct ggml_tensor * a);
 struct ggml_tensor * ggml_mul_mat(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b);
 void ggml_mul_mat_set_prec(struct ggml_tensor * a, enum ggml_prec prec);
-/* ---- mixture-of-experts and state-space operators (upstream ggml.h) ----
+/* ---- mixture-of-experts, state-space and linear-attention operators (upstream ggml.h) ----
  * The constructors of this group return NULL, with a message on stderr, for
  * shapes or types that do not fit. */
 /* as [K, M, n_expert], b [K, 1 | n_used, n_tokens] f32, ids [n_used, n_tokens]
@@ -124,6 +124,20 @@ struct ggml_tensor * ggml_ssm_conv(struct ggml_context * ctx, struct ggml_tensor
 struct ggml_tensor * ggml_ssm_scan(struct ggml_context * ctx, struct ggml_tensor * s, struct ggml_tensor * x,
                                    struct ggml_tensor * dt, struct ggml_tensor * A, struct ggml_tensor * B,
                                    struct ggml_tensor * C, struct ggml_tensor * ids);
+/* a's rows over their length: x / max(|x|, eps) */
+struct ggml_tensor * ggml_l2_norm(struct ggml_context * ctx, struct ggml_tensor * a, float eps);
+/* the gated delta rule, a linear attention whose state is corrected by what it
+ * holds for a key: q and k [K, Hk, n_t, n_s], v [V, H, n_t, n_s] (H a multiple
+ * of Hk: head h reads key head h % Hk), g [1 | K, H, n_t, n_s] the logarithm of
+ * the decay (a head's, or one a key element), beta [1, H, n_t, n_s], state [K,
+ * V, H, n_s]. A head's state S [K, V] takes a token by S <- e^g S, S <- S +
+ * beta k (v - S^T k)^T, y = S^T q / sqrt(K). The result is one row: y, laid out
+ * as a contiguous v, then each sequence's state after its last token, laid out
+ * as a contiguous state. state itself is only read. Sums are f32's, in an order
+ * that depends on the number of tokens. */
+struct ggml_tensor * ggml_gated_delta_net(struct ggml_context * ctx, struct ggml_tensor * q, struct ggml_tensor * k,
+                                          struct ggml_tensor * v, struct ggml_tensor * g, struct ggml_tensor * beta,
+                                          struct ggml_tensor * state);
 struct ggml_tensor * ggml_get_rows(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b);
 struct ggml_tensor * ggml_set_rows(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b,
                                    struct ggml_tensor * c);

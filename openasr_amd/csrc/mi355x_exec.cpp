@@ -542,6 +542,12 @@ struct planner {
     bool plan_top_k(int i, const ggml_tensor * t);
     bool plan_ssm_conv(int i, const ggml_tensor * t);
     bool plan_ssm_scan(const ggml_tensor * t);
+    // L2_NORMs evaluated inside the GATED_DELTA_NET that alone reads them
+    // (norm, the reader's position)
+    std::vector<std::pair<const ggml_tensor *, int>> deferred_l2;
+    bool plan_l2_norm(int i, const ggml_tensor * t);
+    const ggml_tensor * states_copy(int i, const ggml_tensor * t) const;
+    bool plan_delta(int i, const ggml_tensor * t);
 };
 
 // The unfused attention chains of the graph (llm_naive_masked_attention,
@@ -2285,9 +2291,94 @@ bool planner::plan_ssm_scan(const ggml_tensor * t) {
     return true;
 }
 
+bool planner::plan_l2_norm(int i, const ggml_tensor * t) {
+    const ggml_tensor * d = no_defer.count(t) ? nullptr : sole_consumer(t, i + 1);
+    if (d && d->op == GGML_OP_GATED_DELTA_NET && (d->src[0] == t || d->src[1] == t) && supports_op(be->dev, d)) {
+        deferred[t] = d;
+        deferred_l2.push_back({t, index.at(d)});
+        return true;
+    }
+    const tview dv = make_view(t), av = view_of(t->src[0]);
+    const float eps = op_f32(t, 0);
+    add_step([=](hipStream_t s) { launch_l2_norm(dv, av, eps, s); }, t, "l2_norm");
+    return true;
+}
+
+// the CPY of t's states (nothing else reads them) to where t's launch at
+// position i may write them instead: contiguous, and either the states it
+// reads, in their place, or apart from all it reads and writes
+const ggml_tensor * planner::states_copy(int i, const ggml_tensor * t) const {
+    const ggml_tensor *v = t->src[2], *s0 = t->src[5];
+    const size_t at = 4 * (size_t) nelem(v), end = at + 4 * (size_t) nelem(s0);
+    if (end == at || (t->flags & GGML_TENSOR_FLAG_OUTPUT)) return nullptr;
+    const ggml_tensor * last = nullptr;
+    for (int k = i + 1; k < cg->n_nodes; k++) {
+        const ggml_tensor * n = cg->nodes[k];
+        for (int q = 0; q < GGML_MAX_SRC; q++)
+            if (n->src[q] == t && (q != 0 || !is_view_op(n->op))) return nullptr;
+        if (n->view_src != t) continue;
+        const size_t lo = (size_t) ((const char *) n->data - (const char *) t->data);
+        if (lo + ggml_nbytes(n) <= at) continue;  // of y
+        if (last || lo != at || nelem(n) != nelem(s0) || !is_contiguous(n)) return nullptr;
+        last = n;
+    }
+    if (!last) return nullptr;
+    const ggml_tensor * c = sole_consumer(last, index.at(last) + 1);
+    if (!c || c->op != GGML_OP_CPY || c->src[0] != last || c->type != GGML_TYPE_F32 || !is_contiguous(c) ||
+        nelem(c) != nelem(s0) || bypass.count(c) || deferred.count(c) || !ready_before(c->src[1], i))
+        return nullptr;
+    hoist h;
+    h.nodes = {c};
+    for (int k = 0; k < 6; k++) {
+        const ggml_tensor * x = t->src[k];
+        auto d = deferred.find(x);
+        if (k < 2 && d != deferred.end() && d->second == t) x = x->src[0];
+        if (k == 5 && c->data == s0->data && is_contiguous(s0)) continue;  // each row is read, then written, by one wave
+        h.reads.push_back(span_of(x));
+    }
+    h.writes = {span_of(c), {(uintptr_t) t->data, (uintptr_t) t->data + at}};
+    return hoist_ok(i, h) ? c : nullptr;
+}
+
+bool planner::plan_delta(int i, const ggml_tensor * t) {
+    if (overlaps_operand(t)) return fail(t, "GATED_DELTA_NET output overlaps its own input");
+    const ggml_tensor *q = t->src[0], *k = t->src[1], *v = t->src[2], *g = t->src[3], *b = t->src[4], *s0 = t->src[5];
+    delta_args a{};
+    auto row_source = [&](const ggml_tensor * x, float & eps) {
+        auto d = deferred.find(x);
+        const bool norm = d != deferred.end() && d->second == t;
+        eps = norm ? op_f32(x, 0) : -1.0f;
+        return norm ? view_of(x->src[0]) : make_view(x);
+    };
+    const tview qv = row_source(q, a.q_eps), kv = row_source(k, a.k_eps);
+    a.q = qv.data, a.q_nb1 = qv.nb[1], a.q_nb2 = qv.nb[2], a.q_nb3 = qv.nb[3];
+    a.k = kv.data, a.k_nb1 = kv.nb[1], a.k_nb2 = kv.nb[2], a.k_nb3 = kv.nb[3];
+    a.v = (const char *) v->data, a.v_nb1 = (int64_t) v->nb[1], a.v_nb2 = (int64_t) v->nb[2], a.v_nb3 = (int64_t) v->nb[3];
+    a.g = (const char *) g->data, a.g_nb1 = (int64_t) g->nb[1], a.g_nb2 = (int64_t) g->nb[2], a.g_nb3 = (int64_t) g->nb[3];
+    a.beta = (const char *) b->data, a.b_nb1 = (int64_t) b->nb[1], a.b_nb2 = (int64_t) b->nb[2], a.b_nb3 = (int64_t) b->nb[3];
+    a.s = (const char *) s0->data, a.s_nb3 = (int64_t) s0->nb[3];
+    a.K = (int) s0->ne[0], a.V = (int) s0->ne[1], a.heads = (int) s0->ne[2], a.seqs = (int) s0->ne[3];
+    a.key_heads = (int) k->ne[1], a.tokens = v->ne[2], a.g_elem = g->ne[0] != 1;
+    a.scale = (float) (1.0 / std::sqrt((double) a.K));
+    a.y = (float *) t->data;
+    a.out = (char *) (a.y + nelem(v));
+    a.out_nb3 = 4 * (int64_t) a.K * a.V * a.heads;
+    std::vector<const ggml_tensor *> writes = {t};
+    if (const ggml_tensor * c = states_copy(i, t)) {
+        deferred[c] = c;
+        a.out = (char *) c->data;
+        writes.push_back(c);
+    }
+    gen_need = std::max(gen_need, delta_scratch_bytes(a, n_cu));
+    backend_state * be_ = be;
+    const int ncu = n_cu;
+    add_step([=](hipStream_t s) { launch_delta(a, gen_base(be_), s, ncu); }, t, "gated_delta_net", writes);
+    return true;
+}
+
 // The plan moves reads later than the graph has them: a bypassed CONT's
-// readers read its source at their own positions, a deferred unary node its
-// source at its consumer's, an expansion's readers its source, a slots' sum the
+// readers read its source at their own positions, a deferred unary node or
+// L2_NORM its source at its consumer's, an expansion's readers its source, a slots' sum the
 // products and weights at its last ADD, a fused attention chain its operands at
 // its output. Under an allocator that reuses dead blocks, a launch between may
 // already have written those bytes. Such a fusion is recorded in no_bypass,
@@ -2318,6 +2409,12 @@ bool planner::validate() {
     for (const auto & du : deferred_unary) {
         if (written_between(span_of(du.first->src[0]), index.at(du.first), du.second, true)) {
             no_defer.insert(du.first);
+            ok = false;
+        }
+    }
+    for (const auto & dl : deferred_l2) {
+        if (written_between(span_of(view_of(dl.first->src[0]), 4), index.at(dl.first), dl.second, false)) {
+            no_defer.insert(dl.first);
             ok = false;
         }
     }
@@ -2584,6 +2681,12 @@ bool planner::plan() {
                 break;
             case GGML_OP_SSM_SCAN:
                 if (!plan_ssm_scan(t)) return false;
+                break;
+            case GGML_OP_L2_NORM:
+                plan_l2_norm(i, t);
+                break;
+            case GGML_OP_GATED_DELTA_NET:
+                if (!plan_delta(i, t)) return false;
                 break;
             default:
                 return fail(t, "no launcher");
@@ -3159,6 +3262,26 @@ bool supports_op(const device_state * dev, const ggml_tensor * t) {
                     return false;
             if (nelem(ids) != ids->ne[0] || ids->ne[0] != x->ne[3] || nelem(t) != nelem(x) + n * p * h * x->ne[3]) return false;
             return p <= INT32_MAX && h <= INT32_MAX && x->ne[3] <= INT32_MAX && ssm_scan_supported(n);
+        }
+        case GGML_OP_L2_NORM:
+            return f32(t) && f32(t->src[0]) && rows_contiguous(t->src[0], 4) && rows_contiguous(t, 4) &&
+                   same_shape(t, t->src[0]) && op_f32(t, 0) >= 0.0f;
+        case GGML_OP_GATED_DELTA_NET: {
+            for (int k = 0; k < 6; k++)
+                if (!f32(t->src[k]) || !rows_contiguous(t->src[k], 4)) return false;
+            const ggml_tensor *q = t->src[0], *k = t->src[1], *v = t->src[2], *g = t->src[3], *b = t->src[4], *s0 = t->src[5];
+            if (!f32(t) || !is_contiguous(t) || !same_shape(q, k)) return false;
+            const int64_t K = s0->ne[0], V = s0->ne[1], H = s0->ne[2], T = v->ne[2], S = s0->ne[3];
+            // a sequence's states contiguous; the other rows at any strides
+            if ((V > 1 && s0->nb[1] != 4 * (size_t) K) || (H > 1 && s0->nb[2] != 4 * (size_t) (K * V))) return false;
+            if (v->ne[0] != V || v->ne[1] != H || v->ne[3] != S || k->ne[0] != K || k->ne[1] < 1 || H % k->ne[1] != 0 ||
+                k->ne[2] != T || k->ne[3] != S)
+                return false;
+            for (const ggml_tensor * x : {g, b})
+                if (x->ne[1] != H || x->ne[2] != T || x->ne[3] != S) return false;
+            if ((g->ne[0] != 1 && g->ne[0] != K) || b->ne[0] != 1 || nelem(t) != nelem(v) + nelem(s0)) return false;
+            return V <= INT32_MAX && H <= INT32_MAX && S <= INT32_MAX && (double) V * (double) H * (double) S < 2147483648.0 &&
+                   delta_supported(K);
         }
         case GGML_OP_CPY:
         case GGML_OP_CONT:

@@ -423,6 +423,29 @@ bool ssm_scan_supported(int64_t n);
 size_t ssm_scan_scratch_bytes(const ssm_scan_args & a, int n_cu);
 void launch_ssm_scan(const ssm_scan_args & a, void * scratch, hipStream_t s, int n_cu);
 
+// GGML_OP_L2_NORM: rows (contiguous) over their length, x / max(|x|, eps)
+void launch_l2_norm(const tview & d, const tview & a, float eps, hipStream_t s);
+
+// GGML_OP_GATED_DELTA_NET: q and k [K, key_heads, tokens, seqs], v [V, heads,
+// tokens, seqs], g [1 or (g_elem) K, heads, tokens, seqs], beta [1, heads,
+// tokens, seqs], strides in bytes [head, token, sequence]; states s and out
+// [K, V, heads] a sequence (contiguous, s_nb3 and out_nb3 bytes apart; out may
+// be s itself); y laid out as a contiguous v. q_eps, k_eps: q's or k's rows are
+// brought to length one here (L2_NORM's eps), below zero: they are as they come
+struct delta_args {
+    const char *q, *k, *v, *g, *beta, *s;
+    int64_t q_nb1, q_nb2, q_nb3, k_nb1, k_nb2, k_nb3, v_nb1, v_nb2, v_nb3;
+    int64_t g_nb1, g_nb2, g_nb3, b_nb1, b_nb2, b_nb3, s_nb3, out_nb3;
+    float * y;
+    char * out;
+    int64_t tokens;
+    int K, V, heads, key_heads, seqs, g_elem;
+    float q_eps, k_eps, scale;
+};
+bool delta_supported(int64_t K);
+size_t delta_scratch_bytes(const delta_args & a, int n_cu);
+void launch_delta(const delta_args & a, void * scratch, hipStream_t s, int n_cu);
+
 // GGML_OP_MUL_MAT_ID: column (slot, token) of out [M, used, tokens] is
 // expert ids[slot, token]'s matrix times column (slot % b_ne1, token) of b;
 // zeros for an id outside [0, experts). Quantized weights read the columns

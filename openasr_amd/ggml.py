@@ -119,6 +119,8 @@ def base() -> C.CDLL:
     _sig(lib, "ggml_sum_rows", T, CTX, T)
     _sig(lib, "ggml_ssm_conv", T, CTX, T, T)
     _sig(lib, "ggml_ssm_scan", T, CTX, T, T, T, T, T, T, T)
+    _sig(lib, "ggml_l2_norm", T, CTX, T, f)
+    _sig(lib, "ggml_gated_delta_net", T, CTX, T, T, T, T, T, T)
     _sig(lib, "ggml_soft_max_ext", T, CTX, T, T, f, f)
     _sig(lib, "ggml_flash_attn_ext", T, CTX, T, T, T, T, f, f, f)
     _sig(lib, "ggml_flash_attn_ext_set_prec", None, T, i)

@@ -119,6 +119,7 @@ static const char * const kOpNames[GGML_OP_COUNT] = {
     "SSM_CONV", "SSM_SCAN", "WIN_PART", "WIN_UNPART", "GET_REL_POS", "ADD_REL_POS", "RWKV_WKV6",
     "GATED_LINEAR_ATTN", "RWKV_WKV7", "SOLVE_TRI", "UNARY", "MAP_CUSTOM1", "MAP_CUSTOM2", "MAP_CUSTOM3", "CUSTOM",
     "CROSS_ENTROPY_LOSS", "CROSS_ENTROPY_LOSS_BACK", "OPT_STEP_ADAMW", "OPT_STEP_SGD", "GLU", "ARGMAX_FIRST",
+    "GATED_DELTA_NET",
 };
 
 const char * ggml_op_name(enum ggml_op op) { return (op >= 0 && op < GGML_OP_COUNT) ? kOpNames[op] : "?"; }
@@ -536,6 +537,37 @@ struct ggml_tensor * ggml_ssm_scan(struct ggml_context * ctx, struct ggml_tensor
     return r;
 }
 
+struct ggml_tensor * ggml_l2_norm(struct ggml_context * ctx, struct ggml_tensor * a, float eps) {
+    GB_REFUSE_UNLESS(a && a->type == GGML_TYPE_F32 && ggml_is_contiguous_rows(a), "l2_norm: needs contiguous f32 rows");
+    GB_REFUSE_UNLESS(eps >= 0.0f, "l2_norm: eps below zero");
+    return norm_op(ctx, a, eps, GGML_OP_L2_NORM);
+}
+
+struct ggml_tensor * ggml_gated_delta_net(struct ggml_context * ctx, struct ggml_tensor * q, struct ggml_tensor * k,
+                                          struct ggml_tensor * v, struct ggml_tensor * g, struct ggml_tensor * beta,
+                                          struct ggml_tensor * state) {
+    ggml_tensor * src[6] = {q, k, v, g, beta, state};
+    for (const ggml_tensor * t : src) {
+        GB_REFUSE_UNLESS(t, "gated_delta_net: null operand");
+        GB_REFUSE_UNLESS(t->type == GGML_TYPE_F32 && ggml_is_contiguous_rows(t), "gated_delta_net: contiguous f32 rows");
+    }
+    const int64_t K = state->ne[0], V = state->ne[1], H = state->ne[2], T = v->ne[2], S = v->ne[3];
+    GB_REFUSE_UNLESS(K >= 1 && V >= 1 && H >= 1, "gated_delta_net: empty state");
+    GB_REFUSE_UNLESS(state->ne[3] == S && v->ne[0] == V && v->ne[1] == H, "gated_delta_net: v does not match the state");
+    GB_REFUSE_UNLESS(k->ne[0] == K && k->ne[1] >= 1 && H % k->ne[1] == 0 && k->ne[2] == T && k->ne[3] == S,
+                     "gated_delta_net: k's shape");
+    for (int d = 0; d < GGML_MAX_DIMS; d++) GB_REFUSE_UNLESS(q->ne[d] == k->ne[d], "gated_delta_net: q's shape is not k's");
+    GB_REFUSE_UNLESS((g->ne[0] == 1 || g->ne[0] == K) && g->ne[1] == H && g->ne[2] == T && g->ne[3] == S,
+                     "gated_delta_net: g's shape");
+    GB_REFUSE_UNLESS(beta->ne[0] == 1 && beta->ne[1] == H && beta->ne[2] == T && beta->ne[3] == S,
+                     "gated_delta_net: beta's shape");
+    ggml_tensor * r = ggml_new_tensor_1d(ctx, GGML_TYPE_F32, ggml_nelements(v) + ggml_nelements(state));
+    if (!r) return nullptr;
+    r->op = GGML_OP_GATED_DELTA_NET;
+    for (int i = 0; i < 6; i++) r->src[i] = src[i];
+    return r;
+}
+
 struct ggml_tensor * ggml_get_rows(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b) {
     GB_REQUIRE(a->ne[2] == b->ne[1] && b->ne[3] == 1 && b->type == GGML_TYPE_I32, "get_rows: bad shapes");
     const enum ggml_type type = a->type == GGML_TYPE_I32 ? GGML_TYPE_I32 : GGML_TYPE_F32;
@@ -658,6 +690,9 @@ struct ggml_tensor * ggml_soft_max(struct ggml_context * ctx, struct ggml_tensor
 struct ggml_tensor * ggml_flash_attn_ext(struct ggml_context * ctx, struct ggml_tensor * q, struct ggml_tensor * k,
                                          struct ggml_tensor * v, struct ggml_tensor * mask, float scale,
                                          float max_bias, float logit_softcap) {
+    GB_REFUSE_UNLESS(max_bias >= 0.0f && max_bias <= 3.0e38f && logit_softcap >= 0.0f && logit_softcap <= 3.0e38f,
+                     "flash_attn_ext: max_bias or logit_softcap below zero or not finite");
+    GB_REFUSE_UNLESS(max_bias == 0.0f || mask, "flash_attn_ext: a max_bias without the mask it scales");
     GB_REQUIRE(q->ne[0] == k->ne[0] && k->ne[1] == v->ne[1], "flash_attn_ext: q/k/v shapes");
     GB_REQUIRE(q->ne[2] % k->ne[2] == 0 && q->ne[3] % k->ne[3] == 0, "flash_attn_ext: head broadcast");
     if (mask) {
