@@ -871,6 +871,7 @@ __global__ __launch_bounds__(kFaThreads) void k_fattn_full(fattn_args a, float *
 static int64_t fa_tiles(const fattn_args & a) { return (int64_t) a.hkv * a.n_seq * a.q_tiles; }
 
 size_t fattn_scratch_bytes(const fattn_args & a) {
+    if (a.scored) return fattn_scored_scratch_bytes(a);
     if (a.mfma) return fattn_mfma_scratch_bytes(a);
     if (a.dec) return fattn_dec_scratch_bytes(a);
     if (!a.split) return 0;
@@ -910,6 +911,7 @@ static void launch_combine(const fattn_args & a, const float * pm, const float *
 }
 
 bool attn_step_supported(const fattn_args & a) {
+    if (a.scored) return false;
     if (a.dec) return a.d == 128;  // the default-precision workgroup form
     return a.d == 128 && a.n_q == 1 && a.split == 2 && fattn_supported(a.d, a.hq, a.hkv);
 }
@@ -1020,6 +1022,10 @@ static void launch_fa_d(const fattn_args & a, void * scratch, float * out, hipSt
 }
 
 void launch_fattn(const fattn_args & a, void * scratch, float * out, hipStream_t stream) {
+    if (a.scored) {
+        launch_fattn_scored(a, scratch, out, stream);
+        return;
+    }
     if (a.mfma) {
         launch_fattn_mfma(a, scratch, out, stream);
         return;

@@ -1542,6 +1542,14 @@ bool planner::plan_binary(const ggml_tensor * t) {
     return true;
 }
 
+// attention for the form of capped or biased scores (k_fattn_scored.hip):
+// those, masks a head, and the head sizes and groups the other forms lack
+static bool fattn_scored(const ggml_tensor * t) {
+    const ggml_tensor *q = t->src[0], *k = t->src[1], *m = t->src[3];
+    return op_f32(t, 1) > 0.0f || op_f32(t, 2) > 0.0f || (m && m->ne[2] > 1) ||
+           !fattn_supported((int) q->ne[0], (int) q->ne[2], (int) k->ne[2]);
+}
+
 bool planner::make_fattn(const ggml_tensor * t, fattn_args & a) {
     const ggml_tensor *q = t->src[0], *k = t->src[1], *v = t->src[2], *m = t->src[3];
     // K and V behind GQA expansions that are not launched: the sources'
@@ -1586,6 +1594,11 @@ bool planner::make_fattn(const ggml_tensor * t, fattn_args & a) {
     // into aligned scratch by plan_fattn)
     if ((k->type == GGML_TYPE_F16 && (uintptr_t) a.k % 16 != 0) || (v->type == GGML_TYPE_F16 && (uintptr_t) a.v % 16 != 0))
         return fail(t, "K/V not 16-byte aligned");
+    a.max_bias = op_f32(t, 1), a.softcap = op_f32(t, 2);
+    if (fattn_scored(t)) {
+        fattn_scored_plan(a, n_cu);
+        return true;
+    }
     fattn_plan(a, n_cu);
     // more than one query at the default precision (op_params[3], the
     // host's flash-attention precision contract): the matrix-core form
@@ -1637,7 +1650,7 @@ bool planner::plan_fattn(int i, const ggml_tensor * t) {
     fattn_args a;
     if (!make_fattn(t, a)) return false;
     const ggml_tensor * view = nullptr;
-    if (!a.mfma) fattn_quant_out(i, t, a, view);
+    if (!a.mfma && !a.scored) fattn_quant_out(i, t, a, view);
     // f32 K / V the kernel does not read itself: rounded to contiguous f16
     // copies in scratch after the partials -- the f16 definition over
     // f16-rounded K / V, the conversion ggml's GPU backends make as well
@@ -1697,7 +1710,7 @@ bool planner::plan_fattn(int i, const ggml_tensor * t) {
             }
             launch_fattn(la, g, out, s);
         },
-        t, a.mfma ? "flash_attn_mfma" : a.dec ? "flash_attn_dec" : "flash_attn_ext");
+        t, a.scored ? "flash_attn_scored" : a.mfma ? "flash_attn_mfma" : a.dec ? "flash_attn_dec" : "flash_attn_ext");
     if (a.qtype >= 0) {
         act_src = view;
         act_wtype = a.qtype;
@@ -3193,10 +3206,18 @@ bool supports_op(const device_state * dev, const ggml_tensor * t) {
             };
             if (!f32(q) || q->nb[0] != 4 || !kv_ok(k) || !kv_ok(v)) return false;
             if (v->ne[0] != k->ne[0] || k->ne[2] != v->ne[2]) return false;
-            if (op_f32(t, 1) != 0.0f || op_f32(t, 2) != 0.0f) return false;  // max_bias, softcap
-            if (m && (m->type != GGML_TYPE_F16 || m->ne[2] != 1 || m->nb[0] != 2)) return false;
-            if (q->ne[3] % k->ne[3] != 0) return false;
-            return fattn_supported((int) q->ne[0], (int) q->ne[2], (int) k->ne[2]) && is_contiguous(t);
+            const float bias = op_f32(t, 1), cap = op_f32(t, 2);
+            if (!(bias >= 0.0f && bias <= 3.0e38f && cap >= 0.0f && cap <= 3.0e38f) || (bias > 0.0f && !m)) return false;
+            if (m && (m->type != GGML_TYPE_F16 || m->nb[0] != 2 || m->ne[2] < 1 || q->ne[2] % m->ne[2] != 0)) return false;
+            if (q->ne[3] % k->ne[3] != 0 || !is_contiguous(t)) return false;
+            if (!fattn_scored(t)) return true;
+            fattn_args a{};
+            a.d = (int) q->ne[0], a.hq = (int) q->ne[2], a.hkv = (int) k->ne[2], a.n_kv = (int) k->ne[1];
+            // (f32 K and V are read as contiguous copies)
+            if (k->type == GGML_TYPE_F16) a.k_nb1 = (int64_t) k->nb[1], a.k_nb2 = (int64_t) k->nb[2], a.k_nb3 = (int64_t) k->nb[3];
+            if (v->type == GGML_TYPE_F16) a.v_nb1 = (int64_t) v->nb[1], a.v_nb2 = (int64_t) v->nb[2], a.v_nb3 = (int64_t) v->nb[3];
+            return a.hkv > 0 && a.hq % a.hkv == 0 && k->ne[1] == v->ne[1] && (!m || q->ne[3] % m->ne[3] == 0) &&
+                   (double) q->ne[1] * (double) q->ne[2] * (double) q->ne[3] < 16777216.0 && fattn_scored_supported(a);
         }
         case GGML_OP_SOFT_MAX:
             return f32(t) && f32(t->src[0]) && op_f32(t, 1) == 0.0f &&

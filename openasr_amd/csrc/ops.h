@@ -227,7 +227,17 @@ struct fattn_args {
     // one query at the default precision: the workgroup form (k_fattn_dec.hip,
     // float tolerance); its KV splits (0: not used; > 1: partials + combine)
     int dec;
+    // capped or biased scores, masks a head, heads of 256, other group sizes
+    // (k_fattn_scored.hip): scores are cap tanh(s / cap) for a softcap above 0,
+    // and the mask is added times a slope a head for a max_bias above 0
+    float softcap, max_bias;
+    int scored;        // this form takes the attention
+    int scored_split;  // its KV splits (> 1: partials, joined by a launch)
 };
+bool fattn_scored_supported(const fattn_args & a);
+void fattn_scored_plan(fattn_args & a, int n_cu);
+size_t fattn_scored_scratch_bytes(const fattn_args & a);
+void launch_fattn_scored(const fattn_args & a, void * scratch, float * out, hipStream_t s);
 // whether the matrix-core form takes this attention (n_q > 1, D 64 / 128)
 bool fattn_mfma_supported(const fattn_args & a);
 void fattn_mfma_plan(fattn_args & a, int n_cu, bool kv_f32);

@@ -1,0 +1,268 @@
+"""FLASH_ATTN_EXT with capped or biased scores, masks a head, heads of 256 and
+any group size, on the device against its definition in float64.
+
+Bounds count roundings: u = 2^-24 is half a step of f32.
+"""
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def slopes(heads, bias):
+    if bias == 0:
+        return np.ones(heads)
+    n = 1 << (heads.bit_length() - 1)
+    return np.array([2.0 ** (-bias / n * (h + 1)) if h < n else 2.0 ** (-bias / 2 / n * (2 * (h - n) + 1)) for h in range(heads)])
+
+
+def attention64(q, k, v, mask, scale, cap, bias):
+    """q [S, H, Q, D] f32 (rounded to f16 here), k, v [S | 1.., G, N, D] f16, mask [1 | S, 1 | H, Q, N] f16 or
+    None -> out [S, Q, H, D] and how far f32 arithmetic may take it off"""
+    S, H, Q, D = q.shape
+    q = q.astype(np.float16).astype(np.float64)
+    k, v = (np.repeat(np.repeat(x, S // x.shape[0], 0), H // x.shape[1], 1).astype(np.float64) for x in (k, v))
+    N = k.shape[2]
+    mk = np.zeros((1, 1, Q, N)) if mask is None else np.tile(mask.astype(np.float64), (1, H // mask.shape[1], 1, 1))
+    mk = mk + np.zeros((S, H, 1, 1))
+    seen = mk != -np.inf
+    k_seen = np.where(seen.any(2)[..., None], k, 0.0)  # what no query sees may hold anything
+    with np.errstate(invalid="ignore"):
+        s = (q @ k_seen.transpose(0, 1, 3, 2)) * scale
+        size = (np.abs(q) @ np.abs(k_seen).transpose(0, 1, 3, 2)) * abs(scale)
+    b = np.where(seen, mk, 0.0) * slopes(H, bias)[:, None, None]
+    z = cap * np.tanh(s / cap) if cap else s
+    t = np.where(seen, z + b, -np.inf)
+    top = t.max(3, keepdims=True)
+    top = np.where(np.isfinite(top), top, 0.0)
+    p = np.where(seen, np.exp(t - top), 0.0)
+    total = p.sum(3, keepdims=True)
+    w = np.divide(p, total, out=np.zeros_like(p), where=total > 0)
+    # a score's own: the product's sum (D roundings of its terms' size), the scale, the cap (its
+    # polynomial or its quotient: ten roundings of the result and of the cap), the slope and the
+    # bias, the sum, the maximum subtracted, all in the exponent's base
+    tiles = N // 64 + 2
+    E = (D + 4) * U * size + 10 * U * (np.abs(z) + cap) + 4 * U * np.abs(b) + 4 * U * (np.abs(z) + np.abs(b) + np.abs(top) + 20) + 8 * U
+    E = np.where(seen, E, 0.0) + (N + 4 * tiles) * U  # the sums over positions and the tiles' factors
+    vv = [np.where(seen[:, :, i, :, None], v, 0.0) for i in range(Q)]
+    out, err = np.zeros((S, H, Q, D)), np.zeros((S, H, Q, D))
+    for i in range(Q):
+        out[:, :, i] = (w[:, :, i, None] @ vv[i])[:, :, 0]
+        err[:, :, i] = ((w * E)[:, :, i, None] @ np.abs(vv[i]))[:, :, 0] + np.abs(out[:, :, i]) * (w * E).sum(3)[:, :, i, None]
+        # p's low half has a smallest step, 2^-25 of numbers scaled by 2^12
+        err[:, :, i] += N * 2.0 ** -36 * np.abs(vv[i]).max(2) + 4 * U * np.abs(out[:, :, i])
+    return out.transpose(0, 2, 1, 3), 2 * err.transpose(0, 2, 1, 3) + 1e-37
+
+
+def make_mask(kind, S, H, Q, N, bias, rng):
+    i, j = np.arange(Q)[:, None] + (N - Q), np.arange(N)[None]
+    dist = -np.abs(i - j).astype(np.float64) if bias else np.zeros((Q, N))
+    m = np.where(j <= i, dist, -np.inf)
+    if kind == "none":
+        return None
+    if kind == "causal":
+        m = m[None, None]
+    elif kind == "documents":
+        cut = np.sort(rng.choice(np.arange(1, N), min(3, N - 1), replace=False)) if N > 1 else np.array([], int)
+        doc = np.searchsorted(cut, np.arange(N), side="right")
+        m = np.where(doc[None] == doc[np.minimum(i, N - 1)[:, 0]][:, None], m, -np.inf)[None, None]
+    elif kind == "prefix":  # all see the first part, the rest is causal
+        m = np.where(j < N // 3, dist, m)[None, None]
+    elif kind == "empty":  # rows that see nothing, in one sequence a whole block of them
+        m = np.repeat(m[None, None], S, 0)
+        m[:, :, rng.random(Q) < 0.3] = -np.inf
+        m[0, :, : (Q + 1) // 2] = -np.inf
+    elif kind == "lowest":  # masked by f16's lowest value, and in one row everything
+        m = np.where(np.isinf(m), -65504.0, m)[None, None]
+        m[:, :, -1] = -65504.0
+    elif kind == "heads":
+        m = np.repeat(np.repeat(m[None, None], S, 0), H, 1)
+        m[rng.random(m.shape) < 0.5] = -np.inf
+        m[..., 0] = 0
+    elif kind == "some heads":  # two masks, in turn over the heads
+        m = np.repeat(m[None, None], 2, 1)
+        m[:, 1] = np.where(rng.random((Q, N)) < 0.7, dist, -np.inf)
+    elif kind == "random":
+        m = np.where(rng.random((S, 1, Q, N)) < 0.4, rng.standard_normal((S, 1, Q, N)) * 3, -np.inf)
+    elif kind == "lengths":
+        m = np.repeat(dist[None, None], S, 0)
+        for s in range(S):
+            m[s, :, :, max(1, N - 1 - (s * 37) % N):] = -np.inf
+    return m.astype(np.float16)
+
+
+def attention(ggml, gpu, q, k, v, mask, scale, cap, bias, prec=None, kv32=False, times=3):
+    S, H, Q, D = q.shape
+    G = ggml.Graph(64, 64)
+    X = G.new(ggml.F32, D, H, Q, S)  # token by token, as a projection leaves them
+    t = ggml.F32 if kv32 else ggml.F16
+    K, V = (G.new(t, D, x.shape[2], x.shape[1], x.shape[0]) for x in (k, v))
+    M = G.new(ggml.F16, mask.shape[3], mask.shape[2], mask.shape[1], mask.shape[0]) if mask is not None else None
+    y = G.lib.ggml_flash_attn_ext(G.ctx, G.lib.ggml_permute(G.ctx, X, 0, 2, 1, 3), K, V, M, scale, bias, cap)
+    assert y
+    if prec is not None:
+        G.lib.ggml_flash_attn_ext_set_prec(y, prec)
+    G.build(y)
+    G.allocate(gpu.buft)
+    G.set(X, q.transpose(0, 2, 1, 3))
+    for T, x in ((K, k), (V, v)):
+        G.set(T, x.astype(np.float32) if kv32 else x.view(np.uint16))
+    if M:
+        G.set(M, mask.view(np.uint16))
+    outs = []
+    for _ in range(times):
+        assert G.compute(gpu.backend) == 0
+        outs.append(G.get(y).reshape(S, Q, H, D))
+    G.free()
+    for o in outs[1:]:
+        assert np.array_equal(o, outs[0], equal_nan=True)
+    return outs[0]
+
+
+def check(got, want, bound, what=""):
+    assert np.isfinite(got).all(), what
+    off = np.abs(got.astype(np.float64) - want) - bound
+    assert (off <= 0).all(), f"{what}: off by {np.abs(got - want).flat[np.argmax(off)]:.3g}, allowed {bound.flat[np.argmax(off)]:.3g}"
+
+
+def operands(rng, S, H, G, Q, N, D, std=1.0, kv_seqs=None):
+    q = (std * rng.standard_normal((S, H, Q, D))).astype(np.float32)
+    k, v = (rng.standard_normal((kv_seqs or S, G, N, D)).astype(np.float16) for _ in range(2))
+    return q, k, v
+
+
+#        D    H   G  Q    N    S  mask        cap   bias
+CASES = [(128, 4, 2, 1, 1, 1, "causal", 30.0, 0.0),
+         (128, 4, 2, 1, 300, 3, "lengths", 50.0, 0.0),
+         (64, 20, 4, 1, 1000, 2, "lengths", 0.0, 8.0),
+         (256, 3, 1, 1, 130, 1, "lengths", 30.0, 8.0),
+         (128, 12, 1, 1, 65, 1, "causal", 0.0, 8.0),
+         (64, 2, 2, 2, 2, 1, "causal", 50.0, 0.0),
+         (128, 4, 2, 65, 65, 1, "causal", 50.0, 0.0),
+         (64, 6, 2, 130, 131, 2, "causal", 0.0, 8.0),
+         (256, 4, 2, 70, 200, 1, "causal", 30.0, 8.0),
+         (128, 6, 2, 77, 77, 1, "documents", 50.0, 0.0),
+         (64, 5, 1, 200, 200, 1, "documents", 0.0, 4.0),
+         (128, 16, 2, 33, 400, 1, "prefix", 30.0, 8.0),
+         (64, 4, 4, 40, 100, 2, "empty", 30.0, 0.0),
+         (128, 4, 1, 20, 129, 2, "empty", 0.0, 8.0),
+         (64, 2, 1, 20, 90, 1, "lowest", 30.0, 0.0),
+         (64, 4, 2, 30, 100, 2, "heads", 30.0, 8.0),
+         (128, 6, 3, 1, 200, 2, "heads", 0.0, 0.0),
+         (64, 4, 2, 70, 72, 1, "some heads", 0.0, 0.0),
+         (128, 4, 2, 50, 257, 2, "random", 0.0, 8.0),
+         (64, 8, 1, 9, 500, 2, "random", 50.0, 0.0),
+         (64, 2, 1, 70, 100, 1, "none", 30.0, 0.0),
+         (256, 2, 2, 5, 64, 1, "none", 0.0, 0.0),
+         (128, 3, 1, 1, 700, 1, "none", 30.0, 0.0),
+         (128, 40, 2, 7, 333, 1, "causal", 50.0, 0.0),
+         (64, 64, 1, 3, 70, 1, "causal", 50.0, 0.0),
+         (128, 2, 1, 300, 1500, 1, "causal", 30.0, 0.0)]
+
+
+@pytest.mark.parametrize("D,H,G,Q,N,S,kind,cap,bias", CASES)
+def test_scored_attention(ggml, gpu, D, H, G, Q, N, S, kind, cap, bias):
+    print(f"scored attention D={D} H={H} G={G} Q={Q} N={N} S={S} {kind} cap={cap} bias={bias}", flush=True)
+    rng = np.random.default_rng(D + H + Q + N)
+    q, k, v = operands(rng, S, H, G, Q, N, D, std=2.0)
+    mask = make_mask(kind, S, H, Q, N, bias, rng)
+    scale = 1 / np.sqrt(D)
+    want, bound = attention64(q, k, v, mask, scale, cap, bias)
+    for prec in (None, ggml.GGML_PREC_F32):
+        check(attention(ggml, gpu, q, k, v, mask, scale, cap, bias, prec), want, bound, f"prec {prec}")
+
+
+@pytest.mark.parametrize("Q,N", [(1, 200), (40, 200)])
+@pytest.mark.parametrize("std", [3.0, 20.0, 300.0])
+def test_scores_past_the_cap(ggml, gpu, Q, N, std):
+    """scores about the cap and far past it: the tanh's other branch"""
+    rng = np.random.default_rng(3)
+    q, k, v = operands(rng, 1, 4, 2, Q, N, 64, std=std)
+    mask = make_mask("causal", 1, 4, Q, N, 0, rng)
+    want, bound = attention64(q, k, v, mask, 0.125, 5.0, 0.0)
+    check(attention(ggml, gpu, q, k, v, mask, 0.125, 5.0, 0.0), want, bound)
+
+
+@pytest.mark.parametrize("D,Q,N", [(64, 1, 150), (128, 30, 200), (64, 100, 130), (256, 9, 80)])
+@pytest.mark.parametrize("bias", [0.0, 8.0])
+def test_masked_places_hold_anything(ggml, gpu, D, Q, N, bias):
+    """NaN and infinities in K and V where the mask hides them, for all queries and for some"""
+    rng = np.random.default_rng(D + Q)
+    q, k, v = operands(rng, 2, 4, 2, Q, N, D)
+    mask = np.repeat(make_mask("causal", 2, 4, Q, N, bias, rng), 2, 0)
+    hidden = rng.random(N) < 0.2          # nobody sees these
+    hidden[0] = False
+    mask[..., hidden] = -np.inf
+    some = ~hidden & (np.arange(N) > N // 2) & (rng.random(N) < 0.2)  # the last query alone does not
+    mask[:, :, -1, some] = -np.inf
+    want, bound = attention64(q, k, v, mask, 0.1, 30.0, bias)
+    k2, v2 = k.copy(), v.copy()
+    for x in (k2, v2):
+        x[:, :, hidden] = np.array([np.nan, np.inf, -np.inf, 3.0], np.float16)[rng.integers(0, 4, (2, 2, hidden.sum(), D))]
+    v3 = v2.copy()
+    v3[:, :, some, 5] = np.inf            # reaches its dim, and only of the queries that see it
+    check(attention(ggml, gpu, q, k2, v2, mask, 0.1, 30.0, bias), want, bound)
+    got = attention(ggml, gpu, q, k2, v3, mask, 0.1, 30.0, bias)
+    sees = (mask[..., some] != -np.inf).any(3)[0, 0] if some.any() else np.zeros(Q, bool)
+    rest = np.ones(got.shape, bool)
+    rest[:, sees, :, 5] = False
+    assert not np.isfinite(got[:, sees, :, 5]).any()
+    check(np.where(rest, got, 0), np.where(rest, want, 0), bound)
+
+
+@pytest.mark.parametrize("Q", [1, 20])
+def test_layouts(ggml, gpu, Q):
+    """f32 K and V, K and V shared by sequences, one mask for all of them, a mask of more rows and odd strides"""
+    rng = np.random.default_rng(5)
+    q, k, v = operands(rng, 4, 6, 2, Q, 101, 64, kv_seqs=2)
+    mask = make_mask("causal", 4, 6, Q, 101, 8.0, rng)
+    want, bound = attention64(q, k, v, mask, 0.125, 30.0, 8.0)
+    check(attention(ggml, gpu, q, k, v, mask, 0.125, 30.0, 8.0), want, bound, "f16")
+    check(attention(ggml, gpu, q, k, v, mask, 0.125, 30.0, 8.0, kv32=True), want, bound, "f32")
+    more = np.concatenate([mask, np.full((1, 1, 3, 101), np.nan, np.float16)], 2)
+    check(attention(ggml, gpu, q, k, v, more, 0.125, 30.0, 8.0), want, bound, "more rows")
+
+
+def test_part_of_a_cache(ggml, gpu):
+    """the first positions of a cache whose other rows are written later"""
+    rng = np.random.default_rng(6)
+    D, H, G, Q, N, S, rows = 128, 4, 2, 9, 70, 2, 256
+    q, k, v = operands(rng, S, H, G, Q, rows, D)
+    mask = make_mask("causal", S, H, Q, N, 0, rng)
+    want, bound = attention64(q, k[:, :, :N], v[:, :, :N], mask, 0.1, 20.0, 0.0)
+    g = ggml.Graph(64, 64)
+    X, K, V = g.new(ggml.F32, D, Q, H, S), g.new(ggml.F16, D, rows, G, S), g.new(ggml.F16, D, rows, G, S)
+    M = g.new(ggml.F16, N, Q, 1, 1)
+    kv = [g.lib.ggml_view_4d(g.ctx, t, D, N, G, S, 2 * D, 2 * D * rows, 2 * D * rows * G, 0) for t in (K, V)]
+    y = g.lib.ggml_flash_attn_ext(g.ctx, X, *kv, M, 0.1, 0.0, 20.0)
+    g.build(y)
+    g.allocate(gpu.buft)
+    for t, a in ((X, q), (K, k.view(np.uint16)), (V, v.view(np.uint16)), (M, mask.view(np.uint16))):
+        g.set(t, a)
+    for _ in range(3):
+        assert g.compute(gpu.backend) == 0
+        check(g.get(y).reshape(S, Q, H, D), want, bound)
+    g.free()
+
+
+def test_supports(ggml, gpu):
+    """what the device refuses, and says so"""
+    G = ggml.Graph(64, 64)
+
+    def ok(D=64, H=4, Gh=2, mask=(9, 5, 1, 1), kv=None, bias=8.0, cap=30.0):
+        q = G.new(ggml.F32, D, 5, H, 1)
+        k = kv or G.new(ggml.F16, D, 9, Gh, 1)
+        m = G.new(ggml.F16, *mask) if mask else None
+        return gpu_supports(G.lib.ggml_flash_attn_ext(G.ctx, q, k, k, m, 0.1, bias, cap))
+
+    def gpu_supports(t):
+        return G.lib.ggml_backend_supports_op(gpu.backend, t)
+
+    assert ok() and ok(D=256) and ok(H=10, Gh=2) and ok(mask=(9, 5, 4, 1)) and ok(mask=(9, 5, 2, 1))
+    assert ok(mask=None, bias=0.0)
+    assert not ok(D=96) and not ok(H=130, Gh=2)
+    wide = G.new(ggml.F16, 68, 9, 2, 1)  # rows of 136 bytes
+    assert not ok(kv=G.lib.ggml_view_4d(G.ctx, wide, 64, 9, 2, 1, 136, 136 * 9, 136 * 18, 0))
+    G.free()
