@@ -12,6 +12,7 @@
 namespace mi355x {
 
 typedef float dl_v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t dl_u2 __attribute__((ext_vector_type(2)));
 
 // ------------------------------------------------------------- l2 norm ---
 
@@ -48,6 +49,17 @@ __device__ __forceinline__ float dl_sum16(float v) {
     add(std::integral_constant<int, 0x124>{});
     add(std::integral_constant<int, 0x122>{});
     add(std::integral_constant<int, 0x121>{});
+    return v;
+}
+
+__device__ __forceinline__ float dl_max16(float v) {  // of values from zero on
+    auto most = [&](auto ctrl) {
+        v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, true)));
+    };
+    most(std::integral_constant<int, 0x128>{});
+    most(std::integral_constant<int, 0x124>{});
+    most(std::integral_constant<int, 0x122>{});
+    most(std::integral_constant<int, 0x121>{});
     return v;
 }
 
@@ -177,48 +189,66 @@ __global__ __launch_bounds__(256) void k_delta_rows(delta_args a) {
 //
 // Chunks of C = 64 tokens as matrix products. With a_t the sum of the chunk's g
 // up to t, L_ts = e^(a_t - a_s) and
-//     A = strictly lower (beta_t k_t . k_s L_ts),   (1 + A) U = beta V,   (1 + A) W = beta e^a K
+//     A = strictly lower (beta_t k_t . k_s L_ts),   T = (1 + A)^-1
 // a chunk turns the state S0 it meets into
-//     D = U - W S0,   Y = (e^a Q S0 + lower(Q K^T L) D) / sqrt(K),   S1 = e^(a_C) S0 + (e^(a_C - a) K)^T D
-// k_delta_solve makes W, U, lower(Q K^T L) and the decays of every chunk at once
+//     D = T (beta V - beta e^a K S0),   Y = (e^a Q S0 + lower(Q K^T L) D) / sqrt(K)
+//     S1 = e^(a_C) S0 + (e^(a_C - a) K)^T D
+// k_delta_solve makes T, lower(Q K^T L) and the decays of every chunk at once
 // (forward substitution by blocks of 16 tokens, whose diagonal blocks are
 // inverted column by column: as stable as the recurrence), k_delta_chunks goes
-// through the chunks, a workgroup a head and 16 columns of the state.
-// All products are f32's, on v_mfma_f32_16x16x4f32: A lane l = row l % 16, k l /
-// 16; B lane l = column l % 16, the same k; result lane l = rows 4 (l / 16) ..
-// + 3, column l % 16. Step i of four takes k = 4 (l / 16) + i, so that a result's
-// four elements are the next product's B operand as they are, and A's rows come
-// in 16-byte pieces.
+// through the chunks, a workgroup a head and 16 or 32 columns of the state.
 //
-// A chunk whose values are not finite, whose g are above zero, or whose sizes
-// could leave f32's range in the products' order, runs token by token: the
-// normalised rows of q and k are at most 2^10, W 2^20, U and the state 2^60, so
-// D is under 2^88, a state after under 2^113, y under 2^122.
-
-typedef uint32_t dl_u4 __attribute__((ext_vector_type(4)));
+// k_delta_solve's products are f32's, on v_mfma_f32_16x16x4f32: A lane l = row l
+// % 16, k l / 16; B lane l = column l % 16, the same k; result lane l = rows 4 (l
+// / 16) .. + 3, column l % 16. Step i of four takes k = 4 (l / 16) + i, so that
+// a result's four elements are the next product's B operand as they are, and A's
+// rows come in 16-byte pieces.
+//
+// k_delta_chunks, whose chain of products is the time, makes them on the f16
+// matrix cores: an operand is the sum of two f16 (22 bits), a product three of
+// theirs, 24 cycles for 16 k where f32's take 128 (three bf16 parts and six
+// products, 48, and their making in the chain took more time than they). Rows of
+// Q, K, T and lower(Q K^T L) are split by k_delta_solve, each row scaled to 2^13 by
+// a power of two that the row's factor takes back; the state, T's operand and D
+// are split as they are made, scaled by powers of two from the largest value that
+// the state and v had a chunk before, with room for 2^7 .. 2^10 times as much. A
+// lane's eight k of 32 are four of one block of 16 and four of the next, so that
+// results are operands here too.
+//
+// A chunk whose values are not finite, whose g are above zero, or whose scaled
+// values would leave f16's range, runs token by token (a state that starts at
+// zero, say, and meets v: the second such chunk has its scale).
 
 constexpr int kDlC = 64;
-constexpr float kDlRow = 0x1p10f, kDlRaw = 0x1p50f, kDlW = 0x1p20f, kDlU = 0x1p60f;
+// what the products take: q's and k's rows as they come, and (the largest element of a
+// row) brought to length; beta; T; scaled values. The state and v: up to 2^40
+constexpr float kDlRaw = 0x1p50f, kDlRow = 0x1p10f, kDlLeast = 0x1p-20f, kDlBeta = 16.0f, kDlT = 0x1p20f, kDlHalf = 60000.0f;
 
 struct dl_chunk_args {
     delta_args a;
     char * rec;          // records [sequence][head][chunk of the slab]
+    char * krec;         // K^T [sequence][key head][chunk]: blocks (16 dims, 16 tokens), lane = row d l % 16, t 4 (l / 16) ..
     const char * s_in;   // the states the slab starts from
     int64_t s_in_nb3;
     int64_t c0, chunks;  // the slab's first chunk and its chunks
-    int vblocks;         // 16-column blocks of the state
-    int rec_size;
+    int cols;            // column blocks of the state: 16 or 32 columns
 };
-// byte offsets in a record
+// byte offsets in a record of a head's chunk
 struct dl_rec {
-    // [64] f32 each: what a row of Q S0 is multiplied by (e^a, q's length and
-    // 1 / sqrt(K)); what a row of D is for the state (e^(a_C - a) and k's length)
-    static constexpr int in = 0, left = 256;
-    static constexpr int end = 512;   // e^(a_C); whether the chunk goes token by token
-    static constexpr int bad = 516;
-    static constexpr int p = 1024;    // lower(Q K^T L) / sqrt(K): blocks (tb, sb <= tb), lane = row t l % 16, s 4 (l / 16) ..
-    static constexpr int w = p + 10 * 1024;  // -W [64][NP]
-    // then U: [column block][token block][lane] of results
+    // [64] f32 each, what a row is multiplied by: of Q S0 (e^a, 1 / sqrt(K) and
+    // what takes the scales back, times that of p's row), of Y (takes p's back), of
+    // K S0 (beta, e^a), of V (beta), of T's product, of D for the state (e^(a_C - a)
+    // over the largest of these)
+    static constexpr int in = 0, y = 256, ks = 512, beta = 768, t_row = 1024, left = 1280;
+    static constexpr int end = 1536;  // e^(a_C); what left was divided by; whether the chunk goes token by token
+    // [4 token blocks][2 steps of 32 tokens][2 parts][lane] of lower(Q K^T L) / sqrt(K), and of T
+    static constexpr int p = 2048, t = p + 16 * 1024;
+    static constexpr int size = t + 16 * 1024;
+};
+// of a key head's: rows of Q and of K [4 token blocks][steps of 32 dims][2 parts][lane], K^T [dim blocks][2 steps of 32 tokens][2 parts][lane]
+template <int NP>
+struct dl_krec {
+    static constexpr int q = 0, k = 4 * kDlC * NP, kt = 2 * k, size = 3 * k;
 };
 __device__ __forceinline__ int dl_pair(int tb, int sb) { return tb * (tb + 1) / 2 + sb; }
 
@@ -229,117 +259,231 @@ __device__ __forceinline__ dl_v4f dl_mfma(dl_v4f a, dl_v4f b, dl_v4f c) {
 }
 __device__ __forceinline__ bool dl_past(float v, float limit) { return !(fabsf(v) <= limit); }
 
+typedef uint32_t dl_u4 __attribute__((ext_vector_type(4)));
+typedef _Float16 dl_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 dl_h8 __attribute__((ext_vector_type(8)));
+// two f32 as the sums of two f16 each
+__device__ __forceinline__ void dl_split2(float a, float b, uint32_t & hi, uint32_t & lo) {
+    const dl_h2 h = __builtin_bit_cast(dl_h2, __builtin_amdgcn_cvt_pkrtz(a, b));
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float) h[0], b - (float) h[1]));
+}
+struct dl_split {  // a lane's eight elements of k
+    dl_u4 v[2];
+};
+__device__ __forceinline__ dl_split dl_split8(dl_v4f a, dl_v4f b) {
+    uint32_t h[4], l[4];
+    dl_split2(a[0], a[1], h[0], l[0]);
+    dl_split2(a[2], a[3], h[1], l[1]);
+    dl_split2(b[0], b[1], h[2], l[2]);
+    dl_split2(b[2], b[3], h[3], l[3]);
+    return {{dl_u4{h[0], h[1], h[2], h[3]}, dl_u4{l[0], l[1], l[2], l[3]}}};
+}
+// the i-th of a product's three, the small ones first
+__device__ __forceinline__ dl_v4f dl_product(int i, const dl_split & a, const dl_split & b, dl_v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(dl_h8, a.v[i == 0]), __builtin_bit_cast(dl_h8, b.v[i == 1]), c, 0, 0, 0);
+}
+// 2^e, and the exponent of the power of two at or under |v| (within what f32's powers and their inverses hold)
+__device__ __forceinline__ float dl_pow2(int e) { return __uint_as_float((uint32_t) (e + 127) << 23); }
+__device__ __forceinline__ int dl_exponent(float v) { return min(max((int) ((__float_as_uint(v) >> 23) & 255) - 127, -100), 100); }
+
 template <int NP>
-__global__ __launch_bounds__(256) void k_delta_solve(dl_chunk_args q) {
-    constexpr int kRow = NP + 4, KB = NP / 16;
-    __shared__ __align__(16) float s_k[kDlC][kRow], s_q[kDlC][kRow];
-    __shared__ float s_klen[kDlC], s_qlen[kDlC], s_beta[kDlC];
+__global__ __launch_bounds__(256, 2) void k_delta_solve(dl_chunk_args q) {
+    constexpr int kRow = NP + 4, KB = NP / 16, kLoads = kDlC * NP / 1024;
+    __shared__ __align__(16) float s_k[kDlC][kRow];
+    __shared__ __align__(16) float s_kexp[kDlC], s_qexp[kDlC], s_beta[kDlC];  // s_kexp, s_qexp: a row's scale, to 2^13
     __shared__ double s_cum[kDlC];
-    __shared__ dl_v4f s_a[10][64];                    // A's blocks, lane = row t l % 16, s 4 (l / 16) ..
-    __shared__ __align__(16) float s_d[4][16][20];    // the diagonal ones, then their inverses, row by row
+    // A's blocks, lane = row t l % 16, s 4 (l / 16) ..; then T's rows
+    __shared__ __align__(16) float s_at[kDlC * (kDlC + 4)];
+    __shared__ __align__(16) float s_d[4][16][20];  // the diagonal blocks, then their inverses, row by row
+    dl_v4f(&s_a)[10][64] = *(dl_v4f(*)[10][64]) s_at;
+    float(&s_t)[kDlC][kDlC + 4] = *(float(*)[kDlC][kDlC + 4]) s_at;
     const delta_args & a = q.a;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, lg = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lg = lane >> 4;
     const int64_t c = blockIdx.x % q.chunks;
     const int hk = (int) (blockIdx.x / q.chunks % a.key_heads), s = (int) (blockIdx.x / q.chunks / a.key_heads);
     const int64_t t0 = (q.c0 + c) * kDlC;
     const int nt = (int) min((int64_t) kDlC, a.tokens - t0);
     const char * kb = a.k + hk * a.k_nb1 + t0 * a.k_nb2 + s * a.k_nb3;
     const char * qb = a.q + hk * a.q_nb1 + t0 * a.q_nb2 + s * a.q_nb3;
+    char * const krec = q.krec + (((int64_t) s * a.key_heads + hk) * q.chunks + c) * dl_krec<NP>::size;
     bool bad = false;
-    for (int i = tid; i < kDlC * NP / 4; i += 256) {
-        const int t = i / (NP / 4), n = i % (NP / 4) * 4;
-        dl_v4f kv = {0, 0, 0, 0}, qv = {0, 0, 0, 0};
-        if (t < nt && n < a.K) {
-            kv = *(const dl_v4f *) (kb + t * a.k_nb2 + 4 * n);
-            qv = *(const dl_v4f *) (qb + t * a.q_nb2 + 4 * n);
-        }
+    // k's rows, and the wave's 16 rows of q as a B operand, all loads in flight
+    dl_v4f kv[kLoads], qr[KB];
 #pragma unroll
-        for (int e = 0; e < 4; e++) bad |= dl_past(kv[e], kDlRaw) || dl_past(qv[e], kDlRaw);
-        *(dl_v4f *) &s_k[t][n] = kv;
-        *(dl_v4f *) &s_q[t][n] = qv;
+    for (int i = 0; i < kLoads; i++) {
+        const int e = tid + 256 * i, t = e / (NP / 4), n = e % (NP / 4) * 4;
+        kv[i] = *(const dl_v4f *) (kb + min(t, nt - 1) * a.k_nb2 + 4 * min(n, a.K - 4));
+    }
+    const int tq = 16 * wave + l16;
+#pragma unroll
+    for (int k = 0; k < KB; k++) qr[k] = *(const dl_v4f *) (qb + min(tq, nt - 1) * a.q_nb2 + 4 * min(16 * k + 4 * lg, a.K - 4));
+    // a head's gates and betas, a token a lane
+    const int tg = min(lane, nt - 1);
+    auto gate = [&](int h) { return *(const float *) (a.g + h * a.g_nb1 + (t0 + tg) * a.g_nb2 + s * a.g_nb3); };
+    auto beta = [&](int h) { return *(const float *) (a.beta + h * a.b_nb1 + (t0 + tg) * a.b_nb2 + s * a.b_nb3); };
+    float next_g = gate(hk), next_b = beta(hk);
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+        const int e = tid + 256 * i, t = e / (NP / 4), n = e % (NP / 4) * 4;
+        if (t >= nt || n >= a.K) kv[i] = dl_v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 4; j++) bad |= dl_past(kv[i][j], kDlRaw);
+        *(dl_v4f *) &s_k[t][n] = kv[i];
+    }
+    {
+        float sum = 0.0f, most = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KB; k++) {
+            if (tq >= nt || 16 * k + 4 * lg >= a.K) qr[k] = dl_v4f{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; j++) bad |= dl_past(qr[k][j], kDlRaw), sum = fmaf(qr[k][j], qr[k][j], sum), most = fmaxf(most, fabsf(qr[k][j]));
+        }
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        const float f = a.q_eps < 0.0f ? 1.0f : 1.0f / fmaxf(sqrtf(sum), a.q_eps);
+        most *= f;
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        bad |= dl_past(most, kDlRow) || (most > 0.0f && most < kDlLeast);
+        const float sc = dl_pow2(13 - dl_exponent(most));
+        dl_u4 * o = (dl_u4 *) (krec + dl_krec<NP>::q) + wave * (KB / 2) * 128 + lane;
+#pragma unroll
+        for (int k = 0; k < KB; k += 2) {
+            qr[k] *= f, qr[k + 1] *= f;
+            const dl_split x = dl_split8(qr[k] * sc, qr[k + 1] * sc);
+            o[64 * k] = x.v[0], o[64 * k + 64] = x.v[1];
+        }
+        if (lg == 0) s_qexp[tq] = sc;
     }
     __syncthreads();
     {
-        // the rows' lengths: four threads a row
+        // k's lengths: four threads a row
         const int t = tid >> 2, n0 = (tid & 3) * (NP / 4);
-        auto scale = [&](float (&rows)[kDlC][kRow], float eps) {
-            float sum = 0.0f, most = 0.0f;
+        float sum = 0.0f, most = 0.0f;
 #pragma unroll
-            for (int n = 0; n < NP / 4; n += 4) {
-                const dl_v4f v = *(const dl_v4f *) &rows[t][n0 + n];
+        for (int n = 0; n < NP / 4; n += 4) {
+            const dl_v4f v = *(const dl_v4f *) &s_k[t][n0 + n];
 #pragma unroll
-                for (int e = 0; e < 4; e++) sum = fmaf(v[e], v[e], sum), most = fmaxf(most, fabsf(v[e]));
-            }
-            sum += __shfl_xor(sum, 1);
-            sum += __shfl_xor(sum, 2);
-            const float f = eps < 0.0f ? 1.0f : 1.0f / fmaxf(sqrtf(sum), eps);
-            bad |= dl_past(most * f, kDlRow);
+            for (int e = 0; e < 4; e++) sum = fmaf(v[e], v[e], sum), most = fmaxf(most, fabsf(v[e]));
+        }
+        sum += __shfl_xor(sum, 1);
+        sum += __shfl_xor(sum, 2);
+        const float f = a.k_eps < 0.0f ? 1.0f : 1.0f / fmaxf(sqrtf(sum), a.k_eps);
 #pragma unroll
-            for (int n = 0; n < NP / 4; n += 4) {
-                dl_v4f v = *(const dl_v4f *) &rows[t][n0 + n];
-                v *= f;
-                *(dl_v4f *) &rows[t][n0 + n] = v;
-            }
-            return f;
-        };
-        const float kl = scale(s_k, a.k_eps), ql = scale(s_q, a.q_eps);
-        if ((tid & 3) == 0) s_klen[t] = t < nt ? kl : 0.0f, s_qlen[t] = t < nt ? ql : 0.0f;
+        for (int n = 0; n < NP / 4; n += 4) {
+            dl_v4f v = *(const dl_v4f *) &s_k[t][n0 + n];
+            v *= f;
+            *(dl_v4f *) &s_k[t][n0 + n] = v;
+        }
+        most *= f;
+        most = fmaxf(most, __shfl_xor(most, 1));
+        most = fmaxf(most, __shfl_xor(most, 2));
+        bad |= dl_past(most, kDlRow) || (most > 0.0f && most < kDlLeast);
+        if ((tid & 3) == 0) s_kexp[t] = dl_pow2(13 - dl_exponent(most));
     }
     bad = __syncthreads_or(bad);
-    // k_s . k_t and k_s . q_t: rows s, columns t, twenty blocks over the waves
-    dl_v4f dots[5];
+    {
+        // K's rows and K^T
+        const float sc = s_kexp[tq];
+        dl_u4 * o = (dl_u4 *) (krec + dl_krec<NP>::k) + wave * (KB / 2) * 128 + lane;
 #pragma unroll
-    for (int n = 0; n < 5; n++) {
-        const int i = wave + 4 * n, pr = i < 10 ? i : i - 10;
-        const int tb = pr < 1 ? 0 : pr < 3 ? 1 : pr < 6 ? 2 : 3, sb = pr - tb * (tb + 1) / 2;
-        const float(&x)[kDlC][kRow] = i < 10 ? s_k : s_q;
-        dots[n] = dl_v4f{0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < KB; k++)
-            dots[n] = dl_mfma(*(const dl_v4f *) &s_k[16 * sb + l16][16 * k + 4 * lg], *(const dl_v4f *) &x[16 * tb + l16][16 * k + 4 * lg], dots[n]);
+        for (int k = 0; k < KB; k += 2) {
+            const dl_split x = dl_split8(*(const dl_v4f *) &s_k[tq][16 * k + 4 * lg] * sc, *(const dl_v4f *) &s_k[tq][16 * k + 16 + 4 * lg] * sc);
+            o[64 * k] = x.v[0], o[64 * k + 64] = x.v[1];
+        }
+        o = (dl_u4 *) (krec + dl_krec<NP>::kt) + lane;
+#pragma unroll 2
+        for (int i = wave; i < 2 * KB; i += 4) {
+            const int t = 32 * (i & 1) + 4 * lg;
+            const float * x = &s_k[t][16 * (i >> 1) + l16];
+            const dl_v4f s0 = *(const dl_v4f *) &s_kexp[t], s1 = *(const dl_v4f *) &s_kexp[t + 16];
+            const dl_split z = dl_split8(dl_v4f{x[0], x[kRow], x[2 * kRow], x[3 * kRow]} * s0,
+                                         dl_v4f{x[16 * kRow], x[17 * kRow], x[18 * kRow], x[19 * kRow]} * s1);
+            o[128 * i] = z.v[0], o[128 * i + 64] = z.v[1];
+        }
     }
+    // k_s . q_t for the wave's t, k_s . k_t for those of wave 3 - w: rows s, columns t, five blocks a wave
+    const int tk = 3 - wave;
+    dl_v4f kq[4], kk[4];
+#pragma unroll
+    for (int sb = 0; sb < 4; sb++) {
+        kq[sb] = kk[sb] = dl_v4f{0, 0, 0, 0};
+        if (sb <= wave) {
+#pragma unroll
+            for (int k = 0; k < KB; k++) kq[sb] = dl_mfma(*(const dl_v4f *) &s_k[16 * sb + l16][16 * k + 4 * lg], qr[k], kq[sb]);
+        }
+        if (sb <= tk) {
+#pragma unroll
+            for (int k = 0; k < KB; k++)
+                kk[sb] = dl_mfma(*(const dl_v4f *) &s_k[16 * sb + l16][16 * k + 4 * lg], *(const dl_v4f *) &s_k[16 * tk + l16][16 * k + 4 * lg], kk[sb]);
+        }
+    }
+    // the wave's rows of a matrix over the chunk's tokens, split
+    auto put_rows = [&](dl_u4 * o, const dl_v4f (&v)[4], float sc) {
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            if (2 * m > wave) continue;
+            const dl_split x = dl_split8(v[2 * m] * sc, v[2 * m + 1] * sc);
+            o[(2 * wave + m) * 128 + lane] = x.v[0], o[(2 * wave + m) * 128 + 64 + lane] = x.v[1];
+        }
+    };
     for (int h = hk; h < a.heads; h += a.key_heads) {
-        char * rec = q.rec + (((int64_t) s * a.heads + h) * q.chunks + c) * q.rec_size;
+        char * rec = q.rec + (((int64_t) s * a.heads + h) * q.chunks + c) * dl_rec::size;
         bool own_bad = bad;
+        const float g = lane < nt ? next_g : 0.0f, b = lane < nt ? next_b : 0.0f;
+        const int more = min(h + a.key_heads, a.heads - 1);
+        next_g = gate(more), next_b = beta(more);
         if (wave == 0) {
-            // the decays: their logarithms summed in f64 (from -1000 on a power is zero)
-            const bool in = lane < nt;
-            const float g = in ? *(const float *) (a.g + h * a.g_nb1 + (t0 + lane) * a.g_nb2 + s * a.g_nb3) : 0.0f;
-            const float b = in ? *(const float *) (a.beta + h * a.b_nb1 + (t0 + lane) * a.b_nb2 + s * a.b_nb3) : 0.0f;
-            own_bad |= !(g <= 0.0f) || dl_past(b, kDlRow);
-            double cum = fmax((double) g, -1000.0);
+            // the decays: their base 2 logarithms summed in f64 (from -1000 on a power is zero)
+            own_bad |= !(g <= 0.0f) || dl_past(b, kDlBeta);
+            double cum = fmax((double) g, -1000.0) * 1.4426950408889634074;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
                 const double v = __shfl_up(cum, o);
                 if (lane >= o) cum += v;
             }
             const double all = __shfl(cum, 63);
+            const float e = __builtin_amdgcn_exp2f((float) cum);
+            const float kinv = 1.0f / s_kexp[lane];
+            float most = kinv;  // (the last token's decay is one)
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
             s_cum[lane] = cum;
             s_beta[lane] = b;
-            ((float *) (rec + dl_rec::in))[lane] = expf((float) cum) * s_qlen[lane] * a.scale;
-            ((float *) (rec + dl_rec::left))[lane] = expf((float) (all - cum)) * s_klen[lane];
-            if (lane == 0) *(float *) (rec + dl_rec::end) = expf((float) all);
+            ((float *) (rec + dl_rec::ks))[lane] = b * e * kinv;
+            ((float *) (rec + dl_rec::beta))[lane] = b;
+            ((float *) (rec + dl_rec::left))[lane] = __builtin_amdgcn_exp2f((float) (all - cum)) * (kinv / most);
+            if (lane == 0) ((float *) (rec + dl_rec::end))[0] = __builtin_amdgcn_exp2f((float) all), ((float *) (rec + dl_rec::end))[1] = most;
         }
         __syncthreads();
+        {
+            const int t = 16 * wave + l16, u = 16 * tk + l16;
+            const double ct = s_cum[t], cu = s_cum[u];
+            const float bu = s_beta[u];
+            dl_v4f v[4];
+            float most = 0.0f;
 #pragma unroll
-        for (int n = 0; n < 5; n++) {
-            const int i = wave + 4 * n, pr = i < 10 ? i : i - 10;
-            const int tb = pr < 1 ? 0 : pr < 3 ? 1 : pr < 6 ? 2 : 3, sb = pr - tb * (tb + 1) / 2;
-            const int t = 16 * tb + l16;
-            const double ct = s_cum[t];
-            const float f = i < 10 ? s_beta[t] : a.scale;
-            dl_v4f v;
+            for (int sb = 0; sb < 4; sb++) {
+                dl_v4f w;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int ss = 16 * sb + 4 * lg + e;
-                const bool in = i < 10 ? ss < t : ss <= t;
-                v[e] = in ? dots[n][e] * f * expf((float) (ct - s_cum[ss])) : 0.0f;
+                for (int e = 0; e < 4; e++) {
+                    const int ss = 16 * sb + 4 * lg + e;
+                    const double cs = s_cum[ss];
+                    v[sb][e] = ss <= t ? kq[sb][e] * a.scale * __builtin_amdgcn_exp2f((float) (ct - cs)) : 0.0f;
+                    w[e] = ss < u ? kk[sb][e] * bu * __builtin_amdgcn_exp2f((float) (cu - cs)) : 0.0f;
+                    most = fmaxf(most, fabsf(v[sb][e]));
+                }
+                if (sb <= tk) s_a[dl_pair(tk, sb)][lane] = w;
+                if (sb == tk) *(dl_v4f *) &s_d[tk][l16][4 * lg] = w;
             }
-            if (i < 10) {
-                s_a[pr][lane] = v;
-                if (tb == sb) *(dl_v4f *) &s_d[tb][l16][4 * lg] = v;
-            } else {
-                ((dl_v4f *) (rec + dl_rec::p))[pr * 64 + lane] = v;
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            const float sc = dl_pow2(13 - max(dl_exponent(most), -60));  // (Y is made in this scale: no larger one)
+            put_rows((dl_u4 *) (rec + dl_rec::p), v, sc);
+            if (lg == 0) {
+                ((float *) (rec + dl_rec::in))[t] = __builtin_amdgcn_exp2f((float) ct) * a.scale * (sc / s_qexp[t]);
+                ((float *) (rec + dl_rec::y))[t] = 1.0f / sc;
             }
         }
         __syncthreads();
@@ -348,187 +492,217 @@ __global__ __launch_bounds__(256) void k_delta_solve(dl_chunk_args q) {
             float x[16];
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                float v = i == l16 ? 1.0f : 0.0f;
+                dl_v4f v = {i == l16 ? 1.0f : 0.0f, 0, 0, 0};
 #pragma unroll
                 for (int j = 0; j < i; j += 4) {
                     const dl_v4f r = *(const dl_v4f *) &s_d[lg][i][j];
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        if (j + e < i) v = fmaf(-r[e], x[j + e], v);
+                        if (j + e < i) v[e] = fmaf(-r[e], x[j + e], v[e]);
                 }
-                x[i] = v;
+                x[i] = (v[0] + v[1]) + (v[2] + v[3]);
             }
 #pragma unroll
             for (int i = 0; i < 16; i++) s_d[lg][i][l16] = x[i];  // (every read of the block came before: one wave)
         }
         __syncthreads();
-        dl_v4f inv[4], off[6];
+        // T's columns of the wave's token block: x_b = inv_b (1 - A_b. x)
+        dl_v4f inv[4], off[6], x[4];
 #pragma unroll
-        for (int b = 0; b < 4; b++) inv[b] = *(const dl_v4f *) &s_d[b][l16][4 * lg];
+        for (int i = 0; i < 4; i++) inv[i] = *(const dl_v4f *) &s_d[i][l16][4 * lg];
 #pragma unroll
-        for (int b = 1; b < 4; b++)
+        for (int i = 1; i < 4; i++)
 #pragma unroll
-            for (int e = 0; e < b; e++) off[b * (b - 1) / 2 + e] = -s_a[dl_pair(b, e)][lane];
-        const char * vb = a.v + h * a.v_nb1 + t0 * a.v_nb2 + s * a.v_nb3;
-        for (int ct = wave; ct < q.vblocks + KB; ct += 4) {
-            const bool is_u = ct < q.vblocks;
-            const int col = 16 * (is_u ? ct : ct - q.vblocks) + l16;
-            dl_v4f x[4];
+            for (int e = 0; e < i; e++) off[i * (i - 1) / 2 + e] = -s_a[dl_pair(i, e)][lane];
+        __syncthreads();  // (s_t lies over s_a)
 #pragma unroll
-            for (int b = 0; b < 4; b++)
+        for (int i = 0; i < 4; i++) {
+            x[i] = dl_v4f{0, 0, 0, 0};
+            if (i < wave) continue;
+            dl_v4f r;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int t = 16 * b + 4 * lg + e;
-                    if (is_u) {
-                        const float v = t < nt && col < a.V ? ((const float *) (vb + t * a.v_nb2))[col] : 0.0f;
-                        x[b][e] = v * s_beta[t];
-                        own_bad |= dl_past(v, kDlU);
-                    } else {
-                        x[b][e] = -s_k[t][col] * s_beta[t] * expf((float) s_cum[t]);
-                    }
-                }
+            for (int e = 0; e < 4; e++) r[e] = i == wave && 4 * lg + e == l16 ? 1.0f : 0.0f;
 #pragma unroll
-            for (int b = 0; b < 4; b++) {
-                dl_v4f r = x[b];
+            for (int e = 0; e < i; e++)
+                if (e >= wave) r = dl_mfma(off[i * (i - 1) / 2 + e], x[e], r);
+            x[i] = dl_mfma(inv[i], r, dl_v4f{0, 0, 0, 0});
 #pragma unroll
-                for (int e = 0; e < b; e++) r = dl_mfma(off[b * (b - 1) / 2 + e], x[e], r);
-                x[b] = dl_mfma(inv[b], r, dl_v4f{0, 0, 0, 0});
-#pragma unroll
-                for (int e = 0; e < 4; e++) own_bad |= dl_past(x[b][e], is_u ? kDlU : kDlW);
-            }
-            if (is_u) {
-                dl_v4f * u = (dl_v4f *) (rec + dl_rec::w + 4 * kDlC * NP) + (int64_t) ct * 256 + lane;
-#pragma unroll
-                for (int b = 0; b < 4; b++) u[64 * b] = x[b];
-            } else {
-                float * w = (float *) (rec + dl_rec::w) + col;
-#pragma unroll
-                for (int b = 0; b < 4; b++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) w[(16 * b + 4 * lg + e) * NP] = x[b][e];
+            for (int e = 0; e < 4; e++) {
+                own_bad |= dl_past(x[i][e], kDlT);
+                s_t[16 * i + 4 * lg + e][16 * wave + l16] = x[i][e];
             }
         }
-        own_bad = __syncthreads_or(own_bad);  // (and LDS has been read)
-        if (tid == 0) *(int *) (rec + dl_rec::bad) = own_bad;
+        own_bad = __syncthreads_or(own_bad);
+        {
+            dl_v4f v[4];
+            float most = 0.0f;
+#pragma unroll
+            for (int sb = 0; sb < 4; sb++) {
+                v[sb] = dl_v4f{0, 0, 0, 0};
+                if (sb <= wave) v[sb] = *(const dl_v4f *) &s_t[16 * wave + l16][16 * sb + 4 * lg];
+#pragma unroll
+                for (int e = 0; e < 4; e++) most = fmaxf(most, fabsf(v[sb][e]));
+            }
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            const float sc = dl_pow2(13 - dl_exponent(most));
+            put_rows((dl_u4 *) (rec + dl_rec::t), v, sc);
+            if (lg == 0) ((float *) (rec + dl_rec::t_row))[16 * wave + l16] = 1.0f / sc;
+        }
+        if (tid == 0) ((int *) (rec + dl_rec::end))[2] = own_bad;
+        __syncthreads();  // (the next head's A lies over it)
     }
 }
 
-// Eight waves: the first four make D's token blocks, the others Y's, and wave w
-// holds the state's rows 16 w .. (and 16 (w + 8) .. for keys past 128) of the
-// workgroup's 16 columns.
-template <int NP>
+// Eight waves. Wave w < 4 makes the token block w's rows of K S0 and so of beta V
+// - beta e^a K S0, the others those of Q S0; all make D's (token block w % 4, for
+// a half of the columns where there are two), then wave w the state's rows 16 w
+// .. (and 16 (w + 8) .. for keys past 128), and the last four Y.
+template <int NP, int NC>
 __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
-    constexpr int KB = NP / 16, NS = (KB + 7) / 8;
-    __shared__ dl_v4f s_s[KB][64], s_dy[4][64], s_ds[4][64];  // S0, D, and D for the state, as B operands
+    constexpr int KB = NP / 16, KS = NP / 32, NS = (KB + 7) / 8;
+    __shared__ dl_u4 s_s[KS][2][NC][64], s_r[2][2][NC][64], s_d[2][2][NC][64], s_ds[2][2][NC][64];  // S0, T's operand, D, D for the state
     __shared__ float s_red[2][8][16];
-    __shared__ int s_large[2];
+    __shared__ uint32_t s_most[2];        // the largest |value| of the state and of v at a chunk's start (its bits)
+    __shared__ int s_past[2], s_late[2];  // a chunk whose S0, or whose D, leaves f16's range
     const delta_args & a = q.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lg = lane >> 4;
     // workgroups of one head on one XCD: they read the same records
     const int n_blk = (int) gridDim.x;
     int b = (int) blockIdx.x;
     if (n_blk % 8 == 0) b = (b % 8) * (n_blk / 8) + b / 8;
-    const int vb = b % q.vblocks, h = b / q.vblocks % a.heads, s = b / q.vblocks / a.heads, hk = h % a.key_heads;
-    const int col = 16 * vb + l16, tb = wave & 3;
-    const bool makes_d = wave < 4;
-    const char * rec0 = q.rec + ((int64_t) s * a.heads + h) * q.chunks * q.rec_size;
+    const int vb = b % q.cols, h = b / q.cols % a.heads, s = b / q.cols / a.heads, hk = h % a.key_heads;
+    const int col0 = 16 * NC * vb + l16, tb = wave & 3;
+    const bool keys = wave < 4;
+    const char * rec0 = q.rec + ((int64_t) s * a.heads + h) * q.chunks * dl_rec::size;
+    const char * krec0 = q.krec + ((int64_t) s * a.key_heads + hk) * q.chunks * dl_krec<NP>::size;
     const char * kp = a.k + hk * a.k_nb1 + s * a.k_nb3;
     const char * qp = a.q + hk * a.q_nb1 + s * a.q_nb3;
+    const char * vp = a.v + h * a.v_nb1 + s * a.v_nb3;
 
-    dl_v4f st[NS];  // rows 16 (w + 8 n) + 4 lg .., column l16
+    dl_v4f st[NS][NC];  // rows 16 (w + 8 n) + 4 lg .., column 16 cb + l16
 #pragma unroll
-    for (int n = 0; n < NS; n++) {
-        const int d = 16 * (wave + 8 * n) + 4 * lg;
-        st[n] = dl_v4f{0, 0, 0, 0};
-        if (col < a.V && d < a.K) st[n] = *(const dl_v4f *) (q.s_in + s * q.s_in_nb3 + 4 * (((int64_t) h * a.V + col) * a.K + d));
-    }
-    if (tid < 2) s_large[tid] = 0;
-    __syncthreads();
+    for (int n = 0; n < NS; n++)
+#pragma unroll
+        for (int cb = 0; cb < NC; cb++) {
+            const int d = 16 * (wave + 8 * n) + 4 * lg, col = col0 + 16 * cb;
+            st[n][cb] = dl_v4f{0, 0, 0, 0};
+            if (col < a.V && d < a.K) st[n][cb] = *(const dl_v4f *) (q.s_in + s * q.s_in_nb3 + 4 * (((int64_t) h * a.V + col) * a.K + d));
+        }
+    if (tid < 2) s_past[tid] = s_late[tid] = s_most[tid] = 0;
 
-    // a chunk's operands: rows of -W or of Q; K^T; U; lower(Q K^T L)
-    dl_v4f a1[KB], kt[NS][4], u, p[4], in, left;
-    float end;
+    // A chunk's operands. Each is loaded for the next chunk as soon as its
+    // registers are free (two sets would spill), and by all waves alike: a
+    // branch's loads would be waited for.
+    dl_split rows[KS], t[2], kt[NS][2], p[2];
+    dl_v4f f, beta, v[NC], t_row, left, y_row;
+    float end, left_most;
     int bad;
-    auto load_1 = [&](int64_t c) {
-        const char * rec = rec0 + c * q.rec_size;
-        const int64_t t0 = (q.c0 + c) * kDlC;
-        if (makes_d) {
-            const float * w = (const float *) (rec + dl_rec::w) + (16 * tb + l16) * NP + 4 * lg;
+    // (a lane's byte offsets in v, of its four tokens and its columns: 32 bits, the rest uniform)
+    uint32_t v_tok[4], v_col[NC];
 #pragma unroll
-            for (int k = 0; k < KB; k++) a1[k] = *(const dl_v4f *) (w + 16 * k);
-            u = ((const dl_v4f *) (rec + dl_rec::w + 4 * kDlC * NP))[(int64_t) vb * 256 + 64 * tb + lane];
-            left = *(const dl_v4f *) (rec + dl_rec::left + 4 * (16 * tb + 4 * lg));
-        } else {
-            const char * row = qp + min(t0 + 16 * tb + l16, a.tokens - 1) * a.q_nb2;
+    for (int cb = 0; cb < NC; cb++) v_col[cb] = 4u * (uint32_t) min(col0 + 16 * cb, a.V - 1);
+    auto v_tokens = [&](int last) {
 #pragma unroll
-            for (int k = 0; k < KB; k++) a1[k] = *(const dl_v4f *) (row + 4 * min(16 * k + 4 * lg, a.K - 4));
-            in = *(const dl_v4f *) (rec + dl_rec::in + 4 * (16 * tb + 4 * lg));
-        }
-        end = *(const float *) (rec + dl_rec::end);
-        bad = *(const int *) (rec + dl_rec::bad);
+        for (int e = 0; e < 4; e++) v_tok[e] = (uint32_t) min(16 * tb + 4 * lg + e, last) * (uint32_t) a.v_nb2;
     };
-    auto load_2 = [&](int64_t c) {
-        const char * rec = rec0 + c * q.rec_size;
+    v_tokens(kDlC - 1);
+    auto load_rows = [&](int64_t c) {
+        const char * rec = rec0 + c * dl_rec::size;
         const int64_t t0 = (q.c0 + c) * kDlC;
+        if (t0 + kDlC > a.tokens) v_tokens((int) (a.tokens - t0) - 1);
+        const dl_u4 * row = (const dl_u4 *) (krec0 + c * dl_krec<NP>::size + (keys ? dl_krec<NP>::k : dl_krec<NP>::q)) + tb * KS * 128 + lane;
 #pragma unroll
-        for (int n = 0; n < NS; n++) {
-            const int d = 16 * (wave + 8 * n) + l16;
+        for (int k = 0; k < KS; k++) rows[k].v[0] = row[128 * k], rows[k].v[1] = row[128 * k + 64];
+        const char * of_rows = rec + 4 * (16 * tb + 4 * lg);
+        f = *(const dl_v4f *) (of_rows + (keys ? dl_rec::ks : dl_rec::in));
+        beta = *(const dl_v4f *) (of_rows + dl_rec::beta);
+        const char * vt = vp + t0 * a.v_nb2;
 #pragma unroll
-            for (int sb = 0; sb < 4; sb++)
+        for (int cb = 0; cb < NC; cb++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float v = *(const float *) (kp + min(t0 + 16 * sb + 4 * lg + e, a.tokens - 1) * a.k_nb2 + 4 * min(d, a.K - 1));
-                    kt[n][sb][e] = d < a.K ? v : 0.0f;  // (rows past K stay zero)
-                }
-        }
-        if (!makes_d) {
-#pragma unroll
-            for (int sb = 0; sb < 4; sb++)
-                if (sb <= tb) p[sb] = ((const dl_v4f *) (rec + dl_rec::p))[dl_pair(tb, sb) * 64 + lane];
-        }
+            for (int e = 0; e < 4; e++) v[cb][e] = *(const float *) (vt + (v_tok[e] + v_col[cb]));
+        // (by vector loads: a wait for LDS would wait for scalar ones)
+        bad = ((const int *) (rec + dl_rec::end))[2 + (lane >> 6)];
     };
-    if (q.chunks > 0) {
-        load_1(0);
-        load_2(0);
-    }
-    for (int64_t c = 0; c < q.chunks; c++) {
-        const int64_t t0 = (q.c0 + c) * kDlC, more = min(c + 1, q.chunks - 1);
-        bool large = false;
+    auto load_t = [&](int64_t c) {
+        const char * rec = rec0 + c * dl_rec::size;
+        const dl_u4 * x = (const dl_u4 *) (rec + dl_rec::t) + tb * 256 + lane;
 #pragma unroll
-        for (int n = 0; n < NS; n++) {
-            if (wave + 8 * n < KB) s_s[wave + 8 * n][lane] = st[n];
+        for (int m = 0; m < 2; m++) t[m].v[0] = x[128 * min(m, tb / 2)], t[m].v[1] = x[128 * min(m, tb / 2) + 64];
+        t_row = *(const dl_v4f *) (rec + 4 * (16 * tb + 4 * lg) + dl_rec::t_row);
+        left = *(const dl_v4f *) (rec + 4 * (16 * tb + 4 * lg) + dl_rec::left);
+    };
+    auto load_kt = [&](int64_t c) {
+        const char * rec = rec0 + c * dl_rec::size;
+        const dl_u4 * k = (const dl_u4 *) (krec0 + c * dl_krec<NP>::size + dl_krec<NP>::kt) + lane;
 #pragma unroll
-            for (int e = 0; e < 4; e++) large |= dl_past(st[n][e], kDlU);
-        }
-        if (large) s_large[c & 1] = 1;
-        __syncthreads();
-        const bool by_token = bad || s_large[c & 1];
-        if (tid == 0) s_large[(c + 1) & 1] = 0;
-        if (by_token) {
-            const int nt = (int) min((int64_t) kDlC, a.tokens - t0);
-            for (int t = 0; t < nt; t++) {
-                const int64_t tt = t0 + t;
-                const float * k = (const float *) (kp + tt * a.k_nb2);
-                const float * qr = (const float *) (qp + tt * a.q_nb2);
-                auto length = [&](const float * x, float eps) {
-                    if (eps < 0.0f) return 1.0f;
-                    float sum = 0.0f;
-                    for (int i = lane; i < a.K; i += 64) sum = fmaf(x[i], x[i], sum);
-                    return 1.0f / fmaxf(sqrtf(wave_sum(sum)), eps);
-                };
-                const float kl = length(k, a.k_eps), ql = length(qr, a.q_eps) * a.scale;
-                const float eg = expf(*(const float *) (a.g + h * a.g_nb1 + tt * a.g_nb2 + s * a.g_nb3));
-                const float beta = *(const float *) (a.beta + h * a.b_nb1 + tt * a.b_nb2 + s * a.b_nb3);
-                const float v = col < a.V ? ((const float *) (a.v + h * a.v_nb1 + tt * a.v_nb2 + s * a.v_nb3))[col] : 0.0f;
-                float kv[NS][4], dot = 0.0f, y = 0.0f;
+        for (int n = 0; n < NS; n++)
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                const int at = 128 * (2 * min(wave + 8 * n, KB - 1) + m);
+                kt[n][m].v[0] = k[at], kt[n][m].v[1] = k[at + 64];
+            }
+        const dl_u4 * x = (const dl_u4 *) (rec + dl_rec::p) + tb * 256 + lane;
+#pragma unroll
+        for (int m = 0; m < 2; m++) p[m].v[0] = x[128 * min(m, tb / 2)], p[m].v[1] = x[128 * min(m, tb / 2) + 64];
+        y_row = *(const dl_v4f *) (rec + 4 * (16 * tb + 4 * lg) + dl_rec::y);
+        end = ((const float *) (rec + dl_rec::end))[lane >> 6];
+        left_most = ((const float *) (rec + dl_rec::end))[1 + (lane >> 6)];
+    };
+    // a result's four rows as the half of a lane's eight k
+    auto put = [&](dl_u4 (&to)[2][NC][64], int cb, int half, dl_v4f v) {
+        uint32_t x[2], y[2];
+        dl_split2(v[0], v[1], x[0], y[0]);
+        dl_split2(v[2], v[3], x[1], y[1]);
+        ((dl_u2 *) &to[0][cb][lane])[half] = dl_u2{x[0], x[1]};
+        ((dl_u2 *) &to[1][cb][lane])[half] = dl_u2{y[0], y[1]};
+    };
+    auto get = [&](const dl_u4 (&from)[2][NC][64], int cb) { return dl_split{{from[0][cb][lane], from[1][cb][lane]}}; };
+    // whether a scaled result might leave f16's range (or is not finite)
+    auto past = [](dl_v4f v) { return dl_past((fabsf(v[0]) + fabsf(v[1])) + (fabsf(v[2]) + fabsf(v[3])), kDlHalf); };
+    auto put_most = [&](int slot) {
+        float m = 0.0f;
+#pragma unroll
+        for (int cb = 0; cb < NC; cb++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                m = fmaxf(m, fabsf(v[cb][e]));
+#pragma unroll
+                for (int n = 0; n < NS; n++)
+                    if (wave + 8 * n < KB) m = fmaxf(m, fabsf(st[n][cb][e]));
+            }
+        m = dl_max16(m);
+        if (l16 == 0) atomicMax(&s_most[slot], __float_as_uint(m));
+    };
+    // token by token, for chunks the products cannot take
+    auto tokens = [&](int64_t t0) {
+        const int nt = (int) min((int64_t) kDlC, a.tokens - t0);
+        for (int t = 0; t < nt; t++) {
+            const int64_t tt = t0 + t;
+            const float * k = (const float *) (kp + tt * a.k_nb2);
+            const float * qr = (const float *) (qp + tt * a.q_nb2);
+            auto length = [&](const float * x, float eps) {
+                if (eps < 0.0f) return 1.0f;
+                float sum = 0.0f;
+                for (int i = lane; i < a.K; i += 64) sum = fmaf(x[i], x[i], sum);
+                return 1.0f / fmaxf(sqrtf(wave_sum(sum)), eps);
+            };
+            const float kl = length(k, a.k_eps), ql = length(qr, a.q_eps) * a.scale;
+            const float eg = expf(*(const float *) (a.g + h * a.g_nb1 + tt * a.g_nb2 + s * a.g_nb3));
+            const float bt = *(const float *) (a.beta + h * a.b_nb1 + tt * a.b_nb2 + s * a.b_nb3);
+#pragma unroll
+            for (int cb = 0; cb < NC; cb++) {
+                const int col = col0 + 16 * cb;
+                const float vt = col < a.V ? ((const float *) (vp + tt * a.v_nb2))[col] : 0.0f;
+                float dot = 0.0f, y = 0.0f;
 #pragma unroll
                 for (int n = 0; n < NS; n++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const int d = 16 * (wave + 8 * n) + 4 * lg + e;
-                        kv[n][e] = d < a.K ? k[d] * kl : 0.0f;
-                        st[n][e] = d < a.K ? st[n][e] * eg : 0.0f;
-                        if (d < a.K) dot = fmaf(st[n][e], kv[n][e], dot);
+                        st[n][cb][e] = d < a.K ? st[n][cb][e] * eg : 0.0f;
+                        if (d < a.K) dot = fmaf(st[n][cb][e], k[d] * kl, dot);
                     }
                 dot += __shfl_xor(dot, 16);
                 dot += __shfl_xor(dot, 32);
@@ -537,15 +711,15 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
                 dot = 0.0f;
 #pragma unroll
                 for (int w = 0; w < 8; w++) dot += s_red[0][w][l16];
-                const float d = beta * (v - dot);
+                const float d = bt * (vt - dot);
 #pragma unroll
                 for (int n = 0; n < NS; n++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const int i = 16 * (wave + 8 * n) + 4 * lg + e;
                         if (i < a.K) {
-                            st[n][e] = fmaf(kv[n][e], d, st[n][e]);
-                            y = fmaf(st[n][e], qr[i] * ql, y);
+                            st[n][cb][e] = fmaf(k[i] * kl, d, st[n][cb][e]);
+                            y = fmaf(st[n][cb][e], qr[i] * ql, y);
                         }
                     }
                 y += __shfl_xor(y, 16);
@@ -558,47 +732,166 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
                     for (int w = 0; w < 8; w++) y += s_red[1][w][l16];
                     a.y[((s * a.tokens + tt) * a.heads + h) * a.V + col] = y;
                 }
+                __syncthreads();
             }
-            load_1(more);
-            load_2(more);
-            __syncthreads();
-            continue;
         }
-        dl_v4f acc = makes_d ? u : dl_v4f{0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < KB; k++) acc = dl_mfma(a1[k], s_s[k][lane], acc);
-        if (makes_d) {
-            s_dy[tb][lane] = acc;
-            s_ds[tb][lane] = acc * left;
-        } else {
-            acc *= in;
-        }
-        const float e_end = end;
-        load_1(more);
-        __syncthreads();
+    };
+    if (q.chunks > 0) load_rows(0), load_t(0), load_kt(0);
+    __syncthreads();
+    put_most(1);
+    __syncthreads();
+    int size = dl_exponent(__uint_as_float(s_most[1]));  // log2 of the largest of the state and v, a chunk before
+    for (int64_t c = 0; c < q.chunks; c++) {
+        const int64_t t0 = (q.c0 + c) * kDlC, more = min(c + 1, q.chunks - 1);
+        bool large = false;
 #pragma unroll
         for (int n = 0; n < NS; n++) {
-            st[n] *= e_end;
+            const int kb = wave + 8 * n;
+            if (kb < KB) {
 #pragma unroll
-            for (int sb = 0; sb < 4; sb++) st[n] = dl_mfma(kt[n][sb], s_ds[sb][lane], st[n]);
-        }
-        if (!makes_d) {
-#pragma unroll
-            for (int sb = 0; sb < 4; sb++)
-                if (sb <= tb) acc = dl_mfma(p[sb], s_dy[sb][lane], acc);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int64_t t = t0 + 16 * tb + 4 * lg + e;
-                if (t < a.tokens && col < a.V) a.y[((s * a.tokens + t) * a.heads + h) * a.V + col] = acc[e];
+                for (int cb = 0; cb < NC; cb++) {
+                    const dl_v4f x = st[n][cb] * dl_pow2(5 - size);
+                    put(s_s[kb >> 1], cb, kb & 1, x);
+                    large |= past(x);
+                }
             }
         }
-        load_2(more);
+        if (large || size > 40) s_past[c & 1] = 1;
+        __syncthreads();
+        const bool by_token = __builtin_amdgcn_readfirstlane(bad) || s_past[c & 1];
+        if (tid == 0) s_past[(c + 1) & 1] = s_late[(c + 1) & 1] = s_most[(c + 1) & 1] = 0;
+        dl_v4f acc[NC];
+        if (by_token) goto one_by_one;
+#pragma unroll
+        for (int cb = 0; cb < NC; cb++) acc[cb] = dl_v4f{0, 0, 0, 0};
+        {
+            // (the reads of LDS ahead of the products, half of them where there are many)
+            constexpr int kReads = KS > 4 ? KS / 2 : KS;
+#pragma unroll
+            for (int k0 = 0; k0 < KS; k0 += kReads) {
+                dl_split x[kReads][NC];
+#pragma unroll
+                for (int k = 0; k < kReads; k++)
+#pragma unroll
+                    for (int cb = 0; cb < NC; cb++) x[k][cb] = get(s_s[k0 + k], cb);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 0; k < kReads; k++)
+#pragma unroll
+                    for (int i = 0; i < 3; i++)
+#pragma unroll
+                        for (int cb = 0; cb < NC; cb++) acc[cb] = dl_product(i, rows[k0 + k], x[k][cb], acc[cb]);
+            }
+        }
+        put_most(c & 1);
+#pragma unroll
+        for (int cb = 0; cb < NC; cb++) {
+            acc[cb] *= f * dl_pow2(size - 5);
+            if (keys) {
+                const dl_v4f x = (v[cb] * beta - acc[cb]) * dl_pow2(8 - size);
+                put(s_r[tb >> 1], cb, tb & 1, x);
+                large |= past(x);
+            }
+        }
+        if (large) s_late[c & 1] = 1;
+        load_rows(more);
+        __syncthreads();
+        {
+            // D: a token block, half of the columns (one column block: the first waves)
+            const int half = NC == 2 ? wave >> 2 : 0, now = dl_exponent(__uint_as_float(s_most[c & 1]));
+            if (NC == 2 || keys) {
+                dl_v4f d = {0, 0, 0, 0};
+#pragma unroll
+                for (int m = 0; m < 2; m++) {
+                    if (2 * m > tb) continue;
+                    const dl_split x = get(s_r[m], half);
+#pragma unroll
+                    for (int i = 0; i < 3; i++) d = dl_product(i, t[m], x, d);
+                }
+                d *= t_row * dl_pow2(size - 8);
+                d *= dl_pow2(6 - now);
+                put(s_d[tb >> 1], half, tb & 1, d);
+                put(s_ds[tb >> 1], half, tb & 1, d * left);
+                if (past(d)) s_late[c & 1] = 1;
+            }
+            size = now;
+        }
+        load_t(more);
+        __syncthreads();
+        if (s_late[c & 1]) goto one_by_one;
+        {
+            // the state in D's scale, and back
+            const float in = end * dl_pow2(6 - size) / left_most, out = left_most * dl_pow2(size - 6);
+            dl_split x[2][NC];
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int cb = 0; cb < NC; cb++) x[m][cb] = get(s_ds[m], cb);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int n = 0; n < NS; n++) {
+#pragma unroll
+                for (int cb = 0; cb < NC; cb++) st[n][cb] *= in;
+#pragma unroll
+                for (int m = 0; m < 2; m++) {
+#pragma unroll
+                    for (int i = 0; i < 3; i++)
+#pragma unroll
+                        for (int cb = 0; cb < NC; cb++) st[n][cb] = dl_product(i, kt[n][m], x[m][cb], st[n][cb]);
+                }
+#pragma unroll
+                for (int cb = 0; cb < NC; cb++) st[n][cb] *= out;
+            }
+            if (!keys) {
+#pragma unroll
+                for (int cb = 0; cb < NC; cb++) acc[cb] *= dl_pow2(6 - size);
+#pragma unroll
+                for (int m = 0; m < 2; m++) {
+                    if (2 * m > tb) continue;
+                    dl_split x[NC];
+#pragma unroll
+                    for (int cb = 0; cb < NC; cb++) x[cb] = get(s_d[m], cb);
+#pragma unroll
+                    for (int i = 0; i < 3; i++)
+#pragma unroll
+                        for (int cb = 0; cb < NC; cb++) acc[cb] = dl_product(i, p[m], x[cb], acc[cb]);
+                }
+                const dl_v4f back = y_row * dl_pow2(size - 6);
+                char * y = (char *) (a.y + ((s * a.tokens + t0) * a.heads + h) * a.V);
+                const uint32_t y_nb = 4u * (uint32_t) a.heads * (uint32_t) a.V, at = (uint32_t) (16 * tb + 4 * lg) * y_nb + 4u * (uint32_t) col0;
+                const int left_over = (int) min((int64_t) kDlC, a.tokens - t0) - 16 * tb - 4 * lg;
+#pragma unroll
+                for (int cb = 0; cb < NC; cb++) {
+                    if (col0 + 16 * cb >= a.V) continue;
+                    if (left_over >= 4) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) *(float *) (y + (int64_t) e * y_nb + (at + 64 * cb)) = acc[cb][e] * back[e];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 3; e++)
+                            if (e < left_over) *(float *) (y + (int64_t) e * y_nb + (at + 64 * cb)) = acc[cb][e] * back[e];
+                    }
+                }
+            }
+            load_kt(more);
+            continue;
+        }
+    one_by_one:
+        tokens(t0);
+        load_rows(more), load_t(more), load_kt(more);
+        if (tid == 0) s_most[c & 1] = 0;
+        __syncthreads();
+        put_most(c & 1);
+        __syncthreads();
+        size = dl_exponent(__uint_as_float(s_most[c & 1]));
     }
 #pragma unroll
-    for (int n = 0; n < NS; n++) {
-        const int d = 16 * (wave + 8 * n) + 4 * lg;
-        if (col < a.V && d < a.K) *(dl_v4f *) (a.out + s * a.out_nb3 + 4 * (((int64_t) h * a.V + col) * a.K + d)) = st[n];
-    }
+    for (int n = 0; n < NS; n++)
+#pragma unroll
+        for (int cb = 0; cb < NC; cb++) {
+            const int d = 16 * (wave + 8 * n) + 4 * lg, col = col0 + 16 * cb;
+            if (col < a.V && d < a.K) *(dl_v4f *) (a.out + s * a.out_nb3 + 4 * (((int64_t) h * a.V + col) * a.K + d)) = st[n][cb];
+        }
 }
 
 // ------------------------------------------------------------- launches ---
@@ -606,14 +899,16 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
 bool delta_supported(int64_t K) { return K >= 1 && K <= 256; }
 
 static int dl_np(const delta_args & a) { return a.K <= 64 ? 64 : a.K <= 96 ? 96 : a.K <= 128 ? 128 : 256; }
-static int64_t dl_rec_size(const delta_args & a) {
-    return dl_rec::w + 4 * kDlC * (int64_t) dl_np(a) + 4 * kDlC * 16 * (int64_t) ((a.V + 15) / 16);
+// of the records of one chunk of all heads
+static int64_t dl_chunk_size(const delta_args & a) {
+    return ((int64_t) dl_rec::size * a.heads + 12 * kDlC * (int64_t) dl_np(a) * a.key_heads) * a.seqs;
 }
-// chunks of one slab: the records of more would not stay in the caches
-constexpr int64_t kDlSlab = 40 << 20;
+// Chunks of one slab, whose records lie in scratch: the two launches take turns.
+// 4096 tokens of 32 heads of 128 x 128 (2.7 MB a chunk), us a call by MB of
+// scratch: 40 333, 60 301, 90 286, 200 285.
 static int64_t dl_slab(const delta_args & a) {
-    const int64_t chunks = (a.tokens + kDlC - 1) / kDlC, one = dl_rec_size(a) * a.heads * a.seqs;
-    const int64_t fit = std::max<int64_t>(1, kDlSlab / one), slabs = (chunks + fit - 1) / fit;
+    const int64_t chunks = (a.tokens + kDlC - 1) / kDlC, one = dl_chunk_size(a);
+    const int64_t fit = std::max<int64_t>(1, a.scratch_bytes / one), slabs = (chunks + fit - 1) / fit;
     return (chunks + slabs - 1) / slabs;
 }
 static bool dl_vec(const delta_args & a) {
@@ -624,29 +919,37 @@ static bool dl_vec(const delta_args & a) {
     return al % 16 == 0;
 }
 // chunks: a gate a head, and tokens enough for the products to pay
-static bool dl_chunked(const delta_args & a) { return !a.g_elem && a.tokens >= 24 && a.K >= 16 && dl_vec(a); }
+static bool dl_chunked(const delta_args & a) {
+    return !a.g_elem && a.tokens >= 24 && a.K >= 16 && dl_vec(a) &&
+           a.v_nb2 >= 0 && a.v_nb2 < 1 << 25 && (int64_t) a.heads * a.V < 1 << 23;  // (a lane's rows of v and y in 32-bit offsets)
+}
 
 size_t delta_scratch_bytes(const delta_args & a, int n_cu) {
     (void) n_cu;
     // (a graph planned before it is allocated: the addresses may still allow chunks)
     if (a.g_elem || a.tokens < 24 || a.K < 16) return 0;
-    return (size_t) (dl_slab(a) * dl_rec_size(a) * a.heads * a.seqs);
+    return (size_t) (dl_slab(a) * dl_chunk_size(a));
 }
 
 template <int NP>
-static void launch_delta_chunks(const delta_args & a, void * scratch, hipStream_t s) {
+static void launch_delta_chunks(const delta_args & a, void * scratch, hipStream_t s, int n_cu) {
     dl_chunk_args q{};
     q.a = a;
     q.rec = (char *) scratch;
-    q.rec_size = (int) dl_rec_size(a);
-    q.vblocks = (a.V + 15) / 16;
+    // 32 columns a workgroup halve what is read of the records, but a chunk takes
+    // longer (3.9 us, of 16 columns 3.3): where these fill the CUs
+    const bool wide = (int64_t) ((a.V + 31) / 32) * a.heads * a.seqs >= n_cu;
+    q.cols = wide ? (a.V + 31) / 32 : (a.V + 15) / 16;
     q.s_in = a.s, q.s_in_nb3 = a.s_nb3;
     const int64_t chunks = (a.tokens + kDlC - 1) / kDlC, slab = dl_slab(a);
+    q.krec = q.rec + slab * dl_rec::size * a.heads * a.seqs;
     for (q.c0 = 0; q.c0 < chunks; q.c0 += slab) {
         q.chunks = std::min(slab, chunks - q.c0);
         hipLaunchKernelGGL(k_delta_solve<NP>, dim3((unsigned) (q.chunks * a.key_heads * a.seqs)), dim3(256), 0, s, q);
         note_hip_error(hipGetLastError());
-        hipLaunchKernelGGL(k_delta_chunks<NP>, dim3((unsigned) ((int64_t) q.vblocks * a.heads * a.seqs)), dim3(512), 0, s, q);
+        const dim3 grid((unsigned) ((int64_t) q.cols * a.heads * a.seqs));
+        if (wide) hipLaunchKernelGGL((k_delta_chunks<NP, 2>), grid, dim3(512), 0, s, q);
+        else hipLaunchKernelGGL((k_delta_chunks<NP, 1>), grid, dim3(512), 0, s, q);
         note_hip_error(hipGetLastError());
         q.s_in = a.out, q.s_in_nb3 = a.out_nb3;
     }
@@ -667,14 +970,13 @@ static void launch_delta_rows(const delta_args & a, bool vec, hipStream_t s) {
 }
 
 void launch_delta(const delta_args & a, void * scratch, hipStream_t s, int n_cu) {
-    (void) n_cu;
     if (a.seqs == 0 || a.heads == 0 || a.V == 0) return;
     if (dl_chunked(a)) {
         switch (dl_np(a)) {
-            case 64: launch_delta_chunks<64>(a, scratch, s); break;
-            case 96: launch_delta_chunks<96>(a, scratch, s); break;
-            case 128: launch_delta_chunks<128>(a, scratch, s); break;
-            default: launch_delta_chunks<256>(a, scratch, s); break;
+            case 64: launch_delta_chunks<64>(a, scratch, s, n_cu); break;
+            case 96: launch_delta_chunks<96>(a, scratch, s, n_cu); break;
+            case 128: launch_delta_chunks<128>(a, scratch, s, n_cu); break;
+            default: launch_delta_chunks<256>(a, scratch, s, n_cu); break;
         }
         return;
     }

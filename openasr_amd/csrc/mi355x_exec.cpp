@@ -2382,6 +2382,7 @@ bool planner::plan_delta(int i, const ggml_tensor * t) {
         a.out = (char *) c->data;
         writes.push_back(c);
     }
+    a.scratch_bytes = be->scratch_limit ? std::min<int64_t>(kDeltaScratch, (int64_t) be->scratch_limit / 2) : kDeltaScratch;
     gen_need = std::max(gen_need, delta_scratch_bytes(a, n_cu));
     backend_state * be_ = be;
     const int ncu = n_cu;
@@ -3028,7 +3029,9 @@ enum ggml_status graph_compute_in(backend_state * be, ggml_cgraph * cg, char * s
     MI_CHECK(hipSetDevice(be->dev->hip_id));
     flush_uploads(be->dev, be->stream, false);  // queued input writes land ahead of the graph
     bool planned;
+    be->scratch_limit = cap;
     auto pp = make_plan(be, cg, planned);
+    be->scratch_limit = 0;
     planner & p = *pp;
     if (!planned) {
         std::fprintf(stderr, "mi355x: cannot plan graph: %s\n", p.error.c_str());

@@ -138,6 +138,7 @@ struct backend_state {
     bool fail_next_launch = false;     // test seam: the next compute's first launch is refused
     char * scratch_override = nullptr; // while graph_compute_in runs: the caller's scratch
     size_t override_gen_off = 0;       // offset of its general region
+    size_t scratch_limit = 0;          // while graph_compute_in plans: its size (0: none)
     ggml_guid guid{};
     ggml_backend backend{};
     std::string name;

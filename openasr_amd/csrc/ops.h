@@ -451,7 +451,9 @@ struct delta_args {
     int64_t tokens;
     int K, V, heads, key_heads, seqs, g_elem;
     float q_eps, k_eps, scale;
+    int64_t scratch_bytes;  // what it may take of scratch (a chunk of all heads at least)
 };
+constexpr int64_t kDeltaScratch = 96 << 20;
 bool delta_supported(int64_t K);
 size_t delta_scratch_bytes(const delta_args & a, int n_cu);
 void launch_delta(const delta_args & a, void * scratch, hipStream_t s, int n_cu);
