@@ -52,6 +52,13 @@ __device__ __forceinline__ float dl_sum16(float v) {
     return v;
 }
 
+// e^x: the product's rounding error put back, so within an ulp or two at any x
+__device__ __forceinline__ float dl_exp(float x) {
+    const float z = x * 1.4426950408889634f, r = fmaf(x, 1.4426950408889634f, -z) + x * 1.925963e-8f;
+    const float p = __builtin_amdgcn_exp2f(z);
+    return x > -200.0f ? fmaf(p, r * 0.6931471805599453f, p) : p;  // (no infinity less itself)
+}
+
 __device__ __forceinline__ float dl_max16(float v) {  // of values from zero on
     auto most = [&](auto ctrl) {
         v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, true)));
@@ -115,14 +122,18 @@ __global__ __launch_bounds__(256) void k_delta_rows(delta_args a) {
 #pragma unroll
         for (int p = 0; p < P; p++) st[u][p] = piece(row, p);
     }
-    auto length = [&](const dl_v4f (&x)[P], float eps) {  // what a row is multiplied by
-        if (eps < 0.0f) return 1.0f;
-        float sum = 0.0f;
+    // what a row is multiplied by: 1 / max(its length, eps)
+    const float k_most = 1.0f / a.k_eps, q_most = 1.0f / a.q_eps;
+    auto dot = [](const dl_v4f (&x)[P], const dl_v4f (&y)[P]) {
+        dl_v4f v = x[0] * y[0];
 #pragma unroll
-        for (int p = 0; p < P; p++)
+        for (int p = 1; p < P; p++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) sum = fmaf(x[p][e], x[p][e], sum);
-        return 1.0f / fmaxf(sqrtf(dl_sum16(sum)), eps);
+            for (int e = 0; e < 4; e++) v[e] = fmaf(x[p][e], y[p][e], v[e]);
+        return (v[0] + v[1]) + (v[2] + v[3]);
+    };
+    auto length = [&](const dl_v4f (&x)[P], float eps, float most) {
+        return eps < 0.0f ? 1.0f : fminf(__builtin_amdgcn_rsqf(dl_sum16(dot(x, x))), most);
     };
     for (int64_t t0 = 0; t0 < a.tokens; t0 += AHEAD) {
 #pragma unroll
@@ -131,40 +142,33 @@ __global__ __launch_bounds__(256) void k_delta_rows(delta_args a) {
             if (t >= a.tokens) break;
             token x = next[n];
             if (t + AHEAD < a.tokens) load(t + AHEAD, next[n]);
-            const float kl = length(x.k, a.k_eps), ql = length(x.q, a.q_eps) * a.scale;
+            const float kl = length(x.k, a.k_eps, k_most), ql = length(x.q, a.q_eps, q_most) * a.scale;
             dl_v4f eg[ELEM ? P : 1];
-#pragma unroll
-            for (int p = 0; p < P; p++) {
-                x.k[p] *= kl, x.q[p] *= ql;
-                if constexpr (ELEM) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) eg[p][e] = expf(x.g[p][e]);
-                }
-            }
-            if constexpr (!ELEM) {
-                const float d = expf(x.g[0][0]);
-                eg[0] = dl_v4f{d, d, d, d};
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                float dot = 0.0f, y = 0.0f;
-#pragma unroll
-                for (int p = 0; p < P; p++) {
-                    st[u][p] *= eg[ELEM ? p : 0];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) dot = fmaf(st[u][p][e], x.k[p][e], dot);
-                }
-                const float d = x.beta * (x.v[u] - dl_sum16(dot));
+            if constexpr (ELEM) {
 #pragma unroll
                 for (int p = 0; p < P; p++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        st[u][p][e] = fmaf(x.k[p][e], d, st[u][p][e]);
-                        y = fmaf(st[u][p][e], x.q[p][e], y);
-                    }
-                y = dl_sum16(y);
-                if (l == 0 && j0 + 4 * u < a.V) a.y[((s * a.tokens + t) * a.heads + h) * a.V + j0 + 4 * u] = y;
+                    for (int e = 0; e < 4; e++) eg[p][e] = dl_exp(x.g[p][e]);
+            } else {
+                const float d = dl_exp(x.g[0][0]);
+                eg[0] = dl_v4f{d, d, d, d};
             }
+            float y[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+#pragma unroll
+                for (int p = 0; p < P; p++) st[u][p] *= eg[ELEM ? p : 0];
+                const float d = x.beta * (x.v[u] - kl * dl_sum16(dot(st[u], x.k))) * kl;
+#pragma unroll
+                for (int p = 0; p < P; p++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) st[u][p][e] = fmaf(x.k[p][e], d, st[u][p][e]);
+                y[u] = ql * dl_sum16(dot(st[u], x.q));
+            }
+            float * to = a.y + ((s * a.tokens + t) * a.heads + h) * a.V + j0;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (l == 0 && j0 + 4 * u < a.V) to[4 * u] = y[u];
         }
     }
 #pragma unroll
@@ -955,18 +959,30 @@ static void launch_delta_chunks(const delta_args & a, void * scratch, hipStream_
     }
 }
 
-template <int P, int U, int AHEAD>
-static void launch_delta_rows(const delta_args & a, bool vec, hipStream_t s) {
+template <int P, int U, int AHEAD, bool VEC>
+static void launch_delta_rows(const delta_args & a, hipStream_t s) {
     const int64_t units = (int64_t) ((a.V + 4 * U - 1) / (4 * U)) * a.heads * a.seqs;
     const dim3 grid((unsigned) ((units + 3) / 4));
-    if (a.g_elem) {
-        if (vec) hipLaunchKernelGGL((k_delta_rows<P, U, AHEAD, true, true>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_delta_rows<P, U, AHEAD, false, true>), grid, dim3(256), 0, s, a);
-    } else {
-        if (vec) hipLaunchKernelGGL((k_delta_rows<P, U, AHEAD, true, false>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_delta_rows<P, U, AHEAD, false, false>), grid, dim3(256), 0, s, a);
-    }
+    if (a.g_elem) hipLaunchKernelGGL((k_delta_rows<P, U, AHEAD, VEC, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_delta_rows<P, U, AHEAD, VEC, false>), grid, dim3(256), 0, s, a);
     note_hip_error(hipGetLastError());
+}
+
+// A wave takes 4 U rows: few where that leaves waves a SIMD, many where there
+// are enough anyhow (the token's work beside the rows is shared). 32 heads of 128
+// x 128, us, U = 1 / 2 / 4: 8 tokens of one sequence 7.9 / 8.7 / 11.5, of 16 37 /
+// 30 / 30; one token of 48 34 / 35 / 34; 500 tokens with gates an element, 16
+// heads of one sequence 365 / 384 / 511, of four 462 / 385 / 505. Four tokens'
+// operands ahead instead of one's take 342 of the 365 us, and more where tokens
+// are few (one token of 48 sequences: 64 for 34 us).
+template <int P>
+static void launch_delta_tokens(const delta_args & a, hipStream_t s, int n_cu) {
+    const int64_t rows = (int64_t) a.V * a.heads * a.seqs, enough = 16 * (int64_t) n_cu;  // four waves a CU, of 4 rows
+    if (!dl_vec(a)) launch_delta_rows<P, 2, 1, false>(a, s);
+    else if (rows >= 4 * enough) launch_delta_rows<P, 4, 1, true>(a, s);
+    else if (rows >= 2 * enough) launch_delta_rows<P, 2, 1, true>(a, s);
+    else if (a.tokens < 32) launch_delta_rows<P, 1, 1, true>(a, s);
+    else launch_delta_rows<P, 1, 4, true>(a, s);
 }
 
 void launch_delta(const delta_args & a, void * scratch, hipStream_t s, int n_cu) {
@@ -980,10 +996,9 @@ void launch_delta(const delta_args & a, void * scratch, hipStream_t s, int n_cu)
         }
         return;
     }
-    const bool vec = dl_vec(a);
-    if (a.K <= 64) launch_delta_rows<1, 2, 2>(a, vec, s);
-    else if (a.K <= 128) launch_delta_rows<2, 2, 2>(a, vec, s);
-    else launch_delta_rows<4, 2, 2>(a, vec, s);
+    if (a.K <= 64) launch_delta_tokens<1>(a, s, n_cu);
+    else if (a.K <= 128) launch_delta_tokens<2>(a, s, n_cu);
+    else launch_delta_tokens<4>(a, s, n_cu);
 }
 
 }  // namespace mi355x

@@ -29,6 +29,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "../fattn_scored_dev.h"
 #include "../mi355x_common.h"
 #include "../ops.h"
 
@@ -38,20 +39,12 @@ namespace {
 
 constexpr int kFsTile = 64;
 constexpr int kFsThreads = 256;
-constexpr float kFsLog2e = 1.4426950408889634f;
-constexpr uint32_t kFsNegInf = 0xFC00u;
 // p is scaled by 2^12: its low half stays a normal f16 down to 2^-15 of the maximum
 constexpr float kFsUp = 12.0f;
-// tanh(x) / x as a polynomial of x^2 up to |x| = 0.625, interpolated at
-// Chebyshev nodes: 4e-9 off
-constexpr float kFsPolyEnd = 0.625f;
-constexpr double kFsPoly[6] = {0.9999999960227207,   -0.3333325986294283,  0.13331114055632276,
-                               -0.05372010765402796, 0.02058819145009359, -0.005657135182291668};
 
 typedef _Float16 fs_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 fs_h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 fs_h2 __attribute__((ext_vector_type(2)));
-typedef float fs_f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t fs_u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t fs_u2 __attribute__((ext_vector_type(2)));
 
@@ -61,14 +54,10 @@ enum : uint8_t { kFsClosed = 0, kFsPlain = 1, kFsAdds = 2, kFsMixed = 3 };
 
 struct fs_args {
     fattn_args a;
-    float poly[6];    // tanh(x) / x times cap log2(e), of x = s / cap
-    float in;         // what a product is multiplied by: scale / cap, or scale log2(e)
-    float cap2;       // cap log2(e)
+    fs_score score;
     int g, qpw;       // query heads a kv head, queries a workgroup
     int q_blocks, n_tiles, split, per;
     int heads_mask;   // the mask differs by head: rows of it by query and head
-    double m0, m1;    // the slopes' bases (log2)
-    int n_low;
     uint64_t * seen;  // [mask sequence][kv head or one][query block][tile]
     uint8_t * cls;
     float * part;
@@ -154,17 +143,6 @@ __device__ __forceinline__ fs_f4 fs_mfma(fs_h8 a, fs_h8 b, fs_f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// cap tanh(x), times log2(e), for any x: 1 - 2 / (e^2x + 1), from the polynomial where that cancels
-__device__ __forceinline__ float fs_cap_any(const fs_args & f, float x) {
-    const float y = x * x;
-    float p = f.poly[5];
-#pragma unroll
-    for (int k = 4; k >= 0; k--) p = fmaf(p, y, f.poly[k]);
-    const float e = __builtin_amdgcn_exp2f(2.0f * kFsLog2e * fabsf(x));  // +inf from |x| = 45 on: the quotient is 0
-    const float t = copysignf(fmaf(-2.0f * f.cap2, __builtin_amdgcn_rcpf(e + 1.0f), f.cap2), x);
-    return fabsf(x) < kFsPolyEnd ? x * p : t;
-}
-
 // MM: 0 no mask, 1 rows of 16-byte pieces, 2 other rows
 template <int D, int RW, bool CAP, int MM>
 __global__ __launch_bounds__(kFsThreads, D == 256 ? 1 : 2) void k_fattn_scored(fs_args f) {
@@ -247,8 +225,7 @@ __global__ __launch_bounds__(kFsThreads, D == 256 ? 1 : 2) void k_fattn_scored(f
         for (int kk = 0; kk < KS; kk++)
 #pragma unroll
             for (int j = 0; j < 8; j++) qa[w][kk][j] = (_Float16) ((const float *) qp)[32 * kk + 8 * lg + j];
-        slope[w] = kFsLog2e;
-        if (a.max_bias > 0.0f) slope[w] = (float) (exp2(head < f.n_low ? f.m0 * (head + 1) : f.m1 * (2 * (head - f.n_low) + 1)) * 1.4426950408889634074);
+        slope[w] = fs_slope(f.score, a.max_bias, head);
         mrow[w] = f.heads_mask ? min(ql * f.g + r % f.g, mrows - 1) : ql;
     }
     if (tid == 0) s_bad = 0;
@@ -335,28 +312,22 @@ __global__ __launch_bounds__(kFsThreads, D == 256 ? 1 : 2) void k_fattn_scored(f
                 for (int t = 0; t < 4; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(sc[w][t][i]));
-                if (__any(!(most * f.in < kFsPolyEnd))) {
+                if (__any(!(most * f.score.in < kFsPolyEnd))) {
 #pragma unroll
                     for (int t = 0; t < 4; t++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) z[t][i] = fs_cap_any(f, sc[w][t][i] * f.in);
+                        for (int i = 0; i < 4; i++) z[t][i] = fs_cap_any(f.score, sc[w][t][i] * f.score.in);
                 } else {
 #pragma unroll
                     for (int t = 0; t < 4; t++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float x = sc[w][t][i] * f.in, y = x * x;
-                            float p = f.poly[5];
-#pragma unroll
-                            for (int k = 4; k >= 0; k--) p = fmaf(p, y, f.poly[k]);
-                            z[t][i] = x * p;
-                        }
+                        for (int i = 0; i < 4; i++) z[t][i] = fs_cap_small(f.score, sc[w][t][i] * f.score.in);
                 }
             } else {
 #pragma unroll
                 for (int t = 0; t < 4; t++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) z[t][i] = sc[w][t][i] * f.in;
+                    for (int i = 0; i < 4; i++) z[t][i] = sc[w][t][i] * f.score.in;
             }
             if constexpr (MM != 0) {
                 if (cls >= kFsAdds) {
@@ -475,32 +446,69 @@ __global__ __launch_bounds__(kFsThreads, D == 256 ? 1 : 2) void k_fattn_scored(f
     }
 }
 
-// a row's splits joined: a thread four dims of it
-template <int D>
-__global__ __launch_bounds__(256) void k_fattn_join(fs_args f, int R) {
-    const fattn_args & a = f.a;
-    const int64_t e = (int64_t) blockIdx.x * 256 + threadIdx.x;
-    const int d = (int) (e % (D / 4)) * 4;
-    const int64_t row = e / (D / 4);  // of (sequence, query, head)
-    if (row >= (int64_t) a.n_seq * a.n_q * a.hq) return;
-    const int head = (int) (row % a.hq), q = (int) (row / a.hq % a.n_q), seq = (int) (row / ((int64_t) a.hq * a.n_q));
-    const int qb = q / f.qpw, r = (q % f.qpw) * f.g + head % f.g;
-    const int64_t blk = ((int64_t) seq * a.hkv + head / f.g) * f.q_blocks + qb;
-    const int64_t rows = (int64_t) a.n_seq * a.hkv * f.q_blocks * f.split * R;
-    float M = -INFINITY;
-    for (int z = 0; z < f.split; z++) M = fmaxf(M, f.part[rows * D + 2 * ((blk * f.split + z) * R + r)]);
+// A row's splits joined: LN lanes of D / 4 threads take every LN-th split, a
+// thread four dims, their sums added through LDS. (A lane a row went through 78
+// splits one after the other: 37 us for 80 rows of 64.)
+template <int D, int LN>
+__global__ __launch_bounds__(256) void k_fattn_join(fs_join f) {
+    constexpr int T = D / 4 * LN, RW = 256 / T;  // threads a row, rows a workgroup
+    __shared__ fs_f4 s_acc[256];
+    __shared__ float2 s_ml[256];
+    const int tid = (int) threadIdx.x, t = tid % T, ln = t / (D / 4), d = t % (D / 4) * 4;
+    const int64_t row = (int64_t) blockIdx.x * RW + tid / T, rc = min(row, f.rows - 1);  // of (sequence, query, head)
+    const int head = (int) (rc % f.hq), q = (int) (rc / f.hq % f.n_q), seq = (int) (rc / ((int64_t) f.hq * f.n_q));
+    const int64_t blk = ((int64_t) seq * (f.hq / f.g) + head / f.g) * f.q_blocks + q / f.qpw;
+    const int64_t p0 = blk * f.split * f.R + (q % f.qpw) * f.g + head % f.g;
+    const float * ml = f.part + f.partials * D;
+    float M = -INFINITY, L = 0.0f;
     fs_f4 acc = {0, 0, 0, 0};
-    float L = 0.0f;
-    for (int z = 0; z < f.split; z++) {
-        const int64_t pr = (blk * f.split + z) * R + r;
-        const float2 ml = *(const float2 *) &f.part[rows * D + 2 * pr];
-        const float w = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
-        L = fmaf(w, ml.y, L);
-        const fs_f4 v = *(const fs_f4 *) &f.part[pr * D + d];
+    for (int z0 = ln; z0 < f.split; z0 += 4 * LN) {
+        float2 v[4];
+        fs_f4 x[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] = fmaf(w, v[i], acc[i]);
+        for (int k = 0; k < 4; k++) {
+            const int64_t p = p0 + (int64_t) min(z0 + k * LN, f.split - 1) * f.R;
+            v[k] = *(const float2 *) &ml[2 * p];
+            x[k] = *(const fs_f4 *) &f.part[p * D + d];
+        }
+        float most = M;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (z0 + k * LN >= f.split) v[k] = make_float2(-INFINITY, 0.0f);
+            most = fmaxf(most, v[k].x);
+        }
+        const float w0 = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - most);
+        L *= w0, acc *= w0, M = most;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (v[k].x == -INFINITY) continue;
+            const float w = __builtin_amdgcn_exp2f(v[k].x - most);
+            L = fmaf(w, v[k].y, L);
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] = fmaf(w, x[k][i], acc[i]);
+        }
     }
-    *(fs_f4 *) &f.out[row * D + d] = L != 0.0f ? acc / L : fs_f4{0, 0, 0, 0};
+    if constexpr (LN > 1) {
+        s_acc[tid] = acc;
+        s_ml[tid] = make_float2(M, L);
+        __syncthreads();
+        if (ln != 0) return;
+        float most = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < LN; k++) most = fmaxf(most, s_ml[tid + k * (D / 4)].x);
+        acc = fs_f4{0, 0, 0, 0}, L = 0.0f;
+#pragma unroll
+        for (int k = 0; k < LN; k++) {
+            const float2 v = s_ml[tid + k * (D / 4)];
+            if (v.x == -INFINITY) continue;
+            const float w = __builtin_amdgcn_exp2f(v.x - most);
+            L = fmaf(w, v.y, L);
+            const fs_f4 x = s_acc[tid + k * (D / 4)];
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] = fmaf(w, x[i], acc[i]);
+        }
+    }
+    if (row < f.rows) *(fs_f4 *) &f.out[row * D + d] = L != 0.0f ? acc / L : fs_f4{0, 0, 0, 0};
 }
 
 size_t fs_al(size_t v) { return (v + 255) & ~(size_t) 255; }
@@ -523,18 +531,7 @@ size_t fs_plan(const fattn_args & a, fs_args & f) {
     f.per = (f.n_tiles + f.split - 1) / f.split;
     f.split = (f.n_tiles + f.per - 1) / f.per;
     f.heads_mask = a.mask && a.m_ne2 > 1;
-    const double log2e = 1.4426950408889634074;
-    if (a.softcap > 0.0f) {
-        f.in = (float) ((double) a.scale / a.softcap);
-        f.cap2 = (float) (a.softcap * log2e);
-        for (int k = 0; k < 6; k++) f.poly[k] = (float) (kFsPoly[k] * a.softcap * log2e);
-    } else {
-        f.in = (float) (a.scale * log2e);
-    }
-    f.n_low = 1;
-    while (2 * f.n_low <= a.hq) f.n_low *= 2;
-    f.m0 = -(double) a.max_bias / f.n_low;
-    f.m1 = 0.5 * f.m0;
+    f.score = fs_score_of(a);
     size_t need = 0;
     if (a.mask) {
         const size_t n = (size_t) a.m_ne3 * (f.heads_mask ? a.hkv : 1) * f.q_blocks * f.n_tiles;
@@ -553,6 +550,7 @@ bool fattn_scored_supported(const fattn_args & a) {
 }
 
 void fattn_scored_plan(fattn_args & a, int n_cu) {
+    if (fattn_scored_dec_supported(a)) return fattn_scored_dec_plan(a, n_cu);
     // splits of the span while one sequence's query blocks leave CUs idle: two
     // workgroups a CU, at least four tiles a split. By one sequence's shape, so
     // that its rows get the same bits alone or in a batch
@@ -564,12 +562,14 @@ void fattn_scored_plan(fattn_args & a, int n_cu) {
 }
 
 size_t fattn_scored_scratch_bytes(const fattn_args & a) {
+    if (fattn_scored_dec_supported(a)) return fattn_scored_dec_scratch_bytes(a);
     fs_args f;
     return fs_plan(a, f);
 }
 
 void launch_fattn_scored(const fattn_args & a, void * scratch, float * out, hipStream_t s) {
     if (a.n_q == 0 || a.n_seq == 0) return;
+    if (fattn_scored_dec_supported(a)) return launch_fattn_scored_dec(a, scratch, out, s);
     fs_args f;
     fs_plan(a, f);
     f.out = out;
@@ -608,13 +608,27 @@ void launch_fattn_scored(const fattn_args & a, void * scratch, float * out, hipS
     else rows(std::integral_constant<int, 64>{}, one{});
     note_hip_error(hipGetLastError());
     if (f.split > 1) {
-        const int64_t threads = (int64_t) a.n_seq * a.n_q * a.hq * (a.d / 4);
-        const dim3 jg((unsigned) ((threads + 255) / 256));
-        if (a.d == 64) hipLaunchKernelGGL(k_fattn_join<64>, jg, dim3(256), 0, s, f, 64 * rw);
-        else if (a.d == 128) hipLaunchKernelGGL(k_fattn_join<128>, jg, dim3(256), 0, s, f, 64 * rw);
-        else hipLaunchKernelGGL(k_fattn_join<256>, jg, dim3(256), 0, s, f, 64 * rw);
-        note_hip_error(hipGetLastError());
+        fs_join j{};
+        j.part = f.part, j.out = out, j.rows = (int64_t) a.n_seq * a.n_q * a.hq;
+        j.partials = (int64_t) a.n_seq * a.hkv * f.q_blocks * f.split * 64 * rw;
+        j.split = f.split, j.d = a.d, j.hq = a.hq, j.n_q = a.n_q, j.g = f.g, j.qpw = f.qpw, j.q_blocks = f.q_blocks, j.R = 64 * rw;
+        launch_fattn_join(j, s);
     }
+}
+
+void launch_fattn_join(const fs_join & j, hipStream_t s) {
+    auto go = [&](auto d, auto ln) {
+        constexpr int D = decltype(d)::value, LN = decltype(ln)::value, RW = 256 / (D / 4 * LN);
+        hipLaunchKernelGGL((k_fattn_join<D, LN>), dim3((unsigned) ((j.rows + RW - 1) / RW)), dim3(256), 0, s, j);
+    };
+    auto lanes = [&](auto d) {
+        if (j.split > 8) go(d, std::integral_constant<int, 4>{});
+        else go(d, std::integral_constant<int, 1>{});
+    };
+    if (j.d == 64) lanes(std::integral_constant<int, 64>{});
+    else if (j.d == 128) lanes(std::integral_constant<int, 128>{});
+    else lanes(std::integral_constant<int, 256>{});
+    note_hip_error(hipGetLastError());
 }
 
 }  // namespace mi355x
