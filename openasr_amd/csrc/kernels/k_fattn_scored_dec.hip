@@ -277,7 +277,21 @@ void fattn_scored_dec_plan(fattn_args & a, int n_cu) {
     const int tp = fc_tile(a.d, fc_heads((g + groups - 1) / groups)), n_tiles = (a.n_kv + tp - 1) / tp;
     const int64_t units = (int64_t) a.n_seq * a.hkv * groups;
     a.scored = 1;
-    a.scored_split = (int) std::max<int64_t>(1, std::min<int64_t>((2 * n_cu + units - 1) / std::max<int64_t>(1, units), n_tiles / kFcWaves));
+    a.scored_split = 1;
+    // The splits by a model of the time, in units of 0.55 us: a workgroup (one a
+    // CU) takes 11 and one for each 32 KB of its K and V, the joining launch 6.
+    // us of splits 1 / 2 / 4 / 8 / 16: heads of 128, 8 kv heads, 1024 positions
+    // 14.8 / 13.3 / 10.7 / 10.2 / 9.4; 8 sequences of 4096 50 / 34 / 27 / 35 / -;
+    // 12 of them, of 2 / 3 / 4 38 / 43 / 44; heads of 64, 500 of 2 sequences of 16 kv
+    // heads 6.9 / 8.5 / 7.8 / 8.4; four of 20000, 4 kv heads of 5 query heads, of
+    // 10 / 14 / 16 / 20 33 / 30 / 27 / 43.
+    double best = 1e30;
+    for (int split = 1; split <= std::min(n_tiles, n_cu); split++) {
+        const int per = (n_tiles + split - 1) / split;
+        const double rounds = std::ceil((double) units * ((n_tiles + per - 1) / per) / n_cu);
+        const double t = rounds * (11.0 + per * (double) (tp * a.d) / 8192) + (per < n_tiles ? 6.0 : 0.0);
+        if (t < best) best = t, a.scored_split = split;
+    }
 }
 
 static void fc_plan(const fattn_args & a, fc_args & f) {
