@@ -3,6 +3,8 @@
 // the cap, the heads' slopes, and the joining of a row's KV splits.
 #pragma once
 
+#include <cmath>
+
 #include "mi355x_common.h"
 #include "ops.h"
 
@@ -18,9 +20,15 @@ constexpr float kFsPolyEnd = 0.625f;
 constexpr double kFsPoly[6] = {0.9999999960227207,   -0.3333325986294283,  0.13331114055632276,
                                -0.05372010765402796, 0.02058819145009359, -0.005657135182291668};
 
+// the same up to |x| = 0.25: 2.5e-9 off
+constexpr float kFsLowEnd = 0.25f;
+constexpr double kFsLow[4] = {0.9999999975205603, -0.33333206285536215, 0.13323126058728388, -0.051327005164006706};
+
 // scores in base 2 exponent units: cap log2(e) tanh(scale / cap product), or scale log2(e) product
 struct fs_score {
     float poly[6];  // tanh(x) / x times cap log2(e), of x = s / cap
+    float low[4];   // the shorter one as a polynomial of the product itself, for products below low_end
+    float low_end;
     float in;       // what a product is multiplied by: scale / cap, or scale log2(e)
     float cap2;     // cap log2(e)
     double m0, m1;  // the slopes' bases (log2)
@@ -34,6 +42,10 @@ inline fs_score fs_score_of(const fattn_args & a) {
         f.in = (float) ((double) a.scale / a.softcap);
         f.cap2 = (float) (a.softcap * log2e);
         for (int k = 0; k < 6; k++) f.poly[k] = (float) (kFsPoly[k] * a.softcap * log2e);
+        const double in = (double) a.scale / a.softcap;
+        // (from 1e-5 on the coefficients, down to in^7, are normal numbers)
+        f.low_end = std::fabs(in) >= 1e-5 ? (float) (kFsLowEnd / std::fabs(in)) : 0.0f;
+        for (int k = 0; k < 4; k++) f.low[k] = (float) (kFsLow[k] * a.softcap * log2e * std::pow(in, 2 * k + 1));
     } else {
         f.in = (float) (a.scale * log2e);
     }
@@ -59,6 +71,12 @@ __device__ __forceinline__ float fs_cap_small(const fs_score & f, float x) {
     return x * p;
 }
 
+// the cap of a product below low_end in size, plus base
+__device__ __forceinline__ float fs_cap_low(const fs_score & f, float s, float base) {
+    const float y = s * s;
+    return fmaf(s, fmaf(fmaf(fmaf(f.low[3], y, f.low[2]), y, f.low[1]), y, f.low[0]), base);
+}
+
 // for any x: 1 - 2 / (e^2x + 1), from the polynomial where that cancels
 __device__ __forceinline__ float fs_cap_any(const fs_score & f, float x) {
     const float e = __builtin_amdgcn_exp2f(2.0f * kFsLog2e * fabsf(x));  // +inf from |x| = 45 on: the quotient is 0
@@ -77,6 +95,7 @@ void launch_fattn_scored_dec(const fattn_args & a, void * scratch, float * out, 
 // of `partials` in all
 struct fs_join {
     const float * part;
+    const int * pieces;  // how many of the `split` partials a (sequence, kv head, query block) has; null: all of them
     float * out;
     int64_t rows, partials;
     int split, d;

@@ -8,23 +8,29 @@
 // in f32, products of f16 (exact in f32), p as the sum of two f16 (22 bits: a
 // single one would leave the result 11).
 //
-// Work: a workgroup of four waves owns R = 64 RW rows -- R / g queries times
-// the g query heads of a kv head -- and walks the open 64-position tiles of its
-// split of the span; wave w owns rows 16 RW w .. of them, RW = 2 reading every
-// K and V fragment once for 32 rows (16 rows a wave read 98 of the 128 bytes a
-// cycle that LDS gives). MFMA 16x16x32 layouts: A lane l = row l % 16, k 8 (l /
+// Work: a workgroup of eight waves owns R = 128 RW rows -- R / g queries times the g
+// query heads of a kv head -- and walks its piece of the open 64-position tiles of
+// the span; wave w owns rows 16 RW w .. of them, RW = 2 reading every K and V
+// fragment once for 32 rows. MFMA 16x16x32 layouts: A lane l = row l % 16, k 8 (l /
 // 16) .. + 7; B lane l = column l % 16, the same k; result lane l = rows 4 (l /
 // 16) .. + 3, column l % 16. Scores are made transposed (rows = positions), so
 // a lane holds 16 positions of a row and its p are the P V product's own B
-// operand, V^T read in the same order of positions.
+// operand, V^T read in the same order of positions (by the transposing LDS reads).
 //
 // A first launch looks at the mask once for all heads: which tiles a block of
 // queries sees at all, which of them have no masked or no nonzero entry, and
-// which positions some query sees.
+// which positions some query sees. From its counts every workgroup finds the same
+// equal pieces, and a third launch joins the pieces of a row where there are several.
 //
-// What bounds it: a score takes about 16 vector instructions beside its MFMA
-// time (the cap 7: a polynomial of (s / cap)^2; 1 mask, 2 maximum and
-// subtraction, a quarter-rate exponential, 2 for the halves of p).
+// What bounds it: 256 rows of 128 by a tile take 8400 cycles of a CU, its 832 matrix
+// instructions 3328 of each SIMD's and its exponentials 4000 to 4900 of the vector
+// units' (9 vector instructions a score with a cap -- a polynomial of the product
+// five, p's halves two -- and a quarter-rate exponential); the two overlap, a
+// request for 1 KB of K or V holds its wave for 150 to 300 cycles of it. us of the
+// call without a barrier between the two kinds of work (four waves a workgroup, two
+// workgroups a CU, which fell into step) and with it: two sequences of 4096 causal
+// queries, 16 heads of 128 over 8, capped 264 / 251, not capped 240 / 227; one of
+// 1777 in three documents, 8 heads of 256 59 / 52.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -38,15 +44,18 @@ namespace mi355x {
 namespace {
 
 constexpr int kFsTile = 64;
-constexpr int kFsThreads = 256;
 // p is scaled by 2^12: its low half stays a normal f16 down to 2^-15 of the maximum
 constexpr float kFsUp = 12.0f;
+constexpr float kFsOver = 3.0f;  // (and stays below f16's 2^16)
 
 typedef _Float16 fs_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 fs_h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 fs_h2 __attribute__((ext_vector_type(2)));
 typedef uint32_t fs_u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t fs_u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t fs_u2h __attribute__((ext_vector_type(2), aligned(2)));  // (the mask's rows have two-byte alignment)
+typedef float fs_f4a __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t fs_u4h __attribute__((ext_vector_type(4), aligned(2)));
 
 // a tile of a query block: nothing seen; seen, and all entries zero; seen, no
 // entry -inf; seen, some entry -inf (or past the span)
@@ -56,68 +65,60 @@ struct fs_args {
     fattn_args a;
     fs_score score;
     int g, qpw;       // query heads a kv head, queries a workgroup
-    int q_blocks, n_tiles, split, per;
+    int q_blocks, n_tiles;
+    int split, slots;  // the most pieces of a query block's open tiles; workgroups that the card holds at once
     int heads_mask;   // the mask differs by head: rows of it by query and head
     uint64_t * seen;  // [mask sequence][kv head or one][query block][tile]
-    uint8_t * cls;
+    uint8_t * cls;    // [n_cls], the same order
+    int64_t n_cls;
+    int * pieces;     // [sequence][kv head][query block]
     float * part;
     float * out;
 };
 
 // eight mask entries at pos of a row, -inf past the span
-template <bool V16>
 __device__ __forceinline__ fs_u4 fs_mask8(const uint16_t * row, int pos, int n_kv) {
-    fs_u4 m;
-    if constexpr (V16) {
-        m = *(const fs_u4 *) (row + min(pos, (n_kv - 1) & ~7));
-    } else {
+    if (pos + 8 <= n_kv) return *(const fs_u4h *) (row + pos);
+    uint32_t e[8];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            m[j] = (uint32_t) row[min(pos + 2 * j, n_kv - 1)] | ((uint32_t) row[min(pos + 2 * j + 1, n_kv - 1)] << 16);
-    }
-    if (pos + 8 > n_kv) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (pos + 2 * j >= n_kv) m[j] = (m[j] & 0xFFFF0000u) | kFsNegInf;
-            if (pos + 2 * j + 1 >= n_kv) m[j] = (m[j] & 0xFFFFu) | (kFsNegInf << 16);
-        }
-    }
-    return m;
+    for (int j = 0; j < 8; j++) e[j] = pos + j < n_kv ? (uint32_t) row[pos + j] : kFsNegInf;
+    return fs_u4{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
 }
 
 __device__ __forceinline__ const char * fs_mask_of(const fattn_args & a, int seq, int head) {
     return a.mask + (int64_t) (seq % a.m_ne3) * a.m_nb3 + (int64_t) (head % a.m_ne2) * a.m_nb2;
 }
 
-// one wave a tile of a query block: lane = 8-position piece l % 8 of rows l / 8, + 8 ..
-template <bool V16>
-__global__ __launch_bounds__(256) void k_fattn_tiles(fs_args f, int64_t units) {
+// One workgroup a tile of a query block: thread = 8-position piece t % 8 of rows t / 8, + 32 ..
+__global__ __launch_bounds__(256) void k_fattn_tiles(fs_args f) {
+    __shared__ uint32_t s_bits[4][2];
+    __shared__ uint64_t s_seen[4];
     const fattn_args & a = f.a;
-    const int lane = threadIdx.x & 63;
-    const int64_t u = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (u >= units) return;
+    const int tid = (int) threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t u = blockIdx.x;
     const int tile = (int) (u % f.n_tiles), qb = (int) (u / f.n_tiles % f.q_blocks);
     const int64_t hs = u / ((int64_t) f.n_tiles * f.q_blocks);
     const int kinds = f.heads_mask ? a.hkv : 1, kvh = (int) (hs % kinds), ms = (int) (hs / kinds);
     const int q0 = qb * f.qpw, nq = min(f.qpw, a.n_q - q0), heads = f.heads_mask ? f.g : 1, rows = nq * heads;
-    const int c = lane & 7, pos = tile * kFsTile + 8 * c;
+    const int pos = tile * kFsTile + 8 * (tid & 7);
+    fs_u4 m[8];  // (at most 256 rows)
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const int r = (tid >> 3) + 32 * k;
+        m[k] = fs_u4{};
+        if (r < rows) m[k] = fs_mask8((const uint16_t *) (fs_mask_of(a, ms, kvh * f.g + r % heads) + (int64_t) (q0 + r / heads) * a.m_nb1), pos, a.n_kv);
+    }
     uint32_t open = 0, closed = 0, adds = 0;
-    for (int r0 = lane >> 3; r0 < rows; r0 += 32) {
-        fs_u4 m[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int r = min(r0 + 8 * k, rows - 1);
-            m[k] = fs_mask8<V16>((const uint16_t *) (fs_mask_of(a, ms, kvh * f.g + r % heads) + (int64_t) (q0 + r / heads) * a.m_nb1), pos, a.n_kv);
+    for (int k = 0; k < 8; k++) {
+        if ((tid >> 3) + 32 * k >= rows) continue;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const bool lo = (m[k][j] & 0xFFFFu) == kFsNegInf, hi = (m[k][j] >> 16) == kFsNegInf;
+            open |= (lo ? 0u : 1u << (2 * j)) | (hi ? 0u : 2u << (2 * j));
+            closed |= lo || hi;
+            adds |= m[k][j] & 0x7FFF7FFFu;  // (-0 adds as 0)
         }
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const bool lo = (m[k][j] & 0xFFFFu) == kFsNegInf, hi = (m[k][j] >> 16) == kFsNegInf;
-                open |= (lo ? 0u : 1u << (2 * j)) | (hi ? 0u : 2u << (2 * j));
-                closed |= lo || hi;
-                adds |= m[k][j] & 0x7FFF7FFFu;  // (-0 adds as 0)
-            }
     }
 #pragma unroll
     for (int o = 8; o < 64; o <<= 1) open |= __shfl_xor(open, o);
@@ -125,10 +126,17 @@ __global__ __launch_bounds__(256) void k_fattn_tiles(fs_args f, int64_t units) {
 #pragma unroll
     for (int k = 0; k < 8; k++) seen |= (uint64_t) (uint32_t) __shfl(open, k) << (8 * k);
     const bool any_closed = __any(closed != 0), any_adds = __any(adds != 0);
-    if (lane == 0) {
-        f.seen[u] = seen;
-        f.cls[u] = !seen ? kFsClosed : any_closed ? kFsMixed : any_adds ? kFsAdds : kFsPlain;
-    }
+    if (lane == 0) s_seen[wave] = seen, s_bits[wave][0] = any_closed, s_bits[wave][1] = any_adds;
+    __syncthreads();
+    if (tid != 0) return;
+    bool c = false, d = false;
+    seen = 0;
+#pragma unroll
+    for (int w = 0; w < 4; w++) seen |= s_seen[w], c |= s_bits[w][0] != 0, d |= s_bits[w][1] != 0;
+    if (u == f.n_cls - 1)
+        for (int64_t i = f.n_cls; i & 15; i++) f.cls[i] = kFsClosed;  // (counted 16 at a time)
+    f.seen[u] = seen;
+    f.cls[u] = !seen ? kFsClosed : c ? kFsMixed : d ? kFsAdds : kFsPlain;
 }
 
 // whether one of eight f16 is infinite or NaN
@@ -143,80 +151,91 @@ __device__ __forceinline__ fs_f4 fs_mfma(fs_h8 a, fs_h8 b, fs_f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// MM: 0 no mask, 1 rows of 16-byte pieces, 2 other rows
-template <int D, int RW, bool CAP, int MM>
-__global__ __launch_bounds__(kFsThreads, D == 256 ? 1 : 2) void k_fattn_scored(fs_args f) {
-    constexpr int R = 64 * RW;                            // rows of a workgroup
+// LDS holds a tile's K and V rows as they lie, 16-byte piece p of row r in slot p
+// ^ 2 fs_turn(r): K's fragments (rows of 16 lanes, a piece each) and V's (two
+// pieces of four rows a group of 16 lanes) then reach all 64 banks
+template <int D>
+__device__ __forceinline__ int fs_turn(int row) {
+    return D == 64 ? (row >> 1) & 3 : row & 7;
+}
+
+typedef short fs_s4 __attribute__((ext_vector_type(4)));
+// column l % 16 of the four rows of 16 halves that the lane's group of 16 reads, four halves a lane
+__device__ __forceinline__ fs_h4 fs_read_turned(const char * p) {
+    return __builtin_bit_cast(fs_h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) fs_s4 *) p));
+}
+
+// the largest of lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float fs_max4(float x) {
+    // (the swaps' results as values: a bit cast of a vector's element takes its first)
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a0 = a[0], a1 = a[1];
+    const uint32_t v = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1)));
+    const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const uint32_t b0 = b[0], b1 = b[1];
+    return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+
+// z less the low, high half of h: one instruction (the compiler takes two)
+__device__ __forceinline__ float fs_less_low(float z, uint32_t h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(z));
+    return r;
+}
+__device__ __forceinline__ float fs_less_high(float z, uint32_t h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(z));
+    return r;
+}
+
+// Sixteen bytes a lane from memory to LDS: lane l's at lds + 16 l. Not by the
+// builtin, after which the compiler waits for all such loads before any read of
+// LDS: here they are waited for by hand, two phases later
+__device__ __forceinline__ void fs_to_lds(const char * src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
+}
+
+// The phases' boundary: LDS reads are done; loads to LDS stay in flight
+__device__ __forceinline__ void fs_phase_end() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+template <int D, int RW, bool CAP, bool MASK>
+__global__ __launch_bounds__(512, 2) void k_fattn_scored(fs_args f) {
+    constexpr int NW = 8, NTH = 64 * NW, R = 16 * RW * NW;  // waves, threads, rows of a workgroup
     constexpr int KS = D / 32, NT = D / 16;
-    constexpr int KP = D + 8, VP = kFsTile + 8, MP = kFsTile + 8;
-    constexpr int PC = D / 8;                             // 16-byte pieces of a K / V row
-    constexpr int KLD = kFsTile * PC / kFsThreads, VLD = KLD / 2;
-    constexpr int MLD = MM ? R * 8 / kFsThreads : 1;
-    __shared__ __align__(16) _Float16 s_k[kFsTile][KP];
-    __shared__ __align__(16) _Float16 s_vt[D][VP];
-    __shared__ __align__(16) uint16_t s_m[MM ? R : 1][MP];
-    __shared__ unsigned long long s_bad;                  // positions of the tile whose V is not finite
+    constexpr int PC = D / 8;                       // 16-byte pieces of a K / V row
+    constexpr int LTH = NTH / 2, KLD = kFsTile * PC / LTH;  // threads that load, and pieces of K, or V, of each
+    constexpr int TB = kFsTile * 2 * D;             // bytes of a tile's K, or V
+    __shared__ __align__(16) char s_kv[2][2][TB];   // [K, V][parity of the tile]
+    __shared__ unsigned long long s_bad[2];         // positions of the tile whose V is not finite
     const fattn_args & a = f.a;
-    const int tid = (int) threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, lg = lane >> 4;
-    // Workgroup b runs on XCD b % 8: an XCD takes a contiguous run of (split,
-    // query block, kv head, sequence), so that those which read the same K and
-    // V share an L2; the last query blocks, whose causal span is the longest, first
-    const int n_blk = (int) gridDim.x;
-    int b = (int) blockIdx.x;
-    if (n_blk % 8 == 0) b = (b % 8) * (n_blk / 8) + b / 8;
-    const int z = b % f.split;
-    const int qb = f.q_blocks - 1 - b / f.split % f.q_blocks, hs = b / f.split / f.q_blocks;
+    const int tid = (int) threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lg = lane >> 4;
+    // Workgroup b runs on XCD b % 8. Where the (sequence, kv head) pairs divide by
+    // eight an XCD takes its share of them, whose K and V its L2 then holds. First
+    // pieces first, and of them the last query blocks, whose causal span is longest
+    const int heads = a.hkv * a.n_seq, units = heads * f.q_blocks;
+    int b = (int) blockIdx.x, z, qb, hs;
+    if (heads % 8 == 0) {
+        const int i = b / 8, h8 = heads / 8;
+        z = i / (units / 8), qb = f.q_blocks - 1 - i % (units / 8) / h8, hs = b % 8 * h8 + i % h8;
+    } else {
+        z = b / units, qb = f.q_blocks - 1 - b % units / heads, hs = b % heads;
+    }
     const int kvh = hs % a.hkv, seq = hs / a.hkv, kv_seq = seq / a.rk3;
     const int q0 = qb * f.qpw, nq = min(f.qpw, a.n_q - q0);
-    const int mheads = f.heads_mask ? f.g : 1, mrows = nq * mheads;
     const char * kbase = a.k + (int64_t) kvh * a.k_nb2 + (int64_t) kv_seq * a.k_nb3;
     const char * vbase = a.v + (int64_t) kvh * a.v_nb2 + (int64_t) kv_seq * a.v_nb3;
-    const int t_begin = z * f.per, t_end = min(f.n_tiles, t_begin + f.per);
-    const int64_t tile0 = MM ? ((int64_t) ((seq % a.m_ne3) * (f.heads_mask ? a.hkv : 1) + (f.heads_mask ? kvh : 0)) * f.q_blocks + qb) * f.n_tiles : 0;
-    auto class_of = [&](int t) -> int {
-        if constexpr (MM != 0) return f.cls[tile0 + t];
-        else return (t + 1) * kFsTile <= a.n_kv ? kFsPlain : kFsMixed;
-    };
-    auto next_open = [&](int t) {
-        if constexpr (MM != 0) {
-            while (t < t_end && f.cls[tile0 + t] == kFsClosed) t++;
-        }
-        return t;
-    };
+    const int64_t tile0 = MASK ? ((int64_t) ((seq % a.m_ne3) * (f.heads_mask ? a.hkv : 1) + (f.heads_mask ? kvh : 0)) * f.q_blocks + qb) * f.n_tiles : 0;
 
-    fs_u4 kr[KLD], vr[VLD][2], mr[MLD];
-    auto issue = [&](int tile, int cls) {
-        const int p0 = tile * kFsTile;
-#pragma unroll
-        for (int i = 0; i < KLD; i++) {
-            const int e = tid + i * kFsThreads, p = e / PC, piece = e % PC;
-            kr[i] = *(const fs_u4 *) (kbase + (int64_t) min(p0 + p, a.n_kv - 1) * a.k_nb1 + 16 * piece);
-        }
-#pragma unroll
-        for (int i = 0; i < VLD; i++) {
-            const int e = tid + i * kFsThreads, pair = e % (kFsTile / 2), piece = e / (kFsTile / 2);
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-                vr[i][h] = *(const fs_u4 *) (vbase + (int64_t) min(p0 + 2 * pair + h, a.n_kv - 1) * a.v_nb1 + 16 * piece);
-        }
-        if constexpr (MM != 0) {
-            if (cls >= kFsAdds) {
-#pragma unroll
-                for (int i = 0; i < MLD; i++) {
-                    const int e = tid + i * kFsThreads, r = min(e >> 3, mrows - 1), c = e & 7;
-                    mr[i] = fs_mask8<MM == 1>((const uint16_t *) (fs_mask_of(a, seq, kvh * f.g + r % mheads) + (int64_t) (q0 + r / mheads) * a.m_nb1),
-                                              p0 + 8 * c, a.n_kv);
-                }
-            }
-        }
-    };
-    int tile = next_open(t_begin), cls = tile < t_end ? class_of(tile) : kFsClosed;
-    if (tile < t_end) issue(tile, cls);
-
-    // this lane's query rows (the score product's B operand), rounded to f16
-    fs_h8 qa[RW][KS];
+    // the rows' queries are on their way while the tiles are looked at
+    fs_f4 qraw[RW][KS][2];
     float slope[RW];
-    int mrow[RW];
+    const char * mrow[RW];
 #pragma unroll
     for (int w = 0; w < RW; w++) {
         const int r = 16 * (RW * wave + w) + l16, ql = min(r / f.g, nq - 1), head = kvh * f.g + r % f.g;
@@ -224,220 +243,400 @@ __global__ __launch_bounds__(kFsThreads, D == 256 ? 1 : 2) void k_fattn_scored(f
 #pragma unroll
         for (int kk = 0; kk < KS; kk++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) qa[w][kk][j] = (_Float16) ((const float *) qp)[32 * kk + 8 * lg + j];
+            for (int h = 0; h < 2; h++) qraw[w][kk][h] = *(const fs_f4a *) (qp + 4 * (32 * kk + 8 * lg + 4 * h));
         slope[w] = fs_slope(f.score, a.max_bias, head);
-        mrow[w] = f.heads_mask ? min(ql * f.g + r % f.g, mrows - 1) : ql;
+        mrow[w] = MASK ? fs_mask_of(a, seq, head) + (int64_t) (q0 + ql) * a.m_nb1 : nullptr;
     }
-    if (tid == 0) s_bad = 0;
 
-    float m[RW], l[RW];
+    // The classes of 64 tiles from w_base on, a bit a tile
+    int w_base = 0;
+    uint64_t w_open, w_adds, w_mixed;
+    auto window = [&]() {
+        const int t = w_base + lane;
+        int c = kFsClosed;
+        if constexpr (MASK) {
+            if (t < f.n_tiles) c = f.cls[tile0 + t];
+        } else {
+            if (t < f.n_tiles) c = (t + 1) * kFsTile <= a.n_kv ? kFsPlain : kFsMixed;
+        }
+        w_open = __ballot(c != kFsClosed), w_adds = __ballot(c >= kFsAdds), w_mixed = __ballot(c == kFsMixed);
+    };
+    // The open tiles of this query block, in equal pieces. A piece is what the
+    // launch's open tiles come to on each place of the card that is left when
+    // every block has one, so that no piece waits for a second round (a block's
+    // last piece is cut short); at least four tiles
+    int n_open = 0, skip = 0, pieces = 1;
+    if (MASK) {
+        for (w_base = 0; w_base < f.n_tiles; w_base += 64) {
+            window();
+            n_open += __popcll(w_open);
+        }
+    } else {
+        n_open = f.n_tiles;
+    }
+    if (f.split > 1) {
+        int64_t all = (int64_t) f.n_tiles * f.q_blocks * a.hkv * a.n_seq;
+        if constexpr (MASK) {
+            __shared__ int s_open[NW];
+            int n = 0;
+            for (int64_t i = 16 * (int64_t) tid; i < f.n_cls; i += 16 * NTH) {
+                const fs_u4 c = *(const fs_u4 *) &f.cls[i];
+#pragma unroll
+                for (int j = 0; j < 4; j++) n += __popc((c[j] | (c[j] >> 1)) & 0x01010101u);
+            }
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o);
+            if (lane == 0) s_open[wave] = n;
+            __syncthreads();
+            int64_t sum = 0;
+#pragma unroll
+            for (int w = 0; w < NW; w++) sum += s_open[w];
+            all = sum * (f.heads_mask ? 1 : a.hkv) * (a.n_seq / a.m_ne3);
+        }
+        const int piece = max(4, (int) ((float) all / (float) max(f.slots - units, f.slots / 2)) + 1);
+        pieces = __builtin_amdgcn_readfirstlane(max(1, min(f.split, (n_open + piece - 1) / piece)));
+        if (z >= pieces) return;
+        if (z == 0 && tid == 0) f.pieces[hs * f.q_blocks + qb] = pieces;
+        const int each = n_open / pieces, more = n_open % pieces;
+        skip = z * each + min(z, more);
+        n_open = each + (z < more ? 1 : 0);
+    }
+    w_base = 0;
+    window();
+    auto next_open = [&]() {  // the first open tile of the window or after it, taken out of it
+        while (w_open == 0) w_base += 64, window();
+        const int t = __builtin_ctzll(w_open);
+        w_open &= w_open - 1;
+        return w_base + t;
+    };
+    auto class_of = [&](int t) { return (w_mixed >> (t & 63)) & 1 ? kFsMixed : (w_adds >> (t & 63)) & 1 ? kFsAdds : kFsPlain; };
+    if (n_open > 0) {
+        while (skip >= __popcll(w_open)) skip -= __popcll(w_open), w_base += 64, window();
+        for (; skip > 0; skip--) w_open &= w_open - 1;
+    }
+
+    // this lane's query rows (the score product's B operand), rounded to f16
+    fs_h8 qa[RW][KS];
+#pragma unroll
+    for (int w = 0; w < RW; w++)
+#pragma unroll
+        for (int kk = 0; kk < KS; kk++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) qa[w][kk][j] = (_Float16) qraw[w][kk][j >> 2][j & 3];
+    if (tid < 2) s_bad[tid] = 0;
+
+    // A tile's K and V go to LDS by themselves, 16 bytes a lane, LTH / PC rows a step
+    // (a multiple of what fs_turn repeats after). Group 0 (below) requests V, group 1 K
+    const int st_row = tid % LTH / PC, st_piece = (tid % PC) ^ (2 * fs_turn<D>(st_row));
+    const char * const st[2] = {kbase + st_row * a.k_nb1 + 16 * st_piece, vbase + st_row * a.v_nb1 + 16 * st_piece};
+    const uint32_t lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) char *) &s_kv[0][0][0] + 1024 * (wave & 3);
+    auto issue_one = [&](int h, int i, int tile, int par) {  // h: 0 K, 1 V
+        const int64_t nb1 = h ? a.v_nb1 : a.k_nb1;
+        const int row = tile * kFsTile + i * (LTH / PC);
+        const char * p = st[h] + row * nb1;
+        if ((tile + 1) * kFsTile > a.n_kv) p += (min(row + st_row, a.n_kv - 1) - (row + st_row)) * nb1;
+        fs_to_lds(p, lds0 + (2 * h + par) * TB + i * LTH * 16);
+    };
+    auto issue = [&](int h, int tile, int par) {
+#pragma unroll
+        for (int i = 0; i < KLD; i++) issue_one(h, i, tile, par);
+    };
+    // Group 0, at the tile's arrival. Where not every query sees everything,
+    // positions of V that no query sees become zeros (0 times anything), and pieces
+    // that are not finite too: those are added query by query
+    auto landed = [&](int tile, int cls, int par) {
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+        asm volatile("" ::: "memory");
+        if (cls != kFsMixed) return;
+        uint64_t seen;
+        if constexpr (MASK) seen = f.seen[tile0 + tile];
+        else seen = ~0ull >> ((tile + 1) * kFsTile - a.n_kv);
+#pragma unroll
+        for (int i = 0; i < KLD; i++) {
+            const int row = st_row + i * (LTH / PC);
+            fs_u4 * p = (fs_u4 *) &s_kv[1][par][(i * LTH + tid) * 16];
+            const bool in = (seen >> row) & 1, odd = fs_odd(*p);
+            if (in && odd) atomicOr(&s_bad[par], 1ull << row);
+            if (!in || odd) *p = fs_u4{0, 0, 0, 0};
+        }
+    };
+    // this lane's entries (positions 16 t + 4 lg + i) of its rows' mask, if the tile needs them
+    fs_u2 mr[RW][4];
+    auto issue_mask = [&](int tile, int cls) {
+        if constexpr (MASK) {
+            const int p0 = tile * kFsTile;
+            if (cls >= kFsAdds && p0 + kFsTile <= a.n_kv) {
+#pragma unroll
+                for (int w = 0; w < RW; w++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++) mr[w][t] = *(const fs_u2h *) (mrow[w] + 2 * (p0 + 16 * t + 4 * lg));
+            } else if (cls >= kFsAdds) {
+#pragma unroll
+                for (int w = 0; w < RW; w++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++) {
+                        uint32_t e[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int pos = p0 + 16 * t + 4 * lg + i;
+                            e[i] = ((const uint16_t *) mrow[w])[min(pos, a.n_kv - 1)];
+                            if (pos >= a.n_kv) e[i] = kFsNegInf;
+                        }
+                        mr[w][t] = fs_u2{e[0] | e[1] << 16, e[2] | e[3] << 16};
+                    }
+            }
+        }
+    };
+
+    // A row's exponents are its scores plus base, which puts its maximum at kFsUp
+    // when it is set; it is set anew where a score goes past that by more than
+    // kFsOver, not with every new maximum
+    float base[RW], l[RW];
     fs_f4 o[RW][NT];
 #pragma unroll
     for (int w = 0; w < RW; w++) {
-        m[w] = -INFINITY, l[w] = 0.0f;
+        base[w] = 0.0f, l[w] = 0.0f;
 #pragma unroll
         for (int ct = 0; ct < NT; ct++) o[w][ct] = fs_f4{0, 0, 0, 0};
     }
 
-    while (tile < t_end) {
-        __syncthreads();  // the tile before has been read
+    // Two groups of four waves, one of each a SIMD, take turns: while one makes
+    // P V of a tile and K Q of the next on the matrix cores, the other makes its
+    // exponentials on the vector units. A phase ends with a barrier; group 1 is a
+    // phase behind:
+    //     group 0   Q K 0 | softmax 0 | P V 0, Q K 1 | softmax 1 | ...
+    //     group 1         | Q K 0     | softmax 0    | P V 0, Q K 1 | ...
+    // In even phase 2 s group 0 requests V s between its products and group 1 K s + 1,
+    // over V s - 2 and K s - 1,
+    // which nobody reads any more; they wait for them at the end of phase 2 s + 1.
+    const int grp = wave >> 2;
+    fs_f4 sc[RW][4];
+    fs_h8 hi[RW][2], lo[RW][2];  // p's halves, k slot 8 lg + j of step kk: position 32 kk + 16 (j / 4) + 4 lg + j % 4
+    // Steps of the products, each of one fragment from LDS, read DIST steps ahead:
+    // O^T += V^T P^T (two steps of 32 positions for each 16 dims), then S^T = K Q^T of
+    // the next tile (lane (lg, l16) gets positions 16 t + 4 lg + i of row l16)
+    constexpr int PV = 2 * NT, QK = 4 * KS, DIST = 4, EVERY = 4;
+    static_assert(1 + EVERY * (KLD - 1) < PV + QK, "a step for each request");
+    auto products = [&](const char * sv, const char * sk, auto from, auto loads, int tile, int par) {
+        constexpr int FROM = decltype(from)::value;
+        constexpr bool LOADS = decltype(loads)::value;  // V of a tile, between the steps
+        fs_h8 ring[DIST + 1];
+        // the rows' sums: products with ones, every lane of a row's column gets it
+        const fs_h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+        fs_f4 sum[RW];
 #pragma unroll
-        for (int i = 0; i < KLD; i++) {
-            const int e = tid + i * kFsThreads;
-            *(fs_u4 *) &s_k[e / PC][8 * (e % PC)] = kr[i];
-        }
-        uint64_t seen = ~0ull;
-        if (cls == kFsMixed) {
-            if constexpr (MM != 0) seen = f.seen[tile0 + tile];
-            else seen = ~0ull >> ((tile + 1) * kFsTile - a.n_kv);
-        }
+        for (int w = 0; w < RW; w++) sum[w] = fs_f4{0, 0, 0, 0};
+        const int lrow = 4 * lg + (l16 >> 2), vturn = 2 * fs_turn<D>(lrow), kturn = 2 * fs_turn<D>(l16);  // (16 rows on: the same turn)
+        auto read = [&](int i) {
+            if (i < PV) {
+                const int ct = i % NT, kk = i / NT;
+                const char * p = &sv[(32 * kk + lrow) * 2 * D + (((2 * ct + ((l16 >> 1) & 1)) ^ vturn) * 16) + 8 * (l16 & 1)];
+                const fs_h4 v0 = fs_read_turned(p), v1 = fs_read_turned(p + 16 * 2 * D);
+                ring[i % (DIST + 1)] = fs_h8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+            } else {
+                const int t = (i - PV) % 4, kk = (i - PV) / 4;
+                ring[i % (DIST + 1)] = *(const fs_h8 *) &sk[(16 * t + l16) * 2 * D + (((4 * kk + lg) ^ kturn) * 16)];
+            }
+        };
 #pragma unroll
-        for (int i = 0; i < VLD; i++) {
-            const int e = tid + i * kFsThreads, pair = e % (kFsTile / 2), piece = e / (kFsTile / 2);
-            if (cls == kFsMixed) {
-                // V rows that no query sees are zeros (0 times anything), and
-                // pieces of rows that are not finite are added query by query
+        for (int i = FROM; i < FROM + DIST; i++) read(i);
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const bool odd = fs_odd(vr[i][h]);
-                    const bool in = (seen >> (2 * pair + h)) & 1;
-                    if (in && odd) atomicOr(&s_bad, 1ull << (2 * pair + h));
-                    if (!in || odd) vr[i][h] = fs_u4{0, 0, 0, 0};
+        for (int i = FROM; i < PV + QK; i++) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + DIST < PV + QK) read(i + DIST);
+            if (LOADS && i % EVERY == 1 && i / EVERY < KLD) issue_one(1, i / EVERY, tile, par);
+            const fs_h8 x = ring[i % (DIST + 1)];
+            if (i < PV) {
+                const int ct = i % NT, kk = i / NT;
+#pragma unroll
+                for (int w = 0; w < RW; w++) o[w][ct] = fs_mfma(x, lo[w][kk], o[w][ct]);
+#pragma unroll
+                for (int w = 0; w < RW; w++) o[w][ct] = fs_mfma(x, hi[w][kk], o[w][ct]);
+                if (ct < 2) {
+#pragma unroll
+                    for (int w = 0; w < RW; w++) sum[w] = fs_mfma(ones, ct ? hi[w][kk] : lo[w][kk], sum[w]);
                 }
-            }
+                if (i == PV - 1) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                *(uint32_t *) &s_vt[8 * piece + 2 * j][2 * pair] = __builtin_amdgcn_perm(vr[i][1][j], vr[i][0][j], 0x05040100u);
-                *(uint32_t *) &s_vt[8 * piece + 2 * j + 1][2 * pair] = __builtin_amdgcn_perm(vr[i][1][j], vr[i][0][j], 0x07060302u);
-            }
-        }
-        if constexpr (MM != 0) {
-            if (cls >= kFsAdds) {
-#pragma unroll
-                for (int i = 0; i < MLD; i++) {
-                    const int e = tid + i * kFsThreads;
-                    if ((e >> 3) < mrows) *(fs_u4 *) &s_m[e >> 3][8 * (e & 7)] = mr[i];
+                    for (int w = 0; w < RW; w++) l[w] += sum[w][0];
                 }
+            } else {
+                const int t = (i - PV) % 4, kk = (i - PV) / 4;
+#pragma unroll
+                for (int w = 0; w < RW; w++) sc[w][t] = fs_mfma(x, qa[w][kk], kk == 0 ? fs_f4{0, 0, 0, 0} : sc[w][t]);
             }
         }
-        __syncthreads();
-        const int nxt = next_open(tile + 1), nxt_cls = nxt < t_end ? class_of(nxt) : kFsClosed;
-        if (nxt < t_end) issue(nxt, nxt_cls);
+        __builtin_amdgcn_sched_barrier(0);
+    };
 
-        // S^T = K Q^T: lane (lg, l16) gets positions 16 t + 4 lg + i of row l16
-        fs_f4 sc[RW][4];
-#pragma unroll
-        for (int w = 0; w < RW; w++)
-#pragma unroll
-            for (int t = 0; t < 4; t++) sc[w][t] = fs_f4{0, 0, 0, 0};
-#pragma unroll
-        for (int kk = 0; kk < KS; kk++) {
-            fs_h8 kb[4];
-#pragma unroll
-            for (int t = 0; t < 4; t++) kb[t] = *(const fs_h8 *) &s_k[16 * t + l16][32 * kk + 8 * lg];
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int w = 0; w < RW; w++) sc[w][t] = fs_mfma(kb[t], qa[w][kk], sc[w][t]);
+    int tile[3] = {0, 0, 0}, cls[3] = {kFsClosed, kFsClosed, kFsClosed}, par = 0;  // of tiles t, t + 1, t + 2
+    auto take = [&](int k, int left) {
+        if (left > 0) tile[k] = next_open(), cls[k] = class_of(tile[k]);
+        else tile[k] = tile[k - 1];
+    };
+    auto run = [&](auto group) {
+        constexpr int GRP = decltype(group)::value;
+        tile[0] = next_open(), cls[0] = class_of(tile[0]), take(1, n_open - 1);
+        if constexpr (GRP == 1) {
+            issue(0, tile[0], 0);
+            __builtin_amdgcn_s_waitcnt(0x0F70);
         }
-        fs_h8 hi[RW][2], lo[RW][2];  // p's halves, k slot 8 lg + j of step kk: position 32 kk + 16 (j / 4) + 4 lg + j % 4
-        const bool odd_rows = cls == kFsMixed && s_bad != 0;
-        fs_f4 pv[RW][4];
+        issue_mask(tile[0], cls[0]);
+        fs_phase_end();
+        if constexpr (GRP == 0) {
+            issue(1, tile[0], 0);
+        } else {
+            issue(0, tile[1], 1);
+            fs_phase_end();
+        }
+        products(s_kv[1][0], s_kv[0][0], std::integral_constant<int, PV>{}, std::false_type{}, 0, 0);
+        if constexpr (GRP == 1) __builtin_amdgcn_s_waitcnt(0x0F70);
+        fs_phase_end();
+        for (; n_open > 0; n_open--, par ^= 1) {
+            take(2, n_open - 2);
 #pragma unroll
-        for (int w = 0; w < RW; w++) {
-            float z[4][4];
-            if constexpr (CAP) {
-                float most = 0.0f;
+            for (int w = 0; w < RW; w++) {
+                if constexpr (GRP == 1) {
 #pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(sc[w][t][i]));
-                if (__any(!(most * f.score.in < kFsPolyEnd))) {
+                    for (int i = w * KLD / RW; i < (w + 1) * KLD / RW; i++) issue_one(0, i, tile[2], par);
+                }
+                float z[4][4];
+                if constexpr (CAP) {
+                    float most = 0.0f;
 #pragma unroll
                     for (int t = 0; t < 4; t++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) z[t][i] = fs_cap_any(f.score, sc[w][t][i] * f.score.in);
+                        for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(sc[w][t][i]));
+                    if (!__any(!(most < f.score.low_end))) {
+#pragma unroll
+                        for (int t = 0; t < 4; t++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) z[t][i] = fs_cap_low(f.score, sc[w][t][i], base[w]);
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < 4; t++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) z[t][i] = fs_cap_any(f.score, sc[w][t][i] * f.score.in) + base[w];
+                    }
                 } else {
 #pragma unroll
                     for (int t = 0; t < 4; t++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) z[t][i] = fs_cap_small(f.score, sc[w][t][i] * f.score.in);
+                        for (int i = 0; i < 4; i++) z[t][i] = fmaf(sc[w][t][i], f.score.in, base[w]);
                 }
-            } else {
+                if constexpr (MASK) {
+                    if (cls[0] >= kFsAdds) {
+                        if (cls[0] == kFsAdds) {
 #pragma unroll
-                for (int t = 0; t < 4; t++)
+                        for (int t = 0; t < 4; t++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) z[t][i] = sc[w][t][i] * f.score.in;
-            }
-            if constexpr (MM != 0) {
-                if (cls >= kFsAdds) {
+                            for (int i = 0; i < 4; i++) z[t][i] = fmaf((float) __builtin_bit_cast(fs_h4, mr[w][t])[i], slope[w], z[t][i]);
+                        } else {
 #pragma unroll
-                    for (int t = 0; t < 4; t++) {
-                        const fs_h4 mk = *(const fs_h4 *) &s_m[mrow[w]][16 * t + 4 * lg];
+                        for (int t = 0; t < 4; t++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float v = (float) mk[i];
-                            z[t][i] = v == -INFINITY ? -INFINITY : fmaf(v, slope[w], z[t][i]);
+                            for (int i = 0; i < 4; i++) {
+                                const float v = (float) __builtin_bit_cast(fs_h4, mr[w][t])[i];
+                                z[t][i] = v == -INFINITY ? -INFINITY : fmaf(v, slope[w], z[t][i]);
+                            }
                         }
                     }
-                }
-            } else if (cls == kFsMixed) {
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (tile * kFsTile + 16 * t + 4 * lg + i >= a.n_kv) z[t][i] = -INFINITY;
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) mx = fmaxf(mx, z[t][i]);
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float mn = fmaxf(m[w], mx);
-            const float base = mn == -INFINITY ? 0.0f : kFsUp - mn;  // a row with nothing open yet
-            const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[w] - mn);
-            m[w] = mn;
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) z[t][i] = __builtin_amdgcn_exp2f(z[t][i] + base);
-                pv[w][t] = fs_f4{z[t][0], z[t][1], z[t][2], z[t][3]};
-#pragma unroll
-                for (int i = 0; i < 4; i += 2) {
-                    const fs_h2 h = __builtin_bit_cast(fs_h2, __builtin_amdgcn_cvt_pkrtz(z[t][i], z[t][i + 1]));
-                    const fs_h2 r = __builtin_bit_cast(fs_h2, __builtin_amdgcn_cvt_pkrtz(z[t][i] - (float) h[0], z[t][i + 1] - (float) h[1]));
-                    hi[w][t >> 1][4 * (t & 1) + i] = h[0], hi[w][t >> 1][4 * (t & 1) + i + 1] = h[1];
-                    lo[w][t >> 1][4 * (t & 1) + i] = r[0], lo[w][t >> 1][4 * (t & 1) + i + 1] = r[1];
-                }
-            }
-            // the row's sum: a product with ones, every lane of the row's column gets it
-            const fs_h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
-            fs_f4 ps = {0, 0, 0, 0};
-#pragma unroll
-            for (int kk = 0; kk < 2; kk++) ps = fs_mfma(ones, hi[w][kk], fs_mfma(ones, lo[w][kk], ps));
-            l[w] = l[w] * alpha + ps[0];
-            if (__any(alpha != 1.0f)) {
-#pragma unroll
-                for (int ct = 0; ct < NT; ct++) o[w][ct] *= alpha;
-            }
-        }
-        // O^T += V^T P^T
-#pragma unroll
-        for (int kk = 0; kk < 2; kk++)
-#pragma unroll
-            for (int ct = 0; ct < NT; ct++) {
-                const _Float16 * vrow = &s_vt[16 * ct + l16][32 * kk + 4 * lg];
-                const fs_h4 v0 = *(const fs_h4 *) vrow, v1 = *(const fs_h4 *) (vrow + 16);
-                const fs_h8 va = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-#pragma unroll
-                for (int w = 0; w < RW; w++) o[w][ct] = fs_mfma(va, hi[w][kk], fs_mfma(va, lo[w][kk], o[w][ct]));
-            }
-        if (odd_rows) {
-            // V rows that are not finite: for the rows that see them alone
-            const uint64_t bad = s_bad;
-            for (int p = 0; p < kFsTile; p++) {
-                if (!((bad >> p) & 1)) continue;
-#pragma unroll
-                for (int w = 0; w < RW; w++) {
-                    float mine = 0.0f;
+                } else if (cls[0] == kFsMixed) {
 #pragma unroll
                     for (int t = 0; t < 4; t++)
 #pragma unroll
                         for (int i = 0; i < 4; i++)
-                            if (t == p >> 4 && i == (p & 3)) mine = pv[w][t][i];
-                    const float pp = __shfl(mine, 16 * ((p & 15) >> 2) + l16);
-                    bool sees = true;
-                    if constexpr (MM != 0) sees = s_m[mrow[w]][p] != kFsNegInf;
-                    if (!sees) continue;
-                    const char * vrow = vbase + (int64_t) (tile * kFsTile + p) * a.v_nb1;
+                            if (tile[0] * kFsTile + 16 * t + 4 * lg + i >= a.n_kv) z[t][i] = -INFINITY;
+                }
+                float mx = -INFINITY;
 #pragma unroll
-                    for (int ct = 0; ct < NT; ct++) {
-                        const fs_h8 v8 = *(const fs_h8 *) (vrow + 2 * (16 * ct + 8 * (lg >> 1)));
-                        if (!fs_odd(__builtin_bit_cast(fs_u4, v8))) continue;  // it is in s_vt
+                for (int t = 0; t < 4; t++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) o[w][ct][i] = fmaf(pp, (float) (lg & 1 ? v8[4 + i] : v8[i]), o[w][ct][i]);
+                    for (int i = 0; i < 4; i++) mx = fmaxf(mx, z[t][i]);
+                // (a sum of 0: no score yet. The first one's exponential is 2^kFsUp)
+                if (__any(mx > kFsUp + kFsOver || (l[w] == 0.0f && mx != -INFINITY))) {
+                    const float most = fs_max4(mx);
+                    const bool first = l[w] == 0.0f;
+                    const float by = (first && most != -INFINITY) || most > kFsUp + kFsOver ? kFsUp - most : 0.0f;
+                    const float alpha = first ? 1.0f : __builtin_amdgcn_exp2f(by);
+                    base[w] += by;
+                    l[w] *= alpha;
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) z[t][i] += by;
+#pragma unroll
+                    for (int ct = 0; ct < NT; ct++) o[w][ct] *= alpha;
+                }
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) z[t][i] = __builtin_amdgcn_exp2f(z[t][i]);
+#pragma unroll
+                    for (int i = 0; i < 4; i += 2) {
+                        const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(z[t][i], z[t][i + 1]));
+                        const fs_h2 hh = __builtin_bit_cast(fs_h2, h);
+                        const fs_h2 r = __builtin_bit_cast(fs_h2, __builtin_amdgcn_cvt_pkrtz(fs_less_low(z[t][i], h), fs_less_high(z[t][i + 1], h)));
+                        hi[w][t >> 1][4 * (t & 1) + i] = hh[0], hi[w][t >> 1][4 * (t & 1) + i + 1] = hh[1];
+                        lo[w][t >> 1][4 * (t & 1) + i] = r[0], lo[w][t >> 1][4 * (t & 1) + i + 1] = r[1];
                     }
                 }
             }
-            __syncthreads();
-            if (tid == 0) s_bad = 0;
+            if constexpr (GRP == 0) landed(tile[0], cls[0], par);
+            fs_phase_end();
+            if (n_open > 1) issue_mask(tile[1], cls[1]);
+            if (cls[0] == kFsMixed && s_bad[par] != 0) {
+                // V rows that are not finite: for the rows that see them alone
+                const uint64_t bad = s_bad[par];
+                for (int p = 0; p < kFsTile; p++) {
+                    if (!((bad >> p) & 1)) continue;
+#pragma unroll
+                    for (int w = 0; w < RW; w++) {
+                        float mine = 0.0f;
+#pragma unroll
+                        for (int t = 0; t < 4; t++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                if (t == p >> 4 && i == (p & 3)) mine = (float) hi[w][t >> 1][4 * (t & 1) + i] + (float) lo[w][t >> 1][4 * (t & 1) + i];
+                        const float pp = __shfl(mine, 16 * ((p & 15) >> 2) + l16);
+                        if constexpr (MASK) {
+                            if (((const uint16_t *) mrow[w])[tile[0] * kFsTile + p] == kFsNegInf) continue;
+                        }
+                        const char * vrow = vbase + (int64_t) (tile[0] * kFsTile + p) * a.v_nb1;
+#pragma unroll
+                        for (int ct = 0; ct < NT; ct++) {
+                            const fs_h8 v8 = *(const fs_h8 *) (vrow + 2 * (16 * ct + 8 * (lg >> 1)));
+                            if (!fs_odd(__builtin_bit_cast(fs_u4, v8))) continue;  // it is in LDS
+#pragma unroll
+                            for (int i = 0; i < 4; i++) o[w][ct][i] = fmaf(pp, (float) (lg & 1 ? v8[4 + i] : v8[i]), o[w][ct][i]);
+                        }
+                    }
+                }
+            }
+            if (tid == 0) s_bad[par ^ 1] = 0;  // read to the end, and not yet of tile t + 1
+            // (behind the last tile V of the last but one is requested again, and K of none read)
+            products(s_kv[1][par], s_kv[0][par ^ 1], std::integral_constant<int, 0>{}, std::integral_constant<bool, GRP == 0>{}, tile[1], par ^ 1);
+            if constexpr (GRP == 1) __builtin_amdgcn_s_waitcnt(0x0F70);  // K of tile t + 2
+            if (GRP == 0 || n_open > 1) fs_phase_end();
+            tile[0] = tile[1], cls[0] = cls[1], tile[1] = tile[2], cls[1] = cls[2];
         }
-        tile = nxt;
-        cls = nxt_cls;
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // (the last requests, before the workgroup's LDS is given back)
+    };
+    if (n_open > 0) {
+        if (grp == 0) run(std::integral_constant<int, 0>{});
+        else run(std::integral_constant<int, 1>{});
     }
 
 #pragma unroll
     for (int w = 0; w < RW; w++) {
         const int r = 16 * (RW * wave + w) + l16;
-        if (f.split > 1) {
-            // partials of split z: O unnormalised, then (m, l), a workgroup row
-            const int64_t rows = (int64_t) n_blk * R;
+        if (pieces > 1) {
+            // partials of piece z: O unnormalised, then (m, l), a workgroup row
+            const int64_t rows = (int64_t) gridDim.x * R;
             const int64_t pr = (((int64_t) hs * f.q_blocks + qb) * f.split + z) * R + r;
 #pragma unroll
             for (int ct = 0; ct < NT; ct++) *(fs_f4 *) &f.part[pr * D + 16 * ct + 4 * lg] = o[w][ct];
-            if (lg == 0) *(float2 *) &f.part[rows * D + 2 * pr] = make_float2(m[w], l[w]);
+            if (lg == 0) *(float2 *) &f.part[rows * D + 2 * pr] = make_float2(l[w] == 0.0f ? -INFINITY : kFsUp - base[w], l[w]);
         } else if (r / f.g < nq) {
             float * op = f.out + (((int64_t) seq * a.n_q + q0 + r / f.g) * a.hq + kvh * f.g + r % f.g) * D;
 #pragma unroll
@@ -459,22 +658,25 @@ __global__ __launch_bounds__(256) void k_fattn_join(fs_join f) {
     const int head = (int) (rc % f.hq), q = (int) (rc / f.hq % f.n_q), seq = (int) (rc / ((int64_t) f.hq * f.n_q));
     const int64_t blk = ((int64_t) seq * (f.hq / f.g) + head / f.g) * f.q_blocks + q / f.qpw;
     const int64_t p0 = blk * f.split * f.R + (q % f.qpw) * f.g + head % f.g;
+    const int split = f.pieces ? f.pieces[blk] : f.split;
+    const bool whole = f.pieces && split == 1;  // written by its one piece
+    if (LN == 1 && whole) return;
     const float * ml = f.part + f.partials * D;
     float M = -INFINITY, L = 0.0f;
     fs_f4 acc = {0, 0, 0, 0};
-    for (int z0 = ln; z0 < f.split; z0 += 4 * LN) {
+    for (int z0 = ln; z0 < split; z0 += 4 * LN) {
         float2 v[4];
         fs_f4 x[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const int64_t p = p0 + (int64_t) min(z0 + k * LN, f.split - 1) * f.R;
+            const int64_t p = p0 + (int64_t) min(z0 + k * LN, split - 1) * f.R;
             v[k] = *(const float2 *) &ml[2 * p];
             x[k] = *(const fs_f4 *) &f.part[p * D + d];
         }
         float most = M;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            if (z0 + k * LN >= f.split) v[k] = make_float2(-INFINITY, 0.0f);
+            if (z0 + k * LN >= split) v[k] = make_float2(-INFINITY, 0.0f);
             most = fmaxf(most, v[k].x);
         }
         const float w0 = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - most);
@@ -508,36 +710,35 @@ __global__ __launch_bounds__(256) void k_fattn_join(fs_join f) {
             for (int i = 0; i < 4; i++) acc[i] = fmaf(w, x[i], acc[i]);
         }
     }
-    if (row < f.rows) *(fs_f4 *) &f.out[row * D + d] = L != 0.0f ? acc / L : fs_f4{0, 0, 0, 0};
+    if (row < f.rows && !whole) *(fs_f4 *) &f.out[row * D + d] = L != 0.0f ? acc / L : fs_f4{0, 0, 0, 0};
 }
 
 size_t fs_al(size_t v) { return (v + 255) & ~(size_t) 255; }
 
-int fs_rw(const fattn_args & a) {
-    // rows of a workgroup: 128, where a kv head has more than 64
-    return a.d != 256 && (int64_t) a.n_q * (a.hq / a.hkv) > 64 ? 2 : 1;
-}
+// Rows of a workgroup: 16 a wave, or 32 (each fragment of K and V read once for
+// them) where a kv head has more than 128; for heads of 256 the outputs of 32
+// would take half of the registers
+int fs_rows(const fattn_args & a) { return a.d != 256 && (int64_t) a.n_q * (a.hq / a.hkv) > 128 ? 256 : 128; }
 
 // the launch's shape, and its scratch: the tiles' classes, then the splits' partials
 size_t fs_plan(const fattn_args & a, fs_args & f) {
     f = fs_args{};
     f.a = a;
-    const int R = 64 * fs_rw(a);
+    const int R = fs_rows(a);
     f.g = a.hq / a.hkv;
     f.qpw = std::min(R / f.g, a.n_q);
     f.q_blocks = (a.n_q + f.qpw - 1) / f.qpw;
     f.n_tiles = (a.n_kv + kFsTile - 1) / kFsTile;
     f.split = std::max(1, a.scored_split);
-    f.per = (f.n_tiles + f.split - 1) / f.split;
-    f.split = (f.n_tiles + f.per - 1) / f.per;
+    f.slots = a.scored_slots;
     f.heads_mask = a.mask && a.m_ne2 > 1;
     f.score = fs_score_of(a);
     size_t need = 0;
     if (a.mask) {
-        const size_t n = (size_t) a.m_ne3 * (f.heads_mask ? a.hkv : 1) * f.q_blocks * f.n_tiles;
-        need = fs_al(8 * n) + fs_al(n);
+        f.n_cls = (int64_t) a.m_ne3 * (f.heads_mask ? a.hkv : 1) * f.q_blocks * f.n_tiles;
+        need = fs_al(8 * f.n_cls) + fs_al(f.n_cls);
     }
-    if (f.split > 1) need += sizeof(float) * (size_t) a.n_seq * a.hkv * f.q_blocks * f.split * R * (a.d + 2);
+    if (f.split > 1) need += fs_al(sizeof(int) * (size_t) a.n_seq * a.hkv * f.q_blocks) + sizeof(float) * (size_t) a.n_seq * a.hkv * f.q_blocks * f.split * R * (a.d + 2);
     return need;
 }
 
@@ -551,14 +752,15 @@ bool fattn_scored_supported(const fattn_args & a) {
 
 void fattn_scored_plan(fattn_args & a, int n_cu) {
     if (fattn_scored_dec_supported(a)) return fattn_scored_dec_plan(a, n_cu);
-    // splits of the span while one sequence's query blocks leave CUs idle: two
-    // workgroups a CU, at least four tiles a split. By one sequence's shape, so
-    // that its rows get the same bits alone or in a batch
-    const int R = 64 * fs_rw(a), g = a.hq / a.hkv, qpw = std::min(R / g, std::max(1, a.n_q));
-    const int64_t base = (int64_t) ((a.n_q + qpw - 1) / qpw) * a.hkv;
+    // Pieces of a query block's open tiles where query blocks leave CUs idle. How
+    // many a block gets is for the launch to say; at most twice as many as an even
+    // split over the card would need, so that a causal mask's long blocks get theirs
+    const int R = fs_rows(a), g = a.hq / a.hkv, qpw = std::min(R / g, std::max(1, a.n_q));
+    const int64_t units = std::max<int64_t>(1, (int64_t) ((a.n_q + qpw - 1) / qpw) * a.hkv * a.n_seq);
     const int n_tiles = (a.n_kv + kFsTile - 1) / kFsTile;
     a.scored = 1;
-    a.scored_split = (int) std::max<int64_t>(1, std::min<int64_t>((2 * n_cu + base - 1) / std::max<int64_t>(1, base), n_tiles / 4));
+    a.scored_slots = n_cu;
+    a.scored_split = (int) std::max<int64_t>(1, std::min<int64_t>(units >= a.scored_slots ? 1 : 2 * a.scored_slots / units, n_tiles / 4));
 }
 
 size_t fattn_scored_scratch_bytes(const fattn_args & a) {
@@ -574,44 +776,43 @@ void launch_fattn_scored(const fattn_args & a, void * scratch, float * out, hipS
     fs_plan(a, f);
     f.out = out;
     char * p = (char *) scratch;
-    const bool v16 = (((uintptr_t) a.mask | (uintptr_t) a.m_nb1 | (uintptr_t) a.m_nb2 | (uintptr_t) a.m_nb3) & 15) == 0;
     if (a.mask) {
-        const int64_t n = (int64_t) a.m_ne3 * (f.heads_mask ? a.hkv : 1) * f.q_blocks * f.n_tiles;
+        const int64_t n = f.n_cls;
         f.seen = (uint64_t *) p;
         f.cls = (uint8_t *) (p + fs_al(8 * (size_t) n));
         p += fs_al(8 * (size_t) n) + fs_al((size_t) n);
-        const dim3 grid((unsigned) ((n + 3) / 4));
-        if (v16) hipLaunchKernelGGL(k_fattn_tiles<true>, grid, dim3(256), 0, s, f, n);
-        else hipLaunchKernelGGL(k_fattn_tiles<false>, grid, dim3(256), 0, s, f, n);
+        hipLaunchKernelGGL(k_fattn_tiles, dim3((unsigned) n), dim3(256), 0, s, f);
         note_hip_error(hipGetLastError());
     }
+    f.pieces = (int *) p;
+    if (f.split > 1) p += fs_al(sizeof(int) * (size_t) a.n_seq * a.hkv * f.q_blocks);
     f.part = (float *) p;
-    const int rw = fs_rw(a);
+    const int rows = fs_rows(a);
     const dim3 grid((unsigned) ((int64_t) f.q_blocks * a.hkv * a.n_seq * f.split));
-    auto go = [&](auto d, auto w, auto cap) {
-        constexpr int D = decltype(d)::value, RW = decltype(w)::value;
-        constexpr bool CAP = decltype(cap)::value;
-        if (!a.mask) hipLaunchKernelGGL((k_fattn_scored<D, RW, CAP, 0>), grid, dim3(kFsThreads), 0, s, f);
-        else if (v16) hipLaunchKernelGGL((k_fattn_scored<D, RW, CAP, 1>), grid, dim3(kFsThreads), 0, s, f);
-        else hipLaunchKernelGGL((k_fattn_scored<D, RW, CAP, 2>), grid, dim3(kFsThreads), 0, s, f);
+    auto go = [&](auto d, auto rw) {
+        constexpr int D = decltype(d)::value, RW = decltype(rw)::value;
+        if (a.softcap > 0.0f) {
+            if (a.mask) hipLaunchKernelGGL((k_fattn_scored<D, RW, true, true>), grid, dim3(512), 0, s, f);
+            else hipLaunchKernelGGL((k_fattn_scored<D, RW, true, false>), grid, dim3(512), 0, s, f);
+        } else {
+            if (a.mask) hipLaunchKernelGGL((k_fattn_scored<D, RW, false, true>), grid, dim3(512), 0, s, f);
+            else hipLaunchKernelGGL((k_fattn_scored<D, RW, false, false>), grid, dim3(512), 0, s, f);
+        }
     };
-    auto rows = [&](auto d, auto w) {
-        if (a.softcap > 0.0f) go(d, w, std::true_type{});
-        else go(d, w, std::false_type{});
+    auto width = [&](auto d) {
+        constexpr int wide = decltype(d)::value == 256 ? 1 : 2;
+        if (rows == 256) go(d, std::integral_constant<int, wide>{});
+        else go(d, std::integral_constant<int, 1>{});
     };
-    using one = std::integral_constant<int, 1>;
-    using two = std::integral_constant<int, 2>;
-    if (a.d == 256) rows(std::integral_constant<int, 256>{}, one{});
-    else if (a.d == 128 && rw == 2) rows(std::integral_constant<int, 128>{}, two{});
-    else if (a.d == 128) rows(std::integral_constant<int, 128>{}, one{});
-    else if (rw == 2) rows(std::integral_constant<int, 64>{}, two{});
-    else rows(std::integral_constant<int, 64>{}, one{});
+    if (a.d == 256) width(std::integral_constant<int, 256>{});
+    else if (a.d == 128) width(std::integral_constant<int, 128>{});
+    else width(std::integral_constant<int, 64>{});
     note_hip_error(hipGetLastError());
     if (f.split > 1) {
         fs_join j{};
-        j.part = f.part, j.out = out, j.rows = (int64_t) a.n_seq * a.n_q * a.hq;
-        j.partials = (int64_t) a.n_seq * a.hkv * f.q_blocks * f.split * 64 * rw;
-        j.split = f.split, j.d = a.d, j.hq = a.hq, j.n_q = a.n_q, j.g = f.g, j.qpw = f.qpw, j.q_blocks = f.q_blocks, j.R = 64 * rw;
+        j.part = f.part, j.pieces = f.pieces, j.out = out, j.rows = (int64_t) a.n_seq * a.n_q * a.hq;
+        j.partials = (int64_t) a.n_seq * a.hkv * f.q_blocks * f.split * rows;
+        j.split = f.split, j.d = a.d, j.hq = a.hq, j.n_q = a.n_q, j.g = f.g, j.qpw = f.qpw, j.q_blocks = f.q_blocks, j.R = rows;
         launch_fattn_join(j, s);
     }
 }

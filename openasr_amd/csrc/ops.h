@@ -232,7 +232,8 @@ struct fattn_args {
     // and the mask is added times a slope a head for a max_bias above 0
     float softcap, max_bias;
     int scored;        // this form takes the attention
-    int scored_split;  // its KV splits (> 1: partials, joined by a launch)
+    int scored_split;  // the most KV splits a row gets (> 1: partials, joined by a launch)
+    int scored_slots;  // many queries: workgroups that the card holds at once
 };
 bool fattn_scored_supported(const fattn_args & a);
 void fattn_scored_plan(fattn_args & a, int n_cu);
