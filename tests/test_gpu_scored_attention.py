@@ -70,6 +70,8 @@ def make_mask(kind, S, H, Q, N, bias, rng):
         m = np.where(doc[None] == doc[np.minimum(i, N - 1)[:, 0]][:, None], m, -np.inf)[None, None]
     elif kind == "prefix":  # all see the first part, the rest is causal
         m = np.where(j < N // 3, dist, m)[None, None]
+    elif kind == "window":  # the first 100 positions and the last 200, beside the causal mask
+        m = np.where((j < 100) | (j > i - 200), m, -np.inf)[None, None]
     elif kind == "empty":  # rows that see nothing, in one sequence a whole block of them
         m = np.repeat(m[None, None], S, 0)
         m[:, :, rng.random(Q) < 0.3] = -np.inf
@@ -172,6 +174,64 @@ def test_scored_attention(ggml, gpu, D, H, G, Q, N, S, kind, cap, bias):
     want, bound = attention64(q, k, v, mask, scale, cap, bias)
     for prec in (None, ggml.GGML_PREC_F32):
         check(attention(ggml, gpu, q, k, v, mask, scale, cap, bias, prec), want, bound, f"prec {prec}")
+
+
+#        D    H   G  Q    N     S  mask        cap   bias
+LONG = [(128, 8, 8, 100, 5000, 1, "window", 30.0, 0.0),  # tiles seen lie more than 64 apart
+        (64, 16, 8, 40, 9001, 1, "window", 0.0, 8.0),
+        (128, 16, 8, 300, 1200, 1, "causal", 50.0, 0.0),  # several blocks of 256 rows, in pieces
+        (64, 8, 8, 700, 700, 2, "causal", 0.0, 8.0),
+        (256, 8, 2, 200, 1000, 1, "prefix", 50.0, 0.0),
+        (128, 3, 3, 500, 2000, 1, "none", 50.0, 0.0),
+        (128, 64, 1, 5, 3000, 2, "random", 30.0, 8.0),
+        (64, 8, 8, 300, 300, 3, "empty", 50.0, 0.0),
+        (256, 8, 8, 130, 700, 2, "heads", 30.0, 8.0)]
+
+
+@pytest.mark.parametrize("D,H,G,Q,N,S,kind,cap,bias", LONG)
+def test_long_spans(ggml, gpu, D, H, G, Q, N, S, kind, cap, bias):
+    print(f"long span D={D} H={H} G={G} Q={Q} N={N} S={S} {kind} cap={cap} bias={bias}", flush=True)
+    rng = np.random.default_rng(D + H + Q + N)
+    q, k, v = operands(rng, S, H, G, Q, N, D, std=2.0)
+    mask = make_mask(kind, S, H, Q, N, bias, rng)
+    want, bound = attention64(q, k, v, mask, 1 / np.sqrt(D), cap, bias)
+    check(attention(ggml, gpu, q, k, v, mask, 1 / np.sqrt(D), cap, bias), want, bound)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("cap", [0.0, 200.0])
+def test_maxima_that_grow(ggml, gpu, D, cap):
+    """each tile's scores lie far over the last one's, in half of the rows far under them"""
+    rng = np.random.default_rng(D)
+    Q, N, H = 150, 700, 2
+    q, k, v = operands(rng, 1, H, 1, Q, N, D)
+    q[..., 0] = np.where(np.arange(Q) % 2, -1.0, 1.0)[None, None]
+    k[..., 0] = (np.arange(N) / 4).astype(np.float16)
+    mask = make_mask("causal", 1, H, Q, N, 0.0, rng)
+    want, bound = attention64(q, k, v, mask, 1.0, cap, 0.0)
+    check(attention(ggml, gpu, q, k, v, mask, 1.0, cap, 0.0), want, bound)
+
+
+@pytest.mark.parametrize("D,Q", [(64, 300), (128, 300), (256, 150)])
+def test_values_not_finite_in_later_tiles(ggml, gpu, D, Q):
+    """an infinite value reaches the rows that see it, in its dims, and no others"""
+    rng = np.random.default_rng(D + Q)
+    N, H = Q, 2
+    q, k, v = operands(rng, 1, H, 2, Q, N, D)
+    clean = v.copy()
+    spots = [(0, 70, 3, np.inf), (1, 130, D - 1, -np.inf), (0, 140, 17, np.nan), (0, N - 1, 40, np.inf)]
+    for g, n, d, x in spots:
+        v[0, g, n, d] = x
+        clean[0, g, n, d] = 0
+    mask = make_mask("causal", 1, H, Q, N, 0.0, rng)
+    got = attention(ggml, gpu, q, k, v, mask, 0.1, 30.0, 0.0)
+    hit = np.zeros(got.shape, bool)
+    for g, n, d, x in spots:
+        hit[0, n:, g, d] = True
+        sign = got[0, n:, g, d]
+        assert np.isnan(sign).all() if np.isnan(x) else (sign == x).all(), (g, n, d)
+    want, bound = attention64(q, k, clean, mask, 0.1, 30.0, 0.0)
+    check(np.where(hit, 0, got), np.where(hit, 0, want), bound)
 
 
 @pytest.mark.parametrize("Q,N", [(1, 200), (40, 200)])
