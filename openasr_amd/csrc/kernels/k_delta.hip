@@ -225,8 +225,12 @@ __global__ __launch_bounds__(256) void k_delta_rows(delta_args a) {
 
 constexpr int kDlC = 64;
 // what the products take: q's and k's rows as they come, and (the largest element of a
-// row) brought to length; beta; T; scaled values. The state and v: up to 2^40
-constexpr float kDlRaw = 0x1p50f, kDlRow = 0x1p10f, kDlLeast = 0x1p-20f, kDlBeta = 16.0f, kDlT = 0x1p20f, kDlHalf = 60000.0f;
+// row) brought to length (the state of keys much shorter than one lies far under v, in
+// whose scale it is split: keys of 1e-4 were 2e-3 off); beta; a row of |T| (1 to 3 for
+// keys of length one and beta up to one; tokens of one key with a beta of 2, which turn
+// the state over and over, come to 127, and were 4e-4 off); scaled values. The state
+// and v: up to 2^40
+constexpr float kDlRaw = 0x1p50f, kDlRow = 0x1p10f, kDlLeastQ = 0x1p-20f, kDlLeastK = 0x1p-7f, kDlBeta = 16.0f, kDlRowSum = 64.0f, kDlHalf = 60000.0f;
 
 struct dl_chunk_args {
     delta_args a;
@@ -349,7 +353,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_solve(dl_chunk_args q) {
         most *= f;
         most = fmaxf(most, __shfl_xor(most, 16));
         most = fmaxf(most, __shfl_xor(most, 32));
-        bad |= dl_past(most, kDlRow) || (most > 0.0f && most < kDlLeast);
+        bad |= dl_past(most, kDlRow) || (most > 0.0f && most < kDlLeastQ);
         const float sc = dl_pow2(13 - dl_exponent(most));
         dl_u4 * o = (dl_u4 *) (krec + dl_krec<NP>::q) + wave * (KB / 2) * 128 + lane;
 #pragma unroll
@@ -383,7 +387,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_solve(dl_chunk_args q) {
         most *= f;
         most = fmaxf(most, __shfl_xor(most, 1));
         most = fmaxf(most, __shfl_xor(most, 2));
-        bad |= dl_past(most, kDlRow) || (most > 0.0f && most < kDlLeast);
+        bad |= dl_past(most, kDlRow) || (most > 0.0f && most < kDlLeastK);
         if ((tid & 3) == 0) s_kexp[t] = dl_pow2(13 - dl_exponent(most));
     }
     bad = __syncthreads_or(bad);
@@ -532,29 +536,31 @@ __global__ __launch_bounds__(256, 2) void k_delta_solve(dl_chunk_args q) {
             x[i] = dl_mfma(inv[i], r, dl_v4f{0, 0, 0, 0});
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                own_bad |= dl_past(x[i][e], kDlT);
                 s_t[16 * i + 4 * lg + e][16 * wave + l16] = x[i][e];
             }
         }
-        own_bad = __syncthreads_or(own_bad);
+        __syncthreads();
         {
             dl_v4f v[4];
-            float most = 0.0f;
+            float most = 0.0f, sum = 0.0f;
 #pragma unroll
             for (int sb = 0; sb < 4; sb++) {
                 v[sb] = dl_v4f{0, 0, 0, 0};
                 if (sb <= wave) v[sb] = *(const dl_v4f *) &s_t[16 * wave + l16][16 * sb + 4 * lg];
 #pragma unroll
-                for (int e = 0; e < 4; e++) most = fmaxf(most, fabsf(v[sb][e]));
+                for (int e = 0; e < 4; e++) most = fmaxf(most, fabsf(v[sb][e])), sum += fabsf(v[sb][e]);
             }
             most = fmaxf(most, __shfl_xor(most, 16));
             most = fmaxf(most, __shfl_xor(most, 32));
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            own_bad |= dl_past(sum, kDlRowSum);
             const float sc = dl_pow2(13 - dl_exponent(most));
             put_rows((dl_u4 *) (rec + dl_rec::t), v, sc);
             if (lg == 0) ((float *) (rec + dl_rec::t_row))[16 * wave + l16] = 1.0f / sc;
         }
+        own_bad = __syncthreads_or(own_bad);  // (and the next head's A lies over it)
         if (tid == 0) ((int *) (rec + dl_rec::end))[2] = own_bad;
-        __syncthreads();  // (the next head's A lies over it)
     }
 }
 

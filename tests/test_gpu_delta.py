@@ -308,3 +308,43 @@ def test_l2_norm(ggml, gpu, n, rows, strided):
         # the sum's rounding to f32, the root, the quotient, the product
         within(G.get(y).reshape(rows, n), want, 5 * U * np.abs(want) + 1e-37)
     G.free()
+
+
+@pytest.mark.parametrize("T", [20, 200, 500])
+@pytest.mark.parametrize("K", [64, 128])
+@pytest.mark.parametrize("case", ["short", "of many lengths", "long", "one key, beta two"])
+def test_keys_of_other_lengths(ggml, gpu, T, K, case):
+    """keys that are not of length one: a state far under v, corrections that turn it over"""
+    V, H = 48, 2
+    q, k, v, g, beta, st = inputs(K, V, 1, H, T, 1, seed=13)
+    q, k = unit(q).astype(np.float32), unit(k)
+    g[:] = -0.5
+    if case == "short":
+        k = k * 1e-4
+    if case == "of many lengths":
+        k = k * np.exp(-8 * np.random.default_rng(1).random((1, T, 1, 1)))
+    if case == "long":
+        k = k * 1.4
+    if case == "one key, beta two":
+        k = np.repeat(k[:, :1], T, 1)
+        beta[:], g[:] = 2.0, -0.125
+    k = k.astype(np.float32)
+    want, end, d, before = rule64(q, k, v, g, beta, st)
+    G, y, _, _ = graph(ggml, gpu, q, k, v, g, beta, st, norm=False)
+    # |1 - beta k k^T| <= 1 here, so an error made at a token is left, s tokens on, at most e^(g s) times
+    # as long: the sum of what 2 K + 100 roundings a token make of the old state, its product with k, d
+    # and its own. A chunk's tokens come through |(1 + A)^-1|, rows of at most 64, or else one by one
+    turns = 64 if case == "one key, beta two" else 4
+    decay, e = np.exp(np.float64(g[0, 0, 0, 0])), np.zeros((1, H, V))
+    by = np.zeros_like(want)
+    for t in range(T):
+        lk = np.sqrt((k[:, t].astype(np.float64) ** 2).sum(2))[..., None]
+        made = np.sqrt((before[:, t] ** 2).sum(3)) * decay + np.abs(d[:, t]) * lk + np.abs(beta[:, t, :, None] * v[:, t]) * lk
+        e = e * decay + turns * (2 * K + 100) * U * made
+        by[:, t] = (e + (2 * K + 100) * U * made) / np.sqrt(K)
+    for _ in range(2):
+        assert G.compute(gpu.backend) == 0
+        got, states = parts(G, y, 1, T, H, V, K)
+        within(got, want, by + 1e-37, "y")
+        within(states, end, e[..., None] + 1e-37, "states")
+    G.free()
