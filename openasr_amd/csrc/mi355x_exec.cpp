@@ -1596,6 +1596,10 @@ bool planner::make_fattn(const ggml_tensor * t, fattn_args & a) {
         return fail(t, "K/V not 16-byte aligned");
     a.max_bias = op_f32(t, 1), a.softcap = op_f32(t, 2);
     if (fattn_scored(t)) {
+        fattn_args rows = a;  // (as they are read: behind a folded expansion, or as contiguous copies)
+        if (k->type == GGML_TYPE_F32) rows.k_nb1 = rows.k_nb2 = rows.k_nb3 = 0;
+        if (v->type == GGML_TYPE_F32) rows.v_nb1 = rows.v_nb2 = rows.v_nb3 = 0;
+        if (vv.ne[3] != kv.ne[3] || !fattn_scored_supported(rows)) return fail(t, "K / V layout");
         fattn_scored_plan(a, n_cu);
         return true;
     }
@@ -3219,7 +3223,8 @@ bool supports_op(const device_state * dev, const ggml_tensor * t) {
             // (f32 K and V are read as contiguous copies)
             if (k->type == GGML_TYPE_F16) a.k_nb1 = (int64_t) k->nb[1], a.k_nb2 = (int64_t) k->nb[2], a.k_nb3 = (int64_t) k->nb[3];
             if (v->type == GGML_TYPE_F16) a.v_nb1 = (int64_t) v->nb[1], a.v_nb2 = (int64_t) v->nb[2], a.v_nb3 = (int64_t) v->nb[3];
-            return a.hkv > 0 && a.hq % a.hkv == 0 && k->ne[1] == v->ne[1] && (!m || q->ne[3] % m->ne[3] == 0) &&
+            return a.hkv > 0 && a.hq % a.hkv == 0 && k->ne[1] == v->ne[1] && k->ne[3] == v->ne[3] &&
+                   (!m || (q->ne[3] % m->ne[3] == 0 && m->ne[0] >= k->ne[1] && m->ne[1] >= q->ne[1])) &&
                    (double) q->ne[1] * (double) q->ne[2] * (double) q->ne[3] < 16777216.0 && fattn_scored_supported(a);
         }
         case GGML_OP_SOFT_MAX:
