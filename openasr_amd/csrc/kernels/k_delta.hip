@@ -189,6 +189,149 @@ __global__ __launch_bounds__(256) void k_delta_rows(delta_args a) {
     }
 }
 
+// Gates an element, many tokens. What every wave of a head would make again of a
+// token's operands is made once: q's and k's rows brought to length (q's times the
+// scale) and the decays, in rows of 64 P elements (zeros past K) [sequence][token][q of
+// the key heads, k of them, decays of the heads]. 16 lanes a row.
+template <int P>
+__global__ __launch_bounds__(256) void k_delta_ready(delta_args a, float * out) {
+    const int l = threadIdx.x & 15, rows = 2 * a.key_heads + a.heads;
+    const int64_t unit = (int64_t) blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int64_t u = min(unit, a.tokens * rows * a.seqs - 1);
+    const int r = (int) (u % rows);
+    const int64_t t = u / rows % a.tokens, s = u / rows / a.tokens;
+    const bool q = r < a.key_heads, k = !q && r < 2 * a.key_heads;
+    const char * x = q   ? a.q + r * a.q_nb1 + t * a.q_nb2 + s * a.q_nb3
+                     : k ? a.k + (r - a.key_heads) * a.k_nb1 + t * a.k_nb2 + s * a.k_nb3
+                         : a.g + (r - 2 * a.key_heads) * a.g_nb1 + t * a.g_nb2 + s * a.g_nb3;
+    dl_v4f v[P];
+    float sum = 0.0f;
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+        const int i = 4 * (l + 16 * p);
+        v[p] = dl_v4f{0, 0, 0, 0};
+        if (i < a.K) v[p] = *(const dl_v4f *) (x + 4 * i);
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum = fmaf(v[p][e], v[p][e], sum);
+    }
+    const float eps = q ? a.q_eps : a.k_eps;
+    const float by = (eps < 0.0f ? 1.0f : 1.0f / fmaxf(sqrtf(dl_sum16(sum)), eps)) * (q ? a.scale : 1.0f);
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+        const int i = 4 * (l + 16 * p);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[p][e] = q || k ? v[p][e] * by : i < a.K ? dl_exp(v[p][e]) : 0.0f;
+        if (unit == u) *(dl_v4f *) &out[u * 64 * P + i] = v[p];
+    }
+}
+
+// k_delta_rows on those rows: 16 lanes a state row, 4 U rows a wave, AHEAD tokens'
+// operands loaded ahead and no branch between them. 500 tokens of 16 heads of 128 x
+// 128: 107 us (and 8 for the rows; k_delta_rows 342), 0.21 a token, of it 190 cycles the
+// CU's two waves' loads. Waves four a workgroup, on half of the CUs: 137
+template <int P, int U>
+__global__ __launch_bounds__(64) void k_delta_steps(delta_args a, const float * ready) {
+    constexpr int AHEAD = P == 4 ? 4 : 8;
+    const int l = threadIdx.x & 15, sub = threadIdx.x >> 4;
+    const uint32_t blocks = (uint32_t) ((a.V + 4 * U - 1) / (4 * U));
+    const int64_t unit = blockIdx.x;
+    const int j0 = (int) (unit % blocks) * 4 * U + sub, h = (int) (unit / blocks % a.heads);
+    const int s = (int) (unit / ((int64_t) blocks * a.heads)), hk = h % a.key_heads, rows = 2 * a.key_heads + a.heads;
+    const int64_t step = (int64_t) rows * 64 * P;
+    const float * at = ready + s * a.tokens * step;
+    const char *v = a.v + h * a.v_nb1 + s * a.v_nb3, *b = a.beta + h * a.b_nb1 + s * a.b_nb3;
+    const int of[3] = {hk * 64 * P + 4 * l, (a.key_heads + hk) * 64 * P + 4 * l, (2 * a.key_heads + h) * 64 * P + 4 * l};
+    int v_of[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) v_of[u] = min(j0 + 4 * u, a.V - 1);
+    struct token {
+        dl_v4f q[P], k[P], g[P];
+        float beta, v[U];
+    };
+    int64_t loaded = 0;
+    auto load = [&](token & x) {  // the next token, or the last one again
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            x.q[p] = *(const dl_v4f *) (at + of[0] + 64 * p);
+            x.k[p] = *(const dl_v4f *) (at + of[1] + 64 * p);
+            x.g[p] = *(const dl_v4f *) (at + of[2] + 64 * p);
+        }
+        x.beta = *(const float *) b;
+#pragma unroll
+        for (int u = 0; u < U; u++) x.v[u] = ((const float *) v)[v_of[u]];
+        const bool more = ++loaded < a.tokens;
+        at += more ? step : 0, v += more ? a.v_nb2 : 0, b += more ? a.b_nb2 : 0;
+    };
+    token next[AHEAD];
+#pragma unroll
+    for (int n = 0; n < AHEAD; n++) load(next[n]);
+    dl_v4f st[U][P];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const char * row = a.s + s * a.s_nb3 + 4 * ((int64_t) h * a.V + v_of[u]) * a.K;
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            st[u][p] = dl_v4f{0, 0, 0, 0};
+            if (4 * (l + 16 * p) < a.K) st[u][p] = *(const dl_v4f *) (row + 16 * (l + 16 * p));
+        }
+    }
+    auto dot = [](const dl_v4f (&x)[P], const dl_v4f (&y)[P]) {
+        dl_v4f v = x[0] * y[0];
+#pragma unroll
+        for (int p = 1; p < P; p++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = fmaf(x[p][e], y[p][e], v[e]);
+        return (v[0] + v[1]) + (v[2] + v[3]);
+    };
+    const int64_t y_step = (int64_t) a.heads * a.V;
+    float * y = a.y + ((int64_t) s * a.y_tokens * a.heads + h) * a.V + j0 + l * y_step;
+    float mine[U];  // y of token l of the AHEAD
+    auto take = [&](const token & x, int n) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+#pragma unroll
+            for (int p = 0; p < P; p++) st[u][p] *= x.g[p];
+            const float d = x.beta * (x.v[u] - dl_sum16(dot(st[u], x.k)));
+#pragma unroll
+            for (int p = 0; p < P; p++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) st[u][p][e] = fmaf(x.k[p][e], d, st[u][p][e]);
+            const float r = dl_sum16(dot(st[u], x.q));
+            mine[u] = l == n ? r : mine[u];
+        }
+    };
+    // (a store a token waited for would hold back the loads that follow it)
+    auto put = [&](int n) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (l < n && j0 + 4 * u < a.V) y[4 * u] = mine[u];
+        y += AHEAD * y_step;
+    };
+#pragma unroll
+    for (int u = 0; u < U; u++) mine[u] = 0.0f;
+    int64_t t = 0;
+    for (; t + AHEAD <= a.tokens; t += AHEAD) {
+#pragma unroll
+        for (int n = 0; n < AHEAD; n++) {
+            take(next[n], n);
+            load(next[n]);
+        }
+        put(AHEAD);
+    }
+#pragma unroll
+    for (int n = 0; n < AHEAD; n++)
+        if (t + n < a.tokens) take(next[n], n);
+    put((int) (a.tokens - t));
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (j0 + 4 * u >= a.V) continue;
+        float * row = (float *) (a.out + s * a.out_nb3) + ((int64_t) h * a.V + j0 + 4 * u) * a.K;
+#pragma unroll
+        for (int p = 0; p < P; p++)
+            if (4 * (l + 16 * p) < a.K) *(dl_v4f *) (row + 4 * (l + 16 * p)) = st[u][p];
+    }
+}
+
 // ---------------------------------------------------------------- chunks ---
 //
 // Chunks of C = 64 tokens as matrix products. With a_t the sum of the chunk's g
@@ -224,6 +367,7 @@ __global__ __launch_bounds__(256) void k_delta_rows(delta_args a) {
 // zero, say, and meets v: the second such chunk has its scale).
 
 constexpr int kDlC = 64;
+constexpr int kDlReady = 32;
 // what the products take: q's and k's rows as they come, and (the largest element of a
 // row) brought to length (the state of keys much shorter than one lies far under v, in
 // whose scale it is split: keys of 1e-4 were 2e-3 off); beta; a row of |T| (1 to 3 for
@@ -934,10 +1078,21 @@ static bool dl_chunked(const delta_args & a) {
            a.v_nb2 >= 0 && a.v_nb2 < 1 << 25 && (int64_t) a.heads * a.V < 1 << 23;  // (a lane's rows of v and y in 32-bit offsets)
 }
 
+// k_delta_ready's tokens a slab; 0: it is not worth its launch (32 tokens, 16 heads of
+// 128, 26 us without and 14 with), or has no room
+static int dl_pieces(const delta_args & a) { return a.K <= 64 ? 1 : a.K <= 128 ? 2 : 4; }  // of 64 elements a row
+static int64_t dl_ready_bytes(const delta_args & a) { return 256ll * dl_pieces(a) * (2 * a.key_heads + a.heads) * a.seqs; }
+static int64_t dl_ready_slab(const delta_args & a) {
+    if (!a.g_elem || a.tokens < kDlReady) return 0;
+    const int64_t room = std::min(kDeltaScratch, a.scratch_bytes) / dl_ready_bytes(a);
+    return room < kDlReady ? 0 : std::min(room, a.tokens);
+}
+
 size_t delta_scratch_bytes(const delta_args & a, int n_cu) {
     (void) n_cu;
     // (a graph planned before it is allocated: the addresses may still allow chunks)
-    if (a.g_elem || a.tokens < 24 || a.K < 16) return 0;
+    if (a.g_elem) return (size_t) (dl_ready_slab(a) * dl_ready_bytes(a));
+    if (a.tokens < 24 || a.K < 16) return 0;
     return (size_t) (dl_slab(a) * dl_chunk_size(a));
 }
 
@@ -974,24 +1129,49 @@ static void launch_delta_rows(const delta_args & a, hipStream_t s) {
     note_hip_error(hipGetLastError());
 }
 
+// gates an element, many tokens: slabs of k_delta_ready's rows, the state handed on.
+// us of U = 1 / 2, 500 tokens of 16 heads of 128 x 128: one sequence 113 / 145, two 146 /
+// 156, four 218 / 164, eight 428 / 325
+template <int P, int U>
+static void launch_delta_ready(const delta_args & a, void * scratch, hipStream_t s) {
+    const int64_t slab = dl_ready_slab(a);
+    delta_args b = a;
+    for (int64_t t0 = 0; t0 < a.tokens; t0 += slab) {
+        b.q = a.q + t0 * a.q_nb2, b.k = a.k + t0 * a.k_nb2, b.g = a.g + t0 * a.g_nb2;
+        b.tokens = std::min(slab, a.tokens - t0);
+        const int64_t rows = b.tokens * (2 * a.key_heads + a.heads) * a.seqs;
+        hipLaunchKernelGGL(k_delta_ready<P>, dim3((unsigned) ((rows + 15) / 16)), dim3(256), 0, s, b, (float *) scratch);
+        note_hip_error(hipGetLastError());
+        b.v = a.v + t0 * a.v_nb2, b.beta = a.beta + t0 * a.b_nb2, b.y = a.y + t0 * a.heads * a.V;
+        const int64_t units = (int64_t) ((a.V + 4 * U - 1) / (4 * U)) * a.heads * a.seqs;
+        hipLaunchKernelGGL((k_delta_steps<P, U>), dim3((unsigned) units), dim3(64), 0, s, b, (const float *) scratch);
+        note_hip_error(hipGetLastError());
+        b.s = a.out, b.s_nb3 = a.out_nb3;
+    }
+}
+
 // A wave takes 4 U rows: few where that leaves waves a SIMD, many where there
 // are enough anyhow (the token's work beside the rows is shared). 32 heads of 128
 // x 128, us, U = 1 / 2 / 4: 8 tokens of one sequence 7.9 / 8.7 / 11.5, of 16 37 /
-// 30 / 30; one token of 48 34 / 35 / 34; 500 tokens with gates an element, 16
-// heads of one sequence 365 / 384 / 511, of four 462 / 385 / 505. Four tokens'
-// operands ahead instead of one's take 342 of the 365 us, and more where tokens
-// are few (one token of 48 sequences: 64 for 34 us).
+// 30 / 30; one token of 48 34 / 35 / 34. Four tokens' operands ahead instead of
+// one's: 500 tokens with gates an element 342 for 365, and more where tokens are
+// few (one token of 48 sequences 64 for 34).
 template <int P>
-static void launch_delta_tokens(const delta_args & a, hipStream_t s, int n_cu) {
+static void launch_delta_tokens(const delta_args & a, void * scratch, hipStream_t s, int n_cu) {
     const int64_t rows = (int64_t) a.V * a.heads * a.seqs, enough = 16 * (int64_t) n_cu;  // four waves a CU, of 4 rows
-    if (!dl_vec(a)) launch_delta_rows<P, 2, 1, false>(a, s);
+    if (dl_vec(a) && dl_ready_slab(a) > 0) {
+        if (rows >= 2 * enough) launch_delta_ready<P, 2>(a, scratch, s);
+        else launch_delta_ready<P, 1>(a, scratch, s);
+    } else if (!dl_vec(a)) launch_delta_rows<P, 2, 1, false>(a, s);
     else if (rows >= 4 * enough) launch_delta_rows<P, 4, 1, true>(a, s);
     else if (rows >= 2 * enough) launch_delta_rows<P, 2, 1, true>(a, s);
     else if (a.tokens < 32) launch_delta_rows<P, 1, 1, true>(a, s);
     else launch_delta_rows<P, 1, 4, true>(a, s);
 }
 
-void launch_delta(const delta_args & a, void * scratch, hipStream_t s, int n_cu) {
+void launch_delta(const delta_args & args, void * scratch, hipStream_t s, int n_cu) {
+    delta_args a = args;
+    a.y_tokens = a.tokens;
     if (a.seqs == 0 || a.heads == 0 || a.V == 0) return;
     if (dl_chunked(a)) {
         switch (dl_np(a)) {
@@ -1002,9 +1182,9 @@ void launch_delta(const delta_args & a, void * scratch, hipStream_t s, int n_cu)
         }
         return;
     }
-    if (a.K <= 64) launch_delta_tokens<1>(a, s, n_cu);
-    else if (a.K <= 128) launch_delta_tokens<2>(a, s, n_cu);
-    else launch_delta_tokens<4>(a, s, n_cu);
+    if (a.K <= 64) launch_delta_tokens<1>(a, scratch, s, n_cu);
+    else if (a.K <= 128) launch_delta_tokens<2>(a, scratch, s, n_cu);
+    else launch_delta_tokens<4>(a, scratch, s, n_cu);
 }
 
 }  // namespace mi355x

@@ -449,7 +449,7 @@ struct delta_args {
     int64_t g_nb1, g_nb2, g_nb3, b_nb1, b_nb2, b_nb3, s_nb3, out_nb3;
     float * y;
     char * out;
-    int64_t tokens;
+    int64_t tokens, y_tokens;  // y_tokens: a sequence's in y (launch_delta sets it)
     int K, V, heads, key_heads, seqs, g_elem;
     float q_eps, k_eps, scale;
     int64_t scratch_bytes;  // what it may take of scratch (a chunk of all heads at least)

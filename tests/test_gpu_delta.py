@@ -348,3 +348,27 @@ def test_keys_of_other_lengths(ggml, gpu, T, K, case):
         within(got, want, by + 1e-37, "y")
         within(states, end, e[..., None] + 1e-37, "states")
     G.free()
+
+
+def test_gates_an_element_over_slabs(ggml, gpu):
+    """more tokens than the rows made ready at once hold: the same bits as in two calls"""
+    K, V, H, S, T, T1 = 256, 8, 32, 1, 1300, 600
+    q, k, v, g, beta, st = inputs(K, V, H, H, T, S, elem=True, seed=17)
+    whole, y, _, _ = graph(ggml, gpu, q, k, v, g, beta, st)
+    first, y1, _, _ = graph(ggml, gpu, q[:, :T1], k[:, :T1], v[:, :T1], g[:, :T1], beta[:, :T1], st)
+    assert whole.compute(gpu.backend) == 0 and first.compute(gpu.backend) == 0
+    got, end = parts(whole, y, S, T, H, V, K)
+    got1, end1 = parts(first, y1, S, T1, H, V, K)
+    second, y2, _, _ = graph(ggml, gpu, q[:, T1:], k[:, T1:], v[:, T1:], g[:, T1:], beta[:, T1:], end1)
+    assert second.compute(gpu.backend) == 0
+    got2, end2 = parts(second, y2, S, T - T1, H, V, K)
+    assert np.array_equal(got[:, :T1], got1) and np.array_equal(got[:, T1:], got2) and np.array_equal(end, end2)
+    # and the state's first heads against the definition
+    n = slice(0, 2)
+    want, last, _, _ = rule64(unit(q[:, :, n].astype(np.float64)), unit(k[:, :, n].astype(np.float64)), v[:, :, n], g[:, :, n], beta[:, :, n], st[:, n])
+    # (decays of 0.5 on the mean: an error is left a few tokens; 2 K + 100 roundings each of sums of terms as large as these)
+    size = 32 * (2 * K + 100) * U * (np.abs(v[:, :, n]).max() + np.abs(st).max() * np.sqrt(K))
+    within(got[:, :, n], want, size / np.sqrt(K), "y")
+    within(end[:, n], last, size, "states")
+    for x in (whole, first, second):
+        x.free()

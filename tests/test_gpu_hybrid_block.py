@@ -105,9 +105,12 @@ def test_blocks_in_turn(ggml, gpu):
 
 
 def test_blocks_at_once(ggml, gpu):
-    """two backends of the device, each on its own stream, from two threads"""
+    """two backends of the device, each on its own stream, from two threads; launched each time (a recording
+    refuses the other thread's transfers while it lasts)"""
     lib = ggml.base()
-    backends = [gpu.backend, lib.ggml_backend_dev_init(gpu.dev, None)]
+    backends = [lib.ggml_backend_dev_init(gpu.dev, None) for _ in range(2)]
+    for b in backends:
+        gpu.cdll.ggml_backend_mi355x_set_hip_graphs(b, False)
     failed = []
 
     def work(backend, seed):
@@ -127,5 +130,6 @@ def test_blocks_at_once(ggml, gpu):
         t.start()
     for t in threads:
         t.join()
-    lib.ggml_backend_free(backends[1])
+    for b in backends:
+        lib.ggml_backend_free(b)
     assert not failed, failed
