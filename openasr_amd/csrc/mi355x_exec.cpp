@@ -1601,6 +1601,8 @@ bool planner::make_fattn(const ggml_tensor * t, fattn_args & a) {
         if (v->type == GGML_TYPE_F32) rows.v_nb1 = rows.v_nb2 = rows.v_nb3 = 0;
         if (vv.ne[3] != kv.ne[3] || !fattn_scored_supported(rows)) return fail(t, "K / V layout");
         fattn_scored_plan(a, n_cu);
+        // (a caller's own scratch may hold fewer splits' partials)
+        while (be->scratch_limit && a.scored_split > 1 && fattn_scratch_bytes(a) > be->scratch_limit / 2) a.scored_split--;
         return true;
     }
     fattn_plan(a, n_cu);

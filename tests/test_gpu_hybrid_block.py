@@ -133,3 +133,99 @@ def test_blocks_at_once(ggml, gpu):
     for b in backends:
         lib.ggml_backend_free(b)
     assert not failed, failed
+
+
+def set_far_rows(G, t, rows, step):
+    """rows [n, m] to a tensor of n rows of step elements (gigabytes in all)"""
+    for i, row in enumerate(np.ascontiguousarray(rows)):
+        assert G.lib.ggml_backend_tensor_set(t, row.ctypes.data, i * step * rows.itemsize, row.nbytes) == 0
+
+
+@pytest.mark.parametrize("Q", [1, 20])
+def test_attention_offsets_past_32_bits(ggml, gpu, Q):
+    """K and V rows 64 MB apart: 5 GB from the first to the last"""
+    rng = np.random.default_rng(Q)
+    N, D, step = 80, 64, 32 << 20
+    q = rng.standard_normal((1, 2, Q, D)).astype(np.float32)
+    kv = rng.standard_normal((N, D)).astype(np.float16)
+    mask = make_mask("causal", 1, 2, Q, N, 0.0, rng)
+    G = ggml.Graph(64, 64)
+    X, M = G.new(ggml.F32, D, Q, 2, 1), G.new(ggml.F16, N, Q)
+    T = G.new(ggml.F16, step, N, weight=True)
+    rows = G.lib.ggml_view_4d(G.ctx, T, D, N, 1, 1, 2 * step, 2 * step * N, 2 * step * N, 0)
+    y = G.lib.ggml_flash_attn_ext(G.ctx, X, rows, rows, M, SCALE / 8, 0.0, CAP)
+    G.build(y)
+    G.allocate(gpu.buft)
+    set_far_rows(G, T, kv, step)
+    G.set(X, q)
+    G.set(M, mask.view(np.uint16))
+    want, by = attention64(q, kv[None, None], kv[None, None], mask, SCALE / 8, CAP, 0.0)
+    for _ in range(3):
+        assert G.compute(gpu.backend) == 0
+        within(G.get(y).reshape(want.shape), want, by)
+    G.free()
+
+
+@pytest.mark.parametrize("elem", [False, True], ids=["head", "element"])
+def test_delta_offsets_past_32_bits(ggml, gpu, elem):
+    """a token's rows 128 MB after the last one's"""
+    Hv = 1
+    T, D, W = 40, 64, 32 << 20
+    rng = np.random.default_rng(5)
+    q, k, v = (rng.standard_normal((1, T, 1, D)).astype(np.float32) for _ in range(3))
+    g = -np.exp(rng.standard_normal((1, T, 1, D if elem else 1))).astype(np.float32)
+    beta, st = rng.random((1, T, 1)).astype(np.float32), rng.standard_normal((1, 1, D, D)).astype(np.float32)
+    G = ggml.Graph(64, 64)
+    x = G.new(ggml.F32, W, T, weight=True)
+    L, ctx = G.lib, G.ctx
+    ge = g.shape[3]
+    view = lambda n, at: L.ggml_view_4d(ctx, x, n, 1, T, 1, 4 * n, 4 * W, 4 * W * T, 4 * at)  # noqa: E731
+    s_ = G.new(ggml.F32, D, D, Hv, 1, weight=True)
+    y = L.ggml_gated_delta_net(ctx, L.ggml_l2_norm(ctx, view(D, 0), EPS), L.ggml_l2_norm(ctx, view(D, D), EPS), view(D, 2 * D),
+                               view(ge, 3 * D), view(1, 3 * D + ge), s_)
+    G.build(y)
+    G.allocate(gpu.buft)
+    set_far_rows(G, x, np.concatenate([a.reshape(T, -1) for a in (q, k, v, g, beta)], 1), W)
+    G.set(s_, st)
+    want, end, by, bs = rule_bounds(unit(q.astype(np.float64)), unit(k.astype(np.float64)), v, g, beta, st)
+    for _ in range(3):
+        assert G.compute(gpu.backend) == 0
+        flat = G.get(y).reshape(-1)
+        within(flat[:T * D].reshape(want.shape), want, by, "y")
+        within(flat[T * D:].reshape(end.shape), end, bs, "states")
+    G.free()
+
+
+def test_static_scratch(ggml, gpu):
+    """prompts whose partials and slabs are cut to a caller's 64 MB"""
+    import ctypes
+    lib = gpu.cdll
+    lib.ggml_backend_mi355x_graph_compute_static.restype = ctypes.c_int
+    lib.ggml_backend_mi355x_graph_compute_static.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    b = Block(ggml, gpu.buft, 300, 1, 300, 3)
+    b.step(gpu.backend)
+    b.check()
+    n = b.rng.standard_normal
+    for _ in range(2):
+        b.gv, b.bv = -np.exp(n((1, 300, H, 1))).astype(np.float32), (1 / (1 + np.exp(-n((1, 300, H))))).astype(np.float32)
+        for t, a in ((b.x, b.xv), (b.g, b.gv), (b.beta, b.bv)):
+            b.G.set(t, a)
+        assert lib.ggml_backend_mi355x_graph_compute_static(gpu.backend, b.G.gf) == 0
+        b.check()
+    b.G.free()
+    # and attention in as many pieces as fit
+    rng = np.random.default_rng(9)
+    q, k, v = rng.standard_normal((1, 4, 900, 128)).astype(np.float32), *(rng.standard_normal((1, 4, 900, 128)).astype(np.float16) for _ in range(2))
+    mask = make_mask("causal", 1, 4, 900, 900, 0.0, rng)
+    G = ggml.Graph(64, 64)
+    X, M = G.new(ggml.F32, 128, 900, 4, 1), G.new(ggml.F16, 900, 900)
+    kt, vt = (G.new(ggml.F16, 128, 900, 4, 1) for _ in range(2))
+    y = G.lib.ggml_flash_attn_ext(G.ctx, X, kt, vt, M, 0.1, 0.0, CAP)
+    G.build(y)
+    G.allocate(gpu.buft)
+    for t, a in ((X, q), (M, mask.view(np.uint16)), (kt, k.view(np.uint16)), (vt, v.view(np.uint16))):
+        G.set(t, a)
+    assert lib.ggml_backend_mi355x_graph_compute_static(gpu.backend, G.gf) == 0
+    want, by = attention64(q, k, v, mask, 0.1, CAP, 0.0)
+    within(G.get(y).reshape(want.shape), want, by, "attention")
+    G.free()
