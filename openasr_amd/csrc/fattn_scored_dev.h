@@ -95,7 +95,7 @@ void launch_fattn_scored_dec(const fattn_args & a, void * scratch, float * out, 
 // of `partials` in all
 struct fs_join {
     const float * part;
-    const int * pieces;  // how many of the `split` partials a (sequence, kv head, query block) has; null: all of them
+    const int2 * pieces;  // of a (sequence, kv head, query block): how many partials, and the first one's place; null: `split` each, in order
     float * out;
     int64_t rows, partials;
     int split, d;

@@ -59,6 +59,7 @@ typedef uint32_t fs_u4h __attribute__((ext_vector_type(4), aligned(2)));
 
 // a tile of a query block: nothing seen; seen, and all entries zero; seen, no
 // entry -inf; seen, some entry -inf (or past the span)
+constexpr int kFsUnits = 512;  // query blocks, and masks, of a launch in pieces, at most
 enum : uint8_t { kFsClosed = 0, kFsPlain = 1, kFsAdds = 2, kFsMixed = 3 };
 
 struct fs_args {
@@ -71,7 +72,8 @@ struct fs_args {
     uint64_t * seen;  // [mask sequence][kv head or one][query block][tile]
     uint8_t * cls;    // [n_cls], the same order
     int64_t n_cls;
-    int * pieces;     // [sequence][kv head][query block]
+    int2 * pieces;    // [sequence][kv head][query block]: how many, and the first one's place in part
+    int64_t partials; // rows of part
     float * part;
     float * out;
 };
@@ -196,6 +198,11 @@ __device__ __forceinline__ void fs_to_lds(const char * src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
 }
 
+// n open tiles in pieces of at most len
+__device__ __forceinline__ int fs_pieces(int n, int len, int most) {
+    return max(1, min(most, (int) ((float) (n + len - 1) / (float) len)));
+}
+
 // The phases' boundary: LDS reads are done; loads to LDS stay in flight
 __device__ __forceinline__ void fs_phase_end() {
     asm volatile("" ::: "memory");
@@ -215,17 +222,78 @@ __global__ __launch_bounds__(512, 2) void k_fattn_scored(fs_args f) {
     __shared__ unsigned long long s_bad[2];         // positions of the tile whose V is not finite
     const fattn_args & a = f.a;
     const int tid = (int) threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lg = lane >> 4;
-    // Workgroup b runs on XCD b % 8. Where the (sequence, kv head) pairs divide by
-    // eight an XCD takes its share of them, whose K and V its L2 then holds. First
-    // pieces first, and of them the last query blocks, whose causal span is longest
-    const int heads = a.hkv * a.n_seq, units = heads * f.q_blocks;
-    int b = (int) blockIdx.x, z, qb, hs;
-    if (heads % 8 == 0) {
-        const int i = b / 8, h8 = heads / 8;
-        z = i / (units / 8), qb = f.q_blocks - 1 - i % (units / 8) / h8, hs = b % 8 * h8 + i % h8;
+    // Workgroup b runs on XCD b % 8. Where the (sequence, kv head) pairs of a mask
+    // divide by eight an XCD takes its share of them, whose K and V its L2 then holds;
+    // the last query blocks, whose causal span is longest, first.
+    const int units = a.hkv * a.n_seq * f.q_blocks, kinds = (f.heads_mask ? a.hkv : 1) * (MASK ? a.m_ne3 : 1);
+    const int like = units / f.q_blocks / kinds;  // pairs that read the same mask
+    int b = (int) blockIdx.x, inst = b % like, r = b / like;
+    if (like % 8 == 0) inst = b % 8 * (like / 8) + b / 8 % (like / 8), r = b / 8 / (like / 8);
+    int pieces = 1, z = 0, at_piece = 0;
+    if (f.split == 1) {
+    } else if constexpr (MASK) {
+        // The open tiles of a query block in equal pieces of at most `len` tiles: the
+        // least len from four on with which all blocks' pieces have a place on the card
+        // at once, since a second round costs as much as the first. Workgroup b is
+        // the b-th of those pieces, and every one counts them for itself. us of the
+        // call PIECEFIG
+        __shared__ int s_open[kFsUnits], s_of[NW];
+        const int n_units = kinds * f.q_blocks;
+        for (int i = tid; i < kFsUnits; i += NTH) s_open[i] = 0;
+        __syncthreads();
+        for (int i = 16 * tid; i < (int) f.n_cls; i += 16 * NTH) {
+            const fs_u4 c = *(const fs_u4 *) &f.cls[i];
+            uint32_t open = 0;  // a bit a tile
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t x = (c[j] | (c[j] >> 1)) & 0x01010101u;
+                open |= ((x | x >> 7 | x >> 14 | x >> 21) & 15u) << (4 * j);
+            }
+            for (int e = 0; e < 16;) {
+                const int u = (i + e) / f.n_tiles, n = min(16 - e, (u + 1) * f.n_tiles - i - e);
+                if (u < n_units) atomicAdd(&s_open[(f.q_blocks - 1 - u % f.q_blocks) * kinds + u / f.q_blocks], __popc((open >> e) & ((1u << n) - 1)));
+                e += n;
+            }
+        }
+        __syncthreads();
+        const int by = f.n_tiles / NTH + 1;  // a thread a length
+        int total = 0;
+        for (int u = 0; u < n_units; u++) total += like * fs_pieces(s_open[u], 4 + tid * by, f.split);
+        const uint64_t fits = __ballot(total <= f.slots);
+        if (lane == 0) s_of[wave] = fits ? 64 * wave + __builtin_ctzll(fits) : NTH - 1;
+        __syncthreads();
+        int first = NTH - 1;
+#pragma unroll
+        for (int w = 0; w < NW; w++) first = min(first, s_of[w]);
+        const int len = 4 + first * by;
+        // the block that piece r of a pair is of: units 64 at a time
+        int before = 0, u = -1;
+        for (int u0 = 0; u0 < n_units; u0 += 64) {
+            const int mine = u0 + lane < n_units ? fs_pieces(s_open[u0 + lane], len, f.split) : 0;
+            int sum = mine;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int x = __shfl_up(sum, o);
+                if (lane >= o) sum += x;
+            }
+            const uint64_t past = __ballot(before + sum > r);
+            if (u < 0 && past) {
+                const int l0 = __builtin_ctzll(past);
+                u = u0 + l0, pieces = __shfl(mine, l0), z = r - (before + __shfl(sum, l0) - pieces);
+            }
+            before += __shfl(sum, 63);
+        }
+        if (u < 0) return;  // (r is past the last piece)
+        at_piece = __builtin_amdgcn_readfirstlane(inst * before + r);
+        pieces = __builtin_amdgcn_readfirstlane(pieces), z = __builtin_amdgcn_readfirstlane(z), r = __builtin_amdgcn_readfirstlane(u);
     } else {
-        z = b / units, qb = f.q_blocks - 1 - b % units / heads, hs = b % heads;
+        pieces = f.split, z = r % f.split, r /= f.split;
+        at_piece = (inst * f.q_blocks + r) * pieces + z;
     }
+    const int qb = f.q_blocks - 1 - r / kinds, kind = r % kinds;
+    const int hs = f.heads_mask ? (kind / a.hkv + a.m_ne3 * inst) * a.hkv + kind % a.hkv
+                                : (kind + kinds * (inst / a.hkv)) * a.hkv + inst % a.hkv;
+    if (f.split > 1 && z == 0 && tid == 0) f.pieces[hs * f.q_blocks + qb] = int2{pieces, at_piece};
     const int kvh = hs % a.hkv, seq = hs / a.hkv, kv_seq = seq / a.rk3;
     const int q0 = qb * f.qpw, nq = min(f.qpw, a.n_q - q0);
     const char * kbase = a.k + (int64_t) kvh * a.k_nb2 + (int64_t) kv_seq * a.k_nb3;
@@ -261,11 +329,7 @@ __global__ __launch_bounds__(512, 2) void k_fattn_scored(fs_args f) {
         }
         w_open = __ballot(c != kFsClosed), w_adds = __ballot(c >= kFsAdds), w_mixed = __ballot(c == kFsMixed);
     };
-    // The open tiles of this query block, in equal pieces. A piece is what the
-    // launch's open tiles come to on each place of the card that is left when
-    // every block has one, so that no piece waits for a second round (a block's
-    // last piece is cut short); at least four tiles
-    int n_open = 0, skip = 0, pieces = 1;
+    int n_open = 0, skip = 0;
     if (MASK) {
         for (w_base = 0; w_base < f.n_tiles; w_base += 64) {
             window();
@@ -274,29 +338,7 @@ __global__ __launch_bounds__(512, 2) void k_fattn_scored(fs_args f) {
     } else {
         n_open = f.n_tiles;
     }
-    if (f.split > 1) {
-        int64_t all = (int64_t) f.n_tiles * f.q_blocks * a.hkv * a.n_seq;
-        if constexpr (MASK) {
-            __shared__ int s_open[NW];
-            int n = 0;
-            for (int64_t i = 16 * (int64_t) tid; i < f.n_cls; i += 16 * NTH) {
-                const fs_u4 c = *(const fs_u4 *) &f.cls[i];
-#pragma unroll
-                for (int j = 0; j < 4; j++) n += __popc((c[j] | (c[j] >> 1)) & 0x01010101u);
-            }
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o);
-            if (lane == 0) s_open[wave] = n;
-            __syncthreads();
-            int64_t sum = 0;
-#pragma unroll
-            for (int w = 0; w < NW; w++) sum += s_open[w];
-            all = sum * (f.heads_mask ? 1 : a.hkv) * (a.n_seq / a.m_ne3);
-        }
-        const int piece = max(4, (int) ((float) all / (float) max(f.slots - units, f.slots / 2)) + 1);
-        pieces = __builtin_amdgcn_readfirstlane(max(1, min(f.split, (n_open + piece - 1) / piece)));
-        if (z >= pieces) return;
-        if (z == 0 && tid == 0) f.pieces[hs * f.q_blocks + qb] = pieces;
+    if (pieces > 1) {
         const int each = n_open / pieces, more = n_open % pieces;
         skip = z * each + min(z, more);
         n_open = each + (z < more ? 1 : 0);
@@ -632,8 +674,8 @@ __global__ __launch_bounds__(512, 2) void k_fattn_scored(fs_args f) {
         const int r = 16 * (RW * wave + w) + l16;
         if (pieces > 1) {
             // partials of piece z: O unnormalised, then (m, l), a workgroup row
-            const int64_t rows = (int64_t) gridDim.x * R;
-            const int64_t pr = (((int64_t) hs * f.q_blocks + qb) * f.split + z) * R + r;
+            const int64_t rows = f.partials;
+            const int64_t pr = (int64_t) at_piece * R + r;
 #pragma unroll
             for (int ct = 0; ct < NT; ct++) *(fs_f4 *) &f.part[pr * D + 16 * ct + 4 * lg] = o[w][ct];
             if (lg == 0) *(float2 *) &f.part[rows * D + 2 * pr] = make_float2(l[w] == 0.0f ? -INFINITY : kFsUp - base[w], l[w]);
@@ -657,8 +699,9 @@ __global__ __launch_bounds__(256) void k_fattn_join(fs_join f) {
     const int64_t row = (int64_t) blockIdx.x * RW + tid / T, rc = min(row, f.rows - 1);  // of (sequence, query, head)
     const int head = (int) (rc % f.hq), q = (int) (rc / f.hq % f.n_q), seq = (int) (rc / ((int64_t) f.hq * f.n_q));
     const int64_t blk = ((int64_t) seq * (f.hq / f.g) + head / f.g) * f.q_blocks + q / f.qpw;
-    const int64_t p0 = blk * f.split * f.R + (q % f.qpw) * f.g + head % f.g;
-    const int split = f.pieces ? f.pieces[blk] : f.split;
+    const int2 piece = f.pieces ? f.pieces[blk] : int2{f.split, (int) blk * f.split};
+    const int64_t p0 = (int64_t) piece.y * f.R + (q % f.qpw) * f.g + head % f.g;
+    const int split = piece.x;
     const bool whole = f.pieces && split == 1;  // written by its one piece
     if (LN == 1 && whole) return;
     const float * ml = f.part + f.partials * D;
@@ -738,7 +781,10 @@ size_t fs_plan(const fattn_args & a, fs_args & f) {
         f.n_cls = (int64_t) a.m_ne3 * (f.heads_mask ? a.hkv : 1) * f.q_blocks * f.n_tiles;
         need = fs_al(8 * f.n_cls) + fs_al(f.n_cls);
     }
-    if (f.split > 1) need += fs_al(sizeof(int) * (size_t) a.n_seq * a.hkv * f.q_blocks) + sizeof(float) * (size_t) a.n_seq * a.hkv * f.q_blocks * f.split * R * (a.d + 2);
+    // (with a mask at most `slots` pieces in all)
+    const int64_t units = (int64_t) a.n_seq * a.hkv * f.q_blocks;
+    f.partials = (a.mask ? std::min<int64_t>(f.slots, units * f.split) : units * f.split) * R;
+    if (f.split > 1) need += fs_al(sizeof(int2) * (size_t) units) + sizeof(float) * (size_t) f.partials * (a.d + 2);
     return need;
 }
 
@@ -752,15 +798,15 @@ bool fattn_scored_supported(const fattn_args & a) {
 
 void fattn_scored_plan(fattn_args & a, int n_cu) {
     if (fattn_scored_dec_supported(a)) return fattn_scored_dec_plan(a, n_cu);
-    // Pieces of a query block's open tiles where query blocks leave CUs idle. How
-    // many a block gets is for the launch to say; at most twice as many as an even
-    // split over the card would need, so that a causal mask's long blocks get theirs
+    // Pieces of a query block's open tiles where query blocks leave CUs idle, of at
+    // least four tiles. How many a block gets under a mask is for the launch to say
     const int R = fs_rows(a), g = a.hq / a.hkv, qpw = std::min(R / g, std::max(1, a.n_q));
     const int64_t units = std::max<int64_t>(1, (int64_t) ((a.n_q + qpw - 1) / qpw) * a.hkv * a.n_seq);
     const int n_tiles = (a.n_kv + kFsTile - 1) / kFsTile;
     a.scored = 1;
     a.scored_slots = n_cu;
-    a.scored_split = (int) std::max<int64_t>(1, std::min<int64_t>(units >= a.scored_slots ? 1 : 2 * a.scored_slots / units, n_tiles / 4));
+    const int64_t most = a.mask ? a.scored_slots : a.scored_slots / units;
+    a.scored_split = units >= a.scored_slots || units > kFsUnits ? 1 : (int) std::max<int64_t>(1, std::min<int64_t>(most, n_tiles / 4));
 }
 
 size_t fattn_scored_scratch_bytes(const fattn_args & a) {
@@ -784,11 +830,11 @@ void launch_fattn_scored(const fattn_args & a, void * scratch, float * out, hipS
         hipLaunchKernelGGL(k_fattn_tiles, dim3((unsigned) n), dim3(256), 0, s, f);
         note_hip_error(hipGetLastError());
     }
-    f.pieces = (int *) p;
-    if (f.split > 1) p += fs_al(sizeof(int) * (size_t) a.n_seq * a.hkv * f.q_blocks);
+    f.pieces = (int2 *) p;
+    if (f.split > 1) p += fs_al(sizeof(int2) * (size_t) a.n_seq * a.hkv * f.q_blocks);
     f.part = (float *) p;
     const int rows = fs_rows(a);
-    const dim3 grid((unsigned) ((int64_t) f.q_blocks * a.hkv * a.n_seq * f.split));
+    const dim3 grid((unsigned) (f.split > 1 ? f.partials / rows : (int64_t) f.q_blocks * a.hkv * a.n_seq));
     auto go = [&](auto d, auto rw) {
         constexpr int D = decltype(d)::value, RW = decltype(rw)::value;
         if (a.softcap > 0.0f) {
@@ -811,7 +857,7 @@ void launch_fattn_scored(const fattn_args & a, void * scratch, float * out, hipS
     if (f.split > 1) {
         fs_join j{};
         j.part = f.part, j.pieces = f.pieces, j.out = out, j.rows = (int64_t) a.n_seq * a.n_q * a.hq;
-        j.partials = (int64_t) a.n_seq * a.hkv * f.q_blocks * f.split * rows;
+        j.partials = f.partials;
         j.split = f.split, j.d = a.d, j.hq = a.hq, j.n_q = a.n_q, j.g = f.g, j.qpw = f.qpw, j.q_blocks = f.q_blocks, j.R = rows;
         launch_fattn_join(j, s);
     }
