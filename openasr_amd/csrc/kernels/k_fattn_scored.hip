@@ -20,7 +20,7 @@
 // A first launch looks at the mask once for all heads: which tiles a block of
 // queries sees at all, which of them have no masked or no nonzero entry, and
 // which positions some query sees. From its counts every workgroup finds the same
-// equal pieces, and a third launch joins the pieces of a row where there are several.
+// pieces of the same length, and a third launch joins a row's where there are several.
 //
 // What bounds it: 256 rows of 128 by a tile take 8400 cycles of a CU, its 832 matrix
 // instructions 3328 of each SIMD's and its exponentials 4000 to 4900 of the vector
@@ -236,7 +236,8 @@ __global__ __launch_bounds__(512, 2) void k_fattn_scored(fs_args f) {
         // least len from four on with which all blocks' pieces have a place on the card
         // at once, since a second round costs as much as the first. Workgroup b is
         // the b-th of those pieces, and every one counts them for itself. us of the
-        // call PIECEFIG
+        // call with a length from the sum of the open tiles alone, and so: 2048 causal
+        // queries 95 / 79, two sequences of 1500 90 / 81, three documents 63 / 61
         __shared__ int s_open[kFsUnits], s_of[NW];
         const int n_units = kinds * f.q_blocks;
         for (int i = tid; i < kFsUnits; i += NTH) s_open[i] = 0;
