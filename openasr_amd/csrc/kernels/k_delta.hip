@@ -374,6 +374,7 @@ constexpr int kDlReady = 32;
 // keys of length one and beta up to one; tokens of one key with a beta of 2, which turn
 // the state over and over, come to 127, and were 4e-4 off); scaled values. The state
 // and v: up to 2^40
+constexpr int kDlLeastKExp = -7;
 constexpr float kDlRaw = 0x1p50f, kDlRow = 0x1p10f, kDlLeastQ = 0x1p-20f, kDlLeastK = 0x1p-7f, kDlBeta = 16.0f, kDlRowSum = 64.0f, kDlHalf = 60000.0f;
 
 struct dl_chunk_args {
@@ -532,7 +533,9 @@ __global__ __launch_bounds__(256, 2) void k_delta_solve(dl_chunk_args q) {
         most = fmaxf(most, __shfl_xor(most, 1));
         most = fmaxf(most, __shfl_xor(most, 2));
         bad |= dl_past(most, kDlRow) || (most > 0.0f && most < kDlLeastK);
-        if ((tid & 3) == 0) s_kexp[t] = dl_pow2(13 - dl_exponent(most));
+        // (a row of zeros is scaled as the shortest keys are: `left` of a chunk of such rows
+        // alone has its largest element in a divisor of k_delta_chunks)
+        if ((tid & 3) == 0) s_kexp[t] = dl_pow2(13 - max(dl_exponent(most), kDlLeastKExp));
     }
     bad = __syncthreads_or(bad);
     {
@@ -974,8 +977,8 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
         __syncthreads();
         if (s_late[c & 1]) goto one_by_one;
         {
-            // the state in D's scale, and back
-            const float in = end * dl_pow2(6 - size) / left_most, out = left_most * dl_pow2(size - 6);
+            // the state in D's scale, and back (left_most is 2^-20 to 2^-3: the factor of end 2^-37 to 2^126)
+            const float in = end * (dl_pow2(6 - size) / left_most), out = left_most * dl_pow2(size - 6);
             dl_split x[2][NC];
 #pragma unroll
             for (int m = 0; m < 2; m++)
@@ -1010,7 +1013,9 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
 #pragma unroll
                         for (int cb = 0; cb < NC; cb++) acc[cb] = dl_product(i, p[m], x[cb], acc[cb]);
                 }
-                const dl_v4f back = y_row * dl_pow2(size - 6);
+                // (in two steps: y_row's inverse may be 2^73, the state's scale 2^106)
+#pragma unroll
+                for (int cb = 0; cb < NC; cb++) acc[cb] *= dl_pow2(size - 6);
                 char * y = (char *) (a.y + ((s * a.tokens + t0) * a.heads + h) * a.V);
                 const uint32_t y_nb = 4u * (uint32_t) a.heads * (uint32_t) a.V, at = (uint32_t) (16 * tb + 4 * lg) * y_nb + 4u * (uint32_t) col0;
                 const int left_over = (int) min((int64_t) kDlC, a.tokens - t0) - 16 * tb - 4 * lg;
@@ -1019,11 +1024,11 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
                     if (col0 + 16 * cb >= a.V) continue;
                     if (left_over >= 4) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) *(float *) (y + (int64_t) e * y_nb + (at + 64 * cb)) = acc[cb][e] * back[e];
+                        for (int e = 0; e < 4; e++) *(float *) (y + (int64_t) e * y_nb + (at + 64 * cb)) = acc[cb][e] * y_row[e];
                     } else {
 #pragma unroll
                         for (int e = 0; e < 3; e++)
-                            if (e < left_over) *(float *) (y + (int64_t) e * y_nb + (at + 64 * cb)) = acc[cb][e] * back[e];
+                            if (e < left_over) *(float *) (y + (int64_t) e * y_nb + (at + 64 * cb)) = acc[cb][e] * y_row[e];
                     }
                 }
             }

@@ -372,3 +372,34 @@ def test_gates_an_element_over_slabs(ggml, gpu):
     within(end[:, n], last, size, "states")
     for x in (whole, first, second):
         x.free()
+
+
+@pytest.mark.parametrize("T", [24, 64, 200])
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("case", ["nothing", "leading", "trailing", "one chunk"])
+def test_chunks_of_zero_keys(ggml, gpu, T, norm, case):
+    """prompts that warm up, or are padded, with rows of zeros: a chunk whose keys are all zero leaves e^g S"""
+    K, V, Hk, H, S = 64, 48, 1, 2, 2
+    x = list(inputs(K, V, Hk, H, T, S, seed=19, rate=0.1))
+    if not norm:
+        x[0], x[1] = unit(x[0]).astype(np.float32), (unit(x[1]) * 0.9).astype(np.float32)
+    zero = {"nothing": slice(0, T), "leading": slice(0, min(T, 70)), "trailing": slice(T // 4, T), "one chunk": slice(64, 128)}[case]
+    x[1][:, zero], x[2][:, zero] = 0, 0
+    if case == "nothing":
+        x[0][:] = 0
+    if case in ("nothing", "leading"):
+        x[5][0] = 0
+        x[5][1] *= 1e-4
+    if case == "trailing":  # what is left of the state lies far under one
+        x[3][:] = -0.15
+        x[5] *= 1e-3
+        x[2] *= 1e-3
+    G, y, _, _ = graph(ggml, gpu, *x, norm=norm)
+    q, k = (unit(np.asarray(a, np.float64)) if norm else a for a in x[:2])
+    want, end, by, bs = rule_bounds(q, k, *x[2:])
+    for _ in range(2):
+        assert G.compute(gpu.backend) == 0
+        got, states = parts(G, y, S, T, H, V, K)
+        within(got, want, by, "y")
+        within(states, end, bs, "states")
+    G.free()
