@@ -723,11 +723,11 @@ __global__ __launch_bounds__(256) void k_fattn_join(fs_join f) {
             if (z0 + k * LN >= split) v[k] = make_float2(-INFINITY, 0.0f);
             most = fmaxf(most, v[k].x);
         }
-        const float w0 = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - most);
+        const float w0 = L == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(M - most);
         L *= w0, acc *= w0, M = most;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            if (v[k].x == -INFINITY) continue;
+            if (v[k].y == 0.0f) continue;  // nothing seen (a NaN is a sum too)
             const float w = __builtin_amdgcn_exp2f(v[k].x - most);
             L = fmaf(w, v[k].y, L);
 #pragma unroll
@@ -746,7 +746,7 @@ __global__ __launch_bounds__(256) void k_fattn_join(fs_join f) {
 #pragma unroll
         for (int k = 0; k < LN; k++) {
             const float2 v = s_ml[tid + k * (D / 4)];
-            if (v.x == -INFINITY) continue;
+            if (v.y == 0.0f) continue;
             const float w = __builtin_amdgcn_exp2f(v.x - most);
             L = fmaf(w, v.y, L);
             const fs_f4 x = s_acc[tid + k * (D / 4)];

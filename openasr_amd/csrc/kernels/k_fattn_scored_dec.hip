@@ -247,7 +247,9 @@ __global__ __launch_bounds__(64 * kFcWaves) void k_fattn_scored_dec(fc_args f) {
         fs_f4 o = {0, 0, 0, 0};
 #pragma unroll
         for (int v = 0; v < kFcWaves; v++) {
-            if (s_m[v][h] == -INFINITY) continue;
+            // (a sum of 0: the wave saw nothing. Its maximum is not asked: it is -inf, too, where
+            // every score is a NaN, and the sum is one then)
+            if (s_l[v][h] == 0.0f) continue;
             const float c = __builtin_amdgcn_exp2f(s_m[v][h] - M);
             L = fmaf(c, s_l[v][h], L);
             const fs_f4 x = *(const fs_f4 *) &s_acc[v][h][d];

@@ -326,3 +326,29 @@ def test_supports(ggml, gpu):
     wide = G.new(ggml.F16, 68, 9, 2, 1)  # rows of 136 bytes
     assert not ok(kv=G.lib.ggml_view_4d(G.ctx, wide, 64, 9, 2, 1, 136, 136 * 9, 136 * 18, 0))
     G.free()
+
+
+@pytest.mark.parametrize("Q", [1, 20])
+@pytest.mark.parametrize("D,N", [(64, 65), (128, 130), (256, 40), (64, 9000)])
+@pytest.mark.parametrize("kind", ["lengths", "heads"])
+@pytest.mark.parametrize("where", ["query", "first", "last", "middle"])
+def test_nan_that_is_seen(ggml, gpu, Q, D, N, kind, where):
+    """a NaN in a query, or in a key that a query sees, is that row's result, wherever the key lies"""
+    rng = np.random.default_rng(D + N + Q)
+    S, H, G = 2, 4, 2
+    q, k, v = operands(rng, S, H, G, Q, N, D)
+    mask = np.zeros((S, H if kind == "heads" else 1, Q, N), np.float16)
+    if kind == "heads":
+        mask[:, 1, :, ::3] = -np.inf
+    want, bound = attention64(q, k, v, mask, 0.1, 30.0, 0.0)
+    hit = np.zeros((S, Q, H), bool)
+    if where == "query":
+        q[1, 2, Q // 2, 7] = np.nan
+        hit[1, Q // 2, 2] = True
+    else:
+        n = {"first": 0, "last": N - 1, "middle": N // 2}[where]
+        k[1, 0, n, 3] = np.nan  # of query heads 0 and 1
+        hit[1] = np.isfinite(np.broadcast_to(mask, (S, H, Q, N))[1, :, :, n]).T & (np.arange(H) < H // G)
+    got = attention(ggml, gpu, q, k, v, mask, 0.1, 30.0, 0.0)
+    assert np.isnan(got[hit]).all()
+    check(got[~hit], want[~hit], bound[~hit])
