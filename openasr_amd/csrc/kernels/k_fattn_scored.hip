@@ -35,6 +35,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "../fattn_pieces.h"
 #include "../fattn_scored_dev.h"
 #include "../mi355x_common.h"
 #include "../ops.h"
@@ -198,11 +199,6 @@ __device__ __forceinline__ void fs_to_lds(const char * src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
 }
 
-// n open tiles in pieces of at most len
-__device__ __forceinline__ int fs_pieces(int n, int len, int most) {
-    return max(1, min(most, (int) ((float) (n + len - 1) / (float) len)));
-}
-
 // The phases' boundary: LDS reads are done; loads to LDS stay in flight
 __device__ __forceinline__ void fs_phase_end() {
     asm volatile("" ::: "memory");
@@ -257,16 +253,17 @@ __global__ __launch_bounds__(512, 2) void k_fattn_scored(fs_args f) {
             }
         }
         __syncthreads();
-        const int by = f.n_tiles / NTH + 1;  // a thread a length
+        static_assert(NTH == kFsLengths, "a thread a length");
+        const int mine_len = fs_length(tid, f.n_tiles);
         int total = 0;
-        for (int u = 0; u < n_units; u++) total += like * fs_pieces(s_open[u], 4 + tid * by, f.split);
+        for (int u = 0; u < n_units; u++) total += like * fs_pieces(s_open[u], mine_len, f.split);
         const uint64_t fits = __ballot(total <= f.slots);
         if (lane == 0) s_of[wave] = fits ? 64 * wave + __builtin_ctzll(fits) : NTH - 1;
         __syncthreads();
         int first = NTH - 1;
 #pragma unroll
         for (int w = 0; w < NW; w++) first = min(first, s_of[w]);
-        const int len = 4 + first * by;
+        const int len = fs_length(first, f.n_tiles);
         // the block that piece r of a pair is of: units 64 at a time
         int before = 0, u = -1;
         for (int u0 = 0; u0 < n_units; u0 += 64) {
