@@ -48,6 +48,7 @@ constexpr int kFsTile = 64;
 // p is scaled by 2^12: its low half stays a normal f16 down to 2^-15 of the maximum
 constexpr float kFsUp = 12.0f;
 constexpr float kFsOver = 3.0f;  // (and stays below f16's 2^16)
+constexpr float kFsBase = 64.0f;
 
 typedef _Float16 fs_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 fs_h4 __attribute__((ext_vector_type(4)));
@@ -430,7 +431,9 @@ __global__ __launch_bounds__(512, 2) void k_fattn_scored(fs_args f) {
 
     // A row's exponents are its scores plus base, which puts its maximum at kFsUp
     // when it is set; it is set anew where a score goes past that by more than
-    // kFsOver, not with every new maximum
+    // kFsOver, not with every new maximum. A score is made as a sum with base only up to
+    // kFsBase, half a step of which is 2^-18: a row whose tiles so far hold a mask's large
+    // finite values has a base of 2^16, which would round the scores that follow to 2^-8
     float base[RW], l[RW];
     fs_f4 o[RW][NT];
 #pragma unroll
@@ -540,7 +543,8 @@ __global__ __launch_bounds__(512, 2) void k_fattn_scored(fs_args f) {
 #pragma unroll
                     for (int i = w * KLD / RW; i < (w + 1) * KLD / RW; i++) issue_one(0, i, tile[2], par);
                 }
-                float z[4][4];
+                float z[4][4];  // with b0
+                const float b0 = fabsf(base[w]) <= kFsBase ? base[w] : 0.0f, off = base[w] - b0;
                 if constexpr (CAP) {
                     float most = 0.0f;
 #pragma unroll
@@ -551,18 +555,18 @@ __global__ __launch_bounds__(512, 2) void k_fattn_scored(fs_args f) {
 #pragma unroll
                         for (int t = 0; t < 4; t++)
 #pragma unroll
-                            for (int i = 0; i < 4; i++) z[t][i] = fs_cap_low(f.score, sc[w][t][i], base[w]);
+                            for (int i = 0; i < 4; i++) z[t][i] = fs_cap_low(f.score, sc[w][t][i], b0);
                     } else {
 #pragma unroll
                         for (int t = 0; t < 4; t++)
 #pragma unroll
-                            for (int i = 0; i < 4; i++) z[t][i] = fs_cap_any(f.score, sc[w][t][i] * f.score.in) + base[w];
+                            for (int i = 0; i < 4; i++) z[t][i] = fs_cap_any(f.score, sc[w][t][i] * f.score.in) + b0;
                     }
                 } else {
 #pragma unroll
                     for (int t = 0; t < 4; t++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) z[t][i] = fmaf(sc[w][t][i], f.score.in, base[w]);
+                        for (int i = 0; i < 4; i++) z[t][i] = fmaf(sc[w][t][i], f.score.in, b0);
                 }
                 if constexpr (MASK) {
                     if (cls[0] >= kFsAdds) {
@@ -594,19 +598,22 @@ __global__ __launch_bounds__(512, 2) void k_fattn_scored(fs_args f) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) mx = fmaxf(mx, z[t][i]);
                 // (a sum of 0: no score yet. The first one's exponential is 2^kFsUp)
-                if (__any(mx > kFsUp + kFsOver || (l[w] == 0.0f && mx != -INFINITY))) {
+                if (__any(mx + off > kFsUp + kFsOver || (l[w] == 0.0f && mx != -INFINITY) || off != 0.0f)) {
                     const float most = fs_max4(mx);
                     const bool first = l[w] == 0.0f;
-                    const float by = (first && most != -INFINITY) || most > kFsUp + kFsOver ? kFsUp - most : 0.0f;
-                    const float alpha = first ? 1.0f : __builtin_amdgcn_exp2f(by);
-                    base[w] += by;
-                    l[w] *= alpha;
+                    const bool anew = (first && most != -INFINITY) || most + off > kFsUp + kFsOver;
+                    const float to = anew ? b0 + (kFsUp - most) : base[w];
+                    if (__any(anew && !first)) {
+                        const float alpha = first ? 1.0f : __builtin_amdgcn_exp2f(to - base[w]);
+                        l[w] *= alpha;
+#pragma unroll
+                        for (int ct = 0; ct < NT; ct++) o[w][ct] *= alpha;
+                    }
+                    base[w] = to;
 #pragma unroll
                     for (int t = 0; t < 4; t++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) z[t][i] += by;
-#pragma unroll
-                    for (int ct = 0; ct < NT; ct++) o[w][ct] *= alpha;
+                        for (int i = 0; i < 4; i++) z[t][i] += to - b0;
                 }
 #pragma unroll
                 for (int t = 0; t < 4; t++) {

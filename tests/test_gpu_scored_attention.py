@@ -352,3 +352,19 @@ def test_nan_that_is_seen(ggml, gpu, Q, D, N, kind, where):
     got = attention(ggml, gpu, q, k, v, mask, 0.1, 30.0, 0.0)
     assert np.isnan(got[hit]).all()
     check(got[~hit], want[~hit], bound[~hit])
+
+
+@pytest.mark.parametrize("D,Q,N,lead,cap,bias", [(256, 30, 150, 64, 0.0, 0.0)] +
+                         [(*x, *y) for x in [(64, 20, 200, 64), (128, 70, 300, 130), (256, 30, 150, 64), (64, 300, 2000, 700), (128, 1, 300, 200)]
+                          for y in [(30.0, 0.0), (0.0, 8.0), (30.0, 8.0)]])
+@pytest.mark.parametrize("low", [-65504.0, -3000.0])
+def test_tiles_of_low_scores_first(ggml, gpu, D, Q, N, lead, cap, bias, low):
+    """a padded front masked by a large finite number: what follows keeps its own precision"""
+    rng = np.random.default_rng(D + Q)
+    q, k, v = operands(rng, 2, 4, 2, Q, N, D)
+    mask = np.repeat(make_mask("causal", 2, 4, Q, N, bias, rng), 2, 0)
+    mask[0, :, :, :lead] = low
+    mask[1, :, :, :lead - 30] = low
+    mask[1, :, 0, :] = low  # a row of nothing else
+    want, bound = attention64(q, k, v, mask, 0.1, cap, bias)
+    check(attention(ggml, gpu, q, k, v, mask, 0.1, cap, bias), want, bound)
