@@ -59,15 +59,15 @@ __device__ __forceinline__ float dl_exp(float x) {
     return x > -200.0f ? fmaf(p, r * 0.6931471805599453f, p) : p;  // (no infinity less itself)
 }
 
-__device__ __forceinline__ float dl_max16(float v) {  // of values from zero on
-    auto most = [&](auto ctrl) {
-        v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, true)));
-    };
-    most(std::integral_constant<int, 0x128>{});
-    most(std::integral_constant<int, 0x124>{});
-    most(std::integral_constant<int, 0x122>{});
-    most(std::integral_constant<int, 0x121>{});
-    return v;
+// the largest of lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float dl_max4(float x) {
+    // (the swaps' results as values: a bit cast of a vector's element takes its first)
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const uint32_t a0 = a[0], a1 = a[1];
+    const uint32_t m = __float_as_uint(fmaxf(__uint_as_float(a0), __uint_as_float(a1)));
+    const auto b = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+    const uint32_t b0 = b[0], b1 = b[1];
+    return fmaxf(__uint_as_float(b0), __uint_as_float(b1));
 }
 
 // 16 lanes hold a state row, P pieces of four elements a lane (4 (l + 16 p) ..),
@@ -354,17 +354,22 @@ __global__ __launch_bounds__(64) void k_delta_steps(delta_args a, const float * 
 // k_delta_chunks, whose chain of products is the time, makes them on the f16
 // matrix cores: an operand is the sum of two f16 (22 bits), a product three of
 // theirs, 24 cycles for 16 k where f32's take 128 (three bf16 parts and six
-// products, 48, and their making in the chain took more time than they). Rows of
-// Q, K, T and lower(Q K^T L) are split by k_delta_solve, each row scaled to 2^13 by
-// a power of two that the row's factor takes back; the state, T's operand and D
-// are split as they are made, scaled by powers of two from the largest value that
-// the state and v had a chunk before, with room for 2^7 .. 2^10 times as much. A
-// lane's eight k of 32 are four of one block of 16 and four of the next, so that
-// results are operands here too.
+// products, 48, and their making in the chain took more time than they). The low
+// parts are kept 2^10 times as large, and the two products with them summed apart:
+// so an operand's error is 2^-22 of its own or 2^-34 of one, whichever is more.
+// Rows of Q, K, T and lower(Q K^T L) are split by k_delta_solve, each row scaled to
+// 2^13 by a power of two that the row's factor takes back; the state, T's operand
+// and D are split as they are made, each of the state's columns in a scale of its
+// own: a power of two from the largest value that the column of the state and of v
+// has at the chunk's start. Columns, which the rule keeps apart, so never share an
+// error, and a column's steps are 2^-40 of its largest value in the chunk (one scale a
+// workgroup, and low parts as they are, had columns of 1e-5 of the largest 4e-4 off).
+// The state itself is split before that value is known, in the scale of a chunk before
+// (steps of 2^-27 of the largest at worst), and again where that is further off. A lane's eight k of 32 are four of one block of 16
+// and four of the next, so that results are operands here too.
 //
-// A chunk whose values are not finite, whose g are above zero, or whose scaled
-// values would leave f16's range, runs token by token (a state that starts at
-// zero, say, and meets v: the second such chunk has its scale).
+// A chunk whose values are not finite or past 2^40, whose g are above zero, or whose scaled
+// values would leave f16's range, runs token by token.
 
 constexpr int kDlC = 64;
 constexpr int kDlReady = 32;
@@ -415,11 +420,13 @@ __device__ __forceinline__ bool dl_past(float v, float limit) { return !(fabsf(v
 typedef uint32_t dl_u4 __attribute__((ext_vector_type(4)));
 typedef _Float16 dl_h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 dl_h8 __attribute__((ext_vector_type(8)));
-// two f32 as the sums of two f16 each
+// two f32 as the sums of two f16 each, the low one times 2^10: so the smallest step is
+// 2^-34 (f16's own is 2^-24)
+constexpr float kDlLow = 0x1p10f;
 __device__ __forceinline__ void dl_split2(float a, float b, uint32_t & hi, uint32_t & lo) {
     const dl_h2 h = __builtin_bit_cast(dl_h2, __builtin_amdgcn_cvt_pkrtz(a, b));
     hi = __builtin_bit_cast(uint32_t, h);
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float) h[0], b - (float) h[1]));
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float) h[0], -kDlLow, a * kDlLow), fmaf((float) h[1], -kDlLow, b * kDlLow)));
 }
 struct dl_split {  // a lane's eight elements of k
     dl_u4 v[2];
@@ -432,9 +439,20 @@ __device__ __forceinline__ dl_split dl_split8(dl_v4f a, dl_v4f b) {
     dl_split2(b[2], b[3], h[3], l[3]);
     return {{dl_u4{h[0], h[1], h[2], h[3]}, dl_u4{l[0], l[1], l[2], l[3]}}};
 }
-// the i-th of a product's three, the small ones first
-__device__ __forceinline__ dl_v4f dl_product(int i, const dl_split & a, const dl_split & b, dl_v4f c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(dl_h8, a.v[i == 0]), __builtin_bit_cast(dl_h8, b.v[i == 1]), c, 0, 0, 0);
+// a sum of products: of the high parts, and of a high and a low one (times 2^10)
+struct dl_sum {
+    dl_v4f hi, lo;
+};
+// the i-th of a product's three
+__device__ __forceinline__ void dl_product(int i, const dl_split & a, const dl_split & b, dl_sum & c) {
+    dl_v4f & to = i < 2 ? c.lo : c.hi;
+    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(dl_h8, a.v[i == 0]), __builtin_bit_cast(dl_h8, b.v[i == 1]), to, 0, 0, 0);
+}
+__device__ __forceinline__ dl_v4f dl_whole(const dl_sum & c) {
+    dl_v4f v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = fmaf(c.lo[e], 1.0f / kDlLow, c.hi[e]);
+    return v;
 }
 // 2^e, and the exponent of the power of two at or under |v| (within what f32's powers and their inverses hold)
 __device__ __forceinline__ float dl_pow2(int e) { return __uint_as_float((uint32_t) (e + 127) << 23); }
@@ -720,7 +738,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
     constexpr int KB = NP / 16, KS = NP / 32, NS = (KB + 7) / 8;
     __shared__ dl_u4 s_s[KS][2][NC][64], s_r[2][2][NC][64], s_d[2][2][NC][64], s_ds[2][2][NC][64];  // S0, T's operand, D, D for the state
     __shared__ float s_red[2][8][16];
-    __shared__ uint32_t s_most[2];        // the largest |value| of the state and of v at a chunk's start (its bits)
+    __shared__ uint32_t s_most[2][NC][16];  // a column's largest |value| of the state and of v at a chunk's start (its bits)
     __shared__ int s_past[2], s_late[2];  // a chunk whose S0, or whose D, leaves f16's range
     const delta_args & a = q.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lg = lane >> 4;
@@ -746,7 +764,8 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
             st[n][cb] = dl_v4f{0, 0, 0, 0};
             if (col < a.V && d < a.K) st[n][cb] = *(const dl_v4f *) (q.s_in + s * q.s_in_nb3 + 4 * (((int64_t) h * a.V + col) * a.K + d));
         }
-    if (tid < 2) s_past[tid] = s_late[tid] = s_most[tid] = 0;
+    if (tid < 2) s_past[tid] = s_late[tid] = 0;
+    if (tid < 2 * NC * 16) (&s_most[0][0][0])[tid] = 0;
 
     // A chunk's operands. Each is loaded for the next chunk as soon as its
     // registers are free (two sets would spill), and by all waves alike: a
@@ -817,11 +836,11 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
     };
     auto get = [&](const dl_u4 (&from)[2][NC][64], int cb) { return dl_split{{from[0][cb][lane], from[1][cb][lane]}}; };
     // whether a scaled result might leave f16's range (or is not finite)
-    auto past = [](dl_v4f v) { return dl_past((fabsf(v[0]) + fabsf(v[1])) + (fabsf(v[2]) + fabsf(v[3])), kDlHalf); };
+    auto past = [](dl_v4f v, float limit) { return dl_past((fabsf(v[0]) + fabsf(v[1])) + (fabsf(v[2]) + fabsf(v[3])), limit); };
     auto put_most = [&](int slot) {
-        float m = 0.0f;
 #pragma unroll
-        for (int cb = 0; cb < NC; cb++)
+        for (int cb = 0; cb < NC; cb++) {
+            float m = 0.0f;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 m = fmaxf(m, fabsf(v[cb][e]));
@@ -829,8 +848,9 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
                 for (int n = 0; n < NS; n++)
                     if (wave + 8 * n < KB) m = fmaxf(m, fabsf(st[n][cb][e]));
             }
-        m = dl_max16(m);
-        if (l16 == 0) atomicMax(&s_most[slot], __float_as_uint(m));
+            m = dl_max4(m);
+            if (lg == 0) atomicMax(&s_most[slot][cb][l16], __float_as_uint(m));
+        }
     };
     // token by token, for chunks the products cannot take
     auto tokens = [&](int64_t t0) {
@@ -895,113 +915,131 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
     };
     if (q.chunks > 0) load_rows(0), load_t(0), load_kt(0);
     __syncthreads();
-    put_most(1);
-    __syncthreads();
-    int size = dl_exponent(__uint_as_float(s_most[1]));  // log2 of the largest of the state and v, a chunk before
-    for (int64_t c = 0; c < q.chunks; c++) {
-        const int64_t t0 = (q.c0 + c) * kDlC, more = min(c + 1, q.chunks - 1);
-        bool large = false;
+    int size[NC], now[NC];  // log2 of a column's largest of the state and v: a chunk before, and in this one
+#pragma unroll
+    for (int cb = 0; cb < NC; cb++) size[cb] = 0;
+    auto put_state = [&]() {  // S0, in its columns' scales; whether all of it is finite
+        bool odd = false;
 #pragma unroll
         for (int n = 0; n < NS; n++) {
             const int kb = wave + 8 * n;
             if (kb < KB) {
 #pragma unroll
                 for (int cb = 0; cb < NC; cb++) {
-                    const dl_v4f x = st[n][cb] * dl_pow2(5 - size);
-                    put(s_s[kb >> 1], cb, kb & 1, x);
-                    large |= past(x);
+                    put(s_s[kb >> 1], cb, kb & 1, st[n][cb] * dl_pow2(5 - size[cb]));
+                    odd |= past(st[n][cb], 0x1p120f);
                 }
             }
         }
-        if (large || size > 40) s_past[c & 1] = 1;
-        __syncthreads();
-        const bool by_token = __builtin_amdgcn_readfirstlane(bad) || s_past[c & 1];
-        if (tid == 0) s_past[(c + 1) & 1] = s_late[(c + 1) & 1] = s_most[(c + 1) & 1] = 0;
-        dl_v4f acc[NC];
-        if (by_token) goto one_by_one;
-#pragma unroll
-        for (int cb = 0; cb < NC; cb++) acc[cb] = dl_v4f{0, 0, 0, 0};
-        {
-            // (the reads of LDS ahead of the products, half of them where there are many)
-            constexpr int kReads = KS > 4 ? KS / 2 : KS;
-#pragma unroll
-            for (int k0 = 0; k0 < KS; k0 += kReads) {
-                dl_split x[kReads][NC];
-#pragma unroll
-                for (int k = 0; k < kReads; k++)
-#pragma unroll
-                    for (int cb = 0; cb < NC; cb++) x[k][cb] = get(s_s[k0 + k], cb);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int k = 0; k < kReads; k++)
-#pragma unroll
-                    for (int i = 0; i < 3; i++)
-#pragma unroll
-                        for (int cb = 0; cb < NC; cb++) acc[cb] = dl_product(i, rows[k0 + k], x[k][cb], acc[cb]);
-            }
-        }
+        return !odd;
+    };
+    for (int64_t c = 0; c < q.chunks; c++) {
+        const int64_t t0 = (q.c0 + c) * kDlC, more = min(c + 1, q.chunks - 1);
         put_most(c & 1);
+        if (!put_state()) s_past[c & 1] = 1;
+        __syncthreads();
+        // (the reads of LDS ahead of the products, half of them where there are many)
+        constexpr int kReads = KS > 4 ? KS / 2 : KS;
+        dl_split x[kReads][NC];
+        auto read_state = [&](int k0) {
+#pragma unroll
+            for (int k = 0; k < kReads; k++)
+#pragma unroll
+                for (int cb = 0; cb < NC; cb++) x[k][cb] = get(s_s[k0 + k], cb);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        read_state(0);
+        bool other = false, large = false;
 #pragma unroll
         for (int cb = 0; cb < NC; cb++) {
-            acc[cb] *= f * dl_pow2(size - 5);
+            now[cb] = dl_exponent(__uint_as_float(s_most[c & 1][cb][l16]));
+            other |= now[cb] > size[cb] + 9 || now[cb] < size[cb] - 12, large |= now[cb] > 40;
+        }
+        const bool by_token = __builtin_amdgcn_readfirstlane(bad) || s_past[c & 1] || __any(large);
+        if (tid == 0) s_past[(c + 1) & 1] = s_late[(c + 1) & 1] = 0;
+        if (tid < NC * 16) (&s_most[(c + 1) & 1][0][0])[tid] = 0;
+        dl_sum sum[NC];
+        dl_v4f acc[NC];
+        if (by_token) goto one_by_one;
+        if (__any(other)) {  // (every wave holds all columns: they agree)
+            __syncthreads();
+#pragma unroll
+            for (int cb = 0; cb < NC; cb++) size[cb] = now[cb];
+            put_state();
+            __syncthreads();
+            read_state(0);
+        }
+#pragma unroll
+        for (int cb = 0; cb < NC; cb++) sum[cb].hi = sum[cb].lo = dl_v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int k0 = 0; k0 < KS; k0 += kReads) {
+            if (k0 > 0) read_state(k0);
+#pragma unroll
+            for (int k = 0; k < kReads; k++)
+#pragma unroll
+                for (int i = 0; i < 3; i++)
+#pragma unroll
+                    for (int cb = 0; cb < NC; cb++) dl_product(i, rows[k0 + k], x[k][cb], sum[cb]);
+        }
+#pragma unroll
+        for (int cb = 0; cb < NC; cb++) {
+            acc[cb] = dl_whole(sum[cb]) * (f * dl_pow2(size[cb] - 5));
+            size[cb] = now[cb];
             if (keys) {
-                const dl_v4f x = (v[cb] * beta - acc[cb]) * dl_pow2(8 - size);
+                const dl_v4f x = (v[cb] * beta - acc[cb]) * dl_pow2(8 - size[cb]);
                 put(s_r[tb >> 1], cb, tb & 1, x);
-                large |= past(x);
+                large |= past(x, kDlHalf);
             }
         }
         if (large) s_late[c & 1] = 1;
         load_rows(more);
         __syncthreads();
         {
-            // D: a token block, half of the columns (one column block: the first waves)
-            const int half = NC == 2 ? wave >> 2 : 0, now = dl_exponent(__uint_as_float(s_most[c & 1]));
+            // D, in the scale 2^(6 - size): a token block, half of the columns (one column block: the first waves)
+            const int half = NC == 2 ? wave >> 2 : 0;
             if (NC == 2 || keys) {
-                dl_v4f d = {0, 0, 0, 0};
+                dl_sum z = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
                 for (int m = 0; m < 2; m++) {
                     if (2 * m > tb) continue;
                     const dl_split x = get(s_r[m], half);
 #pragma unroll
-                    for (int i = 0; i < 3; i++) d = dl_product(i, t[m], x, d);
+                    for (int i = 0; i < 3; i++) dl_product(i, t[m], x, z);
                 }
-                d *= t_row * dl_pow2(size - 8);
-                d *= dl_pow2(6 - now);
+                const dl_v4f d = dl_whole(z) * (t_row * 0.25f);
                 put(s_d[tb >> 1], half, tb & 1, d);
                 put(s_ds[tb >> 1], half, tb & 1, d * left);
-                if (past(d)) s_late[c & 1] = 1;
+                if (past(d, kDlHalf)) s_late[c & 1] = 1;
             }
-            size = now;
         }
         load_t(more);
         __syncthreads();
         if (s_late[c & 1]) goto one_by_one;
         {
-            // the state in D's scale, and back (left_most is 2^-20 to 2^-3: the factor of end 2^-37 to 2^126)
-            const float in = end * (dl_pow2(6 - size) / left_most), out = left_most * dl_pow2(size - 6);
-            dl_split x[2][NC];
+            dl_split z[2][NC];
 #pragma unroll
             for (int m = 0; m < 2; m++)
 #pragma unroll
-                for (int cb = 0; cb < NC; cb++) x[m][cb] = get(s_ds[m], cb);
+                for (int cb = 0; cb < NC; cb++) z[m][cb] = get(s_ds[m], cb);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int n = 0; n < NS; n++) {
+                // the state in D's scale, and back (left_most is 2^-20 to 2^-3: the factor of end 2^-37 to 2^126)
 #pragma unroll
-                for (int cb = 0; cb < NC; cb++) st[n][cb] *= in;
+                for (int cb = 0; cb < NC; cb++) sum[cb].hi = st[n][cb] * (end * (dl_pow2(6 - size[cb]) / left_most)), sum[cb].lo = dl_v4f{0, 0, 0, 0};
 #pragma unroll
                 for (int m = 0; m < 2; m++) {
 #pragma unroll
                     for (int i = 0; i < 3; i++)
 #pragma unroll
-                        for (int cb = 0; cb < NC; cb++) st[n][cb] = dl_product(i, kt[n][m], x[m][cb], st[n][cb]);
+                        for (int cb = 0; cb < NC; cb++) dl_product(i, kt[n][m], z[m][cb], sum[cb]);
                 }
 #pragma unroll
-                for (int cb = 0; cb < NC; cb++) st[n][cb] *= out;
+                for (int cb = 0; cb < NC; cb++) st[n][cb] = dl_whole(sum[cb]) * (left_most * dl_pow2(size[cb] - 6));
             }
             if (!keys) {
 #pragma unroll
-                for (int cb = 0; cb < NC; cb++) acc[cb] *= dl_pow2(6 - size);
+                for (int cb = 0; cb < NC; cb++) sum[cb].hi = acc[cb] * dl_pow2(6 - size[cb]), sum[cb].lo = dl_v4f{0, 0, 0, 0};
 #pragma unroll
                 for (int m = 0; m < 2; m++) {
                     if (2 * m > tb) continue;
@@ -1011,11 +1049,11 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
 #pragma unroll
                     for (int i = 0; i < 3; i++)
 #pragma unroll
-                        for (int cb = 0; cb < NC; cb++) acc[cb] = dl_product(i, p[m], x[cb], acc[cb]);
+                        for (int cb = 0; cb < NC; cb++) dl_product(i, p[m], x[cb], sum[cb]);
                 }
                 // (in two steps: y_row's inverse may be 2^73, the state's scale 2^106)
 #pragma unroll
-                for (int cb = 0; cb < NC; cb++) acc[cb] *= dl_pow2(size - 6);
+                for (int cb = 0; cb < NC; cb++) acc[cb] = dl_whole(sum[cb]) * dl_pow2(size[cb] - 6);
                 char * y = (char *) (a.y + ((s * a.tokens + t0) * a.heads + h) * a.V);
                 const uint32_t y_nb = 4u * (uint32_t) a.heads * (uint32_t) a.V, at = (uint32_t) (16 * tb + 4 * lg) * y_nb + 4u * (uint32_t) col0;
                 const int left_over = (int) min((int64_t) kDlC, a.tokens - t0) - 16 * tb - 4 * lg;
@@ -1038,11 +1076,6 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
     one_by_one:
         tokens(t0);
         load_rows(more), load_t(more), load_kt(more);
-        if (tid == 0) s_most[c & 1] = 0;
-        __syncthreads();
-        put_most(c & 1);
-        __syncthreads();
-        size = dl_exponent(__uint_as_float(s_most[c & 1]));
     }
 #pragma unroll
     for (int n = 0; n < NS; n++)

@@ -403,3 +403,54 @@ def test_chunks_of_zero_keys(ggml, gpu, T, norm, case):
         within(got, want, by, "y")
         within(states, end, bs, "states")
     G.free()
+
+
+def token_bounds(q, k, v, g, beta, st):
+    """As rule_bounds, for a gate a head and keys and queries of length at most one: an error made at a
+    token is left, later on, at most as long as the decays since then leave it (a token's turn is no longer
+    than one; a chunk's tokens come through |(1 + A)^-1|, rows of at most 4 for keys like these). A token
+    makes c = 2 K + 100 roundings of the old state's row, of its value and of its correction."""
+    want, end, d, before = rule64(q, k, v, g, beta, st)
+    K, c = k.shape[3], (2 * k.shape[3] + 100) * U
+    by, e = np.zeros_like(want), np.zeros(end.shape[:3])
+    for t in range(want.shape[1]):
+        decay = np.exp(np.float64(g[:, t]))
+        made = np.sqrt((before[:, t] ** 2).sum(3)) * decay + np.abs(d[:, t]) + beta[:, t, :, None] * np.abs(v[:, t].astype(np.float64))
+        e = e * decay + 4 * c * made
+        by[:, t] = (e + c * made) / np.sqrt(K)
+    return want, end, by + 1e-37, e[..., None] + 1e-37
+
+
+@pytest.mark.parametrize("K,V,T,S", [(64, 32, 100, 2), (128, 48, 200, 1), (128, 20, 24, 1), (96, 64, 130, 3), (256, 32, 150, 1)])
+@pytest.mark.parametrize("case", ["columns", "one column", "states", "tokens", "forgotten", "falling"])
+def test_values_of_many_sizes(ggml, gpu, K, V, T, S, case):
+    """small columns beside large ones, and small tokens before or after large ones: each as good as alone"""
+    Hk, H = 1, 2
+    x = list(inputs(K, V, Hk, H, T, S, seed=23, rate=0.05))
+    col = np.array([1, 1e-3, 1e-5, 1e-6], np.float32)[np.arange(V) % 4]
+    if case == "columns":
+        x[2] *= col
+        x[5] *= col[:, None]
+    if case == "one column":
+        x[2][..., 5] *= 1e6
+    if case == "states":
+        x[5] *= 1e4 * col[:, None]
+        x[2] *= col
+    if case == "tokens":  # a chunk's first values are far under its last ones
+        x[2] *= (10.0 ** (np.arange(T) % 64 / 63 * 5 - 5)).astype(np.float32)[:, None, None]
+        x[5][:] = 0
+    if case == "forgotten":  # what was large is gone, in the middle of a chunk
+        x[2][:, :T // 3] *= 1e4
+        x[3][:, T // 3] = -40.0
+    if case == "falling":  # the state of a chunk lies far under the last one's
+        x[2][:, T // 4:] *= 1e-5
+        x[3][:, T // 4:T // 2] = -1.0
+    G, y, _, _ = graph(ggml, gpu, *x)
+    q, k = (unit(np.asarray(a, np.float64)) for a in x[:2])
+    want, end, by, bs = token_bounds(q, k, *x[2:])
+    for _ in range(2):
+        assert G.compute(gpu.backend) == 0
+        got, states = parts(G, y, S, T, H, V, K)
+        within(got, want, by, "y")
+        within(states, end, bs, "states")
+    G.free()
