@@ -1128,6 +1128,7 @@ static int64_t dl_ready_slab(const delta_args & a) {
 
 size_t delta_scratch_bytes(const delta_args & a, int n_cu) {
     (void) n_cu;
+    if (a.seqs == 0 || a.heads == 0 || a.V == 0) return 0;
     // (a graph planned before it is allocated: the addresses may still allow chunks)
     if (a.g_elem) return (size_t) (dl_ready_slab(a) * dl_ready_bytes(a));
     if (a.tokens < 24 || a.K < 16) return 0;

@@ -1653,6 +1653,7 @@ bool planner::fattn_kv32(const ggml_tensor * t, const fattn_args & a) const {
 }
 
 bool planner::plan_fattn(int i, const ggml_tensor * t) {
+    if (nelem(t) == 0) return true;  // no queries: nothing to launch
     fattn_args a;
     if (!make_fattn(t, a)) return false;
     const ggml_tensor * view = nullptr;
@@ -3217,8 +3218,8 @@ bool supports_op(const device_state * dev, const ggml_tensor * t) {
             if (v->ne[0] != k->ne[0] || k->ne[2] != v->ne[2]) return false;
             const float bias = op_f32(t, 1), cap = op_f32(t, 2);
             if (!(bias >= 0.0f && bias <= 3.0e38f && cap >= 0.0f && cap <= 3.0e38f) || (bias > 0.0f && !m)) return false;
-            if (m && (m->type != GGML_TYPE_F16 || m->nb[0] != 2 || m->ne[2] < 1 || q->ne[2] % m->ne[2] != 0)) return false;
-            if (q->ne[3] % k->ne[3] != 0 || !is_contiguous(t)) return false;
+            if (m && (m->type != GGML_TYPE_F16 || m->nb[0] != 2 || m->ne[2] < 1 || m->ne[3] < 1 || q->ne[2] % m->ne[2] != 0)) return false;
+            if (k->ne[3] < 1 || q->ne[3] % k->ne[3] != 0 || !is_contiguous(t)) return false;
             if (!fattn_scored(t)) return true;
             fattn_args a{};
             a.d = (int) q->ne[0], a.hq = (int) q->ne[2], a.hkv = (int) k->ne[2], a.n_kv = (int) k->ne[1];

@@ -693,6 +693,8 @@ struct ggml_tensor * ggml_flash_attn_ext(struct ggml_context * ctx, struct ggml_
     GB_REFUSE_UNLESS(max_bias >= 0.0f && max_bias <= 3.0e38f && logit_softcap >= 0.0f && logit_softcap <= 3.0e38f,
                      "flash_attn_ext: max_bias or logit_softcap below zero or not finite");
     GB_REFUSE_UNLESS(max_bias == 0.0f || mask, "flash_attn_ext: a max_bias without the mask it scales");
+    GB_REFUSE_UNLESS(k->ne[2] > 0 && k->ne[3] > 0 && (!mask || (mask->ne[2] > 0 && mask->ne[3] > 0)),
+                     "flash_attn_ext: no heads or sequences in k or the mask");
     GB_REQUIRE(q->ne[0] == k->ne[0] && k->ne[1] == v->ne[1], "flash_attn_ext: q/k/v shapes");
     GB_REQUIRE(q->ne[2] % k->ne[2] == 0 && q->ne[3] % k->ne[3] == 0, "flash_attn_ext: head broadcast");
     if (mask) {

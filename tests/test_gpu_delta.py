@@ -454,3 +454,14 @@ def test_values_of_many_sizes(ggml, gpu, K, V, T, S, case):
         within(got, want, by, "y")
         within(states, end, bs, "states")
     G.free()
+
+
+@pytest.mark.parametrize("T", [1, 100])
+@pytest.mark.parametrize("elem", [False, True], ids=["head", "element"])
+def test_no_sequences(ggml, gpu, T, elem):
+    """a batch that has run empty: nothing is launched, and no size of it divides anything"""
+    x = inputs(64, 32, 1, 2, T, 0, elem)
+    G, y, _, _ = graph(ggml, gpu, *x)
+    assert G.lib.ggml_backend_supports_op(gpu.backend, y)
+    assert G.compute(gpu.backend) == 0 and G.get(y).size == 0
+    G.free()

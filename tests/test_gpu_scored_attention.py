@@ -368,3 +368,16 @@ def test_tiles_of_low_scores_first(ggml, gpu, D, Q, N, lead, cap, bias, low):
     mask[1, :, 0, :] = low  # a row of nothing else
     want, bound = attention64(q, k, v, mask, 0.1, cap, bias)
     check(attention(ggml, gpu, q, k, v, mask, 0.1, cap, bias), want, bound)
+
+
+@pytest.mark.parametrize("Q,S,kv_seqs", [(0, 2, 2), (0, 2, 1), (1, 0, 1), (5, 0, 1)])
+def test_no_queries(ggml, gpu, Q, S, kv_seqs):
+    """a batch that has run empty: nothing is launched, and no size of it divides anything"""
+    G = ggml.Graph(16, 16)
+    q, k, m = G.new(ggml.F32, 64, Q, 4, S), G.new(ggml.F16, 64, 9, 2, kv_seqs), G.new(ggml.F16, 9, max(Q, 1), 1, 1)
+    y = G.lib.ggml_flash_attn_ext(G.ctx, q, k, k, m, 0.1, 0.0, 30.0)
+    assert G.lib.ggml_backend_supports_op(gpu.backend, y)
+    G.build(y)
+    G.allocate(gpu.buft)
+    assert G.compute(gpu.backend) == 0 and G.get(y).size == 0
+    G.free()

@@ -60,3 +60,14 @@ def test_attention_refuses(ggml, G):
     assert not fa(G.ctx, q, k, v, None, 0.1, 8.0, 0.0)  # a bias is the mask's
     for bias, cap in ((-1.0, 0.0), (0.0, -1.0), (float("inf"), 0.0), (0.0, float("inf")), (float("nan"), 0.0), (0.0, float("nan"))):
         assert not fa(G.ctx, q, k, v, m, 0.1, bias, cap)
+
+
+def test_attention_refuses_what_has_no_heads(ggml, G):
+    q = G.new(ggml.F32, 64, 5, 4, 2)
+    fa = G.lib.ggml_flash_attn_ext
+    k = G.new(ggml.F16, 64, 9, 2, 2)
+    for other in ((64, 9, 0, 2), (64, 9, 2, 0)):
+        e = G.new(ggml.F16, *other)
+        assert not fa(G.ctx, q, e, e, None, 0.1, 0.0, 30.0)
+    for other in ((9, 5, 0, 1), (9, 5, 1, 0)):
+        assert not fa(G.ctx, q, k, k, G.new(ggml.F16, *other), 0.1, 0.0, 30.0)
