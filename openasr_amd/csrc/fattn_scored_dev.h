@@ -43,9 +43,13 @@ inline fs_score fs_score_of(const fattn_args & a) {
         f.cap2 = (float) (a.softcap * log2e);
         for (int k = 0; k < 6; k++) f.poly[k] = (float) (kFsPoly[k] * a.softcap * log2e);
         const double in = (double) a.scale / a.softcap;
-        // (from 1e-5 on the coefficients, down to in^7, are normal numbers)
-        f.low_end = std::fabs(in) >= 1e-5 ? (float) (kFsLowEnd / std::fabs(in)) : 0.0f;
-        for (int k = 0; k < 4; k++) f.low[k] = (float) (kFsLow[k] * a.softcap * log2e * std::pow(in, 2 * k + 1));
+        bool normal = true;  // (the coefficients, up to in^7)
+        for (int k = 0; k < 4; k++) {
+            const double c = kFsLow[k] * a.softcap * log2e * std::pow(in, 2 * k + 1);
+            normal = normal && std::fabs(c) >= 1e-37 && std::fabs(c) <= 1e38;
+            f.low[k] = (float) c;
+        }
+        f.low_end = normal ? (float) (kFsLowEnd / std::fabs(in)) : 0.0f;
     } else {
         f.in = (float) (a.scale * log2e);
     }

@@ -3217,7 +3217,9 @@ bool supports_op(const device_state * dev, const ggml_tensor * t) {
             if (!f32(q) || q->nb[0] != 4 || !kv_ok(k) || !kv_ok(v)) return false;
             if (v->ne[0] != k->ne[0] || k->ne[2] != v->ne[2]) return false;
             const float bias = op_f32(t, 1), cap = op_f32(t, 2);
-            if (!(bias >= 0.0f && bias <= 3.0e38f && cap >= 0.0f && cap <= 3.0e38f) || (bias > 0.0f && !m)) return false;
+            if (!(bias >= 0.0f && bias <= 3.0e38f) || (bias > 0.0f && !m)) return false;
+            // (the cap times log2(e), and a score over the cap, in f32)
+            if (cap != 0.0f && !(cap >= 1e-30f && cap <= 1e30f && std::fabs((double) op_f32(t, 0) / cap) <= 1e30)) return false;
             if (m && (m->type != GGML_TYPE_F16 || m->nb[0] != 2 || m->ne[2] < 1 || m->ne[3] < 1 || q->ne[2] % m->ne[2] != 0)) return false;
             if (k->ne[3] < 1 || q->ne[3] % k->ne[3] != 0 || !is_contiguous(t)) return false;
             if (!fattn_scored(t)) return true;

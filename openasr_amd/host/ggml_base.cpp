@@ -690,8 +690,9 @@ struct ggml_tensor * ggml_soft_max(struct ggml_context * ctx, struct ggml_tensor
 struct ggml_tensor * ggml_flash_attn_ext(struct ggml_context * ctx, struct ggml_tensor * q, struct ggml_tensor * k,
                                          struct ggml_tensor * v, struct ggml_tensor * mask, float scale,
                                          float max_bias, float logit_softcap) {
-    GB_REFUSE_UNLESS(max_bias >= 0.0f && max_bias <= 3.0e38f && logit_softcap >= 0.0f && logit_softcap <= 3.0e38f,
-                     "flash_attn_ext: max_bias or logit_softcap below zero or not finite");
+    GB_REFUSE_UNLESS(max_bias >= 0.0f && max_bias <= 3.0e38f, "flash_attn_ext: max_bias below zero or not finite");
+    GB_REFUSE_UNLESS(logit_softcap == 0.0f || (logit_softcap >= 1e-30f && logit_softcap <= 1e30f),
+                     "flash_attn_ext: logit_softcap neither zero nor from 1e-30 to 1e30");
     GB_REFUSE_UNLESS(max_bias == 0.0f || mask, "flash_attn_ext: a max_bias without the mask it scales");
     GB_REFUSE_UNLESS(k->ne[2] > 0 && k->ne[3] > 0 && (!mask || (mask->ne[2] > 0 && mask->ne[3] > 0)),
                      "flash_attn_ext: no heads or sequences in k or the mask");

@@ -381,3 +381,28 @@ def test_no_queries(ggml, gpu, Q, S, kv_seqs):
     G.allocate(gpu.buft)
     assert G.compute(gpu.backend) == 0 and G.get(y).size == 0
     G.free()
+
+
+@pytest.mark.parametrize("Q,N", [(1, 100), (40, 200)])
+@pytest.mark.parametrize("scale,cap", [(0.1, 1e-30), (0.1, 1e-9), (1e7, 50.0), (1e-20, 1e-9), (0.1, 1e30), (1e-30, 1e-10), (0.0, 30.0), (-0.1, 30.0)])
+def test_caps_and_scales_at_their_ends(ggml, gpu, Q, N, scale, cap):
+    """caps far under and over the scores, scales far from one, rows of queries that are zero"""
+    rng = np.random.default_rng(Q)
+    q, k, v = operands(rng, 1, 4, 2, Q, N, 64)
+    q[:, 1:3] = 0
+    mask = make_mask("causal", 1, 4, Q, N, 0, rng)
+    want, bound = attention64(q, k, v, mask, scale, cap, 0.0)
+    # (the cap's roundings are relative to a score while that is far under the cap)
+    if cap == 1e30:
+        want, bound = attention64(q, k, v, mask, scale, 0.0, 0.0)
+        bound = 2 * bound
+    check(attention(ggml, gpu, q, k, v, mask, scale, cap, 0.0), want, bound)
+
+
+def test_caps_refused(ggml, gpu):
+    G = ggml.Graph(16, 16)
+    q, k = G.new(ggml.F32, 64, 5, 4, 1), G.new(ggml.F16, 64, 9, 2, 1)
+    for scale, cap, ok in ((0.1, 1e-30, True), (1e5, 1e-30, False), (0.1, 1e30, True), (float("inf"), 30.0, False)):
+        y = G.lib.ggml_flash_attn_ext(G.ctx, q, k, k, None, scale, 0.0, cap)
+        assert G.lib.ggml_backend_supports_op(gpu.backend, y) == ok
+    G.free()

@@ -71,3 +71,12 @@ def test_attention_refuses_what_has_no_heads(ggml, G):
         assert not fa(G.ctx, q, e, e, None, 0.1, 0.0, 30.0)
     for other in ((9, 5, 0, 1), (9, 5, 1, 0)):
         assert not fa(G.ctx, q, k, k, G.new(ggml.F16, *other), 0.1, 0.0, 30.0)
+
+
+def test_attention_refuses_caps_past_f32(ggml, G):
+    q, k = G.new(ggml.F32, 64, 5, 4, 2), G.new(ggml.F16, 64, 9, 2, 2)
+    fa = G.lib.ggml_flash_attn_ext
+    for cap in (0.0, 1e-30, 30.0, 1e30):
+        assert fa(G.ctx, q, k, k, None, 0.1, 0.0, cap)
+    for cap in (1e-40, 1e-38, 3e30, 2.9e38):
+        assert not fa(G.ctx, q, k, k, None, 0.1, 0.0, cap)
