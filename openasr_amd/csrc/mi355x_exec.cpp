@@ -248,10 +248,13 @@ struct planner {
     // GQA expansions (match_gqa) every reader of which reads the source's kv
     // heads instead: the REPEAT is not launched
     std::unordered_set<const ggml_tensor *> gqa_skip;
-    // x read through a skipped REPEAT: the view of its source
+    // x read through a skipped REPEAT: the view of its source (else v is left as it is)
     bool gqa_fold(const ggml_tensor * x, tview & v) const {
         const ggml_tensor * r = nullptr;
-        return match_gqa(x, r, v) && gqa_skip.count(r);
+        tview source;
+        if (!match_gqa(x, r, source) || !gqa_skip.count(r)) return false;
+        v = source;
+        return true;
     }
     // The unfused attention chain (nn/decoder.rs:2154-2200) as one launch at
     // its output CONT: the scores MUL_MAT S, the SOFT_MAX P, the V^T CONT VT
@@ -1543,11 +1546,12 @@ bool planner::plan_binary(const ggml_tensor * t) {
 }
 
 // attention for the form of capped or biased scores (k_fattn_scored.hip):
-// those, masks a head, and the head sizes and groups the other forms lack
-static bool fattn_scored(const ggml_tensor * t) {
-    const ggml_tensor *q = t->src[0], *k = t->src[1], *m = t->src[3];
+// those, masks a head, and the head sizes and groups the other forms lack;
+// hkv: the kv heads as they are read (behind a folded expansion fewer than k's)
+static bool fattn_scored(const ggml_tensor * t, int64_t hkv) {
+    const ggml_tensor *q = t->src[0], *m = t->src[3];
     return op_f32(t, 1) > 0.0f || op_f32(t, 2) > 0.0f || (m && m->ne[2] > 1) ||
-           !fattn_supported((int) q->ne[0], (int) q->ne[2], (int) k->ne[2]);
+           !fattn_supported((int) q->ne[0], (int) q->ne[2], (int) hkv);
 }
 
 bool planner::make_fattn(const ggml_tensor * t, fattn_args & a) {
@@ -1556,7 +1560,13 @@ bool planner::make_fattn(const ggml_tensor * t, fattn_args & a) {
     // kv heads (query head h reads head h / (hq / hkv), the kernel's rule)
     tview kv = make_view(k), vv = make_view(v);
     const bool kf = gqa_fold(k, kv), vf = gqa_fold(v, vv);
-    if (kf != vf) return fail(t, "only one of K and V is a folded GQA expansion");
+    // an attention that cannot read the sources reads the expansions: planned again without the fold
+    auto unfold = [&](const char * why) {
+        for (const ggml_tensor * x : {kf ? k : nullptr, vf ? v : nullptr})
+            if (x) no_fold.insert(root_of(x)), replan = true;
+        return fail(t, why);
+    };
+    if (kf != vf) return unfold("only one of K and V is a folded GQA expansion");
     a = fattn_args{};
     a.q = (const char *) q->data;
     a.k = kv.data;
@@ -1595,11 +1605,11 @@ bool planner::make_fattn(const ggml_tensor * t, fattn_args & a) {
     if ((k->type == GGML_TYPE_F16 && (uintptr_t) a.k % 16 != 0) || (v->type == GGML_TYPE_F16 && (uintptr_t) a.v % 16 != 0))
         return fail(t, "K/V not 16-byte aligned");
     a.max_bias = op_f32(t, 1), a.softcap = op_f32(t, 2);
-    if (fattn_scored(t)) {
+    if (fattn_scored(t, a.hkv)) {
         fattn_args rows = a;  // (as they are read: behind a folded expansion, or as contiguous copies)
         if (k->type == GGML_TYPE_F32) rows.k_nb1 = rows.k_nb2 = rows.k_nb3 = 0;
         if (v->type == GGML_TYPE_F32) rows.v_nb1 = rows.v_nb2 = rows.v_nb3 = 0;
-        if (vv.ne[3] != kv.ne[3] || !fattn_scored_supported(rows)) return fail(t, "K / V layout");
+        if (vv.ne[3] != kv.ne[3] || !fattn_scored_supported(rows)) return unfold("K / V layout");
         fattn_scored_plan(a, n_cu);
         // (a caller's own scratch may hold fewer splits' partials)
         while (be->scratch_limit && a.scored_split > 1 && fattn_scratch_bytes(a) > be->scratch_limit / 2) a.scored_split--;
@@ -3222,7 +3232,7 @@ bool supports_op(const device_state * dev, const ggml_tensor * t) {
             if (cap != 0.0f && !(cap >= 1e-30f && cap <= 1e30f && std::fabs((double) op_f32(t, 0) / cap) <= 1e30)) return false;
             if (m && (m->type != GGML_TYPE_F16 || m->nb[0] != 2 || m->ne[2] < 1 || m->ne[3] < 1 || q->ne[2] % m->ne[2] != 0)) return false;
             if (k->ne[3] < 1 || q->ne[3] % k->ne[3] != 0 || !is_contiguous(t)) return false;
-            if (!fattn_scored(t)) return true;
+            if (!fattn_scored(t, k->ne[2])) return true;
             fattn_args a{};
             a.d = (int) q->ne[0], a.hq = (int) q->ne[2], a.hkv = (int) k->ne[2], a.n_kv = (int) k->ne[1];
             // (f32 K and V are read as contiguous copies)

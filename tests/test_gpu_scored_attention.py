@@ -406,3 +406,37 @@ def test_caps_refused(ggml, gpu):
         y = G.lib.ggml_flash_attn_ext(G.ctx, q, k, k, None, scale, 0.0, cap)
         assert G.lib.ggml_backend_supports_op(gpu.backend, y) == ok
     G.free()
+
+
+def expanded(ggml, G, x, heads):
+    """a cache's kv heads [D, N, heads] repeated to the query heads"""
+    L, (D, N, g) = G.lib, (int(n) for n in ggml.tensor(x).ne[:3])
+    x = L.ggml_repeat_4d(G.ctx, L.ggml_reshape_4d(G.ctx, x, D, N, 1, g), D, N, heads // g, g)
+    return L.ggml_reshape_3d(G.ctx, x, D, N, heads)
+
+
+@pytest.mark.parametrize("D,H,G", [(64, 6, 2), (128, 7, 1), (64, 32, 2), (128, 24, 2), (64, 128, 1), (256, 4, 2)])
+@pytest.mark.parametrize("Q", [1, 30])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_expanded_heads_of_any_group(ggml, gpu, D, H, G, Q, cap):
+    """K and V repeated to the query heads: groups that only this form has, and one that none has"""
+    if H // G > 64 and cap == 0.0:
+        cap = 50.0  # (read as they are repeated, so in a form of one head a group)
+    rng = np.random.default_rng(H)
+    N = 150
+    q, k, v = operands(rng, 1, H, G, Q, N, D)
+    mask = make_mask("causal", 1, H, Q, N, 0, rng)
+    want, bound = attention64(q, k, v, mask, 0.1, cap, 0.0)
+    g = ggml.Graph(64, 64)
+    X, K, V, M = g.new(ggml.F32, D, Q, H, 1), g.new(ggml.F16, D, N, G), g.new(ggml.F16, D, N, G), g.new(ggml.F16, N, Q, 1, 1)
+    y = g.lib.ggml_flash_attn_ext(g.ctx, X, expanded(ggml, g, K, H), expanded(ggml, g, V, H), M, 0.1, 0.0, cap)
+    g.build(y)
+    g.allocate(gpu.buft)
+    for t, a in ((X, q), (K, k.view(np.uint16)), (V, v.view(np.uint16)), (M, mask.view(np.uint16))):
+        g.set(t, a)
+    for _ in range(3):
+        assert g.compute(gpu.backend) == 0
+        check(g.get(y).reshape(1, Q, H, D), want, bound)
+    names = [x.split(":", 1)[0] for x, _ in gpu.profile(g.gf, 1)]
+    assert "flash_attn_scored" in names and ("repeat" in names) == (H // G > 64)
+    g.free()
