@@ -2450,9 +2450,9 @@ bool planner::validate() {
         }
     }
     // an expansion not launched: its readers read the source later than the
-    // REPEAT would have
+    // REPEAT would have, and the last one's own output may lie over it
     for (const fold_read & fr : fold_reads) {
-        if (written_between(fr.src, fr.from, fr.to - 1, false)) {
+        if (written_between(fr.src, fr.from, fr.to, false)) {
             no_fold.insert(fr.rep);
             ok = false;
         }

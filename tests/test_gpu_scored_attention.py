@@ -440,3 +440,28 @@ def test_expanded_heads_of_any_group(ggml, gpu, D, H, G, Q, cap):
     names = [x.split(":", 1)[0] for x, _ in gpu.profile(g.gf, 1)]
     assert "flash_attn_scored" in names and ("repeat" in names) == (H // G > 64)
     g.free()
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_output_over_the_source_of_repeated_heads(ggml, gpu, cap):
+    """an allocator may give the attention's output the memory of K before it was repeated: it is not read then"""
+    rng = np.random.default_rng(8)
+    D, H, G, Q, N = 64, 8, 2, 32, 512
+    q, k, v = operands(rng, 1, H, G, Q, N, D)
+    want, bound = attention64(q, k, v, None, 0.1, cap, 0.0)
+    g = ggml.Graph(64, 64)
+    X, K, V = g.new(ggml.F32, D, Q, H, 1), g.new(ggml.F16, D, G, N), g.new(ggml.F16, D, G, N)
+    kc, vc = (g.lib.ggml_cont(g.ctx, g.lib.ggml_permute(g.ctx, t, 0, 2, 1, 3)) for t in (K, V))
+    y = g.lib.ggml_flash_attn_ext(g.ctx, X, expanded(ggml, g, kc, H), expanded(ggml, g, vc, H), None, 0.1, 0.0, cap)
+    g.lib.ggml_flash_attn_ext_set_prec(y, ggml.GGML_PREC_F32)
+    g.build(y)
+    g.allocate(gpu.buft)
+    at = [(ggml.tensor(t).data, g.lib.ggml_nbytes(t)) for t in (kc, vc, y)]
+    assert any(a < at[2][0] + at[2][1] and at[2][0] < a + n for a, n in at[:2])
+    for t, a in ((X, q), (K, k[0].transpose(1, 0, 2).view(np.uint16)), (V, v[0].transpose(1, 0, 2).view(np.uint16))):
+        g.set(t, a)
+    for _ in range(3):
+        assert g.compute(gpu.backend) == 0
+        check(g.get(y).reshape(1, Q, H, D), want, bound)
+    assert "repeat" in [x.split(":", 1)[0] for x, _ in gpu.profile(g.gf, 1)]
+    g.free()
