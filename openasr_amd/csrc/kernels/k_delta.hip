@@ -16,7 +16,8 @@ typedef uint32_t dl_u2 __attribute__((ext_vector_type(2)));
 
 // ------------------------------------------------------------- l2 norm ---
 
-// a wave a row, the sum of squares in f64; memory bounds it
+// a wave a row, the sum of squares and its root in f64 (f32's squares end at rows of
+// 1e-19 and 1e19); memory bounds it
 __global__ __launch_bounds__(256) void k_l2_norm(tview d, tview a, float eps, int64_t rows) {
     const int lane = threadIdx.x & 63;
     const int64_t n = a.ne[0];
@@ -26,7 +27,7 @@ __global__ __launch_bounds__(256) void k_l2_norm(tview d, tview a, float eps, in
         float * y = (float *) (d.data + i1 * d.nb[1] + i2 * d.nb[2] + i3 * d.nb[3]);
         double sum = 0.0;
         for (int64_t i = lane; i < n; i += 64) sum += (double) x[i] * (double) x[i];
-        const float inv = 1.0f / fmaxf(sqrtf((float) wave_sum_d(sum)), eps);
+        const float inv = 1.0f / fmaxf((float) sqrt(wave_sum_d(sum)), eps);
         for (int64_t i = lane; i < n; i += 64) y[i] = x[i] * inv;
     }
 }
@@ -69,6 +70,9 @@ __device__ __forceinline__ float dl_max4(float x) {
     const uint32_t b0 = b[0], b1 = b[1];
     return fmaxf(__uint_as_float(b0), __uint_as_float(b1));
 }
+
+// a row's sum of squares past this is made again of the row times 2^-64
+constexpr float kDlSquares = 0x1p126f;
 
 // 16 lanes hold a state row, P pieces of four elements a lane (4 (l + 16 p) ..),
 // a wave 4 U rows of one head; the next tokens' operands are loaded ahead. VEC:
@@ -133,7 +137,16 @@ __global__ __launch_bounds__(256) void k_delta_rows(delta_args a) {
         return (v[0] + v[1]) + (v[2] + v[3]);
     };
     auto length = [&](const dl_v4f (&x)[P], float eps, float most) {
-        return eps < 0.0f ? 1.0f : fminf(__builtin_amdgcn_rsqf(dl_sum16(dot(x, x))), most);
+        if (eps < 0.0f) return 1.0f;
+        const float sum = dl_sum16(dot(x, x));
+        float by = __builtin_amdgcn_rsqf(sum);
+        if (sum > kDlSquares) {
+            dl_v4f z[P];
+#pragma unroll
+            for (int p = 0; p < P; p++) z[p] = x[p] * 0x1p-64f;
+            by = __builtin_amdgcn_rsqf(dl_sum16(dot(z, z))) * 0x1p-64f;
+        }
+        return fminf(by, most);
     };
     for (int64_t t0 = 0; t0 < a.tokens; t0 += AHEAD) {
 #pragma unroll
@@ -215,7 +228,17 @@ __global__ __launch_bounds__(256) void k_delta_ready(delta_args a, float * out) 
         for (int e = 0; e < 4; e++) sum = fmaf(v[p][e], v[p][e], sum);
     }
     const float eps = q ? a.q_eps : a.k_eps;
-    const float by = (eps < 0.0f ? 1.0f : 1.0f / fmaxf(sqrtf(dl_sum16(sum)), eps)) * (q ? a.scale : 1.0f);
+    sum = dl_sum16(sum);
+    float len = sqrtf(sum);
+    if (sum > kDlSquares) {  // (all 16 lanes alike)
+        sum = 0.0f;
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum = fmaf(v[p][e] * 0x1p-64f, v[p][e] * 0x1p-64f, sum);
+        len = sqrtf(dl_sum16(sum)) * 0x1p64f;
+    }
+    const float by = (eps < 0.0f ? 1.0f : 1.0f / fmaxf(len, eps)) * (q ? a.scale : 1.0f);
 #pragma unroll
     for (int p = 0; p < P; p++) {
         const int i = 4 * (l + 16 * p);
@@ -861,9 +884,9 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
             const float * qr = (const float *) (qp + tt * a.q_nb2);
             auto length = [&](const float * x, float eps) {
                 if (eps < 0.0f) return 1.0f;
-                float sum = 0.0f;
-                for (int i = lane; i < a.K; i += 64) sum = fmaf(x[i], x[i], sum);
-                return 1.0f / fmaxf(sqrtf(wave_sum(sum)), eps);
+                double sum = 0.0;
+                for (int i = lane; i < a.K; i += 64) sum += (double) x[i] * (double) x[i];
+                return 1.0f / fmaxf((float) sqrt(wave_sum_d(sum)), eps);
             };
             const float kl = length(k, a.k_eps), ql = length(qr, a.q_eps) * a.scale;
             const float eg = expf(*(const float *) (a.g + h * a.g_nb1 + tt * a.g_nb2 + s * a.g_nb3));

@@ -2322,7 +2322,8 @@ bool planner::plan_ssm_scan(const ggml_tensor * t) {
 }
 
 bool planner::plan_l2_norm(int i, const ggml_tensor * t) {
-    const ggml_tensor * d = no_defer.count(t) ? nullptr : sole_consumer(t, i + 1);
+    // (the rule's sums of squares are f32's: rows of 1e-15 and more, which an eps under them would tell apart)
+    const ggml_tensor * d = no_defer.count(t) || op_f32(t, 0) < 1e-12f ? nullptr : sole_consumer(t, i + 1);
     if (d && d->op == GGML_OP_GATED_DELTA_NET && (d->src[0] == t || d->src[1] == t) && supports_op(be->dev, d)) {
         deferred[t] = d;
         deferred_l2.push_back({t, index.at(d)});

@@ -465,3 +465,68 @@ def test_no_sequences(ggml, gpu, T, elem):
     assert G.lib.ggml_backend_supports_op(gpu.backend, y)
     assert G.compute(gpu.backend) == 0 and G.get(y).size == 0
     G.free()
+
+
+@pytest.mark.parametrize("T", [1, 100])
+@pytest.mark.parametrize("eps", [0.0, 1e-25, 1e-12])
+def test_small_eps(ggml, gpu, T, eps):
+    """rows far shorter than f32's squares reach, brought to length by an eps that lets them"""
+    K, V, Hk, H, S = 64, 32, 1, 2, 2
+    x = list(inputs(K, V, Hk, H, T, S, seed=29))
+    x[0] *= np.float32(max(eps, 1e-22))
+    x[1] *= np.float32(max(eps, 1e-22))
+    G = ggml.Graph(64, 64)
+    q_, k_, v_ = G.new(ggml.F32, K, Hk, T, S), G.new(ggml.F32, K, Hk, T, S), G.new(ggml.F32, V, H, T, S)
+    g_, b_, s_ = G.new(ggml.F32, 1, H, T, S), G.new(ggml.F32, 1, H, T, S), G.new(ggml.F32, K, V, H, S)
+    y = G.lib.ggml_gated_delta_net(G.ctx, G.lib.ggml_l2_norm(G.ctx, q_, eps), G.lib.ggml_l2_norm(G.ctx, k_, eps), v_, g_, b_, s_)
+    G.build(y)
+    G.allocate(gpu.buft)
+    for t, a in zip((q_, k_, v_, g_, b_, s_), x):
+        G.set(t, a)
+    q, k = (np.asarray(a, np.float64) / np.sqrt((np.asarray(a, np.float64) ** 2).sum(-1, keepdims=True)) for a in x[:2])
+    want, end, by, bs = rule_bounds(q, k, *x[2:])
+    for _ in range(3):
+        assert G.compute(gpu.backend) == 0
+        got, states = parts(G, y, S, T, H, V, K)
+        within(got, want, by, "y")
+        within(states, end, bs, "states")
+    G.free()
+
+
+@pytest.mark.parametrize("n", [1, 64, 300])
+def test_l2_norm_of_any_length(ggml, gpu, n):
+    """rows whose squares leave f32, on both sides"""
+    r = np.random.default_rng(n)
+    x = (r.standard_normal((9, n)) * 10.0 ** np.array([-30, -24, -20, -15, 0, 15, 19, 25, 36])[:, None]).astype(np.float32)
+    for eps in (0.0, 1e-28):
+        G = ggml.Graph(16, 16)
+        X = G.new(ggml.F32, n, 9)
+        y = G.lib.ggml_l2_norm(G.ctx, X, eps)
+        G.build(y)
+        G.allocate(gpu.buft)
+        G.set(X, x)
+        z = x.astype(np.float64)
+        want = z / np.maximum(np.sqrt((z * z).sum(1, keepdims=True)), eps)
+        assert G.compute(gpu.backend) == 0
+        within(G.get(y).reshape(9, n), want, 5 * U * np.abs(want) + 1e-37)
+        G.free()
+
+
+@pytest.mark.parametrize("K", [64, 128, 33, 256])
+@pytest.mark.parametrize("T", [1, 100])
+@pytest.mark.parametrize("elem", [False, True], ids=["head", "element"])
+def test_long_rows_brought_to_length(ggml, gpu, K, T, elem):
+    """rows whose squares are past f32 come to length one inside the rule as they do in L2_NORM"""
+    V, Hk, H, S = 32, 1, 2, 2
+    x = list(inputs(K, V, Hk, H, T, S, elem, seed=31))
+    for a in x[:2]:
+        a *= np.where(np.random.default_rng(1).random((S, T, Hk, 1)) < 0.3, 1e25, 1.0).astype(np.float32)
+    x[0][0, 0] *= np.float32(1e30 / np.abs(x[0][0, 0]).max())
+    G, y, _, _ = graph(ggml, gpu, *x)
+    q, k = (unit(np.asarray(a, np.float64)) for a in x[:2])
+    want, end, by, bs = rule_bounds(q, k, *x[2:])
+    assert G.compute(gpu.backend) == 0
+    got, states = parts(G, y, S, T, H, V, K)
+    within(got, want, by, "y")
+    within(states, end, bs, "states")
+    G.free()
