@@ -137,7 +137,7 @@ struct ggml_tensor * ggml_l2_norm(struct ggml_context * ctx, struct ggml_tensor 
  * that depends on the number of tokens. From 24 tokens on (a gate a head) the
  * operands of the sums are rounded to 22 bits; what is smaller than others of
  * its column (of v, and of the state's rows for it) in the same 64 tokens, to
- * 2^-40 of the largest there, a state's element to 2^-27. */
+ * 2^-40 of the largest there, a state's element to 2^-33. */
 struct ggml_tensor * ggml_gated_delta_net(struct ggml_context * ctx, struct ggml_tensor * q, struct ggml_tensor * k,
                                           struct ggml_tensor * v, struct ggml_tensor * g, struct ggml_tensor * beta,
                                           struct ggml_tensor * state);

@@ -388,7 +388,7 @@ __global__ __launch_bounds__(64) void k_delta_steps(delta_args a, const float * 
 // error, and a column's steps are 2^-40 of its largest value in the chunk (one scale a
 // workgroup, and low parts as they are, had columns of 1e-5 of the largest 4e-4 off).
 // The state itself is split before that value is known, in the scale of a chunk before
-// (steps of 2^-27 of the largest at worst), and again where that is further off. A lane's eight k of 32 are four of one block of 16
+// (steps of 2^-33 of the largest at worst), and again where that is further off. A lane's eight k of 32 are four of one block of 16
 // and four of the next, so that results are operands here too.
 //
 // A chunk whose values are not finite or past 2^40, whose g are above zero, or whose scaled
@@ -976,7 +976,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
 #pragma unroll
         for (int cb = 0; cb < NC; cb++) {
             now[cb] = dl_exponent(__uint_as_float(s_most[c & 1][cb][l16]));
-            other |= now[cb] > size[cb] + 9 || now[cb] < size[cb] - 12, large |= now[cb] > 40;
+            other |= now[cb] > size[cb] + 9 || now[cb] < size[cb] - 6, large |= now[cb] > 40;
         }
         const bool by_token = __builtin_amdgcn_readfirstlane(bad) || s_past[c & 1] || __any(large);
         if (tid == 0) s_past[(c + 1) & 1] = s_late[(c + 1) & 1] = 0;
