@@ -71,13 +71,14 @@ __device__ __forceinline__ float dl_max4(float x) {
     return fmaxf(__uint_as_float(b0), __uint_as_float(b1));
 }
 
-// a row's sum of squares past this is made again of the row times 2^-64
-constexpr float kDlSquares = 0x1p126f;
+// a row's sum of squares past this (an infinity) is made again of the row times 2^-64
+constexpr float kDlSquares = 0x1.fffffep127f;
 
 // 16 lanes hold a state row, P pieces of four elements a lane (4 (l + 16 p) ..),
-// a wave 4 U rows of one head; the next tokens' operands are loaded ahead. VEC:
+// a wave 4 U rows of one head; the next token's operands are loaded ahead (four
+// tokens' measured the same: 500 tokens of 16 heads of 12 x 128 255 us for 252). VEC:
 // every row in whole 16-byte pieces.
-template <int P, int U, int AHEAD, bool VEC, bool ELEM>
+template <int P, int U, bool VEC, bool ELEM>
 __global__ __launch_bounds__(256) void k_delta_rows(delta_args a) {
     const int lane = threadIdx.x & 63, l = lane & 15, sub = lane >> 4;
     const uint32_t blocks = (uint32_t) ((a.V + 4 * U - 1) / (4 * U));
@@ -115,10 +116,8 @@ __global__ __launch_bounds__(256) void k_delta_rows(delta_args a) {
 #pragma unroll
         for (int u = 0; u < U; u++) x.v[u] = ((const float *) (v + t * a.v_nb2))[min(j0 + 4 * u, a.V - 1)];
     };
-    token next[AHEAD];
-#pragma unroll
-    for (int n = 0; n < AHEAD; n++)
-        if (a.tokens > 0) load(min((int64_t) n, a.tokens - 1), next[n]);
+    token next;
+    if (a.tokens > 0) load(0, next);
     dl_v4f st[U][P];
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -126,7 +125,8 @@ __global__ __launch_bounds__(256) void k_delta_rows(delta_args a) {
 #pragma unroll
         for (int p = 0; p < P; p++) st[u][p] = piece(row, p);
     }
-    // what a row is multiplied by: 1 / max(its length, eps)
+    // what a row is multiplied by: 1 / max(its length, eps), by v_rsq_f32, an ulp off (the
+    // other forms take a root and a quotient)
     const float k_most = 1.0f / a.k_eps, q_most = 1.0f / a.q_eps;
     auto dot = [](const dl_v4f (&x)[P], const dl_v4f (&y)[P]) {
         dl_v4f v = x[0] * y[0];
@@ -136,53 +136,60 @@ __global__ __launch_bounds__(256) void k_delta_rows(delta_args a) {
             for (int e = 0; e < 4; e++) v[e] = fmaf(x[p][e], y[p][e], v[e]);
         return (v[0] + v[1]) + (v[2] + v[3]);
     };
-    auto length = [&](const dl_v4f (&x)[P], float eps, float most) {
-        if (eps < 0.0f) return 1.0f;
-        const float sum = dl_sum16(dot(x, x));
-        float by = __builtin_amdgcn_rsqf(sum);
-        if (sum > kDlSquares) {
-            dl_v4f z[P];
+    auto squares = [&](const dl_v4f (&x)[P], float eps) { return eps < 0.0f ? 1.0f : dl_sum16(dot(x, x)); };
+    auto by_small = [&](const dl_v4f (&x)[P]) {
+        dl_v4f z[P];
 #pragma unroll
-            for (int p = 0; p < P; p++) z[p] = x[p] * 0x1p-64f;
-            by = __builtin_amdgcn_rsqf(dl_sum16(dot(z, z))) * 0x1p-64f;
-        }
-        return fminf(by, most);
+        for (int p = 0; p < P; p++) z[p] = x[p] * 0x1p-64f;
+        return __builtin_amdgcn_rsqf(dl_sum16(dot(z, z))) * 0x1p-64f;
     };
-    for (int64_t t0 = 0; t0 < a.tokens; t0 += AHEAD) {
+    for (int64_t t = 0; t < a.tokens; t++) {
+        token x = next;
+        if (t + 1 < a.tokens) load(t + 1, next);
+        const float kk = squares(x.k, a.k_eps), qq = squares(x.q, a.q_eps);
+        const float kl = a.k_eps < 0.0f ? 1.0f : fminf(__builtin_amdgcn_rsqf(kk), k_most);
+        const float ql = (a.q_eps < 0.0f ? 1.0f : fminf(__builtin_amdgcn_rsqf(qq), q_most)) * a.scale;
+        dl_v4f eg[ELEM ? P : 1];
+        if constexpr (ELEM) {
 #pragma unroll
-        for (int n = 0; n < AHEAD; n++) {
-            const int64_t t = t0 + n;
-            if (t >= a.tokens) break;
-            token x = next[n];
-            if (t + AHEAD < a.tokens) load(t + AHEAD, next[n]);
-            const float kl = length(x.k, a.k_eps, k_most), ql = length(x.q, a.q_eps, q_most) * a.scale;
-            dl_v4f eg[ELEM ? P : 1];
-            if constexpr (ELEM) {
+            for (int p = 0; p < P; p++)
 #pragma unroll
-                for (int p = 0; p < P; p++)
+                for (int e = 0; e < 4; e++) eg[p][e] = dl_exp(x.g[p][e]);
+        } else {
+            const float d = dl_exp(x.g[0][0]);
+            eg[0] = dl_v4f{d, d, d, d};
+        }
+        float y[U];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) eg[p][e] = dl_exp(x.g[p][e]);
-            } else {
-                const float d = dl_exp(x.g[0][0]);
-                eg[0] = dl_v4f{d, d, d, d};
-            }
-            float y[U];
+        for (int u = 0; u < U; u++) {
+#pragma unroll
+            for (int p = 0; p < P; p++) st[u][p] *= eg[ELEM ? p : 0];
+            const float d = x.beta * (x.v[u] - kl * dl_sum16(dot(st[u], x.k))) * kl;
+#pragma unroll
+            for (int p = 0; p < P; p++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) st[u][p][e] = fmaf(x.k[p][e], d, st[u][p][e]);
+            y[u] = ql * dl_sum16(dot(st[u], x.q));
+        }
+        if (fmaxf(kk, qq) > kDlSquares) {
+            // Squares past f32: kl, or ql, came out as 0, and the state is only decayed. The
+            // token again (asked here, where nothing waits for the sums: before, 10 % of a token)
+            const bool anew = kk > kDlSquares;
+            const float kn = anew ? fminf(by_small(x.k), k_most) : kl, qn = qq > kDlSquares ? fminf(by_small(x.q), q_most) * a.scale : ql;
 #pragma unroll
             for (int u = 0; u < U; u++) {
-#pragma unroll
-                for (int p = 0; p < P; p++) st[u][p] *= eg[ELEM ? p : 0];
-                const float d = x.beta * (x.v[u] - kl * dl_sum16(dot(st[u], x.k))) * kl;
+                const float d = anew ? x.beta * (x.v[u] - kn * dl_sum16(dot(st[u], x.k))) * kn : 0.0f;
 #pragma unroll
                 for (int p = 0; p < P; p++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) st[u][p][e] = fmaf(x.k[p][e], d, st[u][p][e]);
-                y[u] = ql * dl_sum16(dot(st[u], x.q));
+                y[u] = qn * dl_sum16(dot(st[u], x.q));
             }
-            float * to = a.y + ((s * a.tokens + t) * a.heads + h) * a.V + j0;
-#pragma unroll
-            for (int u = 0; u < U; u++)
-                if (l == 0 && j0 + 4 * u < a.V) to[4 * u] = y[u];
         }
+        float * to = a.y + ((s * a.tokens + t) * a.heads + h) * a.V + j0;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (l == 0 && j0 + 4 * u < a.V) to[4 * u] = y[u];
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -392,7 +399,9 @@ __global__ __launch_bounds__(64) void k_delta_steps(delta_args a, const float * 
 // and four of the next, so that results are operands here too.
 //
 // A chunk whose values are not finite or past 2^40, whose g are above zero, or whose scaled
-// values would leave f16's range, runs token by token.
+// values would leave f16's range, runs token by token, 120 us a chunk: 2048 tokens of 32
+// heads of 128 x 128 with keys of length 1e-3 3860 us, of length one 139 (and those short
+// ones by k_delta_rows 923).
 
 constexpr int kDlC = 64;
 constexpr int kDlReady = 32;
@@ -962,7 +971,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(dl_chunk_args q) {
         if (!put_state()) s_past[c & 1] = 1;
         __syncthreads();
         // (the reads of LDS ahead of the products, half of them where there are many)
-        constexpr int kReads = KS > 4 ? KS / 2 : KS;
+        constexpr int kReads = KS * NC > 8 ? 2 : KS > 4 ? KS / 2 : KS;
         dl_split x[kReads][NC];
         auto read_state = [&](int k0) {
 #pragma unroll
@@ -1120,7 +1129,7 @@ static int64_t dl_chunk_size(const delta_args & a) {
 }
 // Chunks of one slab, whose records lie in scratch: the two launches take turns.
 // 4096 tokens of 32 heads of 128 x 128 (2.7 MB a chunk), us a call by MB of
-// scratch: 40 333, 60 301, 90 286, 200 285.
+// scratch: 40 350, 60 312, 96 290, 200 298.
 static int64_t dl_slab(const delta_args & a) {
     const int64_t chunks = (a.tokens + kDlC - 1) / kDlC, one = dl_chunk_size(a);
     const int64_t fit = std::max<int64_t>(1, a.scratch_bytes / one), slabs = (chunks + fit - 1) / fit;
@@ -1133,14 +1142,19 @@ static bool dl_vec(const delta_args & a) {
                          (a.g_elem ? (uintptr_t) a.g | (uintptr_t) a.g_nb1 | (uintptr_t) a.g_nb2 | (uintptr_t) a.g_nb3 : 0);
     return al % 16 == 0;
 }
-// chunks: a gate a head, and tokens enough for the products to pay
+// chunks: a gate a head, and tokens enough for the products to pay. us of rows and of
+// chunks, which take the same from 24 to 64 tokens: 32 heads of 128, one sequence, 24
+// tokens 19.5 / 29.9, 40 29.0 / 30.0, 64 43 / 30; 16 of them, 24 63 / 90, 40 97 / 93, 64
+// 150 / 96; three of 12 heads of 64 x 96, 24 15.6 / 19.6, 32 20.8 / 19.7: they meet at 30
+// to 40 tokens, above this border
 static bool dl_chunked(const delta_args & a) {
     return !a.g_elem && a.tokens >= 24 && a.K >= 16 && dl_vec(a) &&
            a.v_nb2 >= 0 && a.v_nb2 < 1 << 25 && (int64_t) a.heads * a.V < 1 << 23;  // (a lane's rows of v and y in 32-bit offsets)
 }
 
-// k_delta_ready's tokens a slab; 0: it is not worth its launch (32 tokens, 16 heads of
-// 128, 26 us without and 14 with), or has no room
+// k_delta_ready's tokens a slab; 0: it is not worth its launch, or has no room. us without
+// and with it, heads of 128: one sequence of 16 heads, 8 tokens 10.0 / 10.2, 16 16.5 / 11.8,
+// 31 28.4 / 14.6; eight of 32 heads, 24 tokens 48.6 / 52.0, 31 60.3 / 58.6
 static int dl_pieces(const delta_args & a) { return a.K <= 64 ? 1 : a.K <= 128 ? 2 : 4; }  // of 64 elements a row
 static int64_t dl_ready_bytes(const delta_args & a) { return 256ll * dl_pieces(a) * (2 * a.key_heads + a.heads) * a.seqs; }
 static int64_t dl_ready_slab(const delta_args & a) {
@@ -1164,7 +1178,9 @@ static void launch_delta_chunks(const delta_args & a, void * scratch, hipStream_
     q.a = a;
     q.rec = (char *) scratch;
     // 32 columns a workgroup halve what is read of the records, but a chunk takes
-    // longer (3.9 us, of 16 columns 3.3): where these fill the CUs
+    // longer: where these fill the CUs. us of 16 / 32 columns, 1000 tokens of 32 heads
+    // of 128 x 128 82 / 96, of 64 143 / 108. (Where 32 columns do not fill the CUs and 16
+    // take two rounds of workgroups, these are the better too, 40 heads 138 / 104, and not taken)
     const bool wide = (int64_t) ((a.V + 31) / 32) * a.heads * a.seqs >= n_cu;
     q.cols = wide ? (a.V + 31) / 32 : (a.V + 15) / 16;
     q.s_in = a.s, q.s_in_nb3 = a.s_nb3;
@@ -1182,12 +1198,12 @@ static void launch_delta_chunks(const delta_args & a, void * scratch, hipStream_
     }
 }
 
-template <int P, int U, int AHEAD, bool VEC>
+template <int P, int U, bool VEC>
 static void launch_delta_rows(const delta_args & a, hipStream_t s) {
     const int64_t units = (int64_t) ((a.V + 4 * U - 1) / (4 * U)) * a.heads * a.seqs;
     const dim3 grid((unsigned) ((units + 3) / 4));
-    if (a.g_elem) hipLaunchKernelGGL((k_delta_rows<P, U, AHEAD, VEC, true>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_delta_rows<P, U, AHEAD, VEC, false>), grid, dim3(256), 0, s, a);
+    if (a.g_elem) hipLaunchKernelGGL((k_delta_rows<P, U, VEC, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_delta_rows<P, U, VEC, false>), grid, dim3(256), 0, s, a);
     note_hip_error(hipGetLastError());
 }
 
@@ -1215,20 +1231,17 @@ static void launch_delta_ready(const delta_args & a, void * scratch, hipStream_t
 // A wave takes 4 U rows: few where that leaves waves a SIMD, many where there
 // are enough anyhow (the token's work beside the rows is shared). 32 heads of 128
 // x 128, us, U = 1 / 2 / 4: 8 tokens of one sequence 7.9 / 8.7 / 11.5, of 16 37 /
-// 30 / 30; one token of 48 34 / 35 / 34. Four tokens' operands ahead instead of
-// one's: 500 tokens with gates an element 342 for 365, and more where tokens are
-// few (one token of 48 sequences 64 for 34).
+// 30 / 30; one token of 48 34 / 35 / 34.
 template <int P>
 static void launch_delta_tokens(const delta_args & a, void * scratch, hipStream_t s, int n_cu) {
     const int64_t rows = (int64_t) a.V * a.heads * a.seqs, enough = 16 * (int64_t) n_cu;  // four waves a CU, of 4 rows
     if (dl_vec(a) && dl_ready_slab(a) > 0) {
         if (rows >= 2 * enough) launch_delta_ready<P, 2>(a, scratch, s);
         else launch_delta_ready<P, 1>(a, scratch, s);
-    } else if (!dl_vec(a)) launch_delta_rows<P, 2, 1, false>(a, s);
-    else if (rows >= 4 * enough) launch_delta_rows<P, 4, 1, true>(a, s);
-    else if (rows >= 2 * enough) launch_delta_rows<P, 2, 1, true>(a, s);
-    else if (a.tokens < 32) launch_delta_rows<P, 1, 1, true>(a, s);
-    else launch_delta_rows<P, 1, 4, true>(a, s);
+    } else if (!dl_vec(a)) launch_delta_rows<P, 2, false>(a, s);
+    else if (rows >= 4 * enough) launch_delta_rows<P, 4, true>(a, s);
+    else if (rows >= 2 * enough) launch_delta_rows<P, 2, true>(a, s);
+    else launch_delta_rows<P, 1, true>(a, s);
 }
 
 void launch_delta(const delta_args & args, void * scratch, hipStream_t s, int n_cu) {
