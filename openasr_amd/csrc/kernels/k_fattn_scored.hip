@@ -22,11 +22,11 @@
 // which positions some query sees. From its counts every workgroup finds the same
 // pieces of the same length, and a third launch joins a row's where there are several.
 //
-// What bounds it: 256 rows of 128 by a tile take 8400 cycles of a CU, its 832 matrix
+// What bounds it: 256 rows of 128 by a tile take 8300 cycles of a CU, its 832 matrix
 // instructions 3328 of each SIMD's and its exponentials 4000 to 4900 of the vector
 // units' (9 vector instructions a score with a cap -- a polynomial of the product
 // five, p's halves two -- and a quarter-rate exponential); the two overlap, a
-// request for 1 KB of K or V holds its wave for 150 to 300 cycles of it. us of the
+// request for 1 KB of K or V holds its wave for 100 to 300 cycles of it. us of the
 // call without a barrier between the two kinds of work (four waves a workgroup, two
 // workgroups a CU, which fell into step) and with it: two sequences of 4096 causal
 // queries, 16 heads of 128 over 8, capped 264 / 251, not capped 240 / 227; one of
@@ -384,7 +384,8 @@ __global__ __launch_bounds__(512, 2) void k_fattn_scored(fs_args f) {
     };
     // Group 0, at the tile's arrival. Where not every query sees everything,
     // positions of V that no query sees become zeros (0 times anything), and pieces
-    // that are not finite too: those are added query by query
+    // that are not finite too: those are added query by query. (Where every query does,
+    // an infinite value comes out infinite, or as a NaN from a p whose low part is zero)
     auto landed = [&](int tile, int cls, int par) {
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
         asm volatile("" ::: "memory");
