@@ -164,6 +164,8 @@ struct ggml_tensor * ggml_cast(struct ggml_context * ctx, struct ggml_tensor * a
 struct ggml_tensor * ggml_soft_max(struct ggml_context * ctx, struct ggml_tensor * a);
 struct ggml_tensor * ggml_soft_max_ext(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * mask,
                                        float scale, float max_bias);
+/* max_bias from 0 on (above 0 with a mask, which it scales), logit_softcap 0 or
+ * from 1e-30 to 1e30, at least one head and sequence in k and the mask: else NULL */
 struct ggml_tensor * ggml_flash_attn_ext(struct ggml_context * ctx, struct ggml_tensor * q, struct ggml_tensor * k,
                                          struct ggml_tensor * v, struct ggml_tensor * mask, float scale,
                                          float max_bias, float logit_softcap);
