@@ -396,8 +396,9 @@ __global__ __launch_bounds__(64) void k_delta_steps(delta_args a, const float * 
 // error, and a column's steps are 2^-40 of its largest value in the chunk (one scale a
 // workgroup, and low parts as they are, had columns of 1e-5 of the largest 4e-4 off).
 // The state itself is split before that value is known, in the scale of a chunk before
-// (steps of 2^-33 of the largest at worst), and again where that is further off. A lane's eight k of 32 are four of one block of 16
-// and four of the next, so that results are operands here too.
+// (steps of 2^-33 of the largest at worst), and again where that is further off. A lane's
+// eight k of 32 are four of one block of 16 and four of the next, so that results are
+// operands here too.
 //
 // A chunk whose values are not finite or past 2^40, whose g are above zero, or whose scaled
 // values would leave f16's range, runs token by token, 120 us a chunk: 2048 tokens of 32
@@ -408,7 +409,7 @@ constexpr int kDlC = 64;
 constexpr int kDlReady = 32;
 // what the products take: q's and k's rows as they come, and (the largest element of a
 // row) brought to length (the state of keys much shorter than one lies far under v, in
-// whose scale it is split: keys of 1e-4 were 2e-3 off); beta; a row of |T| (1 to 3 for
+// whose scale it is split: with low parts as they are, keys of 1e-4 were 2e-3 off); beta; a row of |T| (1 to 3 for
 // keys of length one and beta up to one; tokens of one key with a beta of 2, which turn
 // the state over and over, come to 127, and were 4e-4 off); scaled values. The state
 // and v: up to 2^40
